@@ -27,6 +27,8 @@ DTYPE_BF16 = 2
 DTYPE_I8 = 3
 DTYPE_FP8_E4M3 = 8
 
+_INT32 = 4  # block tables and lengths (no dtype of activations or caches)
+
 OK = 0
 ERR_INVALID_ARGUMENT = -1
 ERR_UNSUPPORTED = -2
@@ -90,6 +92,12 @@ def _load() -> ctypes.CDLL:
     lib.ffkv_rope_append.restype = i32
     lib.ffkv_rope_append.argtypes = [vp, vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
                                      i32, ctypes.c_float, vp]
+    rule = [f32, vp, i32]  # score_cap, slopes, window
+    lib.ffkv_decode_scored_workspace_bytes.restype = sz
+    lib.ffkv_decode_scored_workspace_bytes.argtypes = [i32] * 6
+    lib.ffkv_paged_decode_scored.restype = i32
+    lib.ffkv_paged_decode_scored.argtypes = [vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
+                                             i32, f32, *rule, vp, vp, vp, i32, vp, vp, f32, ctypes.c_int64, vp, sz, vp]
     lib.ffkv_last_error.restype = ctypes.c_char_p
     lib.ffkv_last_error.argtypes = []
     lib.ffkv_version.restype = ctypes.c_char_p
@@ -102,9 +110,9 @@ def _load() -> ctypes.CDLL:
 def _bind(lib, torch) -> None:
     """Point the native front end (``_front``, csrc/python/front.cpp) at ``lib``'s functions."""
     names = ("append", "paged_decode", "append_paged_decode", "paged_decode_shared_prefix", "paged_decode_noalloc",
-             "prefill_workspace_bytes", "paged_prefill_ws", "rope", "rope_append")
+             "prefill_workspace_bytes", "paged_prefill_ws", "rope", "rope_append", "paged_decode_scored")
     _front.bind(tuple(ctypes.cast(getattr(lib, "ffkv_" + n), ctypes.c_void_p).value for n in names),
-                list(_torch_dtypes(torch).items()), getattr(torch._C, "_cuda_getDevice", None),
+                [*_torch_dtypes(torch).items(), (torch.int32, _INT32)], getattr(torch._C, "_cuda_getDevice", None),
                 getattr(torch._C, "_cuda_getCurrentRawStream", None), lambda: torch.cuda.current_stream().cuda_stream)
 
 
@@ -291,4 +299,29 @@ def paged_attention(q, k_cache, v_cache, block_table, context_lens, out=None, k_
     out = _decode_out(q, out)
     check(_front.decode(q, out, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, max_context_len, scale,
                         num_blocks, workspace, stream))
+    return out
+
+
+def decode_scored_workspace(batch: int, num_heads: int, head_dim: int, max_blocks: int, max_context_len: int = 0,
+                            weights: bool = False, device=None):
+    """A workspace for ``paged_attention_scored`` (``ffkv_decode_scored_workspace_bytes``)."""
+    import torch
+
+    n = int(lib.ffkv_decode_scored_workspace_bytes(batch, num_heads, head_dim, max_blocks, max_context_len, int(weights)))
+    return torch.empty(max(n, 256), dtype=torch.uint8, device=device if device is not None else "cuda")
+
+
+def paged_attention_scored(q, k_cache, v_cache, block_table, context_lens, score_cap: float = 0.0, slopes=None,
+                           window: int = 0, key_begin=None, k_new=None, v_new=None, weights=None, prior=None,
+                           decay: float = 1.0, out=None, k_scale=None, v_scale=None, max_context_len: int = 0,
+                           scale: float = 0.0, workspace=None, num_blocks: int | None = None, stream=None):
+    """PagedAttention decode under a score rule (``ffkv_paged_decode_scored``): scores capped to ``score_cap *
+    tanh(s / score_cap)`` (0: not), less ``slopes[head] * distance`` (fp32 ``[Hq]``), over the last ``window`` keys (0: all)
+    from key ``key_begin[b]`` on (int32 ``[B]``).  ``k_new``/``v_new`` ``[B, 1, Hkv, D]`` are appended first.  ``weights``
+    fp32 ``[B, Hkv, T]`` becomes ``decay * prior`` plus the attention weight of every cached token of the row (``prior`` may
+    be ``weights``; None: nothing earlier); give ``max_context_len`` then where the table is wide."""
+    out = _decode_out(q, out)
+    check(_front.decode_scored(q, out, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, max_context_len, scale,
+                               num_blocks, k_new, v_new, score_cap, slopes, window, key_begin, weights, prior, decay,
+                               workspace, stream))
     return out

@@ -9,8 +9,6 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <map>
@@ -18,47 +16,12 @@
 #include <string>
 #include <utility>
 
-#include "ffkv.h"
-#include "ffkv_internal.h"
+#include "capi_util.h"
+
+using namespace ffkv::capi;
 
 namespace
 {
-
-thread_local std::string g_last_error;
-
-int fail(int code, const char* fmt, ...)
-{
-    char    buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    g_last_error = buf;
-    return code;
-}
-
-int ok()
-{
-    g_last_error.clear();
-    return FFKV_OK;
-}
-
-bool is_act(int dt) { return dt == FFKV_DTYPE_F32 || dt == FFKV_DTYPE_F16 || dt == FFKV_DTYPE_BF16; }
-bool is_cache(int dt) { return is_act(dt) || dt == FFKV_DTYPE_I8 || dt == FFKV_DTYPE_FP8_E4M3; }
-bool quantized(int dt) { return dt == FFKV_DTYPE_I8 || dt == FFKV_DTYPE_FP8_E4M3; }
-// Append and decode take any head_dim that is a multiple of 8 up to 128 (as the reference's decode, one 8-element
-// vector per lane of a 16-lane group: src/kernels/attention.cu:307-316), and 256; prefill and rope+append take 64,
-// 128 and 256 (the reference's prefill and rope take 128, and 64 / 128).
-bool head_dim_ok(int d) { return d == 256 || (d >= 8 && d <= 128 && d % 8 == 0); }
-bool head_dim_mfma(int d) { return d == 64 || d == 128 || d == 256; }
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-int hip_fail(hipError_t e, const char* what)
-{
-    return fail(FFKV_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), static_cast<int>(e));
-}
 
 int env_chunk()
 {
@@ -81,8 +44,6 @@ bool env_force_generic()
     return v;
 }
 
-int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
-
 }  // namespace
 
 namespace ffkv
@@ -96,15 +57,7 @@ bool decode_use_mfma(int cache_dtype, int /*group*/, int head_dim)
            (head_dim_mfma(head_dim) || head_dim == 80 || head_dim == 96 || head_dim == 112);
 }
 
-// MFMA workspace layout: [row meta: batch x 2 int32 | (m, l): slots x num_heads x 2 fp32 | acc: slots x num_heads
-// x head_dim fp32], each region 256-byte aligned, slots = items + batch (slot = work item + row) plus, in
-// shared-prefix mode, prefix_chunks slots per row after those.  The public size query assumes kMfmaMaxItems items.
-struct MfmaLayout
-{
-    int64_t meta, ml, acc, total;
-};
-
-MfmaLayout mfma_layout(int batch, int num_heads, int head_dim, int prefix_chunks = 0, int items = kMfmaMaxItems)
+MfmaLayout mfma_layout(int batch, int num_heads, int head_dim, int prefix_chunks, int items)
 {
     const int64_t slots = static_cast<int64_t>(items) + batch + static_cast<int64_t>(prefix_chunks) * batch;
     MfmaLayout    l{};

@@ -1,0 +1,258 @@
+// capi_scored.cpp - the extern "C" boundary of attention under a score rule, attention weights and cache eviction
+// (include/ffkv.h): argument validation, workspaces and error reporting around the HIP launchers.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "capi_util.h"
+
+using namespace ffkv::capi;
+
+namespace
+{
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+float softmax_scale(float scale, int head_dim)
+{
+    return scale > 0.0f ? scale : 1.0f / sqrtf(static_cast<float>(head_dim));
+}
+
+// The rule's own arguments; FFKV_OK or the error.
+int check_rule(float score_cap, const float* slopes, int window, const int32_t* key_begin, const int32_t* key_end)
+{
+    if (!(score_cap >= 0.0f) || std::isinf(score_cap))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "score_cap must be finite and not negative, got %g",
+                    static_cast<double>(score_cap));
+    if (window < 0) return fail(FFKV_ERR_INVALID_ARGUMENT, "window must not be negative, got %d", window);
+    if (!aligned4(slopes) || !aligned4(key_begin) || !aligned4(key_end))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "slopes, key_begin and key_end must be 4-byte aligned");
+    return FFKV_OK;
+}
+
+ffkv::ScoreRule make_rule(float score_cap, const float* slopes, int window, const int32_t* key_begin,
+                          const int32_t* key_end)
+{
+    ffkv::ScoreRule r{};
+    r.cap = score_cap * kLog2e;  // the kernels' scores are in log2 units
+    r.inv_cap = score_cap > 0.0f ? 1.0f / r.cap : 0.0f;
+    if (!std::isfinite(r.cap) || !std::isfinite(r.inv_cap)) r.cap = r.inv_cap = 0.0f;  // beyond fp32: no score reaches it
+    r.window = window;
+    r.slopes = slopes;
+    r.key_begin = key_begin;
+    r.key_end = key_end;
+    return r;
+}
+
+int check_weights(const float* weights, const float* prior, float decay, int64_t weight_stride, int cap_tokens)
+{
+    if (prior != nullptr && weights == nullptr) return fail(FFKV_ERR_INVALID_ARGUMENT, "prior without weights");
+    if (weights == nullptr) return FFKV_OK;
+    if (!(decay >= 0.0f) || std::isinf(decay))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "decay must be finite and not negative, got %g", static_cast<double>(decay));
+    if (weight_stride < cap_tokens)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "weight_stride %lld is less than the rows' bound of %d tokens",
+                    static_cast<long long>(weight_stride), cap_tokens);
+    if (!aligned4(weights) || !aligned4(prior))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "weights and prior must be 4-byte aligned");
+    return FFKV_OK;
+}
+
+// The matrix-core decode takes it (whatever kernel the plain decode is forced to).
+bool scored_mfma(int cache_dtype, int head_dim)
+{
+    return cache_dtype != FFKV_DTYPE_F32 && (head_dim_mfma(head_dim) || head_dim == 80 || head_dim == 96 || head_dim == 112);
+}
+
+// Regions of the weights' pass behind the decode's partials: scores [batch, num_heads, stride] and final states
+// [batch, num_heads, 2].
+struct ScoreLayout
+{
+    int64_t stride, scores, final, total;
+};
+
+constexpr double kMostBytes = 1e15;
+
+ScoreLayout score_layout(int64_t at, int batch, int num_heads, int cap_tokens)
+{
+    ScoreLayout l{};
+    l.stride = ceil_div(cap_tokens, FFKV_BLOCK_SIZE) * FFKV_BLOCK_SIZE;
+    l.scores = align256(at);
+    l.final = l.scores + align256(static_cast<int64_t>(batch) * num_heads * l.stride * 4);
+    l.total = l.final + align256(static_cast<int64_t>(batch) * num_heads * 8);
+    return l;
+}
+
+bool score_layout_fits(int batch, int num_heads, int cap_tokens)
+{
+    return 4.0 * batch * num_heads * (static_cast<double>(cap_tokens) + 16) < kMostBytes;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ffkv_decode_scored_workspace_bytes(int batch, int num_heads, int head_dim, int max_blocks, int max_context_len,
+                                          int with_weights)
+{
+    const size_t plain = ffkv_decode_workspace_bytes(batch, num_heads, head_dim, max_blocks, max_context_len);
+    if (plain == 0 || with_weights == 0) return plain;
+    const int cap = ffkv::decode_cap_tokens(max_blocks, max_context_len);
+    if (!score_layout_fits(batch, num_heads, cap)) return 0;  // refused by the call
+    return static_cast<size_t>(score_layout(static_cast<int64_t>(plain), batch, num_heads, cap).total);
+}
+
+int ffkv_paged_decode_scored(const void* q, void* out, int qo_dtype, void* k_cache, void* v_cache, int cache_dtype,
+                             float* k_scale, float* v_scale, const int32_t* block_table, const int32_t* context_lens,
+                             int batch, int num_heads, int num_kv_heads, int head_dim, int block_size, int max_blocks,
+                             int num_blocks, int max_context_len, float scale, float score_cap, const float* slopes,
+                             int window, const int32_t* key_begin, const void* k_new, const void* v_new, int src_dtype,
+                             float* weights, const float* prior, float decay, int64_t weight_stride, void* workspace,
+                             size_t workspace_bytes, void* stream)
+{
+    if (block_size != FFKV_BLOCK_SIZE) return fail(FFKV_ERR_UNSUPPORTED, "block_size must be 16, got %d", block_size);
+    if (!is_act(qo_dtype)) return fail(FFKV_ERR_UNSUPPORTED, "unsupported q/out dtype %d", qo_dtype);
+    if (!is_cache(cache_dtype)) return fail(FFKV_ERR_UNSUPPORTED, "unsupported cache dtype %d", cache_dtype);
+    if (!head_dim_ok(head_dim))
+        return fail(FFKV_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 up to 128, or 256, got %d", head_dim);
+    if (batch < 0 || num_heads <= 0 || num_kv_heads <= 0 || max_blocks < 0 || num_blocks < 0)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "bad size (batch %d heads %d kv_heads %d max_blocks %d num_blocks %d)",
+                    batch, num_heads, num_kv_heads, max_blocks, num_blocks);
+    if (num_heads % num_kv_heads != 0)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "num_heads %d is not a multiple of num_kv_heads %d", num_heads,
+                    num_kv_heads);
+    const int  group = num_heads / num_kv_heads;
+    const bool mfma = scored_mfma(cache_dtype, head_dim);
+    if (group > 16 && !mfma)
+        return fail(FFKV_ERR_UNSUPPORTED, "GQA group size %d exceeds 16 (fp32 caches, or this head_dim)", group);
+    if (batch > 65535 || num_heads > 65535)
+        return fail(FFKV_ERR_UNSUPPORTED, "batch and num_heads must be <= 65535");
+    if (const int rc = check_rule(score_cap, slopes, window, key_begin, nullptr)) return rc;
+    if ((k_new == nullptr) != (v_new == nullptr))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "k_new and v_new come together");
+    if (k_new != nullptr && !is_act(src_dtype)) return fail(FFKV_ERR_UNSUPPORTED, "unsupported source dtype %d", src_dtype);
+    const int cap = ffkv::decode_cap_tokens(max_blocks, max_context_len);
+    if (const int rc = check_weights(weights, prior, decay, weight_stride, cap)) return rc;
+    if (batch == 0) return ok();
+    if (!q || !out || !k_cache || !v_cache || !block_table || !context_lens)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "null q, out, cache, block_table or context_lens pointer");
+    if (quantized(cache_dtype) && (!k_scale || !v_scale))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "quantized cache needs k_scale and v_scale");
+    if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_new) ||
+        !aligned16(v_new))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "q, out, cache, k_new and v_new pointers must be 16-byte aligned");
+    if (static_cast<int64_t>(batch) * ceil_div(cap, FFKV_BLOCK_SIZE) > INT32_MAX)
+        return fail(FFKV_ERR_UNSUPPORTED, "batch * pages per row exceeds 2^31 - 1 (batch %d, %d tokens per row)",
+                    batch, cap);
+    if (weights != nullptr && !score_layout_fits(batch, num_heads, cap))
+        return fail(FFKV_ERR_UNSUPPORTED, "the scores of %d x %d rows of %d tokens are too many: give max_context_len",
+                    batch, num_heads, cap);
+
+    ffkv::DecodeArgs a{};
+    a.q = q;
+    a.out = out;
+    a.k_cache = k_cache;
+    a.v_cache = v_cache;
+    a.k_scale = k_scale;
+    a.v_scale = v_scale;
+    a.block_table = block_table;
+    a.context_lens = context_lens;
+    a.qo_dtype = qo_dtype;
+    a.cache_dtype = cache_dtype;
+    a.batch = batch;
+    a.num_heads = num_heads;
+    a.num_kv_heads = num_kv_heads;
+    a.group = group;
+    a.head_dim = head_dim;
+    a.max_blocks = max_blocks;
+    a.num_blocks = num_blocks;
+    a.chunk = ffkv::decode_chunk(batch, num_kv_heads, cap);
+    a.max_chunks = static_cast<int>(ceil_div(cap > 0 ? cap : 1, a.chunk));
+    a.scale_log2 = softmax_scale(scale, head_dim) * kLog2e;
+    a.rule = make_rule(score_cap, slopes, window, key_begin, nullptr);
+
+    // Tokens that a row's query sees at most: a window's, which may begin and end inside a page.  The plain decode's rules
+    // for the number of work items and for its one-launch form go by these.
+    const int span = window > 0 ? static_cast<int>(std::min<int64_t>(cap, static_cast<int64_t>(window) + 2 * FFKV_BLOCK_SIZE))
+                                : cap;
+    a.cap_tokens = span;
+    const bool row = mfma && ffkv::decode_use_row(a);
+    if (mfma) a.items = std::min(ffkv::decode_scored_launch_items(a), ffkv::decode_most_items(batch, span));
+    a.cap_tokens = cap;
+
+    ffkv::MfmaLayout lay{};
+    int64_t          need = 0;
+    if (mfma && !row)
+    {
+        lay = ffkv::mfma_layout(batch, num_heads, head_dim, 0, a.items);
+        need = lay.total;
+    }
+    else if (!mfma && a.max_chunks > 1)
+    {
+        const int64_t parts = static_cast<int64_t>(batch) * num_heads * a.max_chunks;
+        lay.acc = align256(parts * 2 * 4);
+        need = lay.acc + parts * head_dim * 4;
+    }
+    ScoreLayout sl{};
+    if (weights != nullptr)
+    {
+        sl = score_layout(need, batch, num_heads, cap);
+        need = sl.total;
+    }
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    void*       ws = workspace;
+    bool        owned = false;
+    if (ws != nullptr && !aligned16(ws)) return fail(FFKV_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+    if (ws != nullptr && workspace_bytes < static_cast<size_t>(need))
+        return fail(FFKV_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %lld bytes needed", workspace_bytes,
+                    static_cast<long long>(need));
+    if (ws == nullptr && need > 0)
+    {
+        const hipError_t e = hipMallocAsync(&ws, static_cast<size_t>(need), s);
+        if (e != hipSuccess) return hip_fail(e, "decode workspace hipMallocAsync");
+        owned = true;
+    }
+    char* wsb = static_cast<char*>(ws);
+    if (mfma && !row) a.ws_meta = reinterpret_cast<int32_t*>(wsb + lay.meta);
+    if (lay.acc > 0)
+    {
+        a.ws_ml = reinterpret_cast<float*>(wsb + lay.ml);
+        a.ws_acc = reinterpret_cast<float*>(wsb + lay.acc);
+    }
+    if (weights != nullptr)
+    {
+        a.ws_scores = reinterpret_cast<float*>(wsb + sl.scores);
+        a.ws_final = reinterpret_cast<float*>(wsb + sl.final);
+        a.score_stride = sl.stride;
+        a.weights = weights;
+        a.prior = prior;
+        a.decay = decay;
+        a.weight_stride = weight_stride;
+    }
+
+    hipError_t e = hipSuccess;
+    if (k_new != nullptr)
+    {
+        if (mfma && src_dtype == cache_dtype)  // 16-bit: the decode kernel writes the step's token to its page and attends it
+        {
+            a.k_new = k_new;
+            a.v_new = v_new;
+        }
+        else
+        {
+            ffkv::AppendArgs ap{k_new, v_new, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, src_dtype,
+                                cache_dtype, batch, 1, num_kv_heads, head_dim, max_blocks, num_blocks};
+            e = ffkv::launch_append(ap, s);
+        }
+    }
+    if (e == hipSuccess) e = ffkv::launch_decode_scored(a, mfma, row, s);
+    if (owned)
+    {
+        const hipError_t fe = hipFreeAsync(ws, s);
+        if (e == hipSuccess) e = fe;
+    }
+    if (e != hipSuccess) return hip_fail(e, "scored decode launch");
+    return ok();
+}
+
+}  // extern "C"

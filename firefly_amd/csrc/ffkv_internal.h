@@ -53,6 +53,17 @@ struct RopeArgs
     float          theta;
 };
 
+// How scores are changed and which keys are seen (score_rule.h).  All zero: plain causal attention.
+struct ScoreRule
+{
+    float          cap;      // tanh cap of the scores in log2 units (0: none)
+    float          inv_cap;  // its reciprocal
+    int            window;   // keys j <= i - window of position i are hidden (0: none)
+    const float*   slopes;   // [num_heads]: score -= slope * |i - j| (null: none)
+    const int32_t* key_begin;  // decode [batch], else [batch, seq_len]: first visible key of each query (null: 0)
+    const int32_t* key_end;    // [batch, seq_len]: end of the visible keys (null: causal); not in the decode
+};
+
 struct PrefillArgs
 {
     const void*    q;    // [B, S, Hq, D]
@@ -94,6 +105,7 @@ struct PrefillArgs
     int            split_slots;
     int            split_from;
     int32_t*       ws_pieces;  // [row blocks]: pieces of each
+    ScoreRule      rule;       // launch_prefill_scored only
 };
 
 struct DecodeArgs
@@ -140,6 +152,17 @@ struct DecodeArgs
     // tokens of rows cut short by cap_tokens).
     const void*    k_new;
     const void*    v_new;
+    // Scored decode only (launch_decode_scored): the rule; with weights, the scores of all visible keys in log2 units,
+    // [batch, num_heads, score_stride] fp32, each row's final (max, denominator) per head, [batch, num_heads, 2], and the
+    // weights themselves (decay * prior + what this call gives), [batch, num_kv_heads, weight_stride].
+    ScoreRule      rule;
+    float*         ws_scores;  // null: no weights
+    float*         ws_final;
+    int64_t        score_stride;
+    float*         weights;
+    const float*   prior;  // null: nothing earlier
+    float          decay;
+    int64_t        weight_stride;
 };
 
 hipError_t launch_append(const AppendArgs& a, hipStream_t stream);
@@ -172,6 +195,12 @@ int decode_mfma_launch_items(const DecodeArgs& a);
 bool       decode_use_row(const DecodeArgs& a);
 hipError_t launch_decode_row(const DecodeArgs& a, hipStream_t stream);
 bool decode_use_mfma(int cache_dtype, int group, int head_dim);
+// The decode under a score rule (paged_decode_scored.hip): `mfma` as the plain decode is chosen, `row` its one-launch form
+// (16- and 8-bit caches at the matrix cores' head dims, else the vector kernel), and the work items of the former.
+int        decode_scored_launch_items(const DecodeArgs& a);
+hipError_t launch_decode_scored(const DecodeArgs& a, bool mfma, bool row, hipStream_t stream);
+hipError_t launch_decode_scored_generic(const DecodeArgs& a, hipStream_t stream);
+hipError_t launch_decode_weights(const DecodeArgs& a, hipStream_t stream);  // the weights from the scores
 
 // Fused shared-prefix decode (paged_decode_pfx.hip): the prefix partials and the decode of the rows' own pages in
 // one grid, then the merge.  decode_pfx_plan sizes it for `a` (dtypes, batch, heads, head_dim set) over

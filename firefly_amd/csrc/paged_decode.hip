@@ -18,6 +18,7 @@
 // kernel is bound by memory latency, not by its arithmetic.
 #include "ffkv_device.h"
 #include "ffkv_internal.h"
+#include "score_rule.h"
 
 namespace ffkv
 {
@@ -79,8 +80,9 @@ __device__ __forceinline__ int row_tokens(const DecodeArgs& a, int b)
 }  // namespace
 
 // DT: head_dim, or 0 for a runtime head_dim (a multiple of 8 up to 8 * LPT); LPT: lanes per token, a power of two
-// (DT / 8 when DT is given).  Lanes past head_dim / 8 hold zeros and store nothing.
-template <int CT, int DT, int LPT, int GP>
+// (DT / 8 when DT is given).  Lanes past head_dim / 8 hold zeros and store nothing.  RULE: the scores are changed and the
+// keys bounded by a.rule, and with a.ws_scores the scores and the rows' final states are written down for the weights.
+template <int CT, int DT, int LPT, int GP, bool RULE = false>
 __global__ __launch_bounds__(256) void paged_decode_generic(DecodeArgs a)
 {
     static_assert(DT == 0 || DT == 8 * LPT, "a given head_dim has head_dim / 8 lanes per token");
@@ -98,12 +100,22 @@ __global__ __launch_bounds__(256) void paged_decode_generic(DecodeArgs a)
     const int wave = tid / 64;
     const bool act = DT != 0 || lane * 8 < D;  // this lane holds dims of the head
 
-    const int L = row_tokens(a, b);
+    RowSpan span{0, 0, 0};
+    if constexpr (RULE) span = row_span(a, b);
+    const int L = RULE ? span.hi : row_tokens(a, b);
     const int nch = (L + a.chunk - 1) / a.chunk;
     if (chunk_id >= nch && !(chunk_id == 0 && nch == 0)) return;  // uniform over the workgroup
-    const int begin = chunk_id * a.chunk;
-    const int end = min(begin + a.chunk, L);
+    // (RULE: chunks before the row's first visible key have no tokens and leave an empty piece)
+    const int begin = RULE ? max(chunk_id * a.chunk, span.lo & ~15) : chunk_id * a.chunk;
+    const int end = min(chunk_id * a.chunk + a.chunk, L);
     const int G = a.group;
+    float     slope[RULE ? GP : 1];
+    if constexpr (RULE)
+    {
+#pragma unroll
+        for (int g = 0; g < GP; ++g)
+            slope[g] = a.rule.slopes != nullptr && g < G ? a.rule.slopes[kvh * G + g] * 1.4426950408889634f : 0.0f;
+    }
 
     const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
     // the chunk's first page in this row and in one of the 256 rows around it, a thread each (see `once`)
@@ -190,7 +202,7 @@ __global__ __launch_bounds__(256) void paged_decode_generic(DecodeArgs a)
             for (int u = 0; u < U; ++u)
             {
                 const int j = base + u * TPI + slot;
-                valid[u] = j < end && phys[u] >= 0 && phys[u] < a.num_blocks;
+                valid[u] = j < end && phys[u] >= 0 && phys[u] < a.num_blocks && (!RULE || j >= span.lo);
                 row[u] = (static_cast<size_t>(valid[u] ? phys[u] : 0) * kBlockSize + (j & 15)) * a.num_kv_heads + kvh;
             }
             Raw8 kr[U], vr[U];
@@ -243,6 +255,22 @@ __global__ __launch_bounds__(256) void paged_decode_generic(DecodeArgs a)
 #pragma unroll
                 for (int g = 0; g < GP; ++g) s[g] = group_sum<LPT>(s[g]);
 
+                const int j = base + u * TPI + slot;
+                if constexpr (RULE)
+                {
+#pragma unroll
+                    for (int g = 0; g < GP; ++g)
+                    {
+                        s[g] *= a.scale_log2;
+                        if (a.rule.cap > 0.0f) s[g] = cap_score(s[g], a.rule.cap, a.rule.inv_cap);
+                        if (a.rule.slopes != nullptr)  // j - i <= 0
+                            s[g] = __builtin_fmaf(slope[g], static_cast<float>(j - span.pos), s[g]);
+                        if (a.ws_scores != nullptr && g < G && lane == 0 && j < end)
+                            a.ws_scores[(static_cast<int64_t>(b) * a.num_heads + kvh * G + g) * a.score_stride + j] =
+                                valid[u] ? s[g] : -__builtin_huge_valf();
+                    }
+                }
+
                 // Online softmax with a lazy reference: m moves (and l, acc are rescaled) only when a score exceeds it
                 // by more than 8 (log2 units), so p = 2^(s - m) < 2^8 and most tokens only add p and p * v.
                 if (valid[u])
@@ -258,7 +286,7 @@ __global__ __launch_bounds__(256) void paged_decode_generic(DecodeArgs a)
 #pragma unroll
                     for (int g = 0; g < GP; ++g)
                     {
-                        const float sg = s[g] * a.scale_log2;
+                        const float sg = RULE ? s[g] : s[g] * a.scale_log2;
                         if (sg > m[g] + 8.0f)
                         {
                             const float alpha = fast_exp2(m[g] - sg);  // 0 for the slot's first token
@@ -362,6 +390,10 @@ __global__ __launch_bounds__(256) void paged_decode_generic(DecodeArgs a)
             const float lsum = s_l[g];
             store_act1(a.out, a.qo_dtype, (static_cast<size_t>(b) * a.num_heads + hq0 + g) * D + d,
                        lsum == 0.0f ? 0.0f : acc_v / lsum);
+            if constexpr (RULE)
+                if (a.ws_final != nullptr && d == 0)
+                    reinterpret_cast<float2*>(a.ws_final)[static_cast<int64_t>(b) * a.num_heads + hq0 + g] =
+                        make_float2(s_m[g], lsum);
         }
         else
         {
@@ -380,6 +412,8 @@ __global__ __launch_bounds__(256) void paged_decode_generic(DecodeArgs a)
 // 4 (k % (D/4)) .. + 3 of head k / (D/4) over the row's chunks, the loads of MF chunks in flight together (one
 // workgroup per head, its threads walking the chunks three times with one load in flight, took 11.6 us on 32 rows of
 // 512 to 4096 tokens; this takes 5.0).
+// FIN: the rows' (max, denominator) of each head go to ws_final too (null: not asked for).
+template <bool FIN = false>
 __global__ __launch_bounds__(256) void paged_decode_merge(DecodeArgs a)
 {
     constexpr int MF = 8;
@@ -428,34 +462,37 @@ __global__ __launch_bounds__(256) void paged_decode_merge(DecodeArgs a)
     const size_t ob = (static_cast<size_t>(b) * a.num_heads + h) * D + d4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) store_act1(a.out, a.qo_dtype, ob + i, o[i] * inv);
+    if constexpr (FIN)
+        if (a.ws_final != nullptr && d4 == 0)
+            reinterpret_cast<float2*>(a.ws_final)[static_cast<int64_t>(b) * a.num_heads + h] = make_float2(m, l);
 }
 
 namespace
 {
 
-template <int CT, int DT, int LPT, int GP>
+template <int CT, int DT, int LPT, int GP, bool RULE>
 hipError_t launch3(const DecodeArgs& a, hipStream_t stream)
 {
     dim3 grid(static_cast<unsigned>(a.max_chunks), static_cast<unsigned>(a.num_kv_heads),
               static_cast<unsigned>(a.batch));
-    hipLaunchKernelGGL((paged_decode_generic<CT, DT, LPT, GP>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((paged_decode_generic<CT, DT, LPT, GP, RULE>), grid, dim3(256), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.max_chunks <= 1) return e;
-    hipLaunchKernelGGL(paged_decode_merge,
+    hipLaunchKernelGGL(paged_decode_merge<RULE>,
                        dim3(static_cast<unsigned>(a.batch),
                             static_cast<unsigned>((a.num_heads * (a.head_dim / 4) + 255) / 256)),
                        dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
-template <int CT, int DT, int LPT>
+template <int CT, int DT, int LPT, bool RULE = false>
 hipError_t launch2(const DecodeArgs& a, hipStream_t stream)
 {
-    if (a.group <= 1) return launch3<CT, DT, LPT, 1>(a, stream);
-    if (a.group <= 2) return launch3<CT, DT, LPT, 2>(a, stream);
-    if (a.group <= 4) return launch3<CT, DT, LPT, 4>(a, stream);
-    if (a.group <= 8) return launch3<CT, DT, LPT, 8>(a, stream);
-    return launch3<CT, DT, LPT, 16>(a, stream);
+    if (a.group <= 1) return launch3<CT, DT, LPT, 1, RULE>(a, stream);
+    if (a.group <= 2) return launch3<CT, DT, LPT, 2, RULE>(a, stream);
+    if (a.group <= 4) return launch3<CT, DT, LPT, 4, RULE>(a, stream);
+    if (a.group <= 8) return launch3<CT, DT, LPT, 8, RULE>(a, stream);
+    return launch3<CT, DT, LPT, 16, RULE>(a, stream);
 }
 
 template <int CT>
@@ -475,6 +512,27 @@ hipError_t launch1(const DecodeArgs& a, hipStream_t stream)
 }
 
 }  // namespace
+
+// fp32 caches at every head_dim, the others at those the matrix cores do not take.
+hipError_t launch_decode_scored_generic(const DecodeArgs& a, hipStream_t stream)
+{
+    switch (a.cache_dtype)
+    {
+        case F32:
+            if (a.head_dim == 64) return launch2<F32, 64, 8, true>(a, stream);
+            if (a.head_dim == 128) return launch2<F32, 128, 16, true>(a, stream);
+            if (a.head_dim == 256) return launch2<F32, 256, 32, true>(a, stream);
+            return launch2<F32, 0, 16, true>(a, stream);
+        case F16:
+            return launch2<F16, 0, 16, true>(a, stream);
+        case BF16:
+            return launch2<BF16, 0, 16, true>(a, stream);
+        case I8:
+            return launch2<I8, 0, 16, true>(a, stream);
+        default:
+            return launch2<FP8, 0, 16, true>(a, stream);
+    }
+}
 
 hipError_t launch_decode(const DecodeArgs& a, hipStream_t stream)
 {

@@ -33,6 +33,7 @@
 //     window), block-table entries come 64 per vector load, and the next row's Q is loaded as soon as the last
 //     page of a row has been scored, so a wave never waits on a dependent scalar load between pages.
 #include "mfma_common.h"
+#include "score_rule.h"
 
 
 #ifndef FFKV_MFMA_MAX_WAVES
@@ -64,6 +65,8 @@ struct PageRegs
     int   nb;  // pages of the row
     int   lp;  // attended tokens of the row
     int   ns;  // fused append: slot of the row's new token in this page, else -1
+    int   lo;  // RULE: first visible slot of the row's first page, its first page, and the query's position
+    int   first, pos;
     float ks;  // int8 caches: K and V scale of token c (lane c of each lane group)
     float vs;
 };
@@ -175,10 +178,12 @@ constexpr int kMfmaMaxWaves =
 // weigh the first pfx_items items less (the fused shared-prefix launch); the plain decode's split otherwise.
 // ROW: the workgroup is one row (item_) and one KV head, or block of 16 of its query heads (y_); its nw_ waves share the
 // row's pages, combine their states through LDS (s_v, as row_lds_bytes sizes it) and write the output: no partials.
-template <int CT, int QT, int D, bool PW = false, bool ROW = false>
+// RULE: the scores are changed and the keys bounded by a.rule (a row's pages begin at its first visible key), and with
+// a.ws_scores the visible keys' scores and the rows' final (max, denominator) are written down for the weights.
+template <int CT, int QT, int D, bool PW = false, bool ROW = false, bool RULE = false>
 __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_, int n_items_, int nw_, uint16_t* s_v)
 {
-    static_assert(!(PW && ROW), "one split or the other");
+    static_assert(!(PW && (ROW || RULE)), "one split or the other; no rule over a shared prefix");
     // (the plain decode reads its indices where it uses them: held in registers from the start, they cost the
     // kernel scalar registers it spills)
     auto item_of = [&]() { return PW || ROW ? item_ : static_cast<int>(blockIdx.x); };
@@ -228,12 +233,23 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         int w0, base, total;
         int toks, n, excl;  // per lane
         int whole;          // per lane: the row's new token (position context_lens) is attended (not truncated)
+        int lo, first, pos;  // RULE, per lane: first visible slot of the row's first page, that page, the position
     };
     auto load_win = [&](int w0, int base)
     {
         const int r = w0 + lane;
         int       t = 0;
         int       whole = 0;
+        if constexpr (RULE)
+        {
+            RowSpan s{0, 0, 0};
+            if (r < B) s = row_span(a, r);
+            const int first = s.lo >> 4;
+            const int n = s.hi > s.lo ? (s.hi + kBlockSize - 1) / kBlockSize - first : 0;
+            const int incl = wave_scan(n);
+            return Win{w0, base, __builtin_amdgcn_readlane(incl, 63), s.hi - first * kBlockSize, n, incl - n,
+                       n > 0 && s.hi == s.pos + 1, s.lo & 15, first, s.pos};
+        }
         if (r < B)
         {
             int64_t L = static_cast<int64_t>(a.context_lens[r]) + 1;  // +1: the token appended this step (:320)
@@ -247,7 +263,7 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         t = t - a.skip_blocks * kBlockSize;
         t = t < 0 ? 0 : t;
         const int incl = wave_scan(n);
-        return Win{w0, base, __builtin_amdgcn_readlane(incl, 63), t, n, incl - n, whole};
+        return Win{w0, base, __builtin_amdgcn_readlane(incl, 63), t, n, incl - n, whole, 0, 0, 0};
     };
 
     // The new tokens (fused append) of the rows in `cut`, counted from row r0, to their slots: rows cut short by
@@ -278,7 +294,17 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
     // ROW: the row's length and its first 64 table entries are loaded together (an entry past the row's pages is never
     // used), so a row of up to 1024 tokens waits for memory once before its pages go out.
     int row_toks = 0, row_whole = 0, row_tvec = -1;
-    if constexpr (ROW)
+    RowSpan row_sp{0, 0, 0};
+    if constexpr (ROW && RULE)
+    {
+        row_tvec = lane < a.max_blocks ? a.block_table[static_cast<int64_t>(item_) * a.max_blocks + lane] : -1;
+        row_sp = row_span(a, item_);
+        const bool any = row_sp.hi > row_sp.lo;
+        row_toks = any ? row_sp.hi - (row_sp.lo & ~15) : 0;
+        row_whole = any && row_sp.hi == row_sp.pos + 1;
+        if (a.k_new != nullptr && !row_whole && y_ == 0 && wave == 0) copy_cut(1, item_);
+    }
+    else if constexpr (ROW)
     {
         row_tvec = lane < a.max_blocks ? a.block_table[static_cast<int64_t>(item_) * a.max_blocks + lane] : -1;
         int64_t L = static_cast<int64_t>(a.context_lens[item_]) + 1;  // +1: the token appended this step (:320)
@@ -377,6 +403,7 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         int            b, pb, nb, lp;
         const int32_t* table;
         int            ns;  // fused append: slot of the new token in the row's last page, or -1
+        int            lo, first, pos;  // RULE: as in Win
     };
     Win  win = win0;  // window of the most advanced row found so far
     auto row_at = [&](int b)  // row b, which lies in `win`
@@ -384,8 +411,10 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         const int l = b - win.w0;
         const int toks = __builtin_amdgcn_readlane(win.toks, l);
         const int ns = a.k_new != nullptr && toks > 0 && __builtin_amdgcn_readlane(win.whole, l) ? (toks - 1) & 15 : -1;
+        const int first = RULE ? __builtin_amdgcn_readlane(win.first, l) : a.skip_blocks;
         return LRow{b, win.base + __builtin_amdgcn_readlane(win.excl, l), __builtin_amdgcn_readlane(win.n, l), toks,
-                    a.block_table + static_cast<int64_t>(b) * a.max_blocks + a.skip_blocks, ns};
+                    a.block_table + static_cast<int64_t>(b) * a.max_blocks + first, ns,
+                    RULE ? __builtin_amdgcn_readlane(win.lo, l) : 0, first, RULE ? __builtin_amdgcn_readlane(win.pos, l) : 0};
     };
     auto find_page = [&](int x)  // row holding page x (x < P), moving `win` forward from its current window
     {
@@ -410,12 +439,13 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
 
     LRow lrow;
     if constexpr (ROW)
-        lrow = LRow{item_, 0, P, row_toks, a.block_table + static_cast<int64_t>(item_) * a.max_blocks,
-                    a.k_new != nullptr && row_toks > 0 && row_whole ? (row_toks - 1) & 15 : -1};
+        lrow = LRow{item_, 0, P, row_toks, a.block_table + static_cast<int64_t>(item_) * a.max_blocks + (row_sp.lo >> 4),
+                    a.k_new != nullptr && row_toks > 0 && row_whole ? (row_toks - 1) & 15 : -1,
+                    row_sp.lo & 15, row_sp.lo >> 4, row_sp.pos};
     else
         lrow = find_page(start);
     int  tb = (start - lrow.pb) & ~63;
-    int  tvec = ROW && tb == 0 ? row_tvec : load_tvec(lrow, tb);
+    int  tvec = ROW && tb == 0 && (!RULE || lrow.first == 0) ? row_tvec : load_tvec(lrow, tb);
     LRow lnxt = lrow;
     int  ntvec = -1;
     auto look_ahead = [&]()  // fetch the row after lrow if the item reaches it
@@ -451,6 +481,12 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         r.pb = lrow.pb;
         r.nb = lrow.nb;
         r.lp = lrow.lp;
+        if constexpr (RULE)
+        {
+            r.lo = pg == 0 ? lrow.lo : 0;
+            r.first = lrow.first;
+            r.pos = lrow.pos;
+        }
         r.phys = phys;
         r.ok = phys >= 0 && phys < a.num_blocks;  // uniform: a masked page is skipped
         r.ns = pg == lrow.nb - 1 ? lrow.ns : -1;  // fused append: the new token sits in the row's last page
@@ -598,7 +634,8 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
 
     // Stage a loaded page: V rows into the wave's LDS tile, scores S^T = K Q^T into s.  Consumes r.k and r.v,
     // so the next page can be loaded into r right after.
-    auto stage_page = [&](int n_tok, const PageRegs<NW, NWV>& r, f32x4& s)
+    // (RULE: slots below n_lo are hidden too)
+    auto stage_page = [&](int n_tok, int n_lo, const PageRegs<NW, NWV>& r, f32x4& s)
     {
         if constexpr (kElemBytes<CT> == 2)
         {
@@ -625,7 +662,7 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         for (int j = 0; j < NWV; ++j)
         {
             const int  t = v_tok(j);
-            const bool tok_ok = t < n_tok;
+            const bool tok_ok = t < n_tok && (!RULE || t >= n_lo);
             if (t >= kBlockSize) continue;
             if constexpr (kElemBytes<CT> == 2)
             {
@@ -667,9 +704,26 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         }
     };
 
-    // Online softmax of a staged page's scores and PV from its LDS tile.  tks / tvs: int8 scales of token c.
-    auto finish_page = [&](int n_tok, float tks, float tvs, f32x4 s)
+    // RULE: the rule's cap and slope of this lane's head; the scores of page `page` of row b written down for the weights
+    float rule_cap = 0.0f, rule_inv = 0.0f, rule_slope = 0.0f;
+    if constexpr (RULE)
     {
+        rule_cap = a.rule.cap;
+        rule_inv = a.rule.inv_cap;
+        if (a.rule.slopes != nullptr && c < gc) rule_slope = a.rule.slopes[kvh * G + h0 + c] * 1.4426950408889634f;
+    }
+    auto write_scores = [&](int b, int page, f32x4 sc)
+    {
+        if (c < gc)
+            *reinterpret_cast<f32x4*>(a.ws_scores +
+                                      (static_cast<int64_t>(b) * a.num_heads + kvh * G + h0 + c) * a.score_stride +
+                                      static_cast<int64_t>(page) * kBlockSize + 4 * g) = sc;
+    };
+
+    // Online softmax of a staged page's scores and PV from its LDS tile.  tks / tvs: int8 scales of token c.
+    auto finish_page = [&](int n_tok, int n_lo, int b, int page, int pos, float tks, float tvs, f32x4 s)
+    {
+        auto seen = [&](int t) { return t < n_tok && (!RULE || t >= n_lo); };
         float ks[4], vs[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -691,10 +745,19 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
 #pragma unroll
         for (int i = 0; i < 4; ++i)
         {
-            const bool ok = 4 * g + i < n_tok;
-            sc[i] = ok ? s[i] * ks[i] * kv_scale_log2 : kNegInf;
+            const bool ok = seen(4 * g + i);
+            float      v = s[i] * ks[i] * kv_scale_log2;
+            if constexpr (RULE)
+            {
+                if (rule_cap > 0.0f) v = cap_score(v, rule_cap, rule_inv);
+                if (a.rule.slopes != nullptr)  // j - i <= 0
+                    v = __builtin_fmaf(rule_slope, static_cast<float>(page * kBlockSize + 4 * g + i - pos), v);
+            }
+            sc[i] = ok ? v : kNegInf;
             mt = fmaxf(mt, sc[i]);
         }
+        if constexpr (RULE)
+            if (a.ws_scores != nullptr) write_scores(b, page, f32x4{sc[0], sc[1], sc[2], sc[3]});
         mt = xor_max(mt);
         const float m_new = fmaxf(m_run, mt);
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
@@ -705,7 +768,7 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         {
             const float pr = __builtin_amdgcn_exp2f(sc[i] - m_new);
             psum += pr;
-            pv[i] = 4 * g + i < n_tok ? pr * vs[i] : 0.0f;
+            pv[i] = seen(4 * g + i) ? pr * vs[i] : 0.0f;
         }
         l_run = l_run * alpha + psum;
         if (__any(m_new > m_run))
@@ -767,6 +830,10 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
                 for (int n = 0; n < NT; ++n)
                     store_out4<QT>(a.out, (static_cast<size_t>(b) * a.num_heads + h) * D + 16 * n + 4 * g,
                                    acc[n] * inv);
+                if constexpr (RULE)
+                    if (a.ws_final != nullptr && g == 0)
+                        reinterpret_cast<float2*>(a.ws_final)[static_cast<int64_t>(b) * a.num_heads + h] =
+                            float2{m_run, l_tot};
             }
         }
         else if (c < gc)
@@ -810,8 +877,9 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         const bool    ok = cur.ok;
         const int     n_tok = min(kBlockSize, cur.lp - (p - pb) * kBlockSize);
         const bool    row_ends = p + 1 == pb + nb;
+        const int     n_lo = RULE ? cur.lo : 0, page = RULE ? cur.first + p - pb : 0, pos = RULE ? cur.pos : 0;
         f32x4         s;
-        if (ok) stage_page(n_tok, cur, s);
+        if (ok) stage_page(n_tok, n_lo, cur, s);
         // The scores of page p have consumed Q: a new row's Q is loaded now, ahead of page p + DEPTH's K/V when
         // page p + 1 is already in flight (loads complete in issue order for the wait counter).
         if constexpr (DEPTH > 1)
@@ -819,7 +887,9 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         if (p + DEPTH < end) load_next(cur);
         if constexpr (DEPTH == 1)
             if (!ROW && row_ends && p + 1 < end) load_q(cur.b);
-        if (ok) finish_page(n_tok, tks, tvs, s);
+        if (ok) finish_page(n_tok, n_lo, b, page, pos, tks, tvs, s);
+        if constexpr (RULE)
+            if (!ok && a.ws_scores != nullptr) write_scores(b, page, f32x4{kNegInf, kNegInf, kNegInf, kNegInf});
         if (!ROW && (row_ends || p + 1 == end))
         {
             finish_segment(b, pb, nb, seg_start, p + 1);
@@ -872,6 +942,10 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
             }
             store_out4<QT>(a.out, (static_cast<size_t>(item_) * a.num_heads + kvh * G + h0 + h) * D + d4,
                            o * softmax_inv(L));
+            if constexpr (RULE)
+                if (a.ws_final != nullptr && d4 == 0)
+                    reinterpret_cast<float2*>(a.ws_final)[static_cast<int64_t>(item_) * a.num_heads + kvh * G + h0 + h] =
+                        float2{M, L};
         }
     }
 }
@@ -907,8 +981,9 @@ void paged_decode_mfma(DecodeArgs a)
 // Combine the partials of rows split over several work items.
 // One workgroup of MW waves per (row, head): wave w folds segments i_lo + w, i_lo + w + MW, ... into an online
 // (max, denominator, output) state (lane = D/64 dims), then the waves' states are combined through LDS.
-// MW waves per (row, head): as many as the rows have pieces for (launch_merge).
-template <int QT, int D, int MW>
+// MW waves per (row, head): as many as the rows have pieces for (launch_merge).  FIN: the row's (max, denominator) of each
+// head goes to ws_final too (null: not asked for).
+template <int QT, int D, int MW, bool FIN = false>
 __global__ __launch_bounds__(64 * MW) void paged_decode_mfma_merge(DecodeArgs a)
 {
     constexpr int PER = (D + 63) / 64;  // dims per lane (head_dim 96: lanes 0 .. 47 hold two)
@@ -994,6 +1069,9 @@ __global__ __launch_bounds__(64 * MW) void paged_decode_mfma_merge(DecodeArgs a)
             O += s_o[w][d] * wt;
         }
         store_act1(a.out, QT, ob + d, L == 0.0f ? 0.0f : O / L);
+        if constexpr (FIN)
+            if (a.ws_final != nullptr && d == 0)
+                reinterpret_cast<float2*>(a.ws_final)[static_cast<int64_t>(b) * a.num_heads + h] = float2{M, L};
     }
 }
 
@@ -1001,7 +1079,7 @@ __global__ __launch_bounds__(64 * MW) void paged_decode_mfma_merge(DecodeArgs a)
 // workgroups owns output dims 4(k % (D/4)) .. +3 of head k / (D/4), folds that chunk of every piece of the row
 // (loads of up to MF = 16 pieces in flight together) and writes it; no cross-thread combine.  Rows written whole by
 // the decode kernel (one piece, no shared-prefix partials) or without tokens are left alone.
-template <int QT, int D>
+template <int QT, int D, bool FIN = false>
 __global__ __launch_bounds__(256) void paged_decode_mfma_merge_rows(DecodeArgs a)
 {
     constexpr int MF = 16;
@@ -1054,6 +1132,9 @@ __global__ __launch_bounds__(256) void paged_decode_mfma_merge_rows(DecodeArgs a
     }
     store_out4<QT>(a.out, (static_cast<size_t>(b) * a.num_heads + h) * D + d4,
                    o * softmax_inv(l));
+    if constexpr (FIN)
+        if (a.ws_final != nullptr && d4 == 0)
+            reinterpret_cast<float2*>(a.ws_final)[static_cast<int64_t>(b) * a.num_heads + h] = float2{m, l};
 }
 
 namespace
@@ -1090,21 +1171,21 @@ int items_m3(const DecodeArgs& a)
 // rows (8) 21.0 / 19.5 / 19.8 / 22.9; 64 rows (4) 28.7 / 25.8 / 24.8 / 25.9, of 512 to 4096 tokens 108.7 / 106.1 / 105.1 /
 // 106.1; 128 rows (2) 35.0 / 28.9 / 26.9 / 26.2.  16 rows (16) take 16 waves (27.7 against 27.9 with 8, 256 to 2048
 // tokens), 120 rows over a shared prefix (2 and 4 chunks) one thread (66.8 against 67.0 with 4 waves).
-template <int QT, int D>
+template <int QT, int D, bool FIN = false>
 hipError_t launch_merge(const DecodeArgs& a, int items, hipStream_t stream)
 {
     const int  pieces = items / a.batch + a.pfx_chunks;
     const dim3 per_head(static_cast<unsigned>(a.batch), static_cast<unsigned>(a.num_heads));
     if (pieces >= 16)
-        hipLaunchKernelGGL((paged_decode_mfma_merge<QT, D, 16>), per_head, dim3(1024), 0, stream, a);
+        hipLaunchKernelGGL((paged_decode_mfma_merge<QT, D, 16, FIN>), per_head, dim3(1024), 0, stream, a);
     else if (pieces >= 8)
-        hipLaunchKernelGGL((paged_decode_mfma_merge<QT, D, 8>), per_head, dim3(512), 0, stream, a);
+        hipLaunchKernelGGL((paged_decode_mfma_merge<QT, D, 8, FIN>), per_head, dim3(512), 0, stream, a);
     else if (pieces >= 4 && a.pfx_chunks == 0)
-        hipLaunchKernelGGL((paged_decode_mfma_merge<QT, D, 4>), per_head, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((paged_decode_mfma_merge<QT, D, 4, FIN>), per_head, dim3(256), 0, stream, a);
     else
     {
         const dim3 mgrid(static_cast<unsigned>(a.batch), static_cast<unsigned>((a.num_heads * (D / 4) + 255) / 256));
-        hipLaunchKernelGGL((paged_decode_mfma_merge_rows<QT, D>), mgrid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((paged_decode_mfma_merge_rows<QT, D, FIN>), mgrid, dim3(256), 0, stream, a);
     }
     return hipGetLastError();
 }

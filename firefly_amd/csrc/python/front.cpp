@@ -11,7 +11,9 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <cstdarg>
 #include <cstdint>
+#include <initializer_list>
 #include <vector>
 
 #include "ffkv.h"
@@ -30,10 +32,12 @@ struct Functions
     decltype(&ffkv_paged_prefill_ws)           prefill;
     decltype(&ffkv_rope)                       rope;
     decltype(&ffkv_rope_append)                rope_append;
+    decltype(&ffkv_paged_decode_scored)        decode_scored;
 };
 Functions fn{};
 
-PyObject *s_shape, *s_dtype, *s_data_ptr, *s_nbytes, *s_cuda_stream;
+PyObject *s_shape, *s_dtype, *s_data_ptr, *s_nbytes, *s_cuda_stream, *s_device, *s_index, *s_is_contiguous, *s_is_cuda;
+constexpr int kInt32 = 4;  // int32 among bind()'s dtypes: tables and lengths, no dtype of activations or caches
 struct DtypeCode
 {
     PyObject* dtype;
@@ -109,7 +113,7 @@ struct Reader
         if (d != nullptr)
         {
             for (const DtypeCode& c : dtypes)
-                if (c.dtype == d)
+                if (c.dtype == d && c.code != kInt32)
                 {
                     Py_DECREF(d);
                     return c.code;
@@ -142,6 +146,78 @@ struct Reader
         Py_XDECREF(f);
         if (f == nullptr) ok = false;
         return static_cast<float>(v);
+    }
+    bool refuse(PyObject* error, const char* format, ...)
+    {
+        va_list va;
+        va_start(va, format);
+        PyErr_FormatV(error, format, va);
+        va_end(va);
+        return ok = false;
+    }
+    // t's (or None's, where that is allowed) dtype is `code`, its sizes are `dims` (-1: any), it is contiguous, and it lies
+    // on the device of `like`.
+    bool holds(PyObject* t, const char* name, int code, std::initializer_list<long long> dims, PyObject* like, bool optional)
+    {
+        if (!ok || (optional && t == Py_None)) return ok;
+        if (t == Py_None) return refuse(PyExc_TypeError, "%s is missing", name);
+        PyObject* d = PyObject_GetAttr(t, s_dtype);
+        if (d == nullptr) return ok = false;
+        bool known = false;
+        for (const DtypeCode& c : dtypes) known = known || (c.dtype == d && c.code == code);
+        if (!known) refuse(PyExc_TypeError, "%s has the wrong dtype (%S)", name, d);
+        Py_DECREF(d);
+        if (!ok) return false;
+        PyObject* s = shape(t, 0, false);
+        if (s == nullptr) return false;
+        bool same = PyTuple_GET_SIZE(s) == static_cast<Py_ssize_t>(dims.size());
+        Py_ssize_t i = 0;
+        for (long long v : dims)
+        {
+            if (same && v >= 0) same = PyLong_AsLongLong(PyTuple_GET_ITEM(s, i)) == v;
+            ++i;
+        }
+        if (!same) refuse(PyExc_ValueError, "%s has the wrong shape %S", name, s);
+        Py_DECREF(s);
+        return ok && plain(t, name, like);
+    }
+    // t is contiguous and on the device of `like`.
+    bool plain(PyObject* t, const char* name, PyObject* like)
+    {
+        if (!ok || t == Py_None) return ok;
+        PyObject* c = PyObject_CallMethodNoArgs(t, s_is_contiguous);
+        if (c == nullptr) return ok = false;
+        const bool yes = c == Py_True;
+        Py_DECREF(c);
+        if (!yes) return refuse(PyExc_ValueError, "%s must be contiguous", name);
+        if (t == like) return true;
+        PyObject* a = PyObject_GetAttr(t, s_device);
+        PyObject* b = a ? PyObject_GetAttr(like, s_device) : nullptr;
+        const int eq = b ? PyObject_RichCompareBool(a, b, Py_EQ) : -1;
+        Py_XDECREF(a);
+        Py_XDECREF(b);
+        if (eq < 0) return ok = false;
+        return eq == 1 || refuse(PyExc_ValueError, "%s is on another device than the other tensors", name);
+    }
+    // t lies on the current device (a call without rows touches no device and may have its tensors anywhere).
+    void current(PyObject* t, bool rows)
+    {
+        if (!ok || !rows) return;
+        PyObject* c = PyObject_GetAttr(t, s_is_cuda);
+        const bool gpu = c == Py_True;
+        Py_XDECREF(c);
+        if (c == nullptr) ok = false;
+        else if (!gpu) refuse(PyExc_ValueError, "the tensors must be on the GPU");
+        if (!ok) return;
+        PyObject* d = PyObject_GetAttr(t, s_device);
+        PyObject* i = d ? PyObject_GetAttr(d, s_index) : nullptr;
+        PyObject* n = i ? PyObject_CallNoArgs(get_device) : nullptr;
+        const int eq = n ? PyObject_RichCompareBool(i, n, Py_EQ) : -1;
+        Py_XDECREF(d);
+        Py_XDECREF(i);
+        Py_XDECREF(n);
+        if (eq < 0) ok = false;
+        else if (eq == 0) refuse(PyExc_ValueError, "the tensors are on another device than the current one");
     }
     size_t nbytes(PyObject* t)
     {
@@ -285,6 +361,94 @@ PyObject* append_decode(PyObject*, PyObject* const* a, Py_ssize_t n)
     });
 }
 
+// A score rule at r: score_cap, slopes, window, key_begin [, key_end].
+struct Rule
+{
+    float    cap = 0.0f;
+    float*   slopes = nullptr;
+    int      window = 0;
+    int32_t *begin = nullptr, *end = nullptr;
+};
+
+// weights, prior, decay at w: fp32 [B, Hkv, T] or None, the same or None, a number.
+struct Weights
+{
+    float * w = nullptr, *prior = nullptr;
+    float   decay = 0.0f;
+    int64_t stride = 0;
+    Weights(Reader& r, PyObject* const* a, int B, int Hkv, PyObject* like)
+    {
+        r.holds(a[0], "weights", FFKV_DTYPE_F32, {B, Hkv, -1}, like, true);
+        if (r.ok && a[0] != Py_None) stride = r.dim(a[0], 2);
+        r.holds(a[1], "prior", FFKV_DTYPE_F32, {B, Hkv, stride}, like, true);
+        decay = r.real(a[2]);
+        w = r.ptr<float>(a[0]), prior = r.ptr<float>(a[1]);
+    }
+};
+
+// The scales of an int8 [N, 16, Hkv] or fp8 [Hkv] cache; another cache's are not read.
+void check_scales(Reader& r, PyObject* s, const char* name, int ct, PyObject* cache, int Hkv, PyObject* like)
+{
+    if (ct == FFKV_DTYPE_I8) r.holds(s, name, FFKV_DTYPE_F32, {r.dim(cache, 0), FFKV_BLOCK_SIZE, Hkv}, like, true);
+    if (ct == FFKV_DTYPE_FP8_E4M3) r.holds(s, name, FFKV_DTYPE_F32, {Hkv}, like, true);
+}
+
+// num_blocks: at most the pool's pages
+void check_blocks(Reader& r, int n, PyObject* cache)
+{
+    if (r.ok && n > r.dim(cache, 0)) r.refuse(PyExc_ValueError, "num_blocks %d is more than the caches' pages", n);
+}
+
+// decode's 11, k_new, v_new, score_cap, slopes, window, key_begin, weights, prior, decay, workspace, stream
+PyObject* decode_scored(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!count(n, 22)) return nullptr;
+    Reader     r{a};
+    Decode     d(r, a);
+    PyObject*  q = a[0];
+    PyObject*  sh = r.shape(q, 3, false);
+    const bool four = r.ok && PyTuple_GET_SIZE(sh) == 4;
+    if (r.ok && (PyTuple_GET_SIZE(sh) > 4 || (four && r.item(sh, 1) != 1)))
+        r.refuse(PyExc_ValueError, "q must be [B, 1, Hq, D] or [B, Hq, D], got %S", sh);
+    Py_XDECREF(sh);
+    r.plain(q, "q", q);
+    r.plain(a[1], "out", q);
+    if (r.ok && r.dtype(a[1]) != d.qt) r.refuse(PyExc_TypeError, "out must have q's dtype");
+    if (r.ok && r.nbytes(a[1]) != r.nbytes(q)) r.refuse(PyExc_ValueError, "out must have as many values as q");
+    r.holds(a[2], "k_cache", d.ct, {-1, FFKV_BLOCK_SIZE, d.Hkv, d.D}, q, false);
+    r.holds(a[3], "v_cache", d.ct, {r.dim(a[2], 0), FFKV_BLOCK_SIZE, d.Hkv, d.D}, q, false);
+    check_scales(r, a[4], "k_scale", d.ct, a[2], d.Hkv, q);
+    check_scales(r, a[5], "v_scale", d.ct, a[2], d.Hkv, q);
+    r.holds(a[6], "block_table", kInt32, {d.B, -1}, q, false);
+    r.holds(a[7], "context_lens", kInt32, {d.B}, q, false);
+    check_blocks(r, d.N, a[2]);
+    int st = d.qt;
+    if (r.ok && a[11] != Py_None)
+    {
+        st = r.dtype(a[11]);
+        r.holds(a[11], "k_new", st, {d.B, 1, d.Hkv, d.D}, q, false);
+    }
+    if (r.ok && a[12] != Py_None) r.holds(a[12], "v_new", st, {d.B, 1, d.Hkv, d.D}, q, false);
+    Rule u;
+    u.cap = r.real(a[13]);
+    r.holds(a[14], "slopes", FFKV_DTYPE_F32, {d.Hq}, q, true);
+    u.window = r.integer(a[15]);
+    r.holds(a[16], "key_begin", kInt32, {d.B}, q, true);
+    Weights w(r, a + 17, d.B, d.Hkv, q);
+    r.plain(a[20], "workspace", q);
+    r.current(q, d.B > 0);
+    void *       k = r.ptr(a[11]), *v = r.ptr(a[12]);
+    u.slopes = r.ptr<float>(a[14]), u.begin = r.ptr<int32_t>(a[16]);
+    void*        ws = r.ptr(a[20]);
+    const size_t wb = r.nbytes(a[20]);
+    void*        s = r.stream(a[21]);
+    return finish(r, [&] {
+        return fn.decode_scored(d.q, d.out, d.qt, d.kc, d.vc, d.ct, d.ks, d.vs, d.bt, d.cx, d.B, d.Hq, d.Hkv, d.D,
+                                FFKV_BLOCK_SIZE, d.mb, d.N, d.mcl, d.scale, u.cap, u.slopes, u.window, u.begin, k, v, st,
+                                w.w, w.prior, w.decay, w.stride, ws, wb, s);
+    });
+}
+
 // decode's 11, stream
 PyObject* decode_noalloc(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
@@ -405,7 +569,8 @@ PyObject* forget_stream(PyObject*, PyObject*)
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(append),         FAST(decode),  FAST(decode_shared), FAST(append_decode),
+PyMethodDef methods[] = {FAST(decode_scored),
+                         FAST(append),         FAST(decode),  FAST(decode_shared), FAST(append_decode),
                          FAST(decode_noalloc), FAST(prefill), FAST(rope),          FAST(rope_append),
                          {"bind", bind, METH_VARARGS, nullptr},
                          {"forget_stream", forget_stream, METH_NOARGS, nullptr},
@@ -422,6 +587,10 @@ PyMODINIT_FUNC PyInit__front(void)
     s_data_ptr = PyUnicode_InternFromString("data_ptr");
     s_nbytes = PyUnicode_InternFromString("nbytes");
     s_cuda_stream = PyUnicode_InternFromString("cuda_stream");
+    s_device = PyUnicode_InternFromString("device");
+    s_index = PyUnicode_InternFromString("index");
+    s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
+    s_is_cuda = PyUnicode_InternFromString("is_cuda");
     if (PyErr_Occurred()) return nullptr;
     return PyModule_Create(&module);
 }

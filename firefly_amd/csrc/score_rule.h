@@ -1,0 +1,59 @@
+// score_rule.h - what a score rule does to a score and to the keys a query sees: the tanh cap, the distance bias, the
+// window and the given ranges, shared by the scored decode, the scored prefill and the attention weights (gfx950).
+#pragma once
+
+#include "ffkv_device.h"
+#include "ffkv_internal.h"
+
+namespace ffkv
+{
+
+namespace
+{
+
+// cap * tanh(v / cap) of a score in log2 units (cap and 1 / cap in them too).  Below 0.6 tanh(x) = x + x^3 P(x^2) with P
+// fitted to a relative error under 2^-23 (1 - 2 / (e^2x + 1) would lose the small scores' low bits: an absolute error of
+// 2^-24 of the cap, 6e-6 at a cap of 50), above it (1 - e) / (1 + e) with e = e^-2|x|, which holds at infinity (e = 0).
+__device__ __forceinline__ float cap_score(float v, float cap, float inv_cap)
+{
+    const float x = v * inv_cap;
+    const float ax = __builtin_fabsf(x);
+    const float t = x * x;
+    float       p = -0.005908978637307882f;
+    p = __builtin_fmaf(p, t, 0.0208087470382452f);
+    p = __builtin_fmaf(p, t, -0.053787969052791595f);
+    p = __builtin_fmaf(p, t, 0.13331978023052216f);
+    p = __builtin_fmaf(p, t, -0.33333301544189453f);
+    const float near = __builtin_fmaf(x * t, p, x);
+    const float e = __builtin_amdgcn_exp2f(ax * -2.8853900817779268f);
+    const float far = __builtin_copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
+    return cap * (ax < 0.6f ? near : far);
+}
+
+// First visible key of the query at position pos (before the row's end is looked at): the window's and the given one's.
+__device__ __forceinline__ int64_t first_key(const ScoreRule& r, int64_t pos, int64_t begin)
+{
+    int64_t lo = begin > 0 ? begin : 0;
+    if (r.window > 0 && lo < pos + 1 - r.window) lo = pos + 1 - r.window;
+    return lo;
+}
+
+// Tokens that the decode of row b attends under the rule: [lo, hi).
+struct RowSpan
+{
+    int lo, hi, pos;  // lo <= hi; pos: the query's position
+};
+__device__ __forceinline__ RowSpan row_span(const DecodeArgs& a, int b)
+{
+    const int64_t pos = a.context_lens[b];
+    int64_t       hi = pos + 1;  // +1: the token appended this step
+    if (hi > a.cap_tokens) hi = a.cap_tokens;
+    if (hi < 0) hi = 0;
+    int64_t lo = first_key(a.rule, pos, a.rule.key_begin != nullptr ? a.rule.key_begin[b] : 0);
+    if (lo > hi) lo = hi;
+    return RowSpan{static_cast<int>(lo), static_cast<int>(hi), static_cast<int>(pos)};
+}
+
+}  // namespace
+
+}  // namespace ffkv

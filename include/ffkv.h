@@ -272,6 +272,44 @@ FFKV_API int ffkv_rope_append(void* q, void* k, const void* v, int src_dtype, vo
                               int head_dim, int block_size, int max_blocks, int num_blocks, float rope_theta,
                               void* stream);
 
+/*
+ * ---- attention under a score rule --------------------------------------------------------------------------------
+ * For the query at position i, head h and the key at position j, with s = scale * q.k:
+ *   score_cap  > 0: s becomes score_cap * tanh(s / score_cap); 0: left as it is
+ *   slopes     fp32 [num_heads], not NULL: s becomes s - slopes[h] * |i - j| (after the cap); finite values
+ *   window     > 0: keys j <= i - window are hidden (a query sees its own and the window - 1 positions before it)
+ *   key_begin  int32, not NULL: keys before key_begin of the query are hidden
+ * A hidden key has weight 0 whatever its K and V hold, NaN and infinities included, and a query that sees no key gives
+ * zeros.  No counterpart in the reference, whose attention is plain causal (src/kernels/attention.cu:173-174, :347-360).
+ *
+ * ffkv_paged_decode_scored is ffkv_paged_decode under a rule (key_begin int32 [batch]), with two options:
+ *   k_new / v_new  (both or neither; src_dtype theirs) the step's new tokens, appended first as
+ *                  ffkv_append_paged_decode does: in the decode's own launch where they have the cache's 16-bit dtype
+ *                  and a head_dim of the matrix cores (no other row of the call may then attend a row's new slot)
+ *   weights        fp32 [batch, num_kv_heads, weight_stride]: the attention weight that each cached token j of row b gets,
+ *                  summed over the query heads of a KV head, is added to what it had:
+ *                    weights[b, kvh, j] = decay * prior[b, kvh, j] + sum of softmax(s)_j    j < context_lens[b]
+ *                    weights[b, kvh, j] = sum of softmax(s)_j                               j = context_lens[b]
+ *                  prior may be weights itself, or NULL (nothing earlier); tokens past the row's end, or at or beyond
+ *                  max_context_len, are left as they were.  weight_stride is at least min(max_blocks * 16,
+ *                  max_context_len); decay is finite and not negative.
+ * q, out, caches, scales, tables, sizes, scale and errors as for ffkv_paged_decode; positions and distances count the
+ * row's cached tokens.  With weights the workspace holds the scores of all visible keys (4 bytes per query head and token
+ * of the bound on a row): give max_context_len where the block table is wide.  workspace NULL: stream-ordered memory.
+ * The calls that share a workspace must not overlap in time.
+ */
+FFKV_API size_t ffkv_decode_scored_workspace_bytes(int batch, int num_heads, int head_dim, int max_blocks,
+                                                   int max_context_len, int with_weights);
+
+FFKV_API int ffkv_paged_decode_scored(const void* q, void* out, int qo_dtype, void* k_cache, void* v_cache,
+                                      int cache_dtype, float* k_scale, float* v_scale, const int32_t* block_table,
+                                      const int32_t* context_lens, int batch, int num_heads, int num_kv_heads,
+                                      int head_dim, int block_size, int max_blocks, int num_blocks, int max_context_len,
+                                      float scale, float score_cap, const float* slopes, int window,
+                                      const int32_t* key_begin, const void* k_new, const void* v_new, int src_dtype,
+                                      float* weights, const float* prior, float decay, int64_t weight_stride,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* Message describing the last error returned on the calling thread ("" if none). */
 FFKV_API const char* ffkv_last_error(void);
 

@@ -1,0 +1,109 @@
+"""What the scored operators refuse, without a GPU: the C ABI's status codes before a device is touched, and the Python
+front end's checks of its tensors."""
+
+import ctypes
+
+import pytest
+import torch
+
+HKV, D = 2, 64
+NAN, INF = float("nan"), float("inf")
+
+
+def _decode(ff, **kw):
+    a = dict(q=16, out=16, qo_dtype=ff.DTYPE_BF16, k_cache=16, v_cache=16, cache_dtype=ff.DTYPE_BF16, k_scale=None,
+             v_scale=None, block_table=16, context_lens=16, batch=1, num_heads=32, num_kv_heads=8, head_dim=128,
+             block_size=16, max_blocks=4, num_blocks=4, max_context_len=0, scale=0.0, score_cap=0.0, slopes=None, window=0,
+             key_begin=None, k_new=None, v_new=None, src_dtype=ff.DTYPE_BF16, weights=None, prior=None, decay=1.0,
+             weight_stride=0, workspace=None, workspace_bytes=0, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return ff.lib.ffkv_paged_decode_scored(*a.values())
+
+
+DECODE = [
+    (dict(block_size=8), -2), (dict(head_dim=84), -2), (dict(head_dim=144), -2), (dict(qo_dtype=3), -2),
+    (dict(cache_dtype=7), -2), (dict(num_heads=30), -1), (dict(num_heads=0), -1), (dict(max_blocks=-1), -1),
+    (dict(num_heads=8 * 17, cache_dtype=0), -2), (dict(num_heads=8 * 17, head_dim=72), -2), (dict(batch=70000), -2),
+    (dict(context_lens=None), -1), (dict(q=None), -1), (dict(cache_dtype=3), -1), (dict(q=20), -1), (dict(k_new=16), -1),
+    (dict(v_new=16), -1), (dict(k_new=24, v_new=16), -1), (dict(k_new=16, v_new=16, src_dtype=3), -2),
+    (dict(score_cap=-1.0), -1), (dict(score_cap=NAN), -1), (dict(score_cap=INF), -1), (dict(window=-1), -1),
+    (dict(slopes=18), -1), (dict(key_begin=17), -1),
+    (dict(prior=16), -1), (dict(weights=16, weight_stride=63), -1), (dict(weights=16, weight_stride=64, decay=-0.5), -1),
+    (dict(weights=16, weight_stride=64, decay=NAN), -1), (dict(weights=18, weight_stride=64), -1),
+    (dict(weights=16, weight_stride=64, prior=18), -1),
+    (dict(workspace=24, workspace_bytes=1 << 30), -1), (dict(workspace=256, workspace_bytes=64, max_blocks=6000), -3),
+    (dict(weights=16, weight_stride=1 << 30, max_blocks=1 << 26, batch=31, num_heads=65528), -2),
+]
+
+
+@pytest.mark.parametrize("kw,code", DECODE)
+def test_decode_rejects(ff, kw, code):
+    assert _decode(ff, **kw) == code
+    assert ff.lib.ffkv_last_error().decode() != ""
+
+
+def test_empty_is_ok(ff):
+    assert _decode(ff, batch=0, q=None) == 0 and ff.lib.ffkv_last_error() == b""
+
+
+def test_decode_workspace_bytes(ff):
+    f = ff.lib.ffkv_decode_scored_workspace_bytes
+    plain = ff.decode_workspace_bytes(4, 32, 128, 600)
+    assert f(4, 32, 128, 600, 0, 0) == plain
+    assert f(4, 32, 128, 600, 0, 1) >= plain + 4 * 32 * 9600 * 4
+    assert f(4, 32, 128, 600, 100, 1) < f(4, 32, 128, 600, 0, 1)
+    assert f(0, 32, 128, 600, 0, 1) == 0 and f(65535, 65535, 128, 1 << 26, 0, 1) == 0
+
+
+def _tensors(B=0, dtype=torch.bfloat16, Hq=4, cache=None):
+    pool = torch.zeros(4, 16, HKV, D, dtype=cache or dtype)
+    return dict(q=torch.zeros(B, 1, Hq, D, dtype=dtype), k_cache=pool, v_cache=pool.clone(),
+                block_table=torch.zeros(B, 3, dtype=torch.int32), context_lens=torch.zeros(B, dtype=torch.int32))
+
+
+def test_decode_front(ff):
+    t = _tensors()
+    w = torch.zeros(0, HKV, 48)
+    k = torch.zeros(0, 1, HKV, D, dtype=torch.bfloat16)
+    out = ff.paged_attention_scored(**t, score_cap=5, slopes=torch.zeros(4), window=3, weights=w, prior=w,
+                                    key_begin=torch.zeros(0, dtype=torch.int32), k_new=k, v_new=k, stream=0)
+    assert out.shape == (0, 1, 4 * D)
+    i8 = _tensors(cache=torch.int8)
+    s = torch.zeros(4, 16, HKV)
+    ff.paged_attention_scored(**i8, k_scale=s, v_scale=s, stream=0)
+    bad = [
+        (ValueError, dict(t, q=torch.zeros(0, 2, 4, D, dtype=torch.bfloat16))),
+        (TypeError, dict(t, block_table=t["block_table"].long())),
+        (ValueError, dict(t, block_table=torch.zeros(1, 3, dtype=torch.int32))),
+        (ValueError, dict(t, context_lens=torch.zeros(2, dtype=torch.int32))),
+        (TypeError, dict(t, context_lens=t["context_lens"].float())),
+        (ValueError, dict(t, v_cache=t["v_cache"][:2])),
+        (ValueError, dict(t, k_cache=t["k_cache"][:, :8])),
+        (ValueError, dict(t, k_cache=torch.zeros(4, 16, HKV, 2 * D, dtype=torch.bfloat16)[..., ::2])),
+        (TypeError, dict(t, v_cache=t["v_cache"].half())),
+        (ValueError, dict(t, slopes=torch.zeros(3))),
+        (TypeError, dict(t, slopes=torch.zeros(4).double())),
+        (ValueError, dict(t, key_begin=torch.zeros(1, dtype=torch.int32))),
+        (ValueError, dict(t, weights=torch.zeros(0, HKV + 1, 48))),
+        (ValueError, dict(t, weights=w, prior=torch.zeros(0, HKV, 47))),
+        (TypeError, dict(t, weights=w.half())),
+        (TypeError, dict(t, k_new=k, v_new=k.half())),
+        (ValueError, dict(t, k_new=k[..., :32], v_new=k[..., :32])),
+        (ff.FFKVError, dict(t, k_new=k)),
+        (ff.FFKVError, dict(t, weights=torch.zeros(0, HKV, 47))),
+        (ff.FFKVError, dict(t, prior=w)),
+        (TypeError, dict(t, window=2.0)),
+        (TypeError, dict(t, out=torch.zeros(0, 1, 4 * D))),
+        (ValueError, dict(t, out=torch.zeros(1, 1, 4 * D, dtype=torch.bfloat16))),
+        (ValueError, dict(t, num_blocks=5)),
+        (ValueError, dict(i8, k_scale=s[:2], v_scale=s)),
+        (TypeError, dict(i8, k_scale=s.half(), v_scale=s)),
+        (TypeError, dict(t, k_cache=torch.zeros(4, 16, HKV, D, dtype=torch.int32))),
+        (ValueError, dict(t, slopes=torch.zeros(4, device="meta"))),
+    ]
+    for error, kw in bad:
+        with pytest.raises(error):
+            ff.paged_attention_scored(**kw, stream=0)
+    with pytest.raises(ValueError, match="GPU"):
+        ff.paged_attention_scored(**_tensors(B=1), stream=0)
