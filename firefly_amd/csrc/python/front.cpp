@@ -380,6 +380,7 @@ struct Weights
     {
         r.holds(a[0], "weights", FFKV_DTYPE_F32, {B, Hkv, -1}, like, true);
         if (r.ok && a[0] != Py_None) stride = r.dim(a[0], 2);
+        if (r.ok && a[0] == Py_None && a[1] != Py_None) r.refuse(PyExc_ValueError, "prior without weights");
         r.holds(a[1], "prior", FFKV_DTYPE_F32, {B, Hkv, stride}, like, true);
         decay = r.real(a[2]);
         w = r.ptr<float>(a[0]), prior = r.ptr<float>(a[1]);
@@ -423,6 +424,7 @@ PyObject* decode_scored(PyObject*, PyObject* const* a, Py_ssize_t n)
     r.holds(a[7], "context_lens", kInt32, {d.B}, q, false);
     check_blocks(r, d.N, a[2]);
     int st = d.qt;
+    if (r.ok && (a[11] == Py_None) != (a[12] == Py_None)) r.refuse(PyExc_ValueError, "k_new and v_new come together");
     if (r.ok && a[11] != Py_None)
     {
         st = r.dtype(a[11]);
