@@ -98,6 +98,11 @@ def _load() -> ctypes.CDLL:
     lib.ffkv_paged_decode_scored.restype = i32
     lib.ffkv_paged_decode_scored.argtypes = [vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
                                              i32, f32, *rule, vp, vp, vp, i32, vp, vp, f32, ctypes.c_int64, vp, sz, vp]
+    lib.ffkv_prefill_scored_workspace_bytes.restype = sz
+    lib.ffkv_prefill_scored_workspace_bytes.argtypes = [i32] * 12
+    lib.ffkv_paged_prefill_scored.restype = i32
+    lib.ffkv_paged_prefill_scored.argtypes = [vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
+                                              i32, i32, f32, *rule, vp, vp, vp, sz, vp]
     lib.ffkv_last_error.restype = ctypes.c_char_p
     lib.ffkv_last_error.argtypes = []
     lib.ffkv_version.restype = ctypes.c_char_p
@@ -110,7 +115,8 @@ def _load() -> ctypes.CDLL:
 def _bind(lib, torch) -> None:
     """Point the native front end (``_front``, csrc/python/front.cpp) at ``lib``'s functions."""
     names = ("append", "paged_decode", "append_paged_decode", "paged_decode_shared_prefix", "paged_decode_noalloc",
-             "prefill_workspace_bytes", "paged_prefill_ws", "rope", "rope_append", "paged_decode_scored")
+             "prefill_workspace_bytes", "paged_prefill_ws", "rope", "rope_append", "paged_decode_scored",
+             "prefill_scored_workspace_bytes", "paged_prefill_scored")
     _front.bind(tuple(ctypes.cast(getattr(lib, "ffkv_" + n), ctypes.c_void_p).value for n in names),
                 [*_torch_dtypes(torch).items(), (torch.int32, _INT32)], getattr(torch._C, "_cuda_getDevice", None),
                 getattr(torch._C, "_cuda_getCurrentRawStream", None), lambda: torch.cuda.current_stream().cuda_stream)
@@ -324,4 +330,22 @@ def paged_attention_scored(q, k_cache, v_cache, block_table, context_lens, score
     check(_front.decode_scored(q, out, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, max_context_len, scale,
                                num_blocks, k_new, v_new, score_cap, slopes, window, key_begin, weights, prior, decay,
                                workspace, stream))
+    return out
+
+
+def paged_prefill_scored(q, k_cache, v_cache, block_table, context_lens, score_cap: float = 0.0, slopes=None,
+                         window: int = 0, key_begin=None, key_end=None, out=None, k_scale=None, v_scale=None,
+                         max_context_len: int = 0, scale: float = 0.0, num_blocks: int | None = None, stream=None):
+    """Prefill attention under a score rule (``ffkv_paged_prefill_scored``): ``paged_prefill``'s tensors, the rule of
+    ``paged_attention_scored``, and for every query the range of keys it sees, ``key_begin``/``key_end`` int32 ``[B, S]``
+    (None: from key 0; up to the query itself): documents, prefixes, padding (an end of 0).  An infinite or NaN value
+    reaches only the queries that see its key."""
+    if out is None:
+        import torch
+
+        B, S, Hq, D = q.shape
+        out = torch.empty((B, S, Hq * D), dtype=q.dtype, device=q.device)
+    check(_front.prefill_scored(q, out, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, max_context_len,
+                                scale, num_blocks, score_cap, slopes, window, key_begin, key_end, stream,
+                                _prefill_scratch))
     return out

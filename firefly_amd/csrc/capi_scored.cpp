@@ -88,6 +88,13 @@ bool score_layout_fits(int batch, int num_heads, int cap_tokens)
     return 4.0 * batch * num_heads * (static_cast<double>(cap_tokens) + 16) < kMostBytes;
 }
 
+// Most keys that a block of 128 query rows sees: a window's of its tokens, else the row's bound.
+int prefill_span(int cap_tokens, int group, int window, bool key_end)
+{
+    if (window <= 0 || key_end) return cap_tokens;
+    return static_cast<int>(std::min<int64_t>(cap_tokens, static_cast<int64_t>(window) + 128 / group + 2 * FFKV_BLOCK_SIZE));
+}
+
 }  // namespace
 
 extern "C" {
@@ -252,6 +259,115 @@ int ffkv_paged_decode_scored(const void* q, void* out, int qo_dtype, void* k_cac
         if (e == hipSuccess) e = fe;
     }
     if (e != hipSuccess) return hip_fail(e, "scored decode launch");
+    return ok();
+}
+
+size_t ffkv_prefill_scored_workspace_bytes(int qo_dtype, int cache_dtype, int batch, int seq_len, int num_heads,
+                                           int num_kv_heads, int head_dim, int paged, int max_blocks,
+                                           int max_context_len, int window, int with_key_end)
+{
+    // sizes that ffkv_paged_prefill_scored refuses need nothing
+    if (!is_act(qo_dtype) || !is_cache(cache_dtype) || cache_dtype == FFKV_DTYPE_F32 || !head_dim_mfma(head_dim) ||
+        batch <= 0 || batch > 65535 || seq_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535 ||
+        num_heads % num_kv_heads != 0 || (paged != 0 && max_blocks < 0) || window < 0)
+        return 0;
+    ffkv::PrefillArgs a{};
+    a.qo_dtype = qo_dtype;
+    a.cache_dtype = cache_dtype;
+    a.batch = batch;
+    a.seq_len = seq_len;
+    a.num_heads = num_heads;
+    a.num_kv_heads = num_kv_heads;
+    a.group = num_heads / num_kv_heads;
+    a.head_dim = head_dim;
+    a.paged = paged != 0;
+    a.cap_tokens = a.paged ? ffkv::decode_cap_tokens(max_blocks, max_context_len) : seq_len;
+    a.span_tokens = prefill_span(a.cap_tokens, a.group, window, with_key_end != 0);
+    ffkv::prefill_scored_plan(a);
+    return static_cast<size_t>(ffkv::prefill_split_layout(a).total);
+}
+
+int ffkv_paged_prefill_scored(const void* q, void* out, int qo_dtype, const void* k_cache, const void* v_cache,
+                              int cache_dtype, const float* k_scale, const float* v_scale, const int32_t* block_table,
+                              const int32_t* context_lens, int batch, int seq_len, int num_heads, int num_kv_heads,
+                              int head_dim, int block_size, int max_blocks, int num_blocks, int max_context_len,
+                              float scale, float score_cap, const float* slopes, int window, const int32_t* key_begin,
+                              const int32_t* key_end, void* workspace, size_t workspace_bytes, void* stream)
+{
+    const bool paged = block_table != nullptr;
+    if (block_size != FFKV_BLOCK_SIZE) return fail(FFKV_ERR_UNSUPPORTED, "block_size must be 16, got %d", block_size);
+    if (!is_act(qo_dtype)) return fail(FFKV_ERR_UNSUPPORTED, "unsupported q/out dtype %d", qo_dtype);
+    if (!is_cache(cache_dtype) || cache_dtype == FFKV_DTYPE_F32)
+        return fail(FFKV_ERR_UNSUPPORTED, "prefill supports F16, BF16, I8 and FP8_E4M3 caches, got dtype %d",
+                    cache_dtype);
+    if (!head_dim_mfma(head_dim)) return fail(FFKV_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256, got %d", head_dim);
+    if (batch < 0 || seq_len < 0 || num_heads <= 0 || num_kv_heads <= 0 || (paged && (max_blocks < 0 || num_blocks < 0)))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "bad size (batch %d seq_len %d heads %d kv_heads %d max_blocks %d "
+                    "num_blocks %d)", batch, seq_len, num_heads, num_kv_heads, max_blocks, num_blocks);
+    if (num_heads % num_kv_heads != 0)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "num_heads %d is not a multiple of num_kv_heads %d", num_heads,
+                    num_kv_heads);
+    if (batch > 65535 || num_kv_heads > 65535)
+        return fail(FFKV_ERR_UNSUPPORTED, "batch and num_kv_heads must be <= 65535");
+    if (static_cast<int64_t>(seq_len) * (num_heads / num_kv_heads) > INT32_MAX - 64)
+        return fail(FFKV_ERR_UNSUPPORTED, "seq_len * group too large");
+    if (static_cast<int64_t>(batch) * num_kv_heads *
+            ((static_cast<int64_t>(seq_len) * (num_heads / num_kv_heads) + 127) / 128) > INT32_MAX - 64 * 1024)
+        return fail(FFKV_ERR_UNSUPPORTED, "batch * num_kv_heads * ceil(seq_len * group / 128) too large");
+    if (const int rc = check_rule(score_cap, slopes, window, key_begin, key_end)) return rc;
+    if (batch == 0 || seq_len == 0) return ok();
+    if (!q || !out || !k_cache || !v_cache || (paged && !context_lens))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "null q, out, cache or context_lens pointer");
+    if (!paged && cache_dtype == FFKV_DTYPE_I8)
+        return fail(FFKV_ERR_UNSUPPORTED, "int8 K/V need a block table (their scales are per page slot)");
+    if (quantized(cache_dtype) && (!k_scale || !v_scale))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "quantized cache needs k_scale and v_scale");
+    if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "q, out, cache and workspace pointers must be 16-byte aligned");
+
+    ffkv::PrefillArgs a{};
+    a.q = q;
+    a.out = out;
+    a.k_cache = k_cache;
+    a.v_cache = v_cache;
+    a.k_scale = k_scale;
+    a.v_scale = v_scale;
+    a.block_table = block_table;
+    a.context_lens = context_lens;
+    a.qo_dtype = qo_dtype;
+    a.cache_dtype = cache_dtype;
+    a.batch = batch;
+    a.seq_len = seq_len;
+    a.num_heads = num_heads;
+    a.num_kv_heads = num_kv_heads;
+    a.group = num_heads / num_kv_heads;
+    a.head_dim = head_dim;
+    a.max_blocks = paged ? max_blocks : 0;
+    a.num_blocks = paged ? num_blocks : 0;
+    a.cap_tokens = paged ? ffkv::decode_cap_tokens(max_blocks, max_context_len) : seq_len;
+    a.paged = paged;
+    a.scale_log2 = softmax_scale(scale, head_dim) * kLog2e;
+    a.rule = make_rule(score_cap, slopes, window, key_begin, key_end);
+    a.span_tokens = prefill_span(a.cap_tokens, a.group, window, key_end != nullptr);
+    a.n_split = 1;
+    if (workspace != nullptr)
+    {
+        ffkv::prefill_scored_plan(a);
+        const ffkv::PrefillSplitLayout lay = ffkv::prefill_split_layout(a);
+        if (a.n_split > 1 && workspace_bytes >= static_cast<size_t>(lay.total))
+        {
+            char* w = static_cast<char*>(workspace);
+            a.ws_pieces = reinterpret_cast<int32_t*>(w + lay.pieces);
+            a.ws_ml = reinterpret_cast<float*>(w + lay.ml);
+            a.ws_acc = reinterpret_cast<float*>(w + lay.acc);
+        }
+        else
+        {
+            a.n_split = 1;
+        }
+    }
+    const hipError_t e = ffkv::launch_prefill_scored(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "scored prefill launch");
     return ok();
 }
 

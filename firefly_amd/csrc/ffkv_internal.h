@@ -105,7 +105,10 @@ struct PrefillArgs
     int            split_slots;
     int            split_from;
     int32_t*       ws_pieces;  // [row blocks]: pieces of each
-    ScoreRule      rule;       // launch_prefill_scored only
+    // launch_prefill_scored only: the rule, and the most keys that a block of 128 query rows sees (cap_tokens, or a
+    // window's)
+    ScoreRule      rule;
+    int            span_tokens;
 };
 
 struct DecodeArgs
@@ -172,6 +175,12 @@ hipError_t launch_prefix_partials(const PrefillArgs& a, hipStream_t stream);  //
 // Sets n_split, split_slots and split_from of a prefill whose sizes and dtypes are set; the partials of a split
 // prefill take prefill_split_layout's bytes.
 void prefill_plan(PrefillArgs& a);
+// The same for a kernel of `threads` threads and `step_keys` keys a step, whose blocks see at most `most_keys` keys.
+void prefill_plan_for(PrefillArgs& a, const void* fn, int threads, int step_keys, int most_keys);
+hipError_t launch_prefill_merge(const PrefillArgs& a, hipStream_t stream);  // of a split prefill's pieces
+// The prefill under a score rule (paged_prefill_scored.hip), its plan from a.span_tokens.
+void       prefill_scored_plan(PrefillArgs& a);
+hipError_t launch_prefill_scored(const PrefillArgs& a, hipStream_t stream);
 struct PrefillSplitLayout
 {
     int64_t pieces, ml, acc, total;  // byte offsets of the three regions and their end (0: no split)

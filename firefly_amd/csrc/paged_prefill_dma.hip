@@ -51,6 +51,7 @@
 // Keys past the row's end and keys on invalid pages are fetched from a zero block instead, so masked keys meet
 // zero V rows (their probabilities are exactly zero) and no lane reads outside the cache.
 #include "mfma_common.h"
+#include "score_rule.h"
 
 #include <algorithm>
 
@@ -121,6 +122,7 @@ constexpr int kXcds = 8;  // MI355X: workgroups are dealt to 8 XCDs (separate L2
 #define FFKV_PREFILL_V16 1  // PV products in f16 for 8-bit caches whose score products are bf16
 #endif
 
+constexpr int kRuleFlags = 5;         // RULE: s_vover, and a mark per stage
 constexpr int kPrefillSplitMin = 4;   // fewest steps of a piece of a split prefill
 constexpr int kPrefillSplitMax = 64;  // most pieces of a row block
 
@@ -279,12 +281,12 @@ __device__ __forceinline__ int nth_largest(uint32_t key, int bound, int n, int r
     return __ffsll(static_cast<long long>(hit)) - 1;
 }
 
-// Steps of the query rows of a row with ctx cached tokens, up to the `n`-th of its chunk.
-template <int KP>
+// Steps of the query rows of a row with ctx cached tokens, up to the `n`-th of its chunk.  RULE: a window bounds them.
+template <int KP, bool RULE = false>
 __device__ __forceinline__ int row_steps(const PrefillArgs& a, int64_t ctx, int n)
 {
     constexpr int KEYS = KP * kBlockSize;
-    const int64_t keys = min(max(ctx + n, int64_t{0}), static_cast<int64_t>(a.cap_tokens));
+    const int64_t keys = min(max(ctx + n, int64_t{0}), static_cast<int64_t>(RULE ? a.span_tokens : a.cap_tokens));
     return static_cast<int>((keys + KEYS - 1) / KEYS);
 }
 
@@ -293,7 +295,7 @@ __device__ __forceinline__ int row_steps(const PrefillArgs& a, int64_t ctx, int 
 // together at about split_slots (the workgroups resident at once).  The call's steps are summed over its rows at the
 // middle of their chunks.  All blocks of a call are split alike: blocks left whole beside split ones would last the
 // longest.
-template <int KP>
+template <int KP, bool RULE = false>
 __device__ __forceinline__ int split_len(const PrefillArgs& a, int nrb, int lane)
 {
     int64_t total = 0;
@@ -302,9 +304,9 @@ __device__ __forceinline__ int split_len(const PrefillArgs& a, int nrb, int lane
     {
         const bool    in = b0 + lane < a.batch;
         const int64_t ctx = in && a.paged ? a.context_lens[b0 + lane] : 0;
-        any = any || __any(in && row_steps<KP>(a, ctx, a.seq_len) >= a.split_from);
+        any = any || __any(in && row_steps<KP, RULE>(a, ctx, a.seq_len) >= a.split_from);
         if (!any && a.batch <= 64) return 0;
-        total += uniform(wave_sum(in ? row_steps<KP>(a, ctx, (a.seq_len + 1) / 2) : 0));
+        total += uniform(wave_sum(in ? row_steps<KP, RULE>(a, ctx, (a.seq_len + 1) / 2) : 0));
     }
     if (!any) return 0;
     total = total * a.num_kv_heads * nrb + a.split_slots - 1;
@@ -354,7 +356,9 @@ struct PrefillLds
 // do not overlap.)
 // SPLIT: a prefill split over its keys (a.n_split > 1), in instances of its own: the pieces cost a workgroup ten scalar
 // registers, which calls that are not split paid for too (int8 at head_dim 64, 15 x 490 tokens over 1500: 216.8 -> 218.7 us).
-template <int QT, int D, int CT, bool PFX, int RG, bool SPLIT = false>
+// RULE: scores are changed and keys hidden by a.rule, each query sees keys [kbeg, kend), and what a query does not see
+// never reaches it, infinite and NaN values included (s_vover is then the first of kRuleFlags ints in LDS).
+template <int QT, int D, int CT, bool PFX, int RG, bool SPLIT = false, bool RULE = false>
 __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t* s_st0, uint8_t* s_st1,
                                            uint8_t* s_st2, uint8_t* s_st3, int& s_vover)
 {
@@ -409,6 +413,7 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (tid == 0) s_vover = 0;
+    if (RULE && tid < kRuleFlags) (&s_vover)[tid] = 0;
     const int c = lane & 15;
     const int g = lane >> 4;
     // Workgroup -> (group, row block).  A group is (row b, kv head) for prefill and (kv head, chunk of prefix
@@ -424,7 +429,7 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
     const int nrb = (R + kDmaRows - 1) / kDmaRows;
     // a prefill split over its keys deals piece p of every group after piece p - 1 of all of them, so that the pieces
     // of one group spread over the XCDs where the groups are fewer
-    static_assert(!(PFX && SPLIT), "prefix partials have chunks of their own");
+    static_assert(!(PFX && (SPLIT || RULE)), "prefix partials have chunks of their own, and no rule");
     const int groups0 = PFX ? Hkv * a.pfx_chunks : a.batch * Hkv;
     const int nsp = SPLIT ? a.n_split : 1;
     const int groups = groups0 * nsp;
@@ -444,7 +449,7 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         // on int8 pages of 64 dims 131 us, 92 now.  By the rows' lengths alone, the idle pieces of long rows lay
         // between: 4 x 33 tokens over 665 to 950 39 us, 25 now.)  A call that stays whole has at most half the blocks that
         // are resident at once, in any order.
-        len = split_len<KP>(a, nrb, lane);
+        len = split_len<KP, RULE>(a, nrb, lane);
         const int pc = grp / groups0;
         if (len == 0 && pc > 0) return;
         int g8 = (groups - xcd + kXcds - 1) / kXcds, j0 = 0;
@@ -460,11 +465,11 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
             if (lane < g8 && gl < groups)
             {
                 const int pl = gl / groups0;
-                const int st = row_steps<KP>(a, a.context_lens[(gl - pl * groups0) / Hkv], S);
+                const int st = row_steps<KP, RULE>(a, a.context_lens[(gl - pl * groups0) / Hkv], S);
                 const int np = split_pieces(a, st, len);
                 key = pl < np ? st / np : 0;
             }
-            const int hit = nth_largest(static_cast<uint32_t>(key), max(len, row_steps<KP>(a, a.cap_tokens, 0) / nsp), g8,
+            const int hit = nth_largest(static_cast<uint32_t>(key), max(len, row_steps<KP, RULE>(a, a.cap_tokens, 0) / nsp), g8,
                                         k_in_xcd / nrb - j0, lane);
             grp = hit >= 0 ? (j0 + hit) * kXcds + xcd : groups;
         }
@@ -490,7 +495,7 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
 #else
     const int grp = wg_index / nrb;
     const int rb = wg_index % nrb;
-    const int len = SPLIT ? split_len<KP>(a, nrb, lane) : 0;
+    const int len = SPLIT ? split_len<KP, RULE>(a, nrb, lane) : 0;
 #endif
     const int piece = nsp == 1 ? 0 : grp / groups0;
     const int grp0 = grp - piece * groups0;
@@ -506,6 +511,8 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
     // as zeros).
     bool   col_ok[RG];
     int    hq[RG], kend[RG], bq[RG];
+    int    kbeg[RG], kpos[RG];  // RULE: first visible key, and the query's position
+    float  slope[RG];           // RULE: of the column's head, in log2 units
     size_t qrow[RG];
     int    L, pg_lo, pg_hi;
     int64_t ctx = 0;
@@ -523,6 +530,16 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         if (Lr < 0) Lr = 0;
         L = __builtin_amdgcn_readfirstlane(static_cast<int>(Lr));
     }
+    // RULE: keys [x, y) that query token t sees, x <= y
+    auto visible = [&](int t) -> int2
+    {
+        const int64_t at = static_cast<int64_t>(b) * S + t;
+        int64_t       hi = a.rule.key_end != nullptr ? a.rule.key_end[at] : ctx + t + 1;
+        hi = hi > L ? L : (hi < 0 ? 0 : hi);
+        int64_t lo = first_key(a.rule, ctx + t, a.rule.key_begin != nullptr ? a.rule.key_begin[at] : 0);
+        lo = lo > hi ? hi : lo;
+        return make_int2(static_cast<int>(lo), static_cast<int>(hi));
+    };
 #pragma unroll
     for (int gi = 0; gi < RG; ++gi)
     {
@@ -545,6 +562,14 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
             int64_t   ke = ctx + t + 1;
             ke = ke > L ? L : (ke < 0 ? 0 : ke);
             kend[gi] = col_ok[gi] ? static_cast<int>(ke) : 0;
+            if constexpr (RULE)
+            {
+                const int2 vis = visible(t);
+                kbeg[gi] = col_ok[gi] ? vis.x : 0;
+                kend[gi] = col_ok[gi] ? vis.y : 0;
+                kpos[gi] = static_cast<int>(ctx + t);
+                slope[gi] = a.rule.slopes != nullptr ? a.rule.slopes[hq[gi]] * 1.4426950408889634f : 0.0f;
+            }
             qrow[gi] = (static_cast<size_t>(b) * S + t) * Hq + hq[gi];
         }
     }
@@ -555,20 +580,43 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         kw = kw > L ? L : (kw < 0 ? 0 : kw);
         pg_lo = 0;
         pg_hi = static_cast<int>((kw + kBlockSize - 1) / kBlockSize);
+        if constexpr (RULE)
+        {
+            // the pages that some query of the workgroup sees (every wave on its own: a lane takes up to two tokens)
+            int lo = INT32_MAX, hi = 0;
+            for (int t = row0 / G + lane; t <= r_last / G; t += 64)
+            {
+                const int2 vis = visible(t);
+                if (vis.x < vis.y)
+                {
+                    lo = min(lo, vis.x);
+                    hi = max(hi, vis.y);
+                }
+            }
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1)
+            {
+                lo = min(lo, __shfl_xor(lo, off, 64));
+                hi = max(hi, __shfl_xor(hi, off, 64));
+            }
+            pg_lo = lo < hi ? lo / kBlockSize : 0;
+            pg_hi = (hi + kBlockSize - 1) / kBlockSize;
+        }
     }
     int64_t part = -1;  // slot of this piece's partials, or -1: the workgroup has all the keys and writes the output
     if constexpr (SPLIT)
     {
-        const int np = split_pieces(a, (pg_hi + KP - 1) / KP, len);
+        const int np = split_pieces(a, (pg_hi - (RULE ? pg_lo : 0) + KP - 1) / KP, len);
         if (piece >= np) return;  // uniform over the workgroup
         const int64_t blk = static_cast<int64_t>(grp0) * nrb + rb;
         if (piece == 0 && tid == 0) a.ws_pieces[blk] = np;
         if (np > 1)
         {
-            const int st = (pg_hi + KP - 1) / KP;
+            const int pg0 = RULE ? pg_lo : 0;
+            const int st = (pg_hi - pg0 + KP - 1) / KP;
             part = blk * nsp + piece;
-            pg_lo = static_cast<int>(static_cast<int64_t>(st) * piece / np) * KP;
-            pg_hi = min(pg_hi, static_cast<int>(static_cast<int64_t>(st) * (piece + 1) / np) * KP);
+            pg_lo = pg0 + static_cast<int>(static_cast<int64_t>(st) * piece / np) * KP;
+            pg_hi = min(pg_hi, pg0 + static_cast<int>(static_cast<int64_t>(st) * (piece + 1) / np) * KP);
         }
     }
     // uniform values computed through divisions: keep them scalar so the loop's branches stay scalar
@@ -893,6 +941,10 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         c_log2 = fmaxf(c_log2 * __builtin_fabsf(ks), 1e-30f);
         v_head_scale = a.v_scale[kvh];
     }
+    // RULE with a cap or a bias: the scores are brought to log2 units first (s_log2), and the softmax takes them as they are
+    const float s_log2 = c_log2;
+    const bool  convert = RULE && (a.rule.cap > 0.0f || a.rule.slopes != nullptr);
+    if (RULE && convert) c_log2 = 1.0f;
     const float thr_raw = 8.0f / c_log2;
     // int8 pages: on the rerun below every p is scaled by 2^kRerunShift, numerator and denominator alike, so the
     // result is the same softmax
@@ -909,6 +961,16 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) kmin = min(kmin, __shfl_xor(kmin, off, 64));
     kmin = __builtin_amdgcn_readfirstlane(kmin);
+    // RULE: the largest first key of the wave's active columns
+    int kbmax = 0;
+    if constexpr (RULE)
+    {
+#pragma unroll
+        for (int gi = 0; gi < RG; ++gi) kbmax = col_ok[gi] ? max(kbmax, kbeg[gi]) : kbmax;
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) kbmax = max(kbmax, __shfl_xor(kbmax, off, 64));
+        kbmax = __builtin_amdgcn_readfirstlane(kbmax);
+    }
 
     // 16-bit K operand of k-step j: key c, dims 32j + 8g .. +8, chunk (4 j + g) ^ ksw of the key's row, at bytes
     // kb4[j % 4] + 64 (j - j % 4) (the swizzle's upper bits XOR j % 4)
@@ -996,7 +1058,38 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         constexpr bool LD = L_DOT || VC;  // the f16 P of converted bf16 V tiles sums by dot products too
         const int pg0 = pg_lo + si * KP;
         // uniform: every key of the step is visible to every column of the wave
-        const bool unmasked = okm == (1 << KP) - 1 && (pg0 + KP) * kBlockSize <= kmin;
+        const bool unmasked = okm == (1 << KP) - 1 && (pg0 + KP) * kBlockSize <= kmin && (!RULE || pg0 * kBlockSize >= kbmax);
+        if constexpr (RULE)
+            if (convert)
+            {
+#pragma unroll
+                for (int gi = 0; gi < RG; ++gi)
+#pragma unroll
+                    for (int u = 0; u < KP; ++u) s[gi][u] *= s_log2;
+                if (a.rule.cap > 0.0f)
+                {
+#pragma unroll
+                    for (int gi = 0; gi < RG; ++gi)
+#pragma unroll
+                        for (int u = 0; u < KP; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[gi][u][i] = cap_score(s[gi][u][i], a.rule.cap, a.rule.inv_cap);
+                }
+                if (a.rule.slopes != nullptr)
+                {
+#pragma unroll
+                    for (int gi = 0; gi < RG; ++gi)
+                    {
+                        const float d0 = static_cast<float>(pg0 * kBlockSize + 4 * g - kpos[gi]);  // key - position
+#pragma unroll
+                        for (int u = 0; u < KP; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                s[gi][u][i] = __builtin_fmaf(-slope[gi], __builtin_fabsf(d0 + static_cast<float>(16 * u + i)),
+                                                             s[gi][u][i]);
+                    }
+                }
+            }
 #pragma unroll
         for (int gi = 0; gi < RG; ++gi)
         {
@@ -1004,12 +1097,13 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
             if (!unmasked)
             {
                 const int kr = kend[gi] - pg0 * kBlockSize - 4 * g;  // key 4g + i of page u visible iff 16u + i < kr
+                const int kl = RULE ? kbeg[gi] - pg0 * kBlockSize - 4 * g : 0;  // (RULE: and at least kl)
 #pragma unroll
                 for (int u = 0; u < KP; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                     {
-                        const bool vis = ((okm >> u) & 1) && u * kBlockSize + i < kr;
+                        const bool vis = ((okm >> u) & 1) && u * kBlockSize + i < kr && (!RULE || u * kBlockSize + i >= kl);
                         s[gi][u][i] = vis ? s[gi][u][i] : kNegInf;
                     }
             }
@@ -1058,6 +1152,17 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
 #pragma unroll
                     for (int i = 0; i < 4; ++i) pv[gi][4 * u + i] *= vsc[i];
             }
+            if constexpr (RULE)
+                if (!unmasked)  // a hidden key's scale may be infinite or NaN: 0 times it counts as 0
+                {
+#pragma unroll
+                    for (int gi = 0; gi < RG; ++gi)
+#pragma unroll
+                        for (int u = 0; u < KP; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                pv[gi][4 * u + i] = s[gi][u][i] == kNegInf ? 0.0f : pv[gi][4 * u + i];
+                }
         }
     };
 
@@ -1199,11 +1304,76 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         }
     };
 
+    // RULE, CF (the rerun of a workgroup whose accumulators are not finite): a value that some of the workgroup's queries
+    // do not see must not reach them, but in the tile products every key meets every query, and 0 * inf is NaN.  So every
+    // wave takes the infinite and NaN values out of the V runs it loaded, and marks the stage with its step where there
+    // were any; the queries that do see such a key then add them one by one (add_bad).  int8 codes are always finite.
+    constexpr bool CAN_CF = RULE && CT != I8;
+    FFKV_LDS int* const s_bad = RULE ? (FFKV_LDS int*)&s_vover + 1 : nullptr;
+    auto clean_v = [&](uint8_t* stage, int si)
+    {
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < LC::RPW; ++k)
+            if (run_is_v(k))
+            {
+                auto* p = (FFKV_LDS u32x4*)(stage + run_dst[k] + 16 * lane);
+                u32x4 w = *p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    constexpr uint32_t EXP = EB == 1 ? 0x7fu : (CT == BF16 ? 0x7f80u : 0x7c00u);
+                    constexpr int      BITS = 8 * EB;
+#pragma unroll
+                    for (int h = 0; h < 32 / BITS; ++h)
+                    {
+                        const bool b = (w[e] >> (BITS * h) & EXP) == EXP;
+                        w[e] = b ? w[e] & ~(static_cast<uint32_t>((uint64_t{1} << BITS) - 1) << (BITS * h)) : w[e];
+                        bad = bad || b;
+                    }
+                }
+                *p = w;
+            }
+        if (__any(bad) && lane == 0) *(volatile FFKV_LDS int*)(s_bad + si % kDmaStages<D>) = si + 1;
+    };
+    auto add_bad = [&](int si, int okm)
+    {
+        for (int t = 0; t < KP * kBlockSize; ++t)
+        {
+            if (!((okm >> (t / kBlockSize)) & 1)) continue;
+            const int      pg = pg_lo + si * KP + t / kBlockSize;
+            const int      key = pg * kBlockSize + t % kBlockSize;
+            if (key >= L) break;
+            const uint64_t page = a.paged ? static_cast<uint32_t>(table_row[pg]) : static_cast<uint32_t>(pg);
+            const char*    v = static_cast<const char*>(a.v_cache) + row_base + page * page_bytes +
+                            (static_cast<size_t>(t % kBlockSize) * Hkv + kvh) * LC::RB;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    const int d = 16 * n + 4 * g + i;
+                    float     x;
+                    if constexpr (EB == 1)
+                        x = e4m3_to_f32(static_cast<uint8_t>(v[d]));
+                    else
+                    {
+                        const uint32_t h = reinterpret_cast<const uint16_t*>(v)[d];
+                        x = CT == BF16 ? bf16_to_f32(h) : f16_to_f32(h);
+                    }
+#pragma unroll
+                    for (int gi = 0; gi < RG; ++gi)
+                        if (!(__builtin_fabsf(x) < __builtin_huge_valf()) && key >= kbeg[gi] && key < kend[gi])
+                            acc[gi][n][i] += x;
+                }
+        }
+    };
+
     // The scores' products are issued before the next loads' scalar address work, which then runs while they
     // execute.
     // With three or more stages, step si + 1 has been requested a step before step si is computed, so its tiles
     // are converted while step si's score products run (AH), instead of at the head of step si + 1.
-    auto body = [&]<bool VC, bool SH>(int si, uint8_t* cur, int okm_cur, uint8_t* nxt, int& okm_nxt, uint8_t* ahead)
+    auto body = [&]<bool VC, bool SH, bool CF>(int si, uint8_t* cur, int okm_cur, uint8_t* nxt, int& okm_nxt, uint8_t* ahead)
     {
         constexpr bool AH = FFKV_PREFILL_AHEAD && NS >= 3 && (VC || C16);
         wait_vm<(NS - 2) * LPS>();
@@ -1223,6 +1393,11 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
                 convert_c16(cur);
                 wait_lgkm0();
             }
+            if constexpr (CF)
+            {
+                clean_v(cur, si);
+                wait_lgkm0();
+            }
         }
         __builtin_amdgcn_s_barrier();  // step si visible to all; every wave is past step si - 1 (stage of si+NS-1)
         f32x4 sx[RG][KP];
@@ -1239,11 +1414,13 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
             float pv[RG][KP * 4];
             softmax.template operator()<VC, SH>(si, cur, okm_cur, sx, pv);
             pv_mma.template operator()<V16 || VC>(cur, pv);
+            if constexpr (CF)
+                if (*(const volatile FFKV_LDS int*)(s_bad + si % kDmaStages<D>) == si + 1) add_bad(si, okm_cur);
         }
     };
 
     // VC: bf16 pages' V tiles converted to f16.  SH: int8 pages' p scaled by 2^kRerunShift (the rerun).
-    auto pipeline = [&]<bool VC, bool SH>()
+    auto pipeline = [&]<bool VC, bool SH, bool CF = false>()
     {
 #pragma unroll
         for (int gi = 0; gi < RG; ++gi)
@@ -1270,27 +1447,27 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         {
             if constexpr (NS == 2)
             {
-                body.template operator()<VC, SH>(si, s_st0, okm0, s_st1, okm1, s_st1);
+                body.template operator()<VC, SH, CF>(si, s_st0, okm0, s_st1, okm1, s_st1);
                 if (si + 1 >= steps) break;
-                body.template operator()<VC, SH>(si + 1, s_st1, okm1, s_st0, okm0, s_st0);
+                body.template operator()<VC, SH, CF>(si + 1, s_st1, okm1, s_st0, okm0, s_st0);
             }
             else if constexpr (NS == 3)
             {
-                body.template operator()<VC, SH>(si, s_st0, okm0, s_st2, okm2, s_st1);
+                body.template operator()<VC, SH, CF>(si, s_st0, okm0, s_st2, okm2, s_st1);
                 if (si + 1 >= steps) break;
-                body.template operator()<VC, SH>(si + 1, s_st1, okm1, s_st0, okm0, s_st2);
+                body.template operator()<VC, SH, CF>(si + 1, s_st1, okm1, s_st0, okm0, s_st2);
                 if (si + 2 >= steps) break;
-                body.template operator()<VC, SH>(si + 2, s_st2, okm2, s_st1, okm1, s_st0);
+                body.template operator()<VC, SH, CF>(si + 2, s_st2, okm2, s_st1, okm1, s_st0);
             }
             else
             {
-                body.template operator()<VC, SH>(si, s_st0, okm0, s_st3, okm3, s_st1);
+                body.template operator()<VC, SH, CF>(si, s_st0, okm0, s_st3, okm3, s_st1);
                 if (si + 1 >= steps) break;
-                body.template operator()<VC, SH>(si + 1, s_st1, okm1, s_st0, okm0, s_st2);
+                body.template operator()<VC, SH, CF>(si + 1, s_st1, okm1, s_st0, okm0, s_st2);
                 if (si + 2 >= steps) break;
-                body.template operator()<VC, SH>(si + 2, s_st2, okm2, s_st1, okm1, s_st3);
+                body.template operator()<VC, SH, CF>(si + 2, s_st2, okm2, s_st1, okm1, s_st3);
                 if (si + 3 >= steps) break;
-                body.template operator()<VC, SH>(si + 3, s_st3, okm3, s_st2, okm2, s_st0);
+                body.template operator()<VC, SH, CF>(si + 3, s_st3, okm3, s_st2, okm2, s_st0);
             }
         }
         wait_vm<0>();  // no load may still be writing this workgroup's LDS when it ends
@@ -1314,7 +1491,7 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         wait_lgkm0();
         __builtin_amdgcn_s_barrier();  // flags written; every wave is past its last reads of the stages
         if (s_vover != 0)              // uniform: some V value of the workgroup's keys does not fit f16
-            pipeline.template operator()<false, false>();
+            pipeline.template operator()<false, false, CAN_CF>();
     }
     else if constexpr (CT == I8)
     {
@@ -1324,11 +1501,38 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         // (|V| up to about 1.3e8); products that the scaling takes below f16's normal range keep an absolute error
         // of at most 2^-13 of the unscaled p times the V scale.
         pipeline.template operator()<false, false>();
-        if (!acc_finite()) s_vover = 1;
+        bool again = !acc_finite();
+        if constexpr (RULE)
+        {
+            // An infinite or NaN scale reaches the queries that see its key as it should, and is nothing to rerun for (the
+            // others would lose p's low bits to the shift): only a finite scale that can overflow is.
+            if (again)
+            {
+                bool big = false;
+                for (int t = pg_lo * kBlockSize + lane; t < min(pg_hi * kBlockSize, L); t += 64)
+                {
+                    const uint32_t pg = static_cast<uint32_t>(table_row[t / kBlockSize]);
+                    if (pg >= static_cast<uint32_t>(a.num_blocks)) continue;
+                    const float vs = __builtin_fabsf(a.v_scale[(static_cast<size_t>(pg) * kBlockSize + t % kBlockSize) * Hkv + kvh]);
+                    big = big || (vs >= 255.0f && vs < __builtin_huge_valf());
+                }
+                again = __any(big);
+            }
+        }
+        if (again) s_vover = 1;
         wait_lgkm0();
         __builtin_amdgcn_s_barrier();  // flags written; every wave is past its last reads of the stages
         if (s_vover != 0)              // uniform
             pipeline.template operator()<false, true>();
+    }
+    else if constexpr (RULE)
+    {
+        pipeline.template operator()<false, false>();
+        if (!acc_finite()) s_vover = 1;
+        wait_lgkm0();
+        __builtin_amdgcn_s_barrier();  // flags written; every wave is past its last reads of the stages
+        if (s_vover != 0)              // uniform
+            pipeline.template operator()<false, false, CAN_CF>();
     }
     else
     {
@@ -1618,22 +1822,27 @@ hipError_t launch_pfd(const PrefillArgs& a, hipStream_t stream)
 // be (1 to 2 us: a first chunk of 256 tokens behind a wide table 12.9 -> 14.8, 4 x 33 tokens over 210 to 300 with their
 // append 20.8 -> 21.8), so it is split from a little earlier on (split_from), where that costs no more than the empty
 // merge.  A caller that gives max_context_len pays it only where rows may be long.
-void prefill_plan(PrefillArgs& a)
+void prefill_plan_for(PrefillArgs& a, const void* fn, int threads, int step_keys, int most_keys)
 {
     a.n_split = 1;
     a.split_slots = 0;
     a.split_from = 0;
-    const int64_t       blocks = prefill_row_blocks(a);
-    const PrefillKernel k = prefill_kernel(a);
-    const int           slots = decode_mfma_items(k.fn, k.threads, 1);
+    const int64_t blocks = prefill_row_blocks(a);
+    const int     slots = decode_mfma_items(fn, threads, 1);
     if (blocks <= 0 || 2 * blocks > slots) return;
     int64_t       n = slots / blocks;
-    const int64_t steps = (static_cast<int64_t>(a.cap_tokens) + k.keys - 1) / k.keys;  // most steps of a block
+    const int64_t steps = (static_cast<int64_t>(most_keys) + step_keys - 1) / step_keys;  // most steps of a block
     if (steps < (n >= 5 ? 12 : (n >= 3 ? 15 : 24))) return;
     a.split_from = n >= 8 ? 8 : (n >= 5 ? 9 : (n >= 3 ? 13 : 19));
     n = std::min(std::min(n, steps / kPrefillSplitMin), static_cast<int64_t>(kPrefillSplitMax));
     a.n_split = static_cast<int>(n);
     a.split_slots = slots;
+}
+
+void prefill_plan(PrefillArgs& a)
+{
+    const PrefillKernel k = prefill_kernel(a);
+    prefill_plan_for(a, k.fn, k.threads, k.keys, a.cap_tokens);
 }
 
 PrefillSplitLayout prefill_split_layout(const PrefillArgs& a)
@@ -1654,7 +1863,11 @@ hipError_t launch_prefill(const PrefillArgs& a, hipStream_t stream)
 {
     if (a.n_split <= 1) return launch_pfd<false, false>(a, stream);
     const hipError_t e = launch_pfd<false, true>(a, stream);
-    if (e != hipSuccess) return e;
+    return e != hipSuccess ? e : launch_prefill_merge(a, stream);
+}
+
+hipError_t launch_prefill_merge(const PrefillArgs& a, hipStream_t stream)
+{
     if (a.qo_dtype == F32) return launch_prefill_merge_q<F32>(a, stream);
     if (a.qo_dtype == F16) return launch_prefill_merge_q<F16>(a, stream);
     return launch_prefill_merge_q<BF16>(a, stream);

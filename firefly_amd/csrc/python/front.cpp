@@ -33,6 +33,8 @@ struct Functions
     decltype(&ffkv_rope)                       rope;
     decltype(&ffkv_rope_append)                rope_append;
     decltype(&ffkv_paged_decode_scored)        decode_scored;
+    decltype(&ffkv_prefill_scored_workspace_bytes) prefill_scored_bytes;
+    decltype(&ffkv_paged_prefill_scored)       prefill_scored;
 };
 Functions fn{};
 
@@ -502,6 +504,71 @@ PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n)
     return rc;
 }
 
+// q, out, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, max_context_len, scale, num_blocks, score_cap,
+// slopes, window, key_begin, key_end, stream, scratch (as prefill's)
+PyObject* prefill_scored(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!count(n, 18)) return nullptr;
+    Reader    r{a};
+    PyObject* q = a[0];
+    int       B, S, Hq, D;
+    r.dims4(q, B, S, Hq, D);
+    const int  Hkv = r.dim(a[2], 2), qt = r.dtype(q), ct = r.dtype(a[2]);
+    const bool paged = a[6] != Py_None;
+    r.plain(q, "q", q);
+    if (r.ok && r.dtype(a[1]) != qt) r.refuse(PyExc_TypeError, "out must have q's dtype");
+    r.plain(a[1], "out", q);
+    if (r.ok && r.nbytes(a[1]) != r.nbytes(q)) r.refuse(PyExc_ValueError, "out must have as many values as q");
+    const int pages = paged ? r.dim(a[2], 0) : B, slots = paged ? FFKV_BLOCK_SIZE : S;
+    r.holds(a[2], "k_cache", ct, {pages, slots, Hkv, D}, q, false);
+    r.holds(a[3], "v_cache", ct, {pages, slots, Hkv, D}, q, false);
+    check_scales(r, a[4], "k_scale", ct, a[2], Hkv, q);
+    check_scales(r, a[5], "v_scale", ct, a[2], Hkv, q);
+    int mb = 0, N = 0;
+    if (paged)
+    {
+        r.holds(a[6], "block_table", kInt32, {B, -1}, q, false);
+        r.holds(a[7], "context_lens", kInt32, {B}, q, false);
+        mb = r.dim(a[6], 1), N = r.blocks(a[10], a[2]);
+        check_blocks(r, N, a[2]);
+    }
+    else if (r.ok && a[7] != Py_None)
+        r.refuse(PyExc_ValueError, "context_lens without a block table: contiguous keys begin at position 0");
+    const int   mcl = r.integer(a[8]);
+    const float scale = r.real(a[9]);
+    Rule        u;
+    u.cap = r.real(a[11]);
+    r.holds(a[12], "slopes", FFKV_DTYPE_F32, {Hq}, q, true);
+    u.window = r.integer(a[13]);
+    r.holds(a[14], "key_begin", kInt32, {B, S}, q, true);
+    r.holds(a[15], "key_end", kInt32, {B, S}, q, true);
+    r.current(q, B > 0 && S > 0);
+    void *out = r.ptr(a[1]), *qp = r.ptr(q), *kc = r.ptr(a[2]), *vc = r.ptr(a[3]);
+    auto *ks = r.ptr<float>(a[4]), *vs = r.ptr<float>(a[5]);
+    auto *bt = r.ptr<int32_t>(a[6]), *cx = r.ptr<int32_t>(a[7]);
+    u.slopes = r.ptr<float>(a[12]), u.begin = r.ptr<int32_t>(a[14]), u.end = r.ptr<int32_t>(a[15]);
+    void* s = r.stream(a[16]);
+    if (!r.ok) return nullptr;
+    PyObject*    ws = nullptr;
+    const size_t need =
+        fn.prefill_scored_bytes(qt, ct, B, S, Hq, Hkv, D, paged, mb, mcl, u.window, u.end != nullptr);
+    if (need > 0)
+    {
+        PyObject* nb = PyLong_FromSize_t(need);
+        ws = nb ? PyObject_CallFunctionObjArgs(a[17], nb, q, a[16], nullptr) : nullptr;
+        Py_XDECREF(nb);
+        if (ws == nullptr) return nullptr;
+    }
+    void*        w = ws ? r.ptr(ws) : nullptr;
+    const size_t wb = ws ? r.nbytes(ws) : 0;
+    PyObject*    rc = finish(r, [&] {
+        return fn.prefill_scored(qp, out, qt, kc, vc, ct, ks, vs, bt, cx, B, S, Hq, Hkv, D, FFKV_BLOCK_SIZE, mb, N, mcl,
+                                    scale, u.cap, u.slopes, u.window, u.begin, u.end, w, wb, s);
+    });
+    Py_XDECREF(ws);
+    return rc;
+}
+
 // q or None, k, context_lens, theta, stream
 PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
@@ -571,7 +638,7 @@ PyObject* forget_stream(PyObject*, PyObject*)
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(decode_scored),
+PyMethodDef methods[] = {FAST(decode_scored),  FAST(prefill_scored),
                          FAST(append),         FAST(decode),  FAST(decode_shared), FAST(append_decode),
                          FAST(decode_noalloc), FAST(prefill), FAST(rope),          FAST(rope_append),
                          {"bind", bind, METH_VARARGS, nullptr},

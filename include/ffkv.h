@@ -310,6 +310,30 @@ FFKV_API int ffkv_paged_decode_scored(const void* q, void* out, int qo_dtype, vo
                                       float* weights, const float* prior, float decay, int64_t weight_stride,
                                       void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * ffkv_paged_prefill_ws under a score rule (see above): query token t of row b at position i = context_lens[b] + t (t
+ * without a block table) sees the keys j of its row with lo <= j < hi,
+ *   lo = max(0, key_begin[b, t], i - window + 1),  hi = min(the row's tokens, key_end[b, t])  (key_end NULL: i + 1, causal)
+ * where the row's tokens are those that ffkv_paged_prefill attends at most, context_lens[b] + seq_len, cut at
+ * max_context_len.  key_begin / key_end int32 [batch, seq_len], either or both NULL: documents in one row (begin of the
+ * query's document), prefixes that all queries see (end = max(prefix, i + 1)), documents seen both ways (end of the
+ * document), queries that see nothing (end 0, padding).  A query's visible keys may lie after it; distances are |i - j|.
+ * Unlike in ffkv_paged_prefill, an infinite or NaN V value reaches only the queries that see its key (a workgroup that
+ * meets one reruns).  V ranges, types, head dims, workspace and errors as for ffkv_paged_prefill_ws; with_key_end: whether
+ * the call has a key_end.
+ */
+FFKV_API size_t ffkv_prefill_scored_workspace_bytes(int qo_dtype, int cache_dtype, int batch, int seq_len, int num_heads,
+                                                    int num_kv_heads, int head_dim, int paged, int max_blocks,
+                                                    int max_context_len, int window, int with_key_end);
+
+FFKV_API int ffkv_paged_prefill_scored(const void* q, void* out, int qo_dtype, const void* k_cache, const void* v_cache,
+                                       int cache_dtype, const float* k_scale, const float* v_scale,
+                                       const int32_t* block_table, const int32_t* context_lens, int batch, int seq_len,
+                                       int num_heads, int num_kv_heads, int head_dim, int block_size, int max_blocks,
+                                       int num_blocks, int max_context_len, float scale, float score_cap,
+                                       const float* slopes, int window, const int32_t* key_begin, const int32_t* key_end,
+                                       void* workspace, size_t workspace_bytes, void* stream);
+
 /* Message describing the last error returned on the calling thread ("" if none). */
 FFKV_API const char* ffkv_last_error(void);
 

@@ -9,7 +9,8 @@ The bounds count roundings (half a step each, relative: bf16 2^-8, fp16 2^-11, f
   weights   p off by exp(2 max |ds|) - 1 (numerator and denominator) and 2^-20 (exponent argument up to 2^6 rounded at 2^-18 of
             its last bits, exponential, sums, reciprocal): (n / 2^12 + 16) 2^-20 for n keys.
   output    as the weights, times sum p |v|; P enters the products in fp16 or as a bf16 pair (2^-11 of it, and 2^-25 absolute
-            where fp16 is subnormal, per key) and the output is rounded to its type.
+            where fp16 is subnormal, per key) and the output is rounded to its type.  The prefill's denominator sums the
+            rounded P too: p_step = 2^-10; its bf16 V enters in fp16 (2^-25 absolute below 2^-14).
 """
 
 from __future__ import annotations
@@ -35,7 +36,8 @@ def values(c, which):
     return cases.decode(pool, c.kv).astype(np.float64)
 
 
-def attention(q, k, v, pos, cap=0.0, slopes=None, window=0, begin=None, end=None, total=None, absent=None, act=None, kv=None):
+def attention(q, k, v, pos, cap=0.0, slopes=None, window=0, begin=None, end=None, total=None, absent=None, act=None, kv=None,
+              p_step=2.0 ** -11):
     """q [S, Hq, D] at positions pos .. pos + S - 1 over k, v [T, Hkv, D] (v None: the weights alone), float64 arrays.
     begin / end [S]: visible range of each query; total: the row's tokens; absent [T]: keys on no page.
     Returns out, its bound, weights [Hkv, T], their bound."""
@@ -84,9 +86,11 @@ def attention(q, k, v, pos, cap=0.0, slopes=None, window=0, begin=None, end=None
         out[:, h] = p @ v0
         exact = kv == O.DTYPE_F32
         step = np.abs(v0).max(initial=0.0) * (2.0 ** -25 * n if not exact else 0.0 * n)
+        if kv == O.DTYPE_BF16:
+            step = step + 2.0 ** -25
         if kv == O.DTYPE_I8:  # P carries the scales: an absolute 2^-25 of codes up to 127
             step = np.maximum(step, 127 * 2.0 ** -25 * n)
-        bound[:, h] = (p * (rel + (0.0 if exact else 2.0 ** -11))) @ np.abs(v0) + step[:, None]
+        bound[:, h] = (p * (rel + (0.0 if exact else p_step))) @ np.abs(v0) + step[:, None]
     if act is not None:
         bound += HALF[act] * np.abs(out) + 1e-30
     return out, bound, w, wb

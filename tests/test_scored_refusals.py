@@ -107,3 +107,51 @@ def test_decode_front(ff):
             ff.paged_attention_scored(**kw, stream=0)
     with pytest.raises(ValueError, match="GPU"):
         ff.paged_attention_scored(**_tensors(B=1), stream=0)
+
+
+def _prefill(ff, **kw):
+    a = dict(q=16, out=16, qo_dtype=ff.DTYPE_BF16, k_cache=16, v_cache=16, cache_dtype=ff.DTYPE_BF16, k_scale=None,
+             v_scale=None, block_table=16, context_lens=16, batch=1, seq_len=4, num_heads=32, num_kv_heads=8, head_dim=128,
+             block_size=16, max_blocks=4, num_blocks=4, max_context_len=0, scale=0.0, score_cap=0.0, slopes=None, window=0,
+             key_begin=None, key_end=None, workspace=None, workspace_bytes=0, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return ff.lib.ffkv_paged_prefill_scored(*a.values())
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(block_size=8), -2), (dict(head_dim=96), -2), (dict(qo_dtype=8), -2), (dict(cache_dtype=0), -2),
+    (dict(cache_dtype=4), -2), (dict(num_heads=30), -1), (dict(batch=-1), -1), (dict(seq_len=-1), -1), (dict(batch=70000), -2),
+    (dict(seq_len=1 << 30), -2), (dict(context_lens=None), -1), (dict(out=None), -1), (dict(cache_dtype=3), -1),
+    (dict(cache_dtype=3, block_table=None, k_scale=16, v_scale=16), -2), (dict(k_cache=24), -1), (dict(workspace=8), -1),
+    (dict(score_cap=-2.0), -1), (dict(score_cap=NAN), -1), (dict(window=-5), -1), (dict(slopes=2), -1),
+    (dict(key_begin=6), -1), (dict(key_end=7), -1),
+])
+def test_prefill_rejects(ff, kw, code):
+    assert _prefill(ff, **kw) == code
+    assert ff.lib.ffkv_last_error().decode() != ""
+    assert _prefill(ff, seq_len=0, q=None) == 0
+
+
+def test_prefill_front(ff):
+    t = _tensors()
+    q = torch.zeros(0, 5, 4, D, dtype=torch.bfloat16)
+    r = torch.zeros(0, 5, dtype=torch.int32)
+    t["q"] = q
+    assert ff.paged_prefill_scored(**t, key_begin=r, key_end=r, slopes=torch.zeros(4), stream=0).shape == (0, 5, 4 * D)
+    k = torch.zeros(0, 5, HKV, D, dtype=torch.bfloat16)
+    assert ff.paged_prefill_scored(q, k, k, None, None, window=2, stream=0).shape == (0, 5, 4 * D)
+    bad = [
+        (ValueError, dict(t, q=q[:, 0])), (ValueError, dict(t, key_begin=r[:, :4])), (TypeError, dict(t, key_end=r.long())),
+        (TypeError, dict(t, block_table=t["block_table"].long())), (ValueError, dict(t, context_lens=torch.zeros(1, dtype=torch.int32))),
+        (ValueError, dict(t, v_cache=t["v_cache"][:1])), (ValueError, dict(t, slopes=torch.zeros(5))),
+        (ValueError, dict(t, block_table=None)), (ValueError, dict(t, num_blocks=9)),
+        (ValueError, dict(q=q, k_cache=k[:, :4], v_cache=k[:, :4], block_table=None, context_lens=None)),
+        (TypeError, dict(t, out=torch.zeros(0, 5, 4 * D))), (ff.FFKVError, dict(t, window=-1)),
+        (ff.FFKVError, dict(t, score_cap=-1.0)), (TypeError, dict(t, window="3")),
+    ]
+    for error, kw in bad:
+        with pytest.raises(error):
+            ff.paged_prefill_scored(**kw, stream=0)
+    with pytest.raises(ValueError, match="GPU"):
+        ff.paged_prefill_scored(**dict(_tensors(B=1), q=torch.zeros(1, 2, 4, D, dtype=torch.bfloat16)), stream=0)
