@@ -103,6 +103,9 @@ def _load() -> ctypes.CDLL:
     lib.ffkv_paged_prefill_scored.restype = i32
     lib.ffkv_paged_prefill_scored.argtypes = [vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
                                               i32, i32, f32, *rule, vp, vp, vp, sz, vp]
+    lib.ffkv_evict.restype = i32
+    lib.ffkv_evict.argtypes = [vp, ctypes.c_int64, vp, i32, i32, i32, vp, vp, i32, vp, vp, vp, i32, vp, i32, vp, vp, vp,
+                               ctypes.c_int64, i32, i32, i32, i32, i32, vp]
     lib.ffkv_last_error.restype = ctypes.c_char_p
     lib.ffkv_last_error.argtypes = []
     lib.ffkv_version.restype = ctypes.c_char_p
@@ -116,7 +119,7 @@ def _bind(lib, torch) -> None:
     """Point the native front end (``_front``, csrc/python/front.cpp) at ``lib``'s functions."""
     names = ("append", "paged_decode", "append_paged_decode", "paged_decode_shared_prefix", "paged_decode_noalloc",
              "prefill_workspace_bytes", "paged_prefill_ws", "rope", "rope_append", "paged_decode_scored",
-             "prefill_scored_workspace_bytes", "paged_prefill_scored")
+             "prefill_scored_workspace_bytes", "paged_prefill_scored", "evict")
     _front.bind(tuple(ctypes.cast(getattr(lib, "ffkv_" + n), ctypes.c_void_p).value for n in names),
                 [*_torch_dtypes(torch).items(), (torch.int32, _INT32)], getattr(torch._C, "_cuda_getDevice", None),
                 getattr(torch._C, "_cuda_getCurrentRawStream", None), lambda: torch.cuda.current_stream().cuda_stream)
@@ -349,3 +352,24 @@ def paged_prefill_scored(q, k_cache, v_cache, block_table, context_lens, score_c
                                 scale, num_blocks, score_cap, slopes, window, key_begin, key_end, stream,
                                 _prefill_scratch))
     return out
+
+
+def evict_tokens(weights, k_cache, v_cache, block_table, context_lens, keep: int, sinks: int = 0, recent: int = 0,
+                 dst_table=None, weights_out=None, kept=None, kept_lens=None, k_scale=None, v_scale=None,
+                 num_blocks: int | None = None, stream=None):
+    """Cut the rows of the cache to their ``keep`` tokens of most attention weight (``ffkv_evict``): ``weights`` fp32
+    ``[B, Hkv, T]``, ``context_lens`` the rows' tokens; the first ``sinks`` and last ``recent`` always stay.  The kept tokens
+    move to the front of the row's pages in ``dst_table`` int32 ``[B, blocks]`` (None: of its own pages, which no other row
+    may hold), their weights to ``weights_out`` (None: not; may be ``weights``).  Returns ``kept`` int32 ``[B, Hkv, keep]``
+    (the kept positions, ascending) and the rows' new lengths."""
+    if kept is None or kept_lens is None:
+        import torch
+
+        like = {"dtype": torch.int32, "device": weights.device}
+        if kept is None:
+            kept = torch.empty((*weights.shape[:2], max(0, keep)), **like)
+        if kept_lens is None:
+            kept_lens = torch.empty(weights.shape[0], **like)
+    check(_front.evict(weights, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, keep, sinks, recent, dst_table,
+                       kept, kept_lens, weights_out, num_blocks, stream))
+    return kept, kept_lens

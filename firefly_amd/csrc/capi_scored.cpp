@@ -371,4 +371,71 @@ int ffkv_paged_prefill_scored(const void* q, void* out, int qo_dtype, const void
     return ok();
 }
 
+int ffkv_evict(const float* weights, int64_t weight_stride, const int32_t* context_lens, int keep, int sinks, int recent,
+               void* k_cache, void* v_cache, int cache_dtype, float* k_scale, float* v_scale, const int32_t* block_table,
+               int max_blocks, const int32_t* dst_table, int dst_blocks, int32_t* kept, int32_t* kept_lens,
+               float* weights_out, int64_t out_stride, int batch, int num_kv_heads, int head_dim, int block_size,
+               int num_blocks, void* stream)
+{
+    if (block_size != FFKV_BLOCK_SIZE) return fail(FFKV_ERR_UNSUPPORTED, "block_size must be 16, got %d", block_size);
+    if (!is_cache(cache_dtype)) return fail(FFKV_ERR_UNSUPPORTED, "unsupported cache dtype %d", cache_dtype);
+    if (!head_dim_ok(head_dim))
+        return fail(FFKV_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 up to 128, or 256, got %d", head_dim);
+    if (batch < 0 || num_kv_heads <= 0 || max_blocks < 0 || num_blocks < 0 || dst_blocks < 0 || weight_stride < 0 ||
+        out_stride < 0)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "bad size (batch %d kv_heads %d max_blocks %d dst_blocks %d num_blocks %d)",
+                    batch, num_kv_heads, max_blocks, dst_blocks, num_blocks);
+    if (batch > 65535 || num_kv_heads > 65535)
+        return fail(FFKV_ERR_UNSUPPORTED, "batch and num_kv_heads must be <= 65535");
+    if (keep < 1 || sinks < 0 || recent < 0 || static_cast<int64_t>(sinks) + recent > keep)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "keep %d must be at least 1 and hold sinks %d and recent %d", keep, sinks,
+                    recent);
+    const int64_t bound = std::min<int64_t>(weight_stride, static_cast<int64_t>(max_blocks) * FFKV_BLOCK_SIZE);
+    if (bound > INT32_MAX - 64 * 1024) return fail(FFKV_ERR_UNSUPPORTED, "rows of 2^31 tokens");
+    if (weights_out != nullptr && out_stride < std::min<int64_t>(keep, bound))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "out_stride %lld is less than the kept tokens",
+                    static_cast<long long>(out_stride));
+    if (weights_out != nullptr && weights_out == weights && out_stride != weight_stride)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "weights_out in place needs the weights' own stride");
+    if (batch == 0) return ok();
+    if (!weights || !context_lens || !k_cache || !v_cache || !block_table || !kept || !kept_lens)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "null weights, context_lens, cache, block_table, kept or kept_lens pointer");
+    if (kept_lens == context_lens)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "kept_lens must not be context_lens");
+    if (cache_dtype == FFKV_DTYPE_I8 && (!k_scale || !v_scale))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "int8 cache needs k_scale and v_scale");
+    if (!aligned16(k_cache) || !aligned16(v_cache))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "cache pointers must be 16-byte aligned");
+    if (!aligned4(weights) || !aligned4(weights_out) || !aligned4(kept) || !aligned4(kept_lens))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "weights, kept and kept_lens must be 4-byte aligned");
+
+    ffkv::EvictArgs a{};
+    a.weights = weights;
+    a.weight_stride = weight_stride;
+    a.context_lens = context_lens;
+    a.keep = keep;
+    a.sinks = sinks;
+    a.recent = recent;
+    a.k_cache = k_cache;
+    a.v_cache = v_cache;
+    a.k_scale = k_scale;
+    a.v_scale = v_scale;
+    a.cache_dtype = cache_dtype;
+    a.block_table = block_table;
+    a.max_blocks = max_blocks;
+    a.dst_table = dst_table;
+    a.dst_blocks = dst_blocks;
+    a.kept = kept;
+    a.kept_lens = kept_lens;
+    a.weights_out = weights_out;
+    a.out_stride = out_stride;
+    a.batch = batch;
+    a.num_kv_heads = num_kv_heads;
+    a.head_dim = head_dim;
+    a.num_blocks = num_blocks;
+    const hipError_t e = ffkv::launch_evict(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "evict launch");
+    return ok();
+}
+
 }  // extern "C"

@@ -168,6 +168,32 @@ struct DecodeArgs
     int64_t        weight_stride;
 };
 
+struct EvictArgs
+{
+    const float*   weights;  // [batch, num_kv_heads, weight_stride]
+    int64_t        weight_stride;
+    const int32_t* context_lens;  // tokens of each row
+    int            keep, sinks, recent;
+    void*          k_cache;
+    void*          v_cache;
+    float*         k_scale;  // int8 caches
+    float*         v_scale;
+    int            cache_dtype;
+    const int32_t* block_table;  // [batch, max_blocks]
+    int            max_blocks;
+    const int32_t* dst_table;  // [batch, dst_blocks], or null: in place
+    int            dst_blocks;
+    int32_t*       kept;       // [batch, num_kv_heads, keep]
+    int32_t*       kept_lens;  // [batch]
+    float*         weights_out;  // [batch, num_kv_heads, out_stride], or null
+    int64_t        out_stride;
+    int            batch;
+    int            num_kv_heads;
+    int            head_dim;
+    int            num_blocks;
+};
+
+hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
 hipError_t launch_append(const AppendArgs& a, hipStream_t stream);
 hipError_t launch_rope_append(const RopeArgs& a, hipStream_t stream);      // rotate q/k, then append when k_cache set
 hipError_t launch_prefill(const PrefillArgs& a, hipStream_t stream);  // matrix-core prefill (16- and 8-bit caches)

@@ -35,6 +35,7 @@ struct Functions
     decltype(&ffkv_paged_decode_scored)        decode_scored;
     decltype(&ffkv_prefill_scored_workspace_bytes) prefill_scored_bytes;
     decltype(&ffkv_paged_prefill_scored)       prefill_scored;
+    decltype(&ffkv_evict)                      evict;
 };
 Functions fn{};
 
@@ -569,6 +570,46 @@ PyObject* prefill_scored(PyObject*, PyObject* const* a, Py_ssize_t n)
     return rc;
 }
 
+// weights, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, keep, sinks, recent, dst_table, kept,
+// kept_lens, weights_out, num_blocks, stream
+PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!count(n, 16)) return nullptr;
+    Reader    r{a};
+    PyObject* w = a[0];
+    const int B = r.dim(w, 0), Hkv = r.dim(a[1], 2), D = r.dim(a[1], 3), ct = r.dtype(a[1]);
+    r.holds(w, "weights", FFKV_DTYPE_F32, {B, Hkv, -1}, w, false);
+    r.holds(a[1], "k_cache", ct, {-1, FFKV_BLOCK_SIZE, Hkv, D}, w, false);
+    r.holds(a[2], "v_cache", ct, {r.dim(a[1], 0), FFKV_BLOCK_SIZE, Hkv, D}, w, false);
+    if (ct == FFKV_DTYPE_I8)
+    {
+        check_scales(r, a[3], "k_scale", ct, a[1], Hkv, w);
+        check_scales(r, a[4], "v_scale", ct, a[1], Hkv, w);
+    }
+    r.holds(a[5], "block_table", kInt32, {B, -1}, w, false);
+    r.holds(a[6], "context_lens", kInt32, {B}, w, false);
+    const int keep = r.integer(a[7]), sinks = r.integer(a[8]), recent = r.integer(a[9]);
+    r.holds(a[10], "dst_table", kInt32, {B, -1}, w, true);
+    r.holds(a[11], "kept", kInt32, {B, Hkv, keep}, w, false);
+    r.holds(a[12], "kept_lens", kInt32, {B}, w, false);
+    r.holds(a[13], "weights_out", FFKV_DTYPE_F32, {B, Hkv, -1}, w, true);
+    const int       mb = r.dim(a[5], 1), N = r.blocks(a[14], a[1]);
+    const int       db = r.ok && a[10] != Py_None ? r.dim(a[10], 1) : 0;
+    const long long stride = r.dim(w, 2), ostride = r.ok && a[13] != Py_None ? r.dim(a[13], 2) : 0;
+    check_blocks(r, N, a[1]);
+    r.current(w, B > 0);
+    auto *wp = r.ptr<float>(w), *wo = r.ptr<float>(a[13]);
+    void *kc = r.ptr(a[1]), *vc = r.ptr(a[2]);
+    auto *ks = r.ptr<float>(a[3]), *vs = r.ptr<float>(a[4]);
+    auto *bt = r.ptr<int32_t>(a[5]), *cx = r.ptr<int32_t>(a[6]), *dt = r.ptr<int32_t>(a[10]), *kp = r.ptr<int32_t>(a[11]),
+         *kl = r.ptr<int32_t>(a[12]);
+    void* s = r.stream(a[15]);
+    return finish(r, [&] {
+        return fn.evict(wp, stride, cx, keep, sinks, recent, kc, vc, ct, ks, vs, bt, mb, dt, db, kp, kl, wo, ostride, B, Hkv,
+                        D, FFKV_BLOCK_SIZE, N, s);
+    });
+}
+
 // q or None, k, context_lens, theta, stream
 PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
@@ -638,7 +679,7 @@ PyObject* forget_stream(PyObject*, PyObject*)
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(decode_scored),  FAST(prefill_scored),
+PyMethodDef methods[] = {FAST(decode_scored),  FAST(prefill_scored), FAST(evict),
                          FAST(append),         FAST(decode),  FAST(decode_shared), FAST(append_decode),
                          FAST(decode_noalloc), FAST(prefill), FAST(rope),          FAST(rope_append),
                          {"bind", bind, METH_VARARGS, nullptr},

@@ -334,6 +334,32 @@ FFKV_API int ffkv_paged_prefill_scored(const void* q, void* out, int qo_dtype, c
                                        const float* slopes, int window, const int32_t* key_begin, const int32_t* key_end,
                                        void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Eviction from the cache by attention weight.  Row b holds context_lens[b] tokens (all appended; clamped to what its
+ * block table and weight_stride hold), whose weights per KV head are weights fp32 [batch, num_kv_heads, weight_stride], as
+ * ffkv_paged_decode_scored and ffkv_attention_weights leave them.  A row of more than `keep` tokens keeps, per KV head, its
+ * first `sinks` and its last `recent` tokens and of those between the keep - sinks - recent with the largest weights (of
+ * equal weights the earlier token stays; NaN is the least); a shorter row keeps all.  Then
+ *   kept       int32 [batch, num_kv_heads, keep]: the kept tokens' positions in ascending order (entries past the row's
+ *              count are left as they were)
+ *   kept_lens  int32 [batch]: min(context_lens[b], keep), the row's tokens from now on; not context_lens itself
+ *   K and V (and int8 scales) of kept token number j go to position j of the row in dst_table int32 [batch, dst_blocks],
+ *              pages of the same pools that no row of the call holds tokens in (pages shared with other rows stay whole);
+ *              dst_table NULL: to position j of the row's own pages, which no other row may hold then
+ *   weights_out fp32 [batch, num_kv_heads, out_stride], NULL or weights itself (with its stride) or apart from it: the kept
+ *              tokens' weights at their new positions, the rest left as it was
+ * Each KV head keeps tokens of its own: position j of a row then holds different tokens in different heads, each with the
+ * rotary embedding it was cached with, and the row goes on from position kept_lens[b] (the new tokens' rotary positions
+ * go on from the old ones).  A kept token whose source or destination page is absent is not copied.  keep >= 1, sinks
+ * and recent >= 0 and together at most keep.  Cache types, head dims and alignment as for ffkv_append.  No workspace.  No
+ * counterpart in the reference, which evicts whole prefix-cache nodes that no request uses (src/radix_tree.cc).
+ */
+FFKV_API int ffkv_evict(const float* weights, int64_t weight_stride, const int32_t* context_lens, int keep, int sinks,
+                        int recent, void* k_cache, void* v_cache, int cache_dtype, float* k_scale, float* v_scale,
+                        const int32_t* block_table, int max_blocks, const int32_t* dst_table, int dst_blocks,
+                        int32_t* kept, int32_t* kept_lens, float* weights_out, int64_t out_stride, int batch,
+                        int num_kv_heads, int head_dim, int block_size, int num_blocks, void* stream);
+
 /* Message describing the last error returned on the calling thread ("" if none). */
 FFKV_API const char* ffkv_last_error(void);
 

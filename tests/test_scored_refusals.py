@@ -155,3 +155,52 @@ def test_prefill_front(ff):
             ff.paged_prefill_scored(**kw, stream=0)
     with pytest.raises(ValueError, match="GPU"):
         ff.paged_prefill_scored(**dict(_tensors(B=1), q=torch.zeros(1, 2, 4, D, dtype=torch.bfloat16)), stream=0)
+
+
+def _evict(ff, **kw):
+    a = dict(weights=16, weight_stride=64, context_lens=16, keep=8, sinks=2, recent=3, k_cache=16, v_cache=16,
+             cache_dtype=ff.DTYPE_BF16, k_scale=None, v_scale=None, block_table=16, max_blocks=4, dst_table=None, dst_blocks=0,
+             kept=16, kept_lens=32, weights_out=None, out_stride=0, batch=1, num_kv_heads=2, head_dim=64, block_size=16,
+             num_blocks=4, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return ff.lib.ffkv_evict(*a.values())
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(block_size=8), -2), (dict(cache_dtype=6), -2), (dict(head_dim=100), -2), (dict(batch=-1), -1), (dict(batch=65536), -2),
+    (dict(num_kv_heads=0), -1), (dict(keep=0), -1), (dict(keep=-4), -1), (dict(sinks=-1), -1), (dict(recent=-1), -1),
+    (dict(sinks=6), -1), (dict(sinks=2 ** 31 - 1, recent=2 ** 31 - 1), -1), (dict(weights_out=64, out_stride=7), -1),
+    (dict(weights_out=16, out_stride=65), -1), (dict(weights=None), -1), (dict(kept=None), -1), (dict(kept_lens=None), -1),
+    (dict(kept_lens=16), -1), (dict(cache_dtype=3), -1), (dict(k_cache=24), -1), (dict(weights=18), -1), (dict(kept=18), -1),
+    (dict(weight_stride=-1), -1), (dict(weight_stride=1 << 40, max_blocks=2 ** 31 - 1), -2), (dict(dst_blocks=-1), -1),
+])
+def test_evict_rejects(ff, kw, code):
+    assert _evict(ff, **kw) == code
+    assert ff.lib.ffkv_last_error().decode() != ""
+    assert _evict(ff, batch=0, weights=None) == 0
+
+
+def test_evict_front(ff):
+    pool = torch.zeros(4, 16, HKV, D)
+    t = dict(weights=torch.zeros(0, HKV, 9), k_cache=pool, v_cache=pool.clone(), block_table=torch.zeros(0, 3, dtype=torch.int32),
+             context_lens=torch.zeros(0, dtype=torch.int32), keep=4)
+    kept, lens = ff.evict_tokens(**t, sinks=1, recent=3, dst_table=torch.zeros(0, 1, dtype=torch.int32), stream=0)
+    assert kept.shape == (0, HKV, 4) and lens.shape == (0,)
+    i = torch.zeros(0, HKV, 4, dtype=torch.int32)
+    bad = [
+        (ff.FFKVError, dict(t, keep=0)), (ff.FFKVError, dict(t, sinks=5)), (ValueError, dict(t, kept=i[..., :3])),
+        (TypeError, dict(t, kept=i.long())), (ValueError, dict(t, weights=torch.zeros(0, HKV + 1, 9))),
+        (ValueError, dict(t, weights=torch.zeros(1, HKV, 9))), (TypeError, dict(t, weights=torch.zeros(0, HKV, 9).half())),
+        (TypeError, dict(t, dst_table=torch.zeros(0, 1))), (ValueError, dict(t, dst_table=torch.zeros(1, 1, dtype=torch.int32))),
+        (ValueError, dict(t, kept_lens=torch.zeros(2, dtype=torch.int32))), (ValueError, dict(t, v_cache=pool[:3])),
+        (TypeError, dict(t, block_table=torch.zeros(0, 3))), (TypeError, dict(t, keep=4.0)),
+        (ValueError, dict(t, weights_out=torch.zeros(0, 1, 9))), (ValueError, dict(t, num_blocks=5)),
+        (ValueError, dict(t, k_cache=torch.zeros(4, 16, HKV, 2 * D)[..., ::2])),
+    ]
+    for error, kw in bad:
+        with pytest.raises(error):
+            ff.evict_tokens(**kw, stream=0)
+    with pytest.raises(ValueError, match="GPU"):
+        ff.evict_tokens(torch.zeros(1, HKV, 9), pool, pool, torch.zeros(1, 3, dtype=torch.int32),
+                        torch.zeros(1, dtype=torch.int32), 4, stream=0)
