@@ -103,6 +103,11 @@ def _load() -> ctypes.CDLL:
     lib.ffkv_paged_prefill_scored.restype = i32
     lib.ffkv_paged_prefill_scored.argtypes = [vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
                                               i32, i32, f32, *rule, vp, vp, vp, sz, vp]
+    lib.ffkv_attention_weights_workspace_bytes.restype = sz
+    lib.ffkv_attention_weights_workspace_bytes.argtypes = [i32] * 7
+    lib.ffkv_attention_weights.restype = i32
+    lib.ffkv_attention_weights.argtypes = [vp, i32, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, f32,
+                                           *rule, vp, vp, vp, vp, f32, ctypes.c_int64, vp, sz, vp]
     lib.ffkv_evict.restype = i32
     lib.ffkv_evict.argtypes = [vp, ctypes.c_int64, vp, i32, i32, i32, vp, vp, i32, vp, vp, vp, i32, vp, i32, vp, vp, vp,
                                ctypes.c_int64, i32, i32, i32, i32, i32, vp]
@@ -119,7 +124,7 @@ def _bind(lib, torch) -> None:
     """Point the native front end (``_front``, csrc/python/front.cpp) at ``lib``'s functions."""
     names = ("append", "paged_decode", "append_paged_decode", "paged_decode_shared_prefix", "paged_decode_noalloc",
              "prefill_workspace_bytes", "paged_prefill_ws", "rope", "rope_append", "paged_decode_scored",
-             "prefill_scored_workspace_bytes", "paged_prefill_scored", "evict")
+             "prefill_scored_workspace_bytes", "paged_prefill_scored", "evict", "attention_weights")
     _front.bind(tuple(ctypes.cast(getattr(lib, "ffkv_" + n), ctypes.c_void_p).value for n in names),
                 [*_torch_dtypes(torch).items(), (torch.int32, _INT32)], getattr(torch._C, "_cuda_getDevice", None),
                 getattr(torch._C, "_cuda_getCurrentRawStream", None), lambda: torch.cuda.current_stream().cuda_stream)
@@ -352,6 +357,35 @@ def paged_prefill_scored(q, k_cache, v_cache, block_table, context_lens, score_c
                                 scale, num_blocks, score_cap, slopes, window, key_begin, key_end, stream,
                                 _prefill_scratch))
     return out
+
+
+def attention_weights_workspace(batch: int, seq_len: int, num_heads: int, num_kv_heads: int, head_dim: int, max_blocks: int,
+                                max_context_len: int = 0, device=None):
+    """A workspace for ``attention_weights`` (``ffkv_attention_weights_workspace_bytes``)."""
+    import torch
+
+    n = int(lib.ffkv_attention_weights_workspace_bytes(batch, seq_len, num_heads, num_kv_heads, head_dim, max_blocks,
+                                                       max_context_len))
+    return torch.empty(max(n, 256), dtype=torch.uint8, device=device if device is not None else "cuda")
+
+
+def attention_weights(q, k_cache, block_table, context_lens, weights=None, prior=None, decay: float = 1.0,
+                      score_cap: float = 0.0, slopes=None, window: int = 0, key_begin=None, key_end=None, k_scale=None,
+                      max_context_len: int = 0, scale: float = 0.0, workspace=None, num_blocks: int | None = None,
+                      stream=None):
+    """The attention weights that queries ``q`` ``[B, S, Hq, D]`` (the rows' last S tokens, at ``context_lens[b] + t``) give to
+    the cached keys under the rule of ``paged_prefill_scored`` (``ffkv_attention_weights``): ``weights`` fp32 ``[B, Hkv, T]``
+    becomes ``decay * prior`` plus them, summed over queries and the heads of a KV head.  Without ``weights`` a new tensor
+    over the block table's (or ``max_context_len``) tokens, zero past a row's end.  Returns ``weights``."""
+    if weights is None:
+        import torch
+
+        most = block_table.shape[-1] * BLOCK_SIZE
+        most = min(most, max_context_len) if max_context_len > 0 else most
+        weights = torch.zeros((q.shape[0], k_cache.shape[2], most), dtype=torch.float32, device=q.device)
+    check(_front.attention_weights(q, k_cache, k_scale, block_table, context_lens, max_context_len, scale, num_blocks,
+                                   score_cap, slopes, window, key_begin, key_end, weights, prior, decay, workspace, stream))
+    return weights
 
 
 def evict_tokens(weights, k_cache, v_cache, block_table, context_lens, keep: int, sinks: int = 0, recent: int = 0,

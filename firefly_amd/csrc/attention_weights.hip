@@ -1,0 +1,622 @@
+// attention_weights.hip - the attention weights that the last S tokens of every row give to its cached keys, under a score
+// rule: what an engine goes by when it cuts a prompt's cache.
+//
+// With the scores s of paged_prefill_scored.hip, for row b, KV head v and key j:
+//   weights[b, v, j] = decay * prior[b, v, j] + sum over the S queries t and the query heads h of v of softmax(s_{t,h})_j
+// (keys of the S tokens themselves have no earlier weight).  No values, no output: K is read twice, V not at all.
+//
+// The sum over queries needs every query's final maximum and denominator first, so there are three launches: the states
+// (max, denominator) of every query row over each split of the keys, their fold, and the weights, which compute the scores
+// again.  (Written down instead, the scores of S * G query rows take 4 S G bytes per key, more than reading its K again
+// from 32 rows on.)  A workgroup of the first and third has the keys in its registers, as MFMA operands that serve all query
+// rows, and the query rows pass by in LDS.
+#include "mfma_common.h"
+#include "score_rule.h"
+
+namespace ffkv
+{
+
+namespace
+{
+
+constexpr int kAwWaves = 4;
+constexpr int kAwThreads = 64 * kAwWaves;
+// Pages of keys a wave holds: 64 registers of 16-bit operands at head_dim 128 and 256.
+template <int D>
+constexpr int kAwPages = D <= 128 ? 4 : 2;
+template <int D>
+constexpr int kAwChunk = kAwWaves * kAwPages<D> * kBlockSize;  // keys of a workgroup at a time
+// Query rows staged in LDS at a time: 64 KiB of them, at most 256.
+template <int D, bool LO>
+constexpr int kAwRows = []
+{
+    const int r = 65536 / (D * 2 * (LO ? 2 : 1)) / 16 * 16;
+    return r > 256 ? 256 : r;
+}();
+constexpr int kAwVecRows = 256;  // the vector kernel's, of which it stages 32 at a time
+constexpr int kAwVecTile = 32;
+constexpr int kAwVecChunk = kAwThreads;
+
+// Keys [x, y) that query token t of row b sees among its row's `total` tokens; z: its position.
+__device__ __forceinline__ int3 aw_visible(const WeightArgs& a, int b, int64_t ctx, int total, int t)
+{
+    const int64_t at = static_cast<int64_t>(b) * a.seq_len + t;
+    int64_t       hi = a.rule.key_end != nullptr ? a.rule.key_end[at] : ctx + t + 1;
+    hi = hi > total ? total : (hi < 0 ? 0 : hi);
+    int64_t lo = first_key(a.rule, ctx + t, a.rule.key_begin != nullptr ? a.rule.key_begin[at] : 0);
+    lo = lo > hi ? hi : lo;
+    return make_int3(static_cast<int>(lo), static_cast<int>(hi), static_cast<int>(ctx + t));
+}
+
+__device__ __forceinline__ int aw_total(const WeightArgs& a, int64_t ctx)
+{
+    int64_t total = ctx + a.seq_len;
+    if (total > a.cap_tokens) total = a.cap_tokens;
+    return total < 0 ? 0 : static_cast<int>(total);
+}
+
+// A state's (max, denominator) joined with another's; the maxima are finite or NaN (kLowest where there was no key).
+__device__ __forceinline__ float2 aw_join(float2 x, float2 y)
+{
+    const float m = __builtin_elementwise_maximum(x.x, y.x);
+    return make_float2(m, x.y * __builtin_amdgcn_exp2f(x.x - m) + y.y * __builtin_amdgcn_exp2f(y.x - m));
+}
+
+__device__ __forceinline__ void aw_store(const WeightArgs& a, int64_t bh, int64_t ctx, int total, int key, float w)
+{
+    if (key >= total) return;
+    const int64_t at = bh * a.weight_stride + key;
+    if (a.prior != nullptr && key < ctx) w = __builtin_fmaf(a.decay, a.prior[at], w);
+    a.weights[at] = w;
+}
+
+}  // namespace
+
+// Workgroup (split, row and KV head) of blockIdx.x: the keys of chunks split, split + splits, ..  SUM = false: the states of
+// query rows blockIdx.y * RB .. over them; SUM = true: the weights of them over all query rows.
+template <int CT, int QT, int D, bool SUM>
+__global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8))) void attention_weights_mfma(WeightArgs a)
+{
+    constexpr bool BF = kBF<CT, QT>;
+    using M = MType<BF>;
+    using X8 = typename M::x8;
+    using X4 = typename M::x4;
+    constexpr int  KSTEPS = D / 32;
+    constexpr bool KT = D % 32 == 16;  // a last k-step of 16 dims
+    constexpr int  DT = 32 * KSTEPS;
+    constexpr bool LO = !((QT == BF16 && BF) || (QT == F16 && !BF));
+    constexpr int  KP = kAwPages<D>;
+    constexpr int  RB = kAwRows<D, LO>;
+    constexpr int  CHUNK = kAwChunk<D>;
+    constexpr int  NP = LO ? 2 : 1;  // parts of q
+    auto dimof = [](int j, int g)    // first of the 8 dims of k-step j in lane group g (as the decode's)
+    {
+        if constexpr (kElemBytes<CT> == 1 && KSTEPS % 2 == 1)
+            if (j == KSTEPS - 1) return 32 * j + 8 * g;
+        return dim_of<CT>(j, g);
+    };
+    // q as MFMA operands in the order the lanes read them: [tile][part][k-step][lane]
+    __shared__ u32x4  s_q[RB / 16 * NP * KSTEPS * 64];
+    __shared__ u32x2  s_qt[KT ? RB / 16 * NP * 64 : 1];
+    __shared__ int3   s_vis[RB];
+    __shared__ float  s_slope[RB];
+    __shared__ float2 s_ml[SUM ? 1 : kAwWaves][RB];  // SUM: (max, 1 / denominator) of the rows; else every wave's states
+
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15;
+    const int g = lane >> 4;
+    const int split = static_cast<int>(blockIdx.x) % a.splits;
+    const int bh = static_cast<int>(blockIdx.x) / a.splits;
+    const int b = bh / a.num_kv_heads;
+    const int kvh = bh - b * a.num_kv_heads;
+    const int G = a.group;
+    const int R = a.seq_len * G;
+    const int64_t ctx = a.context_lens[b];
+    const int total = __builtin_amdgcn_readfirstlane(aw_total(a, ctx));
+    const int chunks = (total + CHUNK - 1) / CHUNK;
+    const int blocks = (R + RB - 1) / RB;
+    const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
+    float c_log2 = a.scale_log2;
+    if constexpr (CT == FP8) c_log2 *= a.k_scale[kvh];
+
+    auto stage = [&](int rb)
+    {
+        const int r0 = rb * RB;
+        const int tiles = (min(RB, R - r0) + 15) / 16;
+        auto      q_at = [&](int r)
+        {
+            const int t = r / G;
+            return ((static_cast<size_t>(b) * a.seq_len + t) * a.num_heads + kvh * G + (r - t * G)) * D;
+        };
+        auto parts = [&](const float* x, int n, uint32_t* hi, uint32_t* lo)
+        {
+            for (int e = 0; e < n; ++e)
+            {
+                hi[e] = M::bits(x[e]);
+                lo[e] = LO ? M::bits(x[e] - M::value(hi[e])) : 0u;
+            }
+        };
+        for (int i = tid; i < tiles * KSTEPS * 64; i += kAwThreads)
+        {
+            const int l = i & 63, j = (i >> 6) % KSTEPS, tile = (i >> 6) / KSTEPS;
+            const int r = r0 + tile * 16 + (l & 15);
+            u32x4*    dst = s_q + ((tile * NP) * KSTEPS + j) * 64 + l;
+            u32x4     hi = u32x4{0u, 0u, 0u, 0u}, lo = hi;
+            if (r < R)
+            {
+                const size_t at = q_at(r) + dimof(j, l >> 4);
+                if constexpr (!LO)
+                    hi = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
+                else
+                {
+                    float    x[8];
+                    uint32_t h[8], w[8];
+                    load_q8<QT>(a.q, at, x);
+                    parts(x, 8, h, w);
+                    hi = u32x4{h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
+                    lo = u32x4{w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16), w[6] | (w[7] << 16)};
+                }
+            }
+            dst[0] = hi;
+            if constexpr (LO) dst[KSTEPS * 64] = lo;
+        }
+        if constexpr (KT)
+            for (int i = tid; i < tiles * 64; i += kAwThreads)
+            {
+                const int l = i & 63, tile = i >> 6;
+                const int r = r0 + tile * 16 + (l & 15);
+                float     x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t  h[4], w[4];
+                if (r < R) load_act4(a.q, QT, q_at(r) + DT + 4 * (l >> 4), x);
+                parts(x, 4, h, w);
+                s_qt[tile * NP * 64 + l] = u32x2{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+                if constexpr (LO) s_qt[(tile * NP + 1) * 64 + l] = u32x2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)};
+            }
+        for (int i = tid; i < tiles * 16; i += kAwThreads)
+        {
+            const int r = r0 + i;
+            s_vis[i] = r < R ? aw_visible(a, b, ctx, total, r / G) : make_int3(0, 0, 0);
+            s_slope[i] = r < R && a.rule.slopes != nullptr ? a.rule.slopes[kvh * G + r % G] * 1.4426950408889634f : 0.0f;
+            if constexpr (SUM) s_ml[0][i] = r < R ? a.fin[static_cast<int64_t>(bh) * R + r] : make_float2(0.0f, 0.0f);
+        }
+        __syncthreads();
+        return tiles;
+    };
+
+    const int rb0 = SUM ? 0 : static_cast<int>(blockIdx.y);
+    int       tiles = 0;
+    if (split < chunks && (!SUM || blocks == 1)) tiles = stage(rb0);
+    if constexpr (!SUM)
+        for (int i = lane; i < RB; i += 64) s_ml[wave][i] = make_float2(kLowest, 0.0f);
+
+    for (int ch = split; ch < chunks; ch += a.splits)
+    {
+        const int key0 = ch * CHUNK + wave * (KP * kBlockSize);
+        // this wave's keys: lane (c, g) holds dims dimof(j, g) .. + 7 of key c of each page
+        X8    k[KP][KSTEPS > 0 ? KSTEPS : 1];
+        X4    kt[KP];
+        f32x4 ks[CT == I8 ? KP : 1];
+        int   okm = 0;
+#pragma unroll
+        for (int u = 0; u < KP; ++u)
+        {
+            const int pg = key0 / kBlockSize + u;
+            const int phys = pg * kBlockSize < total ? __builtin_amdgcn_readfirstlane(table[pg]) : -1;
+            const bool ok = phys >= 0 && phys < a.num_blocks;
+            okm |= ok ? 1 << u : 0;
+            const size_t row = (static_cast<size_t>(ok ? phys : 0) * kBlockSize + c) * a.num_kv_heads + kvh;
+            const char*  kp = static_cast<const char*>(a.k_cache) + row * D * kElemBytes<CT>;
+            if constexpr (kElemBytes<CT> == 2)
+            {
+#pragma unroll
+                for (int j = 0; j < KSTEPS; ++j)
+                    k[u][j] = __builtin_bit_cast(X8, ok ? *reinterpret_cast<const u32x4*>(kp + 2 * dimof(j, g))
+                                                        : u32x4{0u, 0u, 0u, 0u});
+                if constexpr (KT)
+                    kt[u] = __builtin_bit_cast(X4, ok ? *reinterpret_cast<const u32x2*>(kp + 2 * (DT + 4 * g)) : u32x2{0u, 0u});
+            }
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < KSTEPS; j += 2)
+                {
+                    u32x4 w = u32x4{0u, 0u, 0u, 0u};
+                    if (j + 1 < KSTEPS)
+                    {
+                        if (ok) w = *reinterpret_cast<const u32x4*>(kp + dimof(j, g));
+                        k[u][j + 1] = __builtin_bit_cast(X8, codes_to_m<CT, BF>(w[2], w[3]));
+                    }
+                    else if (ok)
+                    {
+                        const u32x2 t = *reinterpret_cast<const u32x2*>(kp + dimof(j, g));
+                        w = u32x4{t[0], t[1], 0u, 0u};
+                    }
+                    k[u][j] = __builtin_bit_cast(X8, codes_to_m<CT, BF>(w[0], w[1]));
+                }
+                if constexpr (KT)
+                {
+                    const u32x4 m = codes_to_m<CT, BF>(ok ? *reinterpret_cast<const uint32_t*>(kp + DT + 4 * g) : 0u, 0u);
+                    kt[u] = __builtin_bit_cast(X4, u32x2{m[0], m[1]});
+                }
+            }
+            if constexpr (CT == I8)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    ks[u][i] = ok ? a.k_scale[(static_cast<size_t>(phys) * kBlockSize + 4 * g + i) * a.num_kv_heads + kvh] : 0.0f;
+        }
+
+        float acc[KP * 4];  // SUM: this lane's columns' weights of key 4g + i of page u
+#pragma unroll
+        for (int e = 0; e < KP * 4; ++e) acc[e] = 0.0f;
+        for (int rb = rb0; rb < (SUM ? blocks : rb0 + 1); ++rb)
+        {
+            if (SUM && blocks > 1)
+            {
+                __syncthreads();  // the last block's rows are done with
+                tiles = stage(rb);
+            }
+            for (int tile = 0; tile < tiles; ++tile)
+            {
+                const int3 vis = s_vis[tile * 16 + c];
+                if (!__any(vis.x < vis.y && vis.x < key0 + KP * kBlockSize && vis.y > key0)) continue;
+                f32x4 s[KP];
+#pragma unroll
+                for (int u = 0; u < KP; ++u) s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+                    {
+                        const X8 q = __builtin_bit_cast(X8, s_q[((tile * NP + p) * KSTEPS + j) * 64 + lane]);
+#pragma unroll
+                        for (int u = 0; u < KP; ++u) s[u] = M::mma32(k[u][j], q, s[u]);
+                    }
+                if constexpr (KT)
+#pragma unroll
+                    for (int u = 0; u < KP; ++u)
+                    {
+                        // (accumulated apart and joined by vector adds, as in the decode: the 16x16x16 product chained on the
+                        // 16x16x32 ones' result got no wait states between them)
+                        f32x4 st = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int p = 0; p < NP; ++p)
+                            st = M::mma16(kt[u], __builtin_bit_cast(X4, s_qt[(tile * NP + p) * 64 + lane]), st);
+                        s[u] += st;
+                    }
+                if constexpr (CT == I8)
+#pragma unroll
+                    for (int u = 0; u < KP; ++u) s[u] *= ks[u];
+                float v[KP * 4];
+#pragma unroll
+                for (int e = 0; e < KP * 4; ++e) v[e] = s[e >> 2][e & 3] * c_log2;
+                if (a.rule.cap > 0.0f)
+                {
+#pragma unroll
+                    for (int e = 0; e < KP * 4; ++e) v[e] = cap_score(v[e], a.rule.cap, a.rule.inv_cap);
+                }
+                if (a.rule.slopes != nullptr)
+                {
+                    const float slope = -s_slope[tile * 16 + c];
+                    const float d0 = static_cast<float>(key0 + 4 * g - vis.z);
+#pragma unroll
+                    for (int e = 0; e < KP * 4; ++e)
+                        v[e] = __builtin_fmaf(slope, __builtin_fabsf(d0 + static_cast<float>(16 * (e >> 2) + (e & 3))), v[e]);
+                }
+                const bool masked = okm != (1 << KP) - 1 || !__all(vis.x <= key0 && vis.y >= key0 + KP * kBlockSize);
+                if (masked)
+                {
+#pragma unroll
+                    for (int e = 0; e < KP * 4; ++e)
+                    {
+                        const int  key = key0 + 4 * g + 16 * (e >> 2) + (e & 3);
+                        const bool seen = (okm >> (e >> 2) & 1) && key >= vis.x && key < vis.y;
+                        v[e] = seen ? v[e] : kNegInf;
+                    }
+                }
+                if constexpr (SUM)
+                {
+                    const float2 f = s_ml[0][tile * 16 + c];
+#pragma unroll
+                    for (int e = 0; e < KP * 4; ++e) v[e] = __builtin_amdgcn_exp2f(v[e] - f.x) * f.y;
+                    // A NaN query's state: NaN for the keys it sees alone.  (By its bits: from `f.y < infinity` in a vote the
+                    // compiler made an unordered compare, which a NaN passes.)
+                    if (masked && __any((f2u(f.y) & 0x7fffffffu) > 0x7f800000u))
+                    {
+#pragma unroll
+                        for (int e = 0; e < KP * 4; ++e)
+                        {
+                            const int  key = key0 + 4 * g + 16 * (e >> 2) + (e & 3);
+                            const bool seen = (okm >> (e >> 2) & 1) && key >= vis.x && key < vis.y;
+                            v[e] = seen ? v[e] : 0.0f;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < KP * 4; ++e) acc[e] += v[e];
+                }
+                else
+                {
+                    float m = kLowest, l = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < KP * 4; ++e) m = __builtin_elementwise_maximum(m, v[e]);
+                    m = swap_max(m);
+#pragma unroll
+                    for (int e = 0; e < KP * 4; ++e) l += __builtin_amdgcn_exp2f(v[e] - m);
+                    l = swap_sum(l);
+                    if (g == 0)
+                    {
+                        float2& st = s_ml[wave][tile * 16 + c];
+                        st = aw_join(st, make_float2(m, l));
+                    }
+                }
+            }
+        }
+        if constexpr (SUM)
+        {
+            // lane c of each 16 takes key 16 (c / 4) + 4g + c % 4 of the wave's
+            float w = 0.0f;
+#pragma unroll
+            for (int e = 0; e < KP * 4; ++e)
+            {
+                const float t = group_sum<16>(acc[e]);
+                w = c == e ? t : w;
+            }
+            if (c < KP * 4) aw_store(a, bh, ctx, total, key0 + 16 * (c >> 2) + 4 * g + (c & 3), w);
+        }
+    }
+    if constexpr (!SUM)
+    {
+        __syncthreads();
+        for (int i = tid; i < RB; i += kAwThreads)
+        {
+            const int r = rb0 * RB + i;
+            if (r >= R) break;
+            float2 st = s_ml[0][i];
+#pragma unroll
+            for (int w = 1; w < kAwWaves; ++w) st = aw_join(st, s_ml[w][i]);
+            a.part[(static_cast<int64_t>(bh) * a.splits + split) * R + r] = st;
+        }
+    }
+}
+
+// The same with vector arithmetic (fp32 caches, and head dims that the matrix cores do not take): a thread has a key, 32
+// query rows at a time pass by in LDS.
+template <int CT, bool SUM>
+__global__ __launch_bounds__(kAwThreads) void attention_weights_vector(WeightArgs a)
+{
+    constexpr int T = kAwVecTile;
+    __shared__ float  s_q[T][256];
+    __shared__ int3   s_vis[T];
+    __shared__ float  s_slope[T];
+    __shared__ float2 s_ml[SUM ? 1 : kAwWaves][SUM ? T : kAwVecRows];
+    const int D = a.head_dim;
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = tid & 63;
+    const int wave = tid >> 6;
+    const int split = static_cast<int>(blockIdx.x) % a.splits;
+    const int bh = static_cast<int>(blockIdx.x) / a.splits;
+    const int b = bh / a.num_kv_heads;
+    const int kvh = bh - b * a.num_kv_heads;
+    const int G = a.group;
+    const int R = a.seq_len * G;
+    const int64_t ctx = a.context_lens[b];
+    const int total = aw_total(a, ctx);
+    const int chunks = (total + kAwVecChunk - 1) / kAwVecChunk;
+    const int r_lo = SUM ? 0 : static_cast<int>(blockIdx.y) * kAwVecRows;
+    const int r_hi = SUM ? R : min(R, r_lo + kAwVecRows);
+    if constexpr (!SUM)
+        for (int i = lane; i < kAwVecRows; i += 64) s_ml[wave][i] = make_float2(kLowest, 0.0f);
+    for (int ch = split; ch < chunks; ch += a.splits)
+    {
+        const int key = ch * kAwVecChunk + tid;
+        int       phys = -1;
+        if (key < total) phys = a.block_table[static_cast<int64_t>(b) * a.max_blocks + (key >> 4)];
+        const bool   ok = phys >= 0 && phys < a.num_blocks;
+        const size_t row = (static_cast<size_t>(ok ? phys : 0) * kBlockSize + (key & 15)) * a.num_kv_heads + kvh;
+        float        sk = a.scale_log2;
+        if constexpr (CT == I8) sk *= ok ? a.k_scale[row] : 0.0f;
+        if constexpr (CT == FP8) sk *= a.k_scale[kvh];
+        float w = 0.0f;
+        for (int r0 = r_lo; r0 < r_hi; r0 += T)
+        {
+            const int m = min(T, r_hi - r0);
+            __syncthreads();  // the last rows are done with
+            for (int i = tid; i < T * (D / 4); i += kAwThreads)
+            {
+                const int rr = i / (D / 4), d = 4 * (i - rr * (D / 4));
+                float     x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (rr < m)
+                {
+                    const int t = (r0 + rr) / G, h = r0 + rr - t * G;
+                    load_act4(a.q, a.qo_dtype,
+                              ((static_cast<size_t>(b) * a.seq_len + t) * a.num_heads + kvh * G + h) * D + d, x);
+                }
+                *reinterpret_cast<float4*>(&s_q[rr][d]) = make_float4(x[0], x[1], x[2], x[3]);
+            }
+            if (tid < T)
+            {
+                const int r = r0 + tid;
+                s_vis[tid] = tid < m ? aw_visible(a, b, ctx, total, r / G) : make_int3(0, 0, 0);
+                s_slope[tid] = tid < m && a.rule.slopes != nullptr ? a.rule.slopes[kvh * G + r % G] * 1.4426950408889634f : 0.0f;
+                if constexpr (SUM) s_ml[0][tid] = tid < m ? a.fin[static_cast<int64_t>(bh) * R + r] : make_float2(0.0f, 0.0f);
+            }
+            __syncthreads();
+            float s[T];
+#pragma unroll
+            for (int rr = 0; rr < T; ++rr) s[rr] = 0.0f;
+            for (int d = 0; d < D; d += 8)
+            {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+                if (ok)
+                {
+                    Raw8 raw;
+                    load_raw8<CT>(a.k_cache, row * D + d, raw);
+                    unpack8<CT>(raw, x);
+                }
+#pragma unroll
+                for (int rr = 0; rr < T; ++rr)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[rr] = __builtin_fmaf(s_q[rr][d + e], x[e], s[rr]);
+            }
+#pragma unroll
+            for (int rr = 0; rr < T; ++rr)
+            {
+                const int3 vis = s_vis[rr];
+                float      v = s[rr] * sk;
+                if (a.rule.cap > 0.0f) v = cap_score(v, a.rule.cap, a.rule.inv_cap);
+                if (a.rule.slopes != nullptr)
+                    v = __builtin_fmaf(-s_slope[rr], __builtin_fabsf(static_cast<float>(key - vis.z)), v);
+                v = ok && key >= vis.x && key < vis.y ? v : kNegInf;
+                if constexpr (SUM)
+                {
+                    const float2 f = s_ml[0][rr];
+                    w += v == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(v - f.x) * f.y;
+                }
+                else if (rr < m)  // uniform
+                {
+                    float mx = group_max<32>(__builtin_elementwise_maximum(v, kLowest));
+                    mx = __builtin_elementwise_maximum(mx, __shfl_xor(mx, 32, 64));
+                    float l = group_sum<32>(__builtin_amdgcn_exp2f(v - mx));
+                    l += __shfl_xor(l, 32, 64);
+                    if (lane == 0)
+                    {
+                        float2& st = s_ml[wave][r0 - r_lo + rr];
+                        st = aw_join(st, make_float2(mx, l));
+                    }
+                }
+            }
+        }
+        if constexpr (SUM) aw_store(a, bh, ctx, total, key, w);
+    }
+    if constexpr (!SUM)
+    {
+        __syncthreads();
+        for (int r = r_lo + tid; r < r_hi; r += kAwThreads)
+        {
+            float2 st = s_ml[0][r - r_lo];
+#pragma unroll
+            for (int v = 1; v < kAwWaves; ++v) st = aw_join(st, s_ml[v][r - r_lo]);
+            a.part[(static_cast<int64_t>(bh) * a.splits + split) * R + r] = st;
+        }
+    }
+}
+
+// The rows' states over all splits as (max, 1 / denominator): 16 rows a workgroup, 16 threads over the splits of each.
+__global__ __launch_bounds__(256) void attention_weights_fold(WeightArgs a)
+{
+    __shared__ float2 s_st[16][17];
+    const int     R = a.seq_len * a.group;
+    const int     i = static_cast<int>(threadIdx.x) & 15;
+    const int     sl = static_cast<int>(threadIdx.x) >> 4;
+    const int     blocks = (R + 15) / 16;
+    const int64_t bh = static_cast<int64_t>(blockIdx.x) / blocks;
+    const int     r = static_cast<int>(blockIdx.x % blocks) * 16 + i;
+    float2        st = make_float2(kLowest, 0.0f);
+    if (r < R)
+        for (int s = sl; s < a.splits; s += 16) st = aw_join(st, a.part[(bh * a.splits + s) * R + r]);
+    s_st[sl][i] = st;
+    __syncthreads();
+    if (sl != 0 || r >= R) return;
+    for (int k = 1; k < 16; ++k) st = aw_join(st, s_st[k][i]);
+    a.fin[bh * R + r] = make_float2(st.x, softmax_inv(st.y));
+}
+
+namespace
+{
+
+// f.operator()<CT, QT, D>() for the call's types and head_dim.
+template <typename F>
+auto weights_for(const WeightArgs& a, F f)
+{
+    auto d = [&]<int CT, int QT>()
+    {
+        switch (a.head_dim)
+        {
+            case 64:
+                return f.template operator()<CT, QT, 64>();
+            case 80:
+                return f.template operator()<CT, QT, 80>();
+            case 96:
+                return f.template operator()<CT, QT, 96>();
+            case 112:
+                return f.template operator()<CT, QT, 112>();
+            case 128:
+                return f.template operator()<CT, QT, 128>();
+            default:
+                return f.template operator()<CT, QT, 256>();
+        }
+    };
+    auto q = [&]<int CT>()
+    {
+        if (a.qo_dtype == F32) return d.template operator()<CT, F32>();
+        if (a.qo_dtype == F16) return d.template operator()<CT, F16>();
+        return d.template operator()<CT, BF16>();
+    };
+    if (a.cache_dtype == BF16) return q.template operator()<BF16>();
+    if (a.cache_dtype == F16) return q.template operator()<F16>();
+    if (a.cache_dtype == I8) return q.template operator()<I8>();
+    return q.template operator()<FP8>();
+}
+
+template <int CT>
+hipError_t launch_vector(const WeightArgs& a, bool sum, dim3 grid, hipStream_t stream)
+{
+    if (sum)
+        hipLaunchKernelGGL((attention_weights_vector<CT, true>), grid, dim3(kAwThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL((attention_weights_vector<CT, false>), grid, dim3(kAwThreads), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+// Splits of a row's keys: one chunk of keys a workgroup, fewer where the rows and heads alone fill the chip several times.
+int attention_weights_splits(int batch, int num_kv_heads, int head_dim, int cap_tokens)
+{
+    const int64_t chunk = head_dim == 256 ? kAwChunk<256> : kAwChunk<128>;
+    const int64_t chunks = (static_cast<int64_t>(cap_tokens) + chunk - 1) / chunk;
+    const int64_t most = 8192 / (static_cast<int64_t>(batch) * num_kv_heads);
+    const int64_t n = chunks < most ? chunks : most;
+    return static_cast<int>(n < 1 ? 1 : n);
+}
+
+hipError_t launch_attention_weights(const WeightArgs& a, bool mfma, hipStream_t stream)
+{
+    const int64_t R = static_cast<int64_t>(a.seq_len) * a.group;
+    const int64_t bh = static_cast<int64_t>(a.batch) * a.num_kv_heads;
+    if (bh * a.splits > INT32_MAX || bh * ((R + 15) / 16) > INT32_MAX) return hipErrorInvalidConfiguration;
+    auto pass = [&](bool sum) -> hipError_t
+    {
+        auto grid = [&](int rows)
+        { return dim3(static_cast<unsigned>(bh * a.splits), sum ? 1u : static_cast<unsigned>((R + rows - 1) / rows)); };
+        if (mfma)
+            return weights_for(a, [&]<int CT, int QT, int D>()
+            {
+                constexpr bool LO = !((QT == BF16 && kBF<CT, QT>) || (QT == F16 && !kBF<CT, QT>));
+                const dim3     n = grid(kAwRows<D, LO>);
+                if (n.y > 65535u) return hipErrorInvalidConfiguration;
+                if (sum)
+                    hipLaunchKernelGGL((attention_weights_mfma<CT, QT, D, true>), n, dim3(kAwThreads), 0, stream, a);
+                else
+                    hipLaunchKernelGGL((attention_weights_mfma<CT, QT, D, false>), n, dim3(kAwThreads), 0, stream, a);
+                return hipGetLastError();
+            });
+        const dim3 n = grid(kAwVecRows);
+        if (n.y > 65535u) return hipErrorInvalidConfiguration;
+        if (a.cache_dtype == F32) return launch_vector<F32>(a, sum, n, stream);
+        if (a.cache_dtype == F16) return launch_vector<F16>(a, sum, n, stream);
+        if (a.cache_dtype == BF16) return launch_vector<BF16>(a, sum, n, stream);
+        if (a.cache_dtype == I8) return launch_vector<I8>(a, sum, n, stream);
+        return launch_vector<FP8>(a, sum, n, stream);
+    };
+    hipError_t e = pass(false);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(attention_weights_fold, dim3(static_cast<unsigned>(bh * ((R + 15) / 16))), dim3(256), 0, stream, a);
+    e = hipGetLastError();
+    return e != hipSuccess ? e : pass(true);
+}
+
+}  // namespace ffkv

@@ -95,6 +95,23 @@ int prefill_span(int cap_tokens, int group, int window, bool key_end)
     return static_cast<int>(std::min<int64_t>(cap_tokens, static_cast<int64_t>(window) + 128 / group + 2 * FFKV_BLOCK_SIZE));
 }
 
+// The attention weights' workspace: the query rows' states per split of the keys, and folded.
+struct WeightLayout
+{
+    int     splits;
+    int64_t part, fin, total;
+};
+
+WeightLayout weight_layout(int batch, int seq_len, int num_heads, int num_kv_heads, int head_dim, int cap_tokens)
+{
+    const int64_t rows = static_cast<int64_t>(batch) * seq_len * num_heads;
+    WeightLayout  l{};
+    l.splits = ffkv::attention_weights_splits(batch, num_kv_heads, head_dim, cap_tokens);
+    l.fin = align256(rows * l.splits * 8);
+    l.total = l.fin + align256(rows * 8);
+    return l;
+}
+
 }  // namespace
 
 extern "C" {
@@ -368,6 +385,97 @@ int ffkv_paged_prefill_scored(const void* q, void* out, int qo_dtype, const void
     }
     const hipError_t e = ffkv::launch_prefill_scored(a, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "scored prefill launch");
+    return ok();
+}
+
+size_t ffkv_attention_weights_workspace_bytes(int batch, int seq_len, int num_heads, int num_kv_heads, int head_dim,
+                                              int max_blocks, int max_context_len)
+{
+    if (batch <= 0 || seq_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || head_dim <= 0)
+        return 0;
+    const int cap = ffkv::decode_cap_tokens(max_blocks, max_context_len);
+    const WeightLayout l = weight_layout(batch, seq_len, num_heads, num_kv_heads, head_dim, cap);
+    return static_cast<size_t>(l.total);
+}
+
+int ffkv_attention_weights(const void* q, int qo_dtype, const void* k_cache, int cache_dtype, const float* k_scale,
+                           const int32_t* block_table, const int32_t* context_lens, int batch, int seq_len, int num_heads,
+                           int num_kv_heads, int head_dim, int block_size, int max_blocks, int num_blocks,
+                           int max_context_len, float scale, float score_cap, const float* slopes, int window,
+                           const int32_t* key_begin, const int32_t* key_end, float* weights, const float* prior,
+                           float decay, int64_t weight_stride, void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (block_size != FFKV_BLOCK_SIZE) return fail(FFKV_ERR_UNSUPPORTED, "block_size must be 16, got %d", block_size);
+    if (!is_act(qo_dtype)) return fail(FFKV_ERR_UNSUPPORTED, "unsupported q dtype %d", qo_dtype);
+    if (!is_cache(cache_dtype)) return fail(FFKV_ERR_UNSUPPORTED, "unsupported cache dtype %d", cache_dtype);
+    if (!head_dim_ok(head_dim))
+        return fail(FFKV_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 up to 128, or 256, got %d", head_dim);
+    if (batch < 0 || seq_len < 0 || num_heads <= 0 || num_kv_heads <= 0 || max_blocks < 0 || num_blocks < 0)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "bad size (batch %d seq_len %d heads %d kv_heads %d max_blocks %d "
+                    "num_blocks %d)", batch, seq_len, num_heads, num_kv_heads, max_blocks, num_blocks);
+    if (num_heads % num_kv_heads != 0)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "num_heads %d is not a multiple of num_kv_heads %d", num_heads,
+                    num_kv_heads);
+    if (batch > 65535 || num_heads > 65535) return fail(FFKV_ERR_UNSUPPORTED, "batch and num_heads must be <= 65535");
+    const int group = num_heads / num_kv_heads;
+    if (static_cast<int64_t>(seq_len) * group > (1 << 20))  // 65536 blocks of 16 query rows
+        return fail(FFKV_ERR_UNSUPPORTED, "seq_len * group must be <= 2^20");
+    if (const int rc = check_rule(score_cap, slopes, window, key_begin, key_end)) return rc;
+    const int cap = ffkv::decode_cap_tokens(max_blocks, max_context_len);
+    if (batch == 0 || seq_len == 0) return ok();
+    if (!q || !k_cache || !block_table || !context_lens || !weights)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "null q, cache, block_table, context_lens or weights pointer");
+    if (const int rc = check_weights(weights, prior, decay, weight_stride, cap)) return rc;
+    if (quantized(cache_dtype) && !k_scale) return fail(FFKV_ERR_INVALID_ARGUMENT, "quantized cache needs k_scale");
+    if (!aligned16(q) || !aligned16(k_cache) || !aligned16(workspace))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "q, cache and workspace pointers must be 16-byte aligned");
+    if (static_cast<int64_t>(batch) * num_kv_heads * ceil_div(static_cast<int64_t>(seq_len) * group, 16) > INT32_MAX)
+        return fail(FFKV_ERR_UNSUPPORTED, "batch * seq_len * num_heads too large");
+
+    const WeightLayout lay = weight_layout(batch, seq_len, num_heads, num_kv_heads, head_dim, cap);
+    hipStream_t        s = static_cast<hipStream_t>(stream);
+    void*              ws = workspace;
+    if (ws != nullptr && workspace_bytes < static_cast<size_t>(lay.total))
+        return fail(FFKV_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %lld bytes needed", workspace_bytes,
+                    static_cast<long long>(lay.total));
+    if (ws == nullptr)
+    {
+        const hipError_t e = hipMallocAsync(&ws, static_cast<size_t>(lay.total), s);
+        if (e != hipSuccess) return hip_fail(e, "attention weights workspace hipMallocAsync");
+    }
+    ffkv::WeightArgs a{};
+    a.q = q;
+    a.k_cache = k_cache;
+    a.k_scale = k_scale;
+    a.block_table = block_table;
+    a.context_lens = context_lens;
+    a.qo_dtype = qo_dtype;
+    a.cache_dtype = cache_dtype;
+    a.batch = batch;
+    a.seq_len = seq_len;
+    a.num_heads = num_heads;
+    a.num_kv_heads = num_kv_heads;
+    a.group = group;
+    a.head_dim = head_dim;
+    a.max_blocks = max_blocks;
+    a.num_blocks = num_blocks;
+    a.cap_tokens = cap;
+    a.scale_log2 = softmax_scale(scale, head_dim) * kLog2e;
+    a.rule = make_rule(score_cap, slopes, window, key_begin, key_end);
+    a.splits = lay.splits;
+    a.part = reinterpret_cast<float2*>(static_cast<char*>(ws) + lay.part);
+    a.fin = reinterpret_cast<float2*>(static_cast<char*>(ws) + lay.fin);
+    a.weights = weights;
+    a.prior = prior;
+    a.decay = decay;
+    a.weight_stride = weight_stride;
+    hipError_t e = ffkv::launch_attention_weights(a, scored_mfma(cache_dtype, head_dim), s);
+    if (workspace == nullptr)
+    {
+        const hipError_t fe = hipFreeAsync(ws, s);
+        if (e == hipSuccess) e = fe;
+    }
+    if (e != hipSuccess) return hip_fail(e, "attention weights launch");
     return ok();
 }
 

@@ -168,6 +168,38 @@ struct DecodeArgs
     int64_t        weight_stride;
 };
 
+struct WeightArgs
+{
+    const void*    q;  // [batch, seq_len, num_heads, head_dim]
+    const void*    k_cache;
+    const float*   k_scale;
+    const int32_t* block_table;
+    const int32_t* context_lens;  // tokens cached before the seq_len ones
+    int            qo_dtype;
+    int            cache_dtype;
+    int            batch;
+    int            seq_len;
+    int            num_heads;
+    int            num_kv_heads;
+    int            group;
+    int            head_dim;
+    int            max_blocks;
+    int            num_blocks;
+    int            cap_tokens;
+    float          scale_log2;
+    ScoreRule      rule;
+    int            splits;  // of a row's keys (attention_weights_splits)
+    float2*        part;    // [batch * num_kv_heads, splits, seq_len * group]: (max, denominator) of each query row
+    float2*        fin;     // [batch * num_kv_heads, seq_len * group]: (max, 1 / denominator)
+    float*         weights;
+    const float*   prior;
+    float          decay;
+    int64_t        weight_stride;
+};
+
+int        attention_weights_splits(int batch, int num_kv_heads, int head_dim, int cap_tokens);
+hipError_t launch_attention_weights(const WeightArgs& a, bool mfma, hipStream_t stream);
+
 struct EvictArgs
 {
     const float*   weights;  // [batch, num_kv_heads, weight_stride]

@@ -72,7 +72,9 @@ __global__ __launch_bounds__(256) void paged_decode_weights(DecodeArgs a)
             for (int h = 0; h < G; ++h)
             {
                 const float2 f = fin[h];
-                w += __builtin_amdgcn_exp2f(sc[h * a.score_stride + j] - f.x) * softmax_inv(f.y);
+                const float  v = sc[h * a.score_stride + j];
+                // (a key on no page weighs nothing, in a NaN query's row too)
+                w += v == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(v - f.x) * softmax_inv(f.y);
             }
         if (a.prior != nullptr && j < s.pos) w = __builtin_fmaf(a.decay, a.prior[at + j], w);
         a.weights[at + j] = w;

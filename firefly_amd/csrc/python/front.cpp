@@ -36,6 +36,7 @@ struct Functions
     decltype(&ffkv_prefill_scored_workspace_bytes) prefill_scored_bytes;
     decltype(&ffkv_paged_prefill_scored)       prefill_scored;
     decltype(&ffkv_evict)                      evict;
+    decltype(&ffkv_attention_weights)          attention_weights;
 };
 Functions fn{};
 
@@ -570,6 +571,47 @@ PyObject* prefill_scored(PyObject*, PyObject* const* a, Py_ssize_t n)
     return rc;
 }
 
+// q, k_cache, k_scale, block_table, context_lens, max_context_len, scale, num_blocks, score_cap, slopes, window, key_begin,
+// key_end, weights, prior, decay, workspace, stream
+PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!count(n, 18)) return nullptr;
+    Reader    r{a};
+    PyObject* q = a[0];
+    int       B, S, Hq, D;
+    r.dims4(q, B, S, Hq, D);
+    const int Hkv = r.dim(a[1], 2), qt = r.dtype(q), ct = r.dtype(a[1]);
+    r.plain(q, "q", q);
+    r.holds(a[1], "k_cache", ct, {-1, FFKV_BLOCK_SIZE, Hkv, D}, q, false);
+    check_scales(r, a[2], "k_scale", ct, a[1], Hkv, q);
+    r.holds(a[3], "block_table", kInt32, {B, -1}, q, false);
+    r.holds(a[4], "context_lens", kInt32, {B}, q, false);
+    const int   mb = r.dim(a[3], 1), mcl = r.integer(a[5]);
+    const float scale = r.real(a[6]);
+    const int   N = r.blocks(a[7], a[1]);
+    check_blocks(r, N, a[1]);
+    Rule u;
+    u.cap = r.real(a[8]);
+    r.holds(a[9], "slopes", FFKV_DTYPE_F32, {Hq}, q, true);
+    u.window = r.integer(a[10]);
+    r.holds(a[11], "key_begin", kInt32, {B, S}, q, true);
+    r.holds(a[12], "key_end", kInt32, {B, S}, q, true);
+    Weights w(r, a + 13, B, Hkv, q);
+    r.plain(a[16], "workspace", q);
+    r.current(q, B > 0 && S > 0);
+    void *qp = r.ptr(q), *kc = r.ptr(a[1]);
+    auto* ks = r.ptr<float>(a[2]);
+    auto *bt = r.ptr<int32_t>(a[3]), *cx = r.ptr<int32_t>(a[4]);
+    u.slopes = r.ptr<float>(a[9]), u.begin = r.ptr<int32_t>(a[11]), u.end = r.ptr<int32_t>(a[12]);
+    void*        ws = r.ptr(a[16]);
+    const size_t wb = r.nbytes(a[16]);
+    void*        s = r.stream(a[17]);
+    return finish(r, [&] {
+        return fn.attention_weights(qp, qt, kc, ct, ks, bt, cx, B, S, Hq, Hkv, D, FFKV_BLOCK_SIZE, mb, N, mcl, scale, u.cap,
+                                    u.slopes, u.window, u.begin, u.end, w.w, w.prior, w.decay, w.stride, ws, wb, s);
+    });
+}
+
 // weights, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, keep, sinks, recent, dst_table, kept,
 // kept_lens, weights_out, num_blocks, stream
 PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n)
@@ -679,7 +721,7 @@ PyObject* forget_stream(PyObject*, PyObject*)
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(decode_scored),  FAST(prefill_scored), FAST(evict),
+PyMethodDef methods[] = {FAST(decode_scored),  FAST(prefill_scored), FAST(evict), FAST(attention_weights),
                          FAST(append),         FAST(decode),  FAST(decode_shared), FAST(append_decode),
                          FAST(decode_noalloc), FAST(prefill), FAST(rope),          FAST(rope_append),
                          {"bind", bind, METH_VARARGS, nullptr},

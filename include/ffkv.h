@@ -335,6 +335,29 @@ FFKV_API int ffkv_paged_prefill_scored(const void* q, void* out, int qo_dtype, c
                                        void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * The attention weights that the last seq_len tokens of every row give to its cached keys, summed over them and over the
+ * query heads of a KV head, under a score rule (see ffkv_paged_prefill_scored, whose q, context_lens, key_begin and key_end
+ * these are; the keys must be appended):
+ *   weights[b, kvh, j] = decay * prior[b, kvh, j] + sum of softmax(s)_j    j < context_lens[b]
+ *   weights[b, kvh, j] = sum of softmax(s)_j                               the seq_len tokens' own keys
+ * weights and prior as for ffkv_paged_decode_scored, which gives the same for single tokens beside the attention itself;
+ * this call reads no V and writes no output: the prompt's part of what ffkv_evict goes by (the last 16 to 64 tokens of a
+ * prompt, a few queries of a chunk).  Caches, head dims and GQA groups as for ffkv_paged_decode_scored, any group size.
+ * Workspace: ffkv_attention_weights_workspace_bytes, or NULL for stream-ordered memory; calls that share one must not
+ * overlap in time.  No counterpart in the reference.
+ */
+FFKV_API size_t ffkv_attention_weights_workspace_bytes(int batch, int seq_len, int num_heads, int num_kv_heads,
+                                                       int head_dim, int max_blocks, int max_context_len);
+
+FFKV_API int ffkv_attention_weights(const void* q, int qo_dtype, const void* k_cache, int cache_dtype, const float* k_scale,
+                                    const int32_t* block_table, const int32_t* context_lens, int batch, int seq_len,
+                                    int num_heads, int num_kv_heads, int head_dim, int block_size, int max_blocks,
+                                    int num_blocks, int max_context_len, float scale, float score_cap,
+                                    const float* slopes, int window, const int32_t* key_begin, const int32_t* key_end,
+                                    float* weights, const float* prior, float decay, int64_t weight_stride,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Eviction from the cache by attention weight.  Row b holds context_lens[b] tokens (all appended; clamped to what its
  * block table and weight_stride hold), whose weights per KV head are weights fp32 [batch, num_kv_heads, weight_stride], as
  * ffkv_paged_decode_scored and ffkv_attention_weights leave them.  A row of more than `keep` tokens keeps, per KV head, its

@@ -204,3 +204,47 @@ def test_evict_front(ff):
     with pytest.raises(ValueError, match="GPU"):
         ff.evict_tokens(torch.zeros(1, HKV, 9), pool, pool, torch.zeros(1, 3, dtype=torch.int32),
                         torch.zeros(1, dtype=torch.int32), 4, stream=0)
+
+
+def _weights(ff, **kw):
+    a = dict(q=16, qo_dtype=ff.DTYPE_BF16, k_cache=16, cache_dtype=ff.DTYPE_BF16, k_scale=None, block_table=16,
+             context_lens=16, batch=1, seq_len=4, num_heads=32, num_kv_heads=8, head_dim=128, block_size=16, max_blocks=4,
+             num_blocks=4, max_context_len=0, scale=0.0, score_cap=0.0, slopes=None, window=0, key_begin=None, key_end=None,
+             weights=16, prior=None, decay=1.0, weight_stride=64, workspace=None, workspace_bytes=0, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return ff.lib.ffkv_attention_weights(*a.values())
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(block_size=8), -2), (dict(head_dim=84), -2), (dict(qo_dtype=3), -2), (dict(cache_dtype=7), -2),
+    (dict(num_heads=30), -1), (dict(batch=-1), -1), (dict(batch=70000), -2), (dict(seq_len=1 << 19), -2), (dict(q=None), -1),
+    (dict(weights=None), -1), (dict(cache_dtype=3), -1), (dict(cache_dtype=8), -1), (dict(q=20), -1), (dict(weights=18), -1),
+    (dict(weight_stride=63), -1), (dict(decay=-1.0), -1), (dict(decay=INF), -1), (dict(score_cap=-1.0), -1),
+    (dict(window=-1), -1), (dict(key_end=5), -1), (dict(workspace=8), -1), (dict(workspace=256, workspace_bytes=16), -3),
+    (dict(batch=65535, seq_len=40000, num_heads=65528, num_kv_heads=65528), -2),
+])
+def test_weights_rejects(ff, kw, code):
+    assert _weights(ff, **kw) == code
+    assert ff.lib.ffkv_last_error().decode() != ""
+    assert _weights(ff, batch=0, q=None) == 0 and _weights(ff, seq_len=0, q=None) == 0
+
+
+def test_weights_front(ff):
+    t = _tensors()
+    t.pop("v_cache")
+    r = torch.zeros(0, 1, dtype=torch.int32)
+    assert ff.attention_weights(**t, key_begin=r, key_end=r, stream=0).shape == (0, HKV, 48)
+    assert ff.attention_weights(**t, max_context_len=20, stream=0).shape == (0, HKV, 20)
+    w = torch.zeros(0, HKV, 48)
+    bad = [
+        (ValueError, dict(t, q=t["q"][:, 0])), (ValueError, dict(t, key_begin=torch.zeros(0, 2, dtype=torch.int32))),
+        (TypeError, dict(t, key_end=r.float())), (ValueError, dict(t, weights=w[..., 0])), (TypeError, dict(t, weights=w.half())),
+        (ValueError, dict(t, weights=w, prior=torch.zeros(0, HKV, 40))), (ValueError, dict(t, slopes=torch.zeros(1))),
+        (TypeError, dict(t, block_table=t["block_table"].long())), (ValueError, dict(t, num_blocks=5)),
+        (ValueError, dict(t, context_lens=torch.zeros(1, dtype=torch.int32))), (ff.FFKVError, dict(t, window=-1)),
+        (ValueError, dict(t, k_cache=torch.zeros(4, 16, HKV, 2 * D, dtype=torch.bfloat16)[..., ::2])),
+    ]
+    for error, kw in bad:
+        with pytest.raises(error):
+            ff.attention_weights(**kw, stream=0)
