@@ -110,7 +110,9 @@ def _load() -> ctypes.CDLL:
                                            *rule, vp, vp, vp, vp, f32, ctypes.c_int64, vp, sz, vp]
     lib.ffkv_evict.restype = i32
     lib.ffkv_evict.argtypes = [vp, ctypes.c_int64, vp, i32, i32, i32, vp, vp, i32, vp, vp, vp, i32, vp, i32, vp, vp, vp,
-                               ctypes.c_int64, i32, i32, i32, i32, i32, vp]
+                               ctypes.c_int64, i32, i32, i32, i32, i32, vp, sz, vp]
+    lib.ffkv_evict_workspace_bytes.restype = sz
+    lib.ffkv_evict_workspace_bytes.argtypes = [i32, i32, i32, ctypes.c_int64, i32]
     lib.ffkv_last_error.restype = ctypes.c_char_p
     lib.ffkv_last_error.argtypes = []
     lib.ffkv_version.restype = ctypes.c_char_p
@@ -388,9 +390,17 @@ def attention_weights(q, k_cache, block_table, context_lens, weights=None, prior
     return weights
 
 
+def evict_workspace(batch: int, num_kv_heads: int, keep: int, weight_stride: int, max_blocks: int, device=None):
+    """A workspace for ``evict_tokens`` (``ffkv_evict_workspace_bytes``)."""
+    import torch
+
+    n = int(lib.ffkv_evict_workspace_bytes(batch, num_kv_heads, keep, weight_stride, max_blocks))
+    return torch.empty(max(n, 256), dtype=torch.uint8, device=device if device is not None else "cuda")
+
+
 def evict_tokens(weights, k_cache, v_cache, block_table, context_lens, keep: int, sinks: int = 0, recent: int = 0,
                  dst_table=None, weights_out=None, kept=None, kept_lens=None, k_scale=None, v_scale=None,
-                 num_blocks: int | None = None, stream=None):
+                 workspace=None, num_blocks: int | None = None, stream=None):
     """Cut the rows of the cache to their ``keep`` tokens of most attention weight (``ffkv_evict``): ``weights`` fp32
     ``[B, Hkv, T]``, ``context_lens`` the rows' tokens; the first ``sinks`` and last ``recent`` always stay.  The kept tokens
     move to the front of the row's pages in ``dst_table`` int32 ``[B, blocks]`` (None: of its own pages, which no other row
@@ -405,5 +415,5 @@ def evict_tokens(weights, k_cache, v_cache, block_table, context_lens, keep: int
         if kept_lens is None:
             kept_lens = torch.empty(weights.shape[0], **like)
     check(_front.evict(weights, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, keep, sinks, recent, dst_table,
-                       kept, kept_lens, weights_out, num_blocks, stream))
+                       kept, kept_lens, weights_out, num_blocks, workspace, stream))
     return kept, kept_lens

@@ -112,6 +112,28 @@ WeightLayout weight_layout(int batch, int seq_len, int num_heads, int num_kv_hea
     return l;
 }
 
+// The eviction's workspace for long rows (evict.hip); nothing for others.
+struct EvictLayout
+{
+    int     parts;
+    int64_t hist0, hist1, state, above, scratch, total;
+};
+
+EvictLayout evict_layout(int batch, int num_kv_heads, int keep, int64_t bound)
+{
+    EvictLayout l{};
+    l.parts = ffkv::evict_parts(batch, num_kv_heads, bound);
+    if (l.parts == 0) return l;
+    const int64_t bh = static_cast<int64_t>(batch) * num_kv_heads;
+    l.hist0 = 0;
+    l.hist1 = l.hist0 + bh * l.parts * 2048 * 4;
+    l.state = l.hist1 + bh * l.parts * 2048 * 4;
+    l.above = l.state + align256(bh * 2 * 2 * 4);
+    l.scratch = l.above + align256(bh * l.parts * 2 * 4);
+    l.total = l.scratch + align256(bh * std::min<int64_t>(keep, bound) * 4);
+    return l;
+}
+
 }  // namespace
 
 extern "C" {
@@ -479,11 +501,18 @@ int ffkv_attention_weights(const void* q, int qo_dtype, const void* k_cache, int
     return ok();
 }
 
+size_t ffkv_evict_workspace_bytes(int batch, int num_kv_heads, int keep, int64_t weight_stride, int max_blocks)
+{
+    if (batch <= 0 || num_kv_heads <= 0 || keep <= 0 || weight_stride <= 0 || max_blocks <= 0) return 0;
+    const int64_t bound = std::min<int64_t>(weight_stride, static_cast<int64_t>(max_blocks) * FFKV_BLOCK_SIZE);
+    return bound > INT32_MAX - 64 * 1024 ? 0 : static_cast<size_t>(evict_layout(batch, num_kv_heads, keep, bound).total);
+}
+
 int ffkv_evict(const float* weights, int64_t weight_stride, const int32_t* context_lens, int keep, int sinks, int recent,
                void* k_cache, void* v_cache, int cache_dtype, float* k_scale, float* v_scale, const int32_t* block_table,
                int max_blocks, const int32_t* dst_table, int dst_blocks, int32_t* kept, int32_t* kept_lens,
                float* weights_out, int64_t out_stride, int batch, int num_kv_heads, int head_dim, int block_size,
-               int num_blocks, void* stream)
+               int num_blocks, void* workspace, size_t workspace_bytes, void* stream)
 {
     if (block_size != FFKV_BLOCK_SIZE) return fail(FFKV_ERR_UNSUPPORTED, "block_size must be 16, got %d", block_size);
     if (!is_cache(cache_dtype)) return fail(FFKV_ERR_UNSUPPORTED, "unsupported cache dtype %d", cache_dtype);
@@ -512,8 +541,8 @@ int ffkv_evict(const float* weights, int64_t weight_stride, const int32_t* conte
         return fail(FFKV_ERR_INVALID_ARGUMENT, "kept_lens must not be context_lens");
     if (cache_dtype == FFKV_DTYPE_I8 && (!k_scale || !v_scale))
         return fail(FFKV_ERR_INVALID_ARGUMENT, "int8 cache needs k_scale and v_scale");
-    if (!aligned16(k_cache) || !aligned16(v_cache))
-        return fail(FFKV_ERR_INVALID_ARGUMENT, "cache pointers must be 16-byte aligned");
+    if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "cache and workspace pointers must be 16-byte aligned");
     if (!aligned4(weights) || !aligned4(weights_out) || !aligned4(kept) || !aligned4(kept_lens))
         return fail(FFKV_ERR_INVALID_ARGUMENT, "weights, kept and kept_lens must be 4-byte aligned");
 
@@ -541,7 +570,33 @@ int ffkv_evict(const float* weights, int64_t weight_stride, const int32_t* conte
     a.num_kv_heads = num_kv_heads;
     a.head_dim = head_dim;
     a.num_blocks = num_blocks;
-    const hipError_t e = ffkv::launch_evict(a, static_cast<hipStream_t>(stream));
+    const EvictLayout lay = evict_layout(batch, num_kv_heads, keep, bound);
+    hipStream_t       s = static_cast<hipStream_t>(stream);
+    void*             ws = workspace;
+    if (ws != nullptr && workspace_bytes < static_cast<size_t>(lay.total))
+        return fail(FFKV_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %lld bytes needed", workspace_bytes,
+                    static_cast<long long>(lay.total));
+    if (ws == nullptr && lay.total > 0)
+    {
+        const hipError_t e = hipMallocAsync(&ws, static_cast<size_t>(lay.total), s);
+        if (e != hipSuccess) return hip_fail(e, "evict workspace hipMallocAsync");
+    }
+    a.parts = lay.parts;
+    if (a.parts > 0)
+    {
+        char* w = static_cast<char*>(ws);
+        a.hist0 = reinterpret_cast<int*>(w + lay.hist0);
+        a.hist1 = reinterpret_cast<int*>(w + lay.hist1);
+        a.state = reinterpret_cast<uint32_t*>(w + lay.state);
+        a.above = reinterpret_cast<int*>(w + lay.above);
+        a.scratch = weights_out == weights ? reinterpret_cast<float*>(w + lay.scratch) : nullptr;
+    }
+    hipError_t e = ffkv::launch_evict(a, s);
+    if (workspace == nullptr && ws != nullptr)
+    {
+        const hipError_t fe = hipFreeAsync(ws, s);
+        if (e == hipSuccess) e = fe;
+    }
     if (e != hipSuccess) return hip_fail(e, "evict launch");
     return ok();
 }

@@ -223,8 +223,18 @@ struct EvictArgs
     int            num_kv_heads;
     int            head_dim;
     int            num_blocks;
+    // Long rows in parts (evict_parts > 0, evict.hip): histograms, what was found, and for weights in place a copy
+    // [batch, num_kv_heads, min(keep, bound)] (else null).
+    int            parts;
+    int*           hist0;
+    int*           hist1;
+    uint32_t*      state;
+    int*           above;
+    float*         scratch;
 };
 
+// Parts of each row's choice for rows of at most `bound` tokens; 0: a workgroup per row and head, without a workspace.
+int        evict_parts(int batch, int num_kv_heads, int64_t bound);
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
 hipError_t launch_append(const AppendArgs& a, hipStream_t stream);
 hipError_t launch_rope_append(const RopeArgs& a, hipStream_t stream);      // rotate q/k, then append when k_cache set

@@ -613,10 +613,10 @@ PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t n)
 }
 
 // weights, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, keep, sinks, recent, dst_table, kept,
-// kept_lens, weights_out, num_blocks, stream
+// kept_lens, weights_out, num_blocks, workspace, stream
 PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
-    if (!count(n, 16)) return nullptr;
+    if (!count(n, 17)) return nullptr;
     Reader    r{a};
     PyObject* w = a[0];
     const int B = r.dim(w, 0), Hkv = r.dim(a[1], 2), D = r.dim(a[1], 3), ct = r.dtype(a[1]);
@@ -645,10 +645,13 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n)
     auto *ks = r.ptr<float>(a[3]), *vs = r.ptr<float>(a[4]);
     auto *bt = r.ptr<int32_t>(a[5]), *cx = r.ptr<int32_t>(a[6]), *dt = r.ptr<int32_t>(a[10]), *kp = r.ptr<int32_t>(a[11]),
          *kl = r.ptr<int32_t>(a[12]);
-    void* s = r.stream(a[15]);
+    r.plain(a[15], "workspace", w);
+    void*        ws = r.ptr(a[15]);
+    const size_t wb = r.nbytes(a[15]);
+    void*        s = r.stream(a[16]);
     return finish(r, [&] {
         return fn.evict(wp, stride, cx, keep, sinks, recent, kc, vc, ct, ks, vs, bt, mb, dt, db, kp, kl, wo, ostride, B, Hkv,
-                        D, FFKV_BLOCK_SIZE, N, s);
+                        D, FFKV_BLOCK_SIZE, N, ws, wb, s);
     });
 }
 

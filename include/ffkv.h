@@ -374,14 +374,19 @@ FFKV_API int ffkv_attention_weights(const void* q, int qo_dtype, const void* k_c
  * Each KV head keeps tokens of its own: position j of a row then holds different tokens in different heads, each with the
  * rotary embedding it was cached with, and the row goes on from position kept_lens[b] (the new tokens' rotary positions
  * go on from the old ones).  A kept token whose source or destination page is absent is not copied.  keep >= 1, sinks
- * and recent >= 0 and together at most keep.  Cache types, head dims and alignment as for ffkv_append.  No workspace.  No
- * counterpart in the reference, which evicts whole prefix-cache nodes that no request uses (src/radix_tree.cc).
+ * and recent >= 0 and together at most keep.  Cache types, head dims and alignment as for ffkv_append.  Workspace:
+ * ffkv_evict_workspace_bytes (0 but for few rows over a long bound), or NULL for stream-ordered memory; calls that share
+ * one must not overlap in time.  No counterpart in the reference, which evicts whole prefix-cache nodes that no request
+ * uses (src/radix_tree.cc).
  */
+FFKV_API size_t ffkv_evict_workspace_bytes(int batch, int num_kv_heads, int keep, int64_t weight_stride, int max_blocks);
+
 FFKV_API int ffkv_evict(const float* weights, int64_t weight_stride, const int32_t* context_lens, int keep, int sinks,
                         int recent, void* k_cache, void* v_cache, int cache_dtype, float* k_scale, float* v_scale,
                         const int32_t* block_table, int max_blocks, const int32_t* dst_table, int dst_blocks,
                         int32_t* kept, int32_t* kept_lens, float* weights_out, int64_t out_stride, int batch,
-                        int num_kv_heads, int head_dim, int block_size, int num_blocks, void* stream);
+                        int num_kv_heads, int head_dim, int block_size, int num_blocks, void* workspace,
+                        size_t workspace_bytes, void* stream);
 
 /* Message describing the last error returned on the calling thread ("" if none). */
 FFKV_API const char* ffkv_last_error(void);

@@ -174,3 +174,28 @@ def test_no_rows_and_streams(ff, gpu):
         b, bl = ff.evict_tokens(c.w, c.k, c.v, c.table, c.ctx, 80, dst_table=c.dst)
         torch.cuda.synchronize()
         assert torch.equal(a, kept) and torch.equal(al, lens) and torch.equal(a, b) and torch.equal(al, bl)
+
+
+def test_long_rows_workspace_and_graph(ff, gpu):
+    """Rows long enough for their choice to be split over workgroups: a workspace of the caller's, weights in place where
+    more than the row is kept, and a captured call replayed between eager ones."""
+    c = Cache(8, [20000, 300, 9000], 4000, 2, 64, "bf16", gpu, kind="ties")
+    ws = ff.evict_workspace(3, 2, 4000, c.w.shape[2], c.table.shape[1], device=gpu)
+    assert ff.lib.ffkv_evict_workspace_bytes(3, 2, 4000, c.w.shape[2], c.table.shape[1]) > 0
+    a, al = run(ff, c, 4000, 5, 70, False, workspace=ws)
+    kept, lens, out = (torch.zeros(3, 2, 4000, dtype=torch.int32, device=gpu), torch.zeros(3, dtype=torch.int32, device=gpu),
+                       torch.zeros(3, 2, 4000, device=gpu))
+    args = (c.w, c.k, c.v, c.table, c.ctx, 4000, 5, 70, c.dst)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ff.evict_tokens(*args, weights_out=out, kept=kept, kept_lens=lens, workspace=ws)
+    for _ in range(3):
+        kept.fill_(-7)
+        g.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(kept.cpu().numpy(), a) and np.array_equal(lens.cpu().numpy(), al)
+        b, _ = ff.evict_tokens(*args, kept=torch.full_like(kept, -7), workspace=ws)
+        torch.cuda.synchronize()
+        assert torch.equal(b, kept)
+    c = Cache(9, [20000, 300, 9000], 30000, 2, 64, "bf16", gpu, kind="positive")
+    run(ff, c, 30000, 5, 70, True, "in place")

@@ -161,7 +161,7 @@ def _evict(ff, **kw):
     a = dict(weights=16, weight_stride=64, context_lens=16, keep=8, sinks=2, recent=3, k_cache=16, v_cache=16,
              cache_dtype=ff.DTYPE_BF16, k_scale=None, v_scale=None, block_table=16, max_blocks=4, dst_table=None, dst_blocks=0,
              kept=16, kept_lens=32, weights_out=None, out_stride=0, batch=1, num_kv_heads=2, head_dim=64, block_size=16,
-             num_blocks=4, stream=None)
+             num_blocks=4, workspace=None, workspace_bytes=0, stream=None)
     assert set(kw) <= set(a)
     a.update(kw)
     return ff.lib.ffkv_evict(*a.values())
@@ -174,6 +174,7 @@ def _evict(ff, **kw):
     (dict(weights_out=16, out_stride=65), -1), (dict(weights=None), -1), (dict(kept=None), -1), (dict(kept_lens=None), -1),
     (dict(kept_lens=16), -1), (dict(cache_dtype=3), -1), (dict(k_cache=24), -1), (dict(weights=18), -1), (dict(kept=18), -1),
     (dict(weight_stride=-1), -1), (dict(weight_stride=1 << 40, max_blocks=2 ** 31 - 1), -2), (dict(dst_blocks=-1), -1),
+    (dict(workspace=8), -1), (dict(workspace=256, workspace_bytes=100, weight_stride=1 << 20, max_blocks=9000), -3),
 ])
 def test_evict_rejects(ff, kw, code):
     assert _evict(ff, **kw) == code
