@@ -13,6 +13,8 @@
 #include "mfma_common.h"
 #include "score_rule.h"
 
+#include <algorithm>
+
 namespace ffkv
 {
 
@@ -33,6 +35,13 @@ constexpr int kAwRows = []
     const int r = 65536 / (D * 2 * (LO ? 2 : 1)) / 16 * 16;
     return r > 256 ? 256 : r;
 }();
+// LDS of a workgroup that stages `rows` of them.
+template <int D, bool LO>
+constexpr int aw_lds(int rows, bool sum)
+{
+    const int q = rows * (LO ? 2 : 1) * D * 2;
+    return q + rows * (16 + 8 * (sum ? 1 : kAwWaves) + 4);
+}
 constexpr int kAwVecRows = 256;  // the vector kernel's, of which it stages 32 at a time
 constexpr int kAwVecTile = 32;
 constexpr int kAwVecChunk = kAwThreads;
@@ -73,7 +82,7 @@ __device__ __forceinline__ void aw_store(const WeightArgs& a, int64_t bh, int64_
 }  // namespace
 
 // Workgroup (split, row and KV head) of blockIdx.x: the keys of chunks split, split + splits, ..  SUM = false: the states of
-// query rows blockIdx.y * RB .. over them; SUM = true: the weights of them over all query rows.
+// query rows blockIdx.y * block_rows .. over them; SUM = true: the weights of them over all query rows.
 template <int CT, int QT, int D, bool SUM>
 __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8))) void attention_weights_mfma(WeightArgs a)
 {
@@ -86,7 +95,6 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
     constexpr int  DT = 32 * KSTEPS;
     constexpr bool LO = !((QT == BF16 && BF) || (QT == F16 && !BF));
     constexpr int  KP = kAwPages<D>;
-    constexpr int  RB = kAwRows<D, LO>;
     constexpr int  CHUNK = kAwChunk<D>;
     constexpr int  NP = LO ? 2 : 1;  // parts of q
     auto dimof = [](int j, int g)    // first of the 8 dims of k-step j in lane group g (as the decode's)
@@ -95,12 +103,16 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
             if (j == KSTEPS - 1) return 32 * j + 8 * g;
         return dim_of<CT>(j, g);
     };
-    // q as MFMA operands in the order the lanes read them: [tile][part][k-step][lane]
-    __shared__ u32x4  s_q[RB / 16 * NP * KSTEPS * 64];
-    __shared__ u32x2  s_qt[KT ? RB / 16 * NP * 64 : 1];
-    __shared__ int3   s_vis[RB];
-    __shared__ float  s_slope[RB];
-    __shared__ float2 s_ml[SUM ? 1 : kAwWaves][RB];  // SUM: (max, 1 / denominator) of the rows; else every wave's states
+    // LDS for the query rows that a workgroup stages (a.block_rows, at most RB), aw_lds bytes: q as MFMA operands in the
+    // order the lanes read them, [tile][part][k-step][lane], the last k-step's, what the rows see, (max, 1 / denominator) of
+    // the rows (SUM) or every wave's states of them, slopes
+    extern __shared__ __align__(16) uint8_t s_aw[];
+    const int rows = a.block_rows;
+    u32x4*    s_q = reinterpret_cast<u32x4*>(s_aw);
+    u32x2*    s_qt = reinterpret_cast<u32x2*>(s_q + rows / 16 * NP * KSTEPS * 64);
+    int4*     s_vis = reinterpret_cast<int4*>(s_qt + (KT ? rows / 16 * NP * 64 : 0));
+    float2*   s_ml = reinterpret_cast<float2*>(s_vis + rows);
+    float*    s_slope = reinterpret_cast<float*>(s_ml + (SUM ? 1 : kAwWaves) * rows);
 
     const int tid = static_cast<int>(threadIdx.x);
     const int lane = tid & 63;
@@ -116,15 +128,15 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
     const int64_t ctx = a.context_lens[b];
     const int total = __builtin_amdgcn_readfirstlane(aw_total(a, ctx));
     const int chunks = (total + CHUNK - 1) / CHUNK;
-    const int blocks = (R + RB - 1) / RB;
+    const int blocks = (R + rows - 1) / rows;
     const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
     float c_log2 = a.scale_log2;
     if constexpr (CT == FP8) c_log2 *= a.k_scale[kvh];
 
     auto stage = [&](int rb)
     {
-        const int r0 = rb * RB;
-        const int tiles = (min(RB, R - r0) + 15) / 16;
+        const int r0 = rb * rows;
+        const int tiles = (min(rows, R - r0) + 15) / 16;
         auto      q_at = [&](int r)
         {
             const int t = r / G;
@@ -177,9 +189,10 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
         for (int i = tid; i < tiles * 16; i += kAwThreads)
         {
             const int r = r0 + i;
-            s_vis[i] = r < R ? aw_visible(a, b, ctx, total, r / G) : make_int3(0, 0, 0);
+            const int3 vis = r < R ? aw_visible(a, b, ctx, total, r / G) : make_int3(0, 0, 0);
+            s_vis[i] = make_int4(vis.x, vis.y, vis.z, 0);
             s_slope[i] = r < R && a.rule.slopes != nullptr ? a.rule.slopes[kvh * G + r % G] * 1.4426950408889634f : 0.0f;
-            if constexpr (SUM) s_ml[0][i] = r < R ? a.fin[static_cast<int64_t>(bh) * R + r] : make_float2(0.0f, 0.0f);
+            if constexpr (SUM) s_ml[i] = r < R ? a.fin[static_cast<int64_t>(bh) * R + r] : make_float2(0.0f, 0.0f);
         }
         __syncthreads();
         return tiles;
@@ -189,7 +202,7 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
     int       tiles = 0;
     if (split < chunks && (!SUM || blocks == 1)) tiles = stage(rb0);
     if constexpr (!SUM)
-        for (int i = lane; i < RB; i += 64) s_ml[wave][i] = make_float2(kLowest, 0.0f);
+        for (int i = lane; i < rows; i += 64) s_ml[wave * rows + i] = make_float2(kLowest, 0.0f);
 
     for (int ch = split; ch < chunks; ch += a.splits)
     {
@@ -259,7 +272,7 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
             }
             for (int tile = 0; tile < tiles; ++tile)
             {
-                const int3 vis = s_vis[tile * 16 + c];
+                const int4 vis = s_vis[tile * 16 + c];
                 if (!__any(vis.x < vis.y && vis.x < key0 + KP * kBlockSize && vis.y > key0)) continue;
                 f32x4 s[KP];
 #pragma unroll
@@ -291,11 +304,7 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
                 float v[KP * 4];
 #pragma unroll
                 for (int e = 0; e < KP * 4; ++e) v[e] = s[e >> 2][e & 3] * c_log2;
-                if (a.rule.cap > 0.0f)
-                {
-#pragma unroll
-                    for (int e = 0; e < KP * 4; ++e) v[e] = cap_score(v[e], a.rule.cap, a.rule.inv_cap);
-                }
+                if (a.rule.cap > 0.0f) cap_scores<KP * 4>(v, a.rule.cap, a.rule.inv_cap);
                 if (a.rule.slopes != nullptr)
                 {
                     const float slope = -s_slope[tile * 16 + c];
@@ -317,7 +326,7 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
                 }
                 if constexpr (SUM)
                 {
-                    const float2 f = s_ml[0][tile * 16 + c];
+                    const float2 f = s_ml[tile * 16 + c];
 #pragma unroll
                     for (int e = 0; e < KP * 4; ++e) v[e] = __builtin_amdgcn_exp2f(v[e] - f.x) * f.y;
                     // A NaN query's state: NaN for the keys it sees alone.  (By its bits: from `f.y < infinity` in a vote the
@@ -346,7 +355,7 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
                     l = swap_sum(l);
                     if (g == 0)
                     {
-                        float2& st = s_ml[wave][tile * 16 + c];
+                        float2& st = s_ml[wave * rows + tile * 16 + c];
                         st = aw_join(st, make_float2(m, l));
                     }
                 }
@@ -368,13 +377,13 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
     if constexpr (!SUM)
     {
         __syncthreads();
-        for (int i = tid; i < RB; i += kAwThreads)
+        for (int i = tid; i < rows; i += kAwThreads)
         {
-            const int r = rb0 * RB + i;
+            const int r = rb0 * rows + i;
             if (r >= R) break;
-            float2 st = s_ml[0][i];
+            float2 st = s_ml[i];
 #pragma unroll
-            for (int w = 1; w < kAwWaves; ++w) st = aw_join(st, s_ml[w][i]);
+            for (int w = 1; w < kAwWaves; ++w) st = aw_join(st, s_ml[w * rows + i]);
             a.part[(static_cast<int64_t>(bh) * a.splits + split) * R + r] = st;
         }
     }
@@ -596,12 +605,16 @@ hipError_t launch_attention_weights(const WeightArgs& a, bool mfma, hipStream_t 
             return weights_for(a, [&]<int CT, int QT, int D>()
             {
                 constexpr bool LO = !((QT == BF16 && kBF<CT, QT>) || (QT == F16 && !kBF<CT, QT>));
-                const dim3     n = grid(kAwRows<D, LO>);
+                // as many query rows as the call has, up to kAwRows: the less LDS, the more workgroups per CU
+                WeightArgs w = a;
+                w.block_rows = static_cast<int>(std::min<int64_t>(kAwRows<D, LO>, (R + 15) / 16 * 16));
+                const int  lds = aw_lds<D, LO>(w.block_rows, sum);
+                const dim3 n = grid(w.block_rows);
                 if (n.y > 65535u) return hipErrorInvalidConfiguration;
                 if (sum)
-                    hipLaunchKernelGGL((attention_weights_mfma<CT, QT, D, true>), n, dim3(kAwThreads), 0, stream, a);
+                    hipLaunchKernelGGL((attention_weights_mfma<CT, QT, D, true>), n, dim3(kAwThreads), lds, stream, w);
                 else
-                    hipLaunchKernelGGL((attention_weights_mfma<CT, QT, D, false>), n, dim3(kAwThreads), 0, stream, a);
+                    hipLaunchKernelGGL((attention_weights_mfma<CT, QT, D, false>), n, dim3(kAwThreads), lds, stream, w);
                 return hipGetLastError();
             });
         const dim3 n = grid(kAwVecRows);

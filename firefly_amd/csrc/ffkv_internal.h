@@ -189,6 +189,7 @@ struct WeightArgs
     float          scale_log2;
     ScoreRule      rule;
     int            splits;  // of a row's keys (attention_weights_splits)
+    int            block_rows;  // query rows that a workgroup stages (set by the launcher)
     float2*        part;    // [batch * num_kv_heads, splits, seq_len * group]: (max, denominator) of each query row
     float2*        fin;     // [batch * num_kv_heads, seq_len * group]: (max, 1 / denominator)
     float*         weights;

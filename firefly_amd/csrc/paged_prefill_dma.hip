@@ -1070,10 +1070,14 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
                 {
 #pragma unroll
                     for (int gi = 0; gi < RG; ++gi)
+                    {
+                        float v[KP * 4];
 #pragma unroll
-                        for (int u = 0; u < KP; ++u)
+                        for (int e = 0; e < KP * 4; ++e) v[e] = s[gi][e >> 2][e & 3];
+                        cap_scores<KP * 4>(v, a.rule.cap, a.rule.inv_cap);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) s[gi][u][i] = cap_score(s[gi][u][i], a.rule.cap, a.rule.inv_cap);
+                        for (int e = 0; e < KP * 4; ++e) s[gi][e >> 2][e & 3] = v[e];
+                    }
                 }
                 if (a.rule.slopes != nullptr)
                 {
