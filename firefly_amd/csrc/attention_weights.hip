@@ -21,18 +21,19 @@ namespace ffkv
 namespace
 {
 
-constexpr int kAwWaves = 4;
+constexpr int kAwWaves = 8;
 constexpr int kAwThreads = 64 * kAwWaves;
-// Pages of keys a wave holds: 64 registers of 16-bit operands at head_dim 128 and 256.
-template <int D>
-constexpr int kAwPages = D <= 128 ? 4 : 2;
-template <int D>
-constexpr int kAwChunk = kAwWaves * kAwPages<D> * kBlockSize;  // keys of a workgroup at a time
-// Query rows staged in LDS at a time: 64 KiB of them, at most 256.
+constexpr int kAwPages = 2;  // pages of keys a wave holds: 32 registers of 16-bit operands at head_dim 128
+constexpr int kAwChunk = kAwWaves * kAwPages * kBlockSize;  // keys of a workgroup at a time
+// q in two parts, as where it is of another type than the products.
+template <int CT, int QT>
+constexpr bool kAwLo = !((QT == BF16 && (kBF<CT, QT> || CT == I8)) || (QT == F16 && !kBF<CT, QT>));
+// Query rows staged in LDS at a time: 32 KiB of them, at most 256 (with 64 KiB a CU has one workgroup of the states' pass
+// instead of three: 16 x 64 tokens over int8 pages 255 -> 224 us).
 template <int D, bool LO>
 constexpr int kAwRows = []
 {
-    const int r = 65536 / (D * 2 * (LO ? 2 : 1)) / 16 * 16;
+    const int r = 32768 / (D * 2 * (LO ? 2 : 1)) / 16 * 16;
     return r > 256 ? 256 : r;
 }();
 // LDS of a workgroup that stages `rows` of them.
@@ -44,7 +45,9 @@ constexpr int aw_lds(int rows, bool sum)
 }
 constexpr int kAwVecRows = 256;  // the vector kernel's, of which it stages 32 at a time
 constexpr int kAwVecTile = 32;
-constexpr int kAwVecChunk = kAwThreads;
+constexpr int kAwVecThreads = 256;
+constexpr int kAwVecWaves = kAwVecThreads / 64;
+constexpr int kAwVecChunk = kAwVecThreads;
 
 // Keys [x, y) that query token t of row b sees among its row's `total` tokens; z: its position.
 __device__ __forceinline__ int3 aw_visible(const WeightArgs& a, int b, int64_t ctx, int total, int t)
@@ -84,7 +87,7 @@ __device__ __forceinline__ void aw_store(const WeightArgs& a, int64_t bh, int64_
 // Workgroup (split, row and KV head) of blockIdx.x: the keys of chunks split, split + splits, ..  SUM = false: the states of
 // query rows blockIdx.y * block_rows .. over them; SUM = true: the weights of them over all query rows.
 template <int CT, int QT, int D, bool SUM>
-__global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8))) void attention_weights_mfma(WeightArgs a)
+__global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 4 : 2, 8))) void attention_weights_mfma(WeightArgs a)
 {
     constexpr bool BF = kBF<CT, QT>;
     using M = MType<BF>;
@@ -93,9 +96,12 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
     constexpr int  KSTEPS = D / 32;
     constexpr bool KT = D % 32 == 16;  // a last k-step of 16 dims
     constexpr int  DT = 32 * KSTEPS;
-    constexpr bool LO = !((QT == BF16 && BF) || (QT == F16 && !BF));
-    constexpr int  KP = kAwPages<D>;
-    constexpr int  CHUNK = kAwChunk<D>;
+    // int8 beside a bf16 q: f16 products with q converted whole (8 significant bits in 11), scaled by a power of two into
+    // f16's range where a staged block holds values of 2^15 and more
+    constexpr bool QX16 = CT == I8 && QT == BF16;
+    constexpr bool LO = kAwLo<CT, QT>;
+    constexpr int  KP = kAwPages;
+    constexpr int  CHUNK = kAwChunk;
     constexpr int  NP = LO ? 2 : 1;  // parts of q
     auto dimof = [](int j, int g)    // first of the 8 dims of k-step j in lane group g (as the decode's)
     {
@@ -130,71 +136,114 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
     const int chunks = (total + CHUNK - 1) / CHUNK;
     const int blocks = (R + rows - 1) / rows;
     const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
-    float c_log2 = a.scale_log2;
-    if constexpr (CT == FP8) c_log2 *= a.k_scale[kvh];
+    // from products to scores in log2 units, or in those of the cap (int8: times the key's scale)
+    float factor = a.rule.cap > 0.0f ? a.scale_log2 * a.rule.inv_cap : a.scale_log2;
+    if constexpr (CT == FP8) factor *= a.k_scale[kvh];
 
-    auto stage = [&](int rb)
+    __shared__ uint32_t s_most;  // QX16: the largest |q| of the block
+    float q_unscale = 1.0f;      // the products come out scaled by 1 / q_unscale
+    // A wave stages whole tiles of 16 query rows: lane (c, g) row c's dims dimof(j, g) .. of every k-step.
+    auto stage_q = [&](int rb, float qs, float& most)
     {
         const int r0 = rb * rows;
         const int tiles = (min(rows, R - r0) + 15) / 16;
-        auto      q_at = [&](int r)
+        auto parts = [&]<int N>(const float (&x)[N], uint32_t (&hi)[N], uint32_t (&lo)[N])
         {
-            const int t = r / G;
-            return ((static_cast<size_t>(b) * a.seq_len + t) * a.num_heads + kvh * G + (r - t * G)) * D;
-        };
-        auto parts = [&](const float* x, int n, uint32_t* hi, uint32_t* lo)
-        {
-            for (int e = 0; e < n; ++e)
+#pragma unroll
+            for (int e = 0; e < N; ++e)
             {
                 hi[e] = M::bits(x[e]);
                 lo[e] = LO ? M::bits(x[e] - M::value(hi[e])) : 0u;
             }
         };
-        for (int i = tid; i < tiles * KSTEPS * 64; i += kAwThreads)
+        for (int tile = wave; tile < tiles; tile += kAwWaves)
         {
-            const int l = i & 63, j = (i >> 6) % KSTEPS, tile = (i >> 6) / KSTEPS;
-            const int r = r0 + tile * 16 + (l & 15);
-            u32x4*    dst = s_q + ((tile * NP) * KSTEPS + j) * 64 + l;
-            u32x4     hi = u32x4{0u, 0u, 0u, 0u}, lo = hi;
-            if (r < R)
+            const int    r = r0 + tile * 16 + c;
+            const int    t = r / G, h = r - t * G;
+            const size_t at = ((static_cast<size_t>(b) * a.seq_len + t) * a.num_heads + kvh * G + h) * D;
+            if (g == 0)
             {
-                const size_t at = q_at(r) + dimof(j, l >> 4);
-                if constexpr (!LO)
-                    hi = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
-                else
+                const int3 vis = r < R ? aw_visible(a, b, ctx, total, t) : make_int3(0, 0, 0);
+                s_vis[tile * 16 + c] = make_int4(vis.x, vis.y, vis.z, 0);
+                s_slope[tile * 16 + c] = r < R && a.rule.slopes != nullptr ? a.rule.slopes[kvh * G + h] * 1.4426950408889634f : 0.0f;
+                if constexpr (SUM)
+                    s_ml[tile * 16 + c] = r < R ? a.fin[static_cast<int64_t>(bh) * R + r] : make_float2(0.0f, 0.0f);
+            }
+            u32x4* dst = s_q + tile * NP * KSTEPS * 64 + lane;
+#pragma unroll
+            for (int j = 0; j < KSTEPS; ++j)
+            {
+                u32x4 hi = u32x4{0u, 0u, 0u, 0u}, lo = hi;
+                if (r < R)
                 {
-                    float    x[8];
-                    uint32_t h[8], w[8];
-                    load_q8<QT>(a.q, at, x);
-                    parts(x, 8, h, w);
-                    hi = u32x4{h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
-                    lo = u32x4{w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16), w[6] | (w[7] << 16)};
+                    if constexpr (QX16)
+                    {
+                        float    x[8];
+                        uint32_t w[4];
+                        load_q8<QT>(a.q, at + dimof(j, g), x);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                        {
+                            most = fmaxf(most, fmaxf(__builtin_fabsf(x[2 * e]), __builtin_fabsf(x[2 * e + 1])));
+                            w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x[2 * e] * qs, x[2 * e + 1] * qs}, h2));
+                        }
+                        hi = u32x4{w[0], w[1], w[2], w[3]};
+                    }
+                    else if constexpr (!LO)
+                        hi = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at + dimof(j, g));
+                    else
+                    {
+                        float    x[8];
+                        uint32_t p[8], w[8];
+                        load_q8<QT>(a.q, at + dimof(j, g), x);
+                        parts(x, p, w);
+                        hi = u32x4{p[0] | (p[1] << 16), p[2] | (p[3] << 16), p[4] | (p[5] << 16), p[6] | (p[7] << 16)};
+                        lo = u32x4{w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16), w[6] | (w[7] << 16)};
+                    }
                 }
+                dst[j * 64] = hi;
+                if constexpr (LO) dst[(KSTEPS + j) * 64] = lo;
             }
-            dst[0] = hi;
-            if constexpr (LO) dst[KSTEPS * 64] = lo;
-        }
-        if constexpr (KT)
-            for (int i = tid; i < tiles * 64; i += kAwThreads)
+            if constexpr (KT)
             {
-                const int l = i & 63, tile = i >> 6;
-                const int r = r0 + tile * 16 + (l & 15);
-                float     x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t  h[4], w[4];
-                if (r < R) load_act4(a.q, QT, q_at(r) + DT + 4 * (l >> 4), x);
-                parts(x, 4, h, w);
-                s_qt[tile * NP * 64 + l] = u32x2{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
-                if constexpr (LO) s_qt[(tile * NP + 1) * 64 + l] = u32x2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)};
+                float    x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t p[4], w[4];
+                if (r < R) load_act4(a.q, QT, at + DT + 4 * g, x);
+                if constexpr (QX16)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        most = fmaxf(most, __builtin_fabsf(x[e]));
+                        x[e] *= qs;
+                    }
+                parts(x, p, w);
+                s_qt[tile * NP * 64 + lane] = u32x2{p[0] | (p[1] << 16), p[2] | (p[3] << 16)};
+                if constexpr (LO) s_qt[(tile * NP + 1) * 64 + lane] = u32x2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)};
             }
-        for (int i = tid; i < tiles * 16; i += kAwThreads)
-        {
-            const int r = r0 + i;
-            const int3 vis = r < R ? aw_visible(a, b, ctx, total, r / G) : make_int3(0, 0, 0);
-            s_vis[i] = make_int4(vis.x, vis.y, vis.z, 0);
-            s_slope[i] = r < R && a.rule.slopes != nullptr ? a.rule.slopes[kvh * G + r % G] * 1.4426950408889634f : 0.0f;
-            if constexpr (SUM) s_ml[i] = r < R ? a.fin[static_cast<int64_t>(bh) * R + r] : make_float2(0.0f, 0.0f);
         }
-        __syncthreads();
+        return tiles;
+    };
+    auto stage = [&](int rb)
+    {
+        float     most = 0.0f;
+        const int tiles = stage_q(rb, 1.0f, most);
+        if constexpr (QX16)
+        {
+            if (tid == 0) s_most = 0;
+            if (__syncthreads_or(most >= 32768.0f) != 0)  // rare: again, scaled
+            {
+                atomicMax(&s_most, f2u(most));  // (NaN is not among them: fmaxf passes it over)
+                __syncthreads();
+                const int e = __builtin_amdgcn_frexp_expf(u2f(s_most));
+                stage_q(rb, __builtin_ldexpf(1.0f, 15 - e), most);
+                q_unscale = __builtin_ldexpf(1.0f, e - 15);
+                __syncthreads();
+            }
+            else
+                q_unscale = 1.0f;
+        }
+        else
+            __syncthreads();
         return tiles;
     };
 
@@ -204,62 +253,97 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
     if constexpr (!SUM)
         for (int i = lane; i < rows; i += 64) s_ml[wave * rows + i] = make_float2(kLowest, 0.0f);
 
-    for (int ch = split; ch < chunks; ch += a.splits)
+    // This wave's keys of a chunk, as loaded: lane (c, g) holds dims dimof(j, g) .. + 7 of key c of each page.  (Loading the
+    // next chunk's ahead of this one's products took the registers over 128 and was no faster: one row of 32.7k tokens 58 us
+    // against 51, and 184 against 187 on 16 rows of int8 pages.)
+    constexpr int NW = kElemBytes<CT> == 2 ? KSTEPS : (KSTEPS + 1) / 2;
+    struct Keys
     {
-        const int key0 = ch * CHUNK + wave * (KP * kBlockSize);
-        // this wave's keys: lane (c, g) holds dims dimof(j, g) .. + 7 of key c of each page
-        X8    k[KP][KSTEPS > 0 ? KSTEPS : 1];
-        X4    kt[KP];
+        u32x4 k[KP][NW > 0 ? NW : 1];
+        u32x2 kt[KP];
         f32x4 ks[CT == I8 ? KP : 1];
-        int   okm = 0;
+        int   okm;  // pages that are there
+    };
+    auto load_keys = [&](int ch, Keys& w)
+    {
+        w.okm = 0;
 #pragma unroll
         for (int u = 0; u < KP; ++u)
         {
-            const int pg = key0 / kBlockSize + u;
-            const int phys = pg * kBlockSize < total ? __builtin_amdgcn_readfirstlane(table[pg]) : -1;
+            const int  pg = (ch * CHUNK + wave * (KP * kBlockSize)) / kBlockSize + u;
+            const int  phys = pg * kBlockSize < total ? __builtin_amdgcn_readfirstlane(table[pg]) : -1;
             const bool ok = phys >= 0 && phys < a.num_blocks;
-            okm |= ok ? 1 << u : 0;
+            w.okm |= ok ? 1 << u : 0;
             const size_t row = (static_cast<size_t>(ok ? phys : 0) * kBlockSize + c) * a.num_kv_heads + kvh;
             const char*  kp = static_cast<const char*>(a.k_cache) + row * D * kElemBytes<CT>;
-            if constexpr (kElemBytes<CT> == 2)
-            {
 #pragma unroll
-                for (int j = 0; j < KSTEPS; ++j)
-                    k[u][j] = __builtin_bit_cast(X8, ok ? *reinterpret_cast<const u32x4*>(kp + 2 * dimof(j, g))
-                                                        : u32x4{0u, 0u, 0u, 0u});
-                if constexpr (KT)
-                    kt[u] = __builtin_bit_cast(X4, ok ? *reinterpret_cast<const u32x2*>(kp + 2 * (DT + 4 * g)) : u32x2{0u, 0u});
-            }
-            else
+            for (int j = 0; j < NW; ++j)
             {
-#pragma unroll
-                for (int j = 0; j < KSTEPS; j += 2)
+                w.k[u][j] = u32x4{0u, 0u, 0u, 0u};
+                if (!ok) continue;
+                if constexpr (kElemBytes<CT> == 2)
+                    w.k[u][j] = *reinterpret_cast<const u32x4*>(kp + 2 * dimof(j, g));
+                else if (2 * j + 1 < KSTEPS)  // two k-steps' codes
+                    w.k[u][j] = *reinterpret_cast<const u32x4*>(kp + dimof(2 * j, g));
+                else
                 {
-                    u32x4 w = u32x4{0u, 0u, 0u, 0u};
-                    if (j + 1 < KSTEPS)
-                    {
-                        if (ok) w = *reinterpret_cast<const u32x4*>(kp + dimof(j, g));
-                        k[u][j + 1] = __builtin_bit_cast(X8, codes_to_m<CT, BF>(w[2], w[3]));
-                    }
-                    else if (ok)
-                    {
-                        const u32x2 t = *reinterpret_cast<const u32x2*>(kp + dimof(j, g));
-                        w = u32x4{t[0], t[1], 0u, 0u};
-                    }
-                    k[u][j] = __builtin_bit_cast(X8, codes_to_m<CT, BF>(w[0], w[1]));
+                    const u32x2 t = *reinterpret_cast<const u32x2*>(kp + dimof(2 * j, g));
+                    w.k[u][j] = u32x4{t[0], t[1], 0u, 0u};
                 }
-                if constexpr (KT)
+            }
+            if constexpr (KT)
+            {
+                w.kt[u] = u32x2{0u, 0u};
+                if (ok)
                 {
-                    const u32x4 m = codes_to_m<CT, BF>(ok ? *reinterpret_cast<const uint32_t*>(kp + DT + 4 * g) : 0u, 0u);
-                    kt[u] = __builtin_bit_cast(X4, u32x2{m[0], m[1]});
+                    if constexpr (kElemBytes<CT> == 2)
+                        w.kt[u] = *reinterpret_cast<const u32x2*>(kp + 2 * (DT + 4 * g));
+                    else
+                        w.kt[u][0] = *reinterpret_cast<const uint32_t*>(kp + DT + 4 * g);
                 }
             }
             if constexpr (CT == I8)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    ks[u][i] = ok ? a.k_scale[(static_cast<size_t>(phys) * kBlockSize + 4 * g + i) * a.num_kv_heads + kvh] : 0.0f;
+                    w.ks[u][i] =
+                        ok ? a.k_scale[(static_cast<size_t>(phys) * kBlockSize + 4 * g + i) * a.num_kv_heads + kvh] : 0.0f;
         }
-
+    };
+    for (int ch = split; ch < chunks; ch += a.splits)
+    {
+        const int key0 = ch * CHUNK + wave * (KP * kBlockSize);
+        Keys      raw_keys;
+        load_keys(ch, raw_keys);
+        X8        k[KP][KSTEPS > 0 ? KSTEPS : 1];
+        X4        kt[KP];
+        f32x4     ks[CT == I8 ? KP : 1];
+        const int okm = raw_keys.okm;
+#pragma unroll
+        for (int u = 0; u < KP; ++u)
+        {
+#pragma unroll
+            for (int j = 0; j < KSTEPS; ++j)
+            {
+                if constexpr (kElemBytes<CT> == 2)
+                    k[u][j] = __builtin_bit_cast(X8, raw_keys.k[u][j]);
+                else
+                {
+                    const u32x4 w = raw_keys.k[u][j / 2];
+                    k[u][j] = __builtin_bit_cast(X8, j & 1 ? codes_to_m<CT, BF>(w[2], w[3]) : codes_to_m<CT, BF>(w[0], w[1]));
+                }
+            }
+            if constexpr (KT)
+            {
+                u32x2 w = raw_keys.kt[u];
+                if constexpr (kElemBytes<CT> == 1)
+                {
+                    const u32x4 m = codes_to_m<CT, BF>(w[0], 0u);
+                    w = u32x2{m[0], m[1]};
+                }
+                kt[u] = __builtin_bit_cast(X4, w);
+            }
+            if constexpr (CT == I8) ks[u] = raw_keys.ks[u] * factor;
+        }
         float acc[KP * 4];  // SUM: this lane's columns' weights of key 4g + i of page u
 #pragma unroll
         for (int e = 0; e < KP * 4; ++e) acc[e] = 0.0f;
@@ -298,13 +382,23 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
                             st = M::mma16(kt[u], __builtin_bit_cast(X4, s_qt[(tile * NP + p) * 64 + lane]), st);
                         s[u] += st;
                     }
-                if constexpr (CT == I8)
+                // Without a cap or a bias the factor is left to the exponent's multiply-add (int8 keys have one each; an fp8
+                // head's scale may be negative or zero, which would turn the maximum around).
+                const bool raw = CT != I8 && a.rule.cap <= 0.0f && a.rule.slopes == nullptr && factor > 0.0f;
+                float      v[KP * 4];
+                if (raw)
+                {
 #pragma unroll
-                    for (int u = 0; u < KP; ++u) s[u] *= ks[u];
-                float v[KP * 4];
+                    for (int e = 0; e < KP * 4; ++e) v[e] = s[e >> 2][e & 3];
+                }
+                else
 #pragma unroll
-                for (int e = 0; e < KP * 4; ++e) v[e] = s[e >> 2][e & 3] * c_log2;
-                if (a.rule.cap > 0.0f) cap_scores<KP * 4>(v, a.rule.cap, a.rule.inv_cap);
+                for (int e = 0; e < KP * 4; ++e) v[e] = s[e >> 2][e & 3] * (CT == I8 ? ks[e >> 2][e & 3] : factor);
+                if constexpr (QX16)
+                    if (q_unscale != 1.0f)  // uniform, rare
+#pragma unroll
+                        for (int e = 0; e < KP * 4; ++e) v[e] *= q_unscale;
+                if (a.rule.cap > 0.0f) cap_scores<KP * 4>(v, a.rule.cap);
                 if (a.rule.slopes != nullptr)
                 {
                     const float slope = -s_slope[tile * 16 + c];
@@ -328,7 +422,8 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
                 {
                     const float2 f = s_ml[tile * 16 + c];
 #pragma unroll
-                    for (int e = 0; e < KP * 4; ++e) v[e] = __builtin_amdgcn_exp2f(v[e] - f.x) * f.y;
+                    for (int e = 0; e < KP * 4; ++e)
+                        v[e] = __builtin_amdgcn_exp2f(CT == I8 ? v[e] - f.x : __builtin_fmaf(v[e], raw ? factor : 1.0f, -f.x));
                     // A NaN query's state: NaN for the keys it sees alone.  (By its bits: from `f.y < infinity` in a vote the
                     // compiler made an unordered compare, which a NaN passes.)
                     if (masked && __any((f2u(f.y) & 0x7fffffffu) > 0x7f800000u))
@@ -338,25 +433,28 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
                         {
                             const int  key = key0 + 4 * g + 16 * (e >> 2) + (e & 3);
                             const bool seen = (okm >> (e >> 2) & 1) && key >= vis.x && key < vis.y;
-                            v[e] = seen ? v[e] : 0.0f;
+                            acc[e] += seen ? v[e] * f.y : 0.0f;
                         }
                     }
+                    else
 #pragma unroll
-                    for (int e = 0; e < KP * 4; ++e) acc[e] += v[e];
+                        for (int e = 0; e < KP * 4; ++e) acc[e] = __builtin_fmaf(v[e], f.y, acc[e]);
                 }
                 else
                 {
-                    float m = kLowest, l = 0.0f;
+                    const float k1 = raw ? factor : 1.0f;
+                    float       m = kNegInf, l = 0.0f;
 #pragma unroll
                     for (int e = 0; e < KP * 4; ++e) m = __builtin_elementwise_maximum(m, v[e]);
-                    m = swap_max(m);
+                    m = __builtin_elementwise_maximum(swap_max(m) * k1, kLowest);
 #pragma unroll
-                    for (int e = 0; e < KP * 4; ++e) l += __builtin_amdgcn_exp2f(v[e] - m);
+                    for (int e = 0; e < KP * 4; ++e)
+                        l += __builtin_amdgcn_exp2f(CT == I8 ? v[e] - m : __builtin_fmaf(v[e], k1, -m));
                     l = swap_sum(l);
                     if (g == 0)
                     {
                         float2& st = s_ml[wave * rows + tile * 16 + c];
-                        st = aw_join(st, make_float2(m, l));
+                        st = ch == split ? make_float2(m, l) : aw_join(st, make_float2(m, l));
                     }
                 }
             }
@@ -392,13 +490,13 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(2, 8
 // The same with vector arithmetic (fp32 caches, and head dims that the matrix cores do not take): a thread has a key, 32
 // query rows at a time pass by in LDS.
 template <int CT, bool SUM>
-__global__ __launch_bounds__(kAwThreads) void attention_weights_vector(WeightArgs a)
+__global__ __launch_bounds__(kAwVecThreads) void attention_weights_vector(WeightArgs a)
 {
     constexpr int T = kAwVecTile;
     __shared__ float  s_q[T][256];
     __shared__ int3   s_vis[T];
     __shared__ float  s_slope[T];
-    __shared__ float2 s_ml[SUM ? 1 : kAwWaves][SUM ? T : kAwVecRows];
+    __shared__ float2 s_ml[SUM ? 1 : kAwVecWaves][SUM ? T : kAwVecRows];
     const int D = a.head_dim;
     const int tid = static_cast<int>(threadIdx.x);
     const int lane = tid & 63;
@@ -431,7 +529,7 @@ __global__ __launch_bounds__(kAwThreads) void attention_weights_vector(WeightArg
         {
             const int m = min(T, r_hi - r0);
             __syncthreads();  // the last rows are done with
-            for (int i = tid; i < T * (D / 4); i += kAwThreads)
+            for (int i = tid; i < T * (D / 4); i += kAwVecThreads)
             {
                 const int rr = i / (D / 4), d = 4 * (i - rr * (D / 4));
                 float     x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -475,7 +573,7 @@ __global__ __launch_bounds__(kAwThreads) void attention_weights_vector(WeightArg
             {
                 const int3 vis = s_vis[rr];
                 float      v = s[rr] * sk;
-                if (a.rule.cap > 0.0f) v = cap_score(v, a.rule.cap, a.rule.inv_cap);
+                if (a.rule.cap > 0.0f) v = cap_score(v * a.rule.inv_cap, a.rule.cap);
                 if (a.rule.slopes != nullptr)
                     v = __builtin_fmaf(-s_slope[rr], __builtin_fabsf(static_cast<float>(key - vis.z)), v);
                 v = ok && key >= vis.x && key < vis.y ? v : kNegInf;
@@ -503,11 +601,11 @@ __global__ __launch_bounds__(kAwThreads) void attention_weights_vector(WeightArg
     if constexpr (!SUM)
     {
         __syncthreads();
-        for (int r = r_lo + tid; r < r_hi; r += kAwThreads)
+        for (int r = r_lo + tid; r < r_hi; r += kAwVecThreads)
         {
             float2 st = s_ml[0][r - r_lo];
 #pragma unroll
-            for (int v = 1; v < kAwWaves; ++v) st = aw_join(st, s_ml[v][r - r_lo]);
+            for (int v = 1; v < kAwVecWaves; ++v) st = aw_join(st, s_ml[v][r - r_lo]);
             a.part[(static_cast<int64_t>(bh) * a.splits + split) * R + r] = st;
         }
     }
@@ -574,20 +672,23 @@ template <int CT>
 hipError_t launch_vector(const WeightArgs& a, bool sum, dim3 grid, hipStream_t stream)
 {
     if (sum)
-        hipLaunchKernelGGL((attention_weights_vector<CT, true>), grid, dim3(kAwThreads), 0, stream, a);
+        hipLaunchKernelGGL((attention_weights_vector<CT, true>), grid, dim3(kAwVecThreads), 0, stream, a);
     else
-        hipLaunchKernelGGL((attention_weights_vector<CT, false>), grid, dim3(kAwThreads), 0, stream, a);
+        hipLaunchKernelGGL((attention_weights_vector<CT, false>), grid, dim3(kAwVecThreads), 0, stream, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
-// Splits of a row's keys: one chunk of keys a workgroup, fewer where the rows and heads alone fill the chip several times.
+// Splits of a row's keys: as many workgroups in all as fit the chip at once (two of eight waves per CU), one chunk of keys
+// each at most; a workgroup then stages its query rows once for several chunks.  us at 256 / 512 / 1024 / 2048 workgroups:
+// 32 tokens over one row of 32.7k 65 / 51 / 59 / 60, 16 x 64 tokens over int8 rows of 400 to 4000 244 / 187 / 191 / 215.
 int attention_weights_splits(int batch, int num_kv_heads, int head_dim, int cap_tokens)
 {
-    const int64_t chunk = head_dim == 256 ? kAwChunk<256> : kAwChunk<128>;
+    constexpr int64_t kMost = 512;
+    const int64_t chunk = kAwChunk;
     const int64_t chunks = (static_cast<int64_t>(cap_tokens) + chunk - 1) / chunk;
-    const int64_t most = 8192 / (static_cast<int64_t>(batch) * num_kv_heads);
+    const int64_t most = kMost / (static_cast<int64_t>(batch) * num_kv_heads);
     const int64_t n = chunks < most ? chunks : most;
     return static_cast<int>(n < 1 ? 1 : n);
 }
@@ -604,7 +705,7 @@ hipError_t launch_attention_weights(const WeightArgs& a, bool mfma, hipStream_t 
         if (mfma)
             return weights_for(a, [&]<int CT, int QT, int D>()
             {
-                constexpr bool LO = !((QT == BF16 && kBF<CT, QT>) || (QT == F16 && !kBF<CT, QT>));
+                constexpr bool LO = kAwLo<CT, QT>;
                 // as many query rows as the call has, up to kAwRows: the less LDS, the more workgroups per CU
                 WeightArgs w = a;
                 w.block_rows = static_cast<int>(std::min<int64_t>(kAwRows<D, LO>, (R + 15) / 16 * 16));

@@ -262,7 +262,7 @@ __global__ __launch_bounds__(256) void paged_decode_generic(DecodeArgs a)
                     for (int g = 0; g < GP; ++g)
                     {
                         s[g] *= a.scale_log2;
-                        if (a.rule.cap > 0.0f) s[g] = cap_score(s[g], a.rule.cap, a.rule.inv_cap);
+                        if (a.rule.cap > 0.0f) s[g] = cap_score(s[g] * a.rule.inv_cap, a.rule.cap);
                         if (a.rule.slopes != nullptr)  // j - i <= 0
                             s[g] = __builtin_fmaf(slope[g], static_cast<float>(j - span.pos), s[g]);
                         if (a.ws_scores != nullptr && g < G && lane == 0 && j < end)

@@ -749,7 +749,7 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
             float      v = s[i] * ks[i] * kv_scale_log2;
             if constexpr (RULE)
             {
-                if (rule_cap > 0.0f) v = cap_score(v, rule_cap, rule_inv);
+                if (rule_cap > 0.0f) v = cap_score(v * rule_inv, rule_cap);
                 if (a.rule.slopes != nullptr)  // j - i <= 0
                     v = __builtin_fmaf(rule_slope, static_cast<float>(page * kBlockSize + 4 * g + i - pos), v);
             }

@@ -941,8 +941,9 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         c_log2 = fmaxf(c_log2 * __builtin_fabsf(ks), 1e-30f);
         v_head_scale = a.v_scale[kvh];
     }
-    // RULE with a cap or a bias: the scores are brought to log2 units first (s_log2), and the softmax takes them as they are
-    const float s_log2 = c_log2;
+    // RULE with a cap or a bias: the scores are brought to log2 units, or those of the cap, first (s_factor), and the softmax
+    // takes them as they come out
+    const float s_factor = RULE && a.rule.cap > 0.0f ? c_log2 * a.rule.inv_cap : c_log2;
     const bool  convert = RULE && (a.rule.cap > 0.0f || a.rule.slopes != nullptr);
     if (RULE && convert) c_log2 = 1.0f;
     const float thr_raw = 8.0f / c_log2;
@@ -1065,7 +1066,7 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
 #pragma unroll
                 for (int gi = 0; gi < RG; ++gi)
 #pragma unroll
-                    for (int u = 0; u < KP; ++u) s[gi][u] *= s_log2;
+                    for (int u = 0; u < KP; ++u) s[gi][u] *= s_factor;
                 if (a.rule.cap > 0.0f)
                 {
 #pragma unroll
@@ -1074,7 +1075,7 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
                         float v[KP * 4];
 #pragma unroll
                         for (int e = 0; e < KP * 4; ++e) v[e] = s[gi][e >> 2][e & 3];
-                        cap_scores<KP * 4>(v, a.rule.cap, a.rule.inv_cap);
+                        cap_scores<KP * 4>(v, a.rule.cap);
 #pragma unroll
                         for (int e = 0; e < KP * 4; ++e) s[gi][e >> 2][e & 3] = v[e];
                     }

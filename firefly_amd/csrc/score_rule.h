@@ -11,47 +11,46 @@ namespace ffkv
 namespace
 {
 
-// cap * tanh(v / cap) of a score in log2 units (cap and 1 / cap in them too).  Below 0.6 tanh(x) = x + x^3 P(x^2) with P
-// fitted to a relative error under 2^-23 (1 - 2 / (e^2x + 1) would lose the small scores' low bits: an absolute error of
-// 2^-24 of the cap, 6e-6 at a cap of 50), above it (1 - e) / (1 + e) with e = e^-2|x|, which holds at infinity (e = 0).
+// cap * tanh(x) of a score x in units of its cap.  Below 0.6 tanh(x) = x + x^3 P(x^2) with P fitted to a relative error
+// under 2^-23 (1 - 2 / (e^2x + 1) would lose the small scores' low bits: an absolute error of 2^-24 of the cap, 6e-6 at a
+// cap of 50), above it (1 - e) / (1 + e) with e = e^-2|x|, which holds at infinity (e = 0).
 constexpr float kCapNear = 0.6f;
-__device__ __forceinline__ float cap_near(float v, float cap, float inv_cap)
+__device__ __forceinline__ float cap_near(float x, float cap)
 {
-    const float x = v * inv_cap;
     const float t = x * x;
     float       p = -0.005908978637307882f;
     p = __builtin_fmaf(p, t, 0.0208087470382452f);
     p = __builtin_fmaf(p, t, -0.053787969052791595f);
     p = __builtin_fmaf(p, t, 0.13331978023052216f);
     p = __builtin_fmaf(p, t, -0.33333301544189453f);
-    return __builtin_fmaf(v * t, p, v);
+    return cap * __builtin_fmaf(x * t, p, x);
 }
-__device__ __forceinline__ float cap_score(float v, float cap, float inv_cap)
+__device__ __forceinline__ float cap_score(float x, float cap)
 {
-    const float x = v * inv_cap;
     const float ax = __builtin_fabsf(x);
     const float e = __builtin_amdgcn_exp2f(ax * -2.8853900817779268f);
     const float far = cap * __builtin_copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
-    return ax < kCapNear ? cap_near(v, cap, inv_cap) : far;
+    return ax < kCapNear ? cap_near(x, cap) : far;
 }
 // The same for N scores of every lane.  Scores are mostly well below their cap (a cap of 30 to 50 over scores of a standard
-// deviation of a few), and a wave all of whose scores are near takes the polynomial alone: 7 vector instructions per score
-// instead of 15 and two transcendental ones of four times the time.
+// deviation of a few), and a wave all of whose scores are near takes the polynomial alone: 8 vector instructions per score
+// instead of 16 and two transcendental ones of four times the time.  (A shorter one up to 0.35 gains less than the waves that
+// then pass it cost: weights of 16 x 64 tokens over int8 pages at a cap of 50, 258 us against 236.)
 template <int N>
-__device__ __forceinline__ void cap_scores(float (&v)[N], float cap, float inv_cap)
+__device__ __forceinline__ void cap_scores(float (&x)[N], float cap)
 {
     float most = 0.0f;
 #pragma unroll
-    for (int e = 0; e < N; ++e) most = fmaxf(most, __builtin_fabsf(v[e]));  // (NaN is passed over: both forms keep it)
-    if (__any(most >= kCapNear * cap))
+    for (int e = 0; e < N; ++e) most = fmaxf(most, __builtin_fabsf(x[e]));  // (NaN is passed over: both forms keep it)
+    if (__any(most >= kCapNear))
     {
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = cap_score(v[e], cap, inv_cap);
+        for (int e = 0; e < N; ++e) x[e] = cap_score(x[e], cap);
     }
     else
     {
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = cap_near(v[e], cap, inv_cap);
+        for (int e = 0; e < N; ++e) x[e] = cap_near(x[e], cap);
     }
 }
 
