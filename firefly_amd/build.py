@@ -42,7 +42,8 @@ DEVICE = [f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-p
 
 
 def _sources() -> list[Path]:
-    return sorted(list(CSRC.glob("*.hip")) + list(CSRC.glob("*.cpp")) + list((CSRC / "host").glob("*.cpp")))
+    # the attention kernels (paged_*.hip), by far the longest to compile, come first
+    return sorted(list(CSRC.glob("*.hip")) + list(CSRC.glob("*.cpp")) + list((CSRC / "host").glob("*.cpp")), reverse=True)
 
 
 def _compile(src: Path, build_dir: Path = BUILD, defines: tuple[str, ...] = ()) -> Path:
@@ -103,9 +104,10 @@ def build_front() -> Path:
 
 def build_test_shims() -> None:
     """Test-only helpers linked against libffkv.so: the C++-API shims under tests/cpp/ (kernels_api_shim.cpp for
-    tests/test_gpu_cxx_api.py, decode_step_shim.cpp for tests/test_gpu_decode_step.py) and engine_calls.bin
+    tests/test_gpu_cxx_api.py, decode_step_shim.cpp for tests/test_gpu_decode_step.py, scored_api_shim.cpp for
+    tests/test_gpu_scored_cxx.py) and engine_calls.bin
     (tests/test_hal.py)."""
-    for name in ("kernels_api_shim", "decode_step_shim"):
+    for name in ("kernels_api_shim", "decode_step_shim", "scored_api_shim"):
         src = ROOT / "tests" / "cpp" / f"{name}.cpp"
         if not src.exists():
             continue

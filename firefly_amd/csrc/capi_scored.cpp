@@ -64,7 +64,7 @@ bool scored_mfma(int cache_dtype, int head_dim)
     return cache_dtype != FFKV_DTYPE_F32 && (head_dim_mfma(head_dim) || head_dim == 80 || head_dim == 96 || head_dim == 112);
 }
 
-// Regions of the weights' pass behind the decode's partials: scores [batch, num_heads, stride] and final states
+// Regions of the weights' pass behind the decode's partials: scores (stride tokens per row and query head) and final states
 // [batch, num_heads, 2].
 struct ScoreLayout
 {

@@ -156,7 +156,7 @@ struct DecodeArgs
     const void*    k_new;
     const void*    v_new;
     // Scored decode only (launch_decode_scored): the rule; with weights, the scores of all visible keys in log2 units,
-    // [batch, num_heads, score_stride] fp32, each row's final (max, denominator) per head, [batch, num_heads, 2], and the
+    // fp32 (score_page of score_rule.h; score_stride tokens per row), each row's final (max, denominator) per head, [batch, num_heads, 2], and the
     // weights themselves (decay * prior + what this call gives), [batch, num_kv_heads, weight_stride].
     ScoreRule      rule;
     float*         ws_scores;  // null: no weights
@@ -250,6 +250,7 @@ hipError_t launch_prefill_merge(const PrefillArgs& a, hipStream_t stream);  // o
 // The prefill under a score rule (paged_prefill_scored.hip), its plan from a.span_tokens.
 void       prefill_scored_plan(PrefillArgs& a);
 hipError_t launch_prefill_scored(const PrefillArgs& a, hipStream_t stream);
+hipError_t launch_prefill_scored_pieces(const PrefillArgs& a, unsigned wgs, hipStream_t stream);  // its split form's launch
 struct PrefillSplitLayout
 {
     int64_t pieces, ml, acc, total;  // byte offsets of the three regions and their end (0: no split)
@@ -278,7 +279,8 @@ bool decode_use_mfma(int cache_dtype, int group, int head_dim);
 int        decode_scored_launch_items(const DecodeArgs& a);
 hipError_t launch_decode_scored(const DecodeArgs& a, bool mfma, bool row, hipStream_t stream);
 hipError_t launch_decode_scored_generic(const DecodeArgs& a, hipStream_t stream);
-hipError_t launch_decode_weights(const DecodeArgs& a, hipStream_t stream);  // the weights from the scores
+hipError_t launch_decode_scores(const DecodeArgs& a, bool row, hipStream_t stream);  // with the scores written down
+hipError_t launch_decode_weights(const DecodeArgs& a, hipStream_t stream);  // the weights from them
 
 // Fused shared-prefix decode (paged_decode_pfx.hip): the prefix partials and the decode of the rows' own pages in
 // one grid, then the merge.  decode_pfx_plan sizes it for `a` (dtypes, batch, heads, head_dim set) over

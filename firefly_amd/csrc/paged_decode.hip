@@ -266,7 +266,7 @@ __global__ __launch_bounds__(256) void paged_decode_generic(DecodeArgs a)
                         if (a.rule.slopes != nullptr)  // j - i <= 0
                             s[g] = __builtin_fmaf(slope[g], static_cast<float>(j - span.pos), s[g]);
                         if (a.ws_scores != nullptr && g < G && lane == 0 && j < end)
-                            a.ws_scores[(static_cast<int64_t>(b) * a.num_heads + kvh * G + g) * a.score_stride + j] =
+                            a.ws_scores[score_page(a, b, kvh, j >> 4) + g * kBlockSize + (j & 15)] =
                                 valid[u] ? s[g] : -__builtin_huge_valf();
                     }
                 }

@@ -179,8 +179,8 @@ constexpr int kMfmaMaxWaves =
 // ROW: the workgroup is one row (item_) and one KV head, or block of 16 of its query heads (y_); its nw_ waves share the
 // row's pages, combine their states through LDS (s_v, as row_lds_bytes sizes it) and write the output: no partials.
 // RULE: the scores are changed and the keys bounded by a.rule (a row's pages begin at its first visible key), and with
-// a.ws_scores the visible keys' scores and the rows' final (max, denominator) are written down for the weights.
-template <int CT, int QT, int D, bool PW = false, bool ROW = false, bool RULE = false>
+// SCORES the visible keys' scores and the rows' final (max, denominator) are written down for the weights.
+template <int CT, int QT, int D, bool PW = false, bool ROW = false, bool RULE = false, bool SCORES = false>
 __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_, int n_items_, int nw_, uint16_t* s_v)
 {
     static_assert(!(PW && (ROW || RULE)), "one split or the other; no rule over a shared prefix");
@@ -712,12 +712,12 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         rule_inv = a.rule.inv_cap;
         if (a.rule.slopes != nullptr && c < gc) rule_slope = a.rule.slopes[kvh * G + h0 + c] * 1.4426950408889634f;
     }
+    // (The lanes' 16 bytes of a page lie together: written head by head along the row, 64 bytes of each at a time, the same
+    // 19 MB cost 64 rows of 512 to 4096 tokens 19 us.)
     auto write_scores = [&](int b, int page, f32x4 sc)
     {
         if (c < gc)
-            *reinterpret_cast<f32x4*>(a.ws_scores +
-                                      (static_cast<int64_t>(b) * a.num_heads + kvh * G + h0 + c) * a.score_stride +
-                                      static_cast<int64_t>(page) * kBlockSize + 4 * g) = sc;
+            *reinterpret_cast<f32x4*>(a.ws_scores + score_page(a, b, kvh, page) + (h0 + c) * kBlockSize + 4 * g) = sc;
     };
 
     // Online softmax of a staged page's scores and PV from its LDS tile.  tks / tvs: int8 scales of token c.
@@ -756,8 +756,7 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
             sc[i] = ok ? v : kNegInf;
             mt = fmaxf(mt, sc[i]);
         }
-        if constexpr (RULE)
-            if (a.ws_scores != nullptr) write_scores(b, page, f32x4{sc[0], sc[1], sc[2], sc[3]});
+        if constexpr (SCORES) write_scores(b, page, f32x4{sc[0], sc[1], sc[2], sc[3]});
         mt = xor_max(mt);
         const float m_new = fmaxf(m_run, mt);
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
@@ -830,8 +829,8 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
                 for (int n = 0; n < NT; ++n)
                     store_out4<QT>(a.out, (static_cast<size_t>(b) * a.num_heads + h) * D + 16 * n + 4 * g,
                                    acc[n] * inv);
-                if constexpr (RULE)
-                    if (a.ws_final != nullptr && g == 0)
+                if constexpr (SCORES)
+                    if (g == 0)
                         reinterpret_cast<float2*>(a.ws_final)[static_cast<int64_t>(b) * a.num_heads + h] =
                             float2{m_run, l_tot};
             }
@@ -888,8 +887,8 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
         if constexpr (DEPTH == 1)
             if (!ROW && row_ends && p + 1 < end) load_q(cur.b);
         if (ok) finish_page(n_tok, n_lo, b, page, pos, tks, tvs, s);
-        if constexpr (RULE)
-            if (!ok && a.ws_scores != nullptr) write_scores(b, page, f32x4{kNegInf, kNegInf, kNegInf, kNegInf});
+        if constexpr (SCORES)
+            if (!ok) write_scores(b, page, f32x4{kNegInf, kNegInf, kNegInf, kNegInf});
         if (!ROW && (row_ends || p + 1 == end))
         {
             finish_segment(b, pb, nb, seg_start, p + 1);
@@ -942,8 +941,8 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
             }
             store_out4<QT>(a.out, (static_cast<size_t>(item_) * a.num_heads + kvh * G + h0 + h) * D + d4,
                            o * softmax_inv(L));
-            if constexpr (RULE)
-                if (a.ws_final != nullptr && d4 == 0)
+            if constexpr (SCORES)
+                if (d4 == 0)
                     reinterpret_cast<float2*>(a.ws_final)[static_cast<int64_t>(item_) * a.num_heads + kvh * G + h0 + h] =
                         float2{M, L};
         }
@@ -982,7 +981,7 @@ void paged_decode_mfma(DecodeArgs a)
 // One workgroup of MW waves per (row, head): wave w folds segments i_lo + w, i_lo + w + MW, ... into an online
 // (max, denominator, output) state (lane = D/64 dims), then the waves' states are combined through LDS.
 // MW waves per (row, head): as many as the rows have pieces for (launch_merge).  FIN: the row's (max, denominator) of each
-// head goes to ws_final too (null: not asked for).
+// head goes to ws_final too.
 template <int QT, int D, int MW, bool FIN = false>
 __global__ __launch_bounds__(64 * MW) void paged_decode_mfma_merge(DecodeArgs a)
 {
@@ -1070,7 +1069,7 @@ __global__ __launch_bounds__(64 * MW) void paged_decode_mfma_merge(DecodeArgs a)
         }
         store_act1(a.out, QT, ob + d, L == 0.0f ? 0.0f : O / L);
         if constexpr (FIN)
-            if (a.ws_final != nullptr && d == 0)
+            if (d == 0)
                 reinterpret_cast<float2*>(a.ws_final)[static_cast<int64_t>(b) * a.num_heads + h] = float2{M, L};
     }
 }
@@ -1133,7 +1132,7 @@ __global__ __launch_bounds__(256) void paged_decode_mfma_merge_rows(DecodeArgs a
     store_out4<QT>(a.out, (static_cast<size_t>(b) * a.num_heads + h) * D + d4,
                    o * softmax_inv(l));
     if constexpr (FIN)
-        if (a.ws_final != nullptr && d4 == 0)
+        if (d4 == 0)
             reinterpret_cast<float2*>(a.ws_final)[static_cast<int64_t>(b) * a.num_heads + h] = float2{m, l};
 }
 

@@ -62,6 +62,13 @@ __device__ __forceinline__ int64_t first_key(const ScoreRule& r, int64_t pos, in
     return lo;
 }
 
+// Scores that the decode writes down for the weights: [batch, num_kv_heads, pages, group, 16 tokens], so that what a wave
+// writes of a page (up to 16 heads of 64 bytes) is contiguous.
+__device__ __forceinline__ int64_t score_page(const DecodeArgs& a, int b, int kvh, int page)
+{
+    return ((static_cast<int64_t>(b) * a.num_kv_heads + kvh) * (a.score_stride / kBlockSize) + page) * a.group * kBlockSize;
+}
+
 // Tokens that the decode of row b attends under the rule: [lo, hi).
 struct RowSpan
 {
