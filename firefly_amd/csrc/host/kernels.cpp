@@ -334,4 +334,120 @@ void rope_append_kv_cache(Tensor& q, Tensor& k, const Tensor& v, Tensor& k_cache
                 context_lens, max_blocks, theta);
 }
 
+namespace
+{
+
+// Tokens per (row, KV head) of a weights tensor [B, Hkv, T], or -1 where it is none.
+int64_t weight_tokens(const Tensor& w, int64_t B, int64_t Hkv)
+{
+    const auto& s = w.shape();
+    return is_gpu(w) && w.dtype() == DType::F32 && s.size() == 3 && s[0] == B && s[1] == Hkv ? s[2] : -1;
+}
+
+const float* scale_of(const Tensor* t) { return t ? t->data_as<const float>() : nullptr; }
+
+}  // namespace
+
+void attention_scored(Tensor& q, Tensor& k, Tensor& v, Tensor& output, void* kv_cache_block_table, int kv_head_num,
+                      int seq_len, int max_context_blocks, const int* context_lens, const ScoreRule& rule,
+                      const Tensor* k_scale, const Tensor* v_scale, Tensor* weights, const Tensor* prior, float decay,
+                      int max_context_len)
+{
+    if (q.shape().size() != 4 || k.shape().size() != 4 || !is_gpu(q) || !is_gpu(k) || !is_gpu(v) || !is_gpu(output))
+        return fail("attention_scored: q must be [B, S, Hq, D] and all tensors on the GPU");
+    const int B = static_cast<int>(q.shape()[0]), S = static_cast<int>(q.shape()[1]);
+    const int Hq = static_cast<int>(q.shape()[2]), D = static_cast<int>(q.shape()[3]);
+    const bool paged = kv_cache_block_table != nullptr;
+    if (output.numel() < static_cast<int64_t>(B) * S * Hq * D || output.dtype() != q.dtype())
+        return fail("attention_scored: output must hold as many elements of q's dtype as q");
+    if (k.shape()[2] != kv_head_num || k.shape()[3] != D || v.shape() != k.shape() || v.dtype() != k.dtype())
+        return fail("attention_scored: k/v must be [.., .., kv_head_num, head_dim] and alike");
+    const auto* table = reinterpret_cast<const int32_t*>(kv_cache_block_table);
+    const int   pages = paged ? static_cast<int>(k.shape()[0]) : 0;
+    size_t      have = 0;
+    if (paged && S == 1)
+    {
+        if (rule.key_end != nullptr) return fail("attention_scored: the decode has no key_end");
+        int64_t stride = 0;
+        if (weights != nullptr && (stride = weight_tokens(*weights, B, kv_head_num)) < 0)
+            return fail("attention_scored: weights must be F32 [B, kv_head_num, T] on the GPU");
+        if (prior != nullptr && (weights == nullptr || weight_tokens(*prior, B, kv_head_num) != stride))
+            return fail("attention_scored: prior must be of the weights' shape");
+        const size_t need = ffkv_decode_scored_workspace_bytes(B, Hq, D, max_context_blocks, max_context_len, weights != nullptr);
+        void*        ws = workspace(need, have);
+        return report(ffkv_paged_decode_scored(
+                          q.data(), output.data(), code(q.dtype()), k.data(), v.data(), code(k.dtype()),
+                          const_cast<float*>(scale_of(k_scale)), const_cast<float*>(scale_of(v_scale)), table, context_lens, B, Hq,
+                          kv_head_num, D, FFKV_BLOCK_SIZE, max_context_blocks, pages, max_context_len, 0.0f, rule.cap,
+                          rule.slopes, rule.window, rule.key_begin, nullptr, nullptr, code(q.dtype()),
+                          weights ? weights->data_as<float>() : nullptr, scale_of(prior), decay, stride, ws, have, t_stream),
+                      "attention_scored failed");
+    }
+    if (weights != nullptr || prior != nullptr) return fail("attention_scored: weights come with the decode (see attention_weights)");
+    if (seq_len != S) return fail("attention_scored (prefill): seq_len must equal q.shape()[1]");
+    if (!paged && (k.shape()[0] != B || k.shape()[1] != S))
+        return fail("attention_scored (prefill): contiguous k/v must be [B, seq_len, kv_head_num, head_dim]");
+    const size_t need = ffkv_prefill_scored_workspace_bytes(code(q.dtype()), code(k.dtype()), B, S, Hq, kv_head_num, D, paged,
+                                                            max_context_blocks, max_context_len, rule.window,
+                                                            rule.key_end != nullptr);
+    void*        ws = need > 0 ? workspace(need, have) : nullptr;
+    report(ffkv_paged_prefill_scored(q.data(), output.data(), code(q.dtype()), k.data(), v.data(), code(k.dtype()),
+                                     scale_of(k_scale), scale_of(v_scale), table, context_lens, B, S, Hq, kv_head_num, D,
+                                     FFKV_BLOCK_SIZE, paged ? max_context_blocks : 0, pages, max_context_len, 0.0f, rule.cap,
+                                     rule.slopes, rule.window, rule.key_begin, rule.key_end, ws, have, t_stream),
+           "attention_scored (prefill) failed");
+}
+
+void attention_weights(const Tensor& q, const Tensor& k_cache, Tensor& weights, const Tensor* prior, float decay,
+                       const int* block_table, int kv_head_num, int max_context_blocks, const int* context_lens,
+                       const ScoreRule& rule, const Tensor* k_scale, int max_context_len)
+{
+    if (q.shape().size() != 4 || k_cache.shape().size() != 4 || !is_gpu(q) || !is_gpu(k_cache))
+        return fail("attention_weights: q must be [B, S, Hq, D] and all tensors on the GPU");
+    const int B = static_cast<int>(q.shape()[0]), S = static_cast<int>(q.shape()[1]);
+    const int Hq = static_cast<int>(q.shape()[2]), D = static_cast<int>(q.shape()[3]);
+    if (k_cache.shape()[2] != kv_head_num || k_cache.shape()[3] != D)
+        return fail("attention_weights: the cache must be [num_blocks, 16, kv_head_num, head_dim]");
+    const int64_t stride = weight_tokens(weights, B, kv_head_num);
+    if (stride < 0) return fail("attention_weights: weights must be F32 [B, kv_head_num, T] on the GPU");
+    if (prior != nullptr && weight_tokens(*prior, B, kv_head_num) != stride)
+        return fail("attention_weights: prior must be of the weights' shape");
+    const size_t need = ffkv_attention_weights_workspace_bytes(B, S, Hq, kv_head_num, D, max_context_blocks, max_context_len);
+    size_t       have = 0;
+    void*        ws = need > 0 ? workspace(need, have) : nullptr;
+    report(ffkv_attention_weights(q.data(), code(q.dtype()), k_cache.data(), code(k_cache.dtype()), scale_of(k_scale),
+                                  reinterpret_cast<const int32_t*>(block_table), context_lens, B, S, Hq, kv_head_num, D,
+                                  FFKV_BLOCK_SIZE, max_context_blocks, static_cast<int>(k_cache.shape()[0]), max_context_len,
+                                  0.0f, rule.cap, rule.slopes, rule.window, rule.key_begin, rule.key_end,
+                                  weights.data_as<float>(), scale_of(prior), decay, stride, ws, have, t_stream),
+           "attention_weights failed");
+}
+
+void evict_kv_cache(Tensor& weights, Tensor& k_cache, Tensor& v_cache, const int* block_table, const int* context_lens,
+                    int max_blocks, int keep, int sinks, int recent, Tensor& kept, Tensor& kept_lens, const int* dst_table,
+                    int dst_blocks, Tensor* weights_out, Tensor* k_scale, Tensor* v_scale)
+{
+    if (weights.shape().size() != 3 || k_cache.shape().size() != 4 || v_cache.shape() != k_cache.shape() ||
+        v_cache.dtype() != k_cache.dtype() || !is_gpu(k_cache) || !is_gpu(v_cache))
+        return fail("evict_kv_cache: weights must be [B, Hkv, T] and the caches both [num_blocks, 16, Hkv, D] on the GPU");
+    const int     B = static_cast<int>(weights.shape()[0]), H = static_cast<int>(k_cache.shape()[2]);
+    const int64_t stride = weight_tokens(weights, B, H);
+    const int64_t out_stride = weights_out ? weight_tokens(*weights_out, B, H) : 0;
+    if (stride < 0 || out_stride < 0) return fail("evict_kv_cache: weights must be F32 [B, Hkv, T] on the GPU");
+    if (!is_gpu(kept) || kept.dtype() != DType::I32 || kept.numel() < static_cast<int64_t>(B) * H * keep || !is_gpu(kept_lens) ||
+        kept_lens.dtype() != DType::I32 || kept_lens.numel() < B)
+        return fail("evict_kv_cache: kept must be I32 [B, Hkv, keep] and kept_lens I32 [B] on the GPU");
+    const size_t need = ffkv_evict_workspace_bytes(B, H, keep, stride, max_blocks);
+    size_t       have = 0;
+    void*        ws = need > 0 ? workspace(need, have) : nullptr;
+    report(ffkv_evict(weights.data_as<const float>(), stride, context_lens, keep, sinks, recent, k_cache.data(), v_cache.data(),
+                      code(k_cache.dtype()), k_scale ? k_scale->data_as<float>() : nullptr,
+                      v_scale ? v_scale->data_as<float>() : nullptr, reinterpret_cast<const int32_t*>(block_table), max_blocks,
+                      reinterpret_cast<const int32_t*>(dst_table), dst_blocks, kept.data_as<int32_t>(),
+                      kept_lens.data_as<int32_t>(), weights_out ? weights_out->data_as<float>() : nullptr, out_stride, B, H,
+                      static_cast<int>(k_cache.shape()[3]), static_cast<int>(k_cache.shape()[1]),
+                      static_cast<int>(k_cache.shape()[0]), ws, have, t_stream),
+           "evict_kv_cache failed");
+}
+
 }  // namespace firefly::kernels

@@ -128,6 +128,53 @@ FIREFLY_API void rope_append_kv_cache(Tensor& q, Tensor& k, const Tensor& v, Ten
                                       Tensor& k_scale, Tensor& v_scale, const int* block_table,
                                       const int* context_lens, int max_blocks, float theta);
 
+// ---- attention under a score rule, attention weights, eviction (no counterpart in the reference) ---------------------
+
+/**
+ * @brief How scores are changed and which keys a query sees (include/ffkv.h has the formulas).  All pointers on the device.
+ */
+struct ScoreRule
+{
+    float        cap = 0.0f;           ///< s becomes cap * tanh(s / cap); 0: not
+    const float* slopes = nullptr;     ///< [Hq]: s -= slopes[h] * distance
+    int          window = 0;           ///< keys j <= position - window are hidden; 0: none
+    const int*   key_begin = nullptr;  ///< decode [B], prefill and weights [B, S]: first visible key of each query
+    const int*   key_end = nullptr;    ///< prefill and weights [B, S]: end of the visible keys (nullptr: causal)
+};
+
+/**
+ * @brief attention() under a score rule: the decode when kv_cache_block_table is given and q is [B, 1, Hq, D]
+ * (ffkv_paged_decode_scored), else the prefill (ffkv_paged_prefill_scored); tensors as for attention(), scales for
+ * quantized caches.  With weights (decode; F32 [B, Hkv, T]) they become decay * prior plus the attention weight of every
+ * cached token (prior may be weights, or nullptr).  max_context_len bounds the rows (0: the table's width); T is at least
+ * that bound.
+ */
+FIREFLY_API void attention_scored(Tensor& q, Tensor& k, Tensor& v, Tensor& output, void* kv_cache_block_table,
+                                  int kv_head_num, int seq_len, int max_context_blocks, const int* context_lens,
+                                  const ScoreRule& rule, const Tensor* k_scale = nullptr, const Tensor* v_scale = nullptr,
+                                  Tensor* weights = nullptr, const Tensor* prior = nullptr, float decay = 1.0f,
+                                  int max_context_len = 0);
+
+/**
+ * @brief The attention weights that q [B, S, Hq, D], the rows' last S tokens, give to the cached keys
+ * (ffkv_attention_weights): weights F32 [B, Hkv, T] becomes decay * prior plus them.
+ */
+FIREFLY_API void attention_weights(const Tensor& q, const Tensor& k_cache, Tensor& weights, const Tensor* prior, float decay,
+                                   const int* block_table, int kv_head_num, int max_context_blocks,
+                                   const int* context_lens, const ScoreRule& rule, const Tensor* k_scale = nullptr,
+                                   int max_context_len = 0);
+
+/**
+ * @brief Cut the rows to their `keep` tokens of most weight (ffkv_evict): weights F32 [B, Hkv, T], context_lens the rows'
+ * tokens, kept I32 [B, Hkv, keep] and kept_lens I32 [B] are written.  dst_table [B, dst_blocks]: the kept tokens' pages
+ * (nullptr: in place, where no other row may hold the row's pages).  weights_out: nullptr, or F32 [B, Hkv, T'] that receives
+ * the kept tokens' weights (may be weights).
+ */
+FIREFLY_API void evict_kv_cache(Tensor& weights, Tensor& k_cache, Tensor& v_cache, const int* block_table,
+                                const int* context_lens, int max_blocks, int keep, int sinks, int recent, Tensor& kept,
+                                Tensor& kept_lens, const int* dst_table = nullptr, int dst_blocks = 0,
+                                Tensor* weights_out = nullptr, Tensor* k_scale = nullptr, Tensor* v_scale = nullptr);
+
 // ---- the reference's off-path operators: declared as in its include/firefly/kernels.h, defined by the caller --
 
 // Embedding lookup (reference include/firefly/kernels.h:18).
