@@ -95,6 +95,8 @@ def _load() -> ctypes.CDLL:
     rule = [f32, vp, i32]  # score_cap, slopes, window
     lib.ffkv_decode_scored_workspace_bytes.restype = sz
     lib.ffkv_decode_scored_workspace_bytes.argtypes = [i32] * 6
+    lib.ffkv_decode_scored_scratch_bytes.restype = sz
+    lib.ffkv_decode_scored_scratch_bytes.argtypes = [i32] * 10
     lib.ffkv_paged_decode_scored.restype = i32
     lib.ffkv_paged_decode_scored.argtypes = [vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
                                              i32, f32, *rule, vp, vp, vp, i32, vp, vp, f32, ctypes.c_int64, vp, sz, vp]
@@ -126,7 +128,8 @@ def _bind(lib, torch) -> None:
     """Point the native front end (``_front``, csrc/python/front.cpp) at ``lib``'s functions."""
     names = ("append", "paged_decode", "append_paged_decode", "paged_decode_shared_prefix", "paged_decode_noalloc",
              "prefill_workspace_bytes", "paged_prefill_ws", "rope", "rope_append", "paged_decode_scored",
-             "prefill_scored_workspace_bytes", "paged_prefill_scored", "evict", "attention_weights")
+             "prefill_scored_workspace_bytes", "paged_prefill_scored", "evict", "attention_weights",
+             "decode_scored_scratch_bytes", "attention_weights_workspace_bytes", "evict_workspace_bytes")
     _front.bind(tuple(ctypes.cast(getattr(lib, "ffkv_" + n), ctypes.c_void_p).value for n in names),
                 [*_torch_dtypes(torch).items(), (torch.int32, _INT32)], getattr(torch._C, "_cuda_getDevice", None),
                 getattr(torch._C, "_cuda_getCurrentRawStream", None), lambda: torch.cuda.current_stream().cuda_stream)
@@ -207,9 +210,9 @@ def paged_prefill(q, k_cache, v_cache, block_table, context_lens, out=None, k_sc
 
 def _prefill_scratch(n: int, q, stream):
     """Scratch of ``n`` bytes for one call on ``stream`` (None: the current one), from torch's allocator and belonging
-    to that stream, so that it can be reused once the call's work on the stream is done.  None, where the call
-    runs unsplit, while the stream is being captured (a capture allocates nothing here) and where there is no memory
-    for it."""
+    to that stream, so that it can be reused once the call's work on the stream is done.  None, where a prefill
+    runs unsplit and the other calls take stream-ordered memory, while the stream is being captured (a capture allocates
+    nothing here) and where there is no memory for it."""
     import torch
 
     if stream is not None:
@@ -339,7 +342,7 @@ def paged_attention_scored(q, k_cache, v_cache, block_table, context_lens, score
     out = _decode_out(q, out)
     check(_front.decode_scored(q, out, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, max_context_len, scale,
                                num_blocks, k_new, v_new, score_cap, slopes, window, key_begin, weights, prior, decay,
-                               workspace, stream))
+                               workspace, stream, _prefill_scratch))
     return out
 
 
@@ -386,7 +389,8 @@ def attention_weights(q, k_cache, block_table, context_lens, weights=None, prior
         most = min(most, max_context_len) if max_context_len > 0 else most
         weights = torch.zeros((q.shape[0], k_cache.shape[2], most), dtype=torch.float32, device=q.device)
     check(_front.attention_weights(q, k_cache, k_scale, block_table, context_lens, max_context_len, scale, num_blocks,
-                                   score_cap, slopes, window, key_begin, key_end, weights, prior, decay, workspace, stream))
+                                   score_cap, slopes, window, key_begin, key_end, weights, prior, decay, workspace, stream,
+                                   _prefill_scratch))
     return weights
 
 
@@ -415,5 +419,5 @@ def evict_tokens(weights, k_cache, v_cache, block_table, context_lens, keep: int
         if kept_lens is None:
             kept_lens = torch.empty(weights.shape[0], **like)
     check(_front.evict(weights, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, keep, sinks, recent, dst_table,
-                       kept, kept_lens, weights_out, num_blocks, workspace, stream))
+                       kept, kept_lens, weights_out, num_blocks, workspace, stream, _prefill_scratch))
     return kept, kept_lens

@@ -95,6 +95,50 @@ int prefill_span(int cap_tokens, int group, int window, bool key_end)
     return static_cast<int>(std::min<int64_t>(cap_tokens, static_cast<int64_t>(window) + 128 / group + 2 * FFKV_BLOCK_SIZE));
 }
 
+// What a scored decode launches and holds in its workspace; sizes and types of `a` are set.
+struct DecodePlan
+{
+    bool             mfma, row;
+    ffkv::MfmaLayout lay;
+    ScoreLayout      scores;
+    int64_t          need;
+};
+
+DecodePlan plan_decode(ffkv::DecodeArgs& a, int cap_tokens, int window, bool with_weights)
+{
+    DecodePlan p{};
+    a.group = a.num_heads / a.num_kv_heads;
+    p.mfma = scored_mfma(a.cache_dtype, a.head_dim);
+    a.chunk = ffkv::decode_chunk(a.batch, a.num_kv_heads, cap_tokens);
+    a.max_chunks = static_cast<int>(ceil_div(cap_tokens > 0 ? cap_tokens : 1, a.chunk));
+    // Tokens that a row's query sees at most: a window's, which may begin and end inside a page.  The plain decode's rules
+    // for the number of work items and for its one-launch form go by these.
+    const int span =
+        window > 0 ? static_cast<int>(std::min<int64_t>(cap_tokens, static_cast<int64_t>(window) + 2 * FFKV_BLOCK_SIZE))
+                   : cap_tokens;
+    a.cap_tokens = span;
+    p.row = p.mfma && ffkv::decode_use_row(a);
+    if (p.mfma) a.items = std::min(ffkv::decode_scored_launch_items(a), ffkv::decode_most_items(a.batch, span));
+    a.cap_tokens = cap_tokens;
+    if (p.mfma && !p.row)
+    {
+        p.lay = ffkv::mfma_layout(a.batch, a.num_heads, a.head_dim, 0, a.items);
+        p.need = p.lay.total;
+    }
+    else if (!p.mfma && a.max_chunks > 1)
+    {
+        const int64_t parts = static_cast<int64_t>(a.batch) * a.num_heads * a.max_chunks;
+        p.lay.acc = align256(parts * 2 * 4);
+        p.need = p.lay.acc + parts * a.head_dim * 4;
+    }
+    if (with_weights)
+    {
+        p.scores = score_layout(p.need, a.batch, a.num_heads, cap_tokens);
+        p.need = p.scores.total;
+    }
+    return p;
+}
+
 // The attention weights' workspace: the query rows' states per split of the keys, and folded.
 struct WeightLayout
 {
@@ -146,6 +190,25 @@ size_t ffkv_decode_scored_workspace_bytes(int batch, int num_heads, int head_dim
     const int cap = ffkv::decode_cap_tokens(max_blocks, max_context_len);
     if (!score_layout_fits(batch, num_heads, cap)) return 0;  // refused by the call
     return static_cast<size_t>(score_layout(static_cast<int64_t>(plain), batch, num_heads, cap).total);
+}
+
+size_t ffkv_decode_scored_scratch_bytes(int qo_dtype, int cache_dtype, int batch, int num_heads, int num_kv_heads,
+                                        int head_dim, int max_blocks, int max_context_len, int window, int with_weights)
+{
+    // sizes that ffkv_paged_decode_scored refuses need nothing
+    if (!is_act(qo_dtype) || !is_cache(cache_dtype) || !head_dim_ok(head_dim) || batch <= 0 || batch > 65535 ||
+        num_heads <= 0 || num_heads > 65535 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || max_blocks < 0 || window < 0)
+        return 0;
+    const int cap = ffkv::decode_cap_tokens(max_blocks, max_context_len);
+    if (with_weights != 0 && !score_layout_fits(batch, num_heads, cap)) return 0;
+    ffkv::DecodeArgs a{};
+    a.qo_dtype = qo_dtype;
+    a.cache_dtype = cache_dtype;
+    a.batch = batch;
+    a.num_heads = num_heads;
+    a.num_kv_heads = num_kv_heads;
+    a.head_dim = head_dim;
+    return static_cast<size_t>(plan_decode(a, cap, window, with_weights != 0).need);
 }
 
 int ffkv_paged_decode_scored(const void* q, void* out, int qo_dtype, void* k_cache, void* v_cache, int cache_dtype,
@@ -212,39 +275,14 @@ int ffkv_paged_decode_scored(const void* q, void* out, int qo_dtype, void* k_cac
     a.head_dim = head_dim;
     a.max_blocks = max_blocks;
     a.num_blocks = num_blocks;
-    a.chunk = ffkv::decode_chunk(batch, num_kv_heads, cap);
-    a.max_chunks = static_cast<int>(ceil_div(cap > 0 ? cap : 1, a.chunk));
     a.scale_log2 = softmax_scale(scale, head_dim) * kLog2e;
     a.rule = make_rule(score_cap, slopes, window, key_begin, nullptr);
 
-    // Tokens that a row's query sees at most: a window's, which may begin and end inside a page.  The plain decode's rules
-    // for the number of work items and for its one-launch form go by these.
-    const int span = window > 0 ? static_cast<int>(std::min<int64_t>(cap, static_cast<int64_t>(window) + 2 * FFKV_BLOCK_SIZE))
-                                : cap;
-    a.cap_tokens = span;
-    const bool row = mfma && ffkv::decode_use_row(a);
-    if (mfma) a.items = std::min(ffkv::decode_scored_launch_items(a), ffkv::decode_most_items(batch, span));
-    a.cap_tokens = cap;
-
-    ffkv::MfmaLayout lay{};
-    int64_t          need = 0;
-    if (mfma && !row)
-    {
-        lay = ffkv::mfma_layout(batch, num_heads, head_dim, 0, a.items);
-        need = lay.total;
-    }
-    else if (!mfma && a.max_chunks > 1)
-    {
-        const int64_t parts = static_cast<int64_t>(batch) * num_heads * a.max_chunks;
-        lay.acc = align256(parts * 2 * 4);
-        need = lay.acc + parts * head_dim * 4;
-    }
-    ScoreLayout sl{};
-    if (weights != nullptr)
-    {
-        sl = score_layout(need, batch, num_heads, cap);
-        need = sl.total;
-    }
+    const DecodePlan       plan = plan_decode(a, cap, window, weights != nullptr);
+    const ffkv::MfmaLayout lay = plan.lay;
+    const ScoreLayout      sl = plan.scores;
+    const bool             row = plan.row;
+    const int64_t          need = plan.need;
     hipStream_t s = static_cast<hipStream_t>(stream);
     void*       ws = workspace;
     bool        owned = false;

@@ -37,6 +37,9 @@ struct Functions
     decltype(&ffkv_paged_prefill_scored)       prefill_scored;
     decltype(&ffkv_evict)                      evict;
     decltype(&ffkv_attention_weights)          attention_weights;
+    decltype(&ffkv_decode_scored_scratch_bytes)       decode_scored_bytes;
+    decltype(&ffkv_attention_weights_workspace_bytes) weights_bytes;
+    decltype(&ffkv_evict_workspace_bytes)             evict_bytes;
 };
 Functions fn{};
 
@@ -404,10 +407,40 @@ void check_blocks(Reader& r, int n, PyObject* cache)
     if (r.ok && n > r.dim(cache, 0)) r.refuse(PyExc_ValueError, "num_blocks %d is more than the caches' pages", n);
 }
 
-// decode's 11, k_new, v_new, score_cap, slopes, window, key_begin, weights, prior, decay, workspace, stream
+// Scratch of `need` bytes for one call without a workspace, from `make` (bytes, like, stream) -> a tensor or None: torch's
+// allocator keeps it, where the library's stream-ordered memory is given back whenever the stream is waited for (a call that
+// is waited for: 125 us against 59 in a row).  Owned until the call has been issued.
+struct Scratch
+{
+    PyObject* t = nullptr;
+    void*     ptr = nullptr;
+    size_t    bytes = 0;
+    Scratch(Reader& r, PyObject* given, PyObject* make, size_t need, PyObject* like, PyObject* stream)
+    {
+        if (!r.ok) return;
+        if (given != Py_None)
+        {
+            t = Py_NewRef(given);
+        }
+        else if (need > 0)
+        {
+            PyObject* n = PyLong_FromSize_t(need);
+            t = n ? PyObject_CallFunctionObjArgs(make, n, like, stream, nullptr) : nullptr;
+            Py_XDECREF(n);
+            if (t == nullptr) r.ok = false;
+        }
+        if (t == nullptr) return;
+        ptr = r.ptr(t), bytes = r.nbytes(t);
+    }
+    ~Scratch() { Py_XDECREF(t); }
+    Scratch(const Scratch&) = delete;
+    Scratch& operator=(const Scratch&) = delete;
+};
+
+// decode's 11, k_new, v_new, score_cap, slopes, window, key_begin, weights, prior, decay, workspace, stream, scratch
 PyObject* decode_scored(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
-    if (!count(n, 22)) return nullptr;
+    if (!count(n, 23)) return nullptr;
     Reader     r{a};
     Decode     d(r, a);
     PyObject*  q = a[0];
@@ -445,13 +478,15 @@ PyObject* decode_scored(PyObject*, PyObject* const* a, Py_ssize_t n)
     r.current(q, d.B > 0);
     void *       k = r.ptr(a[11]), *v = r.ptr(a[12]);
     u.slopes = r.ptr<float>(a[14]), u.begin = r.ptr<int32_t>(a[16]);
-    void*        ws = r.ptr(a[20]);
-    const size_t wb = r.nbytes(a[20]);
-    void*        s = r.stream(a[21]);
+    void*         s = r.stream(a[21]);
+    const size_t  need = r.ok && a[20] == Py_None ? fn.decode_scored_bytes(d.qt, d.ct, d.B, d.Hq, d.Hkv, d.D, d.mb, d.mcl,
+                                                                           u.window, w.w != nullptr)
+                                                  : 0;
+    const Scratch ws(r, a[20], a[22], need, q, a[21]);
     return finish(r, [&] {
         return fn.decode_scored(d.q, d.out, d.qt, d.kc, d.vc, d.ct, d.ks, d.vs, d.bt, d.cx, d.B, d.Hq, d.Hkv, d.D,
                                 FFKV_BLOCK_SIZE, d.mb, d.N, d.mcl, d.scale, u.cap, u.slopes, u.window, u.begin, k, v, st,
-                                w.w, w.prior, w.decay, w.stride, ws, wb, s);
+                                w.w, w.prior, w.decay, w.stride, ws.ptr, ws.bytes, s);
     });
 }
 
@@ -572,10 +607,10 @@ PyObject* prefill_scored(PyObject*, PyObject* const* a, Py_ssize_t n)
 }
 
 // q, k_cache, k_scale, block_table, context_lens, max_context_len, scale, num_blocks, score_cap, slopes, window, key_begin,
-// key_end, weights, prior, decay, workspace, stream
+// key_end, weights, prior, decay, workspace, stream, scratch
 PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
-    if (!count(n, 18)) return nullptr;
+    if (!count(n, 19)) return nullptr;
     Reader    r{a};
     PyObject* q = a[0];
     int       B, S, Hq, D;
@@ -603,20 +638,21 @@ PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t n)
     auto* ks = r.ptr<float>(a[2]);
     auto *bt = r.ptr<int32_t>(a[3]), *cx = r.ptr<int32_t>(a[4]);
     u.slopes = r.ptr<float>(a[9]), u.begin = r.ptr<int32_t>(a[11]), u.end = r.ptr<int32_t>(a[12]);
-    void*        ws = r.ptr(a[16]);
-    const size_t wb = r.nbytes(a[16]);
-    void*        s = r.stream(a[17]);
+    void*         s = r.stream(a[17]);
+    const size_t  need = r.ok && a[16] == Py_None ? fn.weights_bytes(B, S, Hq, Hkv, D, mb, mcl) : 0;
+    const Scratch ws(r, a[16], a[18], need, q, a[17]);
     return finish(r, [&] {
         return fn.attention_weights(qp, qt, kc, ct, ks, bt, cx, B, S, Hq, Hkv, D, FFKV_BLOCK_SIZE, mb, N, mcl, scale, u.cap,
-                                    u.slopes, u.window, u.begin, u.end, w.w, w.prior, w.decay, w.stride, ws, wb, s);
+                                    u.slopes, u.window, u.begin, u.end, w.w, w.prior, w.decay, w.stride, ws.ptr, ws.bytes,
+                                    s);
     });
 }
 
 // weights, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, keep, sinks, recent, dst_table, kept,
-// kept_lens, weights_out, num_blocks, workspace, stream
+// kept_lens, weights_out, num_blocks, workspace, stream, scratch
 PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
-    if (!count(n, 17)) return nullptr;
+    if (!count(n, 18)) return nullptr;
     Reader    r{a};
     PyObject* w = a[0];
     const int B = r.dim(w, 0), Hkv = r.dim(a[1], 2), D = r.dim(a[1], 3), ct = r.dtype(a[1]);
@@ -646,12 +682,12 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n)
     auto *bt = r.ptr<int32_t>(a[5]), *cx = r.ptr<int32_t>(a[6]), *dt = r.ptr<int32_t>(a[10]), *kp = r.ptr<int32_t>(a[11]),
          *kl = r.ptr<int32_t>(a[12]);
     r.plain(a[15], "workspace", w);
-    void*        ws = r.ptr(a[15]);
-    const size_t wb = r.nbytes(a[15]);
-    void*        s = r.stream(a[16]);
+    void*         s = r.stream(a[16]);
+    const size_t  need = r.ok && a[15] == Py_None ? fn.evict_bytes(B, Hkv, keep, stride, mb) : 0;
+    const Scratch ws(r, a[15], a[17], need, w, a[16]);
     return finish(r, [&] {
         return fn.evict(wp, stride, cx, keep, sinks, recent, kc, vc, ct, ks, vs, bt, mb, dt, db, kp, kl, wo, ostride, B, Hkv,
-                        D, FFKV_BLOCK_SIZE, N, ws, wb, s);
+                        D, FFKV_BLOCK_SIZE, N, ws.ptr, ws.bytes, s);
     });
 }
 

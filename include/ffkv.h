@@ -294,12 +294,18 @@ FFKV_API int ffkv_rope_append(void* q, void* k, const void* v, int src_dtype, vo
  *                  max_context_len, are left as they were.  weight_stride is at least min(max_blocks * 16,
  *                  max_context_len); decay is finite and not negative.
  * q, out, caches, scales, tables, sizes, scale and errors as for ffkv_paged_decode; positions and distances count the
- * row's cached tokens.  With weights the workspace holds the scores of all visible keys (4 bytes per query head and token
+ * row's cached tokens.  ffkv_decode_scored_workspace_bytes is enough for every type, KV head count and window at these
+ * sizes; ffkv_decode_scored_scratch_bytes is what the one call needs (0 for small batches, which take one launch).  With
+ * weights the workspace holds the scores of all visible keys (4 bytes per query head and token
  * of the bound on a row): give max_context_len where the block table is wide.  workspace NULL: stream-ordered memory.
  * The calls that share a workspace must not overlap in time.
  */
 FFKV_API size_t ffkv_decode_scored_workspace_bytes(int batch, int num_heads, int head_dim, int max_blocks,
                                                    int max_context_len, int with_weights);
+
+FFKV_API size_t ffkv_decode_scored_scratch_bytes(int qo_dtype, int cache_dtype, int batch, int num_heads, int num_kv_heads,
+                                                 int head_dim, int max_blocks, int max_context_len, int window,
+                                                 int with_weights);
 
 FFKV_API int ffkv_paged_decode_scored(const void* q, void* out, int qo_dtype, void* k_cache, void* v_cache,
                                       int cache_dtype, float* k_scale, float* v_scale, const int32_t* block_table,

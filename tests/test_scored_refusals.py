@@ -53,6 +53,14 @@ def test_decode_workspace_bytes(ff):
     assert f(4, 32, 128, 600, 0, 0) == plain
     assert f(4, 32, 128, 600, 0, 1) >= plain + 4 * 32 * 9600 * 4
     assert f(4, 32, 128, 600, 100, 1) < f(4, 32, 128, 600, 0, 1)
+    g = ff.lib.ffkv_decode_scored_scratch_bytes
+    for types in ((ff.DTYPE_BF16, ff.DTYPE_BF16), (ff.DTYPE_F32, ff.DTYPE_F32), (ff.DTYPE_BF16, ff.DTYPE_I8)):
+        for B, Hq, Hkv, D, mb, window in ((4, 32, 8, 128, 600, 0), (4, 32, 8, 128, 600, 100), (70, 8, 8, 64, 33, 0),
+                                          (1, 16, 1, 256, 9000, 0), (3, 4, 2, 72, 700, 50)):
+            for w in (0, 1):
+                assert g(*types, B, Hq, Hkv, D, mb, 0, window, w) <= f(B, Hq, D, mb, 0, w)
+    assert g(ff.DTYPE_BF16, ff.DTYPE_BF16, 2, 8, 8, 128, 8, 0, 0, 0) == 0  # one launch, no partials
+    assert g(ff.DTYPE_BF16, ff.DTYPE_BF16, 2, 8, 3, 128, 8, 0, 0, 1) == 0 and g(3, 2, 2, 8, 8, 128, 8, 0, 0, 1) == 0
     assert f(0, 32, 128, 600, 0, 1) == 0 and f(65535, 65535, 128, 1 << 26, 0, 1) == 0
 
 
