@@ -96,8 +96,8 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
     constexpr int  KSTEPS = D / 32;
     constexpr bool KT = D % 32 == 16;  // a last k-step of 16 dims
     constexpr int  DT = 32 * KSTEPS;
-    // int8 beside a bf16 q: f16 products with q converted whole (8 significant bits in 11), scaled by a power of two into
-    // f16's range where a staged block holds values of 2^15 and more
+    // int8 beside a bf16 q: f16 products with q converted whole (8 significant bits in 11), each row scaled by a power of two
+    // into f16's range where one of its tile holds values of 2^15 and more
     constexpr bool QX16 = CT == I8 && QT == BF16;
     constexpr bool LO = kAwLo<CT, QT>;
     constexpr int  KP = kAwPages;
@@ -140,10 +140,8 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
     float factor = a.rule.cap > 0.0f ? a.scale_log2 * a.rule.inv_cap : a.scale_log2;
     if constexpr (CT == FP8) factor *= a.k_scale[kvh];
 
-    __shared__ uint32_t s_most;  // QX16: the largest |q| of the block
-    float q_unscale = 1.0f;      // the products come out scaled by 1 / q_unscale
     // A wave stages whole tiles of 16 query rows: lane (c, g) row c's dims dimof(j, g) .. of every k-step.
-    auto stage_q = [&](int rb, float qs, float& most)
+    auto stage = [&](int rb)
     {
         const int r0 = rb * rows;
         const int tiles = (min(rows, R - r0) + 15) / 16;
@@ -161,89 +159,103 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
             const int    r = r0 + tile * 16 + c;
             const int    t = r / G, h = r - t * G;
             const size_t at = ((static_cast<size_t>(b) * a.seq_len + t) * a.num_heads + kvh * G + h) * D;
+            float        most = 0.0f;  // QX16: the largest |q| of the lane's dims
+            auto stage_tile = [&](float qs)
+            {
+                u32x4* dst = s_q + tile * NP * KSTEPS * 64 + lane;
+#pragma unroll
+                for (int j = 0; j < KSTEPS; ++j)
+                {
+                    u32x4 hi = u32x4{0u, 0u, 0u, 0u}, lo = hi;
+                    if (r < R)
+                    {
+                        if constexpr (QX16)
+                        {
+                            float    x[8];
+                            uint32_t w[4];
+                            load_q8<QT>(a.q, at + dimof(j, g), x);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                            {
+                                most = fmaxf(most, fmaxf(__builtin_fabsf(x[2 * e]), __builtin_fabsf(x[2 * e + 1])));
+                                w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x[2 * e] * qs, x[2 * e + 1] * qs}, h2));
+                            }
+                            hi = u32x4{w[0], w[1], w[2], w[3]};
+                        }
+                        else if constexpr (!LO)
+                            hi = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at + dimof(j, g));
+                        else
+                        {
+                            float    x[8];
+                            uint32_t p[8], w[8];
+                            load_q8<QT>(a.q, at + dimof(j, g), x);
+                            parts(x, p, w);
+                            hi = u32x4{p[0] | (p[1] << 16), p[2] | (p[3] << 16), p[4] | (p[5] << 16), p[6] | (p[7] << 16)};
+                            lo = u32x4{w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16), w[6] | (w[7] << 16)};
+                        }
+                    }
+                    dst[j * 64] = hi;
+                    if constexpr (LO) dst[(KSTEPS + j) * 64] = lo;
+                }
+                if constexpr (KT)
+                {
+                    float    x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    uint32_t p[4], w[4];
+                    if (r < R) load_act4(a.q, QT, at + DT + 4 * g, x);
+                    if constexpr (QX16)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                        {
+                            most = fmaxf(most, __builtin_fabsf(x[e]));
+                            x[e] *= qs;
+                        }
+                    parts(x, p, w);
+                    s_qt[tile * NP * 64 + lane] = u32x2{p[0] | (p[1] << 16), p[2] | (p[3] << 16)};
+                    if constexpr (LO) s_qt[(tile * NP + 1) * 64 + lane] = u32x2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)};
+                }
+            };
+            stage_tile(1.0f);
+            float unscale = 1.0f;
+            if constexpr (QX16)
+                if (__any(most >= 32768.0f))  // rare: again, every row scaled by its largest finite value
+                {
+                    float fin = 0.0f;
+                    auto  take = [&](float x)
+                    { fin = fmaxf(fin, __builtin_fabsf(x) < __builtin_huge_valf() ? __builtin_fabsf(x) : 0.0f); };
+                    if (r < R)
+                    {
+#pragma unroll 1
+                        for (int j = 0; j < KSTEPS; ++j)
+                        {
+                            float x[8];
+                            load_q8<QT>(a.q, at + dimof(j, g), x);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) take(x[e]);
+                        }
+                        if constexpr (KT)
+                        {
+                            float x[4];
+                            load_act4(a.q, QT, at + DT + 4 * g, x);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) take(x[e]);
+                        }
+                    }
+                    fin = fmaxf(fin, __shfl_xor(fin, 16, 64));
+                    fin = fmaxf(fin, __shfl_xor(fin, 32, 64));
+                    const int e = max(0, __builtin_amdgcn_frexp_expf(fin) - 15);
+                    unscale = __builtin_ldexpf(1.0f, e);
+                    stage_tile(__builtin_ldexpf(1.0f, -e));
+                }
             if (g == 0)
             {
                 const int3 vis = r < R ? aw_visible(a, b, ctx, total, t) : make_int3(0, 0, 0);
-                s_vis[tile * 16 + c] = make_int4(vis.x, vis.y, vis.z, 0);
+                s_vis[tile * 16 + c] = make_int4(vis.x, vis.y, vis.z, __builtin_bit_cast(int, unscale));
                 s_slope[tile * 16 + c] = r < R && a.rule.slopes != nullptr ? a.rule.slopes[kvh * G + h] * 1.4426950408889634f : 0.0f;
                 if constexpr (SUM)
                     s_ml[tile * 16 + c] = r < R ? a.fin[static_cast<int64_t>(bh) * R + r] : make_float2(0.0f, 0.0f);
             }
-            u32x4* dst = s_q + tile * NP * KSTEPS * 64 + lane;
-#pragma unroll
-            for (int j = 0; j < KSTEPS; ++j)
-            {
-                u32x4 hi = u32x4{0u, 0u, 0u, 0u}, lo = hi;
-                if (r < R)
-                {
-                    if constexpr (QX16)
-                    {
-                        float    x[8];
-                        uint32_t w[4];
-                        load_q8<QT>(a.q, at + dimof(j, g), x);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                        {
-                            most = fmaxf(most, fmaxf(__builtin_fabsf(x[2 * e]), __builtin_fabsf(x[2 * e + 1])));
-                            w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x[2 * e] * qs, x[2 * e + 1] * qs}, h2));
-                        }
-                        hi = u32x4{w[0], w[1], w[2], w[3]};
-                    }
-                    else if constexpr (!LO)
-                        hi = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at + dimof(j, g));
-                    else
-                    {
-                        float    x[8];
-                        uint32_t p[8], w[8];
-                        load_q8<QT>(a.q, at + dimof(j, g), x);
-                        parts(x, p, w);
-                        hi = u32x4{p[0] | (p[1] << 16), p[2] | (p[3] << 16), p[4] | (p[5] << 16), p[6] | (p[7] << 16)};
-                        lo = u32x4{w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16), w[6] | (w[7] << 16)};
-                    }
-                }
-                dst[j * 64] = hi;
-                if constexpr (LO) dst[(KSTEPS + j) * 64] = lo;
-            }
-            if constexpr (KT)
-            {
-                float    x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t p[4], w[4];
-                if (r < R) load_act4(a.q, QT, at + DT + 4 * g, x);
-                if constexpr (QX16)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                    {
-                        most = fmaxf(most, __builtin_fabsf(x[e]));
-                        x[e] *= qs;
-                    }
-                parts(x, p, w);
-                s_qt[tile * NP * 64 + lane] = u32x2{p[0] | (p[1] << 16), p[2] | (p[3] << 16)};
-                if constexpr (LO) s_qt[(tile * NP + 1) * 64 + lane] = u32x2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)};
-            }
         }
-        return tiles;
-    };
-    auto stage = [&](int rb)
-    {
-        float     most = 0.0f;
-        const int tiles = stage_q(rb, 1.0f, most);
-        if constexpr (QX16)
-        {
-            if (tid == 0) s_most = 0;
-            if (__syncthreads_or(most >= 32768.0f) != 0)  // rare: again, scaled
-            {
-                atomicMax(&s_most, f2u(most));  // (NaN is not among them: fmaxf passes it over)
-                __syncthreads();
-                const int e = __builtin_amdgcn_frexp_expf(u2f(s_most));
-                stage_q(rb, __builtin_ldexpf(1.0f, 15 - e), most);
-                q_unscale = __builtin_ldexpf(1.0f, e - 15);
-                __syncthreads();
-            }
-            else
-                q_unscale = 1.0f;
-        }
-        else
-            __syncthreads();
+        __syncthreads();
         return tiles;
     };
 
@@ -395,9 +407,9 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
 #pragma unroll
                 for (int e = 0; e < KP * 4; ++e) v[e] = s[e >> 2][e & 3] * (CT == I8 ? ks[e >> 2][e & 3] : factor);
                 if constexpr (QX16)
-                    if (q_unscale != 1.0f)  // uniform, rare
+                    if (__any(vis.w != 0x3f800000))  // rare: the row's scale of q
 #pragma unroll
-                        for (int e = 0; e < KP * 4; ++e) v[e] *= q_unscale;
+                        for (int e = 0; e < KP * 4; ++e) v[e] *= __builtin_bit_cast(float, vis.w);
                 if (a.rule.cap > 0.0f) cap_scores<KP * 4>(v, a.rule.cap);
                 if (a.rule.slopes != nullptr)
                 {
@@ -726,6 +738,7 @@ hipError_t launch_attention_weights(const WeightArgs& a, bool mfma, hipStream_t 
         if (a.cache_dtype == I8) return launch_vector<I8>(a, sum, n, stream);
         return launch_vector<FP8>(a, sum, n, stream);
     };
+    if (R == 0) return pass(true);  // no queries: the earlier weights' decay alone
     hipError_t e = pass(false);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(attention_weights_fold, dim3(static_cast<unsigned>(bh * ((R + 15) / 16))), dim3(256), 0, stream, a);

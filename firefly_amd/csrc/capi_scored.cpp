@@ -35,8 +35,9 @@ ffkv::ScoreRule make_rule(float score_cap, const float* slopes, int window, cons
 {
     ffkv::ScoreRule r{};
     r.cap = score_cap * kLog2e;  // the kernels' scores are in log2 units
-    r.inv_cap = score_cap > 0.0f ? 1.0f / r.cap : 0.0f;
-    if (!std::isfinite(r.cap) || !std::isfinite(r.inv_cap)) r.cap = r.inv_cap = 0.0f;  // beyond fp32: no score reaches it
+    if (score_cap > 0.0f) r.cap = std::max(r.cap, 1e-30f);  // (its inverse stays far from infinity; below it all scores are as good as 0)
+    if (!std::isfinite(r.cap)) r.cap = 0.0f;                // beyond fp32: no score reaches it
+    r.inv_cap = r.cap > 0.0f ? 1.0f / r.cap : 0.0f;
     r.window = window;
     r.slopes = slopes;
     r.key_begin = key_begin;
@@ -482,8 +483,8 @@ int ffkv_attention_weights(const void* q, int qo_dtype, const void* k_cache, int
         return fail(FFKV_ERR_UNSUPPORTED, "seq_len * group must be <= 2^20");
     if (const int rc = check_rule(score_cap, slopes, window, key_begin, key_end)) return rc;
     const int cap = ffkv::decode_cap_tokens(max_blocks, max_context_len);
-    if (batch == 0 || seq_len == 0) return ok();
-    if (!q || !k_cache || !block_table || !context_lens || !weights)
+    if (batch == 0) return ok();
+    if ((seq_len > 0 && !q) || !k_cache || !block_table || !context_lens || !weights)
         return fail(FFKV_ERR_INVALID_ARGUMENT, "null q, cache, block_table, context_lens or weights pointer");
     if (const int rc = check_weights(weights, prior, decay, weight_stride, cap)) return rc;
     if (quantized(cache_dtype) && !k_scale) return fail(FFKV_ERR_INVALID_ARGUMENT, "quantized cache needs k_scale");
@@ -498,7 +499,7 @@ int ffkv_attention_weights(const void* q, int qo_dtype, const void* k_cache, int
     if (ws != nullptr && workspace_bytes < static_cast<size_t>(lay.total))
         return fail(FFKV_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %lld bytes needed", workspace_bytes,
                     static_cast<long long>(lay.total));
-    if (ws == nullptr)
+    if (ws == nullptr && lay.total > 0)
     {
         const hipError_t e = hipMallocAsync(&ws, static_cast<size_t>(lay.total), s);
         if (e != hipSuccess) return hip_fail(e, "attention weights workspace hipMallocAsync");
@@ -530,7 +531,7 @@ int ffkv_attention_weights(const void* q, int qo_dtype, const void* k_cache, int
     a.decay = decay;
     a.weight_stride = weight_stride;
     hipError_t e = ffkv::launch_attention_weights(a, scored_mfma(cache_dtype, head_dim), s);
-    if (workspace == nullptr)
+    if (workspace == nullptr && ws != nullptr)
     {
         const hipError_t fe = hipFreeAsync(ws, s);
         if (e == hipSuccess) e = fe;
@@ -577,6 +578,8 @@ int ffkv_evict(const float* weights, int64_t weight_stride, const int32_t* conte
         return fail(FFKV_ERR_INVALID_ARGUMENT, "null weights, context_lens, cache, block_table, kept or kept_lens pointer");
     if (kept_lens == context_lens)
         return fail(FFKV_ERR_INVALID_ARGUMENT, "kept_lens must not be context_lens");
+    if (dst_table == block_table)
+        return fail(FFKV_ERR_INVALID_ARGUMENT, "dst_table must not be block_table: NULL moves within the rows' own pages");
     if (cache_dtype == FFKV_DTYPE_I8 && (!k_scale || !v_scale))
         return fail(FFKV_ERR_INVALID_ARGUMENT, "int8 cache needs k_scale and v_scale");
     if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))

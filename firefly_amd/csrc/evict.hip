@@ -60,6 +60,9 @@ __device__ __forceinline__ void write_kept(const float (&x)[PER], int t0, int n,
         const uint64_t bs = __ballot(s), be = __ballot(e);
         if (lane == 0) s_cnt[k * kSelWaves + wave] = __popcll(bs) | (__popcll(be) << 16);
     }
+    // Weights in place: every wave has its tokens' before any wave writes over them.  (A barrier waits for LDS alone, and the
+    // weights of a wave at the row's ends, which no comparison has needed, may still be on their way.)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     // exclusive sums over the stretches in order, kPerLane per lane of the first wave
     if (wave == 0)

@@ -275,7 +275,7 @@ FFKV_API int ffkv_rope_append(void* q, void* k, const void* v, int src_dtype, vo
 /*
  * ---- attention under a score rule --------------------------------------------------------------------------------
  * For the query at position i, head h and the key at position j, with s = scale * q.k:
- *   score_cap  > 0: s becomes score_cap * tanh(s / score_cap); 0: left as it is
+ *   score_cap  > 0: s becomes score_cap * tanh(s / score_cap) (caps below 7e-31 as 7e-31); 0: left as it is
  *   slopes     fp32 [num_heads], not NULL: s becomes s - slopes[h] * |i - j| (after the cap); finite values
  *   window     > 0: keys j <= i - window are hidden (a query sees its own and the window - 1 positions before it)
  *   key_begin  int32, not NULL: keys before key_begin of the query are hidden
@@ -348,7 +348,7 @@ FFKV_API int ffkv_paged_prefill_scored(const void* q, void* out, int qo_dtype, c
  *   weights[b, kvh, j] = sum of softmax(s)_j                               the seq_len tokens' own keys
  * weights and prior as for ffkv_paged_decode_scored, which gives the same for single tokens beside the attention itself;
  * this call reads no V and writes no output: the prompt's part of what ffkv_evict goes by (the last 16 to 64 tokens of a
- * prompt, a few queries of a chunk).  Caches, head dims and GQA groups as for ffkv_paged_decode_scored, any group size.
+ * prompt, a few queries of a chunk).  seq_len 0: the earlier weights' decay alone.  Caches, head dims and GQA groups as for ffkv_paged_decode_scored, any group size.
  * Workspace: ffkv_attention_weights_workspace_bytes, or NULL for stream-ordered memory; calls that share one must not
  * overlap in time.  No counterpart in the reference.
  */
@@ -373,7 +373,8 @@ FFKV_API int ffkv_attention_weights(const void* q, int qo_dtype, const void* k_c
  *              count are left as they were)
  *   kept_lens  int32 [batch]: min(context_lens[b], keep), the row's tokens from now on; not context_lens itself
  *   K and V (and int8 scales) of kept token number j go to position j of the row in dst_table int32 [batch, dst_blocks],
- *              pages of the same pools that no row of the call holds tokens in (pages shared with other rows stay whole);
+ *              pages of the same pools that no row of the call holds tokens in (pages shared with other rows stay whole;
+ *              block_table itself is refused);
  *              dst_table NULL: to position j of the row's own pages, which no other row may hold then
  *   weights_out fp32 [batch, num_kv_heads, out_stride], NULL or weights itself (with its stride) or apart from it: the kept
  *              tokens' weights at their new positions, the rest left as it was

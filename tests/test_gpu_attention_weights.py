@@ -124,6 +124,50 @@ def test_cut_and_absent(ff, gpu, kv):
     check(c, call(ff, c, su.device(c, gpu), r, weights=w, max_context_len=310), expected(c, r, 310), left=5)
 
 
+@pytest.mark.parametrize("kv,D", [("bf16", 128), ("i8", 112), ("fp8", 64), ("f32", 40)])
+def test_no_queries(ff, gpu, kv, D):
+    """No tokens: what the rows have decays, whether or not anything earlier is given."""
+    c = make(19, [300, 0, 17, -4], 1, 4, 2, D, "f32" if kv == "f32" else "bf16", kv)
+    d = list(su.device(c, gpu))
+    d[8] = d[8][:, :0]
+    r = rule_of(c, **RULES["plain"])
+    prior = torch.rand(4, 2, 310, device=gpu)
+    for given in (prior, None):
+        w = call(ff, c, d, r, weights=torch.full_like(prior, 3.0), prior=given, decay=0.25, max_context_len=310)
+        for b, n in enumerate(c.ctx):
+            n = max(int(n), 0)
+            assert torch.equal(w[b, :, :n], prior[b, :, :n] * 0.25 if given is not None else torch.zeros_like(w[b, :, :n]))
+            assert (w[b, :, n:] == 3.0).all()
+
+
+@pytest.mark.parametrize("D", [64, 112, 128, 256])
+def test_large_queries_int8(ff, gpu, D):
+    """bf16 queries over int8 keys, far beyond fp16's range, infinite and ordinary ones side by side in two tiles of 16 rows:
+    each one's weights are its own.  (Every query has ten keys of its own; beyond the cap any score weighs as the cap, and
+    the rows that are too large for a bound on their scores still give every head's weights a sum of 1.)"""
+    c = make(21, [200], 16, 2, 1, D, "bf16", "i8")
+    q = cases.decode(c.q, c.act)
+    q[0, 3] *= np.float32(2.0 ** 20)
+    q[0, 4] *= np.float32(2.0 ** -10)
+    q[0, 5] *= np.float32(2.0 ** 60)
+    c.q = cases.encode(q, c.act)
+    r = dict(rule_of(c, cap=6.0), begin=10 * np.arange(16, dtype=np.int32)[None], end=10 * np.arange(1, 17, dtype=np.int32)[None])
+    small = r["end"].copy()
+    small[0, [3, 5]] = 0
+    (want, bound), = expected(c, dict(r, end=small))
+    for infinite in (False, True):
+        if infinite:
+            c.q[0, 6, :, 2] = su.INF[c.act]
+        got = su.host(call(ff, c, su.device(c, gpu), r))[0, 0]
+        for t in range(16):
+            at = slice(10 * t, 10 * t + 10)
+            if t in (3, 5):
+                assert abs(got[at].sum() - 2) <= 2.0 ** -14
+            elif not (infinite and t == 6):
+                su.check(got[at], want[0, at], bound[0, at], f"query {t}")
+        assert (got[160:] == 0).all()
+
+
 def test_as_the_decode(ff, gpu):
     """One query per row: the weights of the scored decode."""
     c = make(13, [2000, 3, 450], 1, 8, 2, 128)

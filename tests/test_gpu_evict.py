@@ -129,6 +129,13 @@ def test_long_rows(ff, gpu, n, kind, in_place):
     run(ff, c, 4099, 17, 1000, in_place, "in place" if kind == "zeros" else "apart")
 
 
+@pytest.mark.parametrize("n,hkv", [(4000, 3), (8100, 2), (9000, 256)])
+def test_wide_ends_in_place(ff, gpu, n, hkv):
+    """Rows mostly of their first and last tokens, the weights in place, in every number of weights a thread holds."""
+    c = Cache(10, [n], n - 100, hkv, 8, "fp8", gpu, kind="positive")
+    run(ff, c, n - 100, n // 4, n // 2, True, "in place")
+
+
 def test_bounds(ff, gpu):
     """Lengths beyond the table or the weights, a destination with too few pages, absent pages, fewer blocks than the
     pool has: nothing else is touched."""

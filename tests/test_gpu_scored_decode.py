@@ -195,6 +195,15 @@ def test_scores_past_the_cap(ff, gpu):
             assert np.abs(out[b, h] - o).max() <= 2.0 ** -8 * np.abs(o).max() + 1e-4
 
 
+@pytest.mark.parametrize("kv", ["bf16", "i8", "f32"])
+def test_smallest_cap(ff, gpu, kv):
+    """A cap of next to nothing leaves all keys the same weight."""
+    c = make(21, [100, 700], 4, 2, 128, "f32" if kv == "f32" else "bf16", kv)
+    for cap in (1e-44, 1e-38, 1e-20):
+        r = rule_of(c, cap=cap)
+        check_out(c, call(ff, c, su.device(c, gpu), r), expected(c, dict(r, cap=1e-20)))
+
+
 def test_streams_graph_and_workspace(ff, gpu):
     """A captured step replays to the same as an eager one, with eager calls in between; a workspace and a stream of the
     caller's give the same bits."""

@@ -182,6 +182,7 @@ def _evict(ff, **kw):
     (dict(weights_out=16, out_stride=65), -1), (dict(weights=None), -1), (dict(kept=None), -1), (dict(kept_lens=None), -1),
     (dict(kept_lens=16), -1), (dict(cache_dtype=3), -1), (dict(k_cache=24), -1), (dict(weights=18), -1), (dict(kept=18), -1),
     (dict(weight_stride=-1), -1), (dict(weight_stride=1 << 40, max_blocks=2 ** 31 - 1), -2), (dict(dst_blocks=-1), -1),
+    (dict(dst_table=16, dst_blocks=4), -1),
     (dict(workspace=8), -1), (dict(workspace=256, workspace_bytes=100, weight_stride=1 << 20, max_blocks=9000), -3),
 ])
 def test_evict_rejects(ff, kw, code):
@@ -236,7 +237,7 @@ def _weights(ff, **kw):
 def test_weights_rejects(ff, kw, code):
     assert _weights(ff, **kw) == code
     assert ff.lib.ffkv_last_error().decode() != ""
-    assert _weights(ff, batch=0, q=None) == 0 and _weights(ff, seq_len=0, q=None) == 0
+    assert _weights(ff, batch=0, q=None) == 0
 
 
 def test_weights_front(ff):
