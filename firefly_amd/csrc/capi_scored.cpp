@@ -105,7 +105,7 @@ struct DecodePlan
     int64_t          need;
 };
 
-DecodePlan plan_decode(ffkv::DecodeArgs& a, int cap_tokens, int window, bool with_weights)
+DecodePlan plan_decode(ffkv::ScoredDecodeArgs& a, int cap_tokens, int window, bool with_weights)
 {
     DecodePlan p{};
     a.group = a.num_heads / a.num_kv_heads;
@@ -202,7 +202,7 @@ size_t ffkv_decode_scored_scratch_bytes(int qo_dtype, int cache_dtype, int batch
         return 0;
     const int cap = ffkv::decode_cap_tokens(max_blocks, max_context_len);
     if (with_weights != 0 && !score_layout_fits(batch, num_heads, cap)) return 0;
-    ffkv::DecodeArgs a{};
+    ffkv::ScoredDecodeArgs a{};
     a.qo_dtype = qo_dtype;
     a.cache_dtype = cache_dtype;
     a.batch = batch;
@@ -258,7 +258,7 @@ int ffkv_paged_decode_scored(const void* q, void* out, int qo_dtype, void* k_cac
         return fail(FFKV_ERR_UNSUPPORTED, "the scores of %d x %d rows of %d tokens are too many: give max_context_len",
                     batch, num_heads, cap);
 
-    ffkv::DecodeArgs a{};
+    ffkv::ScoredDecodeArgs a{};
     a.q = q;
     a.out = out;
     a.k_cache = k_cache;

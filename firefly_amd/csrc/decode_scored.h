@@ -26,7 +26,7 @@ constexpr int scored_row_lds(int heads)
 
 template <int CT, int QT, int D, bool SCORES>
 __global__ __launch_bounds__((64 * kMfmaMaxWaves<CT, D>)) __attribute__((amdgpu_waves_per_eu(kMfmaWaves<CT, QT, D>, 8)))
-void paged_decode_scored(DecodeArgs a)
+void paged_decode_scored(ScoredDecodeArgs a)
 {
     __shared__ uint16_t s_v[kMfmaMaxWaves<CT, D> * kBlockSize * D];
     decode_wg<CT, QT, D, false, false, true, SCORES>(a, static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.y),
@@ -35,7 +35,7 @@ void paged_decode_scored(DecodeArgs a)
 
 template <int CT, int QT, int D, bool SCORES>
 __global__ __launch_bounds__(64 * kScoredRowWaves) __attribute__((amdgpu_waves_per_eu(2, 8)))
-void paged_decode_scored_row(DecodeArgs a)
+void paged_decode_scored_row(ScoredDecodeArgs a)
 {
     extern __shared__ __align__(16) uint8_t s_scored_row[];
     decode_wg<CT, QT, D, false, true, true, SCORES>(a, static_cast<int>(blockIdx.y), static_cast<int>(blockIdx.x), 0,
@@ -46,14 +46,14 @@ namespace
 {
 
 template <int CT, int QT, int D>
-int scored_items3(const DecodeArgs& a)
+int scored_items3(const ScoredDecodeArgs& a)
 {
     const MfmaShape sh = mfma_shape<CT, D>(a);
     return decode_mfma_items(reinterpret_cast<const void*>(paged_decode_scored<CT, QT, D, false>), 64 * sh.nw, sh.gy);
 }
 
 template <int CT, int QT, int D, bool SCORES>
-hipError_t launch_scored3(const DecodeArgs& a, bool row, hipStream_t stream)
+hipError_t launch_scored3(const ScoredDecodeArgs& a, bool row, hipStream_t stream)
 {
     if (row)
     {
@@ -73,7 +73,7 @@ hipError_t launch_scored3(const DecodeArgs& a, bool row, hipStream_t stream)
 
 // f.operator()<CT, QT, D>() for the call's types and head_dim.
 template <typename F>
-auto scored_for(const DecodeArgs& a, F f)
+auto scored_for(const ScoredDecodeArgs& a, F f)
 {
     auto d = [&]<int CT, int QT>()
     {

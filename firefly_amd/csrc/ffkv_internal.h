@@ -155,9 +155,14 @@ struct DecodeArgs
     // tokens of rows cut short by cap_tokens).
     const void*    k_new;
     const void*    v_new;
-    // Scored decode only (launch_decode_scored): the rule; with weights, the scores of all visible keys in log2 units,
-    // fp32 (score_page of score_rule.h; score_stride tokens per row), each row's final (max, denominator) per head, [batch, num_heads, 2], and the
-    // weights themselves (decay * prior + what this call gives), [batch, num_kv_heads, weight_stride].
+};
+
+// The decode under a score rule (launch_decode_scored): the rule; with weights, the scores of all visible keys in log2 units,
+// fp32 (score_page of score_rule.h; score_stride tokens per row), each row's final (max, denominator) per head,
+// [batch, num_heads, 2], and the weights themselves (decay * prior + what this call gives), [batch, num_kv_heads,
+// weight_stride].  (A type of its own: 96 bytes more of arguments cost the plain decode of a few rows 0.3 of 7 us.)
+struct ScoredDecodeArgs : DecodeArgs
+{
     ScoreRule      rule;
     float*         ws_scores;  // null: no weights
     float*         ws_final;
@@ -276,11 +281,11 @@ hipError_t launch_decode_row(const DecodeArgs& a, hipStream_t stream);
 bool decode_use_mfma(int cache_dtype, int group, int head_dim);
 // The decode under a score rule (paged_decode_scored.hip): `mfma` as the plain decode is chosen, `row` its one-launch form
 // (16- and 8-bit caches at the matrix cores' head dims, else the vector kernel), and the work items of the former.
-int        decode_scored_launch_items(const DecodeArgs& a);
-hipError_t launch_decode_scored(const DecodeArgs& a, bool mfma, bool row, hipStream_t stream);
-hipError_t launch_decode_scored_generic(const DecodeArgs& a, hipStream_t stream);
-hipError_t launch_decode_scores(const DecodeArgs& a, bool row, hipStream_t stream);  // with the scores written down
-hipError_t launch_decode_weights(const DecodeArgs& a, hipStream_t stream);  // the weights from them
+int        decode_scored_launch_items(const ScoredDecodeArgs& a);
+hipError_t launch_decode_scored(const ScoredDecodeArgs& a, bool mfma, bool row, hipStream_t stream);
+hipError_t launch_decode_scored_generic(const ScoredDecodeArgs& a, hipStream_t stream);
+hipError_t launch_decode_scores(const ScoredDecodeArgs& a, bool row, hipStream_t stream);  // with the scores written down
+hipError_t launch_decode_weights(const ScoredDecodeArgs& a, hipStream_t stream);  // the weights from them
 
 // Fused shared-prefix decode (paged_decode_pfx.hip): the prefix partials and the decode of the rows' own pages in
 // one grid, then the merge.  decode_pfx_plan sizes it for `a` (dtypes, batch, heads, head_dim set) over

@@ -83,7 +83,7 @@ __device__ __forceinline__ int row_tokens(const DecodeArgs& a, int b)
 // (DT / 8 when DT is given).  Lanes past head_dim / 8 hold zeros and store nothing.  RULE: the scores are changed and the
 // keys bounded by a.rule, and with a.ws_scores the scores and the rows' final states are written down for the weights.
 template <int CT, int DT, int LPT, int GP, bool RULE = false>
-__global__ __launch_bounds__(256) void paged_decode_generic(DecodeArgs a)
+__global__ __launch_bounds__(256) void paged_decode_generic(KernelArgs<RULE> a)
 {
     static_assert(DT == 0 || DT == 8 * LPT, "a given head_dim has head_dim / 8 lanes per token");
     constexpr int TPI = 256 / LPT; // token slots per workgroup
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(256) void paged_decode_generic(DecodeArgs a)
 // 512 to 4096 tokens; this takes 5.0).
 // FIN: the rows' (max, denominator) of each head go to ws_final too (null: not asked for).
 template <bool FIN = false>
-__global__ __launch_bounds__(256) void paged_decode_merge(DecodeArgs a)
+__global__ __launch_bounds__(256) void paged_decode_merge(KernelArgs<FIN> a)
 {
     constexpr int MF = 8;
     const int     D = a.head_dim;
@@ -471,7 +471,7 @@ namespace
 {
 
 template <int CT, int DT, int LPT, int GP, bool RULE>
-hipError_t launch3(const DecodeArgs& a, hipStream_t stream)
+hipError_t launch3(const KernelArgs<RULE>& a, hipStream_t stream)
 {
     dim3 grid(static_cast<unsigned>(a.max_chunks), static_cast<unsigned>(a.num_kv_heads),
               static_cast<unsigned>(a.batch));
@@ -486,7 +486,7 @@ hipError_t launch3(const DecodeArgs& a, hipStream_t stream)
 }
 
 template <int CT, int DT, int LPT, bool RULE = false>
-hipError_t launch2(const DecodeArgs& a, hipStream_t stream)
+hipError_t launch2(const KernelArgs<RULE>& a, hipStream_t stream)
 {
     if (a.group <= 1) return launch3<CT, DT, LPT, 1, RULE>(a, stream);
     if (a.group <= 2) return launch3<CT, DT, LPT, 2, RULE>(a, stream);
@@ -514,7 +514,7 @@ hipError_t launch1(const DecodeArgs& a, hipStream_t stream)
 }  // namespace
 
 // fp32 caches at every head_dim, the others at those the matrix cores do not take.
-hipError_t launch_decode_scored_generic(const DecodeArgs& a, hipStream_t stream)
+hipError_t launch_decode_scored_generic(const ScoredDecodeArgs& a, hipStream_t stream)
 {
     switch (a.cache_dtype)
     {

@@ -181,7 +181,7 @@ constexpr int kMfmaMaxWaves =
 // RULE: the scores are changed and the keys bounded by a.rule (a row's pages begin at its first visible key), and with
 // SCORES the visible keys' scores and the rows' final (max, denominator) are written down for the weights.
 template <int CT, int QT, int D, bool PW = false, bool ROW = false, bool RULE = false, bool SCORES = false>
-__device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_, int n_items_, int nw_, uint16_t* s_v)
+__device__ __forceinline__ void decode_wg(const KernelArgs<RULE>& a, int item_, int y_, int n_items_, int nw_, uint16_t* s_v)
 {
     static_assert(!(PW && (ROW || RULE)), "one split or the other; no rule over a shared prefix");
     // (the plain decode reads its indices where it uses them: held in registers from the start, they cost the
@@ -716,8 +716,9 @@ __device__ __forceinline__ void decode_wg(const DecodeArgs& a, int item_, int y_
     // 19 MB cost 64 rows of 512 to 4096 tokens 19 us.)
     auto write_scores = [&](int b, int page, f32x4 sc)
     {
-        if (c < gc)
-            *reinterpret_cast<f32x4*>(a.ws_scores + score_page(a, b, kvh, page) + (h0 + c) * kBlockSize + 4 * g) = sc;
+        if constexpr (SCORES)
+            if (c < gc)
+                *reinterpret_cast<f32x4*>(a.ws_scores + score_page(a, b, kvh, page) + (h0 + c) * kBlockSize + 4 * g) = sc;
     };
 
     // Online softmax of a staged page's scores and PV from its LDS tile.  tks / tvs: int8 scales of token c.
@@ -983,7 +984,7 @@ void paged_decode_mfma(DecodeArgs a)
 // MW waves per (row, head): as many as the rows have pieces for (launch_merge).  FIN: the row's (max, denominator) of each
 // head goes to ws_final too.
 template <int QT, int D, int MW, bool FIN = false>
-__global__ __launch_bounds__(64 * MW) void paged_decode_mfma_merge(DecodeArgs a)
+__global__ __launch_bounds__(64 * MW) void paged_decode_mfma_merge(KernelArgs<FIN> a)
 {
     constexpr int PER = (D + 63) / 64;  // dims per lane (head_dim 96: lanes 0 .. 47 hold two)
     const int     b = blockIdx.x;
@@ -1079,7 +1080,7 @@ __global__ __launch_bounds__(64 * MW) void paged_decode_mfma_merge(DecodeArgs a)
 // (loads of up to MF = 16 pieces in flight together) and writes it; no cross-thread combine.  Rows written whole by
 // the decode kernel (one piece, no shared-prefix partials) or without tokens are left alone.
 template <int QT, int D, bool FIN = false>
-__global__ __launch_bounds__(256) void paged_decode_mfma_merge_rows(DecodeArgs a)
+__global__ __launch_bounds__(256) void paged_decode_mfma_merge_rows(KernelArgs<FIN> a)
 {
     constexpr int MF = 16;
     const int     b = blockIdx.x;
@@ -1171,7 +1172,7 @@ int items_m3(const DecodeArgs& a)
 // 106.1; 128 rows (2) 35.0 / 28.9 / 26.9 / 26.2.  16 rows (16) take 16 waves (27.7 against 27.9 with 8, 256 to 2048
 // tokens), 120 rows over a shared prefix (2 and 4 chunks) one thread (66.8 against 67.0 with 4 waves).
 template <int QT, int D, bool FIN = false>
-hipError_t launch_merge(const DecodeArgs& a, int items, hipStream_t stream)
+hipError_t launch_merge(const KernelArgs<FIN>& a, int items, hipStream_t stream)
 {
     const int  pieces = items / a.batch + a.pfx_chunks;
     const dim3 per_head(static_cast<unsigned>(a.batch), static_cast<unsigned>(a.num_heads));

@@ -18,12 +18,12 @@
 namespace ffkv
 {
 
-int decode_scored_launch_items(const DecodeArgs& a)
+int decode_scored_launch_items(const ScoredDecodeArgs& a)
 {
     return scored_for(a, [&]<int CT, int QT, int D>() { return scored_items3<CT, QT, D>(a); });
 }
 
-hipError_t launch_decode_scored(const DecodeArgs& a, bool mfma, bool row, hipStream_t stream)
+hipError_t launch_decode_scored(const ScoredDecodeArgs& a, bool mfma, bool row, hipStream_t stream)
 {
     if (a.ws_scores == nullptr)
         return mfma ? scored_for(a, [&]<int CT, int QT, int D>() { return launch_scored3<CT, QT, D, false>(a, row, stream); })

@@ -9,7 +9,7 @@ namespace ffkv
 // took 17 us on 64 rows of 512 to 4096 tokens, this takes 10).  The row's own new token has no earlier weight.  Tokens
 // at or past the row's end (or past max_context_len) are left alone.
 constexpr int kWeightTokens = 4;
-__global__ __launch_bounds__(256) void paged_decode_weights(DecodeArgs a)
+__global__ __launch_bounds__(256) void paged_decode_weights(ScoredDecodeArgs a)
 {
     constexpr int T = kWeightTokens;
     const int     b = static_cast<int>(blockIdx.z);
@@ -62,12 +62,12 @@ __global__ __launch_bounds__(256) void paged_decode_weights(DecodeArgs a)
     }
 }
 
-hipError_t launch_decode_scores(const DecodeArgs& a, bool row, hipStream_t stream)
+hipError_t launch_decode_scores(const ScoredDecodeArgs& a, bool row, hipStream_t stream)
 {
     return scored_for(a, [&]<int CT, int QT, int D>() { return launch_scored3<CT, QT, D, true>(a, row, stream); });
 }
 
-hipError_t launch_decode_weights(const DecodeArgs& a, hipStream_t stream)
+hipError_t launch_decode_weights(const ScoredDecodeArgs& a, hipStream_t stream)
 {
     // enough workgroups for the longest row's tokens, up to 64 per (row, KV head): beyond that each takes several stretches
     const int64_t blocks = (static_cast<int64_t>(a.cap_tokens) + 256 * kWeightTokens - 1) / (256 * kWeightTokens);

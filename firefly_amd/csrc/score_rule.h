@@ -5,6 +5,8 @@
 #include "ffkv_device.h"
 #include "ffkv_internal.h"
 
+#include <type_traits>
+
 namespace ffkv
 {
 
@@ -62,9 +64,13 @@ __device__ __forceinline__ int64_t first_key(const ScoreRule& r, int64_t pos, in
     return lo;
 }
 
+// What a decode kernel takes, with a rule or without.
+template <bool RULE>
+using KernelArgs = std::conditional_t<RULE, ScoredDecodeArgs, DecodeArgs>;
+
 // Scores that the decode writes down for the weights: [batch, num_kv_heads, pages, group, 16 tokens], so that what a wave
 // writes of a page (up to 16 heads of 64 bytes) is contiguous.
-__device__ __forceinline__ int64_t score_page(const DecodeArgs& a, int b, int kvh, int page)
+__device__ __forceinline__ int64_t score_page(const ScoredDecodeArgs& a, int b, int kvh, int page)
 {
     return ((static_cast<int64_t>(b) * a.num_kv_heads + kvh) * (a.score_stride / kBlockSize) + page) * a.group * kBlockSize;
 }
@@ -74,7 +80,7 @@ struct RowSpan
 {
     int lo, hi, pos;  // lo <= hi; pos: the query's position
 };
-__device__ __forceinline__ RowSpan row_span(const DecodeArgs& a, int b)
+__device__ __forceinline__ RowSpan row_span(const ScoredDecodeArgs& a, int b)
 {
     const int64_t pos = a.context_lens[b];
     int64_t       hi = pos + 1;  // +1: the token appended this step
