@@ -48,6 +48,8 @@ constexpr int kAwVecTile = 32;
 constexpr int kAwVecThreads = 256;
 constexpr int kAwVecWaves = kAwVecThreads / 64;
 constexpr int kAwVecChunk = kAwVecThreads;
+static_assert(kAwVecChunk == kAwChunk, "one number of splits");
+constexpr int kAwMost = 512;  // workgroups, but for more rows times KV heads (attention_weights_splits)
 
 // Keys [x, y) that query token t of row b sees among its row's `total` tokens; z: its position.
 __device__ __forceinline__ int3 aw_visible(const WeightArgs& a, int b, int64_t ctx, int total, int t)
@@ -67,6 +69,74 @@ __device__ __forceinline__ int aw_total(const WeightArgs& a, int64_t ctx)
     return total < 0 ? 0 : static_cast<int>(total);
 }
 
+// A workgroup's share of the call: chunks split, split + splits, .. of row b's keys for KV head kvh, and the slot of its states
+// (of a row's splits, of seq_len * group states each) in a.part.  b < 0: none.
+struct AwShare
+{
+    int     b, kvh, split, splits;
+    int64_t slot;
+};
+
+// Share `i` of the call's batch * num_kv_heads * a.splits; or, with i < 0, row b's first one (kvh 0).  Every row is cut into
+// pieces of the same number of chunks, the fewest that leave no more pieces than there are shares (each row a.splits
+// instead: 16 x 64 tokens over rows of 400 to 4000 on int8 pages 164 us, 146 so).  All waves find it by themselves.
+__device__ __forceinline__ AwShare aw_share(const WeightArgs& a, int i, int b_of)
+{
+    const int H = a.num_kv_heads;
+    const int at = i / H, kvh = i - at * H;  // (a KV head per XCD where there are eight: 5 % faster than a stretch of rows)
+    if (a.splits == 1 || a.batch == 1)
+    {
+        if (i < 0) return AwShare{b_of, 0, 0, a.splits, static_cast<int64_t>(b_of) * H * a.splits};
+        const int b = a.splits == 1 ? at : 0, split = a.splits == 1 ? 0 : at;
+        return AwShare{b, kvh, split, a.splits, (static_cast<int64_t>(b) * H + kvh) * a.splits + split};
+    }
+    constexpr int N = kAwMost / 2 / 64;  // batch <= kAwMost / 2, as there are two splits and more
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int budget = a.batch * a.splits;
+    int       c[N], total = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+    {
+        const int r = 64 * k + lane;
+        c[k] = r < a.batch ? (aw_total(a, a.context_lens[r]) + kAwChunk - 1) / kAwChunk : 0;
+        total += c[k];
+    }
+    total = __builtin_amdgcn_readlane(wave_scan(total), 63);
+    int len = max(1, (total + budget - 1) / budget);
+    int s[N];
+    for (;; len += 1 + len / 16)  // (ends: at the longest row's length every row is one piece)
+    {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+        {
+            s[k] = 64 * k + lane < a.batch ? max(1, (c[k] + len - 1) / len) : 0;
+            n += s[k];
+        }
+        if (__builtin_amdgcn_readlane(wave_scan(n), 63) <= budget) break;
+    }
+    AwShare got{-1, 0, 0, 1, 0};
+    int     base = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+    {
+        const int      incl = wave_scan(s[k]), excl = base + incl - s[k];
+        const uint64_t hit = __ballot(i < 0 ? 64 * k + lane == b_of : at >= excl && at < excl + s[k]);
+        if (hit != 0)
+        {
+            const int l = __ffsll(static_cast<long long>(hit)) - 1;
+            const int first = __builtin_amdgcn_readlane(excl, l), n = __builtin_amdgcn_readlane(s[k], l);
+            got.b = 64 * k + l;
+            got.splits = n;
+            got.split = i < 0 ? 0 : at - first;
+            got.kvh = i < 0 ? 0 : kvh;
+            got.slot = static_cast<int64_t>(first) * H + static_cast<int64_t>(got.kvh) * n + got.split;
+        }
+        base += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return got;
+}
+
 // A state's (max, denominator) joined with another's; the maxima are finite or NaN (kLowest where there was no key).
 __device__ __forceinline__ float2 aw_join(float2 x, float2 y)
 {
@@ -84,8 +154,8 @@ __device__ __forceinline__ void aw_store(const WeightArgs& a, int64_t bh, int64_
 
 }  // namespace
 
-// Workgroup (split, row and KV head) of blockIdx.x: the keys of chunks split, split + splits, ..  SUM = false: the states of
-// query rows blockIdx.y * block_rows .. over them; SUM = true: the weights of them over all query rows.
+// Workgroup blockIdx.x: the keys of its share (aw_share).  SUM = false: the states of query rows blockIdx.y * block_rows ..
+// over them; SUM = true: the weights of them over all query rows.
 template <int CT, int QT, int D, bool SUM>
 __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 4 : 2, 8))) void attention_weights_mfma(WeightArgs a)
 {
@@ -125,10 +195,10 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15;
     const int g = lane >> 4;
-    const int split = static_cast<int>(blockIdx.x) % a.splits;
-    const int bh = static_cast<int>(blockIdx.x) / a.splits;
-    const int b = bh / a.num_kv_heads;
-    const int kvh = bh - b * a.num_kv_heads;
+    const AwShare share = aw_share(a, static_cast<int>(blockIdx.x), 0);
+    const int     b = share.b, kvh = share.kvh, split = share.split, splits = share.splits;
+    if (b < 0) return;
+    const int bh = b * a.num_kv_heads + kvh;
     const int G = a.group;
     const int R = a.seq_len * G;
     const int64_t ctx = a.context_lens[b];
@@ -261,13 +331,12 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
 
     const int rb0 = SUM ? 0 : static_cast<int>(blockIdx.y);
     int       tiles = 0;
-    if (split < chunks && (!SUM || blocks == 1)) tiles = stage(rb0);
     if constexpr (!SUM)
         for (int i = lane; i < rows; i += 64) s_ml[wave * rows + i] = make_float2(kLowest, 0.0f);
 
     // This wave's keys of a chunk, as loaded: lane (c, g) holds dims dimof(j, g) .. + 7 of key c of each page.  (Loading the
     // next chunk's ahead of this one's products took the registers over 128 and was no faster: one row of 32.7k tokens 58 us
-    // against 51, and 184 against 187 on 16 rows of int8 pages.)
+    // against 51, and 184 against 187 on 16 rows of int8 pages; the first chunk's ahead of the query rows 48 against 47.)
     constexpr int NW = kElemBytes<CT> == 2 ? KSTEPS : (KSTEPS + 1) / 2;
     struct Keys
     {
@@ -321,7 +390,8 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
                         ok ? a.k_scale[(static_cast<size_t>(phys) * kBlockSize + 4 * g + i) * a.num_kv_heads + kvh] : 0.0f;
         }
     };
-    for (int ch = split; ch < chunks; ch += a.splits)
+    if (split < chunks && (!SUM || blocks == 1)) tiles = stage(rb0);
+    for (int ch = split; ch < chunks; ch += splits)
     {
         const int key0 = ch * CHUNK + wave * (KP * kBlockSize);
         Keys      raw_keys;
@@ -494,7 +564,7 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
             float2 st = s_ml[i];
 #pragma unroll
             for (int w = 1; w < kAwWaves; ++w) st = aw_join(st, s_ml[w * rows + i]);
-            a.part[(static_cast<int64_t>(bh) * a.splits + split) * R + r] = st;
+            a.part[share.slot * R + r] = st;
         }
     }
 }
@@ -513,10 +583,10 @@ __global__ __launch_bounds__(kAwVecThreads) void attention_weights_vector(Weight
     const int tid = static_cast<int>(threadIdx.x);
     const int lane = tid & 63;
     const int wave = tid >> 6;
-    const int split = static_cast<int>(blockIdx.x) % a.splits;
-    const int bh = static_cast<int>(blockIdx.x) / a.splits;
-    const int b = bh / a.num_kv_heads;
-    const int kvh = bh - b * a.num_kv_heads;
+    const AwShare share = aw_share(a, static_cast<int>(blockIdx.x), 0);
+    const int     b = share.b, kvh = share.kvh, split = share.split, splits = share.splits;
+    if (b < 0) return;
+    const int bh = b * a.num_kv_heads + kvh;
     const int G = a.group;
     const int R = a.seq_len * G;
     const int64_t ctx = a.context_lens[b];
@@ -526,7 +596,7 @@ __global__ __launch_bounds__(kAwVecThreads) void attention_weights_vector(Weight
     const int r_hi = SUM ? R : min(R, r_lo + kAwVecRows);
     if constexpr (!SUM)
         for (int i = lane; i < kAwVecRows; i += 64) s_ml[wave][i] = make_float2(kLowest, 0.0f);
-    for (int ch = split; ch < chunks; ch += a.splits)
+    for (int ch = split; ch < chunks; ch += splits)
     {
         const int key = ch * kAwVecChunk + tid;
         int       phys = -1;
@@ -618,7 +688,7 @@ __global__ __launch_bounds__(kAwVecThreads) void attention_weights_vector(Weight
             float2 st = s_ml[0][r - r_lo];
 #pragma unroll
             for (int v = 1; v < kAwVecWaves; ++v) st = aw_join(st, s_ml[v][r - r_lo]);
-            a.part[(static_cast<int64_t>(bh) * a.splits + split) * R + r] = st;
+            a.part[share.slot * R + r] = st;
         }
     }
 }
@@ -633,9 +703,12 @@ __global__ __launch_bounds__(256) void attention_weights_fold(WeightArgs a)
     const int     blocks = (R + 15) / 16;
     const int64_t bh = static_cast<int64_t>(blockIdx.x) / blocks;
     const int     r = static_cast<int>(blockIdx.x % blocks) * 16 + i;
+    const int     b = static_cast<int>(bh / a.num_kv_heads);
+    const AwShare share = aw_share(a, -1, b);
+    const int64_t slot = share.slot + (bh - static_cast<int64_t>(b) * a.num_kv_heads) * share.splits;
     float2        st = make_float2(kLowest, 0.0f);
     if (r < R)
-        for (int s = sl; s < a.splits; s += 16) st = aw_join(st, a.part[(bh * a.splits + s) * R + r]);
+        for (int s = sl; s < share.splits; s += 16) st = aw_join(st, a.part[(slot + s) * R + r]);
     s_st[sl][i] = st;
     __syncthreads();
     if (sl != 0 || r >= R) return;
@@ -692,15 +765,15 @@ hipError_t launch_vector(const WeightArgs& a, bool sum, dim3 grid, hipStream_t s
 
 }  // namespace
 
-// Splits of a row's keys: as many workgroups in all as fit the chip at once (two of eight waves per CU), one chunk of keys
-// each at most; a workgroup then stages its query rows once for several chunks.  us at 256 / 512 / 1024 / 2048 workgroups:
-// 32 tokens over one row of 32.7k 65 / 51 / 59 / 60, 16 x 64 tokens over int8 rows of 400 to 4000 244 / 187 / 191 / 215.
+// Splits of a row's keys, on average over the rows (aw_share): as many workgroups in all as fit the chip at once (two of eight
+// waves per CU), one chunk of keys each at most; a workgroup then stages its query rows once for several chunks.  us at 512 /
+// 768 / 1024 workgroups: 32 tokens over one row of 32.7k 47 / 52 / 57, 16 x 64 tokens over int8 rows of 400 to 4000
+// 146 / 157 / 160 (with rows cut alike, 256 took 65 and 244 where 512 took 51 and 187).
 int attention_weights_splits(int batch, int num_kv_heads, int head_dim, int cap_tokens)
 {
-    constexpr int64_t kMost = 512;
     const int64_t chunk = kAwChunk;
     const int64_t chunks = (static_cast<int64_t>(cap_tokens) + chunk - 1) / chunk;
-    const int64_t most = kMost / (static_cast<int64_t>(batch) * num_kv_heads);
+    const int64_t most = kAwMost / (static_cast<int64_t>(batch) * num_kv_heads);
     const int64_t n = chunks < most ? chunks : most;
     return static_cast<int>(n < 1 ? 1 : n);
 }

@@ -214,3 +214,15 @@ def test_streams_and_graph(ff, gpu):
         ff.attention_weights(d[8], d[0], d[4], d[5], eager, eager, 0.5, r["cap"], sl, r["window"], begin, workspace=ws)
         torch.cuda.synchronize()
         assert torch.equal(total, eager)
+
+
+@pytest.mark.parametrize("B,Hkv", [(5, 2), (70, 1), (130, 2), (256, 1), (255, 2)])
+def test_uneven_rows(ff, gpu, B, Hkv):
+    """Rows of very different lengths, empty ones among them, in calls whose rows are cut into pieces and in ones of too many
+    rows for that."""
+    g = np.random.default_rng(23)
+    ctx = [int(x) for x in g.integers(0, 60, B)]
+    ctx[B // 2], ctx[-1], ctx[0] = 9000, 2500, -9
+    c = make(23, ctx, 3, 2 * Hkv, Hkv, 64, "bf16", "bf16")
+    r = rule_of(c, cap=9.0, slopes=True)
+    check(c, call(ff, c, su.device(c, gpu), r, max_context_len=9003), expected(c, r, 9003), left=0)
