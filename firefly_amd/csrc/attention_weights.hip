@@ -143,6 +143,32 @@ __device__ __forceinline__ AwShare aw_share(const WeightArgs& a, int i, int b_of
     return got;
 }
 
+// Chunks [x, y) of row b that some query sees: the others' keys are not read.  Every wave by itself, a lane a query.
+__device__ __forceinline__ int2 aw_chunks(const WeightArgs& a, int b, int64_t ctx, int total)
+{
+    const int all = (total + kAwChunk - 1) / kAwChunk;
+    if (a.rule.window <= 0 && a.rule.key_begin == nullptr && a.rule.key_end == nullptr) return make_int2(0, all);
+    int lo = INT32_MAX, hi = 0;
+    for (int t = static_cast<int>(threadIdx.x) & 63; t < a.seq_len; t += 64)
+    {
+        const int3 vis = aw_visible(a, b, ctx, total, t);
+        if (vis.x < vis.y)
+        {
+            lo = min(lo, vis.x);
+            hi = max(hi, vis.y);
+        }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+    {
+        lo = min(lo, __shfl_xor(lo, off, 64));
+        hi = max(hi, __shfl_xor(hi, off, 64));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    return lo < hi ? make_int2(lo / kAwChunk, (hi + kAwChunk - 1) / kAwChunk) : make_int2(0, 0);
+}
+
 // A state's (max, denominator) joined with another's; the maxima are finite or NaN (kLowest where there was no key).
 __device__ __forceinline__ float2 aw_join(float2 x, float2 y)
 {
@@ -210,6 +236,8 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
     const int64_t ctx = a.context_lens[b];
     const int total = __builtin_amdgcn_readfirstlane(aw_total(a, ctx));
     const int chunks = (total + CHUNK - 1) / CHUNK;
+    const int2 live = aw_chunks(a, b, ctx, total);
+    const int  first = live.x <= split ? split : split + (live.x - split + splits - 1) / splits * splits;  // of this share
     const int blocks = (R + rows - 1) / rows;
     const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
     // from products to scores in log2 units, or in those of the cap (int8: times the key's scale)
@@ -396,11 +424,16 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
                         ok ? a.k_scale[(static_cast<size_t>(phys) * kBlockSize + 4 * g + i) * a.num_kv_heads + kvh] : 0.0f;
         }
     };
-    if (split < chunks && (!SUM || blocks == 1)) tiles = stage(rb0);
-    for (int ch = split; ch < chunks; ch += splits)
+    if (first < live.y && (!SUM || blocks == 1)) tiles = stage(rb0);
+    for (int ch = SUM ? split : first; ch < (SUM ? chunks : live.y); ch += splits)
     {
         const int key0 = ch * CHUNK + wave * (KP * kBlockSize);
-        Keys      raw_keys;
+        if (SUM && (ch < live.x || ch >= live.y))  // seen by none: what it had
+        {
+            if (lane < KP * kBlockSize) aw_store(a, bh, ctx, total, key0 + lane, 0.0f);
+            continue;
+        }
+        Keys raw_keys;
         load_keys(ch, raw_keys);
         X8        k[KP][KSTEPS > 0 ? KSTEPS : 1];
         X4        kt[KP];
@@ -542,7 +575,7 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
                     if (g == 0)
                     {
                         float2& st = s_ml[wave * rows + tile * 16 + c];
-                        st = ch == split ? make_float2(m, l) : aw_join(st, make_float2(m, l));
+                        st = ch == first ? make_float2(m, l) : aw_join(st, make_float2(m, l));
                     }
                 }
             }
@@ -598,13 +631,20 @@ __global__ __launch_bounds__(kAwVecThreads) void attention_weights_vector(Weight
     const int64_t ctx = a.context_lens[b];
     const int total = aw_total(a, ctx);
     const int chunks = (total + kAwVecChunk - 1) / kAwVecChunk;
+    const int2 live = aw_chunks(a, b, ctx, total);
+    const int  first = live.x <= split ? split : split + (live.x - split + splits - 1) / splits * splits;
     const int r_lo = SUM ? 0 : static_cast<int>(blockIdx.y) * kAwVecRows;
     const int r_hi = SUM ? R : min(R, r_lo + kAwVecRows);
     if constexpr (!SUM)
         for (int i = lane; i < kAwVecRows; i += 64) s_ml[wave][i] = make_float2(kLowest, 0.0f);
-    for (int ch = split; ch < chunks; ch += splits)
+    for (int ch = SUM ? split : first; ch < (SUM ? chunks : live.y); ch += splits)
     {
         const int key = ch * kAwVecChunk + tid;
+        if (SUM && (ch < live.x || ch >= live.y))
+        {
+            aw_store(a, bh, ctx, total, key, 0.0f);
+            continue;
+        }
         int       phys = -1;
         if (key < total) phys = a.block_table[static_cast<int64_t>(b) * a.max_blocks + (key >> 4)];
         const bool   ok = phys >= 0 && phys < a.num_blocks;

@@ -226,3 +226,19 @@ def test_uneven_rows(ff, gpu, B, Hkv):
     c = make(23, ctx, 3, 2 * Hkv, Hkv, 64, "bf16", "bf16")
     r = rule_of(c, cap=9.0, slopes=True)
     check(c, call(ff, c, su.device(c, gpu), r, max_context_len=9003), expected(c, r, 9003), left=0)
+
+
+@pytest.mark.parametrize("act,kv,Hq,Hkv,D", [CONFIGS[i] for i in (0, 2, 12)])
+def test_few_keys_seen(ff, gpu, act, kv, Hq, Hkv, D):
+    """Windows and ranges that leave most of a row out, at its front, its end and whole; earlier weights decay everywhere."""
+    c = make(25, [3000, 900, 2600, 5], 70, Hq, Hkv, D, act, kv)
+    d = su.device(c, gpu)
+    prior = torch.rand(4, Hkv, 3070, device=gpu)
+    for kind in ("window", "front", "middle", "none"):
+        r = rule_of(c, cap=7.0, window=100 if kind == "window" else 0)
+        if kind != "window":
+            lo, hi = {"front": (-4, 30), "middle": (700, 1300), "none": (50, 50)}[kind]
+            r["begin"], r["end"] = np.full((4, 70), lo, np.int32), np.full((4, 70), hi, np.int32)
+            r["end"][2, 3] = lo
+        w = call(ff, c, d, r, weights=torch.zeros_like(prior), prior=prior, decay=0.5, max_context_len=3070)
+        check(c, w, expected(c, r), prior, 0.5, left=0)
