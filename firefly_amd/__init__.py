@@ -210,9 +210,9 @@ def paged_prefill(q, k_cache, v_cache, block_table, context_lens, out=None, k_sc
 
 def _prefill_scratch(n: int, q, stream):
     """Scratch of ``n`` bytes for one call on ``stream`` (None: the current one), from torch's allocator and belonging
-    to that stream, so that it can be reused once the call's work on the stream is done.  None, where a prefill
-    runs unsplit and the other calls take stream-ordered memory, while the stream is being captured (a capture allocates
-    nothing here) and where there is no memory for it."""
+    to that stream, so that it can be reused once the call's work on the stream is done.  None while the stream is
+    being captured (a capture allocates nothing here) and where there is no memory for it: a prefill then runs unsplit,
+    and the other calls take stream-ordered memory, or refuse a capture."""
     import torch
 
     if stream is not None:
@@ -338,7 +338,8 @@ def paged_attention_scored(q, k_cache, v_cache, block_table, context_lens, score
     tanh(s / score_cap)`` (0: not), less ``slopes[head] * distance`` (fp32 ``[Hq]``), over the last ``window`` keys (0: all)
     from key ``key_begin[b]`` on (int32 ``[B]``).  ``k_new``/``v_new`` ``[B, 1, Hkv, D]`` are appended first.  ``weights``
     fp32 ``[B, Hkv, T]`` becomes ``decay * prior`` plus the attention weight of every cached token of the row (``prior`` may
-    be ``weights``; None: nothing earlier); give ``max_context_len`` then where the table is wide."""
+    be ``weights``; None: nothing earlier); give ``max_context_len`` then where the table is wide.  A captured call needs a
+    workspace (``decode_scored_workspace``; small batches without weights need none)."""
     out = _decode_out(q, out)
     check(_front.decode_scored(q, out, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, max_context_len, scale,
                                num_blocks, k_new, v_new, score_cap, slopes, window, key_begin, weights, prior, decay,
@@ -381,7 +382,8 @@ def attention_weights(q, k_cache, block_table, context_lens, weights=None, prior
     """The attention weights that queries ``q`` ``[B, S, Hq, D]`` (the rows' last S tokens, at ``context_lens[b] + t``) give to
     the cached keys under the rule of ``paged_prefill_scored`` (``ffkv_attention_weights``): ``weights`` fp32 ``[B, Hkv, T]``
     becomes ``decay * prior`` plus them, summed over queries and the heads of a KV head.  Without ``weights`` a new tensor
-    over the block table's (or ``max_context_len``) tokens, zero past a row's end.  Returns ``weights``."""
+    over the block table's (or ``max_context_len``) tokens, zero past a row's end.  Returns ``weights``.  A captured call needs
+    a workspace (``attention_weights_workspace``)."""
     if weights is None:
         import torch
 
@@ -409,7 +411,8 @@ def evict_tokens(weights, k_cache, v_cache, block_table, context_lens, keep: int
     ``[B, Hkv, T]``, ``context_lens`` the rows' tokens; the first ``sinks`` and last ``recent`` always stay.  The kept tokens
     move to the front of the row's pages in ``dst_table`` int32 ``[B, blocks]`` (None: of its own pages, which no other row
     may hold), their weights to ``weights_out`` (None: not; may be ``weights``).  Returns ``kept`` int32 ``[B, Hkv, keep]``
-    (the kept positions, ascending) and the rows' new lengths."""
+    (the kept positions, ascending) and the rows' new lengths.  A captured call over few long rows needs a workspace
+    (``evict_workspace``)."""
     if kept is None or kept_lens is None:
         import torch
 

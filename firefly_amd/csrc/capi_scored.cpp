@@ -96,6 +96,19 @@ int prefill_span(int cap_tokens, int group, int window, bool key_end)
     return static_cast<int>(std::min<int64_t>(cap_tokens, static_cast<int64_t>(window) + 128 / group + 2 * FFKV_BLOCK_SIZE));
 }
 
+// Stream-ordered memory for a call without a workspace.  Not while the stream is being captured: a graph of three such calls
+// that allocated and freed inside it has faulted on its first replay.
+int take_memory(void** ws, int64_t bytes, hipStream_t s)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    hipError_t             e = hipStreamIsCapturing(s, &status);
+    if (e != hipSuccess) return hip_fail(e, "hipStreamIsCapturing");
+    if (status != hipStreamCaptureStatusNone)
+        return fail(FFKV_ERR_WORKSPACE, "a captured call needs a workspace, of %lld bytes", static_cast<long long>(bytes));
+    e = hipMallocAsync(ws, static_cast<size_t>(bytes), s);
+    return e == hipSuccess ? FFKV_OK : hip_fail(e, "workspace hipMallocAsync");
+}
+
 // What a scored decode launches and holds in its workspace; sizes and types of `a` are set.
 struct DecodePlan
 {
@@ -293,8 +306,7 @@ int ffkv_paged_decode_scored(const void* q, void* out, int qo_dtype, void* k_cac
                     static_cast<long long>(need));
     if (ws == nullptr && need > 0)
     {
-        const hipError_t e = hipMallocAsync(&ws, static_cast<size_t>(need), s);
-        if (e != hipSuccess) return hip_fail(e, "decode workspace hipMallocAsync");
+        if (const int rc = take_memory(&ws, need, s)) return rc;
         owned = true;
     }
     char* wsb = static_cast<char*>(ws);
@@ -500,10 +512,7 @@ int ffkv_attention_weights(const void* q, int qo_dtype, const void* k_cache, int
         return fail(FFKV_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %lld bytes needed", workspace_bytes,
                     static_cast<long long>(lay.total));
     if (ws == nullptr && lay.total > 0)
-    {
-        const hipError_t e = hipMallocAsync(&ws, static_cast<size_t>(lay.total), s);
-        if (e != hipSuccess) return hip_fail(e, "attention weights workspace hipMallocAsync");
-    }
+        if (const int rc = take_memory(&ws, lay.total, s)) return rc;
     ffkv::WeightArgs a{};
     a.q = q;
     a.k_cache = k_cache;
@@ -618,10 +627,7 @@ int ffkv_evict(const float* weights, int64_t weight_stride, const int32_t* conte
         return fail(FFKV_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %lld bytes needed", workspace_bytes,
                     static_cast<long long>(lay.total));
     if (ws == nullptr && lay.total > 0)
-    {
-        const hipError_t e = hipMallocAsync(&ws, static_cast<size_t>(lay.total), s);
-        if (e != hipSuccess) return hip_fail(e, "evict workspace hipMallocAsync");
-    }
+        if (const int rc = take_memory(&ws, lay.total, s)) return rc;
     a.parts = lay.parts;
     if (a.parts > 0)
     {

@@ -5,7 +5,7 @@
 // max_context_blocks argument, and the launch goes to the thread's default stream.  The decode workspace (split
 // partial results) is cached per (thread, device, stream) and grown outside of stream capture; while a stream is
 // being captured a missing or too-small workspace makes the library allocate stream-ordered memory inside the graph
-// instead.
+// instead (the scored decode, the attention weights and the eviction refuse the call).
 #include <hip/hip_runtime_api.h>
 
 #include <algorithm>

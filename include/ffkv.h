@@ -297,8 +297,9 @@ FFKV_API int ffkv_rope_append(void* q, void* k, const void* v, int src_dtype, vo
  * row's cached tokens.  ffkv_decode_scored_workspace_bytes is enough for every type, KV head count and window at these
  * sizes; ffkv_decode_scored_scratch_bytes is what the one call needs (0 for small batches, which take one launch).  With
  * weights the workspace holds the scores of all visible keys (4 bytes per query head and token
- * of the bound on a row): give max_context_len where the block table is wide.  workspace NULL: stream-ordered memory.
- * The calls that share a workspace must not overlap in time.
+ * of the bound on a row): give max_context_len where the block table is wide.  workspace NULL: stream-ordered memory,
+ * or FFKV_ERR_WORKSPACE where the stream is being captured (and any is needed).  The calls that share a workspace must not
+ * overlap in time.
  */
 FFKV_API size_t ffkv_decode_scored_workspace_bytes(int batch, int num_heads, int head_dim, int max_blocks,
                                                    int max_context_len, int with_weights);
@@ -349,7 +350,7 @@ FFKV_API int ffkv_paged_prefill_scored(const void* q, void* out, int qo_dtype, c
  * weights and prior as for ffkv_paged_decode_scored, which gives the same for single tokens beside the attention itself;
  * this call reads no V and writes no output: the prompt's part of what ffkv_evict goes by (the last 16 to 64 tokens of a
  * prompt, a few queries of a chunk).  seq_len 0: the earlier weights' decay alone.  Caches, head dims and GQA groups as for ffkv_paged_decode_scored, any group size.
- * Workspace: ffkv_attention_weights_workspace_bytes, or NULL for stream-ordered memory; calls that share one must not
+ * Workspace: ffkv_attention_weights_workspace_bytes, or NULL as for ffkv_paged_decode_scored; calls that share one must not
  * overlap in time.  No counterpart in the reference.
  */
 FFKV_API size_t ffkv_attention_weights_workspace_bytes(int batch, int seq_len, int num_heads, int num_kv_heads,
@@ -382,7 +383,7 @@ FFKV_API int ffkv_attention_weights(const void* q, int qo_dtype, const void* k_c
  * rotary embedding it was cached with, and the row goes on from position kept_lens[b] (the new tokens' rotary positions
  * go on from the old ones).  A kept token whose source or destination page is absent is not copied.  keep >= 1, sinks
  * and recent >= 0 and together at most keep.  Cache types, head dims and alignment as for ffkv_append.  Workspace:
- * ffkv_evict_workspace_bytes (0 but for few rows over a long bound), or NULL for stream-ordered memory; calls that share
+ * ffkv_evict_workspace_bytes (0 but for few rows over a long bound), or NULL as for ffkv_paged_decode_scored; calls that share
  * one must not overlap in time.  No counterpart in the reference, which evicts whole prefix-cache nodes that no request
  * uses (src/radix_tree.cc).
  */

@@ -134,3 +134,122 @@ def test_prompt_cut_decode_cut_decode(ff, gpu, kv, rule):
     steps(20, w)
     cut(w, None)
     steps(3, w)
+
+
+@pytest.mark.skip(reason="the replay faulted when the library still allocated inside a capture; such calls are refused now "
+                         "(test_capture_needs_workspaces), and graphs are given workspaces (test_captured_together)")
+def test_captured_without_workspaces(ff, gpu):
+    """Weights of a prompt's end, a decode step with weights and an eviction of long rows, captured in one graph with memory of
+    their own: every replay gives what the eager calls give, with eager calls in between."""
+    B, n, keep, Hq, Hkv, D = 2, 9000, 4000, 4, 2, 64
+    g = torch.Generator(device=gpu).manual_seed(3)
+    room = (n + 16) // 16
+    rnd = lambda *s: torch.randn(s, generator=g, device=gpu, dtype=torch.float32).to(torch.bfloat16)  # noqa: E731
+    k, v = rnd(B * room * 2, 16, Hkv, D), rnd(B * room * 2, 16, Hkv, D)
+    order = torch.randperm(B * room * 2, generator=g, device=gpu).to(torch.int32)
+    table, dst = order[:B * room].view(B, room).contiguous(), order[B * room:].view(B, room).contiguous()
+    lens = torch.tensor([n, n - 500], dtype=torch.int32, device=gpu)
+    before = lens - 16
+    ql, q = rnd(B, 16, Hq, D), rnd(B, 1, Hq, D)
+    T = n + 1
+
+    def calls(w, kept, left, out, cut):
+        ff.attention_weights(ql, k, table, before, weights=w, max_context_len=T, score_cap=20.0)
+        ff.paged_attention_scored(q, k, v, table, lens, weights=w, prior=w, decay=0.5, out=out, max_context_len=T, window=3000)
+        ff.evict_tokens(w, k, v, table, lens, keep, 4, 300, dst, cut, kept, left)
+
+    def buffers():
+        return (torch.zeros(B, Hkv, T, device=gpu), torch.zeros(B, Hkv, keep, dtype=torch.int32, device=gpu),
+                torch.zeros(B, dtype=torch.int32, device=gpu), torch.zeros(B, 1, Hq * D, dtype=torch.bfloat16, device=gpu),
+                torch.zeros(B, Hkv, keep, device=gpu))
+
+    eager, got = buffers(), buffers()
+    calls(*eager)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(*got)
+    for _ in range(4):
+        for t in got:
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(eager, got):
+            assert torch.equal(a, b)
+        again = buffers()
+        calls(*again)
+        torch.cuda.synchronize()
+        for a, b in zip(eager, again):
+            assert torch.equal(a, b)
+
+
+def test_capture_needs_workspaces(ff, gpu):
+    """A captured call that would have to allocate is refused before anything is launched; one that needs nothing is not."""
+    q = torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16, device=gpu)
+    k, v = (torch.zeros(600, 16, 2, 64, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+    table = torch.arange(600, dtype=torch.int32, device=gpu)[None]
+    lens = torch.tensor([9500], dtype=torch.int32, device=gpu)
+    w, out = torch.zeros(1, 2, 9600, device=gpu), torch.zeros(1, 1, 256, dtype=torch.bfloat16, device=gpu)
+    kept, left = torch.zeros(1, 2, 100, dtype=torch.int32, device=gpu), torch.zeros(1, dtype=torch.int32, device=gpu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out.fill_(1.0)
+        for call in (lambda: ff.attention_weights(q, k, table, lens, weights=w),
+                     lambda: ff.paged_attention_scored(q, k, v, table, lens, weights=w, out=out),
+                     lambda: ff.evict_tokens(w, k, v, table, lens, 100, kept=kept, kept_lens=left)):
+            with pytest.raises(ff.FFKVError, match="workspace"):
+                call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (out == 1.0).all() and (w == 0).all() and (kept == 0).all()
+
+
+def test_captured_together(ff, gpu):
+    """Weights of a prompt's end, a decode step with weights and an eviction of long rows in one graph, one workspace for all:
+    every replay gives what the eager calls give, with eager calls on the same workspace in between."""
+    B, n, keep, Hq, Hkv, D = 2, 9000, 4000, 4, 2, 64
+    g = torch.Generator(device=gpu).manual_seed(3)
+    room = (n + 16) // 16
+    rnd = lambda *s: torch.randn(s, generator=g, device=gpu, dtype=torch.float32).to(torch.bfloat16)  # noqa: E731
+    k, v = rnd(B * room * 2, 16, Hkv, D), rnd(B * room * 2, 16, Hkv, D)
+    order = torch.randperm(B * room * 2, generator=g, device=gpu).to(torch.int32)
+    table, dst = order[:B * room].view(B, room).contiguous(), order[B * room:].view(B, room).contiguous()
+    lens = torch.tensor([n, n - 500], dtype=torch.int32, device=gpu)
+    before = lens - 16
+    ql, q = rnd(B, 16, Hq, D), rnd(B, 1, Hq, D)
+    T = n + 1
+    ws = max((ff.decode_scored_workspace(B, Hq, D, room, T, weights=True, device=gpu),
+              ff.attention_weights_workspace(B, 16, Hq, Hkv, D, room, T, device=gpu),
+              ff.evict_workspace(B, Hkv, keep, T, room, device=gpu)), key=lambda t: t.numel())
+
+    def calls(w, kept, left, out, cut):
+        ff.attention_weights(ql, k, table, before, weights=w, max_context_len=T, score_cap=20.0, workspace=ws)
+        ff.paged_attention_scored(q, k, v, table, lens, weights=w, prior=w, decay=0.5, out=out, max_context_len=T, window=3000,
+                                  workspace=ws)
+        ff.evict_tokens(w, k, v, table, lens, keep, 4, 300, dst, cut, kept, left, workspace=ws)
+
+    def buffers():
+        return (torch.zeros(B, Hkv, T, device=gpu), torch.zeros(B, Hkv, keep, dtype=torch.int32, device=gpu),
+                torch.zeros(B, dtype=torch.int32, device=gpu), torch.zeros(B, 1, Hq * D, dtype=torch.bfloat16, device=gpu),
+                torch.zeros(B, Hkv, keep, device=gpu))
+
+    eager, got = buffers(), buffers()
+    calls(*eager)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(*got)
+    for _ in range(4):
+        for t in got:
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(eager, got):
+            assert torch.equal(a, b)
+        again = buffers()
+        calls(*again)
+        torch.cuda.synchronize()
+        for a, b in zip(eager, again):
+            assert torch.equal(a, b)
