@@ -208,6 +208,27 @@ def paged_prefill(q, k_cache, v_cache, block_table, context_lens, out=None, k_sc
     return out
 
 
+def _torch_stream(stream, device):
+    """A call's ``stream`` argument (a torch stream, anything with a ``cuda_stream``, or a raw handle) as a torch stream."""
+    import torch
+
+    if isinstance(stream, torch.cuda.Stream):
+        return stream
+    return torch.cuda.ExternalStream(int(getattr(stream, "cuda_stream", stream)), device=device)
+
+
+def _zeros(shape, q, stream):
+    """A new fp32 tensor on ``q``'s device, its memory the current stream's like that of the other calls' outputs, its
+    zeros written on the call's ``stream``: on the current one they could land after what the call writes."""
+    import torch
+
+    t = torch.empty(shape, dtype=torch.float32, device=q.device)
+    if stream is None or not t.is_cuda:
+        return t.zero_()
+    with torch.cuda.stream(_torch_stream(stream, q.device)):
+        return t.zero_()
+
+
 def _prefill_scratch(n: int, q, stream):
     """Scratch of ``n`` bytes for one call on ``stream`` (None: the current one), from torch's allocator and belonging
     to that stream, so that it can be reused once the call's work on the stream is done.  None while the stream is
@@ -216,9 +237,7 @@ def _prefill_scratch(n: int, q, stream):
     import torch
 
     if stream is not None:
-        if not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(getattr(stream, "cuda_stream", stream)), device=q.device)
-        with torch.cuda.stream(stream):
+        with torch.cuda.stream(_torch_stream(stream, q.device)):
             return _prefill_scratch(n, q, None)
     if torch.cuda.is_current_stream_capturing():
         return None
@@ -385,11 +404,9 @@ def attention_weights(q, k_cache, block_table, context_lens, weights=None, prior
     over the block table's (or ``max_context_len``) tokens, zero past a row's end.  Returns ``weights``.  A captured call needs
     a workspace (``attention_weights_workspace``)."""
     if weights is None:
-        import torch
-
         most = block_table.shape[-1] * BLOCK_SIZE
         most = min(most, max_context_len) if max_context_len > 0 else most
-        weights = torch.zeros((q.shape[0], k_cache.shape[2], most), dtype=torch.float32, device=q.device)
+        weights = _zeros((q.shape[0], k_cache.shape[2], most), q, stream)
     check(_front.attention_weights(q, k_cache, k_scale, block_table, context_lens, max_context_len, scale, num_blocks,
                                    score_cap, slopes, window, key_begin, key_end, weights, prior, decay, workspace, stream,
                                    _prefill_scratch))

@@ -242,3 +242,21 @@ def test_few_keys_seen(ff, gpu, act, kv, Hq, Hkv, D):
             r["end"][2, 3] = lo
         w = call(ff, c, d, r, weights=torch.zeros_like(prior), prior=prior, decay=0.5, max_context_len=3070)
         check(c, w, expected(c, r), prior, 0.5, left=0)
+
+
+def test_new_weights_on_another_stream(ff, gpu):
+    """Without `weights` the new tensor's zeros are written on the call's stream, however busy the current one is."""
+    c = make(29, [900, 40], 30)
+    r = rule_of(c, cap=5.0)
+    d = su.device(c, gpu)
+    want = call(ff, c, d, r)
+    side = torch.cuda.Stream()
+    x = torch.randn(4096, 4096, device=gpu)
+    for stream in (side, side.cuda_stream):
+        torch.cuda.synchronize()
+        for _ in range(40):  # some tens of milliseconds
+            x = (x @ x).mul_(1.0 / 64.0)
+        w = call(ff, c, d, r, stream=stream)
+        side.synchronize()
+        torch.cuda.synchronize()
+        assert torch.equal(w, want)
