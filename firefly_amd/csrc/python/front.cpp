@@ -633,7 +633,7 @@ PyObject* attention_weights(PyObject*, PyObject* const* a, Py_ssize_t n)
     r.holds(a[12], "key_end", kInt32, {B, S}, q, true);
     Weights w(r, a + 13, B, Hkv, q);
     r.plain(a[16], "workspace", q);
-    r.current(q, B > 0 && S > 0);
+    r.current(q, B > 0);  // (without queries the earlier weights still decay)
     void *qp = r.ptr(q), *kc = r.ptr(a[1]);
     auto* ks = r.ptr<float>(a[2]);
     auto *bt = r.ptr<int32_t>(a[3]), *cx = r.ptr<int32_t>(a[4]);

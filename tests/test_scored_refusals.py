@@ -258,3 +258,16 @@ def test_weights_front(ff):
     for error, kw in bad:
         with pytest.raises(error):
             ff.attention_weights(**kw, stream=0)
+
+
+@pytest.mark.parametrize("S", [1, 0])
+def test_weights_front_device(ff, S):
+    """Rows in CPU tensors are refused, also where there are no queries: their earlier weights would still be decayed."""
+    t = _tensors(B=1)
+    t.pop("v_cache")
+    t["q"] = torch.zeros(1, S, 4, D, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="GPU"):
+        ff.attention_weights(**t, stream=0)
+    w = torch.zeros(1, HKV, 48)
+    with pytest.raises(ValueError, match="GPU"):
+        ff.attention_weights(**t, weights=w, prior=w, stream=0)
