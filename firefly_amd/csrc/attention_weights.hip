@@ -18,8 +18,7 @@
 // issue is 70 % of the time).
 #include "mfma_common.h"
 #include "score_rule.h"
-
-#include <algorithm>
+#include "weight_rows.h"
 
 namespace ffkv
 {
@@ -143,9 +142,11 @@ __device__ __forceinline__ AwShare aw_share(const WeightArgs& a, int i, int b_of
     return got;
 }
 
-// Chunks [x, y) of row b that some query sees: the others' keys are not read.  Every wave by itself, a lane a query.
+// Chunks [x, y) of row b that some query sees: the others' keys are not read (without queries, none).  Every wave by itself, a
+// lane a query.
 __device__ __forceinline__ int2 aw_chunks(const WeightArgs& a, int b, int64_t ctx, int total)
 {
+    if (a.seq_len == 0) return make_int2(0, 0);
     const int all = (total + kAwChunk - 1) / kAwChunk;
     if (a.rule.window <= 0 && a.rule.key_begin == nullptr && a.rule.key_end == nullptr) return make_int2(0, all);
     int lo = INT32_MAX, hi = 0;
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
     const int chunks = (total + CHUNK - 1) / CHUNK;
     const int2 live = aw_chunks(a, b, ctx, total);
     const int  first = live.x <= split ? split : split + (live.x - split + splits - 1) / splits * splits;  // of this share
-    const int blocks = (R + rows - 1) / rows;
+    const int blocks = weight_row_blocks(R, rows);
     const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
     // from products to scores in log2 units, or in those of the cap (int8: times the key's scale)
     float factor = a.rule.cap > 0.0f ? a.scale_log2 * a.rule.inv_cap : a.scale_log2;
@@ -839,7 +840,7 @@ hipError_t launch_attention_weights(const WeightArgs& a, bool mfma, hipStream_t 
                 constexpr bool LO = kAwLo<CT, QT>;
                 // as many query rows as the call has, up to kAwRows: the less LDS, the more workgroups per CU
                 WeightArgs w = a;
-                w.block_rows = static_cast<int>(std::min<int64_t>(kAwRows<D, LO>, (R + 15) / 16 * 16));
+                w.block_rows = weight_block_rows(R, kAwRows<D, LO>);
                 const int  lds = aw_lds<D, LO>(w.block_rows, sum);
                 const dim3 n = grid(w.block_rows);
                 if (n.y > 65535u) return hipErrorInvalidConfiguration;
