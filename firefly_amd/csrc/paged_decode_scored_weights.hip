@@ -14,7 +14,8 @@ __global__ __launch_bounds__(256) void paged_decode_weights(ScoredDecodeArgs a)
     constexpr int T = kWeightTokens;
     const int     b = static_cast<int>(blockIdx.z);
     const int     kvh = static_cast<int>(blockIdx.y);
-    const RowSpan s = row_span(a, b);
+    RowSpan       s = row_span(a, b);
+    if (a.num_blocks <= 0) s.lo = s.hi;  // no key is on a page, and some vector kernels then write no scores down
     const int     G = a.group;
     const float2* fin = reinterpret_cast<const float2*>(a.ws_final) + static_cast<int64_t>(b) * a.num_heads + kvh * G;
     const float*  sc = a.ws_scores + score_page(a, b, kvh, 0);

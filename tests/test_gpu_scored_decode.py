@@ -248,3 +248,20 @@ def test_long_row(ff, gpu):
         want = expected(c, r)
         check_out(c, out, want)
         su.check(su.host(w)[0], want[0][2], want[0][3], "weights")
+
+
+@pytest.mark.parametrize("act,kv,Hq,Hkv,D", [("f32", "f32", 16, 2, 128), ("bf16", "bf16", 8, 2, 72), ("f16", "i8", 16, 1, 40),
+                                             ("f32", "f32", 4, 2, 64), ("bf16", "bf16", 8, 2, 128)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_no_pages(ff, gpu, act, kv, Hq, Hkv, D, window):
+    """num_blocks 0: no key is on a page, so the rows' outputs are zeros and their weights the earlier ones decayed, whatever
+    the workspace held."""
+    c = make(31, [300, 5000, 0], Hq, Hkv, D, act, kv)
+    T = 16 * c.max_blocks
+    prior, w = torch.rand(3, Hkv, T, device=gpu), torch.full((3, Hkv, T), -7.0, device=gpu)
+    ws = ff.decode_scored_workspace(3, Hq, D, c.max_blocks, weights=True, device=gpu).fill_(0x7f)
+    out = call(ff, c, su.device(c, gpu), rule_of(c, window=window), weights=w, prior=prior, decay=0.5, workspace=ws, num_blocks=0)
+    assert not out.float().any()
+    for b, n in enumerate([300, 5000, 0]):
+        assert torch.equal(w[b, :, :n], 0.5 * prior[b, :, :n])
+        assert not w[b, :, n].any() and (w[b, :, n + 1:] == -7.0).all()
