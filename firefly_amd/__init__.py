@@ -333,7 +333,8 @@ def paged_attention_noalloc(q, k_cache, v_cache, block_table, context_lens, out,
 def paged_attention(q, k_cache, v_cache, block_table, context_lens, out=None, k_scale=None, v_scale=None,
                     max_context_len: int = 0, scale: float = 0.0, workspace=None, num_blocks: int | None = None,
                     stream=None):
-    """PagedAttention decode (``ffkv_paged_decode``).  ``q`` is ``[B, 1, Hq, D]`` (or ``[B, Hq, D]``)."""
+    """PagedAttention decode (``ffkv_paged_decode``).  ``q`` is ``[B, 1, Hq, D]`` (or ``[B, Hq, D]``).  Give captured calls a
+    workspace: without one they leave their rows whole, which is slower for few or long ones."""
     out = _decode_out(q, out)
     check(_front.decode(q, out, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, max_context_len, scale,
                         num_blocks, workspace, stream))

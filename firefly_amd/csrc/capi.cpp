@@ -454,6 +454,10 @@ int scratch_for_device(void** ptr)
 // nothing; sizes whose partials do not fit it are rejected.
 void* const kNoAlloc = reinterpret_cast<void*>(~uintptr_t{0});
 
+// workspace == kWhole: rows are not split and write no partials, so nothing is held in memory; a shared prefix is attended
+// with the rows' own pages.
+void* const kWhole = reinterpret_cast<void*>(~uintptr_t{1});
+
 int decode_impl(const void* q, void* out, int qo_dtype, const void* k_cache, const void* v_cache, int cache_dtype,
                 const float* k_scale, const float* v_scale, const int32_t* block_table, const int32_t* context_lens,
                 int batch, int num_heads, int num_kv_heads, int head_dim, int block_size, int max_blocks,
@@ -494,14 +498,17 @@ int decode_impl(const void* q, void* out, int qo_dtype, const void* k_cache, con
         return fail(FFKV_ERR_INVALID_ARGUMENT, "shared_blocks %d outside 0 .. max_blocks %d", shared_blocks,
                     max_blocks);
     const bool mfma = ffkv::decode_use_mfma(cache_dtype, group, head_dim);
+    const bool whole = workspace == kWhole;
     // shared-prefix split: matrix-core decode (16- and 8-bit caches; fp32 caches take the plain decode, same results)
-    const int skip = mfma && head_dim_mfma(head_dim)  // the prefix partials' kernel takes 64, 128 and 256
+    const int skip = mfma && !whole && head_dim_mfma(head_dim)  // the prefix partials' kernel takes 64, 128 and 256
                          ? std::min(shared_blocks, static_cast<int>(ceil_div(cap, FFKV_BLOCK_SIZE)))
                          : 0;
     int pfx_chunks = 0, pfx_chunk_pages = 0;
     if (skip > 0) ffkv::prefix_chunking(batch, group, num_kv_heads, skip, pfx_chunks, pfx_chunk_pages);
-    const int  chunk = ffkv::decode_chunk(batch, num_kv_heads, cap);
-    const int  max_chunks = static_cast<int>(ceil_div(cap > 0 ? cap : 1, chunk));
+    const int  most = cap > 0 ? cap : 1;
+    const int  chunk = whole ? static_cast<int>(ceil_div(most, FFKV_BLOCK_SIZE) * FFKV_BLOCK_SIZE)
+                             : ffkv::decode_chunk(batch, num_kv_heads, cap);
+    const int  max_chunks = static_cast<int>(ceil_div(most, chunk));
 
     ffkv::DecodeArgs a{};
     a.qo_dtype = qo_dtype;
@@ -543,9 +550,9 @@ int decode_impl(const void* q, void* out, int qo_dtype, const void* k_cache, con
     if (mfma && skip == 0) a.items = std::min(a.items, ffkv::decode_most_items(batch, cap));
 
     a.cap_tokens = cap;
-    const bool  row = mfma && skip == 0 && ffkv::decode_use_row(a);  // writes no partials
+    const bool  row = mfma && skip == 0 && (whole || ffkv::decode_use_row(a));  // writes no partials
     hipStream_t s = static_cast<hipStream_t>(stream);
-    void*       ws = workspace;
+    void*       ws = whole ? nullptr : workspace;
     bool        owned = false;
     if (ws == kNoAlloc)
     {
@@ -565,6 +572,13 @@ int decode_impl(const void* q, void* out, int qo_dtype, const void* k_cache, con
         }
         else if (ws == nullptr)
         {
+            // No memory is allocated inside a capture (capi_util.h): such a call leaves its rows whole.
+            bool capturing = false;
+            if (const int rc = is_capturing(s, capturing)) return rc;
+            if (capturing)
+                return decode_impl(q, out, qo_dtype, k_cache, v_cache, cache_dtype, k_scale, v_scale, block_table, context_lens,
+                                   batch, num_heads, num_kv_heads, head_dim, block_size, max_blocks, num_blocks,
+                                   max_context_len, scale, 0, kWhole, 0, stream, k_new, v_new);
             hipError_t e = hipMallocAsync(&ws, static_cast<size_t>(need), s);
             if (e != hipSuccess) return hip_fail(e, "decode workspace hipMallocAsync");
             owned = true;

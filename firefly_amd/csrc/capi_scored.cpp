@@ -96,16 +96,14 @@ int prefill_span(int cap_tokens, int group, int window, bool key_end)
     return static_cast<int>(std::min<int64_t>(cap_tokens, static_cast<int64_t>(window) + 128 / group + 2 * FFKV_BLOCK_SIZE));
 }
 
-// Stream-ordered memory for a call without a workspace.  Not while the stream is being captured: a graph of three such calls
-// that allocated and freed inside it has faulted on its first replay.
+// Stream-ordered memory for a call without a workspace; not while the stream is being captured (is_capturing).
 int take_memory(void** ws, int64_t bytes, hipStream_t s)
 {
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    hipError_t             e = hipStreamIsCapturing(s, &status);
-    if (e != hipSuccess) return hip_fail(e, "hipStreamIsCapturing");
-    if (status != hipStreamCaptureStatusNone)
+    bool capturing = false;
+    if (const int rc = is_capturing(s, capturing)) return rc;
+    if (capturing)
         return fail(FFKV_ERR_WORKSPACE, "a captured call needs a workspace, of %lld bytes", static_cast<long long>(bytes));
-    e = hipMallocAsync(ws, static_cast<size_t>(bytes), s);
+    const hipError_t e = hipMallocAsync(ws, static_cast<size_t>(bytes), s);
     return e == hipSuccess ? FFKV_OK : hip_fail(e, "workspace hipMallocAsync");
 }
 

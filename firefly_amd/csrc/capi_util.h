@@ -39,6 +39,16 @@ inline int hip_fail(hipError_t e, const char* what)
     return fail(FFKV_ERR_HIP, "%s: %s (%d)", what, hipGetErrorString(e), static_cast<int>(e));
 }
 
+// Whether `s` is being captured; FFKV_OK or the error.  The library allocates no stream-ordered memory inside a capture: a
+// graph of three calls that each allocated and freed their own faulted on its first replay.
+inline int is_capturing(hipStream_t s, bool& yes)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const hipError_t       e = hipStreamIsCapturing(s, &status);
+    yes = status != hipStreamCaptureStatusNone;
+    return e == hipSuccess ? FFKV_OK : hip_fail(e, "hipStreamIsCapturing");
+}
+
 inline bool is_act(int dt) { return dt == FFKV_DTYPE_F32 || dt == FFKV_DTYPE_F16 || dt == FFKV_DTYPE_BF16; }
 inline bool is_cache(int dt) { return is_act(dt) || dt == FFKV_DTYPE_I8 || dt == FFKV_DTYPE_FP8_E4M3; }
 inline bool quantized(int dt) { return dt == FFKV_DTYPE_I8 || dt == FFKV_DTYPE_FP8_E4M3; }

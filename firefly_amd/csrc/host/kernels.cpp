@@ -3,9 +3,8 @@
 // Shapes and conventions follow the reference dispatcher (src/kernels/attention.cu:452-493): batch = q.shape[0],
 // num_heads = q.shape[2], head_dim = q.shape[3], scale = 1/sqrt(head_dim), the block-table row stride is the
 // max_context_blocks argument, and the launch goes to the thread's default stream.  The decode workspace (split
-// partial results) is cached per (thread, device, stream) and grown outside of stream capture; while a stream is
-// being captured a missing or too-small workspace makes the library allocate stream-ordered memory inside the graph
-// instead (the scored decode, the attention weights and the eviction refuse the call).
+// partial results) is cached per (thread, device, stream) and grown when a call needs more, also while the stream is
+// being captured.
 #include <hip/hip_runtime_api.h>
 
 #include <algorithm>
@@ -73,9 +72,10 @@ struct WorkspaceCache
 };
 thread_local WorkspaceCache t_ws;
 
-// A workspace of at least `bytes` for the current device and the default stream, or nullptr while that stream is
-// being captured and its workspace is too small (the library then allocates stream-ordered memory inside the
-// graph instead; allocating here would be an unsafe call during capture).
+// A workspace of at least `bytes` for the current device and the default stream, or nullptr where there is no memory for
+// it.  While the stream is being captured too: the memory is allocated here, beside the graph, and held like any other
+// workspace, so the address that the graph keeps stays good.  (hipMalloc puts nothing on a stream; a capture forbids its
+// threads such calls unless they say that they mean it, which the relaxed mode does, for this thread and this call.)
 void* workspace(size_t bytes, size_t& have)
 {
     int dev = 0;
@@ -86,19 +86,17 @@ void* workspace(size_t bytes, size_t& have)
         have = ws.bytes;
         return ws.ptr;
     }
+    have = 0;
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(t_stream, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone)
-    {
-        have = 0;
-        return nullptr;
-    }
+    if (hipStreamIsCapturing(t_stream, &cap) != hipSuccess) return nullptr;
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool           capturing = cap != hipStreamCaptureStatusNone;
+    if (capturing && hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) return nullptr;
     const size_t grow = std::max(bytes, 2 * ws.bytes);
     void*        p = nullptr;
-    if (hipMalloc(&p, grow) != hipSuccess)
-    {
-        have = 0;
-        return nullptr;
-    }
+    if (hipMalloc(&p, grow) != hipSuccess) p = nullptr;
+    if (capturing) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    if (p == nullptr) return nullptr;
     if (ws.ptr != nullptr)
     {
         std::lock_guard<std::mutex> lock(g_retired_mu);
