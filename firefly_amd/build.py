@@ -105,9 +105,9 @@ def build_front() -> Path:
 def build_test_shims() -> None:
     """Test-only helpers linked against libffkv.so: the C++-API shims under tests/cpp/ (kernels_api_shim.cpp for
     tests/test_gpu_cxx_api.py, decode_step_shim.cpp for tests/test_gpu_decode_step.py, scored_api_shim.cpp for
-    tests/test_gpu_scored_cxx.py) and engine_calls.bin
+    tests/test_gpu_scored_cxx.py, scored_prompt_shim.cpp for tests/test_gpu_scored_prompt.py) and engine_calls.bin
     (tests/test_hal.py)."""
-    for name in ("kernels_api_shim", "decode_step_shim", "scored_api_shim"):
+    for name in ("kernels_api_shim", "decode_step_shim", "scored_api_shim", "scored_prompt_shim"):
         src = ROOT / "tests" / "cpp" / f"{name}.cpp"
         if not src.exists():
             continue

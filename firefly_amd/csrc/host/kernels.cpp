@@ -363,9 +363,10 @@ void attention_scored(Tensor& q, Tensor& k, Tensor& v, Tensor& output, void* kv_
     const auto* table = reinterpret_cast<const int32_t*>(kv_cache_block_table);
     const int   pages = paged ? static_cast<int>(k.shape()[0]) : 0;
     size_t      have = 0;
-    if (paged && S == 1)
+    if (paged && S == 1 && !rule.prefill)
     {
-        if (rule.key_end != nullptr) return fail("attention_scored: the decode has no key_end");
+        if (rule.key_end != nullptr)
+            return fail("attention_scored: the decode has no key_end (a prompt's chunk of one token sets rule.prefill)");
         int64_t stride = 0;
         if (weights != nullptr && (stride = weight_tokens(*weights, B, kv_head_num)) < 0)
             return fail("attention_scored: weights must be F32 [B, kv_head_num, T] on the GPU");

@@ -140,11 +140,12 @@ struct ScoreRule
     int          window = 0;           ///< keys j <= position - window are hidden; 0: none
     const int*   key_begin = nullptr;  ///< decode [B], prefill and weights [B, S]: first visible key of each query
     const int*   key_end = nullptr;    ///< prefill and weights [B, S]: end of the visible keys (nullptr: causal)
+    bool         prefill = false;      ///< attention_scored: a q of one token is a prompt's chunk, not a decode step
 };
 
 /**
  * @brief attention() under a score rule: the decode when kv_cache_block_table is given and q is [B, 1, Hq, D]
- * (ffkv_paged_decode_scored), else the prefill (ffkv_paged_prefill_scored); tensors as for attention(), scales for
+ * (ffkv_paged_decode_scored; no key_end), else, or with rule.prefill, the prefill (ffkv_paged_prefill_scored); tensors as for attention(), scales for
  * quantized caches.  With weights (decode; F32 [B, Hkv, T]) they become decay * prior plus the attention weight of every
  * cached token (prior may be weights, or nullptr).  max_context_len bounds the rows (0: the table's width); T is at least
  * that bound.
