@@ -359,7 +359,7 @@ size_t ffkv_prefill_scored_workspace_bytes(int qo_dtype, int cache_dtype, int ba
         batch <= 0 || batch > 65535 || seq_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535 ||
         num_heads % num_kv_heads != 0 || (paged != 0 && max_blocks < 0) || window < 0)
         return 0;
-    ffkv::PrefillArgs a{};
+    ffkv::ScoredPrefillArgs a{};
     a.qo_dtype = qo_dtype;
     a.cache_dtype = cache_dtype;
     a.batch = batch;
@@ -413,7 +413,7 @@ int ffkv_paged_prefill_scored(const void* q, void* out, int qo_dtype, const void
     if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))
         return fail(FFKV_ERR_INVALID_ARGUMENT, "q, out, cache and workspace pointers must be 16-byte aligned");
 
-    ffkv::PrefillArgs a{};
+    ffkv::ScoredPrefillArgs a{};
     a.q = q;
     a.out = out;
     a.k_cache = k_cache;

@@ -105,8 +105,13 @@ struct PrefillArgs
     int            split_slots;
     int            split_from;
     int32_t*       ws_pieces;  // [row blocks]: pieces of each
-    // launch_prefill_scored only: the rule, and the most keys that a block of 128 query rows sees (cap_tokens, or a
-    // window's)
+};
+
+// The prefill under a score rule (launch_prefill_scored): the rule, and the most keys that a block of 128 query rows sees
+// (cap_tokens, or a window's).  (A type of its own, as for the decode: 56 bytes more of arguments cost the plain prefill of
+// a few short rows 0.1 of 7 us.)
+struct ScoredPrefillArgs : PrefillArgs
+{
     ScoreRule      rule;
     int            span_tokens;
 };
@@ -253,9 +258,9 @@ void prefill_plan(PrefillArgs& a);
 void prefill_plan_for(PrefillArgs& a, const void* fn, int threads, int step_keys, int most_keys);
 hipError_t launch_prefill_merge(const PrefillArgs& a, hipStream_t stream);  // of a split prefill's pieces
 // The prefill under a score rule (paged_prefill_scored.hip), its plan from a.span_tokens.
-void       prefill_scored_plan(PrefillArgs& a);
-hipError_t launch_prefill_scored(const PrefillArgs& a, hipStream_t stream);
-hipError_t launch_prefill_scored_pieces(const PrefillArgs& a, unsigned wgs, hipStream_t stream);  // its split form's launch
+void       prefill_scored_plan(ScoredPrefillArgs& a);
+hipError_t launch_prefill_scored(const ScoredPrefillArgs& a, hipStream_t stream);
+hipError_t launch_prefill_scored_pieces(const ScoredPrefillArgs& a, unsigned wgs, hipStream_t stream);  // its split form's launch
 struct PrefillSplitLayout
 {
     int64_t pieces, ml, acc, total;  // byte offsets of the three regions and their end (0: no split)

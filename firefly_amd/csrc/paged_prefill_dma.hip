@@ -281,12 +281,14 @@ __device__ __forceinline__ int nth_largest(uint32_t key, int bound, int n, int r
     return __ffsll(static_cast<long long>(hit)) - 1;
 }
 
-// Steps of the query rows of a row with ctx cached tokens, up to the `n`-th of its chunk.  RULE: a window bounds them.
-template <int KP, bool RULE = false>
-__device__ __forceinline__ int row_steps(const PrefillArgs& a, int64_t ctx, int n)
+// Steps of the query rows of a row with ctx cached tokens, up to the `n`-th of its chunk.  Under a rule a window bounds them.
+template <int KP, typename A>
+__device__ __forceinline__ int row_steps(const A& a, int64_t ctx, int n)
 {
     constexpr int KEYS = KP * kBlockSize;
-    const int64_t keys = min(max(ctx + n, int64_t{0}), static_cast<int64_t>(RULE ? a.span_tokens : a.cap_tokens));
+    int64_t       most = a.cap_tokens;
+    if constexpr (std::is_same_v<A, ScoredPrefillArgs>) most = a.span_tokens;
+    const int64_t keys = min(max(ctx + n, int64_t{0}), most);
     return static_cast<int>((keys + KEYS - 1) / KEYS);
 }
 
@@ -295,8 +297,8 @@ __device__ __forceinline__ int row_steps(const PrefillArgs& a, int64_t ctx, int 
 // together at about split_slots (the workgroups resident at once).  The call's steps are summed over its rows at the
 // middle of their chunks.  All blocks of a call are split alike: blocks left whole beside split ones would last the
 // longest.
-template <int KP, bool RULE = false>
-__device__ __forceinline__ int split_len(const PrefillArgs& a, int nrb, int lane)
+template <int KP, typename A>
+__device__ __forceinline__ int split_len(const A& a, int nrb, int lane)
 {
     int64_t total = 0;
     bool    any = false;
@@ -304,9 +306,9 @@ __device__ __forceinline__ int split_len(const PrefillArgs& a, int nrb, int lane
     {
         const bool    in = b0 + lane < a.batch;
         const int64_t ctx = in && a.paged ? a.context_lens[b0 + lane] : 0;
-        any = any || __any(in && row_steps<KP, RULE>(a, ctx, a.seq_len) >= a.split_from);
+        any = any || __any(in && row_steps<KP>(a, ctx, a.seq_len) >= a.split_from);
         if (!any && a.batch <= 64) return 0;
-        total += uniform(wave_sum(in ? row_steps<KP, RULE>(a, ctx, (a.seq_len + 1) / 2) : 0));
+        total += uniform(wave_sum(in ? row_steps<KP>(a, ctx, (a.seq_len + 1) / 2) : 0));
     }
     if (!any) return 0;
     total = total * a.num_kv_heads * nrb + a.split_slots - 1;
@@ -359,7 +361,7 @@ struct PrefillLds
 // RULE: scores are changed and keys hidden by a.rule, each query sees keys [kbeg, kend), and what a query does not see
 // never reaches it, infinite and NaN values included (s_vover is then the first of kRuleFlags ints in LDS).
 template <int QT, int D, int CT, bool PFX, int RG, bool SPLIT = false, bool RULE = false>
-__device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t* s_st0, uint8_t* s_st1,
+__device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_index, uint8_t* s_st0, uint8_t* s_st1,
                                            uint8_t* s_st2, uint8_t* s_st3, int& s_vover)
 {
     constexpr int  W = 8 / RG;  // waves per workgroup
@@ -449,7 +451,7 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         // on int8 pages of 64 dims 131 us, 92 now.  By the rows' lengths alone, the idle pieces of long rows lay
         // between: 4 x 33 tokens over 665 to 950 39 us, 25 now.)  A call that stays whole has at most half the blocks that
         // are resident at once, in any order.
-        len = split_len<KP, RULE>(a, nrb, lane);
+        len = split_len<KP>(a, nrb, lane);
         const int pc = grp / groups0;
         if (len == 0 && pc > 0) return;
         int g8 = (groups - xcd + kXcds - 1) / kXcds, j0 = 0;
@@ -465,11 +467,11 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
             if (lane < g8 && gl < groups)
             {
                 const int pl = gl / groups0;
-                const int st = row_steps<KP, RULE>(a, a.context_lens[(gl - pl * groups0) / Hkv], S);
+                const int st = row_steps<KP>(a, a.context_lens[(gl - pl * groups0) / Hkv], S);
                 const int np = split_pieces(a, st, len);
                 key = pl < np ? st / np : 0;
             }
-            const int hit = nth_largest(static_cast<uint32_t>(key), max(len, row_steps<KP, RULE>(a, a.cap_tokens, 0) / nsp), g8,
+            const int hit = nth_largest(static_cast<uint32_t>(key), max(len, row_steps<KP>(a, a.cap_tokens, 0) / nsp), g8,
                                         k_in_xcd / nrb - j0, lane);
             grp = hit >= 0 ? (j0 + hit) * kXcds + xcd : groups;
         }
@@ -495,7 +497,7 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
 #else
     const int grp = wg_index / nrb;
     const int rb = wg_index % nrb;
-    const int len = SPLIT ? split_len<KP, RULE>(a, nrb, lane) : 0;
+    const int len = SPLIT ? split_len<KP>(a, nrb, lane) : 0;
 #endif
     const int piece = nsp == 1 ? 0 : grp / groups0;
     const int grp0 = grp - piece * groups0;
@@ -530,13 +532,14 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
         if (Lr < 0) Lr = 0;
         L = __builtin_amdgcn_readfirstlane(static_cast<int>(Lr));
     }
+    const ScoreRule rule = rule_in(a);
     // RULE: keys [x, y) that query token t sees, x <= y
     auto visible = [&](int t) -> int2
     {
         const int64_t at = static_cast<int64_t>(b) * S + t;
-        int64_t       hi = a.rule.key_end != nullptr ? a.rule.key_end[at] : ctx + t + 1;
+        int64_t       hi = rule.key_end != nullptr ? rule.key_end[at] : ctx + t + 1;
         hi = hi > L ? L : (hi < 0 ? 0 : hi);
-        int64_t lo = first_key(a.rule, ctx + t, a.rule.key_begin != nullptr ? a.rule.key_begin[at] : 0);
+        int64_t lo = first_key(rule, ctx + t, rule.key_begin != nullptr ? rule.key_begin[at] : 0);
         lo = lo > hi ? hi : lo;
         return make_int2(static_cast<int>(lo), static_cast<int>(hi));
     };
@@ -568,7 +571,7 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
                 kbeg[gi] = col_ok[gi] ? vis.x : 0;
                 kend[gi] = col_ok[gi] ? vis.y : 0;
                 kpos[gi] = static_cast<int>(ctx + t);
-                slope[gi] = a.rule.slopes != nullptr ? a.rule.slopes[hq[gi]] * 1.4426950408889634f : 0.0f;
+                slope[gi] = rule.slopes != nullptr ? rule.slopes[hq[gi]] * 1.4426950408889634f : 0.0f;
             }
             qrow[gi] = (static_cast<size_t>(b) * S + t) * Hq + hq[gi];
         }
@@ -943,8 +946,8 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
     }
     // RULE with a cap or a bias: the scores are brought to log2 units, or those of the cap, first (s_factor), and the softmax
     // takes them as they come out
-    const float s_factor = RULE && a.rule.cap > 0.0f ? c_log2 * a.rule.inv_cap : c_log2;
-    const bool  convert = RULE && (a.rule.cap > 0.0f || a.rule.slopes != nullptr);
+    const float s_factor = RULE && rule.cap > 0.0f ? c_log2 * rule.inv_cap : c_log2;
+    const bool  convert = RULE && (rule.cap > 0.0f || rule.slopes != nullptr);
     if (RULE && convert) c_log2 = 1.0f;
     const float thr_raw = 8.0f / c_log2;
     // int8 pages: on the rerun below every p is scaled by 2^kRerunShift, numerator and denominator alike, so the
@@ -1067,7 +1070,7 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
                 for (int gi = 0; gi < RG; ++gi)
 #pragma unroll
                     for (int u = 0; u < KP; ++u) s[gi][u] *= s_factor;
-                if (a.rule.cap > 0.0f)
+                if (rule.cap > 0.0f)
                 {
 #pragma unroll
                     for (int gi = 0; gi < RG; ++gi)
@@ -1075,12 +1078,12 @@ __device__ __forceinline__ void prefill_wg(PrefillArgs a, int wg_index, uint8_t*
                         float v[KP * 4];
 #pragma unroll
                         for (int e = 0; e < KP * 4; ++e) v[e] = s[gi][e >> 2][e & 3];
-                        cap_scores<KP * 4>(v, a.rule.cap);
+                        cap_scores<KP * 4>(v, rule.cap);
 #pragma unroll
                         for (int e = 0; e < KP * 4; ++e) s[gi][e >> 2][e & 3] = v[e];
                     }
                 }
-                if (a.rule.slopes != nullptr)
+                if (rule.slopes != nullptr)
                 {
 #pragma unroll
                     for (int gi = 0; gi < RG; ++gi)

@@ -18,7 +18,7 @@
 namespace ffkv
 {
 
-hipError_t launch_prefill_scored(const PrefillArgs& a, hipStream_t stream)
+hipError_t launch_prefill_scored(const ScoredPrefillArgs& a, hipStream_t stream)
 {
     const bool    split = a.n_split > 1;
     const int64_t groups = static_cast<int64_t>(a.batch) * a.num_kv_heads * (split ? a.n_split : 1);

@@ -4,7 +4,7 @@
 namespace ffkv
 {
 
-void prefill_scored_plan(PrefillArgs& a)
+void prefill_scored_plan(ScoredPrefillArgs& a)
 {
     prefill_for(a, [&]<int QT, int D, int CT, int RG>()
     {
@@ -13,7 +13,7 @@ void prefill_scored_plan(PrefillArgs& a)
     });
 }
 
-hipError_t launch_prefill_scored_pieces(const PrefillArgs& a, unsigned wgs, hipStream_t stream)
+hipError_t launch_prefill_scored_pieces(const ScoredPrefillArgs& a, unsigned wgs, hipStream_t stream)
 {
     return launch_scored<true>(a, wgs, stream);
 }

@@ -12,7 +12,7 @@ namespace ffkv
 template <int QT, int D, int CT, int RG, bool SPLIT>
 __global__ __launch_bounds__(512 / RG)
 __attribute__((amdgpu_waves_per_eu(RG == 2 ? (D == 256 ? 1 : 2) : 1)))
-void paged_prefill_scored(PrefillArgs a)
+void paged_prefill_scored(ScoredPrefillArgs a)
 {
     using L = PrefillLds<QT, D, CT, false, RG>;
     __shared__ __align__(16) uint8_t s_st0[L::STAGE];
@@ -28,7 +28,7 @@ namespace
 
 // f.operator()<QT, D, CT, RG>() for the call's types and head_dim.
 template <typename F>
-auto prefill_for(const PrefillArgs& a, F f)
+auto prefill_for(const ScoredPrefillArgs& a, F f)
 {
     auto d = [&]<int CT, int QT>()
     {
@@ -55,7 +55,7 @@ namespace
 
 // The main launch, for a grid of `wgs` workgroups.
 template <bool SPLIT>
-hipError_t launch_scored(const PrefillArgs& a, unsigned wgs, hipStream_t stream)
+hipError_t launch_scored(const ScoredPrefillArgs& a, unsigned wgs, hipStream_t stream)
 {
     return prefill_for(a, [&]<int QT, int D, int CT, int RG>()
     {

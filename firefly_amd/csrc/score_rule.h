@@ -64,9 +64,21 @@ __device__ __forceinline__ int64_t first_key(const ScoreRule& r, int64_t pos, in
     return lo;
 }
 
-// What a decode kernel takes, with a rule or without.
+// What a decode kernel, and a prefill kernel, takes, with a rule or without.
 template <bool RULE>
 using KernelArgs = std::conditional_t<RULE, ScoredDecodeArgs, DecodeArgs>;
+template <bool RULE>
+using PrefillKernelArgs = std::conditional_t<RULE, ScoredPrefillArgs, PrefillArgs>;
+
+// The rule of a kernel's arguments: none in a plain kernel's.
+template <typename A>
+__device__ __forceinline__ ScoreRule rule_in(const A& a)
+{
+    if constexpr (requires { a.rule; })
+        return a.rule;
+    else
+        return ScoreRule{};
+}
 
 // Scores that the decode writes down for the weights: [batch, num_kv_heads, pages, group, 16 tokens], so that what a wave
 // writes of a page (up to 16 heads of 64 bytes) is contiguous.
