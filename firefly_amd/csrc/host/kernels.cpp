@@ -150,7 +150,8 @@ void decode(Tensor& q, Tensor& k, Tensor& v, const float* k_scale, const float* 
     const int D = static_cast<int>(q.shape()[3]);
     if (out.numel() < static_cast<int64_t>(B) * Hq * D || out.dtype() != q.dtype())
         return fail("PagedAttention: output must hold B*Hq*D elements of q's dtype");
-    if (k.shape()[2] != kv_head_num || k.shape()[3] != D || v.shape() != k.shape() || v.dtype() != k.dtype())
+    if (k.shape()[1] != FFKV_BLOCK_SIZE || k.shape()[2] != kv_head_num || k.shape()[3] != D ||
+        v.shape() != k.shape() || v.dtype() != k.dtype())
         return fail("PagedAttention: k/v caches must both be [num_blocks, 16, kv_head_num, head_dim]");
     const size_t need = shared_blocks > 0 ? ffkv_decode_shared_prefix_workspace_bytes(B, Hq, kv_head_num, D,
                                                                                        max_context_blocks, 0,
@@ -182,6 +183,8 @@ void prefill(Tensor& q, Tensor& k, Tensor& v, const float* k_scale, const float*
         return fail("attention (prefill): output must hold B*S*Hq*D elements of q's dtype");
     if (k.shape()[2] != kv_head_num || k.shape()[3] != D || v.shape() != k.shape() || v.dtype() != k.dtype())
         return fail("attention (prefill): k/v must be [.., .., kv_head_num, head_dim] and alike");
+    if (block_table != nullptr && k.shape()[1] != FFKV_BLOCK_SIZE)
+        return fail("attention (prefill): k/v caches must both be [num_blocks, 16, kv_head_num, head_dim]");
     if (block_table == nullptr && (k.shape()[0] != B || k.shape()[1] != S))
         return fail("attention (prefill): contiguous k/v must be [B, seq_len, kv_head_num, head_dim]");
     const size_t need = ffkv_prefill_workspace_bytes(code(q.dtype()), code(k.dtype()), B, S, Hq, kv_head_num, D,
@@ -284,8 +287,8 @@ void append_kv_cache_attention(const Tensor& k, const Tensor& v, Tensor& q, Tens
         return fail("append_kv_cache_attention: k / v must be [B, 1, kv_head_num, head_dim]");
     if (output.numel() < static_cast<int64_t>(B) * Hq * D || output.dtype() != q.dtype())
         return fail("append_kv_cache_attention: output must hold B*Hq*D elements of q's dtype");
-    if (k_cache.shape()[2] != kv_head_num || k_cache.shape()[3] != D || v_cache.shape() != k_cache.shape() ||
-        v_cache.dtype() != k_cache.dtype())
+    if (k_cache.shape()[1] != FFKV_BLOCK_SIZE || k_cache.shape()[2] != kv_head_num || k_cache.shape()[3] != D ||
+        v_cache.shape() != k_cache.shape() || v_cache.dtype() != k_cache.dtype())
         return fail("append_kv_cache_attention: k/v caches must both be [num_blocks, 16, kv_head_num, head_dim]");
     const size_t need = ffkv_decode_workspace_bytes(B, Hq, D, max_context_blocks, 0);
     size_t       have = 0;
@@ -360,6 +363,8 @@ void attention_scored(Tensor& q, Tensor& k, Tensor& v, Tensor& output, void* kv_
         return fail("attention_scored: output must hold as many elements of q's dtype as q");
     if (k.shape()[2] != kv_head_num || k.shape()[3] != D || v.shape() != k.shape() || v.dtype() != k.dtype())
         return fail("attention_scored: k/v must be [.., .., kv_head_num, head_dim] and alike");
+    if (paged && k.shape()[1] != FFKV_BLOCK_SIZE)
+        return fail("attention_scored: k/v caches must both be [num_blocks, 16, kv_head_num, head_dim]");
     const auto* table = reinterpret_cast<const int32_t*>(kv_cache_block_table);
     const int   pages = paged ? static_cast<int>(k.shape()[0]) : 0;
     size_t      have = 0;
@@ -405,7 +410,7 @@ void attention_weights(const Tensor& q, const Tensor& k_cache, Tensor& weights, 
         return fail("attention_weights: q must be [B, S, Hq, D] and all tensors on the GPU");
     const int B = static_cast<int>(q.shape()[0]), S = static_cast<int>(q.shape()[1]);
     const int Hq = static_cast<int>(q.shape()[2]), D = static_cast<int>(q.shape()[3]);
-    if (k_cache.shape()[2] != kv_head_num || k_cache.shape()[3] != D)
+    if (k_cache.shape()[1] != FFKV_BLOCK_SIZE || k_cache.shape()[2] != kv_head_num || k_cache.shape()[3] != D)
         return fail("attention_weights: the cache must be [num_blocks, 16, kv_head_num, head_dim]");
     const int64_t stride = weight_tokens(weights, B, kv_head_num);
     if (stride < 0) return fail("attention_weights: weights must be F32 [B, kv_head_num, T] on the GPU");

@@ -30,4 +30,30 @@ int sps_attention(void* q, void* k, void* v, void* out, int* table, int* ctx, in
     return kernels::last_error().empty() ? 0 : -1;
 }
 
+// Call `op` over caches of 4 pages of `block` tokens, nothing of which is read where the call is refused; rows 0: no rows.
+int sps_block_size(int op, int block, int rows)
+{
+    void* const p = reinterpret_cast<void*>(uintptr_t{256});
+    int* const  i = static_cast<int*>(p);
+    const int   S = op == 1 || op == 3 ? 2 : 1;
+    Tensor      q = Tensor::from_external(p, {rows, S, 4, 64}, DType::BF16, Device::GPU);
+    Tensor      o = Tensor::from_external(p, {rows, S, 256}, DType::BF16, Device::GPU);
+    Tensor      n = Tensor::from_external(p, {rows, 1, 2, 64}, DType::BF16, Device::GPU);
+    Tensor      k = Tensor::from_external(p, {4, block, 2, 64}, DType::BF16, Device::GPU);
+    Tensor      v = Tensor::from_external(p, {4, block, 2, 64}, DType::BF16, Device::GPU);
+    Tensor      w = Tensor::from_external(p, {rows, 2, 64}, DType::F32, Device::GPU);
+    const kernels::ScoreRule rule{};
+    switch (op)
+    {
+        case 0:
+        case 1: kernels::attention_scored(q, k, v, o, p, 2, S, 4, i, rule); break;
+        case 2:
+        case 3: kernels::attention(q, k, v, o, p, 2, S, 4, i); break;
+        case 4: kernels::attention_weights(q, k, w, nullptr, 1.0f, i, 2, 4, i, rule); break;
+        case 5: kernels::attention_shared_prefix(q, k, v, o, p, 2, 4, i, 1); break;
+        default: kernels::append_kv_cache_attention(n, n, q, k, v, o, p, 2, 4, i);
+    }
+    return kernels::last_error().empty() ? 0 : -1;
+}
+
 }  // extern "C"

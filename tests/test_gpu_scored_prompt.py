@@ -36,6 +36,15 @@ def test_decode_has_no_key_end(shim):
     assert shim.sps_attention(*a) == 0 and shim.sps_last_error() == b""  # no rows
 
 
+@pytest.mark.parametrize("op", range(7))
+@pytest.mark.parametrize("block", [8, 32])
+def test_block_size(shim, op, block):
+    """Caches whose pages are not of 16 tokens would be read past their end."""
+    assert shim.sps_block_size(op, block, 1) == -1
+    assert b"num_blocks, 16, " in shim.sps_last_error()
+    assert shim.sps_block_size(op, 16, 0) == 0 and shim.sps_last_error() == b""
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("S", [1, 2, 33])
 @pytest.mark.parametrize("ends", [False, True])
