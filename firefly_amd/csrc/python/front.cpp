@@ -11,6 +11,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <climits>
 #include <cstdarg>
 #include <cstdint>
 #include <initializer_list>
@@ -141,8 +142,11 @@ struct Reader
             return 0;
         }
         const long long v = PyLong_AsLongLong(o);
-        if (v == -1 && PyErr_Occurred()) ok = false;
-        return static_cast<int>(v);
+        if (v == -1 && PyErr_Occurred())
+            ok = false;
+        else if (v < INT_MIN || v > INT_MAX)
+            refuse(PyExc_OverflowError, "%lld does not fit in 32 bits", v);
+        return ok ? static_cast<int>(v) : 0;
     }
     int blocks(PyObject* num_blocks, PyObject* cache) { return num_blocks == Py_None ? dim(cache, 0) : integer(num_blocks); }
     float real(PyObject* o)  // whatever float() takes

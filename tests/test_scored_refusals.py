@@ -271,3 +271,23 @@ def test_weights_front_device(ff, S):
     w = torch.zeros(1, HKV, 48)
     with pytest.raises(ValueError, match="GPU"):
         ff.attention_weights(**t, weights=w, prior=w, stream=0)
+
+
+@pytest.mark.parametrize("n", [2 ** 31, 2 ** 32 + 4, -2 ** 31 - 1, 2 ** 63 - 1, -2 ** 80])
+def test_front_integers(ff, n):
+    """An int that does not fit the library's 32 bits is refused, not cut to its lower ones (a window of 2^32 + 4 keys was
+    one of 4)."""
+    t = _tensors()
+    with pytest.raises(OverflowError):
+        ff.paged_attention_scored(**t, window=n, stream=0)
+    with pytest.raises(OverflowError):
+        ff.paged_prefill_scored(**t, max_context_len=n, stream=0)
+    with pytest.raises(OverflowError):
+        ff.paged_attention(**t, max_context_len=n, stream=0)
+    t.pop("v_cache")
+    with pytest.raises(OverflowError):
+        ff.attention_weights(**t, weights=torch.zeros(0, HKV, 48), window=n, stream=0)
+    pool = torch.zeros(4, 16, HKV, D)
+    with pytest.raises(OverflowError):
+        ff.evict_tokens(torch.zeros(0, HKV, 9), pool, pool, t["block_table"], t["context_lens"], 4, sinks=n,
+                        kept=torch.zeros(0, HKV, 4, dtype=torch.int32), stream=0)
