@@ -352,7 +352,7 @@ const float* scale_of(const Tensor* t) { return t ? t->data_as<const float>() : 
 void attention_scored(Tensor& q, Tensor& k, Tensor& v, Tensor& output, void* kv_cache_block_table, int kv_head_num,
                       int seq_len, int max_context_blocks, const int* context_lens, const ScoreRule& rule,
                       const Tensor* k_scale, const Tensor* v_scale, Tensor* weights, const Tensor* prior, float decay,
-                      int max_context_len)
+                      int max_context_len, const Tensor* k_new, const Tensor* v_new)
 {
     if (q.shape().size() != 4 || k.shape().size() != 4 || !is_gpu(q) || !is_gpu(k) || !is_gpu(v) || !is_gpu(output))
         return fail("attention_scored: q must be [B, S, Hq, D] and all tensors on the GPU");
@@ -377,17 +377,25 @@ void attention_scored(Tensor& q, Tensor& k, Tensor& v, Tensor& output, void* kv_
             return fail("attention_scored: weights must be F32 [B, kv_head_num, T] on the GPU");
         if (prior != nullptr && (weights == nullptr || weight_tokens(*prior, B, kv_head_num) != stride))
             return fail("attention_scored: prior must be of the weights' shape");
+        if ((k_new == nullptr) != (v_new == nullptr)) return fail("attention_scored: k_new and v_new come together");
+        for (const Tensor* t : {k_new, v_new})
+            if (t != nullptr && (!is_gpu(*t) || t->shape().size() != 4 || t->shape()[0] != B || t->shape()[1] != 1 ||
+                                 t->shape()[2] != kv_head_num || t->shape()[3] != D || t->dtype() != k_new->dtype()))
+                return fail("attention_scored: k_new and v_new must be [B, 1, kv_head_num, head_dim] of one dtype on the GPU");
         const size_t need = ffkv_decode_scored_workspace_bytes(B, Hq, D, max_context_blocks, max_context_len, weights != nullptr);
         void*        ws = workspace(need, have);
         return report(ffkv_paged_decode_scored(
                           q.data(), output.data(), code(q.dtype()), k.data(), v.data(), code(k.dtype()),
                           const_cast<float*>(scale_of(k_scale)), const_cast<float*>(scale_of(v_scale)), table, context_lens, B, Hq,
                           kv_head_num, D, FFKV_BLOCK_SIZE, max_context_blocks, pages, max_context_len, 0.0f, rule.cap,
-                          rule.slopes, rule.window, rule.key_begin, nullptr, nullptr, code(q.dtype()),
+                          rule.slopes, rule.window, rule.key_begin, k_new ? k_new->data() : nullptr,
+                          v_new ? v_new->data() : nullptr, code(k_new ? k_new->dtype() : q.dtype()),
                           weights ? weights->data_as<float>() : nullptr, scale_of(prior), decay, stride, ws, have, t_stream),
                       "attention_scored failed");
     }
     if (weights != nullptr || prior != nullptr) return fail("attention_scored: weights come with the decode (see attention_weights)");
+    if (k_new != nullptr || v_new != nullptr)
+        return fail("attention_scored (prefill): append the chunk first (append_kv_cache); k_new and v_new come with the decode");
     if (seq_len != S) return fail("attention_scored (prefill): seq_len must equal q.shape()[1]");
     if (!paged && (k.shape()[0] != B || k.shape()[1] != S))
         return fail("attention_scored (prefill): contiguous k/v must be [B, seq_len, kv_head_num, head_dim]");

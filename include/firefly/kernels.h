@@ -148,13 +148,16 @@ struct ScoreRule
  * (ffkv_paged_decode_scored; no key_end), else, or with rule.prefill, the prefill (ffkv_paged_prefill_scored); tensors as for attention(), scales for
  * quantized caches.  With weights (decode; F32 [B, Hkv, T]) they become decay * prior plus the attention weight of every
  * cached token (prior may be weights, or nullptr).  max_context_len bounds the rows (0: the table's width); T is at least
- * that bound.
+ * that bound.  With k_new and v_new (decode; [B, 1, kv_head_num, D] of one dtype, both or neither) the step's new tokens are
+ * appended first, as append_kv_cache_attention does: in the decode's launch where they have the cache's 16-bit dtype, and
+ * then no other row of the call may attend a row's new slot.
  */
 FIREFLY_API void attention_scored(Tensor& q, Tensor& k, Tensor& v, Tensor& output, void* kv_cache_block_table,
                                   int kv_head_num, int seq_len, int max_context_blocks, const int* context_lens,
                                   const ScoreRule& rule, const Tensor* k_scale = nullptr, const Tensor* v_scale = nullptr,
                                   Tensor* weights = nullptr, const Tensor* prior = nullptr, float decay = 1.0f,
-                                  int max_context_len = 0);
+                                  int max_context_len = 0, const Tensor* k_new = nullptr,
+                                  const Tensor* v_new = nullptr);
 
 /**
  * @brief The attention weights that q [B, S, Hq, D], the rows' last S tokens, give to the cached keys

@@ -1,5 +1,5 @@
-"""A prompt's chunks through the C++ API of scored attention (include/firefly/kernels.h), down to one token under a mask,
-against the Python calls: the same bits."""
+"""A prompt's chunks through the C++ API of scored attention (include/firefly/kernels.h), down to one token under a mask, and
+decode steps with their append, against the Python calls: the same bits."""
 
 import ctypes
 import os
@@ -20,6 +20,7 @@ def shim(ff):
     lib = ctypes.CDLL(str(SHIM), mode=os.RTLD_NOW)
     vp, i, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
     lib.sps_attention.argtypes = [vp] * 6 + [i] * 8 + [f, i, vp, vp, i, vp]
+    lib.sps_step.argtypes = [vp] * 8 + [i] * 10 + [vp] * 4 + [i, i, vp]
     lib.sps_last_error.restype = ctypes.c_char_p
     return lib
 
@@ -64,3 +65,34 @@ def test_chunks(ff, gpu, shim, S, ends):
     assert rc == 0, shim.sps_last_error()
     assert torch.equal(want, out)
     assert not ends or not out[1].float().any()
+
+
+def test_new_tokens_refused(shim):
+    a = [256] * 3 + [None, None] + [256] * 3 + [0, 1, 4, 2, 64, 4, 2, 2, 2, 0, 256, 256, None, None, 0, 0, None]
+    assert shim.sps_step(*a) == 0 and shim.sps_last_error() == b""  # no rows
+    for at, value in ((19, None), (18, None), (9, 2), (23, 1)):  # half a pair, two tokens a row, a prompt's chunk
+        b = list(a)
+        b[at] = value
+        assert shim.sps_step(*b) == -1
+        assert b"k_new" in shim.sps_last_error()
+    assert shim.sps_step(*a) == 0 and shim.sps_last_error() == b""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,kv,D", [("bf16", "bf16", 128), ("bf16", "i8", 128), ("f16", "f16", 72), ("f32", "f32", 64)])
+@pytest.mark.parametrize("ctx", [[0, 31, 200], [5000, 9, 777]])
+def test_step_with_append(ff, gpu, shim, act, kv, D, ctx):
+    c = make(9, ctx, 1, 8, 2, D, act, kv)
+    a, b = su.device(c, gpu), su.device(c, gpu)
+    T = 16 * c.max_blocks
+    prior = torch.rand(3, 2, T, device=gpu)
+    w, w2 = torch.zeros_like(prior), torch.zeros_like(prior)
+    want = ff.paged_attention_scored(a[8], *a[:2], a[4], a[5], window=600, k_new=a[6], v_new=a[7], weights=w, prior=prior, decay=0.5,
+                                     k_scale=a[2], v_scale=a[3], max_context_len=T)
+    out = torch.full_like(want, float("nan"))
+    rc = shim.sps_step(_p(b[8]), *map(_p, b[:4]), _p(out), _p(b[4]), _p(b[5]), 3, 1, 8, 2, D, c.num_blocks, c.max_blocks, c.act, c.kv,
+                       600, _p(b[6]), _p(b[7]), _p(w2), _p(prior), T, 0, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, shim.sps_last_error()
+    assert torch.equal(want, out) and torch.equal(w, w2)
+    for x, y in zip(a[:4], b[:4]):
+        assert x is None or torch.equal(x.view(torch.uint8), y.view(torch.uint8))
