@@ -14,8 +14,8 @@
 // Bound by vector work (per score a cap, a maximum or a sum, an exponential, 25 instructions with what is shared) and, with
 // few query rows, by the latency of loads that one chunk after the other waits for.  Measured (32/8 heads of 128 dims): 32
 // tokens over one row of 32.7k, bf16, 47 us (two passes of 22 over 67 MB, the fold 4); 16 x 64 tokens over int8 rows of 400 to
-// 4000 under a cap 146 us (72 and 70; the products alone are 14 each at the rate of a large one, and the vector instructions'
-// issue is 70 % of the time).
+// 4000 under a cap 147 us (72 and 70; the products alone are 14 each at the rate of a large one, and vector instructions
+// take 80 % of the issue slots).
 #include "mfma_common.h"
 #include "score_rule.h"
 #include "weight_rows.h"
@@ -610,7 +610,8 @@ __global__ __launch_bounds__(kAwThreads) __attribute__((amdgpu_waves_per_eu(D <=
 }
 
 // The same with vector arithmetic (fp32 caches, and head dims that the matrix cores do not take): a thread has a key, 32
-// query rows at a time pass by in LDS.
+// query rows at a time pass by in LDS.  Bound by its loads: a thread reads its own key, 32 bytes at a time, and again for every
+// 32 query rows (32/8 heads of 128 dims, fp32: 32 tokens over one row of 32.7k 525 us, 16 x 64 tokens over 400 to 4000 1.5 ms).
 template <int CT, bool SUM>
 __global__ __launch_bounds__(kAwVecThreads) void attention_weights_vector(WeightArgs a)
 {

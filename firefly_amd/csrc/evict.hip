@@ -7,7 +7,8 @@
 //
 // Bound by HBM in the copy and by latency in the choice.  Measured (8 KV heads of 128 dims): 64 int8 rows of 900 to 8000 tokens
 // cut to 1000 87 us (choice 17, copy 62: 4.6 TB/s); one bf16 row of 131k cut to 16k 65 us (choice in parts 30, copy 26:
-// 5.1 TB/s); 4 fp32 rows of 200 to 1000 cut to 256 12.6 us (two launches of 6).
+// 5.1 TB/s); 4 fp32 rows of 200 to 1000 cut to 256 12.6 us (two launches of 6).  In place 82, 207 and 14.5 us: one long row has
+// two workgroups per KV head there (evict_move).
 #include "mfma_common.h"
 
 #include <algorithm>

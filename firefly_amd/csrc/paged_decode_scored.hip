@@ -16,7 +16,8 @@
 //
 // Measured (32/8 heads of 128 dims, bf16): 64 rows of 512 to 4096 tokens behind a window of 1024, capped, 56 us (4.6 TB/s); 8
 // rows of 32k f16 tokens, 28/4 heads, with a distance bias 93 us (5.8 TB/s); 64 rows of 512 to 4096 tokens with their weights 136 us
-// (decode 120, merge 5, weights 9), 106 without; 4 rows of up to 255 tokens 7.6 us in one launch.
+// (decode 120, merge 5, weights 9), 101 without, on int8 pages 92 and 73, on fp8 pages 81 and 69; 32 rows of 512 to 4096 fp32
+// tokens (the vector kernel) 125; 4 rows of up to 255 tokens 7.6 us in one launch.
 #include "decode_scored.h"
 
 namespace ffkv

@@ -11,8 +11,9 @@
 //
 // Bound by vector work and matrix work that overlap in part, as the plain prefill; the cap adds eight vector instructions per
 // score to the softmax's eight.  Measured (32/8 heads of 128 dims): 8 x 512 tokens over 2000 to 2900 cached ones behind a window
-// of 1024 and a cap, bf16, 134 us (512 TFLOP/s of visible pairs); 2000 f16 tokens of several documents 30 to 36 us; 256 tokens over
-// 7.9k on fp8 pages with a distance bias 60 us, split over the keys (8 of it the merge).
+// of 1024 and a cap, bf16, 134 us (512 TFLOP/s of visible pairs); 2000 f16 tokens of several documents 25 to 46 us by the
+// longest one (430 to 1050 tokens); 256 tokens over 7.9k on fp8 pages with a distance bias 60 us, split over the keys (8 of it the
+// merge).
 #include "prefill_scored.h"
 
 namespace ffkv
