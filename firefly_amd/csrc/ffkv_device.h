@@ -436,6 +436,14 @@ __device__ __forceinline__ void load_act4(const void* base, int dt, size_t i, fl
 // NaN where l is NaN (a NaN or infinite score among the keys), whichever launches the row was split over.
 __device__ __forceinline__ float softmax_inv(float l, float scale = 1.0f) { return l == 0.0f ? 0.0f : scale / l; }
 
+// The V scale of a KV head (fp8 caches; 1 elsewhere) for a part of a row with denominator l, whose accumulators are all zero
+// where it met no key: an infinite or NaN scale must not make NaN of those.
+template <int CT>
+__device__ __forceinline__ float seen_scale(float l, float scale)
+{
+    return CT == FP8 && l == 0.0f ? 0.0f : scale;
+}
+
 __device__ __forceinline__ void store_act1(void* base, int dt, size_t i, float x)
 {
     if (dt == F32)

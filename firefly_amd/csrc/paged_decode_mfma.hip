@@ -840,9 +840,10 @@ __device__ __forceinline__ void decode_wg(const KernelArgs<RULE>& a, int item_, 
         {
             const int64_t slot = static_cast<int64_t>(item) + b;
             float*        dst = a.ws_acc + (slot * a.num_heads + h) * D;
+            const float   piece_scale = seen_scale<CT>(l_tot, v_head_scale);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-                *reinterpret_cast<f32x4*>(dst + 16 * n + 4 * g) = acc[n] * v_head_scale;
+                *reinterpret_cast<f32x4*>(dst + 16 * n + 4 * g) = acc[n] * piece_scale;
             if (g == 0)
             {
                 a.ws_ml[(slot * a.num_heads + h) * 2] = m_run;
@@ -920,9 +921,10 @@ __device__ __forceinline__ void decode_wg(const KernelArgs<RULE>& a, int item_, 
         __syncthreads();
         if (c < gc)
         {
+            const float piece_scale = seen_scale<CT>(l_tot, v_head_scale);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-                *reinterpret_cast<f32x4*>(s_acc + (wave * gc + c) * D + 16 * n + 4 * g) = acc[n] * v_head_scale;
+                *reinterpret_cast<f32x4*>(s_acc + (wave * gc + c) * D + 16 * n + 4 * g) = acc[n] * piece_scale;
             if (g == 0) s_ml[wave * 16 + c] = float2{m_run, l_tot};
         }
         __syncthreads();

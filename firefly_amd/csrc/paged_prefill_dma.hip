@@ -1558,10 +1558,11 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
             {
                 const int64_t slot =
                     static_cast<int64_t>(a.pfx_slot0) + static_cast<int64_t>(chunk) * a.batch + bq[gi];
-                float* dst = a.ws_acc + (slot * Hq + hq[gi]) * D;
+                float*      dst = a.ws_acc + (slot * Hq + hq[gi]) * D;
+                const float piece_scale = seen_scale<CT>(l_tot, v_head_scale);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    *reinterpret_cast<f32x4*>(dst + 16 * n + 4 * g) = acc[gi][n] * v_head_scale;
+                    *reinterpret_cast<f32x4*>(dst + 16 * n + 4 * g) = acc[gi][n] * piece_scale;
                 if (g == 0)
                 {
                     // (an int8 rerun scaled p by 2^kRerunShift, which the partial's max carries)
@@ -1579,8 +1580,9 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
             {
                 const int rg = RG * wave + gi;
                 f32x4*    dst = reinterpret_cast<f32x4*>(a.ws_acc) + (part * (kDmaRows / 16) + rg) * NT * 64 + lane;
+                const float piece_scale = seen_scale<CT>(l_tot, v_head_scale);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) dst[n * 64] = acc[gi][n] * v_head_scale;
+                for (int n = 0; n < NT; ++n) dst[n * 64] = acc[gi][n] * piece_scale;
                 if (g == 0)
                 {
                     const float shift = CT == I8 && s_vover != 0 ? kRerunShift : 0.0f;

@@ -253,3 +253,21 @@ def test_streams_and_graph(ff, gpu):
         torch.cuda.synchronize()
         assert torch.equal(call(ff, c, d, r), want)
         assert torch.allclose(out.float(), want.float(), rtol=2.0 ** -7, atol=1e-3)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("ctx", [[6000], [200, 30]])
+def test_fp8_head_scale_not_finite(ff, gpu, bad, ctx):
+    """A head whose V scale is infinite or NaN: queries that see nothing still give zeros, whole and split over the keys, the
+    others nothing finite; the other head is untouched."""
+    c = make(33, ctx, 40, 8, 2, 128, "bf16", "fp8")
+    kp, vp, ks, vs, bt, cx, _, _, q = su.device(c, gpu)
+    end = cx[:, None].repeat(1, 40)
+    end[:, 1::2] = 0
+    call = lambda: ff.paged_prefill_scored(q, kp, vp, bt, cx, key_end=end, k_scale=ks, v_scale=vs).view(len(ctx), 40, 2, -1)  # noqa: E731
+    want = call()
+    vs[0] = bad
+    got = call()
+    assert not got[:, 1::2].float().any()
+    assert not got[:, ::2, 0].isfinite().any()
+    assert torch.equal(got[:, :, 1], want[:, :, 1])

@@ -177,3 +177,26 @@ def test_split_prefill(ff, gpu, act, kv, kind, t):
     tol = 2e-2 if kv in ("i8", "fp8") else 2e-3
     d = np.abs(got - whole)[ok] - 2 * half_ulp(np.maximum(np.abs(got), np.abs(whole))[ok], c.act)
     assert float(d.max()) <= 2 * tol
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("D", [128, 64, 72])
+@pytest.mark.parametrize("ctx", [[200, 40, 16], [5000, 40, 16], [40, 3000, 700]])
+@pytest.mark.parametrize("scored", [False, True])
+def test_fp8_head_scale_not_finite(ff, gpu, bad, D, ctx, scored):
+    """A head whose V scale is infinite or NaN: a row without a valid token still gives zeros in every launch form, the others
+    nothing finite in that head; the other head is untouched."""
+    import torch
+
+    c = cases.make_case(61, 3, 8, 2, D, ctx, act="bf16", kv="fp8")
+    c.block_table[1] = -1
+    dk, dv, q = gu.to_dev(c.k_pool, c.kv, gpu), gu.to_dev(c.v_pool, c.kv, gpu), gu.to_dev(c.q, c.act, gpu)
+    up = lambda a: torch.from_numpy(a.copy()).to(gpu)  # noqa: E731
+    bt, cx, ks, vs = up(c.block_table), up(c.ctx), up(c.k_scale), up(c.v_scale)
+    call = ff.paged_attention_scored if scored else ff.paged_attention
+    want = call(q, dk, dv, bt, cx, k_scale=ks, v_scale=vs).view(3, 2, -1)
+    vs[0] = bad
+    got = call(q, dk, dv, bt, cx, k_scale=ks, v_scale=vs).view(3, 2, -1)
+    assert not got[1].float().any()
+    assert not got[::2, 0].isfinite().any()
+    assert torch.equal(got[:, 1], want[:, 1])
