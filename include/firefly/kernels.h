@@ -34,7 +34,8 @@ FIREFLY_API std::string last_error();
 
 // The decode operators keep one split-K workspace per (thread, device, stream), held for the life of the thread
 // (a graph captured on the stream has its address; a capture may be what first needs it).  Graphs captured on one stream
-// share its workspace: they must not run at the same time, nor beside eager calls on that stream.  release_workspace(stream) synchronizes `stream` and frees
+// share its workspace: they must not run at the same time, nor beside eager calls on that stream.
+// release_workspace(stream) synchronizes `stream` and frees
 // the calling thread's workspace for it on the current device; call it when a stream is retired and no graph
 // captured on it will be replayed again (the next call on that stream allocates a new one).  No counterpart in the
 // reference, whose temporaries are stream-ordered allocations.
