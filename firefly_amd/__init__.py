@@ -115,6 +115,23 @@ def _load() -> ctypes.CDLL:
                                ctypes.c_int64, i32, i32, i32, i32, i32, vp, sz, vp]
     lib.ffkv_evict_workspace_bytes.restype = sz
     lib.ffkv_evict_workspace_bytes.argtypes = [i32, i32, i32, ctypes.c_int64, i32]
+    i64 = ctypes.c_int64
+    axes = [vp, ctypes.POINTER(i32), i32, i32]  # positions, sections, axes, interleaved
+    lib.ffkv_rope_axes.restype = i32
+    lib.ffkv_rope_axes.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i32, *axes, i32, i32, i32, i32, i32, f32, vp]
+    lib.ffkv_rope_append_axes.restype = i32
+    lib.ffkv_rope_append_axes.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, vp, i32, vp, vp, vp, vp, *axes, i32,
+                                          i32, i32, i32, i32, i32, i32, i32, f32, vp]
+    lib.ffkv_key_bounds.restype = i32
+    lib.ffkv_key_bounds.argtypes = [vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp]
+    lib.ffkv_select_blocks_workspace_bytes.restype = sz
+    lib.ffkv_select_blocks_workspace_bytes.argtypes = [i32] * 7
+    lib.ffkv_select_blocks.restype = i32
+    lib.ffkv_select_blocks.argtypes = [vp, i32, vp, i32, vp, vp, vp, *[i32] * 13, vp, sz, vp]
+    lib.ffkv_paged_attention_blocks_workspace_bytes.restype = sz
+    lib.ffkv_paged_attention_blocks_workspace_bytes.argtypes = [i32] * 8
+    lib.ffkv_paged_attention_blocks.restype = i32
+    lib.ffkv_paged_attention_blocks.argtypes = [vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, vp, *[i32] * 10, f32, vp, sz, vp]
     lib.ffkv_last_error.restype = ctypes.c_char_p
     lib.ffkv_last_error.argtypes = []
     lib.ffkv_version.restype = ctypes.c_char_p
@@ -129,7 +146,9 @@ def _bind(lib, torch) -> None:
     names = ("append", "paged_decode", "append_paged_decode", "paged_decode_shared_prefix", "paged_decode_noalloc",
              "prefill_workspace_bytes", "paged_prefill_ws", "rope", "rope_append", "paged_decode_scored",
              "prefill_scored_workspace_bytes", "paged_prefill_scored", "evict", "attention_weights",
-             "decode_scored_scratch_bytes", "attention_weights_workspace_bytes", "evict_workspace_bytes")
+             "decode_scored_scratch_bytes", "attention_weights_workspace_bytes", "evict_workspace_bytes", "rope_axes",
+             "rope_append_axes", "key_bounds", "select_blocks", "select_blocks_workspace_bytes", "paged_attention_blocks",
+             "paged_attention_blocks_workspace_bytes")
     _front.bind(tuple(ctypes.cast(getattr(lib, "ffkv_" + n), ctypes.c_void_p).value for n in names),
                 [*_torch_dtypes(torch).items(), (torch.int32, _INT32)], getattr(torch._C, "_cuda_getDevice", None),
                 getattr(torch._C, "_cuda_getCurrentRawStream", None), lambda: torch.cuda.current_stream().cuda_stream)
@@ -442,3 +461,97 @@ def evict_tokens(weights, k_cache, v_cache, block_table, context_lens, keep: int
     check(_front.evict(weights, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, keep, sinks, recent, dst_table,
                        kept, kept_lens, weights_out, num_blocks, workspace, stream, _prefill_scratch))
     return kept, kept_lens
+
+
+def apply_rope_axes(q, k, positions, sections, interleaved: bool = False, theta: float = 1e6, q_out=None, k_out=None,
+                    stream=None):
+    """Rotary embedding by positions on several axes (``ffkv_rope_axes``): ``q`` ``[B, S, Hq, D]`` (or None) and ``k``
+    ``[B, S, Hkv, D]``, views into a packed projection among them, turned by ``positions`` int32 ``[axes, B, S]``.
+    ``sections`` has the pairs of dims of each axis, D / 2 together, one section behind the other, or dealt out in turn
+    (``interleaved``).  In place, or into ``q_out`` / ``k_out``.  Returns the two."""
+    q_out = q if q_out is None else q_out
+    k_out = k if k_out is None else k_out
+    check(_front.rope_axes(q, k, positions, sections, interleaved, theta, q_out, k_out, stream))
+    return q_out, k_out
+
+
+def rope_append_axes(q, k, v, positions, sections, k_cache, v_cache, block_table, context_lens=None,
+                     interleaved: bool = False, theta: float = 1e6, q_out=None, k_scale=None, v_scale=None,
+                     num_blocks: int | None = None, stream=None):
+    """``apply_rope_axes(q, k)`` then ``append_kv_cache(k, v, ...)`` in one kernel (``ffkv_rope_append_axes``): q is turned in
+    place or into ``q_out``; k and v are only read, the rotated k is in the pages alone.  Returns the rotated q."""
+    q_out = q if q_out is None else q_out
+    check(_front.rope_append_axes(q, k, v, positions, sections, interleaved, theta, k_cache, v_cache, block_table, context_lens,
+                                  q_out, k_scale, v_scale, num_blocks, stream))
+    return q_out
+
+
+def key_bounds(k_cache):
+    """Memory for the key bounds of a pool of K pages: ``[N, Hkv, 2, D]`` of the cache's type, bf16 beside 8-bit caches."""
+    import torch
+
+    n, _, heads, dim = k_cache.shape
+    eight = k_cache.element_size() == 1
+    return torch.empty((n, heads, 2, dim), dtype=torch.bfloat16 if eight else k_cache.dtype, device=k_cache.device)
+
+
+def update_key_bounds(k_cache, bounds, block_table, context_lens, new_tokens: int, k_scale=None,
+                      num_blocks: int | None = None, stream=None) -> None:
+    """The smallest and largest key, per KV head and dim, of the pages that the rows' tokens ``context_lens[b] ..
+    context_lens[b] + new_tokens - 1`` lie on, into ``bounds`` (``ffkv_key_bounds``; see ``key_bounds``).  Call it after every
+    append to rows that ``select_blocks`` will choose from."""
+    check(_front.key_bounds(k_cache, bounds, block_table, context_lens, new_tokens, k_scale, num_blocks, stream))
+
+
+def select_blocks_workspace(batch: int, seq_len: int, num_kv_heads: int, count: int, query_block: int, max_blocks: int,
+                            max_context_len: int = 0, device=None):
+    """A workspace for ``select_blocks`` (``ffkv_select_blocks_workspace_bytes``)."""
+    import torch
+
+    n = int(lib.ffkv_select_blocks_workspace_bytes(batch, seq_len, num_kv_heads, count, query_block, max_blocks, max_context_len))
+    return torch.empty(max(n, 256), dtype=torch.uint8, device=device if device is not None else "cuda")
+
+
+def select_blocks(q, bounds, block_table, context_lens, count: int, sinks: int = 1, recent: int = 1, query_block: int = 1,
+                  blocks=None, max_context_len: int = 0, workspace=None, num_blocks: int | None = None, stream=None):
+    """The ``count`` pages of its row that every block of ``query_block`` queries attends, per KV head (``ffkv_select_blocks``):
+    the first ``sinks``, the last ``recent`` (up to the block's last query's), and those whose key ``bounds`` allow the largest
+    scores, summed over the block's queries and the KV head's query heads.  ``q`` ``[B, S, Hq, D]`` at ``context_lens[b] + t``.
+    Returns ``blocks`` int32 ``[B, ceil(S / query_block), Hkv, count]``, ascending, -1 behind a row of fewer pages.  A captured
+    call needs a workspace (``select_blocks_workspace``) unless no row can have more than ``count`` pages."""
+    if blocks is None:
+        import torch
+
+        lists = -(-q.shape[1] // query_block) if query_block > 0 else 0
+        blocks = torch.empty((q.shape[0], lists, bounds.shape[1], max(0, count)), dtype=torch.int32, device=q.device)
+    check(_front.select_blocks(q, bounds, block_table, context_lens, count, sinks, recent, query_block, blocks, max_context_len,
+                               workspace, num_blocks, stream, _prefill_scratch))
+    return blocks
+
+
+def attention_blocks_workspace(cache_dtype: int, batch: int, seq_len: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                               count: int, query_block: int = 1, device=None):
+    """A workspace for ``paged_attention_blocks`` (``ffkv_paged_attention_blocks_workspace_bytes``)."""
+    import torch
+
+    n = int(lib.ffkv_paged_attention_blocks_workspace_bytes(cache_dtype, batch, seq_len, num_heads, num_kv_heads, head_dim, count,
+                                                            query_block))
+    return torch.empty(max(n, 256), dtype=torch.uint8, device=device if device is not None else "cuda")
+
+
+def paged_attention_blocks(q, k_cache, v_cache, block_table, context_lens, blocks, query_block: int = 1, out=None,
+                           k_scale=None, v_scale=None, scale: float = 0.0, workspace=None, num_blocks: int | None = None,
+                           stream=None):
+    """Causal attention over listed pages alone (``ffkv_paged_attention_blocks``): ``q`` ``[B, S, Hq, D]`` (a step's also
+    ``[B, Hq, D]``) at ``context_lens[b] + t``, ``blocks`` int32 ``[B, ceil(S / query_block), Hkv, count]`` the logical pages of
+    every ``query_block`` queries per KV head, in any order; entries that are no page of the row (-1) count for nothing.
+    Returns ``out`` ``[B, S, Hq * D]``.  Give captured calls of few lists a workspace (``attention_blocks_workspace``): without
+    one they leave them whole, which is slower."""
+    if out is None:
+        import torch
+
+        seq = q.shape[1] if q.dim() == 4 else 1
+        out = torch.empty((q.shape[0], seq, q.shape[-2] * q.shape[-1]), dtype=q.dtype, device=q.device)
+    check(_front.attention_blocks(q, out, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, blocks, query_block, scale,
+                                  workspace, num_blocks, stream, _prefill_scratch))
+    return out

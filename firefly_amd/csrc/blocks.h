@@ -1,0 +1,133 @@
+// blocks.h - argument blocks and launchers of rotary positions on several axes, the pages' key bounds, the choice of pages
+// and the attention over chosen pages.
+#pragma once
+
+#include "ffkv_internal.h"
+
+namespace ffkv
+{
+
+constexpr int kMaxAxes = 4;
+
+struct RopeAxesArgs
+{
+    const void*    q;  // [batch, seq_len, num_heads, head_dim], q_stride elements from token to token; null without q
+    const void*    k;
+    const void*    v;      // null: rotate only
+    void*          q_out;  // the same (may be q), out_stride of its own
+    void*          k_out;  // rotate only; null: the rotated key goes to the pages alone
+    void*          k_cache;  // null: rotate only
+    void*          v_cache;
+    float*         k_scale;
+    float*         v_scale;
+    const int32_t* block_table;
+    const int32_t* context_lens;
+    const int32_t* positions;  // [axes, batch, seq_len]
+    int64_t        q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+    double         rate_log2;  // log2 of the ratio of neighbouring pairs' frequencies: -2 log2(theta) / head_dim
+    int            section_end[kMaxAxes];  // sections: first pair past axis a's; interleaved: pairs of axis a
+    int            axes;
+    int            interleaved;
+    int            src_dtype;
+    int            cache_dtype;
+    int            batch;
+    int            seq_len;
+    int            num_heads;
+    int            num_kv_heads;
+    int            head_dim;
+    int            max_blocks;
+    int            num_blocks;
+};
+
+struct KeyBoundsArgs
+{
+    const void*    k_cache;
+    const float*   k_scale;
+    void*          bounds;  // [num_blocks, num_kv_heads, 2, head_dim]
+    const int32_t* block_table;
+    const int32_t* context_lens;
+    int            cache_dtype;
+    int            batch;
+    int            new_tokens;
+    int            num_kv_heads;
+    int            head_dim;
+    int            max_blocks;
+    int            num_blocks;
+};
+
+struct SelectArgs
+{
+    const void*    q;       // [batch, seq_len, num_heads, head_dim]
+    const void*    bounds;  // [num_blocks, num_kv_heads, 2, head_dim]
+    const int32_t* block_table;
+    const int32_t* context_lens;
+    int32_t*       blocks;  // [batch, lists, num_kv_heads, count]
+    float*         scores;  // workspace [batch, lists, num_kv_heads, stride]
+    int64_t        stride;
+    int            q_dtype;
+    int            bounds_dtype;
+    int            batch;
+    int            seq_len;
+    int            num_heads;
+    int            num_kv_heads;
+    int            group;
+    int            head_dim;
+    int            max_blocks;
+    int            num_blocks;
+    int            most_pages;  // of a row
+    int            query_block;
+    int            lists;  // per row: blocks of queries
+    int            count;
+    int            sinks;
+    int            recent;
+};
+
+struct BlocksArgs
+{
+    const void*    q;  // [batch, seq_len, num_heads, head_dim]
+    void*          out;
+    const void*    k_cache;
+    const void*    v_cache;
+    const float*   k_scale;
+    const float*   v_scale;
+    const int32_t* block_table;
+    const int32_t* context_lens;
+    const int32_t* blocks;  // [batch, lists, num_kv_heads, count]
+    int            qo_dtype;
+    int            cache_dtype;
+    int            batch;
+    int            seq_len;
+    int            num_heads;
+    int            num_kv_heads;
+    int            group;
+    int            head_dim;
+    int            max_blocks;
+    int            num_blocks;
+    int            query_block;
+    int            lists;
+    int            count;
+    int            splits;  // pieces of a list, each by a workgroup of its own
+    float          scale_log2;
+    float2*        ws_ml;   // [batch * seq_len * num_heads, splits]: (max in the log2 domain, denominator)
+    float*         ws_acc;  // [batch * seq_len * num_heads, splits, head_dim]: unnormalised output
+};
+
+// Which kernel attends: the decode's on the matrix cores (a list per token), the prefill's (a list per block of tokens), or
+// the vector kernel (fp32 caches, other head dims).
+enum class BlocksKernel
+{
+    kDecode,
+    kPrefill,
+    kVector,
+};
+BlocksKernel blocks_kernel(const BlocksArgs& a);
+int          blocks_splits(const BlocksArgs& a);  // sizes and types of `a` set
+
+hipError_t launch_rope_axes(const RopeAxesArgs& a, hipStream_t stream);
+hipError_t launch_key_bounds(const KeyBoundsArgs& a, hipStream_t stream);
+hipError_t launch_select(const SelectArgs& a, hipStream_t stream);
+hipError_t launch_blocks(const BlocksArgs& a, hipStream_t stream);
+hipError_t launch_blocks_decode(const BlocksArgs& a, hipStream_t stream);
+hipError_t launch_blocks_prefill(const BlocksArgs& a, hipStream_t stream);
+
+}  // namespace ffkv

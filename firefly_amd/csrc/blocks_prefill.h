@@ -1,0 +1,51 @@
+// blocks_prefill.h - the prefill over listed pages: its kernel, instantiated by paged_blocks_prefill_*.hip for a type of cache
+// each (files of their own, as each takes a minute to compile).
+#pragma once
+
+#define FFKV_DEVICE_BODIES_ONLY 1
+#include "paged_prefill_dma.hip"
+#undef FFKV_DEVICE_BODIES_ONLY
+
+namespace ffkv
+{
+
+template <int QT, int D, int CT, int RG>
+__global__ __launch_bounds__(512 / RG)
+__attribute__((amdgpu_waves_per_eu(RG == 2 ? (D == 256 ? 1 : 2) : 1)))
+void paged_blocks_prefill(ListPrefillArgs a)
+{
+    using L = PrefillLds<QT, D, CT, false, RG>;
+    __shared__ __align__(16) uint8_t s_st0[L::STAGE];
+    __shared__ __align__(16) uint8_t s_st1[L::STAGE];
+    __shared__ __align__(16) uint8_t s_st2[L::S2];
+    __shared__ __align__(16) uint8_t s_st3[L::S3];
+    __shared__ int s_flags[kRuleFlags];
+    prefill_wg<QT, D, CT, false, RG, false, true, true>(a, static_cast<int>(blockIdx.x), s_st0, s_st1, s_st2, s_st3, s_flags[0]);
+}
+
+// One type of cache's launch.
+template <int CT>
+hipError_t launch_blocks_prefill_t(const ListPrefillArgs& a, hipStream_t stream)
+{
+    const int64_t groups = static_cast<int64_t>(a.batch) * a.lists * a.num_kv_heads;
+    const int64_t nrb = (static_cast<int64_t>(a.query_block) * a.group + kDmaRows - 1) / kDmaRows;
+    const int64_t wgs = (groups + kXcds - 1) / kXcds * kXcds * nrb;
+    if (wgs <= 0) return hipSuccess;
+    if (wgs > INT32_MAX) return hipErrorInvalidConfiguration;
+    auto go = [&]<int QT, int D, int RG>()
+    {
+        hipLaunchKernelGGL((paged_blocks_prefill<QT, D, CT, RG>), dim3(static_cast<unsigned>(wgs)), dim3(512 / RG), 0, stream, a);
+        return hipGetLastError();
+    };
+    auto d = [&]<int QT>()
+    {
+        if (a.head_dim == 64) return go.template operator()<QT, 64, FFKV_PREFILL_RG>();
+        if (a.head_dim == 128) return go.template operator()<QT, 128, FFKV_PREFILL_RG>();
+        return go.template operator()<QT, 256, FFKV_PREFILL_RG256>();
+    };
+    if (a.qo_dtype == F32) return d.template operator()<F32>();
+    if (a.qo_dtype == F16) return d.template operator()<F16>();
+    return d.template operator()<BF16>();
+}
+
+}  // namespace ffkv

@@ -116,6 +116,16 @@ struct ScoredPrefillArgs : PrefillArgs
     int            span_tokens;
 };
 
+// The prefill over listed pages (launch_blocks_prefill): every block of query_block tokens of a row has a list of `count`
+// logical pages per KV head.
+struct ListPrefillArgs : ScoredPrefillArgs
+{
+    const int32_t* blocks;  // [batch, lists, num_kv_heads, count]
+    int            lists;
+    int            count;
+    int            query_block;
+};
+
 struct DecodeArgs
 {
     const void*    q;
@@ -261,6 +271,11 @@ hipError_t launch_prefill_merge(const PrefillArgs& a, hipStream_t stream);  // o
 void       prefill_scored_plan(ScoredPrefillArgs& a);
 hipError_t launch_prefill_scored(const ScoredPrefillArgs& a, hipStream_t stream);
 hipError_t launch_prefill_scored_pieces(const ScoredPrefillArgs& a, unsigned wgs, hipStream_t stream);  // its split form's launch
+// The prefill over listed pages (paged_blocks_prefill_*.hip), by the cache's type.
+hipError_t launch_blocks_prefill_bf16(const ListPrefillArgs& a, hipStream_t stream);
+hipError_t launch_blocks_prefill_f16(const ListPrefillArgs& a, hipStream_t stream);
+hipError_t launch_blocks_prefill_i8(const ListPrefillArgs& a, hipStream_t stream);
+hipError_t launch_blocks_prefill_fp8(const ListPrefillArgs& a, hipStream_t stream);
 struct PrefillSplitLayout
 {
     int64_t pieces, ml, acc, total;  // byte offsets of the three regions and their end (0: no split)

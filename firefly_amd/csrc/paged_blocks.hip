@@ -1,0 +1,737 @@
+// paged_blocks.hip - attention over listed pages of the cache alone: every query token and KV head has a list of its row's
+// pages (logical ones, in any order; entries that are none, or past the query, count for nothing).
+//
+//   out[b, t, h] = sum over listed pages and their tokens j <= context_lens[b] + t of softmax_j(scale q.k_j) v_j
+//
+// Bound by HBM: the listed pages are read once, at about Hq / Hkv operations a byte.
+//
+// On the matrix cores (16- and 8-bit caches) a workgroup of four waves takes a list, or a piece of one, and up to 16 query
+// heads of its KV head; a wave takes every fourth page, with the products and the page loads of the plain decode
+// (paged_decode_mfma.hip): S^T = K Q^T with K from its registers, an online softmax, O^T += V^T P^T with V^T read transposed
+// from LDS.  Lane l holds the list's entry 64 k + l and its page, so a page's address waits for no load.  The waves' states
+// meet in LDS; pieces of a list go to the workspace and blocks_merge folds them.
+//
+// fp32 caches and the other head dims take the vector kernel: 16 (head_dim 256: 32) lanes per token, four query heads a
+// workgroup.
+#define FFKV_DEVICE_BODIES_ONLY 1
+#include "paged_decode_mfma.hip"
+#undef FFKV_DEVICE_BODIES_ONLY
+#include "blocks.h"
+
+#include <algorithm>
+
+namespace ffkv
+{
+
+namespace
+{
+
+constexpr int kBlocksWaves = 4;
+
+// LDS of a workgroup of up to `heads` query heads: the waves' V tiles, and over them their accumulators and (max,
+// denominator) pairs once all pages are done.
+template <int D>
+constexpr int blocks_lds_bytes(int heads)
+{
+    const int v = kBlocksWaves * kBlockSize * D * 2;
+    const int state = kBlocksWaves * heads * D * 4 + kBlocksWaves * 16 * 8;
+    return v > state ? v : state;
+}
+static_assert(blocks_lds_bytes<256>(16) <= 160 * 1024, "a workgroup's LDS fits a CU");
+
+// One page in flight.
+template <int NW, int NWV>
+struct ListedPage
+{
+    u32x4 k[NW];
+    u32x4 v[NWV];
+    int   n_tok;  // its visible tokens; 0: none of it
+    float ks, vs; // int8: K and V scale of token c
+};
+
+// Entry e of a list: the logical page, or -1 where it is none of the row's visible pages.
+__device__ __forceinline__ int listed_page(const BlocksArgs& a, const int32_t* list, int e, int end, int64_t pos)
+{
+    const int lp = e < end ? list[e] : -1;
+    return lp >= 0 && lp < a.max_blocks && static_cast<int64_t>(lp) * kBlockSize <= pos ? lp : -1;
+}
+
+// A state of (max, denominator, accumulator) to the output, or to its piece's place in the workspace.
+template <int QT>
+__device__ __forceinline__ void store_state4(const BlocksArgs& a, int64_t row_h, int split, int D, int d4, float M, float L, f32x4 o)
+{
+    if (a.splits == 1)
+    {
+        store_out4<QT>(a.out, static_cast<size_t>(row_h) * D + d4, o * softmax_inv(L));
+        return;
+    }
+    *reinterpret_cast<f32x4*>(a.ws_acc + (row_h * a.splits + split) * D + d4) = o;
+    if (d4 == 0) a.ws_ml[row_h * a.splits + split] = float2{M, L};
+}
+
+}  // namespace
+
+template <int CT, int QT, int D>
+__global__ __launch_bounds__(64 * kBlocksWaves) __attribute__((amdgpu_waves_per_eu(2, 8)))
+void paged_blocks_decode(BlocksArgs a)
+{
+    extern __shared__ __align__(16) uint8_t s_blocks[];
+    constexpr bool BF = kBF<CT, QT>;
+    constexpr bool VBF = CT == BF16 || (kElemBytes<CT> == 1 && BF && !FFKV_DECODE_V16);
+    using M = MType<BF>;
+    using MV = MType<VBF>;
+    using X8 = typename M::x8;
+    static_assert(D % 32 == 0, "whole k-steps of 32 dims");
+    constexpr int  KSTEPS = D / 32;
+    constexpr int  NT = D / 16;
+    constexpr bool NEED_LO = !((QT == BF16 && BF) || (QT == F16 && !BF));
+    constexpr bool P_LO = VBF;
+    constexpr int  DEPTH = D == 256 ? 1 : 2;
+    constexpr int  EB = kElemBytes<CT>;
+    constexpr int  NW = EB == 2 ? KSTEPS : (KSTEPS + 1) / 2;
+    constexpr int  VCPR = D * EB / 16;
+    constexpr int  NWV = (kBlockSize * VCPR + 63) / 64;
+    auto dimof = [](int j, int g)
+    {
+        if constexpr (EB == 1 && KSTEPS % 2 == 1)
+            if (j == KSTEPS - 1) return 32 * j + 8 * g;
+        return dim_of<CT>(j, g);
+    };
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int wave = uniform(static_cast<int>(threadIdx.x) >> 6);
+    const int c = lane & 15;
+    const int g = lane >> 4;
+    const int G = a.group;
+    const int HB = (G + 15) >> 4;
+    const int y = a.num_kv_heads * HB;
+    int64_t   id = blockIdx.x;
+    const int split = static_cast<int>(id % a.splits);
+    id /= a.splits;
+    const int     vh = static_cast<int>(id % y);
+    const int64_t row = id / y;  // b * seq_len + t
+    const int     b = static_cast<int>(row / a.seq_len);
+    const int     kvh = vh / HB;
+    const int     h0 = (vh - kvh * HB) * 16;
+    const int     gc = min(16, G - h0);
+    const int64_t pos = static_cast<int64_t>(a.context_lens[b]) + (row - static_cast<int64_t>(b) * a.seq_len);
+    const int32_t* list = a.blocks + (row * a.num_kv_heads + kvh) * a.count;
+    const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
+    // this wave's entries: begin + kBlocksWaves i, i < n
+    const int begin = static_cast<int>(static_cast<int64_t>(a.count) * split / a.splits) + wave;
+    const int end = static_cast<int>(static_cast<int64_t>(a.count) * (split + 1) / a.splits);
+    const int n = end > begin ? (end - begin + kBlocksWaves - 1) / kBlocksWaves : 0;
+    uint16_t* sv = reinterpret_cast<uint16_t*>(s_blocks) + wave * (kBlockSize * D);
+
+    float kv_scale_log2 = a.scale_log2;
+    float v_head_scale = 1.0f;
+    if constexpr (CT == FP8)
+    {
+        kv_scale_log2 *= a.k_scale[kvh];
+        v_head_scale = a.v_scale[kvh];
+    }
+
+    const int v_row_bytes = a.num_kv_heads * D * EB;
+    auto      v_tok = [&](int j) { return (64 * j + lane) / VCPR; };
+    auto      v_chk = [&](int j) { return (64 * j + lane) % VCPR; };
+
+    int  tb = 0, lvec, pvec;  // lane l: logical and physical page of entry tb + l
+    auto load_entries = [&]()
+    {
+        lvec = listed_page(a, list, begin + kBlocksWaves * (tb + lane), end, pos);
+        pvec = lvec >= 0 ? table[lvec] : -1;
+    };
+    load_entries();
+    int  next = 0;
+    auto load_next = [&](ListedPage<NW, NWV>& r)
+    {
+        if (next - tb >= 64)
+        {
+            tb += 64;
+            load_entries();
+        }
+        const int lp = __builtin_amdgcn_readlane(lvec, next - tb);
+        const int phys = __builtin_amdgcn_readlane(pvec, next - tb);
+        ++next;
+        r.n_tok = phys >= 0 && phys < a.num_blocks
+                      ? static_cast<int>(min(pos + 1 - static_cast<int64_t>(lp) * kBlockSize, static_cast<int64_t>(kBlockSize)))
+                      : 0;
+        if (r.n_tok <= 0) return;
+        const size_t row_c = (static_cast<size_t>(phys) * kBlockSize + c) * a.num_kv_heads + kvh;
+        if constexpr (CT == I8)
+        {
+            r.ks = a.k_scale[row_c];
+            r.vs = a.v_scale[row_c];
+        }
+        const char* kp = static_cast<const char*>(a.k_cache) + row_c * D * EB;
+        const char* vpage = static_cast<const char*>(a.v_cache) +
+                            (static_cast<size_t>(phys) * kBlockSize * a.num_kv_heads + kvh) * D * EB;
+        if constexpr (EB == 2)
+        {
+#pragma unroll
+            for (int j = 0; j < KSTEPS; ++j) r.k[j] = *reinterpret_cast<const u32x4*>(kp + dim_of<CT>(j, g) * 2);
+        }
+        else
+        {
+#pragma unroll
+            for (int j = 0; j < KSTEPS; j += 2)
+            {
+                if (j + 1 < KSTEPS)
+                    r.k[j / 2] = *reinterpret_cast<const u32x4*>(kp + dimof(j, g));
+                else  // an odd last k-step: its 8 codes alone
+                {
+                    const u32x2 tk = *reinterpret_cast<const u32x2*>(kp + dimof(j, g));
+                    r.k[j / 2] = u32x4{tk[0], tk[1], 0u, 0u};
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NWV; ++j)
+            r.v[j] = v_tok(j) < kBlockSize
+                         ? load16<FFKV_DECODE_NT_V>(vpage + static_cast<uint32_t>(v_tok(j) * v_row_bytes + 16 * v_chk(j)))
+                         : u32x4{0u, 0u, 0u, 0u};
+    };
+
+    // Q of the head block as MFMA B operands (column c = head, zero beyond it)
+    X8 qhi[KSTEPS], qlo[KSTEPS];
+#pragma unroll
+    for (int j = 0; j < KSTEPS; ++j)
+    {
+        const size_t at = (static_cast<size_t>(row) * a.num_heads + kvh * G + h0 + c) * D + dimof(j, g);
+        if constexpr (!NEED_LO)
+        {
+            u32x4 w = u32x4{0u, 0u, 0u, 0u};
+            if (c < gc) w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
+            qhi[j] = qlo[j] = __builtin_bit_cast(X8, w);
+        }
+        else
+        {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+            if (c < gc) load_q8<QT>(a.q, at, x);
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                hi[e] = M::bits(x[e]);
+                lo[e] = M::bits(x[e] - M::value(hi[e]));
+            }
+            qhi[j] = __builtin_bit_cast(X8, u32x4{hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16), hi[4] | (hi[5] << 16),
+                                                  hi[6] | (hi[7] << 16)});
+            qlo[j] = __builtin_bit_cast(X8, u32x4{lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16), lo[4] | (lo[5] << 16),
+                                                  lo[6] | (lo[7] << 16)});
+        }
+    }
+
+    float m_run = kLowest, l_run = 0.0f;
+    f32x4 acc[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // V rows into the wave's LDS tile (zero past the visible tokens) and the scores S^T = K Q^T; consumes r.k and r.v
+    auto stage_page = [&](const ListedPage<NW, NWV>& r, f32x4& s)
+    {
+#pragma unroll
+        for (int j = 0; j < NWV; ++j)
+        {
+            const int t = v_tok(j);
+            if (t >= kBlockSize) continue;
+            const bool  ok = t < r.n_tok;
+            const u32x4 zero = u32x4{0u, 0u, 0u, 0u};
+            if constexpr (EB == 2)
+                *reinterpret_cast<u32x4*>(sv + vt_pos<D>(t, 8 * v_chk(j))) = ok ? r.v[j] : zero;
+            else
+            {
+                *reinterpret_cast<u32x4*>(sv + vt_pos<D>(t, 16 * v_chk(j))) =
+                    ok ? codes_to_m<CT, VBF>(r.v[j][0], r.v[j][1]) : zero;
+                *reinterpret_cast<u32x4*>(sv + vt_pos<D>(t, 16 * v_chk(j) + 8)) =
+                    ok ? codes_to_m<CT, VBF>(r.v[j][2], r.v[j][3]) : zero;
+            }
+        }
+        s = f32x4{0.0f, 0.0f, 0.0f, 0.0f};  // lane (c, g): tokens 4g + i of head c
+#pragma unroll
+        for (int j = 0; j < KSTEPS; ++j)
+        {
+            u32x4 w;
+            if constexpr (EB == 2)
+                w = r.k[j];
+            else
+                w = (j & 1) ? codes_to_m<CT, BF>(r.k[j / 2][2], r.k[j / 2][3]) : codes_to_m<CT, BF>(r.k[j / 2][0], r.k[j / 2][1]);
+            const X8 kj = __builtin_bit_cast(X8, w);
+            s = M::mma32(kj, qhi[j], s);
+            if constexpr (NEED_LO) s = M::mma32(kj, qlo[j], s);
+        }
+    };
+
+    // Online softmax of a staged page and its products with V.  P in bf16 takes a hi + lo pair (16 bits); in f16 its 11 bits.
+    auto finish_page = [&](int n_tok, float tks, float tvs, f32x4 s)
+    {
+        float sc[4], vs[4];
+        float mt = kNegInf;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            float x = s[i] * kv_scale_log2;
+            vs[i] = 1.0f;
+            if constexpr (CT == I8)  // token 4g + i's scales sit in lane 4g + i
+            {
+                x = s[i] * __shfl(tks, 4 * g + i, 64) * kv_scale_log2;
+                vs[i] = __shfl(tvs, 4 * g + i, 64);
+            }
+            sc[i] = 4 * g + i < n_tok ? x : kNegInf;
+            mt = fmaxf(mt, sc[i]);
+        }
+        mt = xor_max(mt);
+        const float m_new = fmaxf(m_run, mt);
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+        float       pv[4], psum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            const float p = __builtin_amdgcn_exp2f(sc[i] - m_new);
+            psum += p;
+            pv[i] = 4 * g + i < n_tok ? p * vs[i] : 0.0f;
+        }
+        l_run = l_run * alpha + psum;
+        if (__any(m_new > m_run))
+        {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) acc[i] *= alpha;
+        }
+        m_run = m_new;
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            ph[i] = MV::bits(pv[i]);
+            pl[i] = P_LO ? MV::bits(pv[i] - MV::value(ph[i])) : 0u;
+        }
+        const auto phi = __builtin_bit_cast(typename MV::x4, u32x2{ph[0] | (ph[1] << 16), ph[2] | (ph[3] << 16)});
+        const auto plo = __builtin_bit_cast(typename MV::x4, u32x2{pl[0] | (pl[1] << 16), pl[2] | (pl[3] << 16)});
+        // the wave's LDS writes are complete before its reads (one queue); the fence keeps the compiler to that order
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+        {
+            const auto raw = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                (__attribute__((address_space(3))) bf16x4*)(sv + vt_pos<D>(4 * g + (c >> 2), 16 * i + 4 * (c & 3))));
+            const auto vt = __builtin_bit_cast(typename MV::x4, raw);
+            acc[i] = MV::mma16(vt, phi, acc[i]);
+            if constexpr (P_LO) acc[i] = MV::mma16(vt, plo, acc[i]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+
+    // entry i sits in r[i % DEPTH]; right after it is staged, entry i + DEPTH is loaded into the same registers
+    ListedPage<NW, NWV> r[DEPTH];
+#pragma unroll
+    for (int sl = 0; sl < DEPTH; ++sl)
+        if (sl < n) load_next(r[sl]);
+    auto step = [&]<int S>(int i)
+    {
+        ListedPage<NW, NWV>& cur = r[S];
+        const int   n_tok = cur.n_tok;
+        const float tks = cur.ks, tvs = cur.vs;
+        f32x4       s;
+        if (n_tok > 0) stage_page(cur, s);
+        if (i + DEPTH < n) load_next(cur);
+        if (n_tok > 0) finish_page(n_tok, tks, tvs, s);
+    };
+    for (int i = 0; i < n; i += DEPTH)
+    {
+        step.template operator()<0>(i);
+        if constexpr (DEPTH > 1)
+            if (i + 1 < n) step.template operator()<1 % DEPTH>(i + 1);
+    }
+
+    // the waves' states: accumulators [wave][head][D] over the V tiles, then (max, denominator) [wave][16]
+    float*      s_acc = reinterpret_cast<float*>(s_blocks);
+    float2*     s_ml = reinterpret_cast<float2*>(s_acc + kBlocksWaves * gc * D);
+    const float l_tot = xor_sum(l_run);
+    __syncthreads();
+    if (c < gc)
+    {
+        const float piece_scale = seen_scale<CT>(l_tot, v_head_scale);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+            *reinterpret_cast<f32x4*>(s_acc + (wave * gc + c) * D + 16 * i + 4 * g) = acc[i] * piece_scale;
+        if (g == 0) s_ml[wave * 16 + c] = float2{m_run, l_tot};
+    }
+    __syncthreads();
+    for (int k = static_cast<int>(threadIdx.x); k < gc * (D / 4); k += 64 * kBlocksWaves)
+    {
+        const int h = k / (D / 4);
+        const int d4 = (k - h * (D / 4)) * 4;
+        float     Mx = kLowest, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kBlocksWaves; ++w) Mx = fmaxf(Mx, s_ml[w * 16 + h].x);
+        f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kBlocksWaves; ++w)
+        {
+            const float2 t = s_ml[w * 16 + h];
+            const float  x = __builtin_amdgcn_exp2f(t.x - Mx);
+            L += t.y * x;
+            o += *reinterpret_cast<const f32x4*>(s_acc + (w * gc + h) * D + d4) * x;
+        }
+        store_state4<QT>(a, row * a.num_heads + kvh * G + h0 + h, split, D, d4, Mx, L, o);
+    }
+}
+
+// The pieces of every (row, head), folded.  A thread takes four output dims and every SG-th piece.
+template <int QT>
+__global__ __launch_bounds__(256) void blocks_merge(BlocksArgs a)
+{
+    __shared__ f32x4  s_o[256];
+    __shared__ float2 s_ml[256];
+    const int     D = a.head_dim, DL = D / 4;  // lanes of a piece
+    const int     SG = 256 / DL;
+    const int     tid = static_cast<int>(threadIdx.x);
+    const int     sg = tid / DL, d4 = (tid - sg * DL) * 4;
+    const int64_t row_h = blockIdx.x;
+    const float2* ml = a.ws_ml + row_h * a.splits;
+    const float*  xs = a.ws_acc + row_h * a.splits * D + d4;
+    float         m = kLowest, l = 0.0f;
+    f32x4         o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (sg < SG)
+    {
+        constexpr int MF = 4;  // pieces whose loads go out together
+        for (int i0 = sg; i0 < a.splits; i0 += SG * MF)
+        {
+            float2 t[MF];
+            f32x4  x[MF];
+            float  mn = m;
+#pragma unroll
+            for (int f = 0; f < MF; ++f)
+            {
+                const int i = i0 + f * SG;
+                t[f] = float2{kLowest, 0.0f};
+                x[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (i < a.splits)
+                {
+                    t[f] = ml[i];
+                    x[f] = *reinterpret_cast<const f32x4*>(xs + static_cast<int64_t>(i) * D);
+                }
+            }
+#pragma unroll
+            for (int f = 0; f < MF; ++f) mn = fmaxf(mn, t[f].x);
+            const float wa = __builtin_amdgcn_exp2f(m - mn);
+            l *= wa;
+            o *= wa;
+#pragma unroll
+            for (int f = 0; f < MF; ++f)
+            {
+                const float w = __builtin_amdgcn_exp2f(t[f].x - mn);
+                l += t[f].y * w;
+                o += x[f] * w;
+            }
+            m = mn;
+        }
+    }
+    s_o[tid] = o;
+    s_ml[tid] = float2{m, l};
+    __syncthreads();
+    if (sg != 0) return;
+    for (int j = 1; j < SG; ++j)
+    {
+        const float2 t = s_ml[j * DL + tid];
+        const float  mn = fmaxf(m, t.x);
+        const float  wa = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(t.x - mn);
+        l = l * wa + t.y * w;
+        o = o * wa + s_o[j * DL + tid] * w;
+        m = mn;
+    }
+    store_out4<QT>(a.out, static_cast<size_t>(row_h) * D + d4, o * softmax_inv(l));
+}
+
+// The vector kernel: a workgroup takes four query heads of a (row, KV head) and a piece of its list, a wave every fourth
+// page; LPT lanes hold a token, 8 dims each, with a softmax state per group of lanes.
+template <int CT, int QT, int LPT>
+__global__ __launch_bounds__(64 * kBlocksWaves) void paged_blocks_vector(BlocksArgs a)
+{
+    constexpr int HC = 4;
+    constexpr int TPW = 64 / LPT;           // tokens of a wave at a time
+    constexpr int NTOK = kBlockSize / TPW;  // of a page per group of lanes
+    constexpr int UN = 4;                   // tokens whose loads go out together
+    constexpr int ST = kBlocksWaves * TPW;  // states of the workgroup
+    __shared__ __align__(16) float s_acc[ST][HC][LPT * 8];
+    __shared__ float2 s_ml[ST][HC];
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int wave = uniform(static_cast<int>(threadIdx.x) >> 6);
+    const int c = lane % LPT;
+    const int g = lane / LPT;
+    const int D = a.head_dim;
+    const bool in = 8 * c < D;
+    const int G = a.group;
+    const int HB = (G + HC - 1) / HC;
+    const int y = a.num_kv_heads * HB;
+    int64_t   id = blockIdx.x;
+    const int split = static_cast<int>(id % a.splits);
+    id /= a.splits;
+    const int     vh = static_cast<int>(id % y);
+    const int64_t row = id / y;
+    const int     b = static_cast<int>(row / a.seq_len);
+    const int     t = static_cast<int>(row - static_cast<int64_t>(b) * a.seq_len);
+    const int     kvh = vh / HB;
+    const int     h0 = (vh - kvh * HB) * HC;
+    const int     gc = min(HC, G - h0);
+    const int64_t pos = static_cast<int64_t>(a.context_lens[b]) + t;
+    const int32_t* list = a.blocks + ((static_cast<int64_t>(b) * a.lists + t / a.query_block) * a.num_kv_heads + kvh) * a.count;
+    const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
+    const int begin = static_cast<int>(static_cast<int64_t>(a.count) * split / a.splits) + wave;
+    const int end = static_cast<int>(static_cast<int64_t>(a.count) * (split + 1) / a.splits);
+
+    float q[HC][8], acc[HC][8], m[HC], l[HC];
+#pragma unroll
+    for (int h = 0; h < HC; ++h)
+    {
+        m[h] = kLowest;
+        l[h] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[h][e] = acc[h][e] = 0.0f;
+        if (h < gc && in)
+            load_q8<QT>(a.q, (static_cast<size_t>(row) * a.num_heads + kvh * G + h0 + h) * D + 8 * c, q[h]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[h][e] *= a.scale_log2;
+    }
+    float k_head = 1.0f, v_head = 1.0f;
+    if constexpr (CT == FP8)
+    {
+        k_head = a.k_scale[kvh];
+        v_head = a.v_scale[kvh];
+    }
+    for (int i0 = begin; i0 < end; i0 += 64 * kBlocksWaves)
+    {
+        const int lvec = listed_page(a, list, i0 + kBlocksWaves * lane, end, pos);
+        const int pvec = lvec >= 0 ? table[lvec] : -1;
+        for (int i = 0; i < 64 && i0 + kBlocksWaves * i < end; ++i)
+        {
+            const int lp = __builtin_amdgcn_readlane(lvec, i);
+            const int phys = __builtin_amdgcn_readlane(pvec, i);
+            if (phys < 0 || phys >= a.num_blocks) continue;
+            const int n_tok = static_cast<int>(min(pos + 1 - static_cast<int64_t>(lp) * kBlockSize, static_cast<int64_t>(kBlockSize)));
+#pragma unroll 1
+            for (int u0 = 0; u0 < NTOK; u0 += UN)
+            {
+                Raw8  kr[UN], vr[UN];
+                float ks[UN], vs[UN];
+#pragma unroll
+                for (int u = 0; u < UN; ++u)
+                {
+                    const int    tok = (u0 + u) * TPW + g;
+                    const size_t row_c = (static_cast<size_t>(phys) * kBlockSize + tok) * a.num_kv_heads + kvh;
+                    ks[u] = k_head;
+                    vs[u] = v_head;
+                    if constexpr (CT == I8)
+                    {
+                        ks[u] = a.k_scale[row_c];
+                        vs[u] = a.v_scale[row_c];
+                    }
+                    if (in)
+                    {
+                        load_raw8<CT>(a.k_cache, row_c * D + 8 * c, kr[u]);
+                        load_raw8<CT>(a.v_cache, row_c * D + 8 * c, vr[u]);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < UN; ++u)
+                {
+                    const bool seen = (u0 + u) * TPW + g < n_tok;
+                    float      k[8], v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.0f;
+                    if (in && seen)
+                    {
+                        unpack8<CT>(kr[u], k);
+                        unpack8<CT>(vr[u], v);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (CT == I8 || CT == FP8) v[e] = seen ? v[e] * vs[u] : 0.0f;
+#pragma unroll
+                    for (int h = 0; h < HC; ++h)
+                    {
+                        float s = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) s = __builtin_fmaf(q[h][e], k[e], s);
+                        s = group_sum<LPT>(s);
+                        if (CT == I8 || CT == FP8) s *= ks[u];
+                        s = seen ? s : kNegInf;
+                        const float mn = fmaxf(m[h], s);
+                        const float wa = __builtin_amdgcn_exp2f(m[h] - mn);
+                        const float p = __builtin_amdgcn_exp2f(s - mn);
+                        l[h] = l[h] * wa + p;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) acc[h][e] = __builtin_fmaf(p, v[e], acc[h][e] * wa);
+                        m[h] = mn;
+                    }
+                }
+            }
+        }
+    }
+    const int st = wave * TPW + g;
+#pragma unroll
+    for (int h = 0; h < HC; ++h)
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s_acc[st][h][8 * c + e] = acc[h][e];
+        if (c == 0) s_ml[st][h] = float2{m[h], l[h]};
+    }
+    __syncthreads();
+    for (int k = static_cast<int>(threadIdx.x); k < gc * (D / 4); k += 64 * kBlocksWaves)
+    {
+        const int h = k / (D / 4);
+        const int d4 = (k - h * (D / 4)) * 4;
+        float     Mx = kLowest, L = 0.0f;
+        for (int w = 0; w < ST; ++w) Mx = fmaxf(Mx, s_ml[w][h].x);
+        f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < ST; ++w)
+        {
+            const float x = __builtin_amdgcn_exp2f(s_ml[w][h].x - Mx);
+            L += s_ml[w][h].y * x;
+            o += *reinterpret_cast<const f32x4*>(&s_acc[w][h][d4]) * x;
+        }
+        store_state4<QT>(a, row * a.num_heads + kvh * G + h0 + h, split, D, d4, Mx, L, o);
+    }
+}
+
+namespace
+{
+
+bool mfma_dim(int d) { return d == 64 || d == 96 || d == 128 || d == 256; }
+
+// Workgroups of an unsplit call.
+int64_t blocks_workgroups(const BlocksArgs& a)
+{
+    const int heads = blocks_kernel(a) == BlocksKernel::kDecode ? 16 : 4;
+    return static_cast<int64_t>(a.batch) * a.seq_len * a.num_kv_heads * ((a.group + heads - 1) / heads);
+}
+
+template <int QT, typename F>
+hipError_t for_cache(const BlocksArgs& a, F f)
+{
+    switch (a.cache_dtype)
+    {
+        case F32:
+            return f.template operator()<QT, F32>();
+        case F16:
+            return f.template operator()<QT, F16>();
+        case BF16:
+            return f.template operator()<QT, BF16>();
+        case I8:
+            return f.template operator()<QT, I8>();
+        default:
+            return f.template operator()<QT, FP8>();
+    }
+}
+
+template <typename F>
+hipError_t for_types(const BlocksArgs& a, F f)
+{
+    if (a.qo_dtype == F32) return for_cache<F32>(a, f);
+    if (a.qo_dtype == F16) return for_cache<F16>(a, f);
+    return for_cache<BF16>(a, f);
+}
+
+}  // namespace
+
+BlocksKernel blocks_kernel(const BlocksArgs& a)
+{
+    if (a.cache_dtype == F32 || !mfma_dim(a.head_dim)) return BlocksKernel::kVector;
+    if (a.query_block == 1) return BlocksKernel::kDecode;
+    return a.head_dim == 96 ? BlocksKernel::kVector : BlocksKernel::kPrefill;
+}
+
+int blocks_splits(const BlocksArgs& a)
+{
+    if (blocks_kernel(a) == BlocksKernel::kPrefill) return 1;
+    const int64_t wgs = blocks_workgroups(a);
+    const int64_t most = a.count / (2 * kBlocksWaves);  // pieces of two pages per wave
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(wgs, 1), most)));
+}
+
+hipError_t launch_blocks_prefill(const BlocksArgs& a, hipStream_t stream)
+{
+    ListPrefillArgs p{};
+    p.q = a.q;
+    p.out = a.out;
+    p.k_cache = a.k_cache;
+    p.v_cache = a.v_cache;
+    p.k_scale = a.k_scale;
+    p.v_scale = a.v_scale;
+    p.block_table = a.block_table;
+    p.context_lens = a.context_lens;
+    p.qo_dtype = a.qo_dtype;
+    p.cache_dtype = a.cache_dtype;
+    p.batch = a.batch;
+    p.seq_len = a.seq_len;
+    p.num_heads = a.num_heads;
+    p.num_kv_heads = a.num_kv_heads;
+    p.group = a.group;
+    p.head_dim = a.head_dim;
+    p.max_blocks = a.max_blocks;
+    p.num_blocks = a.num_blocks;
+    p.cap_tokens = decode_cap_tokens(a.max_blocks, 0);
+    p.paged = true;
+    p.scale_log2 = a.scale_log2;
+    p.n_split = 1;
+    p.span_tokens = p.cap_tokens;
+    p.blocks = a.blocks;
+    p.lists = a.lists;
+    p.count = a.count;
+    p.query_block = a.query_block;
+    if (a.cache_dtype == BF16) return launch_blocks_prefill_bf16(p, stream);
+    if (a.cache_dtype == F16) return launch_blocks_prefill_f16(p, stream);
+    if (a.cache_dtype == I8) return launch_blocks_prefill_i8(p, stream);
+    return launch_blocks_prefill_fp8(p, stream);
+}
+
+hipError_t launch_blocks(const BlocksArgs& a, hipStream_t stream)
+{
+    const BlocksKernel kernel = blocks_kernel(a);
+    if (kernel == BlocksKernel::kPrefill) return launch_blocks_prefill(a, stream);
+    const int64_t wgs = blocks_workgroups(a) * a.splits;
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.seq_len * a.num_heads;
+    if (wgs > INT32_MAX || rows > INT32_MAX) return hipErrorInvalidConfiguration;
+    const dim3 grid(static_cast<unsigned>(wgs)), block(64 * kBlocksWaves);
+    hipError_t e;
+    if (kernel == BlocksKernel::kDecode)
+        e = for_types(a, [&]<int QT, int CT>()
+        {
+            auto go = [&]<int D>()
+            {
+                if constexpr (CT != F32)
+                    hipLaunchKernelGGL((paged_blocks_decode<CT, QT, D>), grid, block,
+                                       static_cast<unsigned>(blocks_lds_bytes<D>(std::min(a.group, 16))), stream, a);
+                return hipGetLastError();
+            };
+            if (a.head_dim == 64) return go.template operator()<64>();
+            if (a.head_dim == 96) return go.template operator()<96>();
+            if (a.head_dim == 128) return go.template operator()<128>();
+            return go.template operator()<256>();
+        });
+    else
+        e = for_types(a, [&]<int QT, int CT>()
+        {
+            if (a.head_dim <= 128)
+                hipLaunchKernelGGL((paged_blocks_vector<CT, QT, 16>), grid, block, 0, stream, a);
+            else
+                hipLaunchKernelGGL((paged_blocks_vector<CT, QT, 32>), grid, block, 0, stream, a);
+            return hipGetLastError();
+        });
+    if (e != hipSuccess || a.splits == 1) return e;
+    const dim3 merge(static_cast<unsigned>(rows));
+    if (a.qo_dtype == F32)
+        hipLaunchKernelGGL((blocks_merge<F32>), merge, dim3(256), 0, stream, a);
+    else if (a.qo_dtype == F16)
+        hipLaunchKernelGGL((blocks_merge<F16>), merge, dim3(256), 0, stream, a);
+    else
+        hipLaunchKernelGGL((blocks_merge<BF16>), merge, dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace ffkv

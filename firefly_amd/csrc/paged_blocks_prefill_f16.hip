@@ -1,0 +1,9 @@
+// paged_blocks_prefill_f16.hip - the prefill over listed pages (blocks_prefill.h) of f16 caches.
+#include "blocks_prefill.h"
+
+namespace ffkv
+{
+
+hipError_t launch_blocks_prefill_f16(const ListPrefillArgs& a, hipStream_t stream) { return launch_blocks_prefill_t<F16>(a, stream); }
+
+}  // namespace ffkv

@@ -360,10 +360,13 @@ struct PrefillLds
 // registers, which calls that are not split paid for too (int8 at head_dim 64, 15 x 490 tokens over 1500: 216.8 -> 218.7 us).
 // RULE: scores are changed and keys hidden by a.rule, each query sees keys [kbeg, kend), and what a query does not see
 // never reaches it, infinite and NaN values included (s_vover is then the first of kRuleFlags ints in LDS).
-template <int QT, int D, int CT, bool PFX, int RG, bool SPLIT = false, bool RULE = false>
-__device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_index, uint8_t* s_st0, uint8_t* s_st1,
-                                           uint8_t* s_st2, uint8_t* s_st3, int& s_vover)
+// LIST: every block of a.query_block tokens of a row has a list of pages per KV head and attends those alone (a rule without
+// a cap, a bias or ranges: its pages are masked and its strange values kept apart as a rule's are).
+template <int QT, int D, int CT, bool PFX, int RG, bool SPLIT = false, bool RULE = false, bool LIST = false>
+__device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillArgs, PrefillKernelArgs<RULE>> a, int wg_index,
+                                           uint8_t* s_st0, uint8_t* s_st1, uint8_t* s_st2, uint8_t* s_st3, int& s_vover)
 {
+    static_assert(!LIST || (RULE && !SPLIT && !PFX), "lists are masked as a rule's ranges are, and not split");
     constexpr int  W = 8 / RG;  // waves per workgroup
     constexpr int  EB = kElemBytes<CT>;
     constexpr bool Q8 = EB == 1;
@@ -427,12 +430,15 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
     const int S = a.seq_len;
     const int Hq = a.num_heads;
     const int Hkv = a.num_kv_heads;
-    const int R = PFX ? a.batch * G : S * G;  // query rows of a group: (token, head) or (row, head) pairs
+    int       tokens = S;  // of a group (LIST: at most)
+    if constexpr (LIST) tokens = a.query_block;
+    int R = PFX ? a.batch * G : tokens * G;  // query rows of a group: (token, head) or (row, head) pairs
     const int nrb = (R + kDmaRows - 1) / kDmaRows;
     // a prefill split over its keys deals piece p of every group after piece p - 1 of all of them, so that the pieces
     // of one group spread over the XCDs where the groups are fewer
     static_assert(!(PFX && (SPLIT || RULE)), "prefix partials have chunks of their own, and no rule");
-    const int groups0 = PFX ? Hkv * a.pfx_chunks : a.batch * Hkv;
+    int groups0 = PFX ? Hkv * a.pfx_chunks : a.batch * Hkv;
+    if constexpr (LIST) groups0 *= a.lists;
     const int nsp = SPLIT ? a.n_split : 1;
     const int groups = groups0 * nsp;
 #if FFKV_PREFILL_XCD
@@ -478,7 +484,7 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
     }
     // (one row has one length: its groups keep their order)
     const int g8 = (groups + kXcds - 1) / kXcds;  // group slots of this XCD: groups j * kXcds + xcd, j < g8
-    if (!PFX && !SPLIT && a.paged && a.batch > 1 && g8 <= 64 && g8 > 1)
+    if (!PFX && !SPLIT && !LIST && a.paged && a.batch > 1 && g8 <= 64 && g8 > 1)
     {
         // The XCD's groups by decreasing cached length (ties by index): lane j ranks group j * kXcds + xcd, and
         // the workgroup takes the group ranked k_in_xcd / nrb.  Absent groups (past `groups`) rank last.
@@ -501,7 +507,17 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
 #endif
     const int piece = nsp == 1 ? 0 : grp / groups0;
     const int grp0 = grp - piece * groups0;
-    const int b = PFX ? 0 : grp0 / Hkv;                 // prefill: the workgroup's row
+    int       b = PFX ? 0 : grp0 / Hkv;                 // prefill: the workgroup's row
+    int       t0 = 0;                                   // LIST: the block's first token
+    const int32_t* list = nullptr;
+    if constexpr (LIST)
+    {
+        const int rl = b;  // (row, block of tokens)
+        b = rl / a.lists;
+        t0 = (rl - b * a.lists) * a.query_block;
+        R = min(a.query_block, S - t0) * G;
+        list = a.blocks + static_cast<int64_t>(grp0) * a.count;
+    }
     const int kvh = PFX ? grp / a.pfx_chunks : grp0 % Hkv;
     const int chunk = PFX ? grp % a.pfx_chunks : 0;  // prefix: pages chunk*pfx_chunk_pages ..
     const int row0 = rb * kDmaRows;
@@ -561,7 +577,7 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
         else
         {
             bq[gi] = 0;
-            const int t = col_ok[gi] ? r / G : 0;
+            const int t = t0 + (col_ok[gi] ? r / G : 0);
             int64_t   ke = ctx + t + 1;
             ke = ke > L ? L : (ke < 0 ? 0 : ke);
             kend[gi] = col_ok[gi] ? static_cast<int>(ke) : 0;
@@ -583,7 +599,19 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
         kw = kw > L ? L : (kw < 0 ? 0 : kw);
         pg_lo = 0;
         pg_hi = static_cast<int>((kw + kBlockSize - 1) / kBlockSize);
-        if constexpr (RULE)
+        if constexpr (LIST)
+        {
+            // entries up to the last that is a page of the row (every wave on its own)
+            pg_hi = 0;
+            for (int e0 = (a.count - 1) & ~63; e0 >= 0 && pg_hi == 0; e0 -= 64)
+            {
+                const int      e = e0 + lane;
+                const int      lp = e < a.count ? list[e] : -1;
+                const uint64_t hit = __ballot(lp >= 0 && lp < a.max_blocks && static_cast<int64_t>(lp) * kBlockSize < L);
+                if (hit != 0) pg_hi = e0 + 64 - __builtin_clzll(hit);
+            }
+        }
+        else if constexpr (RULE)
         {
             // the pages that some query of the workgroup sees (every wave on its own: a lane takes up to two tokens)
             int lo = INT32_MAX, hi = 0;
@@ -813,23 +841,51 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
     const uint32_t page_bytes = static_cast<uint32_t>(kBlockSize * row_bytes);
     const uint64_t row_base = a.paged ? 0 : static_cast<uint64_t>(b) * S * row_bytes;
 
+    // LIST: the pages of a step are listed ones, logical page lp[u] each (0 where it is absent).
+    struct ListStep
+    {
+        int okm;
+        int lp[KP];
+    };
+    using Step = std::conditional_t<LIST, ListStep, int>;
+    auto mask_of = [](const Step& st) -> int
+    {
+        if constexpr (LIST) return st.okm;
+        else return st;
+    };
+    auto page_of = [&](const Step& st, int si, int u) -> int
+    {
+        if constexpr (LIST) return st.lp[u];
+        else return pg_lo + si * KP + u;
+    };
+    const FFKV_CONST int32_t* list_row = (const FFKV_CONST int32_t*)list;
+
     // Requests step si into `stage`; returns its page mask (bit u: page pg_lo + si*KP + u is present; keys on absent
     // pages are masked).  Block-table entries are uniform and come through the scalar cache.  Pages whose 16
     // rows are all keys of the row load with a uniform base; the row's last, partial page (and absent pages)
     // fetch the zero block for the missing rows.  The scalar work is kept short: it runs once per step in every
     // wave, in order with the wave's matrix and vector work.
-    auto issue = [&](int si, uint8_t* stage) -> int
+    auto issue = [&](int si, uint8_t* stage) -> Step
     {
         int      okm = 0, full = 0;
         uint64_t page_off[KP];
         uint32_t page_row[KP];  // physical page of present pages (int8 scales are indexed by it), else 0
+        int      lpage[KP];     // LIST: logical page
 #pragma unroll
         for (int u = 0; u < KP; ++u)
         {
-            const int pg = pg_lo + si * KP + u;
+            int       pg = pg_lo + si * KP + u;
             uint32_t  idx = 0;
             bool      present = false;
-            if (pg < pg_hi)  // pg_hi <= max_blocks
+            if constexpr (LIST)
+            {
+                int lp = pg < pg_hi ? list_row[pg] : -1;
+                lp = lp >= 0 && lp < a.max_blocks && static_cast<int64_t>(lp) * kBlockSize < L ? lp : -1;
+                idx = lp >= 0 ? static_cast<uint32_t>(table_row[lp]) : ~0u;
+                present = idx < static_cast<uint32_t>(a.num_blocks);
+                pg = lpage[u] = present ? lp : 0;
+            }
+            else if (pg < pg_hi)  // pg_hi <= max_blocks
             {
                 if (a.paged)
                 {
@@ -860,7 +916,14 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
                 const char* base = run_src[j * RPP] + row_base + static_cast<uint64_t>(idx) * page_bytes;
                 const bool  fl = (full >> u) & 1;
                 const bool  pres = (okm >> u) & 1;
-                const int   tok0 = (pg_lo + si * KP + u) * kBlockSize;
+                int         tok0 = (pg_lo + si * KP + u) * kBlockSize;
+                if constexpr (LIST)
+                {
+                    int lp = lpage[0];
+#pragma unroll
+                    for (int uu = 1; uu < KP; ++uu) lp = u == uu ? lpage[uu] : lp;
+                    tok0 = lp * kBlockSize;
+                }
                 if (fl)
                 {
 #pragma unroll
@@ -919,14 +982,30 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
                 uint32_t   pr = page_row[0];
 #pragma unroll
                 for (int uu = 1; uu < KP; ++uu) pr = u == uu ? page_row[uu] : pr;
-                const bool take = ((okm >> u) & 1) && (pg_lo + si * KP + u) * kBlockSize + t < L;
+                int        pgu = pg_lo + si * KP + u;
+                if constexpr (LIST)
+                {
+                    pgu = lpage[0];
+#pragma unroll
+                    for (int uu = 1; uu < KP; ++uu) pgu = u == uu ? lpage[uu] : pgu;
+                }
+                const bool take = ((okm >> u) & 1) && pgu * kBlockSize + t < L;
                 const float* src = (is_v ? a.v_scale : a.k_scale) +
                                    (static_cast<size_t>(pr) * kBlockSize + t) * Hkv + kvh;
                 load_lds4(take ? static_cast<const void*>(src) : static_cast<const void*>(zero_src),
                           (const FFKV_LDS void*)(stage + 2 * C::TILEB + 256 * sr));
             }
         }
-        return okm;
+        if constexpr (LIST)
+        {
+            ListStep st;
+            st.okm = okm;
+#pragma unroll
+            for (int u = 0; u < KP; ++u) st.lp[u] = lpage[u];
+            return st;
+        }
+        else
+            return okm;
     };
 
     // ---- compute ---------------------------------------------------------------------------------------------
@@ -1056,14 +1135,22 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
     };
 
     // Online softmax of a step's scores: the probabilities pv (int8: times the keys' V scales).
-    auto softmax = [&]<bool VC, bool SH>(int si, const uint8_t* stage, int okm, f32x4 (&s)[RG][KP],
+    auto softmax = [&]<bool VC, bool SH>(int si, const uint8_t* stage, const Step& pages, f32x4 (&s)[RG][KP],
                                          float (&pv)[RG][KP * 4])
     {
         constexpr bool LD = L_DOT || VC;  // the f16 P of converted bf16 V tiles sums by dot products too
+        const int okm = mask_of(pages);
         const int pg0 = pg_lo + si * KP;
         // uniform: every key of the step is visible to every column of the wave
-        const bool unmasked = okm == (1 << KP) - 1 && (pg0 + KP) * kBlockSize <= kmin && (!RULE || pg0 * kBlockSize >= kbmax);
-        if constexpr (RULE)
+        bool unmasked = okm == (1 << KP) - 1 && (pg0 + KP) * kBlockSize <= kmin && (!RULE || pg0 * kBlockSize >= kbmax);
+        if constexpr (LIST)
+        {
+            int most = 0;
+#pragma unroll
+            for (int u = 0; u < KP; ++u) most = max(most, page_of(pages, si, u));
+            unmasked = okm == (1 << KP) - 1 && (most + 1) * kBlockSize <= kmin;
+        }
+        if constexpr (RULE && !LIST)
             if (convert)
             {
 #pragma unroll
@@ -1111,7 +1198,8 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                     {
-                        const bool vis = ((okm >> u) & 1) && u * kBlockSize + i < kr && (!RULE || u * kBlockSize + i >= kl);
+                        bool vis = ((okm >> u) & 1) && u * kBlockSize + i < kr && (!RULE || u * kBlockSize + i >= kl);
+                        if constexpr (LIST) vis = ((okm >> u) & 1) && page_of(pages, si, u) * kBlockSize + 4 * g + i < kend[gi];
                         s[gi][u][i] = vis ? s[gi][u][i] : kNegInf;
                     }
             }
@@ -1344,13 +1432,15 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
             }
         if (__any(bad) && lane == 0) *(volatile FFKV_LDS int*)(s_bad + si % kDmaStages<D>) = si + 1;
     };
-    auto add_bad = [&](int si, int okm)
+    auto add_bad = [&](int si, const Step& pages)
     {
+        const int okm = mask_of(pages);
         for (int t = 0; t < KP * kBlockSize; ++t)
         {
             if (!((okm >> (t / kBlockSize)) & 1)) continue;
-            const int      pg = pg_lo + si * KP + t / kBlockSize;
+            const int      pg = page_of(pages, si, t / kBlockSize);
             const int      key = pg * kBlockSize + t % kBlockSize;
+            if (LIST && key >= L) continue;
             if (key >= L) break;
             const uint64_t page = a.paged ? static_cast<uint32_t>(table_row[pg]) : static_cast<uint32_t>(pg);
             const char*    v = static_cast<const char*>(a.v_cache) + row_base + page * page_bytes +
@@ -1381,7 +1471,7 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
     // execute.
     // With three or more stages, step si + 1 has been requested a step before step si is computed, so its tiles
     // are converted while step si's score products run (AH), instead of at the head of step si + 1.
-    auto body = [&]<bool VC, bool SH, bool CF>(int si, uint8_t* cur, int okm_cur, uint8_t* nxt, int& okm_nxt, uint8_t* ahead)
+    auto body = [&]<bool VC, bool SH, bool CF>(int si, uint8_t* cur, Step okm_cur, uint8_t* nxt, Step& okm_nxt, uint8_t* ahead)
     {
         constexpr bool AH = FFKV_PREFILL_AHEAD && NS >= 3 && (VC || C16);
         wait_vm<(NS - 2) * LPS>();
@@ -1441,8 +1531,8 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[gi][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        int okm0 = issue(0, s_st0);
-        int okm1 = 0, okm2 = 0, okm3 = 0;
+        Step okm0 = issue(0, s_st0);
+        Step okm1{}, okm2{}, okm3{};
         if constexpr (NS >= 3) okm1 = issue(1, s_st1);
         if constexpr (NS == 4) okm2 = issue(2, s_st2);
         if constexpr (FFKV_PREFILL_AHEAD && NS >= 3 && (VC || C16))  // step 0's tiles, converted ahead of the loop
@@ -1517,9 +1607,15 @@ __device__ __forceinline__ void prefill_wg(PrefillKernelArgs<RULE> a, int wg_ind
             if (again)
             {
                 bool big = false;
-                for (int t = pg_lo * kBlockSize + lane; t < min(pg_hi * kBlockSize, L); t += 64)
+                for (int t = pg_lo * kBlockSize + lane; t < (LIST ? pg_hi * kBlockSize : min(pg_hi * kBlockSize, L)); t += 64)
                 {
-                    const uint32_t pg = static_cast<uint32_t>(table_row[t / kBlockSize]);
+                    int lp = t / kBlockSize;
+                    if constexpr (LIST)
+                    {
+                        lp = list[lp];
+                        if (lp < 0 || lp >= a.max_blocks || static_cast<int64_t>(lp) * kBlockSize + t % kBlockSize >= L) continue;
+                    }
+                    const uint32_t pg = static_cast<uint32_t>(table_row[lp]);
                     if (pg >= static_cast<uint32_t>(a.num_blocks)) continue;
                     const float vs = __builtin_fabsf(a.v_scale[(static_cast<size_t>(pg) * kBlockSize + t % kBlockSize) * Hkv + kvh]);
                     big = big || (vs >= 255.0f && vs < __builtin_huge_valf());

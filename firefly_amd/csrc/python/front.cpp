@@ -41,10 +41,17 @@ struct Functions
     decltype(&ffkv_decode_scored_scratch_bytes)       decode_scored_bytes;
     decltype(&ffkv_attention_weights_workspace_bytes) weights_bytes;
     decltype(&ffkv_evict_workspace_bytes)             evict_bytes;
+    decltype(&ffkv_rope_axes)                  rope_axes;
+    decltype(&ffkv_rope_append_axes)           rope_append_axes;
+    decltype(&ffkv_key_bounds)                 key_bounds;
+    decltype(&ffkv_select_blocks)              select_blocks;
+    decltype(&ffkv_select_blocks_workspace_bytes) select_bytes;
+    decltype(&ffkv_paged_attention_blocks)     attention_blocks;
+    decltype(&ffkv_paged_attention_blocks_workspace_bytes) attention_blocks_bytes;
 };
 Functions fn{};
 
-PyObject *s_shape, *s_dtype, *s_data_ptr, *s_nbytes, *s_cuda_stream, *s_device, *s_index, *s_is_contiguous, *s_is_cuda;
+PyObject *s_shape, *s_dtype, *s_data_ptr, *s_nbytes, *s_cuda_stream, *s_device, *s_index, *s_is_contiguous, *s_is_cuda, *s_stride;
 constexpr int kInt32 = 4;  // int32 among bind()'s dtypes: tables and lengths, no dtype of activations or caches
 struct DtypeCode
 {
@@ -201,7 +208,12 @@ struct Reader
         const bool yes = c == Py_True;
         Py_DECREF(c);
         if (!yes) return refuse(PyExc_ValueError, "%s must be contiguous", name);
-        if (t == like) return true;
+        return beside(t, name, like);
+    }
+    // t is on the device of `like`.
+    bool beside(PyObject* t, const char* name, PyObject* like)
+    {
+        if (!ok || t == Py_None || t == like) return ok;
         PyObject* a = PyObject_GetAttr(t, s_device);
         PyObject* b = a ? PyObject_GetAttr(like, s_device) : nullptr;
         const int eq = b ? PyObject_RichCompareBool(a, b, Py_EQ) : -1;
@@ -209,6 +221,39 @@ struct Reader
         Py_XDECREF(b);
         if (eq < 0) return ok = false;
         return eq == 1 || refuse(PyExc_ValueError, "%s is on another device than the other tensors", name);
+    }
+    // t, of type `code`, holds heads [B, S, H, D] token by token: heads and dims are contiguous, the tokens of all rows evenly
+    // spaced.  Elements from token to token.
+    long long tokens(PyObject* t, const char* name, int code, int B, int S, int H, int D, PyObject* like)
+    {
+        if (!ok) return 0;
+        if (dtype(t) != code && ok) refuse(PyExc_TypeError, "%s has another dtype than k", name);
+        PyObject* s = shape(t, 4, true);
+        const long long want[4] = {B, S, H, D};
+        for (int i = 0; ok && i < 4; ++i)
+            if (PyLong_AsLongLong(PyTuple_GET_ITEM(s, i)) != want[i]) refuse(PyExc_ValueError, "%s has the wrong shape %S", name, s);
+        Py_XDECREF(s);
+        if (!ok || !beside(t, name, like)) return 0;
+        PyObject* st = PyObject_CallMethodNoArgs(t, s_stride);
+        if (st == nullptr || !PyTuple_Check(st) || PyTuple_GET_SIZE(st) != 4)
+        {
+            Py_XDECREF(st);
+            ok = false;
+            return 0;
+        }
+        long long v[4];
+        for (int i = 0; i < 4; ++i) v[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(st, i));
+        Py_DECREF(st);
+        const long long row = static_cast<long long>(H) * D;
+        if (B == 0 || S == 0) return row;
+        // (a dimension of one has any stride)
+        const long long step = S > 1 ? v[1] : (B > 1 ? v[0] : row);
+        if ((D > 1 && v[3] != 1) || (H > 1 && v[2] != D) || (B > 1 && v[0] != S * step) || step < row)
+        {
+            refuse(PyExc_ValueError, "%s must hold its heads contiguously and its tokens evenly spaced", name);
+            return 0;
+        }
+        return step;
     }
     // t lies on the current device (a call without rows touches no device and may have its tensors anywhere).
     void current(PyObject* t, bool rows)
@@ -729,6 +774,200 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n)
     });
 }
 
+// positions at p, sections at p + 1, interleaved at p + 2, theta at p + 3 of a rotation on several axes: int32 [axes, B, S], a
+// sequence of ints, a truth value, a number.
+struct Axes
+{
+    int      axes = 0, interleaved = 0;
+    int      sections[4] = {0, 0, 0, 0};
+    int32_t* positions = nullptr;
+    float    theta = 0.0f;
+    Axes(Reader& r, PyObject* const* p, int B, int S, PyObject* like)
+    {
+        if (!r.ok) return;
+        PyObject* seq = PySequence_Fast(p[1], "sections must be a sequence of ints");
+        if (seq == nullptr)
+        {
+            r.ok = false;
+            return;
+        }
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+        if (n < 1 || n > 4) r.refuse(PyExc_ValueError, "1 to 4 sections are required, not %zd", n);
+        for (Py_ssize_t i = 0; r.ok && i < n; ++i) sections[i] = r.integer(PySequence_Fast_GET_ITEM(seq, i));
+        Py_DECREF(seq);
+        axes = static_cast<int>(n);
+        r.holds(p[0], "positions", kInt32, {n, B, S}, like, false);
+        positions = r.ptr<int32_t>(p[0]);
+        if (r.ok && (interleaved = PyObject_IsTrue(p[2])) < 0) r.ok = false;
+        theta = r.real(p[3]);
+    }
+};
+
+// q or None, k, positions, sections, interleaved, theta, q_out, k_out, stream
+PyObject* rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!count(n, 9)) return nullptr;
+    Reader r{a};
+    int    B, S, Hkv, D;
+    r.dims4(a[1], B, S, Hkv, D);
+    const int  st = r.dtype(a[1]), Hq = a[0] == Py_None ? 0 : r.dim(a[0], -2);
+    const auto ks = r.tokens(a[1], "k", st, B, S, Hkv, D, a[1]);
+    const auto kos = r.tokens(a[7], "k_out", st, B, S, Hkv, D, a[1]);
+    long long  qs = 0, qos = 0;
+    if (r.ok && a[0] != Py_None)
+    {
+        qs = r.tokens(a[0], "q", st, B, S, Hq, D, a[1]);
+        qos = r.tokens(a[6], "q_out", st, B, S, Hq, D, a[1]);
+    }
+    const Axes x(r, a + 2, B, S, a[1]);
+    r.current(a[1], B > 0 && S > 0);
+    void *q = r.ptr(a[0]), *k = r.ptr(a[1]), *qo = a[0] == Py_None ? nullptr : r.ptr(a[6]), *ko = r.ptr(a[7]);
+    void* s = r.stream(a[8]);
+    return finish(r, [&] {
+        return fn.rope_axes(q, qs, qo, qos, k, ks, ko, kos, st, x.positions, x.sections, x.axes, x.interleaved, B, S, Hq, Hkv, D,
+                            x.theta, s);
+    });
+}
+
+// q or None, k, v, positions, sections, interleaved, theta, k_cache, v_cache, block_table, context_lens, q_out, k_scale,
+// v_scale, num_blocks, stream
+PyObject* rope_append_axes(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!count(n, 16)) return nullptr;
+    Reader r{a};
+    int    B, S, Hkv, D;
+    r.dims4(a[1], B, S, Hkv, D);
+    const int  st = r.dtype(a[1]), ct = r.dtype(a[7]), Hq = a[0] == Py_None ? 0 : r.dim(a[0], -2);
+    const auto ks = r.tokens(a[1], "k", st, B, S, Hkv, D, a[1]);
+    const auto vs = r.tokens(a[2], "v", st, B, S, Hkv, D, a[1]);
+    long long  qs = 0, qos = 0;
+    if (r.ok && a[0] != Py_None)
+    {
+        qs = r.tokens(a[0], "q", st, B, S, Hq, D, a[1]);
+        qos = r.tokens(a[11], "q_out", st, B, S, Hq, D, a[1]);
+    }
+    const Axes x(r, a + 3, B, S, a[1]);
+    r.holds(a[7], "k_cache", ct, {-1, FFKV_BLOCK_SIZE, Hkv, D}, a[1], false);
+    r.holds(a[8], "v_cache", ct, {r.dim(a[7], 0), FFKV_BLOCK_SIZE, Hkv, D}, a[1], false);
+    r.holds(a[9], "block_table", kInt32, {B, -1}, a[1], false);
+    r.holds(a[10], "context_lens", kInt32, {B}, a[1], true);
+    check_scales(r, a[12], "k_scale", ct, a[7], Hkv, a[1]);
+    check_scales(r, a[13], "v_scale", ct, a[7], Hkv, a[1]);
+    const int mb = r.dim(a[9], 1), N = r.blocks(a[14], a[7]);
+    check_blocks(r, N, a[7]);
+    r.current(a[1], B > 0 && S > 0);
+    void *q = r.ptr(a[0]), *qo = a[0] == Py_None ? nullptr : r.ptr(a[11]), *k = r.ptr(a[1]), *v = r.ptr(a[2]);
+    void *kc = r.ptr(a[7]), *vc = r.ptr(a[8]);
+    auto *bt = r.ptr<int32_t>(a[9]), *cx = r.ptr<int32_t>(a[10]);
+    auto *ksc = r.ptr<float>(a[12]), *vsc = r.ptr<float>(a[13]);
+    void* s = r.stream(a[15]);
+    return finish(r, [&] {
+        return fn.rope_append_axes(q, qs, qo, qos, k, ks, v, vs, st, kc, vc, ct, ksc, vsc, bt, cx, x.positions, x.sections,
+                                   x.axes, x.interleaved, B, S, Hq, Hkv, D, FFKV_BLOCK_SIZE, mb, N, x.theta, s);
+    });
+}
+
+// The type of a cache's key bounds.
+int bounds_code(int ct) { return ct == FFKV_DTYPE_I8 || ct == FFKV_DTYPE_FP8_E4M3 ? FFKV_DTYPE_BF16 : ct; }
+
+// k_cache, bounds, block_table, context_lens, new_tokens, k_scale, num_blocks, stream
+PyObject* key_bounds(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!count(n, 8)) return nullptr;
+    Reader    r{a};
+    PyObject* kc = a[0];
+    const int ct = r.dtype(kc), Hkv = r.dim(kc, 2), D = r.dim(kc, 3), B = r.dim(a[3], 0);
+    r.holds(kc, "k_cache", ct, {-1, FFKV_BLOCK_SIZE, Hkv, D}, kc, false);
+    r.holds(a[1], "bounds", bounds_code(ct), {r.dim(kc, 0), Hkv, 2, D}, kc, false);
+    r.holds(a[2], "block_table", kInt32, {B, -1}, kc, false);
+    r.holds(a[3], "context_lens", kInt32, {B}, kc, false);
+    check_scales(r, a[5], "k_scale", ct, kc, Hkv, kc);
+    const int news = r.integer(a[4]), mb = r.dim(a[2], 1), N = r.blocks(a[6], kc);
+    check_blocks(r, N, kc);
+    r.current(kc, B > 0 && news > 0);
+    void *k = r.ptr(kc), *bo = r.ptr(a[1]);
+    auto *bt = r.ptr<int32_t>(a[2]), *cx = r.ptr<int32_t>(a[3]);
+    auto* ks = r.ptr<float>(a[5]);
+    void* s = r.stream(a[7]);
+    return finish(r, [&] { return fn.key_bounds(k, ct, ks, bo, bt, cx, B, news, Hkv, D, FFKV_BLOCK_SIZE, mb, N, s); });
+}
+
+// Blocks of queries of a row (0 where query_block is refused by the call).
+int lists_of(int S, int query_block) { return query_block > 0 ? static_cast<int>((static_cast<int64_t>(S) + query_block - 1) / query_block) : 0; }
+
+// q, bounds, block_table, context_lens, count, sinks, recent, query_block, blocks, max_context_len, workspace, num_blocks,
+// stream, scratch
+PyObject* select_blocks(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!count(n, 14)) return nullptr;
+    Reader    r{a};
+    PyObject* q = a[0];
+    int       B, S, Hq, D;
+    r.dims4(q, B, S, Hq, D);
+    const int qt = r.dtype(q), bt = r.dtype(a[1]), Hkv = r.dim(a[1], 1);
+    r.plain(q, "q", q);
+    r.holds(a[1], "bounds", bt, {-1, Hkv, 2, D}, q, false);
+    r.holds(a[2], "block_table", kInt32, {B, -1}, q, false);
+    r.holds(a[3], "context_lens", kInt32, {B}, q, false);
+    const int keep = r.integer(a[4]), sinks = r.integer(a[5]), recent = r.integer(a[6]), T = r.integer(a[7]);
+    if (r.ok && T > 0) r.holds(a[8], "blocks", kInt32, {B, lists_of(S, T), Hkv, keep}, q, false);
+    const int mcl = r.integer(a[9]), mb = r.dim(a[2], 1), N = r.blocks(a[11], a[1]);
+    check_blocks(r, N, a[1]);
+    r.plain(a[10], "workspace", q);
+    r.current(q, B > 0 && S > 0);
+    void *qp = r.ptr(q), *bo = r.ptr(a[1]);
+    auto *tab = r.ptr<int32_t>(a[2]), *cx = r.ptr<int32_t>(a[3]), *out = r.ptr<int32_t>(a[8]);
+    void*         s = r.stream(a[12]);
+    const size_t  need = r.ok && a[10] == Py_None ? fn.select_bytes(B, S, Hkv, keep, T, mb, mcl) : 0;
+    const Scratch ws(r, a[10], a[13], need, q, a[12]);
+    return finish(r, [&] {
+        return fn.select_blocks(qp, qt, bo, bt, tab, cx, out, keep, sinks, recent, T, B, S, Hq, Hkv, D, FFKV_BLOCK_SIZE, mb, N,
+                                mcl, ws.ptr, ws.bytes, s);
+    });
+}
+
+// q, out, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, blocks, query_block, scale, workspace, num_blocks,
+// stream, scratch
+PyObject* attention_blocks(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!count(n, 15)) return nullptr;
+    Reader    r{a};
+    PyObject* q = a[0];
+    PyObject* sh = r.shape(q, 3, false);
+    if (r.ok && PyTuple_GET_SIZE(sh) > 4) r.refuse(PyExc_ValueError, "q must be [B, S, Hq, D] or [B, Hq, D], got %S", sh);
+    const bool four = r.ok && PyTuple_GET_SIZE(sh) == 4;
+    Py_XDECREF(sh);
+    const int B = r.dim(q, 0), S = four ? r.dim(q, 1) : 1, Hq = r.dim(q, -2), D = r.dim(q, -1);
+    const int qt = r.dtype(q), ct = r.dtype(a[2]), Hkv = r.dim(a[2], 2);
+    r.plain(q, "q", q);
+    r.plain(a[1], "out", q);
+    if (r.ok && r.dtype(a[1]) != qt) r.refuse(PyExc_TypeError, "out must have q's dtype");
+    if (r.ok && r.nbytes(a[1]) != r.nbytes(q)) r.refuse(PyExc_ValueError, "out must have as many values as q");
+    r.holds(a[2], "k_cache", ct, {-1, FFKV_BLOCK_SIZE, Hkv, D}, q, false);
+    r.holds(a[3], "v_cache", ct, {r.dim(a[2], 0), FFKV_BLOCK_SIZE, Hkv, D}, q, false);
+    check_scales(r, a[4], "k_scale", ct, a[2], Hkv, q);
+    check_scales(r, a[5], "v_scale", ct, a[2], Hkv, q);
+    r.holds(a[6], "block_table", kInt32, {B, -1}, q, false);
+    r.holds(a[7], "context_lens", kInt32, {B}, q, false);
+    const int T = r.integer(a[9]);
+    if (r.ok && T > 0) r.holds(a[8], "blocks", kInt32, {B, lists_of(S, T), Hkv, -1}, q, false);
+    const int   keep = r.dim(a[8], -1), mb = r.dim(a[6], 1), N = r.blocks(a[12], a[2]);
+    const float scale = r.real(a[10]);
+    check_blocks(r, N, a[2]);
+    r.plain(a[11], "workspace", q);
+    r.current(q, B > 0 && S > 0);
+    void *qp = r.ptr(q), *out = r.ptr(a[1]), *kc = r.ptr(a[2]), *vc = r.ptr(a[3]);
+    auto *ks = r.ptr<float>(a[4]), *vs = r.ptr<float>(a[5]);
+    auto *bt = r.ptr<int32_t>(a[6]), *cx = r.ptr<int32_t>(a[7]), *bl = r.ptr<int32_t>(a[8]);
+    void*         s = r.stream(a[13]);
+    const size_t  need = r.ok && a[11] == Py_None ? fn.attention_blocks_bytes(ct, B, S, Hq, Hkv, D, keep, T) : 0;
+    const Scratch ws(r, a[11], a[14], need, q, a[13]);
+    return finish(r, [&] {
+        return fn.attention_blocks(qp, out, qt, kc, vc, ct, ks, vs, bt, cx, bl, keep, T, B, S, Hq, Hkv, D, FFKV_BLOCK_SIZE, mb, N,
+                                   scale, ws.ptr, ws.bytes, s);
+    });
+}
+
 // bind(addresses, [(dtype, code), ..], get_device, raw_stream, first_stream): the library's functions in Functions'
 // order, torch's dtypes, and how the current stream's handle is found (first_stream() until it has succeeded once,
 // which initialises torch's GPU state; then raw_stream(get_device())).
@@ -765,6 +1004,8 @@ PyObject* forget_stream(PyObject*, PyObject*)
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(decode_scored),  FAST(prefill_scored), FAST(evict), FAST(attention_weights),
+                         FAST(rope_axes),      FAST(rope_append_axes), FAST(key_bounds), FAST(select_blocks),
+                         FAST(attention_blocks),
                          FAST(append),         FAST(decode),  FAST(decode_shared), FAST(append_decode),
                          FAST(decode_noalloc), FAST(prefill), FAST(rope),          FAST(rope_append),
                          {"bind", bind, METH_VARARGS, nullptr},
@@ -786,6 +1027,7 @@ PyMODINIT_FUNC PyInit__front(void)
     s_index = PyUnicode_InternFromString("index");
     s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
     s_is_cuda = PyUnicode_InternFromString("is_cuda");
+    s_stride = PyUnicode_InternFromString("stride");
     if (PyErr_Occurred()) return nullptr;
     return PyModule_Create(&module);
 }

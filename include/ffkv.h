@@ -399,6 +399,92 @@ FFKV_API int ffkv_evict(const float* weights, int64_t weight_stride, const int32
                         int num_kv_heads, int head_dim, int block_size, int num_blocks, void* workspace,
                         size_t workspace_bytes, void* stream);
 
+/* ---- positions on several axes, and attention over selected pages (no counterpart in the reference) ------------------ */
+
+/*
+ * Rotary embedding by positions on several axes (time, height and width of image and video tokens).  Pair i of a head (dims
+ * i, i + head_dim/2) of token t of row b turns by positions[axis(i)][b][t] * rope_theta^(-2i/head_dim), in ffkv_rope's form;
+ * with equal positions on all axes that is ffkv_rope's rotation.  positions int32 [axes, batch, seq_len], any int32; axes 1 to
+ * 4; sections (host memory): the pairs of dims of each axis, head_dim/2 together.  interleaved 0: the first sections[0] pairs
+ * turn by axis 0, the next sections[1] by axis 1, ..; else pair i turns by axis i % axes while that axis has pairs left
+ * (sections[a] of the pairs a, a + axes, ..), all others by axis 0.  The turns are one fp64 product, whose fraction enters cos
+ * and sin: good to 2^-22 at any position.  (ffkv_rope rounds its angle to fp32: far positions differ by 2^-24 of the angle.)
+ *
+ * q [batch, seq_len, num_heads, head_dim] (NULL: none) and k [batch, seq_len, num_kv_heads, head_dim] of one dtype (F32, F16,
+ * BF16), head_dim 64, 128 or 256; q_stride etc.: elements from token to token (0: one behind the other; a view into a packed
+ * projection has the projection's width), a multiple of 16 bytes; row b's tokens begin batch-contiguously, seq_len * stride
+ * behind row b - 1's.  q_out and k_out: q and k themselves (in place, with their strides) or memory that overlaps neither.
+ */
+FFKV_API int ffkv_rope_axes(const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, const void* k,
+                            int64_t k_stride, void* k_out, int64_t k_out_stride, int dtype, const int32_t* positions,
+                            const int* sections, int axes, int interleaved, int batch, int seq_len, int num_heads,
+                            int num_kv_heads, int head_dim, float rope_theta, void* stream);
+
+/*
+ * ffkv_rope_axes and ffkv_append of the rotated k (as rounded in src_dtype) and v in one pass.  Token t of row b goes to cache
+ * position context_lens[b] + t (NULL: t), whatever its positions on the axes are.  k and v are only read: the rotated k is in
+ * the pages alone.  The pages are those of ffkv_rope_axes followed by ffkv_append.
+ */
+FFKV_API int ffkv_rope_append_axes(const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, const void* k,
+                                   int64_t k_stride, const void* v, int64_t v_stride, int src_dtype, void* k_cache,
+                                   void* v_cache, int cache_dtype, float* k_scale, float* v_scale,
+                                   const int32_t* block_table, const int32_t* context_lens, const int32_t* positions,
+                                   const int* sections, int axes, int interleaved, int batch, int seq_len, int num_heads,
+                                   int num_kv_heads, int head_dim, int block_size, int max_blocks, int num_blocks,
+                                   float rope_theta, void* stream);
+
+/*
+ * Key bounds of the pages that the new_tokens tokens from position context_lens[b] on of every row lie on (already appended):
+ * for each KV head and dim the smallest and the largest key of the page's tokens of the row, earlier ones included, into
+ * bounds [num_blocks, num_kv_heads, 2, head_dim] (lo, then hi).  bounds have the cache's type, or bf16 beside int8 and fp8
+ * caches, there rounded outward.  A NaN key gives NaN bounds.  Call it after every append; pages without their row's later
+ * tokens (a prefix that rows share, once full) keep their bounds.  Pages on no block-table entry are skipped.
+ */
+FFKV_API int ffkv_key_bounds(const void* k_cache, int cache_dtype, const float* k_scale, void* bounds,
+                             const int32_t* block_table, const int32_t* context_lens, int batch, int new_tokens,
+                             int num_kv_heads, int head_dim, int block_size, int max_blocks, int num_blocks, void* stream);
+
+/*
+ * Which pages to attend: for every block of query_block query tokens (the last may be shorter) and KV head, `count` logical
+ * pages of the row.  Queries q [batch, seq_len, num_heads, head_dim] sit at positions context_lens[b] + t.  Of the pages up to
+ * the block's last query's, the first `sinks` and the last `recent` are taken, and of the rest those with the largest
+ *     score(page) = sum over the block's queries and the KV head's query heads of sum_d max(q_d lo_d, q_d hi_d)
+ * (fp64 sums rounded once to fp32; of equal scores the lower page; NaN counts as the largest; a page on no block-table entry
+ * as the lowest).  blocks int32 [batch, ceil(seq_len / query_block), num_kv_heads, count]: ascending, -1 behind a row of fewer
+ * pages.  `recent` pages count back from the block's last query: with query_block > 1 give at least query_block / 16 + 1 for
+ * every query to have its own page.  bounds_dtype F32, F16 or BF16 (ffkv_key_bounds' type).  max_context_len bounds the rows'
+ * tokens, this call's included (0: the table's width); pages past it are not taken.  workspace: NULL or
+ * ffkv_select_blocks_workspace_bytes (a captured call needs one where that is not 0).
+ */
+FFKV_API size_t ffkv_select_blocks_workspace_bytes(int batch, int seq_len, int num_kv_heads, int count, int query_block,
+                                                   int max_blocks, int max_context_len);
+
+FFKV_API int ffkv_select_blocks(const void* q, int q_dtype, const void* bounds, int bounds_dtype, const int32_t* block_table,
+                                const int32_t* context_lens, int32_t* blocks, int count, int sinks, int recent,
+                                int query_block, int batch, int seq_len, int num_heads, int num_kv_heads, int head_dim,
+                                int block_size, int max_blocks, int num_blocks, int max_context_len, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/*
+ * Causal attention over listed pages alone: query token t of row b at position context_lens[b] + t attends the tokens up to
+ * its own of the pages that blocks[b][t / query_block][kv_head] lists (int32 [batch, ceil(seq_len / query_block), num_kv_heads,
+ * count], as ffkv_select_blocks gives them).  Lists may be in any order; entries outside [0, max_blocks), on no block-table
+ * entry or past the query count for nothing, and a page listed twice counts twice.  A query without any key gives zeros.  What
+ * a query does not attend never reaches it, infinite and NaN values included.  q, out [batch, seq_len, num_heads, head_dim];
+ * caches as ffkv_paged_decode takes them (all types; every query_block).  The tokens are already appended.  workspace: NULL or
+ * ffkv_paged_attention_blocks_workspace_bytes (0 but for few lists, which are then split; a captured call without one leaves
+ * them whole).
+ */
+FFKV_API size_t ffkv_paged_attention_blocks_workspace_bytes(int cache_dtype, int batch, int seq_len, int num_heads,
+                                                            int num_kv_heads, int head_dim, int count, int query_block);
+
+FFKV_API int ffkv_paged_attention_blocks(const void* q, void* out, int qo_dtype, const void* k_cache, const void* v_cache,
+                                         int cache_dtype, const float* k_scale, const float* v_scale,
+                                         const int32_t* block_table, const int32_t* context_lens, const int32_t* blocks,
+                                         int count, int query_block, int batch, int seq_len, int num_heads,
+                                         int num_kv_heads, int head_dim, int block_size, int max_blocks, int num_blocks,
+                                         float scale, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Message describing the last error returned on the calling thread ("" if none). */
 FFKV_API const char* ffkv_last_error(void);
 

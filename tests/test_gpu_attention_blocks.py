@@ -1,0 +1,181 @@
+"""Attention over listed pages, against float64."""
+
+import numpy as np
+import pytest
+import torch
+
+import blocks_util as bu
+import cases
+import oracle as O
+import scored_util as su
+
+pytestmark = pytest.mark.gpu
+
+
+def make(seed, ctx, S, Hq, Hkv, D, act="bf16", kv=None, spread=2.0, **kw):
+    c = cases.make_case(seed, len(ctx), Hq, Hkv, D, ctx, act=act, kv=kv, S=S, **kw)
+    c.rng = np.random.default_rng(seed + 1)
+    c.q = cases.encode(c.rng.standard_normal((c.B, S, Hq, D), dtype=np.float32) * np.float32(spread), c.act)
+    return c
+
+
+def lists(c, S, count, T, shuffle=False):
+    """Lists of a row's pages: some of them, in order, -1 behind; shuffled: in any order, with pages that are none."""
+    blocks = -(-S // T)
+    out = np.full((c.B, blocks, c.Hkv, count), -1, np.int32)
+    for b in range(c.B):
+        for r in range(blocks):
+            n = (int(c.ctx[b]) + min((r + 1) * T, S) - 1) // 16 + 1
+            for h in range(c.Hkv):
+                got = np.sort(c.rng.permutation(n)[:count])
+                out[b, r, h, :len(got)] = got
+                if shuffle:
+                    bad = c.rng.random(count) < 0.2
+                    out[b, r, h, bad] = c.rng.choice([-1, -7, c.max_blocks, c.max_blocks + 3, 2 ** 31 - 1, -2 ** 31], bad.sum())
+                    out[b, r, h] = c.rng.permutation(out[b, r, h])
+    return out
+
+
+def run(ff, c, li, T, dev, workspace=None, **kw):
+    kp, vp, ks, vs, bt, cx, _, _, q = su.device(c, dev)
+    return ff.paged_attention_blocks(q, kp, vp, bt, cx, torch.from_numpy(li).to(dev), query_block=T, k_scale=ks, v_scale=vs,
+                                     workspace=workspace, **kw)
+
+
+def check(ff, c, li, T, dev, what="out"):
+    S = c.q.shape[1]
+    got = su.host(run(ff, c, li, T, dev)).reshape(c.B, S, c.Hq, c.D)
+    q = cases.decode(c.q, c.act).astype(np.float64)
+    want, bound = bu.attend(c, q, li, T, c.act, S, 2.0 ** -10 if T > 1 else 2.0 ** -11)
+    su.check(got, want, bound, what)
+    return got
+
+
+KV = [("bf16", "bf16"), ("f16", "f16"), ("bf16", "i8"), ("bf16", "fp8"), ("f32", "f32"), ("f16", "i8"), ("f32", "bf16"),
+      ("f16", "fp8"), ("bf16", "f16")]
+
+
+@pytest.mark.parametrize("act,kv", KV)
+@pytest.mark.parametrize("Hq,Hkv,D,ctx,count", [
+    (16, 8, 128, [17, 64, 100, 255], 4), (28, 4, 128, [3000], 150), (5, 1, 64, [0, 15, 16, 900], 7), (8, 8, 256, [500, 31], 20),
+    (6, 2, 96, [1000, 3], 33), (3, 3, 80, [200, 400], 5), (4, 2, 112, [640], 41), (20, 1, 128, [800, 900], 30),
+    (2, 2, 8, [100], 3), (36, 2, 64, [333], 9),
+])
+def test_step(ff, gpu, act, kv, Hq, Hkv, D, ctx, count):
+    c = make(Hq + D, ctx, 1, Hq, Hkv, D, act, kv)
+    check(ff, c, lists(c, 1, count, 1), 1, gpu)
+
+
+@pytest.mark.parametrize("act,kv", KV)
+@pytest.mark.parametrize("Hq,Hkv,D,ctx,S,count,T", [
+    (8, 2, 128, [700, 0], 70, 12, 64), (4, 4, 64, [100], 33, 6, 16), (10, 2, 256, [300, 15], 40, 9, 40),
+    (14, 2, 128, [64], 17, 3, 100), (8, 2, 128, [257], 5, 8, 2), (6, 2, 96, [90], 20, 5, 8), (32, 1, 64, [500], 9, 21, 9),
+    (4, 1, 128, [40, 300], 6, 7, 1),
+])
+def test_chunk(ff, gpu, act, kv, Hq, Hkv, D, ctx, S, count, T):
+    c = make(Hq + S, ctx, S, Hq, Hkv, D, act, kv)
+    check(ff, c, lists(c, S, count, T), T, gpu)
+
+
+@pytest.mark.parametrize("act,kv", [("bf16", "bf16"), ("bf16", "i8"), ("bf16", "fp8"), ("f32", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("S,T", [(1, 1), (9, 1), (50, 16)])
+def test_any_order(ff, gpu, act, kv, S, T):
+    """Lists out of order, with entries that are no page, pages past the query, and pages on no table entry."""
+    c = make(S + T, [700, 40, 0], S, 8, 2, 128, act, kv)
+    c.block_table[0, 5], c.block_table[0, 9], c.block_table[1, 1] = -1, c.num_blocks, -3
+    li = lists(c, S, 30, T, shuffle=True)
+    li[:, :, :, 3] = np.maximum(li[:, :, :, 3], 40)  # past the shorter rows
+    check(ff, c, li, T, gpu)
+
+
+@pytest.mark.parametrize("S,T", [(1, 1), (20, 10)])
+def test_nothing_and_twice(ff, gpu, S, T):
+    """Lists without any page give zeros; a page listed twice counts twice."""
+    c = make(4, [300, 200, 100], S, 4, 2, 128)
+    li = lists(c, S, 6, T)
+    li[0, :, 0], li[1] = -1, 99
+    li[2, :, :, 4] = li[2, :, :, 1]
+    got = check(ff, c, li, T, gpu)
+    assert not got[0, :, :2].any() and not got[1].any() and got[2].any()
+
+
+@pytest.mark.parametrize("act,kv", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "fp8"), ("bf16", "i8"), ("f32", "f32")])
+@pytest.mark.parametrize("S,T", [(1, 1), (6, 1), (40, 16)])
+def test_hidden_values_do_not_reach(ff, gpu, act, kv, S, T):
+    """NaN and infinite values in the slots behind the row and, of a chunk, behind each query; in pages that are not listed."""
+    c = make(31, [90, 205], S, 8, 2, 128, act, kv)
+    li = lists(c, S, 8, T)
+    for b in range(2):
+        last = int(c.ctx[b]) + S - 1
+        li[b, :, :, -1] = last // 16 if S == 1 else -1
+        for r in range(li.shape[1]):  # the page of the block's first query, whose later slots it must not see
+            li[b, r, :, -1] = (int(c.ctx[b]) + r * T) // 16
+            for h in range(c.Hkv):
+                li[b, r, h, :-1][li[b, r, h, :-1] == li[b, r, h, -1]] = -1
+        for t in range(last + 1, 16 * ((last + 16) // 16)):
+            su.poison(c, b, t)
+    dense = bu.attend(c, cases.decode(c.q, c.act).astype(np.float64), li, T, c.act, S, 2.0 ** -10)
+    if S > 1 and kv != "i8":  # a value that only the last queries see: the others are what they were
+        seen = int(c.ctx[0]) + S - 2
+        su.poison(c, 0, seen)
+    got = su.host(run(ff, c, li, T, gpu)).reshape(c.B, S, c.Hq, c.D)
+    upto = S - 2 if S > 1 and kv != "i8" else S
+    su.check(got[:1, :upto], dense[0][:1, :upto], dense[1][:1, :upto], "row 0")
+    su.check(got[1:], dense[0][1:], dense[1][1:], "row 1")
+    assert np.isfinite(got[:1, :upto]).all() and np.isfinite(got[1:]).all()
+
+
+@pytest.mark.parametrize("act,kv", [("bf16", "bf16"), ("bf16", "i8"), ("f32", "f32")])
+def test_all_pages_are_the_dense_attention(ff, gpu, act, kv):
+    c = make(12, [500, 33], 1, 8, 2, 128, act, kv)
+    li = np.broadcast_to(np.arange(c.max_blocks, dtype=np.int32), (2, 1, 2, c.max_blocks)).copy()
+    got = check(ff, c, li, 1, gpu)
+    kp, vp, ks, vs, bt, cx, _, _, q = su.device(c, gpu)
+    dense = su.host(ff.paged_attention(q, kp, vp, bt, cx, k_scale=ks, v_scale=vs)).reshape(got.shape)
+    _, bound = bu.attend(c, cases.decode(c.q, c.act).astype(np.float64), li, 1, c.act, 1, 2.0 ** -11)
+    su.check(got, dense, 2 * bound, "dense")  # each is off by the bound
+
+
+@pytest.mark.parametrize("scale", [0.0, 0.5])
+def test_scale_workspace_stream(ff, gpu, scale):
+    """A split call with its workspace, without one, and on another stream gives the same bits."""
+    c = make(21, [4000], 1, 8, 2, 128)
+    li = lists(c, 1, 200, 1)
+    n = ff.lib.ffkv_paged_attention_blocks_workspace_bytes(c.kv, 1, 1, 8, 2, 128, 200, 1)
+    assert n > 0
+    ws = ff.attention_blocks_workspace(c.kv, 1, 1, 8, 2, 128, 200)
+    a = run(ff, c, li, 1, gpu, workspace=ws, scale=scale)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    b = run(ff, c, li, 1, gpu, scale=scale, stream=side)
+    side.synchronize()
+    assert torch.equal(a, b)
+    c.q = cases.encode(cases.decode(c.q, c.act) * np.float32(scale * 128 ** 0.5 if scale else 1), c.act)
+    if scale == 0.0:
+        check(ff, c, li, 1, gpu)
+
+
+@pytest.mark.parametrize("S,T", [(1, 1), (24, 8)])
+def test_capture(ff, gpu, S, T):
+    """Captured with and without a workspace, replayed over new queries, lists and lengths."""
+    c = make(6, [4000, 900], S, 8, 2, 128)
+    kp, vp, ks, vs, bt, cx, _, _, q = su.device(c, gpu)
+    li = torch.from_numpy(lists(c, S, 200, T)).to(gpu)
+    ws = ff.attention_blocks_workspace(c.kv, 2, S, 8, 2, 128, 200, T)
+    out, whole = torch.empty(2, S, 8 * 128, dtype=q.dtype, device=gpu), torch.empty(2, S, 8 * 128, dtype=q.dtype, device=gpu)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ff.paged_attention_blocks(q, kp, vp, bt, cx, li, query_block=T, out=out, workspace=ws)
+        ff.paged_attention_blocks(q, kp, vp, bt, cx, li, query_block=T, out=whole)
+    for i in range(3):
+        q.mul_(-0.7)
+        li.copy_(li.roll(1, dims=-1))
+        cx.sub_(30)
+        graph.replay()
+        got, got_whole = out.clone(), whole.clone()
+        torch.cuda.synchronize()
+        eager = ff.paged_attention_blocks(q, kp, vp, bt, cx, li, query_block=T, workspace=ws)
+        assert torch.equal(got, eager)
+        # an unsplit softmax is the same up to its sums' roundings and the output's
+        assert (got.float() - got_whole.float()).abs().max().item() <= 2.0 ** -7 * got.float().abs().max().item()
