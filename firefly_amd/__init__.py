@@ -125,7 +125,7 @@ def _load() -> ctypes.CDLL:
     lib.ffkv_key_bounds.restype = i32
     lib.ffkv_key_bounds.argtypes = [vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp]
     lib.ffkv_select_blocks_workspace_bytes.restype = sz
-    lib.ffkv_select_blocks_workspace_bytes.argtypes = [i32] * 7
+    lib.ffkv_select_blocks_workspace_bytes.argtypes = [i32] * 9
     lib.ffkv_select_blocks.restype = i32
     lib.ffkv_select_blocks.argtypes = [vp, i32, vp, i32, vp, vp, vp, *[i32] * 13, vp, sz, vp]
     lib.ffkv_paged_attention_blocks_workspace_bytes.restype = sz
@@ -503,12 +503,13 @@ def update_key_bounds(k_cache, bounds, block_table, context_lens, new_tokens: in
     check(_front.key_bounds(k_cache, bounds, block_table, context_lens, new_tokens, k_scale, num_blocks, stream))
 
 
-def select_blocks_workspace(batch: int, seq_len: int, num_kv_heads: int, count: int, query_block: int, max_blocks: int,
-                            max_context_len: int = 0, device=None):
+def select_blocks_workspace(batch: int, seq_len: int, num_heads: int, num_kv_heads: int, head_dim: int, count: int,
+                            query_block: int, max_blocks: int, max_context_len: int = 0, device=None):
     """A workspace for ``select_blocks`` (``ffkv_select_blocks_workspace_bytes``)."""
     import torch
 
-    n = int(lib.ffkv_select_blocks_workspace_bytes(batch, seq_len, num_kv_heads, count, query_block, max_blocks, max_context_len))
+    n = int(lib.ffkv_select_blocks_workspace_bytes(batch, seq_len, num_heads, num_kv_heads, head_dim, count, query_block,
+                                                   max_blocks, max_context_len))
     return torch.empty(max(n, 256), dtype=torch.uint8, device=device if device is not None else "cuda")
 
 

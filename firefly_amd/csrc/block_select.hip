@@ -2,13 +2,13 @@
 // bounds, and the pages with the largest.
 //
 //   score(page) = sum over the block's queries and the KV head's query heads of sum_d max(q_d lo_d, q_d hi_d)
-//               = sum_d Q+_d hi_d + Q-_d lo_d,   Q+ = sum of max(q, 0), Q- = sum of min(q, 0)
+//               = sum_d Q-_d lo_d + Q+_d hi_d,   Q- = sum of min(q, 0), Q+ = sum of max(q, 0)
 // No query's score with any of the page's keys exceeds its share of that.  The sums over queries and heads go first, so a
 // block of any size costs two dot products of head_dim per page.
 //
 // Scores are fp64 sums rounded once to fp32: they decide between pages, and the choice must not depend on how a row is
-// split, on the batch or on the form that was launched (products of 16-bit values are exact in fp64, and the sums' errors of
-// 2^-50 are far below the rounding's step).
+// split, on the batch or on the form that was launched (products of 16-bit values are exact in fp64, the sums' errors of
+// 2^-50 are far below the rounding's step, and all forms add up a score in the same order).
 //
 // Of a block's pages - those up to its last query's - the first `sinks` and the last `recent` are taken, and of the rest
 // those with the largest scores, of equal ones the lower; NaN (a NaN or infinite key) counts as the largest.  The list is in
@@ -25,26 +25,68 @@ namespace
 {
 
 constexpr int kScoreThreads = 256;
-constexpr int kScoreWaves = kScoreThreads / 64;
-constexpr int kScoreUnroll = 4;  // pages a group of lanes has in flight
+constexpr int kScorePages = 4;  // neighbouring pages that a group of lanes scores together
 
-// v of lane ^ MASK within groups of N lanes summed up, in every lane of the group: fp64 in two 32-bit halves.
-template <int N>
-__device__ __forceinline__ double group_sum64(double v)
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v)
 {
-    auto step = [&](auto ctrl)
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, 0xf, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// v plus that of the lane 32 (16) away, in both.
+template <bool HALF>
+__device__ __forceinline__ double swap_sum64(double v)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = static_cast<uint32_t>(u), hi = static_cast<uint32_t>(u >> 32);
+    const auto     l = HALF ? __builtin_amdgcn_permlane32_swap(lo, lo, false, false)
+                            : __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+    const auto     h = HALF ? __builtin_amdgcn_permlane32_swap(hi, hi, false, false)
+                            : __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(static_cast<uint32_t>(h[0])) << 32 | static_cast<uint32_t>(l[0])) +
+           __builtin_bit_cast(double, static_cast<uint64_t>(static_cast<uint32_t>(h[1])) << 32 | static_cast<uint32_t>(l[1]));
+}
+
+// The sums over LPP lanes of four values each, value k in the group's lanes with lane % 4 == k: two exchanges halve the
+// values a lane holds, the rest add up across the quads (5 exchanges where four sums one by one take 16).
+template <int LPP>
+__device__ __forceinline__ double group_sums4(const double (&v)[4], int lane)
+{
+    const bool   b0 = lane & 1, b1 = lane & 2;
+    const double a = (b0 ? v[1] : v[0]) + dpp64<0xb1>(b0 ? v[0] : v[1]);  // quad lanes 1, 0, 3, 2
+    const double b = (b0 ? v[3] : v[2]) + dpp64<0xb1>(b0 ? v[2] : v[3]);
+    double       c = (b1 ? b : a) + dpp64<0x4e>(b1 ? a : b);              // quad lanes 2, 3, 0, 1
+    if constexpr (LPP == 8)
+        c += dpp64<0x141>(dpp64<0x1b>(c));  // lane 7 - (i ^ 3) of its 8: the other quad's same lane
+    else
     {
-        const uint64_t u = __builtin_bit_cast(uint64_t, v);
-        const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), decltype(ctrl)::value, 0xf, 0xf, false);
-        const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), decltype(ctrl)::value, 0xf, 0xf, false);
-        v += __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+        c += dpp64<0x124>(c);  // lanes 4 and 8 before it in its row of 16
+        c += dpp64<0x128>(c);
+    }
+    if constexpr (LPP == 32) c = swap_sum64<false>(c);
+    return c;
+}
+
+// Largest x of the wave, in every lane.
+__device__ __forceinline__ uint32_t wave_max(uint32_t x)
+{
+    auto take = [&x](auto ctrl, auto rows, auto zero)
+    {
+        const uint32_t o = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, decltype(rows)::value, 0xf,
+                                                       decltype(zero)::value);
+        x = o > x ? o : x;
     };
-    step(std::integral_constant<int, 0xb1>{});                            // quad lanes 1, 0, 3, 2
-    step(std::integral_constant<int, 0x4e>{});                            // quad lanes 2, 3, 0, 1
-    if constexpr (N >= 8) step(std::integral_constant<int, 0x141>{});     // lane 7 - i of its 8
-    if constexpr (N >= 16) step(std::integral_constant<int, 0x140>{});    // lane 15 - i of its 16
-    if constexpr (N >= 32) v += __shfl_xor(v, 16, 64);
-    return v;
+    using std::integral_constant;
+    take(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{}, integral_constant<bool, true>{});  // row_shr:1
+    take(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{}, integral_constant<bool, true>{});
+    take(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{}, integral_constant<bool, true>{});
+    take(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{}, integral_constant<bool, true>{});
+    take(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{}, integral_constant<bool, false>{});  // row_bcast:15
+    take(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{}, integral_constant<bool, false>{});  // row_bcast:31
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), 63));
 }
 
 // Visible pages of the block of queries `list` of row b.
@@ -63,136 +105,348 @@ __device__ __forceinline__ uint32_t score_key(float w)
     return w != w ? 0xffffffffu : u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
 
-// Q- and Q+ of a block of queries into LDS, [2][D], by all threads of the workgroup; s_part: [kScoreWaves][2][D].
-template <int LPP>
-__device__ __forceinline__ void sum_queries(const SelectArgs& a, int b, int list, int kvh, double* s_q, double* s_part)
+// A lane's share of Q- and Q+: its 8 dims of query row r of a block (rows: tokens, and the group's heads of each).
+__device__ __forceinline__ size_t query_at(const SelectArgs& a, int b, int t0, int kvh, int r, int c)
 {
-    const int  D = a.head_dim;
-    const int  tid = static_cast<int>(threadIdx.x);
-    const int  lane = tid & 63, wave = tid >> 6;
-    const int  c = lane % LPP;
-    const bool in = 8 * c < D;
-    const int  t0 = list * a.query_block;
-    const int  rows = min(a.query_block, a.seq_len - t0) * a.group;
-    double     down[8], up[8];
+    const int t = r / a.group;
+    return ((static_cast<size_t>(b) * a.seq_len + t0 + t) * a.num_heads + kvh * a.group + r - t * a.group) * a.head_dim + 8 * c;
+}
+__device__ __forceinline__ void add_query(const float (&x)[8], double (&down)[8], double (&up)[8])
+{
 #pragma unroll
-    for (int e = 0; e < 8; ++e) down[e] = up[e] = 0.0;
-    for (int r = tid / LPP; r < rows; r += kScoreThreads / LPP)
+    for (int e = 0; e < 8; ++e)  // (a NaN goes to both)
     {
-        if (!in) continue;
-        const int    t = r / a.group;
-        const size_t at = ((static_cast<size_t>(b) * a.seq_len + t0 + t) * a.num_heads + kvh * a.group + r - t * a.group) * D + 8 * c;
-        float        x[8];
-        load_act8(a.q, a.q_dtype, at, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-        {
-            // (a NaN goes to both)
-            down[e] += x[e] > 0.0f ? 0.0 : static_cast<double>(x[e]);
-            up[e] += x[e] < 0.0f ? 0.0 : static_cast<double>(x[e]);
-        }
+        down[e] += static_cast<double>(__builtin_elementwise_minimum(x[e], 0.0f));
+        up[e] += static_cast<double>(__builtin_elementwise_maximum(x[e], 0.0f));
     }
-#pragma unroll
-    for (int off = LPP; off < 64; off <<= 1)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-        {
-            down[e] += __shfl_xor(down[e], off, 64);
-            up[e] += __shfl_xor(up[e], off, 64);
-        }
-    if (lane < LPP && in)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-        {
-            s_part[(wave * 2) * D + 8 * c + e] = down[e];
-            s_part[(wave * 2 + 1) * D + 8 * c + e] = up[e];
-        }
-    __syncthreads();
-    for (int i = tid; i < 2 * D; i += kScoreThreads)
-    {
-        double s = 0.0;
-#pragma unroll
-        for (int w = 0; w < kScoreWaves; ++w) s += s_part[w * 2 * D + i];
-        s_q[i] = s;
-    }
-    __syncthreads();
 }
 
-}  // namespace
-
-// A workgroup scores `tile` pages of a block of queries and KV head: LPP lanes take a page's bounds, 8 dims each, and
-// kScoreUnroll pages in flight.  Grid: (tile, KV head, block of queries of a row).
-template <int BT, int LPP>
-__global__ __launch_bounds__(kScoreThreads) void block_scores(SelectArgs a, int tile, int tiles)
+// The lane's share of a page's score, in the order that every form keeps.
+__device__ __forceinline__ double lane_score(const double (&down)[8], const double (&up)[8], const double (&lo)[8],
+                                             const double (&hi)[8])
 {
-    constexpr int GROUPS = kScoreThreads / LPP;  // pages of a round
-    __shared__ double s_q[2 * LPP * 8];
-    __shared__ double s_part[kScoreWaves * 2 * LPP * 8];
-    const int64_t wg = blockIdx.x;
-    const int     kvh = static_cast<int>(wg / tiles % a.num_kv_heads);
-    const int     row = static_cast<int>(wg / tiles / a.num_kv_heads);
-    const int     b = row / a.lists, list = row - b * a.lists;
-    const int     n = visible_pages(a, b, list);
-    const int     p0 = static_cast<int>(wg % tiles) * tile;
-    if (p0 >= n) return;
-    const int  p1 = min(n, p0 + tile);
-    const int  D = a.head_dim;
-    const int  tid = static_cast<int>(threadIdx.x);
-    const int  c = tid % LPP, grp = tid / LPP;
-    const bool in = 8 * c < D;
-    sum_queries<LPP>(a, b, list, kvh, s_q, s_part);
-    double down[8], up[8];
+    double s = 0.0;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
     {
-        down[e] = in ? s_q[8 * c + e] : 0.0;
-        up[e] = in ? s_q[D + 8 * c + e] : 0.0;
+        s = __builtin_fma(down[e], lo[e], s);
+        s = __builtin_fma(up[e], hi[e], s);
     }
-    const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
-    float* out = a.scores + (static_cast<int64_t>(row) * a.num_kv_heads + kvh) * a.stride;
-    for (int q0 = p0; q0 < p1; q0 += GROUPS * kScoreUnroll)
+    return s;
+}
+
+// Four pages' bounds in flight.  FULL: head_dim fills the LPP lanes.  Pages on no table entry read page 0 instead (a pool has
+// one), and lanes past head_dim the first dims: their scores are not used, their sums of queries zero.
+template <int BT, int LPP, bool FULL>
+struct PageBounds
+{
+    Raw8 lo[kScorePages], hi[kScorePages];
+    int  on;  // bit k: page k is on a table entry
+
+    // Physical pages of logical pages p .. p + 3 below end.
+    __device__ __forceinline__ static void entries(const int32_t* table, int p, int end, int (&phys)[kScorePages])
     {
-        Raw8 lo[kScoreUnroll], hi[kScoreUnroll];
-        bool ok[kScoreUnroll];
 #pragma unroll
-        for (int k = 0; k < kScoreUnroll; ++k)
+        for (int k = 0; k < kScorePages; ++k) phys[k] = p + k < end ? table[p + k] : -1;
+    }
+    __device__ __forceinline__ void load(const SelectArgs& a, const int (&phys)[kScorePages], int kvh, int c)
+    {
+        const int D = FULL ? LPP * 8 : a.head_dim;
+        on = 0;
+#pragma unroll
+        for (int k = 0; k < kScorePages; ++k)
         {
-            const int p = q0 + k * GROUPS + grp;
-            const int phys = p < p1 ? table[p] : -1;
-            ok[k] = phys >= 0 && phys < a.num_blocks;
-            if (ok[k] && in)
-            {
-                const size_t at = (static_cast<size_t>(phys) * a.num_kv_heads + kvh) * 2 * D + 8 * c;
-                load_raw8<BT>(a.bounds, at, lo[k]);
-                load_raw8<BT>(a.bounds, at + D, hi[k]);
-            }
+            const bool     ok = phys[k] >= 0 && phys[k] < a.num_blocks;
+            const uint32_t page = ok ? phys[k] : 0;
+            on |= ok ? 1 << k : 0;
+            const size_t at = (static_cast<size_t>(page) * a.num_kv_heads + kvh) * (2 * D) + (FULL || 8 * c < D ? 8 * c : 0);
+            load_raw8<BT>(a.bounds, at, lo[k]);
+            load_raw8<BT>(a.bounds, at + D, hi[k]);
         }
+    }
+    __device__ __forceinline__ void values(int k, bool in, double (&l)[8], double (&h)[8]) const
+    {
+        float x[8], y[8];
+        unpack8<BT>(lo[k], x);
+        unpack8<BT>(hi[k], y);
 #pragma unroll
-        for (int k = 0; k < kScoreUnroll; ++k)
+        for (int e = 0; e < 8; ++e)
         {
-            double s = 0.0;
-            if (ok[k] && in)
+            l[e] = static_cast<double>(FULL || in ? x[e] : 0.0f);
+            h[e] = static_cast<double>(FULL || in ? y[e] : 0.0f);
+        }
+    }
+};
+
+}  // namespace
+
+// A step (a few query rows, one block of them).  The rounds of ROUND pages of all rows and KV heads form one sequence, of
+// which every workgroup takes an equal share, as many workgroups as fit the chip: rows of 125 to 1000 pages in tiles of their
+// own left it waiting for the longest (64 rows, 8 heads: 38 us, 28 so).  LPP lanes take four neighbouring pages' bounds, 8
+// dims each, and every lane adds up its dims of the queries by itself; while a round is added up the next one's bounds are on
+// their way, and the table's entries of the one after.
+template <int BT, int QT, int LPP, bool FULL>
+__global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a)
+{
+    constexpr int ROUND = kScoreThreads / LPP * kScorePages;  // pages of a round
+    const int  tid = static_cast<int>(threadIdx.x);
+    const int  lane = tid & 63;
+    const int  c = tid % LPP, grp = tid / LPP;
+    const bool in = FULL || 8 * c < a.head_dim;
+    auto rounds_of = [&](int b) { return (visible_pages(a, b, 0) + ROUND - 1) / ROUND; };
+
+    // this workgroup's share (every wave on its own)
+    const int H = a.num_kv_heads;
+    int64_t   total = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64)
+        total += uniform(wave_sum(b0 + lane < a.batch ? rounds_of(b0 + lane) : 0));
+    total *= H;
+    const int64_t wgs = min(static_cast<int64_t>(gridDim.x), total);
+    if (blockIdx.x >= wgs) return;
+    int64_t x0, x1;
+    if (total < 1 << 20)  // (their product with the grid's at most 2048 workgroups in 32 bits)
+    {
+        const uint32_t t = static_cast<uint32_t>(total), w = static_cast<uint32_t>(wgs);
+        x0 = blockIdx.x * t / w;
+        x1 = (blockIdx.x + 1) * t / w;
+    }
+    else
+    {
+        x0 = blockIdx.x * total / wgs;
+        x1 = (blockIdx.x + 1) * total / wgs;
+    }
+    // its first round: row, KV head, round of the row
+    struct Place
+    {
+        int b, kvh, round, rounds;
+    };
+    Place at{0, 0, 0, 0};
+    {
+        int64_t base = 0;
+        for (int b0 = 0;; b0 += 64)
+        {
+            const int r = b0 + lane < a.batch ? rounds_of(b0 + lane) : 0;
+            const int upto = wave_scan(r);  // (rounds of 64 rows: below 2^31 / 64 pages each)
+            const int64_t mine = base + static_cast<int64_t>(upto - r) * H;
+            const uint64_t hit = __ballot(mine <= x0 && x0 < mine + static_cast<int64_t>(r) * H);
+            if (hit != 0)
             {
-                float x[8], y[8];
-                unpack8<BT>(lo[k], x);
-                unpack8<BT>(hi[k], y);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                {
-                    s = __builtin_fma(down[e], static_cast<double>(x[e]), s);
-                    s = __builtin_fma(up[e], static_cast<double>(y[e]), s);
-                }
+                const int l = __ffsll(static_cast<long long>(hit)) - 1;
+                at.b = b0 + l;
+                at.rounds = __builtin_amdgcn_readlane(r, l);
+                const int off = static_cast<int>(x0 - base) - __builtin_amdgcn_readlane(upto - r, l) * H;
+                at.kvh = off / at.rounds;
+                at.round = off - at.kvh * at.rounds;
+                break;
             }
-            s = group_sum64<LPP>(s);
-            const int p = q0 + k * GROUPS + grp;
-            if (c == 0 && p < p1) out[p] = ok[k] ? static_cast<float>(s) : kNegInf;  // on no page: last
+            base += static_cast<int64_t>(__builtin_amdgcn_readlane(upto, 63)) * H;
+        }
+    }
+    auto next = [&](Place p)
+    {
+        if (++p.round < p.rounds) return p;
+        p.round = 0;
+        if (++p.kvh < H) return p;
+        p.kvh = 0;
+        do
+            p.rounds = ++p.b < a.batch ? rounds_of(p.b) : 1;
+        while (p.rounds == 0);
+        return p;
+    };
+    int  phys[kScorePages];
+    auto entries = [&](const Place& p)  // (those past the row's last page are not used: they lie in the table's row)
+    {
+        const int first = p.round * ROUND + grp * kScorePages;
+        PageBounds<BT, LPP, FULL>::entries(a.block_table + static_cast<int64_t>(p.b) * a.max_blocks, first, a.most_pages, phys);
+    };
+    constexpr int QROWS = 4;  // query rows whose loads go out together
+    const int     rows = a.seq_len * a.group;
+    double        down[8], up[8];
+    auto sum_queries = [&](const Place& p)
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) down[e] = up[e] = 0.0;
+        for (int r0 = 0; r0 < rows; r0 += QROWS)
+        {
+            Raw8 q[QROWS];
+#pragma unroll
+            for (int u = 0; u < QROWS; ++u)
+                if (r0 + u < rows && in) load_raw8<QT>(a.q, query_at(a, p.b, 0, p.kvh, r0 + u, c), q[u]);
+#pragma unroll
+            for (int u = 0; u < QROWS; ++u)
+                if (r0 + u < rows && in)
+                {
+                    float x[8];
+                    unpack8<QT>(q[u], x);
+                    add_query(x, down, up);
+                }
+        }
+    };
+    Place ahead = next(at);
+    entries(at);
+    PageBounds<BT, LPP, FULL> cur, nxt;
+    cur.load(a, phys, at.kvh, c);
+    if (x0 + 1 < x1) entries(ahead);
+    sum_queries(at);
+    for (int64_t x = x0; x < x1; ++x)
+    {
+        if (x + 1 < x1) nxt.load(a, phys, ahead.kvh, c);
+        const Place after = next(ahead);
+        if (x + 2 < x1) entries(after);
+        double s[kScorePages];
+#pragma unroll
+        for (int k = 0; k < kScorePages; ++k)
+        {
+            double lo[8], hi[8];
+            cur.values(k, in, lo, hi);
+            s[k] = lane_score(down, up, lo, hi);
+        }
+        const double sum = group_sums4<LPP>(s, c);
+        const int    p = at.round * ROUND + grp * kScorePages + (c & 3);
+        float*       out = a.scores + (static_cast<int64_t>(at.b) * H + at.kvh) * a.stride;
+        // (behind the row's last page up to stride: read by nobody)
+        if (c < 4 && p < a.most_pages) out[p] = cur.on >> c & 1 ? static_cast<float>(sum) : kNegInf;  // on no page: last
+        if (x + 1 < x1 && (ahead.b != at.b || ahead.kvh != at.kvh)) sum_queries(ahead);
+        cur = nxt;
+        at = ahead;
+        ahead = after;
+    }
+}
+
+// Q- and Q+ of every block of queries and KV head.
+constexpr int kSumThreads = 1024;
+template <int QT, int LPP>
+__global__ __launch_bounds__(kSumThreads) void block_queries(SelectArgs a)
+{
+    constexpr int WAVES = kSumThreads / 64;
+    constexpr int STEP = kSumThreads / LPP;  // query rows that the workgroup takes at a time
+    constexpr int UN = 4;
+    __shared__ double s_part[WAVES][2][LPP * 8];
+    const int64_t wg = blockIdx.x;
+    const Split   u = split_index(blockIdx.x, a.num_kv_heads), v = split_index(u.div, a.lists);
+    const int     kvh = u.rem, b = static_cast<int>(v.div);
+    const int     t0 = v.rem * a.query_block;
+    const int     rows = min(a.query_block, a.seq_len - t0) * a.group;
+    const int     tid = static_cast<int>(threadIdx.x);
+    const int     lane = tid & 63, wave = tid >> 6;
+    const int     c = tid % LPP;
+    const bool    in = 8 * c < a.head_dim;
+    double        down[8], up[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) down[e] = up[e] = 0.0;
+    for (int r0 = tid / LPP; r0 < rows; r0 += UN * STEP)
+    {
+        Raw8 q[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+            if (r0 + u * STEP < rows && in) load_raw8<QT>(a.q, query_at(a, b, t0, kvh, r0 + u * STEP, c), q[u]);
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+            if (r0 + u * STEP < rows && in)
+            {
+                float x[8];
+                unpack8<QT>(q[u], x);
+                add_query(x, down, up);
+            }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+    {
+        if constexpr (LPP == 8)
+        {
+            down[e] += dpp64<0x128>(down[e]);  // 8 lanes before it in its row of 16
+            up[e] += dpp64<0x128>(up[e]);
+        }
+        if constexpr (LPP <= 16)
+        {
+            down[e] = swap_sum64<false>(down[e]);
+            up[e] = swap_sum64<false>(up[e]);
+        }
+        down[e] = swap_sum64<true>(down[e]);
+        up[e] = swap_sum64<true>(up[e]);
+        if (lane < LPP)
+        {
+            s_part[wave][0][8 * c + e] = down[e];
+            s_part[wave][1][8 * c + e] = up[e];
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < 2 * a.head_dim; i += kSumThreads)
+    {
+        const int half = i >= a.head_dim, d = i - half * a.head_dim;
+        double    s = 0.0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) s += s_part[w][half][d];
+        a.query_sums[wg * 2 * a.head_dim + i] = s;
+    }
+}
+
+// Many blocks of queries: a workgroup holds one round of a row's pages, as fp64, and goes through `per` blocks of queries of
+// the row, whose sums block_queries has left, LISTS of them at a time through LDS.
+template <int BT, int LPP, bool FULL>
+__global__ __launch_bounds__(kScoreThreads) void block_scores_lists(SelectArgs a, int tiles, int per, int parts)
+{
+    constexpr int ROUND = kScoreThreads / LPP * kScorePages;
+    constexpr int LISTS = 8;
+    __shared__ __align__(16) double s_q[LISTS][2][LPP * 8];
+    const Split u = split_index(blockIdx.x, tiles), v = split_index(u.div, parts), w = split_index(v.div, a.num_kv_heads);
+    const int  p0 = u.rem * ROUND, l0 = v.rem * per, kvh = w.rem, b = static_cast<int>(w.div);
+    const int  l1 = min(a.lists, l0 + per);
+    const int  tid = static_cast<int>(threadIdx.x);
+    const int  c = tid % LPP, grp = tid / LPP;
+    const int  D = FULL ? LPP * 8 : a.head_dim;
+    const bool in = FULL || 8 * c < D;
+    const int  p = p0 + grp * kScorePages;
+    int        phys[kScorePages];  // (entries past the row's end are read, not used: they lie in the table's row)
+    PageBounds<BT, LPP, FULL>::entries(a.block_table + static_cast<int64_t>(b) * a.max_blocks, p, a.most_pages, phys);
+    const int n1 = visible_pages(a, b, l1 - 1);  // earlier blocks see no more
+    if (p0 >= n1) return;
+#pragma unroll
+    for (int k = 0; k < kScorePages; ++k) phys[k] = p + k < n1 ? phys[k] : -1;
+    PageBounds<BT, LPP, FULL> raw;
+    raw.load(a, phys, kvh, c);
+    double lo[kScorePages][8], hi[kScorePages][8];
+    for (int m0 = l0; m0 < l1; m0 += LISTS)
+    {
+        const int m1 = min(l1, m0 + LISTS);
+        __syncthreads();  // the sums before are read
+        for (int i = tid; i < (m1 - m0) * 2 * D; i += kScoreThreads)
+        {
+            const int l = i / (2 * D), r = i - l * 2 * D, half = r >= D;
+            s_q[l][half][r - half * D] =
+                a.query_sums[((static_cast<int64_t>(b) * a.lists + m0 + l) * a.num_kv_heads + kvh) * 2 * D + r];
+        }
+        __syncthreads();
+        if (m0 == l0)
+#pragma unroll
+            for (int k = 0; k < kScorePages; ++k) raw.values(k, in, lo[k], hi[k]);
+        for (int l = m0; l < m1; ++l)
+        {
+            const int n = visible_pages(a, b, l);
+            if (p0 >= n) continue;
+            double down[8], up[8], s[kScorePages];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                down[e] = in ? s_q[l - m0][0][8 * c + e] : 0.0;
+                up[e] = in ? s_q[l - m0][1][8 * c + e] : 0.0;
+            }
+#pragma unroll
+            for (int k = 0; k < kScorePages; ++k) s[k] = lane_score(down, up, lo[k], hi[k]);
+            const double sum = group_sums4<LPP>(s, c);
+            float*       out = a.scores + ((static_cast<int64_t>(b) * a.lists + l) * a.num_kv_heads + kvh) * a.stride;
+            if (c < 4 && p + c < n) out[p + c] = raw.on >> c & 1 ? static_cast<float>(sum) : kNegInf;
         }
     }
 }
 
-// One workgroup per list.  The score of the last page to stay is found by three passes over the keys' bits, 11, 11 and 10 of
-// them, each a histogram in LDS of the keys that agree in the bits above and a search from its top; then the pages above it
-// and the first of those equal to it are written in order.  A list of up to THREADS * PER pages is read once.
+// One workgroup per list.  The score of the last page to stay: the keys between the smallest and the largest are dealt to
+// 2048 bins of one width (neighbouring scores share their leading bits: bins by those would hold nearly all of them, and
+// their counts in LDS wait for each other), the bin in which it lies is divided again while it holds more than kChooseMost,
+// and those left are ranked against each other.  Then the pages above it and the first of those equal to it are written in
+// order.  A thread holds PER neighbouring pages, and a list of up to THREADS * PER is read once.
+constexpr int kChooseMost = 256;
+
 template <int THREADS, int PER>
 __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
 {
@@ -200,18 +454,21 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
     constexpr int TILE = THREADS * PER;
     constexpr int BINS = 2048;
     constexpr int BPT = BINS / THREADS;  // bins a thread sums up
-    __shared__ int s_hist[BINS];
-    __shared__ int s_tot[WAVES];
-    __shared__ int s_found[2];
-    __shared__ int s_cnt[2][PER * WAVES];
+    static_assert(PER % 4 == 0 && TILE < 1 << 16, "16-byte reads; counts of a tile in 16 bits");
+    __shared__ __align__(16) int s_hist[BINS];
+    __shared__ int      s_tot[WAVES];
+    __shared__ uint32_t s_ends[2][WAVES];
+    __shared__ uint32_t s_keys[kChooseMost];
+    __shared__ uint32_t s_found[3];  // bin, of those in it how many stay, how many it holds
+    __shared__ int      s_left;
     const int64_t wg = blockIdx.x;
-    const int     row = static_cast<int>(wg / a.num_kv_heads);
-    const int     b = row / a.lists, list = row - b * a.lists;
-    const int     n = visible_pages(a, b, list);
+    const Split   u = split_index(split_index(blockIdx.x, a.num_kv_heads).div, a.lists);
+    const int     b = static_cast<int>(u.div), list = u.rem;
     const int     tid = static_cast<int>(threadIdx.x);
     const int     lane = tid & 63, wave = tid >> 6;
     const float*  w = a.scores + wg * a.stride;
     int32_t*      out = a.blocks + wg * a.count;
+    const int     n = visible_pages(a, b, list);
     if (n <= a.count)
     {
         for (int i = tid; i < a.count; i += THREADS) out[i] = i < n ? i : -1;
@@ -220,36 +477,55 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
     const int lo = a.sinks, hi = n - a.recent;  // the pages between: more than are taken of them
     const int most = a.count - a.sinks - a.recent;
     uint32_t  x[PER];
-    auto load = [&](int t0)
+    auto load = [&](int t0)  // (rows of scores are whole 16-byte words; past the last page they hold anything)
     {
+        const int i0 = t0 + tid * PER;
 #pragma unroll
-        for (int k = 0; k < PER; ++k)
+        for (int k = 0; k < PER; k += 4)
         {
-            const int i = t0 + k * THREADS + tid;
-            x[k] = i < n ? score_key(w[i]) : 0u;
+            f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (i0 + k < n) v = *reinterpret_cast<const f32x4*>(w + i0 + k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[k + j] = score_key(v[j]);
         }
     };
+    auto between = [&](int t0, int k) { return t0 + tid * PER + k >= lo && t0 + tid * PER + k < hi; };
     const bool one = n <= TILE;
     if (one) load(0);
     uint32_t key = 0;
     int      need = most;
     if (most > 0)
-        for (int pass = 0; pass < 3; ++pass)
+    {
+        // the keys' range
+        uint32_t least = 0xffffffffu, largest = 0u;
+        for (int t0 = 0; t0 < n; t0 += TILE)
         {
-            const int      shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-            const uint32_t bins = pass == 2 ? 1024u : 2048u;
-            const uint32_t above = pass == 0 ? 0u : ~uint32_t{0} << (pass == 1 ? 21 : 10);  // bits found so far
-            for (int i = tid; i < BINS; i += THREADS) s_hist[i] = 0;
-            __syncthreads();
+            if (!one) load(t0);
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (between(t0, k)) least = min(least, x[k]), largest = max(largest, x[k]);
+        }
+        largest = wave_max(largest);
+        least = ~wave_max(~least);
+        if (lane == 0) s_ends[0][wave] = least, s_ends[1][wave] = largest;
+        for (int i = tid; i < BINS; i += THREADS) s_hist[i] = 0;
+        if (tid == 0) s_left = 0;
+        __syncthreads();
+        const int e = lane < WAVES ? lane : 0;
+        least = ~wave_max(~s_ends[0][e]);
+        largest = wave_max(s_ends[1][e]);
+        for (;;)
+        {
+            // bins of 2^shift keys from `least` on
+            const uint32_t range = largest - least;
+            const int      bits = range == 0 ? 0 : 32 - __builtin_clz(range);
+            const int      shift = bits > 11 ? bits - 11 : 0;
             for (int t0 = 0; t0 < n; t0 += TILE)
             {
                 if (!one) load(t0);
 #pragma unroll
                 for (int k = 0; k < PER; ++k)
-                {
-                    const int i = t0 + k * THREADS + tid;
-                    if (i >= lo && i < hi && (x[k] & above) == key) atomicAdd(&s_hist[(x[k] >> shift) & (bins - 1)], 1);
-                }
+                    if (between(t0, k) && x[k] >= least && x[k] <= largest) atomicAdd(&s_hist[(x[k] - least) >> shift], 1);
             }
             __syncthreads();
             const int top = BINS - 1 - BPT * tid;  // this thread's bins: top, top - 1, ..
@@ -260,23 +536,64 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
             if (lane == 63) s_tot[wave] = incl;
             __syncthreads();
             const int tot = lane < WAVES ? s_tot[lane] : 0;
-            int       before = incl - sum + __shfl(wave_scan(tot) - tot, wave, 64);
+            int       before = incl - sum + __builtin_amdgcn_readlane(wave_scan(tot) - tot, uniform(wave));
 #pragma unroll
             for (int j = 0; j < BPT; ++j)
             {
                 if (before < need && need <= before + c[j])
                 {
-                    s_found[0] = top - j;
-                    s_found[1] = need - before;
+                    s_found[0] = static_cast<uint32_t>(top - j);
+                    s_found[1] = static_cast<uint32_t>(need - before);
+                    s_found[2] = static_cast<uint32_t>(c[j]);
                 }
                 before += c[j];
             }
+            for (int i = tid; i < BINS; i += THREADS) s_hist[i] = 0;
             __syncthreads();
-            key |= static_cast<uint32_t>(s_found[0]) << shift;
-            need = s_found[1];
+            least += s_found[0] << shift;
+            largest = min(largest - least, (1u << shift) - 1u) + least;  // (the range may end inside its last bin)
+            need = static_cast<int>(s_found[1]);
+            const int held = static_cast<int>(s_found[2]);
+            if (held <= kChooseMost || shift == 0) break;
             __syncthreads();
         }
+        if (least == largest)
+            key = least;
+        else
+        {
+            for (int t0 = 0; t0 < n; t0 += TILE)
+            {
+                if (!one) load(t0);
+#pragma unroll
+                for (int k = 0; k < PER; ++k)
+                    if (between(t0, k) && x[k] >= least && x[k] <= largest) s_keys[atomicAdd(&s_left, 1)] = x[k];
+            }
+            const int held = static_cast<int>(s_found[2]);
+            __syncthreads();
+            if (tid < held)
+            {
+                const uint32_t mine = s_keys[tid];
+                int            above = 0, equal = 0;
+                for (int j = 0; j < held; ++j)
+                {
+                    above += s_keys[j] > mine;
+                    equal += s_keys[j] == mine;
+                }
+                if (above < need && need <= above + equal)  // (every one of the equal ones writes the same)
+                {
+                    s_found[0] = mine;
+                    s_found[1] = static_cast<uint32_t>(need - above);
+                }
+            }
+            __syncthreads();
+            key = s_found[0];
+            need = static_cast<int>(s_found[1]);
+        }
+        __syncthreads();  // s_tot is read
+    }
 
+    // The pages that stay, in order: a thread's place is the number of pages before its own that stay for sure, and of those
+    // equal to the key the first `need`.
     int base_sure = 0, base_equal = 0;
     for (int t0 = 0; t0 < n; t0 += TILE)
     {
@@ -285,35 +602,30 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
 #pragma unroll
         for (int k = 0; k < PER; ++k)
         {
-            const int  i = t0 + k * THREADS + tid;
-            const bool ends = i < lo || (i >= hi && i < n);
-            const bool between = i >= lo && i < hi && most > 0;
-            const bool s = ends || (between && x[k] > key), e = between && x[k] == key;
-            sure |= static_cast<uint32_t>(s) << k;
-            equal |= static_cast<uint32_t>(e) << k;
-            const uint64_t bs = __ballot(s), be = __ballot(e);
-            if (lane == 0) s_cnt[0][k * WAVES + wave] = __popcll(bs), s_cnt[1][k * WAVES + wave] = __popcll(be);
+            const int  i = t0 + tid * PER + k;
+            const bool mid = between(t0, k) && most > 0;
+            sure |= static_cast<uint32_t>(i < lo || (i >= hi && i < n) || (mid && x[k] > key)) << k;
+            equal |= static_cast<uint32_t>(mid && x[k] == key) << k;
         }
+        const int mine = __popc(sure) | (__popc(equal) << 16);
+        const int incl = wave_scan(mine);
+        if (lane == 63) s_tot[wave] = incl;
         __syncthreads();
-        int cs = base_sure, ce = base_equal;
+        const int tot = lane < WAVES ? s_tot[lane] : 0;
+        const int upto = wave_scan(tot);
+        const int before = incl - mine + __builtin_amdgcn_readlane(upto - tot, uniform(wave));
+        const int all = __builtin_amdgcn_readlane(upto, 63);
+        int       es = base_equal + (before >> 16);
+        int       at = base_sure + (before & 0xffff);
 #pragma unroll
         for (int k = 0; k < PER; ++k)
         {
-            // counts of the stretches of 64 pages before this one, of this k and the k before
-            int ps = cs, pe = ce;
-            for (int v = 0; v < WAVES; ++v)
-            {
-                const int ns = s_cnt[0][k * WAVES + v], ne = s_cnt[1][k * WAVES + v];
-                if (v < wave) ps += ns, pe += ne;
-                cs += ns, ce += ne;
-            }
-            const bool     s = sure >> k & 1, e = equal >> k & 1;
-            const uint64_t bs = __ballot(s), be = __ballot(e);
-            const uint64_t below = (uint64_t{1} << lane) - 1;
-            const int      es = pe + __popcll(be & below);
-            if (s || (e && es < need)) out[ps + __popcll(bs & below) + min(es, need)] = t0 + k * THREADS + tid;
+            const bool s = sure >> k & 1, q = equal >> k & 1;
+            if (s || (q && es < need)) out[at + min(es, need)] = t0 + tid * PER + k;
+            at += s;
+            es += q;
         }
-        base_sure = cs, base_equal = ce;
+        base_sure += all & 0xffff, base_equal += all >> 16;
         __syncthreads();
     }
 }
@@ -321,28 +633,53 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
 namespace
 {
 
+template <int BT, int QT, int LPP, bool FULL>
+hipError_t launch_scores_l(const SelectArgs& a, hipStream_t stream)
+{
+    constexpr int ROUND = kScoreThreads / LPP * kScorePages;
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.num_kv_heads;
+    const int64_t all = (a.most_pages + ROUND - 1) / ROUND;  // rounds of a row
+    if (!select_by_lists(a.seq_len, a.lists, a.group))
+    {
+        const void*   kernel = reinterpret_cast<const void*>(block_scores_step<BT, QT, LPP, FULL>);
+        const int64_t wgs = std::min<int64_t>(decode_mfma_items(kernel, kScoreThreads, 1), rows * all);
+        hipLaunchKernelGGL((block_scores_step<BT, QT, LPP, FULL>), dim3(static_cast<unsigned>(wgs)), dim3(kScoreThreads), 0,
+                           stream, a);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((block_queries<QT, LPP>), dim3(static_cast<unsigned>(rows * a.lists)), dim3(kSumThreads), 0, stream, a);
+    // blocks of queries that a workgroup goes through: as many as leave two workgroups per CU
+    const int64_t per = std::max<int64_t>(1, std::min<int64_t>(a.lists, (rows * all * a.lists + 511) / 512));
+    const int64_t parts = (a.lists + per - 1) / per;
+    if (rows * parts * all > INT32_MAX) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((block_scores_lists<BT, LPP, FULL>), dim3(static_cast<unsigned>(rows * parts * all)), dim3(kScoreThreads), 0,
+                       stream, a, static_cast<int>(all), static_cast<int>(per), static_cast<int>(parts));
+    return hipGetLastError();
+}
+
+template <int BT, int QT>
+hipError_t launch_scores_q(const SelectArgs& a, hipStream_t stream)
+{
+    // lanes that hold a page's bounds
+    if (a.head_dim == 64) return launch_scores_l<BT, QT, 8, true>(a, stream);
+    if (a.head_dim < 64) return launch_scores_l<BT, QT, 8, false>(a, stream);
+    if (a.head_dim < 128) return launch_scores_l<BT, QT, 16, false>(a, stream);
+    if (a.head_dim == 128) return launch_scores_l<BT, QT, 16, true>(a, stream);
+    return launch_scores_l<BT, QT, 32, true>(a, stream);
+}
+
 template <int BT>
 hipError_t launch_scores(const SelectArgs& a, hipStream_t stream)
 {
-    const int64_t lists = static_cast<int64_t>(a.batch) * a.lists * a.num_kv_heads;
-    auto go = [&]<int LPP>()
-    {
-        constexpr int ROUND = kScoreThreads / LPP * kScoreUnroll;
-        // a workgroup's tile: as many rounds as leave 2048 workgroups
-        int64_t rounds = (a.most_pages + ROUND - 1) / ROUND;
-        const int64_t per = std::max<int64_t>(1, std::min<int64_t>(rounds, lists * rounds / 2048));
-        const int64_t tiles = (rounds + per - 1) / per;
-        if (lists * tiles > INT32_MAX) return hipErrorInvalidConfiguration;
-        hipLaunchKernelGGL((block_scores<BT, LPP>), dim3(static_cast<unsigned>(lists * tiles)), dim3(kScoreThreads), 0, stream, a,
-                           static_cast<int>(per * ROUND), static_cast<int>(tiles));
-        return hipGetLastError();
-    };
-    if (a.head_dim <= 64) return go.template operator()<8>();
-    if (a.head_dim <= 128) return go.template operator()<16>();
-    return go.template operator()<32>();
+    if (a.q_dtype == F32) return launch_scores_q<BT, F32>(a, stream);
+    if (a.q_dtype == F16) return launch_scores_q<BT, F16>(a, stream);
+    return launch_scores_q<BT, BF16>(a, stream);
 }
 
 }  // namespace
+
+// A step sums its few query rows in the workgroups that score; several blocks of queries, or a long one, are summed once.
+bool select_by_lists(int seq_len, int lists, int group) { return lists > 1 || static_cast<int64_t>(seq_len) * group > 32; }
 
 hipError_t launch_select(const SelectArgs& a, hipStream_t stream)
 {
@@ -358,6 +695,8 @@ hipError_t launch_select(const SelectArgs& a, hipStream_t stream)
     const dim3 grid(static_cast<unsigned>(lists));
     if (a.most_pages <= 1024)
         hipLaunchKernelGGL((block_choose<256, 4>), grid, dim3(256), 0, stream, a);
+    else if (a.most_pages <= 4096)
+        hipLaunchKernelGGL((block_choose<512, 8>), grid, dim3(512), 0, stream, a);
     else
         hipLaunchKernelGGL((block_choose<1024, 8>), grid, dim3(1024), 0, stream, a);
     return hipGetLastError();

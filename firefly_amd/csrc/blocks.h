@@ -63,6 +63,7 @@ struct SelectArgs
     const int32_t* context_lens;
     int32_t*       blocks;  // [batch, lists, num_kv_heads, count]
     float*         scores;  // workspace [batch, lists, num_kv_heads, stride]
+    double*        query_sums;  // workspace [batch, lists, num_kv_heads, 2, head_dim] (select_by_lists)
     int64_t        stride;
     int            q_dtype;
     int            bounds_dtype;
@@ -112,6 +113,18 @@ struct BlocksArgs
     float*         ws_acc;  // [batch * seq_len * num_heads, splits, head_dim]: unnormalised output
 };
 
+// i / n and i % n, in 32 bits: a workgroup's index is one (an int64 division is a hundred instructions and a branch).
+struct Split
+{
+    uint32_t div;
+    int      rem;
+};
+__device__ __forceinline__ Split split_index(uint32_t i, int n)
+{
+    const uint32_t d = i / static_cast<uint32_t>(n);
+    return Split{d, static_cast<int>(i - d * static_cast<uint32_t>(n))};
+}
+
 // Which kernel attends: the decode's on the matrix cores (a list per token), the prefill's (a list per block of tokens), or
 // the vector kernel (fp32 caches, other head dims).
 enum class BlocksKernel
@@ -125,6 +138,7 @@ int          blocks_splits(const BlocksArgs& a);  // sizes and types of `a` set
 
 hipError_t launch_rope_axes(const RopeAxesArgs& a, hipStream_t stream);
 hipError_t launch_key_bounds(const KeyBoundsArgs& a, hipStream_t stream);
+bool       select_by_lists(int seq_len, int lists, int group);  // whether the choice takes query_sums
 hipError_t launch_select(const SelectArgs& a, hipStream_t stream);
 hipError_t launch_blocks(const BlocksArgs& a, hipStream_t stream);
 hipError_t launch_blocks_decode(const BlocksArgs& a, hipStream_t stream);

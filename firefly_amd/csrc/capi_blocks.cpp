@@ -73,6 +73,8 @@ int rope_axes(ffkv::RopeAxesArgs a, const int* sections, int axes, int interleav
                     "num_blocks %d)", a.batch, a.seq_len, a.num_heads, a.num_kv_heads, a.max_blocks, a.num_blocks);
     if (a.num_heads > 65535 || a.num_kv_heads > 65535)
         return fail(FFKV_ERR_UNSUPPORTED, "num_heads and num_kv_heads must be <= 65535");
+    if (static_cast<int64_t>(a.batch) * a.seq_len > INT32_MAX / 4)
+        return fail(FFKV_ERR_UNSUPPORTED, "batch * seq_len must be <= 2^29 - 1");
     if (!(rope_theta > 0.0f) || std::isinf(rope_theta))
         return fail(FFKV_ERR_INVALID_ARGUMENT, "rope_theta must be positive and finite, got %g", static_cast<double>(rope_theta));
     if (const int rc = set_sections(a, sections, axes, interleaved)) return rc;
@@ -117,13 +119,25 @@ int most_pages(int max_blocks, int max_context_len)
 
 constexpr double kMostBytes = 1e15;
 
-// Bytes of a choice's scores: one per block of queries, KV head and page; -1 where they are beyond all memory.
-int64_t score_bytes(int batch, int lists, int num_kv_heads, int pages, int count)
+// A choice's workspace: the scores, one per block of queries, KV head and page, and the queries' sums.
+struct SelectLayout
 {
-    if (pages <= count) return 0;  // nothing is left out
-    const double bytes = 4.0 * batch * lists * num_kv_heads * (static_cast<double>(pages) + 64);
-    if (bytes > kMostBytes) return -1;
-    return static_cast<int64_t>(batch) * lists * num_kv_heads * pages * 4;
+    int64_t stride, sums, total;  // total -1: beyond all memory
+};
+
+SelectLayout select_layout(int batch, int seq_len, int num_heads, int num_kv_heads, int head_dim, int pages, int count,
+                           int query_block)
+{
+    if (pages <= count) return SelectLayout{};  // nothing is left out
+    const int     lists = lists_of(seq_len, query_block);
+    const double  each = 4.0 * pages + 16.0 * head_dim + 256.0;
+    if (each * batch * lists * num_kv_heads > kMostBytes) return SelectLayout{0, 0, -1};
+    const int64_t all = static_cast<int64_t>(batch) * lists * num_kv_heads;
+    SelectLayout  l{};
+    l.stride = ceil_div(pages, 4) * 4;  // whole 16-byte words
+    l.sums = align256(all * l.stride * 4);
+    l.total = l.sums + (ffkv::select_by_lists(seq_len, lists, num_heads / num_kv_heads) ? all * head_dim * 16 : 0);
+    return l;
 }
 
 // What the pieces of the lists take in the workspace.
@@ -244,11 +258,15 @@ int ffkv_key_bounds(const void* k_cache, int cache_dtype, const float* k_scale, 
     return e == hipSuccess ? ok() : hip_fail(e, "key bounds launch");
 }
 
-size_t ffkv_select_blocks_workspace_bytes(int batch, int seq_len, int num_kv_heads, int count, int query_block, int max_blocks,
-                                          int max_context_len)
+size_t ffkv_select_blocks_workspace_bytes(int batch, int seq_len, int num_heads, int num_kv_heads, int head_dim, int count,
+                                          int query_block, int max_blocks, int max_context_len)
 {
-    if (batch <= 0 || seq_len <= 0 || num_kv_heads <= 0 || count <= 0 || query_block <= 0 || max_blocks <= 0) return 0;
-    const int64_t n = score_bytes(batch, lists_of(seq_len, query_block), num_kv_heads, most_pages(max_blocks, max_context_len), count);
+    // sizes that ffkv_select_blocks refuses need nothing
+    if (batch <= 0 || batch > 65535 || seq_len <= 0 || num_heads <= 0 || num_heads > 65535 || num_kv_heads <= 0 ||
+        num_heads % num_kv_heads != 0 || !head_dim_ok(head_dim) || count <= 0 || query_block <= 0 || max_blocks <= 0)
+        return 0;
+    const int64_t n = select_layout(batch, seq_len, num_heads, num_kv_heads, head_dim, most_pages(max_blocks, max_context_len),
+                                    count, query_block).total;
     return n > 0 ? static_cast<size_t>(n) : 0;
 }
 
@@ -269,6 +287,7 @@ int ffkv_select_blocks(const void* q, int q_dtype, const void* bounds, int bound
         return fail(FFKV_ERR_INVALID_ARGUMENT, "num_heads %d is not a multiple of num_kv_heads %d", num_heads, num_kv_heads);
     if (batch > 65535 || num_heads > 65535) return fail(FFKV_ERR_UNSUPPORTED, "batch and num_heads must be <= 65535");
     if (query_block < 1) return fail(FFKV_ERR_INVALID_ARGUMENT, "query_block must be at least 1, got %d", query_block);
+    if (num_blocks < 1 && batch > 0) return fail(FFKV_ERR_INVALID_ARGUMENT, "bounds of no page");
     if (count < 1 || sinks < 0 || recent < 0 || static_cast<int64_t>(sinks) + recent > count)
         return fail(FFKV_ERR_INVALID_ARGUMENT, "count %d must be at least 1 and hold sinks %d and recent %d", count, sinks, recent);
     if (batch == 0 || seq_len == 0) return ok();
@@ -280,7 +299,8 @@ int ffkv_select_blocks(const void* q, int q_dtype, const void* bounds, int bound
     const int     lists = lists_of(seq_len, query_block);
     const int     group = num_heads / num_kv_heads;
     const int     pages = most_pages(max_blocks, max_context_len);
-    const int64_t need = score_bytes(batch, lists, num_kv_heads, pages, count);
+    const SelectLayout lay = select_layout(batch, seq_len, num_heads, num_kv_heads, head_dim, pages, count, query_block);
+    const int64_t need = lay.total;
     if (static_cast<int64_t>(batch) * lists * num_kv_heads > INT32_MAX)
         return fail(FFKV_ERR_UNSUPPORTED, "batch * blocks of queries * num_kv_heads too large");
     if (static_cast<int64_t>(std::min(query_block, seq_len)) * group > INT32_MAX / 2)
@@ -308,7 +328,8 @@ int ffkv_select_blocks(const void* q, int q_dtype, const void* bounds, int bound
     a.context_lens = context_lens;
     a.blocks = blocks;
     a.scores = static_cast<float*>(ws);
-    a.stride = pages;
+    a.query_sums = need > 0 ? reinterpret_cast<double*>(static_cast<char*>(ws) + lay.sums) : nullptr;
+    a.stride = lay.stride;
     a.q_dtype = q_dtype;
     a.bounds_dtype = bounds_dtype;
     a.batch = batch;

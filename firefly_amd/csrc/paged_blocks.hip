@@ -103,17 +103,14 @@ void paged_blocks_decode(BlocksArgs a)
     const int g = lane >> 4;
     const int G = a.group;
     const int HB = (G + 15) >> 4;
-    const int y = a.num_kv_heads * HB;
-    int64_t   id = blockIdx.x;
-    const int split = static_cast<int>(id % a.splits);
-    id /= a.splits;
-    const int     vh = static_cast<int>(id % y);
-    const int64_t row = id / y;  // b * seq_len + t
-    const int     b = static_cast<int>(row / a.seq_len);
+    const Split u = split_index(blockIdx.x, a.splits), v = split_index(u.div, a.num_kv_heads * HB);
+    const Split w = split_index(v.div, a.seq_len);
+    const int     split = u.rem, vh = v.rem, b = static_cast<int>(w.div);
+    const int64_t row = v.div;  // b * seq_len + t
     const int     kvh = vh / HB;
     const int     h0 = (vh - kvh * HB) * 16;
     const int     gc = min(16, G - h0);
-    const int64_t pos = static_cast<int64_t>(a.context_lens[b]) + (row - static_cast<int64_t>(b) * a.seq_len);
+    const int64_t pos = static_cast<int64_t>(a.context_lens[b]) + w.rem;
     const int32_t* list = a.blocks + (row * a.num_kv_heads + kvh) * a.count;
     const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
     // this wave's entries: begin + kBlocksWaves i, i < n
@@ -468,14 +465,10 @@ __global__ __launch_bounds__(64 * kBlocksWaves) void paged_blocks_vector(BlocksA
     const bool in = 8 * c < D;
     const int G = a.group;
     const int HB = (G + HC - 1) / HC;
-    const int y = a.num_kv_heads * HB;
-    int64_t   id = blockIdx.x;
-    const int split = static_cast<int>(id % a.splits);
-    id /= a.splits;
-    const int     vh = static_cast<int>(id % y);
-    const int64_t row = id / y;
-    const int     b = static_cast<int>(row / a.seq_len);
-    const int     t = static_cast<int>(row - static_cast<int64_t>(b) * a.seq_len);
+    const Split u = split_index(blockIdx.x, a.splits), v = split_index(u.div, a.num_kv_heads * HB);
+    const Split w = split_index(v.div, a.seq_len);
+    const int     split = u.rem, vh = v.rem, b = static_cast<int>(w.div), t = w.rem;
+    const int64_t row = v.div;  // b * seq_len + t
     const int     kvh = vh / HB;
     const int     h0 = (vh - kvh * HB) * HC;
     const int     gc = min(HC, G - h0);
@@ -604,11 +597,11 @@ namespace
 
 bool mfma_dim(int d) { return d == 64 || d == 96 || d == 128 || d == 256; }
 
-// Workgroups of an unsplit call.
-int64_t blocks_workgroups(const BlocksArgs& a)
+// Workgroups of a token in an unsplit call: KV heads, and blocks of their query heads.
+int64_t blocks_heads(const BlocksArgs& a)
 {
     const int heads = blocks_kernel(a) == BlocksKernel::kDecode ? 16 : 4;
-    return static_cast<int64_t>(a.batch) * a.seq_len * a.num_kv_heads * ((a.group + heads - 1) / heads);
+    return static_cast<int64_t>(a.num_kv_heads) * ((a.group + heads - 1) / heads);
 }
 
 template <int QT, typename F>
@@ -649,7 +642,7 @@ BlocksKernel blocks_kernel(const BlocksArgs& a)
 int blocks_splits(const BlocksArgs& a)
 {
     if (blocks_kernel(a) == BlocksKernel::kPrefill) return 1;
-    const int64_t wgs = blocks_workgroups(a);
+    const int64_t wgs = static_cast<int64_t>(a.batch) * a.seq_len * blocks_heads(a);
     const int64_t most = a.count / (2 * kBlocksWaves);  // pieces of two pages per wave
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(wgs, 1), most)));
 }
@@ -694,7 +687,7 @@ hipError_t launch_blocks(const BlocksArgs& a, hipStream_t stream)
 {
     const BlocksKernel kernel = blocks_kernel(a);
     if (kernel == BlocksKernel::kPrefill) return launch_blocks_prefill(a, stream);
-    const int64_t wgs = blocks_workgroups(a) * a.splits;
+    const int64_t wgs = static_cast<int64_t>(a.batch) * a.seq_len * blocks_heads(a) * a.splits;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.seq_len * a.num_heads;
     if (wgs > INT32_MAX || rows > INT32_MAX) return hipErrorInvalidConfiguration;
     const dim3 grid(static_cast<unsigned>(wgs)), block(64 * kBlocksWaves);

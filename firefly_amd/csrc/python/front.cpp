@@ -918,7 +918,7 @@ PyObject* select_blocks(PyObject*, PyObject* const* a, Py_ssize_t n)
     void *qp = r.ptr(q), *bo = r.ptr(a[1]);
     auto *tab = r.ptr<int32_t>(a[2]), *cx = r.ptr<int32_t>(a[3]), *out = r.ptr<int32_t>(a[8]);
     void*         s = r.stream(a[12]);
-    const size_t  need = r.ok && a[10] == Py_None ? fn.select_bytes(B, S, Hkv, keep, T, mb, mcl) : 0;
+    const size_t  need = r.ok && a[10] == Py_None ? fn.select_bytes(B, S, Hq, Hkv, D, keep, T, mb, mcl) : 0;
     const Scratch ws(r, a[10], a[13], need, q, a[12]);
     return finish(r, [&] {
         return fn.select_blocks(qp, qt, bo, bt, tab, cx, out, keep, sinks, recent, T, B, S, Hq, Hkv, D, FFKV_BLOCK_SIZE, mb, N,

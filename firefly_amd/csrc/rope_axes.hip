@@ -79,11 +79,11 @@ __global__ __launch_bounds__(kRopeThreads) void rope_axes_kernel(RopeAxesArgs a,
 
     const int     tid = static_cast<int>(threadIdx.x);
     const int     lane = tid & 63;
-    const int     wave = tid >> 6;
+    const int     wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int     col = lane % LPR;
     const int     sub = lane / LPR;
     const int     rows = a.num_heads + a.num_kv_heads;
-    const int64_t items = static_cast<int64_t>(a.batch) * a.seq_len * parts;
+    const uint32_t items = static_cast<uint32_t>(a.batch) * a.seq_len * parts;
     float*        s_cos = s_cs[wave][0];
     float*        s_sin = s_cs[wave][1];
 
@@ -103,13 +103,12 @@ __global__ __launch_bounds__(kRopeThreads) void rope_axes_kernel(RopeAxesArgs a,
             axis[p] = (i >= a.section_end[0]) + (i >= a.section_end[1]) + (i >= a.section_end[2]);
     }
 
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (kRopeThreads / 64);
-    for (int64_t item = static_cast<int64_t>(blockIdx.x) * (kRopeThreads / 64) + wave; item < items; item += step)
+    for (uint32_t item = blockIdx.x * (kRopeThreads / 64) + wave; item < items; item += gridDim.x * (kRopeThreads / 64))
     {
-        const int64_t tok = item / parts;
-        const int     part = static_cast<int>(item - tok * parts);
-        const int     b = static_cast<int>(tok / a.seq_len);
-        const int     t = static_cast<int>(tok - static_cast<int64_t>(b) * a.seq_len);
+        // (a token's parts lie side by side: apart, its rows' lines are fetched twice, 64 -> 69 us for 12000 tokens)
+        const Split    v = split_index(item, parts), u = split_index(v.div, a.seq_len);
+        const uint32_t tok = v.div;
+        const int      part = v.rem, b = static_cast<int>(u.div), t = u.rem;
         int           at[PPL];
 #pragma unroll
         for (int p = 0; p < PPL; ++p)
@@ -257,6 +256,7 @@ hipError_t launch_axes_d(const RopeAxesArgs& a, hipStream_t stream)
     {
         const int     parts = (passes + PASS - 1) / PASS;
         const int64_t wgs = (tokens * parts + kRopeThreads / 64 - 1) / (kRopeThreads / 64);
+        if (tokens * parts > INT32_MAX) return hipErrorInvalidConfiguration;
         hipLaunchKernelGGL((rope_axes_kernel<SRC, CACHE, D, APPEND, PASS>),
                            dim3(static_cast<unsigned>(std::min<int64_t>(wgs, 16384))), dim3(kRopeThreads), 0, stream, a, parts);
         return hipGetLastError();

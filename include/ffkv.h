@@ -456,8 +456,8 @@ FFKV_API int ffkv_key_bounds(const void* k_cache, int cache_dtype, const float* 
  * tokens, this call's included (0: the table's width); pages past it are not taken.  workspace: NULL or
  * ffkv_select_blocks_workspace_bytes (a captured call needs one where that is not 0).
  */
-FFKV_API size_t ffkv_select_blocks_workspace_bytes(int batch, int seq_len, int num_kv_heads, int count, int query_block,
-                                                   int max_blocks, int max_context_len);
+FFKV_API size_t ffkv_select_blocks_workspace_bytes(int batch, int seq_len, int num_heads, int num_kv_heads, int head_dim,
+                                                   int count, int query_block, int max_blocks, int max_context_len);
 
 FFKV_API int ffkv_select_blocks(const void* q, int q_dtype, const void* bounds, int bounds_dtype, const int32_t* block_table,
                                 const int32_t* context_lens, int32_t* blocks, int count, int sinks, int recent,

@@ -128,10 +128,12 @@ def test_empty_is_ok(ff):
 
 def test_workspace_bytes(ff):
     f = ff.lib.ffkv_select_blocks_workspace_bytes
-    assert f(2, 100, 4, 8, 32, 50, 0) == 2 * 4 * 4 * 50 * 4
-    assert f(2, 100, 4, 8, 32, 50, 300) == 2 * 4 * 4 * 19 * 4
-    assert f(2, 100, 4, 50, 32, 50, 0) == 0 and f(2, 100, 4, 19, 32, 50, 300) == 0
-    assert f(0, 1, 1, 1, 1, 9, 0) == 0 and f(1, 1, 1, 0, 1, 9, 0) == 0 and f(1, 1, 1, 1, 0, 9, 0) == 0
+    lists = 2 * 4 * 4
+    assert f(2, 100, 8, 4, 64, 8, 32, 50, 0) == lists * (52 * 4 + 64 * 16)
+    assert f(2, 100, 8, 4, 64, 8, 32, 50, 300) == lists * (20 * 4 + 64 * 16)
+    assert f(2, 1, 8, 4, 64, 8, 1, 64, 0) == 8 * 64 * 4  # a step's queries are summed where they are used
+    assert f(2, 100, 8, 4, 64, 50, 32, 50, 0) == 0 and f(2, 100, 8, 4, 64, 19, 32, 50, 300) == 0
+    assert f(0, 1, 1, 1, 64, 1, 1, 9, 0) == 0 and f(1, 1, 1, 1, 64, 0, 1, 9, 0) == 0 and f(1, 1, 1, 1, 64, 1, 0, 9, 0) == 0
     g = ff.lib.ffkv_paged_attention_blocks_workspace_bytes
     assert g(ff.DTYPE_BF16, 64, 1, 32, 8, 128, 64, 1) == 0  # enough lists for the chip
     assert g(ff.DTYPE_BF16, 1, 1, 32, 8, 128, 256, 1) > 0

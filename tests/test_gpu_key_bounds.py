@@ -150,7 +150,7 @@ def test_capture(ff, gpu):
     box = boxes(rng, c.num_blocks, 2, 128, torch.bfloat16, gpu)
     q = torch.randn(4, 1, 8, 128, device=gpu).bfloat16()
     _, _, bt, cx = tensors(c, gpu)
-    ws = ff.select_blocks_workspace(4, 1, 2, 64, 1, c.max_blocks)
+    ws = ff.select_blocks_workspace(4, 1, 8, 2, 128, 64, 1, c.max_blocks)
     out = torch.empty(4, 1, 2, 64, dtype=torch.int32, device=gpu)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
