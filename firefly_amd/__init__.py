@@ -129,7 +129,7 @@ def _load() -> ctypes.CDLL:
     lib.ffkv_select_blocks.restype = i32
     lib.ffkv_select_blocks.argtypes = [vp, i32, vp, i32, vp, vp, vp, *[i32] * 13, vp, sz, vp]
     lib.ffkv_paged_attention_blocks_workspace_bytes.restype = sz
-    lib.ffkv_paged_attention_blocks_workspace_bytes.argtypes = [i32] * 8
+    lib.ffkv_paged_attention_blocks_workspace_bytes.argtypes = [i32] * 9
     lib.ffkv_paged_attention_blocks.restype = i32
     lib.ffkv_paged_attention_blocks.argtypes = [vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, vp, *[i32] * 10, f32, vp, sz, vp]
     lib.ffkv_last_error.restype = ctypes.c_char_p
@@ -530,13 +530,13 @@ def select_blocks(q, bounds, block_table, context_lens, count: int, sinks: int =
     return blocks
 
 
-def attention_blocks_workspace(cache_dtype: int, batch: int, seq_len: int, num_heads: int, num_kv_heads: int, head_dim: int,
-                               count: int, query_block: int = 1, device=None):
+def attention_blocks_workspace(q_dtype: int, cache_dtype: int, batch: int, seq_len: int, num_heads: int, num_kv_heads: int,
+                               head_dim: int, count: int, query_block: int = 1, device=None):
     """A workspace for ``paged_attention_blocks`` (``ffkv_paged_attention_blocks_workspace_bytes``)."""
     import torch
 
-    n = int(lib.ffkv_paged_attention_blocks_workspace_bytes(cache_dtype, batch, seq_len, num_heads, num_kv_heads, head_dim, count,
-                                                            query_block))
+    n = int(lib.ffkv_paged_attention_blocks_workspace_bytes(q_dtype, cache_dtype, batch, seq_len, num_heads, num_kv_heads,
+                                                            head_dim, count, query_block))
     return torch.empty(max(n, 256), dtype=torch.uint8, device=device if device is not None else "cuda")
 
 

@@ -468,15 +468,7 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
     const int     lane = tid & 63, wave = tid >> 6;
     const float*  w = a.scores + wg * a.stride;
     int32_t*      out = a.blocks + wg * a.count;
-    const int     n = visible_pages(a, b, list);
-    if (n <= a.count)
-    {
-        for (int i = tid; i < a.count; i += THREADS) out[i] = i < n ? i : -1;
-        return;
-    }
-    const int lo = a.sinks, hi = n - a.recent;  // the pages between: more than are taken of them
-    const int most = a.count - a.sinks - a.recent;
-    uint32_t  x[PER];
+    uint32_t      x[PER];
     auto load = [&](int t0)  // (rows of scores are whole 16-byte words; past the last page they hold anything)
     {
         const int i0 = t0 + tid * PER;
@@ -484,14 +476,22 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
         for (int k = 0; k < PER; k += 4)
         {
             f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (i0 + k < n) v = *reinterpret_cast<const f32x4*>(w + i0 + k);
+            if (i0 + k < a.most_pages) v = *reinterpret_cast<const f32x4*>(w + i0 + k);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[k + j] = score_key(v[j]);
         }
     };
+    if (a.most_pages > a.count) load(0);  // (on their way while the row's length is)
+    const int n = visible_pages(a, b, list);
+    if (n <= a.count)
+    {
+        for (int i = tid; i < a.count; i += THREADS) out[i] = i < n ? i : -1;
+        return;
+    }
+    const int lo = a.sinks, hi = n - a.recent;  // the pages between: more than are taken of them
+    const int most = a.count - a.sinks - a.recent;
     auto between = [&](int t0, int k) { return t0 + tid * PER + k >= lo && t0 + tid * PER + k < hi; };
     const bool one = n <= TILE;
-    if (one) load(0);
     uint32_t key = 0;
     int      need = most;
     if (most > 0)

@@ -108,7 +108,9 @@ struct BlocksArgs
     int            lists;
     int            count;
     int            splits;  // pieces of a list, each by a workgroup of its own
+    int            waves;   // of a workgroup
     float          scale_log2;
+    int32_t*       ws_pieces;  // the prefill's pieces of each block of query rows
     float2*        ws_ml;   // [batch * seq_len * num_heads, splits]: (max in the log2 domain, denominator)
     float*         ws_acc;  // [batch * seq_len * num_heads, splits, head_dim]: unnormalised output
 };
@@ -134,7 +136,12 @@ enum class BlocksKernel
     kVector,
 };
 BlocksKernel blocks_kernel(const BlocksArgs& a);
-int          blocks_splits(const BlocksArgs& a);  // sizes and types of `a` set
+struct BlocksLayout
+{
+    int64_t ml, acc, total;  // byte offsets in the workspace, and its size (0: none)
+};
+BlocksLayout plan_blocks(BlocksArgs& a);
+void         set_blocks_workspace(BlocksArgs& a, const BlocksLayout& l, void* ws);
 
 hipError_t launch_rope_axes(const RopeAxesArgs& a, hipStream_t stream);
 hipError_t launch_key_bounds(const KeyBoundsArgs& a, hipStream_t stream);

@@ -140,22 +140,6 @@ SelectLayout select_layout(int batch, int seq_len, int num_heads, int num_kv_hea
     return l;
 }
 
-// What the pieces of the lists take in the workspace.
-struct PieceLayout
-{
-    int64_t acc, total;
-};
-
-PieceLayout piece_layout(const ffkv::BlocksArgs& a)
-{
-    if (a.splits <= 1) return PieceLayout{};
-    const int64_t parts = static_cast<int64_t>(a.batch) * a.seq_len * a.num_heads * a.splits;
-    PieceLayout   l{};
-    l.acc = align256(parts * 8);
-    l.total = l.acc + parts * a.head_dim * 4;
-    return l;
-}
-
 }  // namespace
 
 extern "C" {
@@ -355,14 +339,15 @@ int ffkv_select_blocks(const void* q, int q_dtype, const void* bounds, int bound
     return e == hipSuccess ? ok() : hip_fail(e, "select blocks launch");
 }
 
-size_t ffkv_paged_attention_blocks_workspace_bytes(int cache_dtype, int batch, int seq_len, int num_heads, int num_kv_heads,
-                                                   int head_dim, int count, int query_block)
+size_t ffkv_paged_attention_blocks_workspace_bytes(int qo_dtype, int cache_dtype, int batch, int seq_len, int num_heads,
+                                                   int num_kv_heads, int head_dim, int count, int query_block)
 {
     // sizes that ffkv_paged_attention_blocks refuses need nothing
-    if (!is_cache(cache_dtype) || !head_dim_ok(head_dim) || batch <= 0 || batch > 65535 || seq_len <= 0 || num_heads <= 0 ||
+    if (!is_act(qo_dtype) || !is_cache(cache_dtype) || !head_dim_ok(head_dim) || batch <= 0 || batch > 65535 || seq_len <= 0 || num_heads <= 0 ||
         num_heads > 65535 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || count <= 0 || query_block <= 0)
         return 0;
     ffkv::BlocksArgs a{};
+    a.qo_dtype = qo_dtype;
     a.cache_dtype = cache_dtype;
     a.batch = batch;
     a.seq_len = seq_len;
@@ -371,9 +356,11 @@ size_t ffkv_paged_attention_blocks_workspace_bytes(int cache_dtype, int batch, i
     a.group = num_heads / num_kv_heads;
     a.head_dim = head_dim;
     a.count = count;
+    a.max_blocks = INT_MAX;
     a.query_block = std::min(query_block, seq_len);  // as the call has it
-    a.splits = ffkv::blocks_splits(a);
-    return static_cast<size_t>(piece_layout(a).total);
+    a.lists = lists_of(seq_len, a.query_block);
+    if (static_cast<int64_t>(batch) * seq_len * num_heads > INT32_MAX) return 0;
+    return static_cast<size_t>(ffkv::plan_blocks(a).total);
 }
 
 int ffkv_paged_attention_blocks(const void* q, void* out, int qo_dtype, const void* k_cache, const void* v_cache,
@@ -431,8 +418,7 @@ int ffkv_paged_attention_blocks(const void* q, void* out, int qo_dtype, const vo
     a.lists = lists_of(seq_len, query_block);
     a.count = count;
     a.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf(static_cast<float>(head_dim))) * kLog2e;
-    a.splits = ffkv::blocks_splits(a);
-    PieceLayout lay = piece_layout(a);
+    const ffkv::BlocksLayout lay = ffkv::plan_blocks(a);
     hipStream_t s = static_cast<hipStream_t>(stream);
     void*       ws = workspace;
     if (ws != nullptr && workspace_bytes < static_cast<size_t>(lay.total))
@@ -443,18 +429,11 @@ int ffkv_paged_attention_blocks(const void* q, void* out, int qo_dtype, const vo
         bool capturing = false;
         if (const int rc = is_capturing(s, capturing)) return rc;
         if (capturing)
-        {
             a.splits = 1;  // whole lists need no workspace
-            lay = PieceLayout{};
-        }
         else if (const int rc = take_memory(&ws, lay.total, s))
             return rc;
     }
-    if (a.splits > 1)
-    {
-        a.ws_ml = static_cast<float2*>(ws);
-        a.ws_acc = reinterpret_cast<float*>(static_cast<char*>(ws) + lay.acc);
-    }
+    if (a.splits > 1) ffkv::set_blocks_workspace(a, lay, ws);
     hipError_t e = ffkv::launch_blocks(a, s);
     if (workspace == nullptr && ws != nullptr)
     {

@@ -271,7 +271,12 @@ hipError_t launch_prefill_merge(const PrefillArgs& a, hipStream_t stream);  // o
 void       prefill_scored_plan(ScoredPrefillArgs& a);
 hipError_t launch_prefill_scored(const ScoredPrefillArgs& a, hipStream_t stream);
 hipError_t launch_prefill_scored_pieces(const ScoredPrefillArgs& a, unsigned wgs, hipStream_t stream);  // its split form's launch
-// The prefill over listed pages (paged_blocks_prefill_*.hip), by the cache's type.
+// The prefill over listed pages (paged_blocks_prefill_*.hip), by the cache's type, its plan, and the merge of its pieces.
+void       plan_blocks_prefill_bf16(ListPrefillArgs& a);
+void       plan_blocks_prefill_f16(ListPrefillArgs& a);
+void       plan_blocks_prefill_i8(ListPrefillArgs& a);
+void       plan_blocks_prefill_fp8(ListPrefillArgs& a);
+hipError_t launch_blocks_prefill_merge(const ListPrefillArgs& a, hipStream_t stream);
 hipError_t launch_blocks_prefill_bf16(const ListPrefillArgs& a, hipStream_t stream);
 hipError_t launch_blocks_prefill_f16(const ListPrefillArgs& a, hipStream_t stream);
 hipError_t launch_blocks_prefill_i8(const ListPrefillArgs& a, hipStream_t stream);

@@ -26,18 +26,18 @@ namespace ffkv
 namespace
 {
 
-constexpr int kBlocksWaves = 4;
+constexpr int kBlocksWaves = 4;  // of the vector kernel
 
-// LDS of a workgroup of up to `heads` query heads: the waves' V tiles, and over them their accumulators and (max,
-// denominator) pairs once all pages are done.
+// LDS of a workgroup of `waves` waves and up to `heads` query heads: the waves' V tiles, and over them their accumulators and
+// (max, denominator) pairs once all pages are done.
 template <int D>
-constexpr int blocks_lds_bytes(int heads)
+constexpr int blocks_lds_bytes(int waves, int heads)
 {
-    const int v = kBlocksWaves * kBlockSize * D * 2;
-    const int state = kBlocksWaves * heads * D * 4 + kBlocksWaves * 16 * 8;
+    const int v = waves * kBlockSize * D * 2;
+    const int state = waves * heads * D * 4 + waves * 16 * 8;
     return v > state ? v : state;
 }
-static_assert(blocks_lds_bytes<256>(16) <= 160 * 1024, "a workgroup's LDS fits a CU");
+static_assert(blocks_lds_bytes<256>(8, 16) <= 160 * 1024, "a workgroup's LDS fits a CU");
 
 // One page in flight.
 template <int NW, int NWV>
@@ -49,11 +49,19 @@ struct ListedPage
     float ks, vs; // int8: K and V scale of token c
 };
 
-// Entry e of a list: the logical page, or -1 where it is none of the row's visible pages.
-__device__ __forceinline__ int listed_page(const BlocksArgs& a, const int32_t* list, int e, int end, int64_t pos)
+// Entry e of a list: the logical page, or -1 where it is none of the table's.  (Whether the query sees it is looked at later:
+// the page's entry in the table need not wait for the row's length.)
+__device__ __forceinline__ int listed_page(const BlocksArgs& a, const int32_t* list, int e, int end)
 {
     const int lp = e < end ? list[e] : -1;
-    return lp >= 0 && lp < a.max_blocks && static_cast<int64_t>(lp) * kBlockSize <= pos ? lp : -1;
+    return lp >= 0 && lp < a.max_blocks ? lp : -1;
+}
+
+// Tokens of logical page lp on physical page phys that the query at pos sees; 0 where it is no page, or past the query.
+__device__ __forceinline__ int listed_tokens(const BlocksArgs& a, int lp, int phys, int64_t pos)
+{
+    const int64_t n = pos + 1 - static_cast<int64_t>(lp) * kBlockSize;
+    return phys < 0 || phys >= a.num_blocks || n <= 0 ? 0 : n < kBlockSize ? static_cast<int>(n) : kBlockSize;
 }
 
 // A state of (max, denominator, accumulator) to the output, or to its piece's place in the workspace.
@@ -71,8 +79,8 @@ __device__ __forceinline__ void store_state4(const BlocksArgs& a, int64_t row_h,
 
 }  // namespace
 
-template <int CT, int QT, int D>
-__global__ __launch_bounds__(64 * kBlocksWaves) __attribute__((amdgpu_waves_per_eu(2, 8)))
+template <int CT, int QT, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 8)))
 void paged_blocks_decode(BlocksArgs a)
 {
     extern __shared__ __align__(16) uint8_t s_blocks[];
@@ -113,10 +121,10 @@ void paged_blocks_decode(BlocksArgs a)
     const int64_t pos = static_cast<int64_t>(a.context_lens[b]) + w.rem;
     const int32_t* list = a.blocks + (row * a.num_kv_heads + kvh) * a.count;
     const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
-    // this wave's entries: begin + kBlocksWaves i, i < n
+    // this wave's entries: begin + WAVES i, i < n
     const int begin = static_cast<int>(static_cast<int64_t>(a.count) * split / a.splits) + wave;
     const int end = static_cast<int>(static_cast<int64_t>(a.count) * (split + 1) / a.splits);
-    const int n = end > begin ? (end - begin + kBlocksWaves - 1) / kBlocksWaves : 0;
+    const int n = end > begin ? (end - begin + WAVES - 1) / WAVES : 0;
     uint16_t* sv = reinterpret_cast<uint16_t*>(s_blocks) + wave * (kBlockSize * D);
 
     float kv_scale_log2 = a.scale_log2;
@@ -134,7 +142,7 @@ void paged_blocks_decode(BlocksArgs a)
     int  tb = 0, lvec, pvec;  // lane l: logical and physical page of entry tb + l
     auto load_entries = [&]()
     {
-        lvec = listed_page(a, list, begin + kBlocksWaves * (tb + lane), end, pos);
+        lvec = listed_page(a, list, begin + WAVES * (tb + lane), end);
         pvec = lvec >= 0 ? table[lvec] : -1;
     };
     load_entries();
@@ -149,10 +157,8 @@ void paged_blocks_decode(BlocksArgs a)
         const int lp = __builtin_amdgcn_readlane(lvec, next - tb);
         const int phys = __builtin_amdgcn_readlane(pvec, next - tb);
         ++next;
-        r.n_tok = phys >= 0 && phys < a.num_blocks
-                      ? static_cast<int>(min(pos + 1 - static_cast<int64_t>(lp) * kBlockSize, static_cast<int64_t>(kBlockSize)))
-                      : 0;
-        if (r.n_tok <= 0) return;
+        r.n_tok = listed_tokens(a, lp, phys, pos);
+        if (r.n_tok == 0) return;
         const size_t row_c = (static_cast<size_t>(phys) * kBlockSize + c) * a.num_kv_heads + kvh;
         if constexpr (CT == I8)
         {
@@ -347,7 +353,7 @@ void paged_blocks_decode(BlocksArgs a)
 
     // the waves' states: accumulators [wave][head][D] over the V tiles, then (max, denominator) [wave][16]
     float*      s_acc = reinterpret_cast<float*>(s_blocks);
-    float2*     s_ml = reinterpret_cast<float2*>(s_acc + kBlocksWaves * gc * D);
+    float2*     s_ml = reinterpret_cast<float2*>(s_acc + WAVES * gc * D);
     const float l_tot = xor_sum(l_run);
     __syncthreads();
     if (c < gc)
@@ -359,16 +365,16 @@ void paged_blocks_decode(BlocksArgs a)
         if (g == 0) s_ml[wave * 16 + c] = float2{m_run, l_tot};
     }
     __syncthreads();
-    for (int k = static_cast<int>(threadIdx.x); k < gc * (D / 4); k += 64 * kBlocksWaves)
+    for (int k = static_cast<int>(threadIdx.x); k < gc * (D / 4); k += 64 * WAVES)
     {
         const int h = k / (D / 4);
         const int d4 = (k - h * (D / 4)) * 4;
         float     Mx = kLowest, L = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kBlocksWaves; ++w) Mx = fmaxf(Mx, s_ml[w * 16 + h].x);
+        for (int w = 0; w < WAVES; ++w) Mx = fmaxf(Mx, s_ml[w * 16 + h].x);
         f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < kBlocksWaves; ++w)
+        for (int w = 0; w < WAVES; ++w)
         {
             const float2 t = s_ml[w * 16 + h];
             const float  x = __builtin_amdgcn_exp2f(t.x - Mx);
@@ -499,14 +505,14 @@ __global__ __launch_bounds__(64 * kBlocksWaves) void paged_blocks_vector(BlocksA
     }
     for (int i0 = begin; i0 < end; i0 += 64 * kBlocksWaves)
     {
-        const int lvec = listed_page(a, list, i0 + kBlocksWaves * lane, end, pos);
+        const int lvec = listed_page(a, list, i0 + kBlocksWaves * lane, end);
         const int pvec = lvec >= 0 ? table[lvec] : -1;
         for (int i = 0; i < 64 && i0 + kBlocksWaves * i < end; ++i)
         {
             const int lp = __builtin_amdgcn_readlane(lvec, i);
             const int phys = __builtin_amdgcn_readlane(pvec, i);
-            if (phys < 0 || phys >= a.num_blocks) continue;
-            const int n_tok = static_cast<int>(min(pos + 1 - static_cast<int64_t>(lp) * kBlockSize, static_cast<int64_t>(kBlockSize)));
+            const int n_tok = listed_tokens(a, lp, phys, pos);
+            if (n_tok == 0) continue;
 #pragma unroll 1
             for (int u0 = 0; u0 < NTOK; u0 += UN)
             {
@@ -639,15 +645,10 @@ BlocksKernel blocks_kernel(const BlocksArgs& a)
     return a.head_dim == 96 ? BlocksKernel::kVector : BlocksKernel::kPrefill;
 }
 
-int blocks_splits(const BlocksArgs& a)
+namespace
 {
-    if (blocks_kernel(a) == BlocksKernel::kPrefill) return 1;
-    const int64_t wgs = static_cast<int64_t>(a.batch) * a.seq_len * blocks_heads(a);
-    const int64_t most = a.count / (2 * kBlocksWaves);  // pieces of two pages per wave
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(wgs, 1), most)));
-}
 
-hipError_t launch_blocks_prefill(const BlocksArgs& a, hipStream_t stream)
+ListPrefillArgs list_prefill_args(const BlocksArgs& a)
 {
     ListPrefillArgs p{};
     p.q = a.q;
@@ -677,6 +678,69 @@ hipError_t launch_blocks_prefill(const BlocksArgs& a, hipStream_t stream)
     p.lists = a.lists;
     p.count = a.count;
     p.query_block = a.query_block;
+    return p;
+}
+
+// The lists as rows of query_block tokens, as the prefill's plan and layout count them.
+ListPrefillArgs list_rows(ListPrefillArgs p)
+{
+    p.batch *= p.lists;
+    p.seq_len = p.query_block;
+    return p;
+}
+
+}  // namespace
+
+// Sets a.splits, and gives the workspace's layout (sizes and types of `a` set).
+BlocksLayout plan_blocks(BlocksArgs& a)
+{
+    BlocksLayout l{};
+    a.splits = 1;
+    a.waves = kBlocksWaves;
+    if (blocks_kernel(a) == BlocksKernel::kPrefill)
+    {
+        if (static_cast<int64_t>(a.batch) * a.lists > INT32_MAX) return l;
+        ListPrefillArgs p = list_rows(list_prefill_args(a));
+        p.count = std::min(a.count, a.max_blocks);  // (pages of a row, but for those listed twice)
+        if (a.cache_dtype == BF16)
+            plan_blocks_prefill_bf16(p);
+        else if (a.cache_dtype == F16)
+            plan_blocks_prefill_f16(p);
+        else if (a.cache_dtype == I8)
+            plan_blocks_prefill_i8(p);
+        else
+            plan_blocks_prefill_fp8(p);
+        a.splits = p.n_split;
+        const PrefillSplitLayout s = prefill_split_layout(p);
+        return BlocksLayout{s.ml, s.acc, s.total};
+    }
+    const int64_t wgs = static_cast<int64_t>(a.batch) * a.seq_len * blocks_heads(a);
+    const int64_t pages = std::min(a.count, a.max_blocks);
+    a.waves = blocks_kernel(a) == BlocksKernel::kDecode && wgs <= 256 ? 8 : 4;
+    const int64_t most = pages < 8 * a.waves ? 1 : pages / (2 * a.waves);
+    a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2048 / a.waves / std::max<int64_t>(wgs, 1), most)));
+    if (a.splits == 1) return l;
+    const int64_t parts = static_cast<int64_t>(a.batch) * a.seq_len * a.num_heads * a.splits;
+    l.acc = (parts * 8 + 255) / 256 * 256;
+    l.total = l.acc + parts * a.head_dim * 4;
+    return l;
+}
+
+void set_blocks_workspace(BlocksArgs& a, const BlocksLayout& l, void* ws)
+{
+    char* w = static_cast<char*>(ws);
+    a.ws_pieces = reinterpret_cast<int32_t*>(w);  // (the prefill's; the others' states begin there)
+    a.ws_ml = reinterpret_cast<float2*>(w + l.ml);
+    a.ws_acc = reinterpret_cast<float*>(w + l.acc);
+}
+
+hipError_t launch_blocks_prefill(const BlocksArgs& a, hipStream_t stream)
+{
+    ListPrefillArgs p = list_prefill_args(a);
+    p.n_split = a.splits;
+    p.ws_pieces = a.ws_pieces;
+    p.ws_ml = reinterpret_cast<float*>(a.ws_ml);
+    p.ws_acc = a.ws_acc;
     if (a.cache_dtype == BF16) return launch_blocks_prefill_bf16(p, stream);
     if (a.cache_dtype == F16) return launch_blocks_prefill_f16(p, stream);
     if (a.cache_dtype == I8) return launch_blocks_prefill_i8(p, stream);
@@ -690,16 +754,21 @@ hipError_t launch_blocks(const BlocksArgs& a, hipStream_t stream)
     const int64_t wgs = static_cast<int64_t>(a.batch) * a.seq_len * blocks_heads(a) * a.splits;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.seq_len * a.num_heads;
     if (wgs > INT32_MAX || rows > INT32_MAX) return hipErrorInvalidConfiguration;
-    const dim3 grid(static_cast<unsigned>(wgs)), block(64 * kBlocksWaves);
+    const dim3 grid(static_cast<unsigned>(wgs)), block(static_cast<unsigned>(64 * a.waves));
     hipError_t e;
     if (kernel == BlocksKernel::kDecode)
         e = for_types(a, [&]<int QT, int CT>()
         {
             auto go = [&]<int D>()
             {
+                const unsigned lds = static_cast<unsigned>(blocks_lds_bytes<D>(a.waves, std::min(a.group, 16)));
                 if constexpr (CT != F32)
-                    hipLaunchKernelGGL((paged_blocks_decode<CT, QT, D>), grid, block,
-                                       static_cast<unsigned>(blocks_lds_bytes<D>(std::min(a.group, 16))), stream, a);
+                {
+                    if (a.waves == 8)
+                        hipLaunchKernelGGL((paged_blocks_decode<CT, QT, D, 8>), grid, block, lds, stream, a);
+                    else
+                        hipLaunchKernelGGL((paged_blocks_decode<CT, QT, D, 4>), grid, block, lds, stream, a);
+                }
                 return hipGetLastError();
             };
             if (a.head_dim == 64) return go.template operator()<64>();

@@ -4,6 +4,7 @@
 namespace ffkv
 {
 
+void       plan_blocks_prefill_i8(ListPrefillArgs& a) { plan_blocks_prefill_t<I8>(a); }
 hipError_t launch_blocks_prefill_i8(const ListPrefillArgs& a, hipStream_t stream) { return launch_blocks_prefill_t<I8>(a, stream); }
 
 }  // namespace ffkv

@@ -366,7 +366,7 @@ template <int QT, int D, int CT, bool PFX, int RG, bool SPLIT = false, bool RULE
 __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillArgs, PrefillKernelArgs<RULE>> a, int wg_index,
                                            uint8_t* s_st0, uint8_t* s_st1, uint8_t* s_st2, uint8_t* s_st3, int& s_vover)
 {
-    static_assert(!LIST || (RULE && !SPLIT && !PFX), "lists are masked as a rule's ranges are, and not split");
+    static_assert(!LIST || (RULE && !PFX), "lists are masked as a rule's ranges are");
     constexpr int  W = 8 / RG;  // waves per workgroup
     constexpr int  EB = kElemBytes<CT>;
     constexpr bool Q8 = EB == 1;
@@ -448,7 +448,7 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
     const int rb = nrb - 1 - k_in_xcd % nrb;
     int       grp = (k_in_xcd / nrb) * kXcds + xcd;
     int       len = 0;
-    if constexpr (SPLIT)
+    if constexpr (SPLIT && !LIST)
     {
         // The pieces of an XCD's groups by decreasing steps, those without any last: the longest go out first and to a CU
         // each.  Lane j holds group slot (j0 + j) * kXcds + xcd, of all pieces, or where those are more than the lanes of
@@ -503,7 +503,7 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
 #else
     const int grp = wg_index / nrb;
     const int rb = wg_index % nrb;
-    const int len = SPLIT ? split_len<KP>(a, nrb, lane) : 0;
+    const int len = SPLIT && !LIST ? split_len<KP>(a, nrb, lane) : 0;
 #endif
     const int piece = nsp == 1 ? 0 : grp / groups0;
     const int grp0 = grp - piece * groups0;
@@ -601,14 +601,20 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
         pg_hi = static_cast<int>((kw + kBlockSize - 1) / kBlockSize);
         if constexpr (LIST)
         {
-            // entries up to the last that is a page of the row (every wave on its own)
+            // entries up to the last that is a page of the row (every wave on its own, 256 entries' loads at a time)
+            constexpr int MF = 4;
             pg_hi = 0;
-            for (int e0 = (a.count - 1) & ~63; e0 >= 0 && pg_hi == 0; e0 -= 64)
+            for (int e0 = (a.count - 1) & ~(64 * MF - 1); e0 >= 0 && pg_hi == 0; e0 -= 64 * MF)
             {
-                const int      e = e0 + lane;
-                const int      lp = e < a.count ? list[e] : -1;
-                const uint64_t hit = __ballot(lp >= 0 && lp < a.max_blocks && static_cast<int64_t>(lp) * kBlockSize < L);
-                if (hit != 0) pg_hi = e0 + 64 - __builtin_clzll(hit);
+                int lp[MF];
+#pragma unroll
+                for (int f = 0; f < MF; ++f) lp[f] = e0 + 64 * f + lane < a.count ? list[e0 + 64 * f + lane] : -1;
+#pragma unroll
+                for (int f = 0; f < MF; ++f)
+                {
+                    const uint64_t hit = __ballot(lp[f] >= 0 && lp[f] < a.max_blocks && static_cast<int64_t>(lp[f]) * kBlockSize < L);
+                    if (hit != 0) pg_hi = e0 + 64 * f + 64 - __builtin_clzll(hit);
+                }
             }
         }
         else if constexpr (RULE)
@@ -637,7 +643,8 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
     int64_t part = -1;  // slot of this piece's partials, or -1: the workgroup has all the keys and writes the output
     if constexpr (SPLIT)
     {
-        const int np = split_pieces(a, (pg_hi - (RULE ? pg_lo : 0) + KP - 1) / KP, len);
+        int np = split_pieces(a, (pg_hi - (RULE ? pg_lo : 0) + KP - 1) / KP, len);
+        if constexpr (LIST) np = max(1, min(nsp, (pg_hi + KP - 1) / KP / kPrefillSplitMin));
         if (piece >= np) return;  // uniform over the workgroup
         const int64_t blk = static_cast<int64_t>(grp0) * nrb + rb;
         if (piece == 0 && tid == 0) a.ws_pieces[blk] = np;
@@ -1717,8 +1724,9 @@ void paged_prefill_dma(PrefillArgs a)
 // (row group, output tile) of each of the block's pieces, as the pieces' waves wrote them, and writes its four output
 // dims.  A piece that saw no key of the row weighs nothing (its accumulators still enter with weight 0, so that a NaN
 // the row would have met in one pass is met here too).
-template <int QT, int D>
-__global__ __launch_bounds__(256) void paged_prefill_merge(PrefillArgs a)
+// LIST: the blocks are those of lists, of query_block tokens each.
+template <int QT, int D, bool LIST = false>
+__global__ __launch_bounds__(256) void paged_prefill_merge(std::conditional_t<LIST, ListPrefillArgs, PrefillArgs> a)
 {
     constexpr int NT = D / 16;
     constexpr int MF = 8;  // pieces whose loads go out together
@@ -1726,7 +1734,9 @@ __global__ __launch_bounds__(256) void paged_prefill_merge(PrefillArgs a)
     const int     np = a.ws_pieces[blk];
     if (np <= 1) return;
     const int G = a.group, S = a.seq_len, Hkv = a.num_kv_heads;
-    const int nrb = (S * G + kDmaRows - 1) / kDmaRows;
+    int       tokens = S;  // of a group
+    if constexpr (LIST) tokens = a.query_block;
+    const int nrb = (tokens * G + kDmaRows - 1) / kDmaRows;
     const int grp = blk / nrb;
     const int k = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
     const int lane = k & 63;
@@ -1734,7 +1744,15 @@ __global__ __launch_bounds__(256) void paged_prefill_merge(PrefillArgs a)
     const int rg = (k >> 6) / NT;
     const int row = 16 * rg + (lane & 15);
     const int r = (blk - grp * nrb) * kDmaRows + row;
-    if (r >= S * G) return;
+    int       b = grp / Hkv, t0 = 0;
+    if constexpr (LIST)
+    {
+        const int rl = b;
+        b = rl / a.lists;
+        t0 = (rl - b * a.lists) * a.query_block;
+        tokens = min(tokens, S - t0);
+    }
+    if (r >= tokens * G) return;
     const int64_t p0 = static_cast<int64_t>(blk) * a.n_split;
     const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + p0 * kDmaRows + row;
     const f32x4*  xs = reinterpret_cast<const f32x4*>(a.ws_acc) + (p0 * (kDmaRows / 16) + rg) * NT * 64 + n * 64 + lane;
@@ -1772,7 +1790,7 @@ __global__ __launch_bounds__(256) void paged_prefill_merge(PrefillArgs a)
         m = mn;
     }
     const int    h = grp % Hkv * G + r % G;
-    const size_t ob = ((static_cast<size_t>(grp / Hkv) * S + r / G) * a.num_heads + h) * D + 16 * n + 4 * (lane >> 4);
+    const size_t ob = ((static_cast<size_t>(b) * S + t0 + r / G) * a.num_heads + h) * D + 16 * n + 4 * (lane >> 4);
     store_out4<QT>(a.out, ob, o * softmax_inv(l));
 }
 
@@ -1977,6 +1995,33 @@ hipError_t launch_prefill_merge(const PrefillArgs& a, hipStream_t stream)
     if (a.qo_dtype == F32) return launch_prefill_merge_q<F32>(a, stream);
     if (a.qo_dtype == F16) return launch_prefill_merge_q<F16>(a, stream);
     return launch_prefill_merge_q<BF16>(a, stream);
+}
+
+namespace
+{
+
+template <int QT>
+hipError_t launch_list_merge(const ListPrefillArgs& a, int64_t blocks, hipStream_t stream)
+{
+    const dim3 grid(static_cast<unsigned>(kDmaRows * a.head_dim / 4 / 256), static_cast<unsigned>(blocks));
+    if (a.head_dim == 64)
+        hipLaunchKernelGGL((paged_prefill_merge<QT, 64, true>), grid, dim3(256), 0, stream, a);
+    else if (a.head_dim == 128)
+        hipLaunchKernelGGL((paged_prefill_merge<QT, 128, true>), grid, dim3(256), 0, stream, a);
+    else
+        hipLaunchKernelGGL((paged_prefill_merge<QT, 256, true>), grid, dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_blocks_prefill_merge(const ListPrefillArgs& a, hipStream_t stream)
+{
+    const int64_t blocks = static_cast<int64_t>(a.batch) * a.lists * a.num_kv_heads *
+                           ((static_cast<int64_t>(a.query_block) * a.group + kDmaRows - 1) / kDmaRows);
+    if (a.qo_dtype == F32) return launch_list_merge<F32>(a, blocks, stream);
+    if (a.qo_dtype == F16) return launch_list_merge<F16>(a, blocks, stream);
+    return launch_list_merge<BF16>(a, blocks, stream);
 }
 
 hipError_t launch_prefix_partials(const PrefillArgs& a, hipStream_t stream) { return launch_pfd<true, false>(a, stream); }

@@ -960,7 +960,7 @@ PyObject* attention_blocks(PyObject*, PyObject* const* a, Py_ssize_t n)
     auto *ks = r.ptr<float>(a[4]), *vs = r.ptr<float>(a[5]);
     auto *bt = r.ptr<int32_t>(a[6]), *cx = r.ptr<int32_t>(a[7]), *bl = r.ptr<int32_t>(a[8]);
     void*         s = r.stream(a[13]);
-    const size_t  need = r.ok && a[11] == Py_None ? fn.attention_blocks_bytes(ct, B, S, Hq, Hkv, D, keep, T) : 0;
+    const size_t  need = r.ok && a[11] == Py_None ? fn.attention_blocks_bytes(qt, ct, B, S, Hq, Hkv, D, keep, T) : 0;
     const Scratch ws(r, a[11], a[14], need, q, a[13]);
     return finish(r, [&] {
         return fn.attention_blocks(qp, out, qt, kc, vc, ct, ks, vs, bt, cx, bl, keep, T, B, S, Hq, Hkv, D, FFKV_BLOCK_SIZE, mb, N,

@@ -475,8 +475,9 @@ FFKV_API int ffkv_select_blocks(const void* q, int q_dtype, const void* bounds, 
  * ffkv_paged_attention_blocks_workspace_bytes (0 but for few lists, which are then split; a captured call without one leaves
  * them whole).
  */
-FFKV_API size_t ffkv_paged_attention_blocks_workspace_bytes(int cache_dtype, int batch, int seq_len, int num_heads,
-                                                            int num_kv_heads, int head_dim, int count, int query_block);
+FFKV_API size_t ffkv_paged_attention_blocks_workspace_bytes(int qo_dtype, int cache_dtype, int batch, int seq_len,
+                                                            int num_heads, int num_kv_heads, int head_dim, int count,
+                                                            int query_block);
 
 FFKV_API int ffkv_paged_attention_blocks(const void* q, void* out, int qo_dtype, const void* k_cache, const void* v_cache,
                                          int cache_dtype, const float* k_scale, const float* v_scale,

@@ -135,10 +135,12 @@ def test_workspace_bytes(ff):
     assert f(2, 100, 8, 4, 64, 50, 32, 50, 0) == 0 and f(2, 100, 8, 4, 64, 19, 32, 50, 300) == 0
     assert f(0, 1, 1, 1, 64, 1, 1, 9, 0) == 0 and f(1, 1, 1, 1, 64, 0, 1, 9, 0) == 0 and f(1, 1, 1, 1, 64, 1, 0, 9, 0) == 0
     g = ff.lib.ffkv_paged_attention_blocks_workspace_bytes
-    assert g(ff.DTYPE_BF16, 64, 1, 32, 8, 128, 64, 1) == 0  # enough lists for the chip
-    assert g(ff.DTYPE_BF16, 1, 1, 32, 8, 128, 256, 1) > 0
-    assert g(ff.DTYPE_BF16, 1, 1, 32, 8, 128, 256, 64) == g(ff.DTYPE_BF16, 1, 1, 32, 8, 128, 256, 1)  # one token, one list
-    assert g(7, 1, 1, 32, 8, 128, 256, 1) == 0 and g(ff.DTYPE_BF16, 1, 1, 30, 8, 128, 256, 1) == 0
+    assert g(ff.DTYPE_BF16, ff.DTYPE_BF16, 64, 1, 32, 8, 128, 64, 1) == 0  # enough lists for the chip
+    assert g(ff.DTYPE_BF16, ff.DTYPE_BF16, 1, 1, 32, 8, 128, 256, 1) > 0
+    assert g(ff.DTYPE_BF16, ff.DTYPE_BF16, 1, 1, 32, 8, 128, 256, 64) == g(ff.DTYPE_BF16, ff.DTYPE_BF16, 1, 1, 32, 8, 128, 256, 1)  # one token, one list
+    assert g(ff.DTYPE_BF16, ff.DTYPE_FP8_E4M3, 1, 64, 32, 8, 128, 256, 64) > 0  # a chunk of few lists is split too
+    assert g(ff.DTYPE_BF16, ff.DTYPE_BF16, 8, 1024, 32, 8, 128, 256, 64) == 0 and g(3, 2, 1, 1, 32, 8, 128, 256, 1) == 0
+    assert g(ff.DTYPE_BF16, 7, 1, 1, 32, 8, 128, 256, 1) == 0 and g(ff.DTYPE_BF16, ff.DTYPE_BF16, 1, 1, 30, 8, 128, 256, 1) == 0
 
 
 # ---- the Python front end's checks (calls without rows touch no GPU) -------------------------------------------------

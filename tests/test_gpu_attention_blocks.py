@@ -141,9 +141,9 @@ def test_scale_workspace_stream(ff, gpu, scale):
     """A split call with its workspace, without one, and on another stream gives the same bits."""
     c = make(21, [4000], 1, 8, 2, 128)
     li = lists(c, 1, 200, 1)
-    n = ff.lib.ffkv_paged_attention_blocks_workspace_bytes(c.kv, 1, 1, 8, 2, 128, 200, 1)
+    n = ff.lib.ffkv_paged_attention_blocks_workspace_bytes(c.act, c.kv, 1, 1, 8, 2, 128, 200, 1)
     assert n > 0
-    ws = ff.attention_blocks_workspace(c.kv, 1, 1, 8, 2, 128, 200)
+    ws = ff.attention_blocks_workspace(c.act, c.kv, 1, 1, 8, 2, 128, 200)
     a = run(ff, c, li, 1, gpu, workspace=ws, scale=scale)
     side = torch.cuda.Stream()
     torch.cuda.synchronize()
@@ -161,7 +161,7 @@ def test_capture(ff, gpu, S, T):
     c = make(6, [4000, 900], S, 8, 2, 128)
     kp, vp, ks, vs, bt, cx, _, _, q = su.device(c, gpu)
     li = torch.from_numpy(lists(c, S, 200, T)).to(gpu)
-    ws = ff.attention_blocks_workspace(c.kv, 2, S, 8, 2, 128, 200, T)
+    ws = ff.attention_blocks_workspace(c.act, c.kv, 2, S, 8, 2, 128, 200, T)
     out, whole = torch.empty(2, S, 8 * 128, dtype=q.dtype, device=gpu), torch.empty(2, S, 8 * 128, dtype=q.dtype, device=gpu)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
@@ -179,3 +179,43 @@ def test_capture(ff, gpu, S, T):
         assert torch.equal(got, eager)
         # an unsplit softmax is the same up to its sums' roundings and the output's
         assert (got.float() - got_whole.float()).abs().max().item() <= 2.0 ** -7 * got.float().abs().max().item()
+
+
+@pytest.mark.parametrize("act,kv", KV)
+@pytest.mark.parametrize("Hq,Hkv,D,ctx,S,count,T", [
+    (8, 2, 128, [2500, 40, 1200], 13, 130, 32), (5, 1, 64, [3000], 40, 170, 7), (20, 4, 256, [1531, 1908], 13, 100, 13),
+])
+def test_split_chunk(ff, gpu, act, kv, Hq, Hkv, D, ctx, S, count, T):
+    """Few blocks of queries over long lists, split over the lists; the same whole, in a capture without a workspace."""
+    c = make(Hq + D, ctx, S, Hq, Hkv, D, act, kv)
+    n = ff.lib.ffkv_paged_attention_blocks_workspace_bytes(c.act, c.kv, c.B, S, Hq, Hkv, D, count, T)
+    assert n > 0
+    li = lists(c, S, count, T, shuffle=True)
+    check(ff, c, li, T, gpu)
+    kp, vp, ks, vs, bt, cx, _, _, q = su.device(c, gpu)
+    ld, out = torch.from_numpy(li).to(gpu), torch.empty(c.B, S, Hq * D, dtype=q.dtype, device=gpu)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ff.paged_attention_blocks(q, kp, vp, bt, cx, ld, query_block=T, out=out, k_scale=ks, v_scale=vs)
+    graph.replay()
+    want, bound = bu.attend(c, cases.decode(c.q, c.act).astype(np.float64), li, T, c.act, S, 2.0 ** -10)
+    su.check(su.host(out).reshape(want.shape), want, bound, "whole")
+
+
+@pytest.mark.parametrize("act,kv", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "fp8"), ("bf16", "i8")])
+def test_split_hidden_values(ff, gpu, act, kv):
+    """As test_hidden_values_do_not_reach, with the strange values in one piece of a split list."""
+    c = make(77, [2000], 12, 8, 2, 128, act, kv)
+    li = lists(c, 12, 120, 12)
+    li[0, 0, :, 60] = 2000 // 16
+    for h in range(2):
+        li[0, 0, h, 61:][li[0, 0, h, 61:] == 2000 // 16] = -1
+        li[0, 0, h, :60][li[0, 0, h, :60] == 2000 // 16] = -1
+    q = cases.decode(c.q, c.act).astype(np.float64)
+    want, bound = bu.attend(c, q, li, 12, c.act, 12, 2.0 ** -10)
+    for t in range(2008, 2016):  # seen by the queries from the eighth on, or by none
+        su.poison(c, 0, t)
+    got = su.host(run(ff, c, li, 12, gpu)).reshape(want.shape)
+    su.check(got[:, :8], want[:, :8], bound[:, :8], "before")
+    assert not np.isfinite(got[:, 8:]).any()
