@@ -462,4 +462,140 @@ void evict_kv_cache(Tensor& weights, Tensor& k_cache, Tensor& v_cache, const int
            "evict_kv_cache failed");
 }
 
+namespace
+{
+
+bool is_cache(const Tensor& t) { return is_gpu(t) && t.shape().size() == 4 && t.shape()[1] == FFKV_BLOCK_SIZE; }
+
+// Blocks I32 [B, ceil(S / query_block), Hkv, count] of a call, or false.
+bool are_lists(const Tensor& blocks, int64_t B, int64_t S, int64_t Hkv, int query_block)
+{
+    const auto& s = blocks.shape();
+    return is_gpu(blocks) && blocks.dtype() == DType::I32 && s.size() == 4 && query_block > 0 && s[0] == B &&
+           s[1] == (S + query_block - 1) / query_block && s[2] == Hkv;
+}
+
+// A quantized cache's scales have its shape (int8 [N, 16, Hkv], fp8 [Hkv]).
+bool scales_fit(const Tensor& cache, const Tensor* scale)
+{
+    if (cache.dtype() != DType::I8 && cache.dtype() != DType::FP8_E4M3) return true;
+    const int64_t n = cache.dtype() == DType::I8 ? cache.shape()[0] * cache.shape()[1] * cache.shape()[2] : cache.shape()[2];
+    return scale != nullptr && is_gpu(*scale) && scale->dtype() == DType::F32 && scale->numel() >= n;
+}
+
+}  // namespace
+
+void apply_rope_axes(Tensor& q, Tensor& k, const AxisPositions& at)
+{
+    const bool has_q = q.data() != nullptr;
+    if (k.shape().size() != 4 || !is_gpu(k) ||
+        (has_q && (q.shape().size() != 4 || !is_gpu(q) || q.shape()[0] != k.shape()[0] || q.shape()[1] != k.shape()[1] ||
+                   q.shape()[3] != k.shape()[3] || q.dtype() != k.dtype())))
+        return fail("apply_rope_axes: q must be [B, S, Hq, D] and k [B, S, Hkv, D] of one dtype on the GPU");
+    report(ffkv_rope_axes(has_q ? q.data() : nullptr, 0, has_q ? q.data() : nullptr, 0, k.data(), 0, k.data(), 0, code(k.dtype()),
+                          at.positions, at.sections, at.axes, at.interleaved, static_cast<int>(k.shape()[0]),
+                          static_cast<int>(k.shape()[1]), has_q ? static_cast<int>(q.shape()[2]) : 0,
+                          static_cast<int>(k.shape()[2]), static_cast<int>(k.shape()[3]), at.theta, t_stream),
+           "apply_rope_axes failed");
+}
+
+void rope_append_kv_cache_axes(Tensor& q, const Tensor& k, const Tensor& v, Tensor& k_cache, Tensor& v_cache,
+                               const int* block_table, const int* context_lens, int max_blocks, const AxisPositions& at,
+                               Tensor* k_scale, Tensor* v_scale, Tensor* q_out)
+{
+    const bool has_q = q.data() != nullptr;
+    if (k.shape().size() != 4 || v.shape() != k.shape() || v.dtype() != k.dtype() || !is_gpu(k) || !is_gpu(v) ||
+        (has_q && (q.shape().size() != 4 || !is_gpu(q) || q.shape()[0] != k.shape()[0] || q.shape()[1] != k.shape()[1] ||
+                   q.shape()[3] != k.shape()[3] || q.dtype() != k.dtype())))
+        return fail("rope_append_kv_cache_axes: q must be [B, S, Hq, D], k and v [B, S, Hkv, D] of one dtype on the GPU");
+    if (has_q && q_out != nullptr && (!is_gpu(*q_out) || q_out->dtype() != q.dtype() || q_out->shape() != q.shape()))
+        return fail("rope_append_kv_cache_axes: q_out must be like q");
+    if (!is_cache(k_cache) || !is_cache(v_cache) || v_cache.shape() != k_cache.shape() || v_cache.dtype() != k_cache.dtype() ||
+        k_cache.shape()[2] != k.shape()[2] || k_cache.shape()[3] != k.shape()[3])
+        return fail("rope_append_kv_cache_axes: the caches must both be [num_blocks, 16, Hkv, D]");
+    if (!scales_fit(k_cache, k_scale) || !scales_fit(v_cache, v_scale))
+        return fail("rope_append_kv_cache_axes: quantized caches need their F32 scales on the GPU");
+    void* qo = has_q ? (q_out ? q_out->data() : q.data()) : nullptr;
+    report(ffkv_rope_append_axes(has_q ? q.data() : nullptr, 0, qo, 0, k.data(), 0, v.data(), 0, code(k.dtype()), k_cache.data(),
+                                 v_cache.data(), code(k_cache.dtype()), k_scale ? k_scale->data_as<float>() : nullptr,
+                                 v_scale ? v_scale->data_as<float>() : nullptr, reinterpret_cast<const int32_t*>(block_table),
+                                 reinterpret_cast<const int32_t*>(context_lens), at.positions, at.sections, at.axes,
+                                 at.interleaved, static_cast<int>(k.shape()[0]), static_cast<int>(k.shape()[1]),
+                                 has_q ? static_cast<int>(q.shape()[2]) : 0, static_cast<int>(k.shape()[2]),
+                                 static_cast<int>(k.shape()[3]), FFKV_BLOCK_SIZE, max_blocks,
+                                 static_cast<int>(k_cache.shape()[0]), at.theta, t_stream),
+           "rope_append_kv_cache_axes failed");
+}
+
+void update_key_bounds(const Tensor& k_cache, Tensor& bounds, const int* block_table, const int* context_lens, int batch,
+                       int max_blocks, int new_tokens, const Tensor* k_scale)
+{
+    if (!is_cache(k_cache)) return fail("update_key_bounds: the cache must be [num_blocks, 16, Hkv, D] on the GPU");
+    const auto& c = k_cache.shape();
+    const bool  eight = k_cache.dtype() == DType::I8 || k_cache.dtype() == DType::FP8_E4M3;
+    const std::vector<int64_t> want{c[0], c[2], 2, c[3]};
+    if (!is_gpu(bounds) || bounds.shape() != want || bounds.dtype() != (eight ? DType::BF16 : k_cache.dtype()))
+        return fail("update_key_bounds: bounds must be [num_blocks, Hkv, 2, D] of the cache's dtype (BF16 beside 8-bit ones)");
+    if (!scales_fit(k_cache, k_scale)) return fail("update_key_bounds: a quantized cache needs its F32 scales on the GPU");
+    report(ffkv_key_bounds(k_cache.data(), code(k_cache.dtype()), scale_of(k_scale), bounds.data(),
+                           reinterpret_cast<const int32_t*>(block_table), reinterpret_cast<const int32_t*>(context_lens), batch,
+                           new_tokens, static_cast<int>(c[2]), static_cast<int>(c[3]), FFKV_BLOCK_SIZE, max_blocks,
+                           static_cast<int>(c[0]), t_stream),
+           "update_key_bounds failed");
+}
+
+void select_blocks(const Tensor& q, const Tensor& bounds, Tensor& blocks, const int* block_table, const int* context_lens,
+                   int max_blocks, int sinks, int recent, int query_block, int max_context_len)
+{
+    if (q.shape().size() != 4 || !is_gpu(q)) return fail("select_blocks: q must be [B, S, Hq, D] on the GPU");
+    const int B = static_cast<int>(q.shape()[0]), S = static_cast<int>(q.shape()[1]);
+    const int Hq = static_cast<int>(q.shape()[2]), D = static_cast<int>(q.shape()[3]);
+    if (bounds.shape().size() != 4 || !is_gpu(bounds) || bounds.shape()[2] != 2 || bounds.shape()[3] != D)
+        return fail("select_blocks: bounds must be [num_blocks, Hkv, 2, head_dim] on the GPU");
+    const int Hkv = static_cast<int>(bounds.shape()[1]);
+    if (!are_lists(blocks, B, S, Hkv, query_block))
+        return fail("select_blocks: blocks must be I32 [B, ceil(S / query_block), Hkv, count] on the GPU, query_block at least 1");
+    const int    count = static_cast<int>(blocks.shape()[3]);
+    const size_t need = ffkv_select_blocks_workspace_bytes(B, S, Hq, Hkv, D, count, query_block, max_blocks, max_context_len);
+    size_t       have = 0;
+    void*        ws = need > 0 ? workspace(need, have) : nullptr;
+    report(ffkv_select_blocks(q.data(), code(q.dtype()), bounds.data(), code(bounds.dtype()),
+                              reinterpret_cast<const int32_t*>(block_table), reinterpret_cast<const int32_t*>(context_lens),
+                              blocks.data_as<int32_t>(), count, sinks, recent, query_block, B, S, Hq, Hkv, D, FFKV_BLOCK_SIZE,
+                              max_blocks, static_cast<int>(bounds.shape()[0]), max_context_len, ws, have, t_stream),
+           "select_blocks failed");
+}
+
+void attention_blocks(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, Tensor& output, const Tensor& blocks,
+                      const int* block_table, const int* context_lens, int max_blocks, int query_block, const Tensor* k_scale,
+                      const Tensor* v_scale)
+{
+    if (q.shape().size() != 4 || !is_gpu(q) || !is_gpu(output))
+        return fail("attention_blocks: q must be [B, S, Hq, D] and all tensors on the GPU");
+    const int B = static_cast<int>(q.shape()[0]), S = static_cast<int>(q.shape()[1]);
+    const int Hq = static_cast<int>(q.shape()[2]), D = static_cast<int>(q.shape()[3]);
+    if (output.numel() < static_cast<int64_t>(B) * S * Hq * D || output.dtype() != q.dtype())
+        return fail("attention_blocks: output must hold as many elements of q's dtype as q");
+    if (!is_cache(k_cache) || !is_cache(v_cache) || v_cache.shape() != k_cache.shape() || v_cache.dtype() != k_cache.dtype() ||
+        k_cache.shape()[3] != D)
+        return fail("attention_blocks: the caches must both be [num_blocks, 16, Hkv, head_dim]");
+    const int Hkv = static_cast<int>(k_cache.shape()[2]);
+    if (!are_lists(blocks, B, S, Hkv, query_block))
+        return fail("attention_blocks: blocks must be I32 [B, ceil(S / query_block), Hkv, count] on the GPU, query_block at least 1");
+    if (!scales_fit(k_cache, k_scale) || !scales_fit(v_cache, v_scale))
+        return fail("attention_blocks: quantized caches need their F32 scales on the GPU");
+    const int    count = static_cast<int>(blocks.shape()[3]);
+    const size_t need = ffkv_paged_attention_blocks_workspace_bytes(code(q.dtype()), code(k_cache.dtype()), B, S, Hq, Hkv, D,
+                                                                    count, query_block);
+    size_t       have = 0;
+    void*        ws = need > 0 ? workspace(need, have) : nullptr;
+    report(ffkv_paged_attention_blocks(q.data(), output.data(), code(q.dtype()), k_cache.data(), v_cache.data(),
+                                       code(k_cache.dtype()), scale_of(k_scale), scale_of(v_scale),
+                                       reinterpret_cast<const int32_t*>(block_table),
+                                       reinterpret_cast<const int32_t*>(context_lens), blocks.data_as<const int32_t>(), count,
+                                       query_block, B, S, Hq, Hkv, D, FFKV_BLOCK_SIZE, max_blocks,
+                                       static_cast<int>(k_cache.shape()[0]), 0.0f, ws, have, t_stream),
+           "attention_blocks failed");
+}
+
 }  // namespace firefly::kernels

@@ -181,6 +181,61 @@ FIREFLY_API void evict_kv_cache(Tensor& weights, Tensor& k_cache, Tensor& v_cach
                                 Tensor& kept_lens, const int* dst_table = nullptr, int dst_blocks = 0,
                                 Tensor* weights_out = nullptr, Tensor* k_scale = nullptr, Tensor* v_scale = nullptr);
 
+// ---- positions on several axes, and attention over selected pages (no counterpart in the reference) ------------------
+
+/**
+ * @brief Positions of tokens on several axes (time, height and width of image and video tokens), and which pairs of dims turn
+ * by which axis (include/ffkv.h has the formulas).
+ */
+struct AxisPositions
+{
+    const int* positions = nullptr;         ///< [axes, B, S] on the device
+    int        axes = 0;                    ///< 1 to 4
+    int        sections[4] = {0, 0, 0, 0};  ///< pairs of dims of each axis, head_dim / 2 together
+    bool       interleaved = false;         ///< pairs dealt out in turn; else one section behind the other
+    float      theta = 1e6f;
+};
+
+/**
+ * @brief apply_rope() by positions on several axes, in place (ffkv_rope_axes): q [B, S, Hq, D] (or empty) and k [B, S, Hkv, D]
+ * of one dtype.
+ */
+FIREFLY_API void apply_rope_axes(Tensor& q, Tensor& k, const AxisPositions& at);
+
+/**
+ * @brief apply_rope_axes() and append_kv_cache() in one kernel (ffkv_rope_append_axes): q is rotated in place, or into q_out;
+ * k and v are only read, the rotated k is in the pages alone.  Scales for quantized caches.
+ */
+FIREFLY_API void rope_append_kv_cache_axes(Tensor& q, const Tensor& k, const Tensor& v, Tensor& k_cache, Tensor& v_cache,
+                                           const int* block_table, const int* context_lens, int max_blocks,
+                                           const AxisPositions& at, Tensor* k_scale = nullptr, Tensor* v_scale = nullptr,
+                                           Tensor* q_out = nullptr);
+
+/**
+ * @brief The smallest and largest key, per KV head and dim, of the pages that the tokens context_lens[b] ..
+ * context_lens[b] + new_tokens - 1 of `batch` rows lie on (ffkv_key_bounds): bounds [num_blocks, Hkv, 2, D] of the cache's dtype, BF16 beside
+ * int8 and fp8 caches.  Call it after every append to rows that select_blocks will choose from.
+ */
+FIREFLY_API void update_key_bounds(const Tensor& k_cache, Tensor& bounds, const int* block_table, const int* context_lens,
+                                   int batch, int max_blocks, int new_tokens, const Tensor* k_scale = nullptr);
+
+/**
+ * @brief Which pages to attend (ffkv_select_blocks): blocks I32 [B, ceil(S / query_block), Hkv, count] receives, for every
+ * block of query_block queries of q [B, S, Hq, D] and KV head, the first `sinks` pages, the last `recent`, and those whose key
+ * bounds allow the largest scores.
+ */
+FIREFLY_API void select_blocks(const Tensor& q, const Tensor& bounds, Tensor& blocks, const int* block_table,
+                               const int* context_lens, int max_blocks, int sinks, int recent, int query_block = 1,
+                               int max_context_len = 0);
+
+/**
+ * @brief Causal attention over listed pages alone (ffkv_paged_attention_blocks): q [B, S, Hq, D] at context_lens[b] + t over
+ * the pages of blocks I32 [B, ceil(S / query_block), Hkv, count]; output [B, S, Hq*D] in q's dtype; scales for quantized caches.
+ */
+FIREFLY_API void attention_blocks(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, Tensor& output,
+                                  const Tensor& blocks, const int* block_table, const int* context_lens, int max_blocks,
+                                  int query_block = 1, const Tensor* k_scale = nullptr, const Tensor* v_scale = nullptr);
+
 // ---- the reference's off-path operators: declared as in its include/firefly/kernels.h, defined by the caller --
 
 // Embedding lookup (reference include/firefly/kernels.h:18).
