@@ -6,9 +6,9 @@
 // No query's score with any of the page's keys exceeds its share of that.  The sums over queries and heads go first, so a
 // block of any size costs two dot products of head_dim per page.
 //
-// Scores are fp64 sums rounded once to fp32: they decide between pages, and the choice must not depend on how a row is
-// split, on the batch or on the form that was launched (products of 16-bit values are exact in fp64, the sums' errors of
-// 2^-50 are far below the rounding's step, and all forms add up a score in the same order).
+// Scores are fp64 sums rounded once to fp32: they decide between pages, and a row's choice must not depend on the rest of the
+// batch or on how the pages are dealt out.  Products of 16-bit values are exact in fp64, and every form adds up a score in the
+// same order; the two that sum queries differ by 2^-50 of a sum at most, far below the rounding's step.
 //
 // Of a block's pages - those up to its last query's - the first `sinks` and the last `recent` are taken, and of the rest
 // those with the largest scores, of equal ones the lower; NaN (a NaN or infinite key) counts as the largest.  The list is in

@@ -119,6 +119,8 @@ int most_pages(int max_blocks, int max_context_len)
 
 constexpr double kMostBytes = 1e15;
 
+constexpr int kMostListed = 1 << 26;  // pages of a list: their tokens count in 32 bits
+
 // A choice's workspace: the scores, one per block of queries, KV head and page, and the queries' sums.
 struct SelectLayout
 {
@@ -247,7 +249,8 @@ size_t ffkv_select_blocks_workspace_bytes(int batch, int seq_len, int num_heads,
 {
     // sizes that ffkv_select_blocks refuses need nothing
     if (batch <= 0 || batch > 65535 || seq_len <= 0 || num_heads <= 0 || num_heads > 65535 || num_kv_heads <= 0 ||
-        num_heads % num_kv_heads != 0 || !head_dim_ok(head_dim) || count <= 0 || query_block <= 0 || max_blocks <= 0)
+        num_heads % num_kv_heads != 0 || !head_dim_ok(head_dim) || count <= 0 || count > kMostListed || query_block <= 0 ||
+        max_blocks <= 0)
         return 0;
     const int64_t n = select_layout(batch, seq_len, num_heads, num_kv_heads, head_dim, most_pages(max_blocks, max_context_len),
                                     count, query_block).total;
@@ -274,6 +277,7 @@ int ffkv_select_blocks(const void* q, int q_dtype, const void* bounds, int bound
     if (num_blocks < 1 && batch > 0) return fail(FFKV_ERR_INVALID_ARGUMENT, "bounds of no page");
     if (count < 1 || sinks < 0 || recent < 0 || static_cast<int64_t>(sinks) + recent > count)
         return fail(FFKV_ERR_INVALID_ARGUMENT, "count %d must be at least 1 and hold sinks %d and recent %d", count, sinks, recent);
+    if (count > kMostListed) return fail(FFKV_ERR_UNSUPPORTED, "count must be <= 2^26, got %d", count);
     if (batch == 0 || seq_len == 0) return ok();
     if (!q || !bounds || !block_table || !context_lens || !blocks)
         return fail(FFKV_ERR_INVALID_ARGUMENT, "null q, bounds, block_table, context_lens or blocks pointer");
@@ -343,8 +347,9 @@ size_t ffkv_paged_attention_blocks_workspace_bytes(int qo_dtype, int cache_dtype
                                                    int num_kv_heads, int head_dim, int count, int query_block)
 {
     // sizes that ffkv_paged_attention_blocks refuses need nothing
-    if (!is_act(qo_dtype) || !is_cache(cache_dtype) || !head_dim_ok(head_dim) || batch <= 0 || batch > 65535 || seq_len <= 0 || num_heads <= 0 ||
-        num_heads > 65535 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || count <= 0 || query_block <= 0)
+    if (!is_act(qo_dtype) || !is_cache(cache_dtype) || !head_dim_ok(head_dim) || batch <= 0 || batch > 65535 || seq_len <= 0 ||
+        num_heads <= 0 || num_heads > 65535 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || count <= 0 ||
+        count > kMostListed || query_block <= 0)
         return 0;
     ffkv::BlocksArgs a{};
     a.qo_dtype = qo_dtype;
@@ -381,6 +386,7 @@ int ffkv_paged_attention_blocks(const void* q, void* out, int qo_dtype, const vo
         return fail(FFKV_ERR_INVALID_ARGUMENT, "num_heads %d is not a multiple of num_kv_heads %d", num_heads, num_kv_heads);
     if (batch > 65535 || num_heads > 65535) return fail(FFKV_ERR_UNSUPPORTED, "batch and num_heads must be <= 65535");
     if (count < 1) return fail(FFKV_ERR_INVALID_ARGUMENT, "count must be at least 1, got %d", count);
+    if (count > kMostListed) return fail(FFKV_ERR_UNSUPPORTED, "count must be <= 2^26, got %d", count);
     if (query_block < 1) return fail(FFKV_ERR_INVALID_ARGUMENT, "query_block must be at least 1, got %d", query_block);
     if (batch == 0 || seq_len == 0) return ok();
     if (!q || !out || !k_cache || !v_cache || !block_table || !context_lens || !blocks)

@@ -10,7 +10,8 @@
 //
 // Angles: far positions turn by 10^5 radians and more, of which fp32 keeps two digits behind the point.  The turns
 // p * rate / 2 pi are one fp64 product; only their fraction, in [-1/2, 1/2], goes on to fp32 as a pair of parts, of which the
-// low one enters to first order: cos and sin are good to about 1.5 ulp at any int32 position.
+// low one enters to first order: what is left is the rounding of cos and sin to fp32 and the errors of the rate, 2^-48 of
+// the angle at most: 2^-22 + |p| 2^-48 in all (theta >= 1).
 #include "blocks.h"
 #include "ffkv_device.h"
 

@@ -213,8 +213,8 @@ FIREFLY_API void rope_append_kv_cache_axes(Tensor& q, const Tensor& k, const Ten
 
 /**
  * @brief The smallest and largest key, per KV head and dim, of the pages that the tokens context_lens[b] ..
- * context_lens[b] + new_tokens - 1 of `batch` rows lie on (ffkv_key_bounds): bounds [num_blocks, Hkv, 2, D] of the cache's dtype, BF16 beside
- * int8 and fp8 caches.  Call it after every append to rows that select_blocks will choose from.
+ * context_lens[b] + new_tokens - 1 of `batch` rows lie on (ffkv_key_bounds): bounds [num_blocks, Hkv, 2, D] of the cache's
+ * dtype, BF16 beside int8 and fp8 caches.  Call it after every append to rows that select_blocks will choose from.
  */
 FIREFLY_API void update_key_bounds(const Tensor& k_cache, Tensor& bounds, const int* block_table, const int* context_lens,
                                    int batch, int max_blocks, int new_tokens, const Tensor* k_scale = nullptr);

@@ -64,7 +64,7 @@ AXES = [
     (dict(sections=_ints(0, 0, 64), interleaved=1), -1), (dict(q_stride=8 * 128 - 8), -1), (dict(q_stride=8 * 128 + 4), -1),
     (dict(k_stride=128), -1), (dict(k_stride=-256), -1), (dict(q_out_stride=8 * 128 + 2), -1), (dict(positions=None), -1),
     (dict(k=None), -1), (dict(q_out=None), -1), (dict(q=24), -1), (dict(k=20), -1), (dict(q_out=8), -1),
-    (dict(positions=18), -1), (dict(q_stride=2048), -1), (dict(num_heads=70000), -2),
+    (dict(positions=18), -1), (dict(q_stride=2048), -1), (dict(num_heads=70000), -2), (dict(batch=2 ** 15, seq_len=2 ** 14), -2),
 ]
 
 
@@ -101,7 +101,8 @@ def test_bounds_rejects(ff, kw, code):
     (dict(workspace=16, workspace_bytes=2 * 64 * 4 - 1), -3),
     (dict(seq_len=2 ** 31 - 1, batch=60000, num_heads=60000, num_kv_heads=60000), -2),
     (dict(seq_len=2 ** 31 - 1, query_block=2 ** 31 - 1, num_heads=64, num_kv_heads=1), -2),
-    (dict(seq_len=2 ** 20, max_blocks=2 ** 26), -2)])
+    (dict(seq_len=2 ** 20, max_blocks=2 ** 26), -2), (dict(count=2 ** 26 + 1), -2), (dict(count=2 ** 31 - 1), -2),
+    (dict(num_blocks=0), -1)])
 def test_select_rejects(ff, kw, code):
     assert _select(ff, **kw) == code and ff.lib.ffkv_last_error() != b""
 
@@ -112,7 +113,8 @@ def test_select_rejects(ff, kw, code):
     (dict(count=0), -1), (dict(query_block=0), -1), (dict(query_block=-4), -1), (dict(q=None), -1), (dict(out=None), -1),
     (dict(v_cache=None), -1), (dict(blocks=None), -1), (dict(context_lens=None), -1), (dict(cache_dtype=3), -1),
     (dict(cache_dtype=8, v_scale=16), -1), (dict(q=8), -1), (dict(out=4), -1), (dict(blocks=18), -1), (dict(workspace=8), -1),
-    (dict(workspace=16, workspace_bytes=16, count=256), -3), (dict(seq_len=2 ** 31 - 1), -2)])
+    (dict(workspace=16, workspace_bytes=16, count=256), -3), (dict(seq_len=2 ** 31 - 1), -2),
+    (dict(count=2 ** 26 + 1), -2), (dict(count=2 ** 31 - 1, query_block=2, seq_len=2), -2)])
 def test_attention_rejects(ff, kw, code):
     assert _attend(ff, **kw) == code and ff.lib.ffkv_last_error() != b""
 

@@ -59,7 +59,7 @@ KV = [("bf16", "bf16"), ("f16", "f16"), ("bf16", "i8"), ("bf16", "fp8"), ("f32",
 @pytest.mark.parametrize("Hq,Hkv,D,ctx,count", [
     (16, 8, 128, [17, 64, 100, 255], 4), (28, 4, 128, [3000], 150), (5, 1, 64, [0, 15, 16, 900], 7), (8, 8, 256, [500, 31], 20),
     (6, 2, 96, [1000, 3], 33), (3, 3, 80, [200, 400], 5), (4, 2, 112, [640], 41), (20, 1, 128, [800, 900], 30),
-    (2, 2, 8, [100], 3), (36, 2, 64, [333], 9),
+    (2, 2, 8, [100], 3), (36, 2, 64, [333], 9), (32, 2, 256, [700], 40),
 ])
 def test_step(ff, gpu, act, kv, Hq, Hkv, D, ctx, count):
     c = make(Hq + D, ctx, 1, Hq, Hkv, D, act, kv)
