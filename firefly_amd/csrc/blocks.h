@@ -109,6 +109,7 @@ struct BlocksArgs
     int            count;
     int            splits;  // pieces of a list, each by a workgroup of its own
     int            waves;   // of a workgroup
+    bool           pair;    // the prefill: whole lists, by two halves of a workgroup
     float          scale_log2;
     int32_t*       ws_pieces;  // the prefill's pieces of each block of query rows
     float2*        ws_ml;   // [batch * seq_len * num_heads, splits]: (max in the log2 domain, denominator)
@@ -141,6 +142,7 @@ struct BlocksLayout
     int64_t ml, acc, total;  // byte offsets in the workspace, and its size (0: none)
 };
 BlocksLayout plan_blocks(BlocksArgs& a);
+bool         blocks_pairable(const BlocksArgs& a);
 void         set_blocks_workspace(BlocksArgs& a, const BlocksLayout& l, void* ws);
 
 hipError_t launch_rope_axes(const RopeAxesArgs& a, hipStream_t stream);

@@ -23,6 +23,22 @@ void paged_blocks_prefill(ListPrefillArgs a)
     prefill_wg<QT, D, CT, false, RG, SPLIT, true, true>(a, static_cast<int>(blockIdx.x), s_st0, s_st1, s_st2, s_st3, s_flags[0]);
 }
 
+// Two halves of a list by the two halves of a workgroup (PAIR).
+template <int QT, int D, int CT, int RG>
+__global__ __launch_bounds__(1024 / RG) __attribute__((amdgpu_waves_per_eu(2)))
+void paged_blocks_prefill_pair(ListPrefillArgs a)
+{
+    using L = PrefillLds<QT, D, CT, false, RG>;
+    static_assert(2 * L::BYTES + 64 <= 160 * 1024, "both halves' stages");
+    __shared__ __align__(16) uint8_t s_st0[2 * L::STAGE];
+    __shared__ __align__(16) uint8_t s_st1[2 * L::STAGE];
+    __shared__ __align__(16) uint8_t s_st2[2 * L::S2];
+    __shared__ __align__(16) uint8_t s_st3[2 * L::S3];
+    __shared__ int s_flags[2 * kRuleFlags - 1];
+    prefill_wg<QT, D, CT, false, RG, false, true, true, true>(a, static_cast<int>(blockIdx.x), s_st0, s_st1, s_st2, s_st3,
+                                                              s_flags[0]);
+}
+
 namespace
 {
 
@@ -55,7 +71,12 @@ hipError_t launch_blocks_prefill_t(const ListPrefillArgs& a, hipStream_t stream)
     const dim3 grid(static_cast<unsigned>(wgs));
     const hipError_t e = list_prefill_for(a, [&]<int QT, int D, int RG>()
     {
-        if (a.n_split > 1)
+        if (a.pair)
+        {
+            if constexpr (D <= 128)
+                hipLaunchKernelGGL((paged_blocks_prefill_pair<QT, D, CT, RG>), grid, dim3(1024 / RG), 0, stream, a);
+        }
+        else if (a.n_split > 1)
             hipLaunchKernelGGL((paged_blocks_prefill<QT, D, CT, RG, true>), grid, dim3(512 / RG), 0, stream, a);
         else
             hipLaunchKernelGGL((paged_blocks_prefill<QT, D, CT, RG, false>), grid, dim3(512 / RG), 0, stream, a);

@@ -434,8 +434,11 @@ int ffkv_paged_attention_blocks(const void* q, void* out, int qo_dtype, const vo
     {
         bool capturing = false;
         if (const int rc = is_capturing(s, capturing)) return rc;
-        if (capturing)
-            a.splits = 1;  // whole lists need no workspace
+        if (capturing)  // whole lists need no workspace
+        {
+            a.splits = 1;
+            a.pair = ffkv::blocks_pairable(a);
+        }
         else if (const int rc = take_memory(&ws, lay.total, s))
             return rc;
     }

@@ -124,6 +124,7 @@ struct ListPrefillArgs : ScoredPrefillArgs
     int            lists;
     int            count;
     int            query_block;
+    bool           pair;  // whole lists, by two halves of a workgroup (head_dim 64 and 128)
 };
 
 struct DecodeArgs

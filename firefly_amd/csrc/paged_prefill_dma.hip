@@ -362,12 +362,16 @@ struct PrefillLds
 // never reaches it, infinite and NaN values included (s_vover is then the first of kRuleFlags ints in LDS).
 // LIST: every block of a.query_block tokens of a row has a list of pages per KV head and attends those alone (a rule without
 // a cap, a bias or ranges: its pages are masked and its strange values kept apart as a rule's are).
-template <int QT, int D, int CT, bool PFX, int RG, bool SPLIT = false, bool RULE = false, bool LIST = false>
+// PAIR: the workgroup has twice the waves, and the second half of them takes the second half of the steps, over stages of its
+// own behind the first half's (each array twice the size; s_vover is the first of 2 kRuleFlags - 1 ints); their states meet in
+// the stages.  Both halves pass the same barriers.
+template <int QT, int D, int CT, bool PFX, int RG, bool SPLIT = false, bool RULE = false, bool LIST = false, bool PAIR = false>
 __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillArgs, PrefillKernelArgs<RULE>> a, int wg_index,
                                            uint8_t* s_st0, uint8_t* s_st1, uint8_t* s_st2, uint8_t* s_st3, int& s_vover)
 {
     static_assert(!LIST || (RULE && !PFX), "lists are masked as a rule's ranges are");
-    constexpr int  W = 8 / RG;  // waves per workgroup
+    static_assert(!PAIR || (LIST && !SPLIT), "halves of lists that are whole");
+    constexpr int  W = 8 / RG;  // waves per workgroup (PAIR: per half)
     constexpr int  EB = kElemBytes<CT>;
     constexpr bool Q8 = EB == 1;
     // int8 codes are exact in bf16 and f16 alike; beside a bf16 q they take f16 products (QX16 below) unless
@@ -414,11 +418,22 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
     static_assert(PrefillLds<QT, D, CT, PFX, RG>::STAGE == 2 * C::TILEB + C::SCB, "stage layout");
     // s_vover: some accumulator is not finite after the f16 PV products (bf16 and int8 pages)
 
-    const int tid = threadIdx.x;
+    const int half = PAIR ? __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * W)) : 0;
+    const int tid = PAIR ? threadIdx.x % (64 * W) : threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (tid == 0) s_vover = 0;
-    if (RULE && tid < kRuleFlags) (&s_vover)[tid] = 0;
+    if (RULE && tid < kRuleFlags) (&s_vover + half * (kRuleFlags - 1))[tid] = 0;
+    uint8_t* const s_pair = s_st0;  // PAIR: both halves' first stages, and their second ones
+    uint8_t* const s_pair_ml = s_st1;
+    if constexpr (PAIR)
+    {
+        using PL = PrefillLds<QT, D, CT, PFX, RG>;
+        s_st0 += half * PL::STAGE;
+        s_st1 += half * PL::STAGE;
+        s_st2 += half * PL::S2;
+        s_st3 += half * PL::S3;
+    }
     const int c = lane & 15;
     const int g = lane >> 4;
     // Workgroup -> (group, row block).  A group is (row b, kv head) for prefill and (kv head, chunk of prefix
@@ -657,10 +672,17 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
             pg_hi = min(pg_hi, pg0 + static_cast<int>(static_cast<int64_t>(st) * (piece + 1) / np) * KP);
         }
     }
+    int pair_steps = 0;  // PAIR: of both halves, the longer's (a step past a half's pages has none)
+    if constexpr (PAIR)
+    {
+        pair_steps = ((pg_hi + KP - 1) / KP + 1) / 2;
+        pg_lo = half * pair_steps * KP;
+        pg_hi = half != 0 ? pg_hi : min(pg_hi, pair_steps * KP);
+    }
     // uniform values computed through divisions: keep them scalar so the loop's branches stay scalar
     pg_lo = __builtin_amdgcn_readfirstlane(pg_lo);
     pg_hi = __builtin_amdgcn_readfirstlane(pg_hi);
-    const int  steps = pg_hi > pg_lo ? (pg_hi - pg_lo + KP - 1) / KP : 0;
+    const int  steps = PAIR ? __builtin_amdgcn_readfirstlane(pair_steps) : pg_hi > pg_lo ? (pg_hi - pg_lo + KP - 1) / KP : 0;
     const bool wave_active = row0 + 16 * RG * wave < R;
 
     // ---- Q^T operands of the wave's RG x 16 query rows -----------------------------------------------------
@@ -1412,7 +1434,7 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
     // wave takes the infinite and NaN values out of the V runs it loaded, and marks the stage with its step where there
     // were any; the queries that do see such a key then add them one by one (add_bad).  int8 codes are always finite.
     constexpr bool CAN_CF = RULE && CT != I8;
-    FFKV_LDS int* const s_bad = RULE ? (FFKV_LDS int*)&s_vover + 1 : nullptr;
+    FFKV_LDS int* const s_bad = RULE ? (FFKV_LDS int*)&s_vover + 1 + half * (kRuleFlags - 1) : nullptr;
     auto clean_v = [&](uint8_t* stage, int si)
     {
         bool bad = false;
@@ -1650,6 +1672,65 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
         pipeline.template operator()<false, false>();
     }
 
+    if constexpr (PAIR)
+    {
+        // the second half's states through the stages, some output tiles of all rows at a time, and the first half's output
+        constexpr int STAGE2 = 2 * PrefillLds<QT, D, CT, PFX, RG>::STAGE;
+        constexpr int NPR = NT < STAGE2 / (kDmaRows * 64) ? NT : STAGE2 / (kDmaRows * 64);  // tiles of 16 dims of a round
+        static_assert(NT % NPR == 0 && STAGE2 >= kDmaRows * 8, "whole rounds; the (max, denominator) pairs fit");
+        f32x4*  s_o = reinterpret_cast<f32x4*>(s_pair);
+        float2* s_s = reinterpret_cast<float2*>(s_pair_ml);
+        float   w0[RG], w1[RG], inv[RG];
+        wait_lgkm0();
+        __builtin_amdgcn_s_barrier();  // every wave is past its last reads of the stages
+#pragma unroll
+        for (int n0 = 0; n0 < NT; n0 += NPR)
+        {
+            if (n0 > 0)
+            {
+                wait_lgkm0();
+                __builtin_amdgcn_s_barrier();  // the round before is read
+            }
+            if (half != 0)
+            {
+#pragma unroll
+                for (int gi = 0; gi < RG; ++gi)
+                {
+                    const int rg = RG * wave + gi;
+#pragma unroll
+                    for (int n = 0; n < NPR; ++n) s_o[(rg * NPR + n) * 64 + lane] = acc[gi][n0 + n];
+                    const float l_tot = swap_sum(l_run[gi]) + lacc[gi][0];
+                    if (n0 == 0 && g == 0)
+                        s_s[16 * rg + c] = float2{m_run[gi] == kNegInf ? kNegInf : m_run[gi] * c_log2, l_tot};
+                }
+            }
+            wait_lgkm0();
+            __builtin_amdgcn_s_barrier();
+            if (half != 0) continue;
+#pragma unroll
+            for (int gi = 0; gi < RG; ++gi)
+            {
+                const int rg = RG * wave + gi;
+                if (n0 == 0)
+                {
+                    const float  l_tot = swap_sum(l_run[gi]) + lacc[gi][0];
+                    const float  m0 = m_run[gi] == kNegInf ? kNegInf : m_run[gi] * c_log2;
+                    const float2 other = s_s[16 * rg + c];
+                    const float  m = fmaxf(fmaxf(m0, other.x), kLowest);
+                    w0[gi] = __builtin_amdgcn_exp2f(m0 - m);
+                    w1[gi] = __builtin_amdgcn_exp2f(other.x - m);
+                    inv[gi] = softmax_inv(l_tot * w0[gi] + other.y * w1[gi], v_head_scale);
+                }
+                if (!col_ok[gi]) continue;
+                const size_t ob = qrow[gi] * D;
+#pragma unroll
+                for (int n = 0; n < NPR; ++n)
+                    store_out4<QT>(a.out, ob + 16 * (n0 + n) + 4 * g,
+                                   (acc[gi][n0 + n] * w0[gi] + s_o[(rg * NPR + n) * 64 + lane] * w1[gi]) * inv[gi]);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int gi = 0; gi < RG; ++gi)
     {

@@ -219,3 +219,46 @@ def test_split_hidden_values(ff, gpu, act, kv):
     got = su.host(run(ff, c, li, 12, gpu)).reshape(want.shape)
     su.check(got[:, :8], want[:, :8], bound[:, :8], "before")
     assert not np.isfinite(got[:, 8:]).any()
+
+
+@pytest.mark.parametrize("act,kv", KV)
+@pytest.mark.parametrize("Hq,Hkv,D,ctx,S,count,T", [
+    (36, 9, 128, [1100, 1300], 120, 61, 16), (24, 12, 64, [1700, 900], 130, 107, 16), (50, 10, 128, [1600, 1], 70, 97, 7),
+    (8, 2, 128, [300, 0, 90], 60, 16, 30), (4, 4, 64, [700], 17, 31, 4),
+])
+def test_lists_in_halves(ff, gpu, act, kv, Hq, Hkv, D, ctx, S, count, T):
+    """At most as many blocks of queries as half fills the chip, or short lists: a list's halves by those of a workgroup."""
+    c = make(Hq + D, ctx, S, Hq, Hkv, D, act, kv)
+    check(ff, c, lists(c, S, count, T, shuffle=True), T, gpu)
+
+
+@pytest.mark.parametrize("act,kv", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "fp8"), ("bf16", "i8")])
+@pytest.mark.parametrize("place", [3, 90])
+def test_halves_hidden_values(ff, gpu, act, kv, place):
+    """As test_split_hidden_values, the strange values in one half of the first list."""
+    c = make(79, [2000, 1700], 100, 40, 10, 128, act, kv)
+    li = lists(c, 100, 100, 10)
+    li[0, 0][li[0, 0] == 125] = -1
+    li[0, 0, :, place] = 125
+    li[0, 1:][li[0, 1:] == 125] = -1
+    q = cases.decode(c.q, c.act).astype(np.float64)
+    want, bound = bu.attend(c, q, li, 10, c.act, 100, 2.0 ** -10)
+    for t in range(2008, 2016):  # seen by the first list's queries from the eighth on
+        su.poison(c, 0, t)
+    got = su.host(run(ff, c, li, 10, gpu)).reshape(want.shape)
+    seen = np.zeros((2, 100), bool)
+    seen[0, 8:10] = True
+    su.check(got[~seen], want[~seen], bound[~seen], "others")
+    assert not np.isfinite(got[seen]).any()
+
+
+@pytest.mark.parametrize("S,T,ctx,count", [(100, 10, [2000, 1700], 100), (12, 12, [2000], 120), (20, 20, [200], 12)])
+def test_int8_large_values(ff, gpu, S, T, ctx, count):
+    """int8 V scales past 256 take the products again in a smaller scale, whichever part of the list they lie in."""
+    c = make(80, ctx, S, 40, 10, 128, "bf16", "i8")
+    c.v_scale[int(c.block_table[0, 2])] *= np.float32(20000)
+    li = lists(c, S, count, T)
+    li[0, :, :, 0] = 2
+    li[0, :, :, 1:][li[0, :, :, 1:] == 2] = -1
+    got = check(ff, c, li, T, gpu)
+    assert np.isfinite(got).all() and np.abs(got[0]).max() > 1e3
