@@ -180,23 +180,25 @@ struct PageBounds
 
 }  // namespace
 
-// A step (a few query rows, one block of them).  The rounds of ROUND pages of all rows and KV heads form one sequence, of
-// which every workgroup takes an equal share, as many workgroups as fit the chip: rows of 125 to 1000 pages in tiles of their
-// own left it waiting for the longest (64 rows, 8 heads: 38 us, 28 so).  LPP lanes take four neighbouring pages' bounds, 8
-// dims each, and every lane adds up its dims of the queries by itself; while a round is added up the next one's bounds are on
-// their way, and the table's entries of the one after.
+// A step (a few query rows, one block of them).  A round is ROUND pages of `heads` KV heads, whose bounds of a page lie
+// together (64 rows of 125 to 1000 pages, 8 heads, 148 MB from memory: 41.5 us with one head a round, 39.5 with two, 39.1 with
+// four, 38.9 with eight, the choice's 5 among them).  The rounds of all rows and heads form one sequence, of which every
+// workgroup takes an equal share, as many workgroups as fit the chip: tiles of their own left it waiting for the longest row
+// (57.5 us in all).  LPP lanes take four neighbouring pages' bounds, 8 dims each, and every lane adds up its dims of the
+// queries by itself; while a round is added up the next one's bounds are on their way, and the table's entries of the one
+// after.  Bound by HBM: about 4.7 TB/s behind a start of 3 us (4 rows of 8188 pages, 4 heads, 67 MB: 15.5 us).
 template <int BT, int QT, int LPP, bool FULL>
-__global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a)
+__global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a, int heads)
 {
-    constexpr int ROUND = kScoreThreads / LPP * kScorePages;  // pages of a round
+    const int  ROUND = kScoreThreads / LPP * kScorePages / heads;  // pages of a round
     const int  tid = static_cast<int>(threadIdx.x);
     const int  lane = tid & 63;
-    const int  c = tid % LPP, grp = tid / LPP;
+    const int  c = tid % LPP, grp = tid / LPP / heads, hd = tid / LPP % heads;
     const bool in = FULL || 8 * c < a.head_dim;
     auto rounds_of = [&](int b) { return (visible_pages(a, b, 0) + ROUND - 1) / ROUND; };
 
     // this workgroup's share (every wave on its own)
-    const int H = a.num_kv_heads;
+    const int H = a.num_kv_heads / heads;  // blocks of heads
     int64_t   total = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64)
         total += uniform(wave_sum(b0 + lane < a.batch ? rounds_of(b0 + lane) : 0));
@@ -215,10 +217,10 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a)
         x0 = blockIdx.x * total / wgs;
         x1 = (blockIdx.x + 1) * total / wgs;
     }
-    // its first round: row, KV head, round of the row
+    // its first round: row, block of heads, round of the row
     struct Place
     {
-        int b, kvh, round, rounds;
+        int b, hb, round, rounds;
     };
     Place at{0, 0, 0, 0};
     {
@@ -235,8 +237,8 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a)
                 at.b = b0 + l;
                 at.rounds = __builtin_amdgcn_readlane(r, l);
                 const int off = static_cast<int>(x0 - base) - __builtin_amdgcn_readlane(upto - r, l) * H;
-                at.kvh = off / at.rounds;
-                at.round = off - at.kvh * at.rounds;
+                at.hb = off / at.rounds;
+                at.round = off - at.hb * at.rounds;
                 break;
             }
             base += static_cast<int64_t>(__builtin_amdgcn_readlane(upto, 63)) * H;
@@ -246,8 +248,8 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a)
     {
         if (++p.round < p.rounds) return p;
         p.round = 0;
-        if (++p.kvh < H) return p;
-        p.kvh = 0;
+        if (++p.hb < H) return p;
+        p.hb = 0;
         do
             p.rounds = ++p.b < a.batch ? rounds_of(p.b) : 1;
         while (p.rounds == 0);
@@ -271,7 +273,7 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a)
             Raw8 q[QROWS];
 #pragma unroll
             for (int u = 0; u < QROWS; ++u)
-                if (r0 + u < rows && in) load_raw8<QT>(a.q, query_at(a, p.b, 0, p.kvh, r0 + u, c), q[u]);
+                if (r0 + u < rows && in) load_raw8<QT>(a.q, query_at(a, p.b, 0, p.hb * heads + hd, r0 + u, c), q[u]);
 #pragma unroll
             for (int u = 0; u < QROWS; ++u)
                 if (r0 + u < rows && in)
@@ -285,12 +287,12 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a)
     Place ahead = next(at);
     entries(at);
     PageBounds<BT, LPP, FULL> cur, nxt;
-    cur.load(a, phys, at.kvh, c);
+    cur.load(a, phys, at.hb * heads + hd, c);
     if (x0 + 1 < x1) entries(ahead);
     sum_queries(at);
     for (int64_t x = x0; x < x1; ++x)
     {
-        if (x + 1 < x1) nxt.load(a, phys, ahead.kvh, c);
+        if (x + 1 < x1) nxt.load(a, phys, ahead.hb * heads + hd, c);
         const Place after = next(ahead);
         if (x + 2 < x1) entries(after);
         double s[kScorePages];
@@ -303,10 +305,10 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a)
         }
         const double sum = group_sums4<LPP>(s, c);
         const int    p = at.round * ROUND + grp * kScorePages + (c & 3);
-        float*       out = a.scores + (static_cast<int64_t>(at.b) * H + at.kvh) * a.stride;
+        float*       out = a.scores + (static_cast<int64_t>(at.b) * a.num_kv_heads + at.hb * heads + hd) * a.stride;
         // (behind the row's last page up to stride: read by nobody)
         if (c < 4 && p < a.most_pages) out[p] = cur.on >> c & 1 ? static_cast<float>(sum) : kNegInf;  // on no page: last
-        if (x + 1 < x1 && (ahead.b != at.b || ahead.kvh != at.kvh)) sum_queries(ahead);
+        if (x + 1 < x1 && (ahead.b != at.b || ahead.hb != at.hb)) sum_queries(ahead);
         cur = nxt;
         at = ahead;
         ahead = after;
@@ -641,10 +643,13 @@ hipError_t launch_scores_l(const SelectArgs& a, hipStream_t stream)
     const int64_t all = (a.most_pages + ROUND - 1) / ROUND;  // rounds of a row
     if (!select_by_lists(a.seq_len, a.lists, a.group))
     {
+        int heads = 1;  // whose bounds of a page a round takes: they lie together
+        while (heads < 8 && a.num_kv_heads % (2 * heads) == 0) heads *= 2;
         const void*   kernel = reinterpret_cast<const void*>(block_scores_step<BT, QT, LPP, FULL>);
-        const int64_t wgs = std::min<int64_t>(decode_mfma_items(kernel, kScoreThreads, 1), rows * all);
+        const int64_t most = rows / heads * ((a.most_pages + ROUND / heads - 1) / (ROUND / heads));  // rounds of all
+        const int64_t wgs = std::min<int64_t>(decode_mfma_items(kernel, kScoreThreads, 1), most);
         hipLaunchKernelGGL((block_scores_step<BT, QT, LPP, FULL>), dim3(static_cast<unsigned>(wgs)), dim3(kScoreThreads), 0,
-                           stream, a);
+                           stream, a, heads);
         return hipGetLastError();
     }
     hipLaunchKernelGGL((block_queries<QT, LPP>), dim3(static_cast<unsigned>(rows * a.lists)), dim3(kSumThreads), 0, stream, a);
