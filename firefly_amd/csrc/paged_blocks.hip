@@ -89,8 +89,8 @@ void paged_blocks_decode(BlocksArgs a)
     using M = MType<BF>;
     using MV = MType<VBF>;
     using X8 = typename M::x8;
-    static_assert(D % 32 == 0, "whole k-steps of 32 dims");
-    constexpr int  KSTEPS = D / 32;
+    static_assert(D % 16 == 0, "whole output tiles of 16 dims");
+    constexpr int  KSTEPS = (D + 31) / 32;  // of 32 dims; head_dim 80 and 112 leave lanes of the last without any
     constexpr int  NT = D / 16;
     constexpr bool NEED_LO = !((QT == BF16 && BF) || (QT == F16 && !BF));
     constexpr bool P_LO = VBF;
@@ -105,6 +105,7 @@ void paged_blocks_decode(BlocksArgs a)
             if (j == KSTEPS - 1) return 32 * j + 8 * g;
         return dim_of<CT>(j, g);
     };
+    auto has = [&](int j, int g) { return D % 32 == 0 || dimof(j, g) < D; };
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int wave = uniform(static_cast<int>(threadIdx.x) >> 6);
     const int c = lane & 15;
@@ -113,13 +114,14 @@ void paged_blocks_decode(BlocksArgs a)
     const int HB = (G + 15) >> 4;
     const Split u = split_index(blockIdx.x, a.splits), v = split_index(u.div, a.num_kv_heads * HB);
     const Split w = split_index(v.div, a.seq_len);
-    const int     split = u.rem, vh = v.rem, b = static_cast<int>(w.div);
+    const int     split = u.rem, vh = v.rem, b = static_cast<int>(w.div), t = w.rem;
     const int64_t row = v.div;  // b * seq_len + t
+    const int64_t rl = a.query_block == 1 ? row : static_cast<int64_t>(b) * a.lists + t / a.query_block;
     const int     kvh = vh / HB;
     const int     h0 = (vh - kvh * HB) * 16;
     const int     gc = min(16, G - h0);
-    const int64_t pos = static_cast<int64_t>(a.context_lens[b]) + w.rem;
-    const int32_t* list = a.blocks + (row * a.num_kv_heads + kvh) * a.count;
+    const int64_t pos = static_cast<int64_t>(a.context_lens[b]) + t;
+    const int32_t* list = a.blocks + (rl * a.num_kv_heads + kvh) * a.count;
     const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
     // this wave's entries: begin + WAVES i, i < n
     const int begin = static_cast<int>(static_cast<int64_t>(a.count) * split / a.splits) + wave;
@@ -171,13 +173,19 @@ void paged_blocks_decode(BlocksArgs a)
         if constexpr (EB == 2)
         {
 #pragma unroll
-            for (int j = 0; j < KSTEPS; ++j) r.k[j] = *reinterpret_cast<const u32x4*>(kp + dim_of<CT>(j, g) * 2);
+            for (int j = 0; j < KSTEPS; ++j)
+            {
+                r.k[j] = u32x4{0u, 0u, 0u, 0u};
+                if (has(j, g)) r.k[j] = *reinterpret_cast<const u32x4*>(kp + dim_of<CT>(j, g) * 2);
+            }
         }
         else
         {
 #pragma unroll
             for (int j = 0; j < KSTEPS; j += 2)
             {
+                r.k[j / 2] = u32x4{0u, 0u, 0u, 0u};
+                if (!has(j, g)) continue;
                 if (j + 1 < KSTEPS)
                     r.k[j / 2] = *reinterpret_cast<const u32x4*>(kp + dimof(j, g));
                 else  // an odd last k-step: its 8 codes alone
@@ -203,7 +211,7 @@ void paged_blocks_decode(BlocksArgs a)
         if constexpr (!NEED_LO)
         {
             u32x4 w = u32x4{0u, 0u, 0u, 0u};
-            if (c < gc) w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
+            if (c < gc && has(j, g)) w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
             qhi[j] = qlo[j] = __builtin_bit_cast(X8, w);
         }
         else
@@ -211,7 +219,7 @@ void paged_blocks_decode(BlocksArgs a)
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-            if (c < gc) load_q8<QT>(a.q, at, x);
+            if (c < gc && has(j, g)) load_q8<QT>(a.q, at, x);
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -601,7 +609,7 @@ __global__ __launch_bounds__(64 * kBlocksWaves) void paged_blocks_vector(BlocksA
 namespace
 {
 
-bool mfma_dim(int d) { return d == 64 || d == 96 || d == 128 || d == 256; }
+bool mfma_dim(int d) { return d == 64 || d == 80 || d == 96 || d == 112 || d == 128 || d == 256; }
 
 // Workgroups of a token in an unsplit call: KV heads, and blocks of their query heads.
 int64_t blocks_heads(const BlocksArgs& a)
@@ -641,8 +649,9 @@ hipError_t for_types(const BlocksArgs& a, F f)
 BlocksKernel blocks_kernel(const BlocksArgs& a)
 {
     if (a.cache_dtype == F32 || !mfma_dim(a.head_dim)) return BlocksKernel::kVector;
-    if (a.query_block == 1) return BlocksKernel::kDecode;
-    return a.head_dim == 96 ? BlocksKernel::kVector : BlocksKernel::kPrefill;
+    // (the prefill has no form of head_dim 80, 96 and 112: their lists are attended token by token)
+    const bool prefill = a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256;
+    return a.query_block > 1 && prefill ? BlocksKernel::kPrefill : BlocksKernel::kDecode;
 }
 
 namespace
@@ -793,7 +802,9 @@ hipError_t launch_blocks(const BlocksArgs& a, hipStream_t stream)
                 return hipGetLastError();
             };
             if (a.head_dim == 64) return go.template operator()<64>();
+            if (a.head_dim == 80) return go.template operator()<80>();
             if (a.head_dim == 96) return go.template operator()<96>();
+            if (a.head_dim == 112) return go.template operator()<112>();
             if (a.head_dim == 128) return go.template operator()<128>();
             return go.template operator()<256>();
         });

@@ -59,7 +59,8 @@ KV = [("bf16", "bf16"), ("f16", "f16"), ("bf16", "i8"), ("bf16", "fp8"), ("f32",
 @pytest.mark.parametrize("Hq,Hkv,D,ctx,count", [
     (16, 8, 128, [17, 64, 100, 255], 4), (28, 4, 128, [3000], 150), (5, 1, 64, [0, 15, 16, 900], 7), (8, 8, 256, [500, 31], 20),
     (6, 2, 96, [1000, 3], 33), (3, 3, 80, [200, 400], 5), (4, 2, 112, [640], 41), (20, 1, 128, [800, 900], 30),
-    (2, 2, 8, [100], 3), (36, 2, 64, [333], 9), (32, 2, 256, [700], 40),
+    (2, 2, 8, [100], 3), (36, 2, 64, [333], 9), (32, 2, 256, [700], 40), (14, 2, 80, [1900, 1400], 90), (3, 1, 112, [33, 0], 2),
+    (21, 1, 112, [777], 25), (4, 4, 72, [100, 333], 11),
 ])
 def test_step(ff, gpu, act, kv, Hq, Hkv, D, ctx, count):
     c = make(Hq + D, ctx, 1, Hq, Hkv, D, act, kv)
@@ -70,7 +71,7 @@ def test_step(ff, gpu, act, kv, Hq, Hkv, D, ctx, count):
 @pytest.mark.parametrize("Hq,Hkv,D,ctx,S,count,T", [
     (8, 2, 128, [700, 0], 70, 12, 64), (4, 4, 64, [100], 33, 6, 16), (10, 2, 256, [300, 15], 40, 9, 40),
     (14, 2, 128, [64], 17, 3, 100), (8, 2, 128, [257], 5, 8, 2), (6, 2, 96, [90], 20, 5, 8), (32, 1, 64, [500], 9, 21, 9),
-    (4, 1, 128, [40, 300], 6, 7, 1),
+    (4, 1, 128, [40, 300], 6, 7, 1), (10, 2, 80, [300, 15], 40, 9, 16), (7, 1, 112, [64], 17, 3, 100), (6, 3, 104, [50], 9, 4, 3),
 ])
 def test_chunk(ff, gpu, act, kv, Hq, Hkv, D, ctx, S, count, T):
     c = make(Hq + S, ctx, S, Hq, Hkv, D, act, kv)
