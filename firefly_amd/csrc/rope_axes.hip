@@ -12,6 +12,9 @@
 // p * rate / 2 pi are one fp64 product; only their fraction, in [-1/2, 1/2], goes on to fp32 as a pair of parts, of which the
 // low one enters to first order: what is left is the rounding of cos and sin to fp32 and the errors of the rate, 2^-48 of
 // the angle at most: 2^-22 + |p| 2^-48 in all (theta >= 1).
+//
+// Bound by HBM (q read and written, k and v read and written once): 8 x 1500 f16 tokens of 32/8 heads of 128, 295 MB, 58.3 us =
+// 5.1 TB/s; 32000 bf16 tokens of 28/4 heads, 590 MB, 104 us = 5.7 TB/s (a copy reaches 5.1).  A step of 4 tokens takes 3.5 us.
 #include "blocks.h"
 #include "ffkv_device.h"
 
@@ -65,11 +68,11 @@ __device__ __forceinline__ float row_scale(const float* scales, int h, const flo
 
 }  // namespace
 
-// A wave takes a token, or a part of its head rows: its lanes evaluate the token's cos and sin, a pair each (head_dim 256:
-// two), and exchange them through the wave's own stretch of LDS, without a barrier; then D/16 lanes rotate a head row, each
-// its 8 dims of the low half and the matching 8 of the high half, PASS rows of 64 / (D/16) at a time with all their loads
-// in flight.
-template <int SRC, int CACHE, int D, bool APPEND, int PASS>
+// A wave takes 64 / (D/16) head rows of a token: its lanes evaluate the token's cos and sin, a pair each (head_dim 256: two), and
+// exchange them through the wave's own stretch of LDS, without a barrier; then D/16 lanes rotate a head row, each its 8 dims of
+// the low half and the matching 8 of the high half.  (A token's other waves evaluate the same table again, behind their
+// loads: twice or three times the rows a wave take as long for 4 tokens, and 59.1 and 60.7 us instead of 58.3 for 12000.)
+template <int SRC, int CACHE, int D, bool APPEND>
 __global__ __launch_bounds__(kRopeThreads) void rope_axes_kernel(RopeAxesArgs a, int parts)
 {
     constexpr int HALF = D / 2;
@@ -106,7 +109,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_axes_kernel(RopeAxesArgs a,
 
     for (uint32_t item = blockIdx.x * (kRopeThreads / 64) + wave; item < items; item += gridDim.x * (kRopeThreads / 64))
     {
-        // (a token's parts lie side by side: apart, its rows' lines are fetched twice, 64 -> 69 us for 12000 tokens)
+        // (a token's parts lie side by side: apart, its rows' lines are fetched twice, 61 -> 69 us for 12000 tokens)
         const Split    v = split_index(item, parts), u = split_index(v.div, a.seq_len);
         const uint32_t tok = v.div;
         const int      part = v.rem, b = static_cast<int>(u.div), t = u.rem;
@@ -124,24 +127,22 @@ __global__ __launch_bounds__(kRopeThreads) void rope_axes_kernel(RopeAxesArgs a,
                 if (phys >= 0 && phys < a.num_blocks) slot = static_cast<int64_t>(phys) * kBlockSize + (pos & 15);
             }
         }
-        const int r0 = part * PASS * RPP;
-        Raw8 rl[PASS], rh[PASS], vl[PASS], vh[PASS];
-#pragma unroll
-        for (int k = 0; k < PASS; ++k)
+        const int  row = part * RPP + sub;
+        const bool in = row < rows;
+        const bool isq = row < a.num_heads;
+        const int  h = isq ? row : row - a.num_heads;
+        Raw8       rl, rh, vl, vh;
+        if (in)
         {
-            const int row = r0 + k * RPP + sub;
-            if (row >= rows) continue;
-            const bool   isq = row < a.num_heads;
-            const int    h = isq ? row : row - a.num_heads;
             const size_t at8 = static_cast<size_t>(tok) * (isq ? a.q_stride : a.k_stride) + h * D + 8 * col;
             const void*  src = isq ? a.q : a.k;
-            load_raw8<SRC>(src, at8, rl[k]);
-            load_raw8<SRC>(src, at8 + HALF, rh[k]);
+            load_raw8<SRC>(src, at8, rl);
+            load_raw8<SRC>(src, at8 + HALF, rh);
             if (APPEND && !isq)
             {
                 const size_t v8 = static_cast<size_t>(tok) * a.v_stride + h * D + 8 * col;
-                load_raw8<SRC>(a.v, v8, vl[k]);
-                load_raw8<SRC>(a.v, v8 + HALF, vh[k]);
+                load_raw8<SRC>(a.v, v8, vl);
+                load_raw8<SRC>(a.v, v8 + HALF, vh);
             }
         }
         // the token's table, behind the loads
@@ -170,74 +171,66 @@ __global__ __launch_bounds__(kRopeThreads) void rope_axes_kernel(RopeAxesArgs a,
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-        for (int k = 0; k < PASS; ++k)
+        float xl[8], xh[8], yl[8], yh[8];
+        if (in)
         {
-            const int  row = r0 + k * RPP + sub;
-            const bool in = row < rows;
-            const bool isq = row < a.num_heads;
-            const int  h = isq ? row : row - a.num_heads;
-            float      xl[8], xh[8], yl[8], yh[8];
-            if (in)
-            {
-                unpack8<SRC>(rl[k], xl);
-                unpack8<SRC>(rh[k], xh);
+            unpack8<SRC>(rl, xl);
+            unpack8<SRC>(rh, xh);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < 8; ++e)
+            {
+                yl[e] = __builtin_fmaf(xl[e], c8[e], -(xh[e] * s8[e]));
+                yh[e] = __builtin_fmaf(xh[e], c8[e], xl[e] * s8[e]);
+            }
+            pack8<SRC>(yl, rl);
+            pack8<SRC>(yh, rh);
+            if (isq || a.k_out != nullptr)
+            {
+                void*        dst = isq ? a.q_out : a.k_out;
+                const size_t at8 = static_cast<size_t>(tok) * (isq ? a.q_out_stride : a.k_out_stride) + h * D + 8 * col;
+                store_raw8<SRC>(dst, at8, rl);
+                store_raw8<SRC>(dst, at8 + HALF, rh);
+            }
+        }
+        if constexpr (APPEND)
+        {
+            const bool   go = in && !isq && slot >= 0;
+            const size_t row_c = static_cast<size_t>(go ? slot : 0) * a.num_kv_heads + (go ? h : 0);
+            if constexpr (SRC == CACHE)
+            {
+                if (go)
                 {
-                    yl[e] = __builtin_fmaf(xl[e], c8[e], -(xh[e] * s8[e]));
-                    yh[e] = __builtin_fmaf(xh[e], c8[e], xl[e] * s8[e]);
-                }
-                pack8<SRC>(yl, rl[k]);
-                pack8<SRC>(yh, rh[k]);
-                if (isq || a.k_out != nullptr)
-                {
-                    void*        dst = isq ? a.q_out : a.k_out;
-                    const size_t at8 = static_cast<size_t>(tok) * (isq ? a.q_out_stride : a.k_out_stride) + h * D + 8 * col;
-                    store_raw8<SRC>(dst, at8, rl[k]);
-                    store_raw8<SRC>(dst, at8 + HALF, rh[k]);
+                    store_raw8<CACHE>(a.k_cache, row_c * D + 8 * col, rl);
+                    store_raw8<CACHE>(a.k_cache, row_c * D + HALF + 8 * col, rh);
+                    store_raw8<CACHE>(a.v_cache, row_c * D + 8 * col, vl);
+                    store_raw8<CACHE>(a.v_cache, row_c * D + HALF + 8 * col, vh);
                 }
             }
-            if constexpr (APPEND)
+            else if (__any(go))  // (the rows' maxima take every lane)
             {
-                const bool   go = in && !isq && slot >= 0;
-                const size_t row_c = static_cast<size_t>(go ? slot : 0) * a.num_kv_heads + (go ? h : 0);
-                if constexpr (SRC == CACHE)
+                if (!go)
                 {
-                    if (go)
-                    {
-                        store_raw8<CACHE>(a.k_cache, row_c * D + 8 * col, rl[k]);
-                        store_raw8<CACHE>(a.k_cache, row_c * D + HALF + 8 * col, rh[k]);
-                        store_raw8<CACHE>(a.v_cache, row_c * D + 8 * col, vl[k]);
-                        store_raw8<CACHE>(a.v_cache, row_c * D + HALF + 8 * col, vh[k]);
-                    }
-                }
-                else if (__any(go))  // (the rows' maxima take every lane)
-                {
-                    if (!go)
-                    {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) rl[k].w[e] = rh[k].w[e] = vl[k].w[e] = vh[k].w[e] = 0u;
-                    }
-                    // k as stored in its own type: what an append of the rotated k reads
-                    unpack8<SRC>(rl[k], xl);
-                    unpack8<SRC>(rh[k], xh);
-                    unpack8<SRC>(vl[k], yl);
-                    unpack8<SRC>(vh[k], yh);
-                    const float ks = row_scale<CACHE, LPR>(a.k_scale, go ? h : 0, xl, xh);
-                    const float vs = row_scale<CACHE, LPR>(a.v_scale, go ? h : 0, yl, yh);
-                    if (go)
+                    for (int e = 0; e < 8; ++e) rl.w[e] = rh.w[e] = vl.w[e] = vh.w[e] = 0u;
+                }
+                // k as stored in its own type: what an append of the rotated k reads
+                unpack8<SRC>(rl, xl);
+                unpack8<SRC>(rh, xh);
+                unpack8<SRC>(vl, yl);
+                unpack8<SRC>(vh, yh);
+                const float ks = row_scale<CACHE, LPR>(a.k_scale, go ? h : 0, xl, xh);
+                const float vs = row_scale<CACHE, LPR>(a.v_scale, go ? h : 0, yl, yh);
+                if (go)
+                {
+                    if (CACHE == I8 && col == 0)
                     {
-                        if (CACHE == I8 && col == 0)
-                        {
-                            a.k_scale[row_c] = ks;
-                            a.v_scale[row_c] = vs;
-                        }
-                        store_cache8<CACHE>(a.k_cache, row_c * D + 8 * col, xl, ks);
-                        store_cache8<CACHE>(a.k_cache, row_c * D + HALF + 8 * col, xh, ks);
-                        store_cache8<CACHE>(a.v_cache, row_c * D + 8 * col, yl, vs);
-                        store_cache8<CACHE>(a.v_cache, row_c * D + HALF + 8 * col, yh, vs);
+                        a.k_scale[row_c] = ks;
+                        a.v_scale[row_c] = vs;
                     }
+                    store_cache8<CACHE>(a.k_cache, row_c * D + 8 * col, xl, ks);
+                    store_cache8<CACHE>(a.k_cache, row_c * D + HALF + 8 * col, xh, ks);
+                    store_cache8<CACHE>(a.v_cache, row_c * D + 8 * col, yl, vs);
+                    store_cache8<CACHE>(a.v_cache, row_c * D + HALF + 8 * col, yh, vs);
                 }
             }
         }
@@ -252,19 +245,12 @@ hipError_t launch_axes_d(const RopeAxesArgs& a, hipStream_t stream)
 {
     constexpr int RPP = 64 / (D / 16);
     const int64_t tokens = static_cast<int64_t>(a.batch) * a.seq_len;
-    const int     passes = (a.num_heads + a.num_kv_heads + RPP - 1) / RPP;
-    auto go = [&]<int PASS>()
-    {
-        const int     parts = (passes + PASS - 1) / PASS;
-        const int64_t wgs = (tokens * parts + kRopeThreads / 64 - 1) / (kRopeThreads / 64);
-        if (tokens * parts > INT32_MAX) return hipErrorInvalidConfiguration;
-        hipLaunchKernelGGL((rope_axes_kernel<SRC, CACHE, D, APPEND, PASS>),
-                           dim3(static_cast<unsigned>(std::min<int64_t>(wgs, 16384))), dim3(kRopeThreads), 0, stream, a, parts);
-        return hipGetLastError();
-    };
-    // few tokens: a wave per pass, so that a step's rows spread over the chip
-    if (tokens * passes <= 8192) return go.template operator()<1>();
-    return go.template operator()<3>();
+    const int     parts = (a.num_heads + a.num_kv_heads + RPP - 1) / RPP;
+    const int64_t wgs = (tokens * parts + kRopeThreads / 64 - 1) / (kRopeThreads / 64);
+    if (tokens * parts > INT32_MAX) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((rope_axes_kernel<SRC, CACHE, D, APPEND>), dim3(static_cast<unsigned>(std::min<int64_t>(wgs, 65536))),
+                       dim3(kRopeThreads), 0, stream, a, parts);
+    return hipGetLastError();
 }
 
 template <int SRC, int CACHE, bool APPEND>

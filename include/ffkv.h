@@ -404,16 +404,18 @@ FFKV_API int ffkv_evict(const float* weights, int64_t weight_stride, const int32
 /*
  * Rotary embedding by positions on several axes (time, height and width of image and video tokens).  Pair i of a head (dims
  * i, i + head_dim/2) of token t of row b turns by positions[axis(i)][b][t] * rope_theta^(-2i/head_dim), in ffkv_rope's form;
- * with equal positions on all axes that is ffkv_rope's rotation.  positions int32 [axes, batch, seq_len]; axes 1 to
- * 4; sections (host memory): the pairs of dims of each axis, head_dim/2 together.  interleaved 0: the first sections[0] pairs
- * turn by axis 0, the next sections[1] by axis 1, ..; else pair i turns by axis i % axes while that axis has pairs left
- * (sections[a] of the pairs a, a + axes, ..), all others by axis 0.  The turns are one fp64 product, whose fraction enters cos
- * and sin: good to 2^-22 + |position| * 2^-48 (rope_theta >= 1).  (ffkv_rope rounds its angle to fp32: far positions differ by 2^-24 of the angle.)
+ * with equal positions on all axes that is ffkv_rope's rotation.  positions int32 [axes, batch, seq_len]; axes 1 to 4; sections
+ * (host memory): the pairs of dims of each axis, head_dim/2 together.  interleaved 0: the first sections[0] pairs turn by axis 0,
+ * the next sections[1] by axis 1, ..; else pair i turns by axis i % axes while that axis has pairs left (sections[a] of the
+ * pairs a, a + axes, ..), all others by axis 0.  The turns are one fp64 product, whose fraction enters cos and sin: good to
+ * 2^-22 + |position| * 2^-48 (rope_theta >= 1).  (ffkv_rope rounds its angle to fp32: far positions differ by 2^-24 of the
+ * angle.)
  *
  * q [batch, seq_len, num_heads, head_dim] (NULL: none) and k [batch, seq_len, num_kv_heads, head_dim] of one dtype (F32, F16,
  * BF16), head_dim 64, 128 or 256; q_stride etc.: elements from token to token (0: one behind the other; a view into a packed
  * projection has the projection's width), a multiple of 16 bytes; row b's tokens begin batch-contiguously, seq_len * stride
- * behind row b - 1's; batch * seq_len up to 2^29 - 1.  q_out and k_out: q and k themselves (in place, with their strides) or memory that overlaps neither.
+ * behind row b - 1's; batch * seq_len up to 2^29 - 1.  q_out and k_out: q and k themselves (in place, with their strides) or
+ * memory that overlaps neither.
  */
 FFKV_API int ffkv_rope_axes(const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, const void* k,
                             int64_t k_stride, void* k_out, int64_t k_out_stride, int dtype, const int32_t* positions,
@@ -450,11 +452,11 @@ FFKV_API int ffkv_key_bounds(const void* k_cache, int cache_dtype, const float* 
  * the block's last query's, the first `sinks` and the last `recent` are taken, and of the rest those with the largest
  *     score(page) = sum over the block's queries and the KV head's query heads of sum_d max(q_d lo_d, q_d hi_d)
  * (sums in fp64, rounded once to fp32; of equal scores the lower page; NaN counts as the largest; a page on no block-table entry
- * as the lowest).  count up to 2^26, num_blocks at least 1.  blocks int32 [batch, ceil(seq_len / query_block), num_kv_heads, count]: ascending, -1 behind a row of fewer
- * pages.  `recent` pages count back from the block's last query: with query_block > 1 give at least
- * (query_block + 14) / 16 + 1 for every query to have its own page.  bounds_dtype F32, F16 or BF16 (ffkv_key_bounds' type).  max_context_len bounds the rows'
- * tokens, this call's included (0: the table's width); pages past it are not taken.  workspace: NULL or
- * ffkv_select_blocks_workspace_bytes (a captured call needs one where that is not 0).
+ * as the lowest).  count up to 2^26, num_blocks at least 1.  blocks int32 [batch, ceil(seq_len / query_block), num_kv_heads,
+ * count]: ascending, -1 behind a row of fewer pages.  `recent` pages count back from the block's last query: with
+ * query_block > 1 give at least (query_block + 14) / 16 + 1 for every query to have its own page.  bounds_dtype F32, F16 or BF16
+ * (ffkv_key_bounds' type).  max_context_len bounds the rows' tokens, this call's included (0: the table's width); pages past it
+ * are not taken.  workspace: NULL or ffkv_select_blocks_workspace_bytes (a captured call needs one where that is not 0).
  */
 FFKV_API size_t ffkv_select_blocks_workspace_bytes(int batch, int seq_len, int num_heads, int num_kv_heads, int head_dim,
                                                    int count, int query_block, int max_blocks, int max_context_len);
@@ -471,9 +473,9 @@ FFKV_API int ffkv_select_blocks(const void* q, int q_dtype, const void* bounds, 
  * count], as ffkv_select_blocks gives them).  Lists may be in any order; entries outside [0, max_blocks), on no block-table
  * entry or past the query count for nothing, and a page listed twice counts twice.  A query without any key gives zeros.  What
  * a query does not attend never reaches it, infinite and NaN values included.  q, out [batch, seq_len, num_heads, head_dim];
- * caches as ffkv_paged_decode takes them (all types; every query_block), count up to 2^26.  The tokens are already appended.  workspace: NULL or
- * ffkv_paged_attention_blocks_workspace_bytes (0 but for few lists, which are then split; a captured call without one leaves
- * them whole).
+ * caches as ffkv_paged_decode takes them (all types; every query_block), count up to 2^26.  The tokens are already appended.
+ * workspace: NULL or ffkv_paged_attention_blocks_workspace_bytes (0 but for few lists, which are then split; a captured call
+ * without one leaves them whole).
  */
 FFKV_API size_t ffkv_paged_attention_blocks_workspace_bytes(int qo_dtype, int cache_dtype, int batch, int seq_len,
                                                             int num_heads, int num_kv_heads, int head_dim, int count,

@@ -146,3 +146,19 @@ def test_streams_and_graphs(ff, gpu):
         assert torch.equal(got, out) and torch.equal(gp, kp)
         if i == 0:
             assert torch.equal(got, first) and not torch.equal(gp, pages)
+
+
+def test_many_tokens(ff, gpu):
+    """More tokens than the launch has waves: each as in a call of its own."""
+    S, sections = 300_007, (16, 8, 8)
+    k = torch.randn(1, S, 2, 64, device=gpu).half()
+    pos = torch.randint(-5, 1 << 20, (3, 1, S), dtype=torch.int32, device=gpu)
+    _, got = ff.apply_rope_axes(None, k, pos, sections, k_out=torch.empty_like(k))
+    at = S // 3
+    for part in (slice(0, at), slice(at, 2 * at), slice(2 * at, S)):
+        x = k[:, part].clone()
+        ff.apply_rope_axes(None, x, pos[:, :, part].contiguous(), sections)
+        assert torch.equal(got[:, part], x)
+    tail = slice(S - 2000, S)
+    want, bound = bu.rotate(f64(k[:, tail]), pos[:, :, tail].cpu().numpy(), sections, False, 1e6, F16)
+    su.check(f64(got[:, tail]), want, bound, "tail")
