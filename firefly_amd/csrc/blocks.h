@@ -128,8 +128,8 @@ __device__ __forceinline__ Split split_index(uint32_t i, int n)
     return Split{d, static_cast<int>(i - d * static_cast<uint32_t>(n))};
 }
 
-// Which kernel attends: the decode's on the matrix cores (token by token), the prefill's (lists of several tokens at head_dim
-// 64, 128 and 256), or the vector kernel (fp32 caches, other head dims).
+// Which kernel attends: the decode's on the matrix cores (token by token), the prefill's (lists that many tokens share, at
+// head_dim 64, 128 and 256), or the vector kernel (fp32 caches, other head dims).
 enum class BlocksKernel
 {
     kDecode,

@@ -656,8 +656,13 @@ BlocksKernel blocks_kernel(const BlocksArgs& a)
 {
     if (a.cache_dtype == F32 || !mfma_dim(a.head_dim)) return BlocksKernel::kVector;
     // (the prefill has no form of head_dim 80, 96 and 112: their lists are attended token by token)
-    const bool prefill = a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256;
-    return a.query_block > 1 && prefill ? BlocksKernel::kPrefill : BlocksKernel::kDecode;
+    if (a.query_block == 1 || a.head_dim == 80 || a.head_dim == 96 || a.head_dim == 112) return BlocksKernel::kDecode;
+    // Few tokens too, while the lists that each reads for itself come from the caches: by workgroups (token, KV head) and pages of
+    // a list, 32/8 heads of 128, bf16, token by token and in the prefill's tiles: 32 x 256 14.7 and 17.3 us, 64 x 256 19.5 and
+    // 18.5 (int8 19.7 and 23.3), 128 x 64 14.1 and 16.1, 128 x 256 28.6 and 19.0, 256 x 16 7.7 and 13.5, 256 x 64 15.7 and
+    // 17.5, 512 x 16 10.5 and 13.5, 512 x 64 25.2 and 18.3, 1024 x 16 18.5 and 13.7.
+    const int64_t wgs = static_cast<int64_t>(a.batch) * a.seq_len * a.num_kv_heads * ((a.group + 15) / 16);
+    return wgs <= 512 && wgs * a.count <= 16384 ? BlocksKernel::kDecode : BlocksKernel::kPrefill;
 }
 
 namespace

@@ -72,6 +72,9 @@ def test_step(ff, gpu, act, kv, Hq, Hkv, D, ctx, count):
     (8, 2, 128, [700, 0], 70, 12, 64), (4, 4, 64, [100], 33, 6, 16), (10, 2, 256, [300, 15], 40, 9, 40),
     (14, 2, 128, [64], 17, 3, 100), (8, 2, 128, [257], 5, 8, 2), (6, 2, 96, [90], 20, 5, 8), (32, 1, 64, [500], 9, 21, 9),
     (4, 1, 128, [40, 300], 6, 7, 1), (10, 2, 80, [300, 15], 40, 9, 16), (7, 1, 112, [64], 17, 3, 100), (6, 3, 104, [50], 9, 4, 3),
+    # of more tokens
+    (8, 2, 128, [1100, 0], 70, 60, 64), (4, 4, 64, [900], 133, 31, 16), (10, 2, 256, [700, 15], 140, 30, 40),
+    (14, 2, 128, [64], 300, 3, 100), (8, 2, 128, [257], 270, 8, 2), (32, 1, 64, [500], 520, 21, 9),
 ])
 def test_chunk(ff, gpu, act, kv, Hq, Hkv, D, ctx, S, count, T):
     c = make(Hq + S, ctx, S, Hq, Hkv, D, act, kv)
@@ -79,7 +82,7 @@ def test_chunk(ff, gpu, act, kv, Hq, Hkv, D, ctx, S, count, T):
 
 
 @pytest.mark.parametrize("act,kv", [("bf16", "bf16"), ("bf16", "i8"), ("bf16", "fp8"), ("f32", "f32"), ("f16", "f16")])
-@pytest.mark.parametrize("S,T", [(1, 1), (9, 1), (50, 16)])
+@pytest.mark.parametrize("S,T", [(1, 1), (9, 1), (50, 16), (200, 16)])
 def test_any_order(ff, gpu, act, kv, S, T):
     """Lists out of order, with entries that are no page, pages past the query, and pages on no table entry."""
     c = make(S + T, [700, 40, 0], S, 8, 2, 128, act, kv)
@@ -89,7 +92,7 @@ def test_any_order(ff, gpu, act, kv, S, T):
     check(ff, c, li, T, gpu)
 
 
-@pytest.mark.parametrize("S,T", [(1, 1), (20, 10)])
+@pytest.mark.parametrize("S,T", [(1, 1), (20, 10), (100, 10)])
 def test_nothing_and_twice(ff, gpu, S, T):
     """Lists without any page give zeros; a page listed twice counts twice."""
     c = make(4, [300, 200, 100], S, 4, 2, 128)
@@ -101,7 +104,7 @@ def test_nothing_and_twice(ff, gpu, S, T):
 
 
 @pytest.mark.parametrize("act,kv", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "fp8"), ("bf16", "i8"), ("f32", "f32")])
-@pytest.mark.parametrize("S,T", [(1, 1), (6, 1), (40, 16)])
+@pytest.mark.parametrize("S,T", [(1, 1), (6, 1), (40, 16), (150, 16)])
 def test_hidden_values_do_not_reach(ff, gpu, act, kv, S, T):
     """NaN and infinite values in the slots behind the row and, of a chunk, behind each query; in pages that are not listed."""
     c = make(31, [90, 205], S, 8, 2, 128, act, kv)
@@ -185,12 +188,13 @@ def test_capture(ff, gpu, S, T):
 @pytest.mark.parametrize("act,kv", KV)
 @pytest.mark.parametrize("Hq,Hkv,D,ctx,S,count,T", [
     (8, 2, 128, [2500, 40, 1200], 13, 130, 32), (5, 1, 64, [3000], 40, 170, 7), (20, 4, 256, [1531, 1908], 13, 100, 13),
+    (8, 2, 128, [2500, 40, 1200], 40, 150, 32), (5, 1, 64, [3000], 107, 170, 7), (20, 4, 256, [1531, 1908], 31, 100, 13),
 ])
 def test_split_chunk(ff, gpu, act, kv, Hq, Hkv, D, ctx, S, count, T):
     """Few blocks of queries over long lists, split over the lists; the same whole, in a capture without a workspace."""
     c = make(Hq + D, ctx, S, Hq, Hkv, D, act, kv)
     n = ff.lib.ffkv_paged_attention_blocks_workspace_bytes(c.act, c.kv, c.B, S, Hq, Hkv, D, count, T)
-    assert n > 0
+    assert n > 0 or kv == "f32"
     li = lists(c, S, count, T, shuffle=True)
     check(ff, c, li, T, gpu)
     kp, vp, ks, vs, bt, cx, _, _, q = su.device(c, gpu)
@@ -205,19 +209,20 @@ def test_split_chunk(ff, gpu, act, kv, Hq, Hkv, D, ctx, S, count, T):
 
 
 @pytest.mark.parametrize("act,kv", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "fp8"), ("bf16", "i8")])
-def test_split_hidden_values(ff, gpu, act, kv):
+@pytest.mark.parametrize("S", [12, 160])
+def test_split_hidden_values(ff, gpu, act, kv, S):
     """As test_hidden_values_do_not_reach, with the strange values in one piece of a split list."""
-    c = make(77, [2000], 12, 8, 2, 128, act, kv)
-    li = lists(c, 12, 120, 12)
+    c = make(77, [2000], S, 8, 2, 128, act, kv)
+    li = lists(c, S, 120, S)
     li[0, 0, :, 60] = 2000 // 16
     for h in range(2):
         li[0, 0, h, 61:][li[0, 0, h, 61:] == 2000 // 16] = -1
         li[0, 0, h, :60][li[0, 0, h, :60] == 2000 // 16] = -1
     q = cases.decode(c.q, c.act).astype(np.float64)
-    want, bound = bu.attend(c, q, li, 12, c.act, 12, 2.0 ** -10)
+    want, bound = bu.attend(c, q, li, S, c.act, S, 2.0 ** -10)
     for t in range(2008, 2016):  # seen by the queries from the eighth on, or by none
         su.poison(c, 0, t)
-    got = su.host(run(ff, c, li, 12, gpu)).reshape(want.shape)
+    got = su.host(run(ff, c, li, S, gpu)).reshape(want.shape)
     su.check(got[:, :8], want[:, :8], bound[:, :8], "before")
     assert not np.isfinite(got[:, 8:]).any()
 
@@ -225,7 +230,8 @@ def test_split_hidden_values(ff, gpu, act, kv):
 @pytest.mark.parametrize("act,kv", KV)
 @pytest.mark.parametrize("Hq,Hkv,D,ctx,S,count,T", [
     (36, 9, 128, [1100, 1300], 120, 61, 16), (24, 12, 64, [1700, 900], 130, 107, 16), (50, 10, 128, [1600, 1], 70, 97, 7),
-    (8, 2, 128, [300, 0, 90], 60, 16, 30), (4, 4, 64, [700], 17, 31, 4),
+    (8, 2, 128, [300, 0, 90], 60, 16, 30), (4, 4, 64, [700], 17, 31, 4), (8, 2, 128, [300, 0, 90], 100, 16, 30),
+    (4, 4, 64, [700], 140, 31, 4),
 ])
 def test_lists_in_halves(ff, gpu, act, kv, Hq, Hkv, D, ctx, S, count, T):
     """At most as many blocks of queries as half fills the chip, or short lists: a list's halves by those of a workgroup."""
@@ -253,7 +259,8 @@ def test_halves_hidden_values(ff, gpu, act, kv, place):
     assert not np.isfinite(got[seen]).any()
 
 
-@pytest.mark.parametrize("S,T,ctx,count", [(100, 10, [2000, 1700], 100), (12, 12, [2000], 120), (20, 20, [200], 12)])
+@pytest.mark.parametrize("S,T,ctx,count", [(100, 10, [2000, 1700], 100), (12, 12, [2000], 120), (24, 24, [2000], 120),
+                                              (20, 20, [200], 12), (60, 60, [200], 12)])
 def test_int8_large_values(ff, gpu, S, T, ctx, count):
     """int8 V scales past 256 take the products again in a smaller scale, whichever part of the list they lie in."""
     c = make(80, ctx, S, 40, 10, 128, "bf16", "i8")

@@ -92,8 +92,8 @@ def test_prompts_and_steps(ff, gpu, kv):
     for b, n in enumerate(prompts):  # each prompt by itself, in chunks
         pos, after = prompt_positions(rng, n)
         nexts.append(after)
-        for at in range(0, n, 128):
-            S = min(128, n - at)
+        for at in range(0, n, 300):
+            S = min(300, n - at)
             packed = rnd(1, S, 12, 64)
             s.call(packed[:, :, :8], packed[:, :, 8:10], packed[:, :, 10:], pos[:, None, at:at + S], S, 10, 1, 5, 32, [b])
     for step in range(20):  # all rows together
