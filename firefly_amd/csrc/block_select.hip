@@ -15,7 +15,7 @@
 // ascending order, -1 behind.
 //
 // The bounds are read once (an eighth of K; in 8-bit caches a quarter), 4 bytes a page and list are written and read again: HBM
-// for long rows, and two or three launches with their chains of loads.
+// for long rows, and two or three launches with their chains of loads (few lists of few pages: one).
 #include "blocks.h"
 #include "mfma_common.h"
 
@@ -29,6 +29,9 @@ namespace
 
 constexpr int kScoreThreads = 256;
 constexpr int kScorePages = 4;  // neighbouring pages that a group of lanes scores together
+constexpr int kOneThreads = 512;
+constexpr int kOneRounds = 4;  // of block_select_one at most
+constexpr int kOwnRows = 8;  // query rows that every lane adds up by itself
 
 template <int CTRL>
 __device__ __forceinline__ double dpp64(double v)
@@ -121,6 +124,28 @@ __device__ __forceinline__ void add_query(const float (&x)[8], double (&down)[8]
     {
         down[e] += static_cast<double>(__builtin_elementwise_minimum(x[e], 0.0f));
         up[e] += static_cast<double>(__builtin_elementwise_maximum(x[e], 0.0f));
+    }
+}
+
+// The sums over a wave's groups of LPP lanes, in every group.
+template <int LPP>
+__device__ __forceinline__ void wave_sums(double (&down)[8], double (&up)[8])
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+    {
+        if constexpr (LPP == 8)
+        {
+            down[e] += dpp64<0x128>(down[e]);  // 8 lanes before it in its row of 16
+            up[e] += dpp64<0x128>(up[e]);
+        }
+        if constexpr (LPP <= 16)
+        {
+            down[e] = swap_sum64<false>(down[e]);
+            up[e] = swap_sum64<false>(up[e]);
+        }
+        down[e] = swap_sum64<true>(down[e]);
+        up[e] = swap_sum64<true>(up[e]);
     }
 }
 
@@ -355,27 +380,14 @@ __global__ __launch_bounds__(kSumThreads) void block_queries(SelectArgs a)
                 add_query(x, down, up);
             }
     }
+    wave_sums<LPP>(down, up);
+    if (lane < LPP)
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-    {
-        if constexpr (LPP == 8)
-        {
-            down[e] += dpp64<0x128>(down[e]);  // 8 lanes before it in its row of 16
-            up[e] += dpp64<0x128>(up[e]);
-        }
-        if constexpr (LPP <= 16)
-        {
-            down[e] = swap_sum64<false>(down[e]);
-            up[e] = swap_sum64<false>(up[e]);
-        }
-        down[e] = swap_sum64<true>(down[e]);
-        up[e] = swap_sum64<true>(up[e]);
-        if (lane < LPP)
+        for (int e = 0; e < 8; ++e)
         {
             s_part[wave][0][8 * c + e] = down[e];
             s_part[wave][1][8 * c + e] = up[e];
         }
-    }
     __syncthreads();
     for (int i = tid; i < 2 * a.head_dim; i += kSumThreads)
     {
@@ -456,47 +468,47 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_lists(SelectArgs a
 // 5.3 us, 16 of 8188 7.5: barriers and LDS latency.)
 constexpr int kChooseMost = 256;
 
+template <int THREADS>
+struct ChooseLds
+{
+    static constexpr int WAVES = THREADS / 64;
+    static constexpr int BINS = 2048;
+    __align__(16) int hist[BINS];
+    int      tot[WAVES];
+    uint32_t ends[2][WAVES];
+    uint32_t keys[kChooseMost];
+    uint32_t found[3];  // bin, of those in it how many stay, how many it holds
+    int      left;
+};
+
+// The keys of the thread's pages of the tile from t0 on (rows of scores are whole 16-byte words; past the last page they hold
+// anything).
+template <int PER>
+__device__ __forceinline__ void load_keys(const SelectArgs& a, const float* w, int t0, uint32_t (&x)[PER])
+{
+    const int i0 = t0 + static_cast<int>(threadIdx.x) * PER;
+#pragma unroll
+    for (int k = 0; k < PER; k += 4)
+    {
+        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (i0 + k < a.most_pages) v = *reinterpret_cast<const f32x4*>(w + i0 + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[k + j] = score_key(v[j]);
+    }
+}
+
+// The choice of a.count of n pages, more than those, by the workgroup: scores w, of which x holds the first tile's keys.
 template <int THREADS, int PER>
-__global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
+__device__ __forceinline__ void choose_pages(const SelectArgs& a, const float* w, int n, uint32_t (&x)[PER], int32_t* out,
+                                             ChooseLds<THREADS>& m)
 {
     constexpr int WAVES = THREADS / 64;
     constexpr int TILE = THREADS * PER;
-    constexpr int BINS = 2048;
+    constexpr int BINS = ChooseLds<THREADS>::BINS;
     constexpr int BPT = BINS / THREADS;  // bins a thread sums up
     static_assert(PER % 4 == 0 && TILE < 1 << 16, "16-byte reads; counts of a tile in 16 bits");
-    __shared__ __align__(16) int s_hist[BINS];
-    __shared__ int      s_tot[WAVES];
-    __shared__ uint32_t s_ends[2][WAVES];
-    __shared__ uint32_t s_keys[kChooseMost];
-    __shared__ uint32_t s_found[3];  // bin, of those in it how many stay, how many it holds
-    __shared__ int      s_left;
-    const int64_t wg = blockIdx.x;
-    const Split   u = split_index(split_index(blockIdx.x, a.num_kv_heads).div, a.lists);
-    const int     b = static_cast<int>(u.div), list = u.rem;
-    const int     tid = static_cast<int>(threadIdx.x);
-    const int     lane = tid & 63, wave = tid >> 6;
-    const float*  w = a.scores + wg * a.stride;
-    int32_t*      out = a.blocks + wg * a.count;
-    uint32_t      x[PER];
-    auto load = [&](int t0)  // (rows of scores are whole 16-byte words; past the last page they hold anything)
-    {
-        const int i0 = t0 + tid * PER;
-#pragma unroll
-        for (int k = 0; k < PER; k += 4)
-        {
-            f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (i0 + k < a.most_pages) v = *reinterpret_cast<const f32x4*>(w + i0 + k);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[k + j] = score_key(v[j]);
-        }
-    };
-    if (a.most_pages > a.count) load(0);  // (on their way while the row's length is)
-    const int n = visible_pages(a, b, list);
-    if (n <= a.count)
-    {
-        for (int i = tid; i < a.count; i += THREADS) out[i] = i < n ? i : -1;
-        return;
-    }
+    const int tid = static_cast<int>(threadIdx.x);
+    const int lane = tid & 63, wave = tid >> 6;
     const int lo = a.sinks, hi = n - a.recent;  // the pages between: more than are taken of them
     const int most = a.count - a.sinks - a.recent;
     auto between = [&](int t0, int k) { return t0 + tid * PER + k >= lo && t0 + tid * PER + k < hi; };
@@ -509,20 +521,20 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
         uint32_t least = 0xffffffffu, largest = 0u;
         for (int t0 = 0; t0 < n; t0 += TILE)
         {
-            if (!one) load(t0);
+            if (!one) load_keys<PER>(a, w, t0, x);
 #pragma unroll
             for (int k = 0; k < PER; ++k)
                 if (between(t0, k)) least = min(least, x[k]), largest = max(largest, x[k]);
         }
         largest = wave_max(largest);
         least = ~wave_max(~least);
-        if (lane == 0) s_ends[0][wave] = least, s_ends[1][wave] = largest;
-        for (int i = tid; i < BINS; i += THREADS) s_hist[i] = 0;
-        if (tid == 0) s_left = 0;
+        if (lane == 0) m.ends[0][wave] = least, m.ends[1][wave] = largest;
+        for (int i = tid; i < BINS; i += THREADS) m.hist[i] = 0;
+        if (tid == 0) m.left = 0;
         __syncthreads();
         const int e = lane < WAVES ? lane : 0;
-        least = ~wave_max(~s_ends[0][e]);
-        largest = wave_max(s_ends[1][e]);
+        least = ~wave_max(~m.ends[0][e]);
+        largest = wave_max(m.ends[1][e]);
         for (;;)
         {
             // bins of 2^shift keys from `least` on
@@ -531,38 +543,38 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
             const int      shift = bits > 11 ? bits - 11 : 0;
             for (int t0 = 0; t0 < n; t0 += TILE)
             {
-                if (!one) load(t0);
+                if (!one) load_keys<PER>(a, w, t0, x);
 #pragma unroll
                 for (int k = 0; k < PER; ++k)
-                    if (between(t0, k) && x[k] >= least && x[k] <= largest) atomicAdd(&s_hist[(x[k] - least) >> shift], 1);
+                    if (between(t0, k) && x[k] >= least && x[k] <= largest) atomicAdd(&m.hist[(x[k] - least) >> shift], 1);
             }
             __syncthreads();
             const int top = BINS - 1 - BPT * tid;  // this thread's bins: top, top - 1, ..
             int       c[BPT], sum = 0;
 #pragma unroll
-            for (int j = 0; j < BPT; ++j) sum += c[j] = s_hist[top - j];
+            for (int j = 0; j < BPT; ++j) sum += c[j] = m.hist[top - j];
             const int incl = wave_scan(sum);
-            if (lane == 63) s_tot[wave] = incl;
+            if (lane == 63) m.tot[wave] = incl;
             __syncthreads();
-            const int tot = lane < WAVES ? s_tot[lane] : 0;
+            const int tot = lane < WAVES ? m.tot[lane] : 0;
             int       before = incl - sum + __builtin_amdgcn_readlane(wave_scan(tot) - tot, uniform(wave));
 #pragma unroll
             for (int j = 0; j < BPT; ++j)
             {
                 if (before < need && need <= before + c[j])
                 {
-                    s_found[0] = static_cast<uint32_t>(top - j);
-                    s_found[1] = static_cast<uint32_t>(need - before);
-                    s_found[2] = static_cast<uint32_t>(c[j]);
+                    m.found[0] = static_cast<uint32_t>(top - j);
+                    m.found[1] = static_cast<uint32_t>(need - before);
+                    m.found[2] = static_cast<uint32_t>(c[j]);
                 }
                 before += c[j];
             }
-            for (int i = tid; i < BINS; i += THREADS) s_hist[i] = 0;
+            for (int i = tid; i < BINS; i += THREADS) m.hist[i] = 0;
             __syncthreads();
-            least += s_found[0] << shift;
+            least += m.found[0] << shift;
             largest = min(largest - least, (1u << shift) - 1u) + least;  // (the range may end inside its last bin)
-            need = static_cast<int>(s_found[1]);
-            const int held = static_cast<int>(s_found[2]);
+            need = static_cast<int>(m.found[1]);
+            const int held = static_cast<int>(m.found[2]);
             if (held <= kChooseMost || shift == 0) break;
             __syncthreads();
         }
@@ -572,33 +584,33 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
         {
             for (int t0 = 0; t0 < n; t0 += TILE)
             {
-                if (!one) load(t0);
+                if (!one) load_keys<PER>(a, w, t0, x);
 #pragma unroll
                 for (int k = 0; k < PER; ++k)
-                    if (between(t0, k) && x[k] >= least && x[k] <= largest) s_keys[atomicAdd(&s_left, 1)] = x[k];
+                    if (between(t0, k) && x[k] >= least && x[k] <= largest) m.keys[atomicAdd(&m.left, 1)] = x[k];
             }
-            const int held = static_cast<int>(s_found[2]);
+            const int held = static_cast<int>(m.found[2]);
             __syncthreads();
             if (tid < held)
             {
-                const uint32_t mine = s_keys[tid];
+                const uint32_t mine = m.keys[tid];
                 int            above = 0, equal = 0;
                 for (int j = 0; j < held; ++j)
                 {
-                    above += s_keys[j] > mine;
-                    equal += s_keys[j] == mine;
+                    above += m.keys[j] > mine;
+                    equal += m.keys[j] == mine;
                 }
                 if (above < need && need <= above + equal)  // (every one of the equal ones writes the same)
                 {
-                    s_found[0] = mine;
-                    s_found[1] = static_cast<uint32_t>(need - above);
+                    m.found[0] = mine;
+                    m.found[1] = static_cast<uint32_t>(need - above);
                 }
             }
             __syncthreads();
-            key = s_found[0];
-            need = static_cast<int>(s_found[1]);
+            key = m.found[0];
+            need = static_cast<int>(m.found[1]);
         }
-        __syncthreads();  // s_tot is read
+        __syncthreads();  // m.tot is read
     }
 
     // The pages that stay, in order: a thread's place is the number of pages before its own that stay for sure, and of those
@@ -606,7 +618,7 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
     int base_sure = 0, base_equal = 0;
     for (int t0 = 0; t0 < n; t0 += TILE)
     {
-        if (!one) load(t0);
+        if (!one) load_keys<PER>(a, w, t0, x);
         uint32_t sure = 0, equal = 0;  // bit k: of page k
 #pragma unroll
         for (int k = 0; k < PER; ++k)
@@ -618,9 +630,9 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
         }
         const int mine = __popc(sure) | (__popc(equal) << 16);
         const int incl = wave_scan(mine);
-        if (lane == 63) s_tot[wave] = incl;
+        if (lane == 63) m.tot[wave] = incl;
         __syncthreads();
-        const int tot = lane < WAVES ? s_tot[lane] : 0;
+        const int tot = lane < WAVES ? m.tot[lane] : 0;
         const int upto = wave_scan(tot);
         const int before = incl - mine + __builtin_amdgcn_readlane(upto - tot, uniform(wave));
         const int all = __builtin_amdgcn_readlane(upto, 63);
@@ -639,12 +651,146 @@ __global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
     }
 }
 
+template <int THREADS, int PER>
+__global__ __launch_bounds__(THREADS) void block_choose(SelectArgs a)
+{
+    __shared__ ChooseLds<THREADS> s_choose;
+    const int64_t wg = blockIdx.x;
+    const Split   u = split_index(split_index(blockIdx.x, a.num_kv_heads).div, a.lists);
+    const int     b = static_cast<int>(u.div), list = u.rem;
+    const float*  w = a.scores + wg * a.stride;
+    int32_t*      out = a.blocks + wg * a.count;
+    uint32_t      x[PER];
+    if (a.most_pages > a.count) load_keys<PER>(a, w, 0, x);  // (on their way while the row's length is)
+    const int n = visible_pages(a, b, list);
+    if (n <= a.count)
+    {
+        for (int i = static_cast<int>(threadIdx.x); i < a.count; i += THREADS) out[i] = i < n ? i : -1;
+        return;
+    }
+    choose_pages<THREADS, PER>(a, w, n, x, out, s_choose);
+}
+
+// All of a list in one workgroup: the sums of its queries, the scores of its pages, which stay in LDS, and the choice.
+template <int BT, int QT, int LPP, bool FULL>
+__global__ __launch_bounds__(kOneThreads) void block_select_one(SelectArgs a)
+{
+    constexpr int PER = 4;                        // pages of a thread in the choice
+    constexpr int WAVES = kOneThreads / 64;
+    constexpr int SLOTS = kOneThreads / LPP;      // groups of lanes
+    constexpr int ROUND = SLOTS * kScorePages;    // pages of a round
+    constexpr int UN = 4;                         // query rows whose loads go out together
+    constexpr int PARTS = WAVES * 2 * LPP * 8 * 8, CHOOSE = static_cast<int>(sizeof(ChooseLds<kOneThreads>));
+    static_assert(kOneRounds * ROUND <= kOneThreads * PER, "the choice holds all scores");
+    __shared__ __align__(16) float s_scores[kOneThreads * PER];
+    __shared__ __align__(16) uint8_t s_mem[PARTS > CHOOSE ? PARTS : CHOOSE];
+    const int64_t wg = blockIdx.x;
+    const Split   u = split_index(blockIdx.x, a.num_kv_heads), v = split_index(u.div, a.lists);
+    const int     kvh = u.rem, list = v.rem, b = static_cast<int>(v.div);
+    const int     tid = static_cast<int>(threadIdx.x);
+    const int     lane = tid & 63, wave = tid >> 6;
+    const int     c = tid % LPP, grp = tid / LPP;
+    const bool    in = FULL || 8 * c < a.head_dim;
+    int32_t*      out = a.blocks + wg * a.count;
+    const int     n = visible_pages(a, b, list);
+    if (n <= a.count)
+    {
+        for (int i = tid; i < a.count; i += kOneThreads) out[i] = i < n ? i : -1;
+        return;
+    }
+    const int32_t* table = a.block_table + static_cast<int64_t>(b) * a.max_blocks;
+    const int      rounds = (n + ROUND - 1) / ROUND;
+    using Bounds = PageBounds<BT, LPP, FULL>;
+    int    phys[kScorePages];
+    Bounds cur, nxt;
+    Bounds::entries(table, grp * kScorePages, n, phys);
+    cur.load(a, phys, kvh, c);
+    if (rounds > 1) Bounds::entries(table, ROUND + grp * kScorePages, n, phys);
+
+    const int t0 = list * a.query_block;
+    const int rows = min(a.query_block, a.seq_len - t0) * a.group;
+    const bool few = rows <= kOwnRows;  // every lane adds up its dims of all rows; else the groups of lanes share the rows
+    double    down[8], up[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) down[e] = up[e] = 0.0;
+    const int step = few ? 1 : SLOTS;
+    for (int r0 = few ? 0 : grp; r0 < rows; r0 += UN * step)
+    {
+        Raw8 q[UN];
+#pragma unroll
+        for (int k = 0; k < UN; ++k)
+            if (r0 + k * step < rows && in) load_raw8<QT>(a.q, query_at(a, b, t0, kvh, r0 + k * step, c), q[k]);
+#pragma unroll
+        for (int k = 0; k < UN; ++k)
+            if (r0 + k * step < rows && in)
+            {
+                float x[8];
+                unpack8<QT>(q[k], x);
+                add_query(x, down, up);
+            }
+    }
+    if (!few)
+    {
+        double* s_part = reinterpret_cast<double*>(s_mem);  // [wave][2][LPP * 8]
+        wave_sums<LPP>(down, up);
+        if (lane < LPP)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                s_part[(wave * 2 + 0) * (LPP * 8) + 8 * c + e] = down[e];
+                s_part[(wave * 2 + 1) * (LPP * 8) + 8 * c + e] = up[e];
+            }
+        __syncthreads();
+        double s = 0.0;  // (as many threads as sums, or more)
+        static_assert(2 * LPP * 8 <= kOneThreads, "a sum per thread");
+        if (tid < 2 * LPP * 8)
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) s += s_part[w * (2 * LPP * 8) + tid];
+        __syncthreads();
+        if (tid < 2 * LPP * 8) s_part[tid] = s;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            down[e] = s_part[8 * c + e];
+            up[e] = s_part[LPP * 8 + 8 * c + e];
+        }
+    }
+    for (int r = 0; r < rounds; ++r)
+    {
+        if (r + 1 < rounds) nxt.load(a, phys, kvh, c);
+        if (r + 2 < rounds) Bounds::entries(table, (r + 2) * ROUND + grp * kScorePages, n, phys);
+        double s[kScorePages];
+#pragma unroll
+        for (int k = 0; k < kScorePages; ++k)
+        {
+            double lo[8], hi[8];
+            cur.values(k, in, lo, hi);
+            s[k] = lane_score(down, up, lo, hi);
+        }
+        const double sum = group_sums4<LPP>(s, c);
+        const int    p = r * ROUND + grp * kScorePages + (c & 3);
+        if (c < 4 && p < n) s_scores[p] = cur.on >> c & 1 ? static_cast<float>(sum) : kNegInf;  // on no page: last
+        cur = nxt;
+    }
+    __syncthreads();
+    uint32_t x[PER];
+    load_keys<PER>(a, s_scores, 0, x);
+    choose_pages<kOneThreads, PER>(a, s_scores, n, x, out, *reinterpret_cast<ChooseLds<kOneThreads>*>(s_mem));
+}
+
 namespace
 {
 
 template <int BT, int QT, int LPP, bool FULL>
 hipError_t launch_scores_l(const SelectArgs& a, hipStream_t stream)
 {
+    if (select_in_one(a))
+    {
+        const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.batch) * a.lists * a.num_kv_heads));
+        hipLaunchKernelGGL((block_select_one<BT, QT, LPP, FULL>), grid, dim3(kOneThreads), 0, stream, a);
+        return hipGetLastError();
+    }
     constexpr int ROUND = kScoreThreads / LPP * kScorePages;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.num_kv_heads;
     const int64_t all = (a.most_pages + ROUND - 1) / ROUND;  // rounds of a row
@@ -694,7 +840,19 @@ hipError_t launch_scores(const SelectArgs& a, hipStream_t stream)
 // than 8 query rows, are summed once, in a launch of their own.  (Whole calls over rows of 1000 pages, 8 KV heads, in place and
 // apart: 4 rows with 4, 8, 12, 16 and 32 query rows 10.8, 12.0, 13.4, 14.8 and 20.3 us against 12.6; 32 rows 29.5, 29.8,
 // 30.9, 31.8 and 38.5 against 33.5.)
-bool select_by_lists(int seq_len, int lists, int group) { return lists > 1 || static_cast<int64_t>(seq_len) * group > 8; }
+bool select_by_lists(int seq_len, int lists, int group) { return lists > 1 || static_cast<int64_t>(seq_len) * group > kOwnRows; }
+
+// Few lists of few pages: a launch each, without a workspace, whose loads are in flight a round at a time only.  Rounds of 128 pages
+// at head_dim 128, whole calls in the other launches and in one: 8 lists of up to 64 pages 8.3 and 6.2 us, of 250 9.1 and 6.6,
+// 128 lists 9.9 and 7.8, 11.4 and 9.6; 32 lists of 1000 11.2 and 17.7; 512 lists of 64 11.9 and 14.4.  Where queries are
+// summed apart, 64 lists of 495 pages 14.9 and 10.4, 128 16.1 and 14.6, 128 lists of 1995 23.0 and 31.5.
+bool select_in_one(const SelectArgs& a)
+{
+    const int64_t lists = static_cast<int64_t>(a.batch) * a.lists * a.num_kv_heads;
+    const int     lanes = a.head_dim <= 64 ? 8 : (a.head_dim <= 128 ? 16 : 32);
+    const int     rounds = select_by_lists(a.seq_len, a.lists, a.group) ? kOneRounds : 2;
+    return lists <= 256 && a.most_pages <= rounds * (kOneThreads / lanes * kScorePages);
+}
 
 hipError_t launch_select(const SelectArgs& a, hipStream_t stream)
 {
@@ -706,7 +864,7 @@ hipError_t launch_select(const SelectArgs& a, hipStream_t stream)
         e = a.bounds_dtype == F32 ? launch_scores<F32>(a, stream)
             : a.bounds_dtype == F16 ? launch_scores<F16>(a, stream)
                                     : launch_scores<BF16>(a, stream);
-    if (e != hipSuccess) return e;
+    if (e != hipSuccess || (a.most_pages > a.count && select_in_one(a))) return e;
     const dim3 grid(static_cast<unsigned>(lists));
     // The smallest that holds a row in registers; one that does not reads it again for every pass.  (Whole calls of 2 rows, 8
     // heads, by 256, 512 and 1024 threads: 1000 pages 10.1, 11.1, 12.0 us; 2000 13.3, 12.0, 13.0; 4000 21.0, 16.2, 16.7; 8187

@@ -131,7 +131,16 @@ SelectLayout select_layout(int batch, int seq_len, int num_heads, int num_kv_hea
                            int query_block)
 {
     if (pages <= count) return SelectLayout{};  // nothing is left out
-    const int     lists = lists_of(seq_len, query_block);
+    const int        lists = lists_of(seq_len, query_block);
+    ffkv::SelectArgs a{};
+    a.batch = batch;
+    a.seq_len = seq_len;
+    a.num_kv_heads = num_kv_heads;
+    a.group = num_heads / num_kv_heads;
+    a.head_dim = head_dim;
+    a.most_pages = pages;
+    a.lists = lists;
+    if (ffkv::select_in_one(a)) return SelectLayout{};
     const double  each = 4.0 * pages + 16.0 * head_dim + 256.0;
     if (each * batch * lists * num_kv_heads > kMostBytes) return SelectLayout{0, 0, -1};
     const int64_t all = static_cast<int64_t>(batch) * lists * num_kv_heads;

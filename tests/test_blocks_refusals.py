@@ -98,7 +98,7 @@ def test_bounds_rejects(ff, kw, code):
     (dict(count=0), -1), (dict(sinks=-1), -1), (dict(recent=-1), -1), (dict(sinks=3, recent=2), -1),
     (dict(sinks=2 ** 31 - 1, recent=2 ** 31 - 1), -1), (dict(q=None), -1), (dict(bounds=None), -1), (dict(blocks=None), -1),
     (dict(context_lens=None), -1), (dict(q=8), -1), (dict(bounds=8), -1), (dict(blocks=18), -1), (dict(workspace=8), -1),
-    (dict(workspace=16, workspace_bytes=2 * 64 * 4 - 1), -3),
+    (dict(workspace=16, workspace_bytes=2 * 6000 * 4 - 1, max_blocks=6000), -3),
     (dict(seq_len=2 ** 31 - 1, batch=60000, num_heads=60000, num_kv_heads=60000), -2),
     (dict(seq_len=2 ** 31 - 1, query_block=2 ** 31 - 1, num_heads=64, num_kv_heads=1), -2),
     (dict(seq_len=2 ** 20, max_blocks=2 ** 26), -2), (dict(count=2 ** 26 + 1), -2), (dict(count=2 ** 31 - 1), -2),
@@ -131,9 +131,10 @@ def test_empty_is_ok(ff):
 def test_workspace_bytes(ff):
     f = ff.lib.ffkv_select_blocks_workspace_bytes
     lists = 2 * 4 * 4
-    assert f(2, 100, 8, 4, 64, 8, 32, 50, 0) == lists * (52 * 4 + 64 * 16)
-    assert f(2, 100, 8, 4, 64, 8, 32, 50, 300) == lists * (20 * 4 + 64 * 16)
-    assert f(2, 1, 8, 4, 64, 8, 1, 64, 0) == 8 * 64 * 4  # a step's queries are summed where they are used
+    assert f(2, 100, 8, 4, 64, 8, 32, 5000, 0) == lists * (5000 * 4 + 64 * 16)
+    assert f(2, 100, 8, 4, 64, 8, 32, 5000, 4000 * 16) == lists * (4000 * 4 + 64 * 16)
+    assert f(2, 1, 8, 4, 64, 8, 1, 2000, 0) == 8 * 2000 * 4  # a step's queries are summed where they are used
+    assert f(2, 100, 8, 4, 64, 8, 32, 50, 0) == 0 and f(2, 1, 8, 4, 64, 8, 1, 64, 0) == 0  # few pages: no scores are written
     assert f(2, 100, 8, 4, 64, 50, 32, 50, 0) == 0 and f(2, 100, 8, 4, 64, 19, 32, 50, 300) == 0
     assert f(0, 1, 1, 1, 64, 1, 1, 9, 0) == 0 and f(1, 1, 1, 1, 64, 0, 1, 9, 0) == 0 and f(1, 1, 1, 1, 64, 1, 0, 9, 0) == 0
     g = ff.lib.ffkv_paged_attention_blocks_workspace_bytes

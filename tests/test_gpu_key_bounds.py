@@ -83,10 +83,11 @@ def boxes(rng, N, Hkv, D, dtype, dev):
     (8, 2, 96, 37, [800, 0, 100], 8, 2, 3, 16),               # blocks of queries, the last one short
     (2, 1, 8, 3, [40000], 100, 1, 1, 4),                      # 2500 pages, a block longer than the call
     (40, 2, 112, 2, [16000, 20000], 1, 0, 0, 1),              # one page
-    (8, 8, 128, 64, [600], 20, 1, 5, 64),
+    (8, 8, 128, 64, [600], 20, 1, 5, 64), (24, 2, 128, 1, [2000, 1999], 30, 1, 2, 1), (18, 1, 64, 3, [9000, 40], 25, 3, 5, 2),
 ])
-def test_choice(ff, gpu, act, dtype, Hq, Hkv, D, S, ctx, count, sinks, recent, T):
-    c = cases.make_case(Hq + S, len(ctx), Hq, Hkv, 8, ctx, act=act, S=S)
+@pytest.mark.parametrize("wide", [False, True])  # behind a wide table the choice takes other kernels
+def test_choice(ff, gpu, act, dtype, Hq, Hkv, D, S, ctx, count, sinks, recent, T, wide):
+    c = cases.make_case(Hq + S, len(ctx), Hq, Hkv, 8, ctx, act=act, S=S, max_blocks=3001 if wide else None)
     rng = np.random.default_rng(D + S)
     q = cases.encode(rng.standard_normal((c.B, S, Hq, D), dtype=np.float32) * np.float32(2), c.act)
     box = boxes(rng, c.num_blocks, Hkv, D, dtype, gpu)
@@ -108,9 +109,10 @@ def test_long_rows(ff, gpu):
         assert np.array_equal(got, bu.select(qv, bv, c.block_table, c.ctx, 300, 4, 9, 1, c.num_blocks, most))
 
 
-def test_ties_and_strange_scores(ff, gpu):
+@pytest.mark.parametrize("wide", [None, 2000])
+def test_ties_and_strange_scores(ff, gpu, wide):
     """Equal scores go to the lower page, NaN before all, pages on no table entry last; zero queries tie everywhere."""
-    c = cases.make_case(9, 3, 4, 2, 8, [1600, 1600, 1600])
+    c = cases.make_case(9, 3, 4, 2, 8, [1600, 1600, 1600], max_blocks=wide)
     rng = np.random.default_rng(6)
     q = cases.encode(np.abs(rng.standard_normal((3, 1, 4, 64), dtype=np.float32)) + np.float32(0.1), c.act)
     q[1] = 0
