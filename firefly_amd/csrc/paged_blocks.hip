@@ -4,7 +4,7 @@
 //   out[b, t, h] = sum over listed pages and their tokens j <= context_lens[b] + t of softmax_j(scale q.k_j) v_j
 //
 // Steps are bound by HBM: the listed pages are read once, at about Hq / Hkv operations a byte.  64 rows of 64 listed pages, 32/8
-// heads of 128, bf16: 270 MB in 49.2 us = 5.5 TB/s (int8 28.9, fp32 98); 4 rows of 256, 28/4 heads, f16: 14.2 us, of which
+// heads of 128, bf16: 270 MB in 49.4 us = 5.5 TB/s (int8 28.9, fp32 98); 4 rows of 256, 28/4 heads, f16: 14.2 us, of which
 // 3.5 of merge; 4 rows of up to 16: 7.2, a launch and its chain of loads.
 //
 // On the matrix cores (16- and 8-bit caches) a workgroup of four or eight waves takes a list, or a piece of one, and up to 16
@@ -15,7 +15,7 @@
 //
 // Blocks of tokens that share their lists take the prefill's kernel (blocks_prefill.h), whose tiles of 128 query rows read a
 // list once; bound by its vector work beside the products (2 x 512 tokens in blocks of 64, 128 listed fp8 pages, 32/8 heads of
-// 128: 34.4 GFLOP in 51 us = 675 TFLOP/s).
+// 128: 34.4 GFLOP in 53.5 us = 640 TFLOP/s).
 //
 // fp32 caches and the other head dims take the vector kernel: 16 (head_dim 256: 32) lanes per token, four query heads a
 // workgroup.

@@ -13,8 +13,8 @@
 // low one enters to first order: what is left is the rounding of cos and sin to fp32 and the errors of the rate, 2^-48 of
 // the angle at most: 2^-22 + |p| 2^-48 in all (theta >= 1).
 //
-// Bound by HBM (q read and written, k and v read and written once): 8 x 1500 f16 tokens of 32/8 heads of 128, 295 MB, 58.3 us =
-// 5.1 TB/s; 32000 bf16 tokens of 28/4 heads, 590 MB, 104 us = 5.7 TB/s (a copy reaches 5.1).  A step of 4 tokens takes 3.5 us.
+// Bound by HBM (q read and written, k and v read and written once): 8 x 1500 f16 tokens of 32/8 heads of 128, 295 MB, 58.4 us =
+// 5.1 TB/s; 32000 bf16 tokens of 28/4 heads, 590 MB, 102 us = 5.8 TB/s (a copy reaches 5.1).  A step of 4 tokens takes 3.5 us.
 #include "blocks.h"
 #include "ffkv_device.h"
 

@@ -84,6 +84,7 @@ int bas_refusal(int op)
     off.sections[1] = 15;
     switch (op)
     {
+        case -1: kernels::update_key_bounds(c, box, i, i, 0, 2, 1); break;  // no rows: nothing to refuse
         case 0: kernels::apply_rope_axes(half, k, at); break;
         case 1: kernels::apply_rope_axes(q, k, off); break;
         case 2: kernels::rope_append_kv_cache_axes(q, k, half, c, c, i, i, 2, at); break;

@@ -32,6 +32,7 @@ def _p(t):
 @pytest.mark.parametrize("op", range(18))
 def test_refusals(shim, op):
     assert shim.bas_refusal(op) == -1 and shim.bas_last_error() != b""
+    assert shim.bas_refusal(-1) == 0 and shim.bas_last_error() == b""  # the next call's own result
 
 
 @pytest.mark.gpu
