@@ -151,7 +151,6 @@ bool       select_by_lists(int seq_len, int lists, int group);  // whether the c
 bool       select_in_one(const SelectArgs& a);  // in one launch, without a workspace (a's sizes and most_pages set)
 hipError_t launch_select(const SelectArgs& a, hipStream_t stream);
 hipError_t launch_blocks(const BlocksArgs& a, hipStream_t stream);
-hipError_t launch_blocks_decode(const BlocksArgs& a, hipStream_t stream);
 hipError_t launch_blocks_prefill(const BlocksArgs& a, hipStream_t stream);
 
 }  // namespace ffkv

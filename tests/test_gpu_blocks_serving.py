@@ -10,6 +10,7 @@ import cases
 import gpu_util as gu
 import oracle as O
 import scored_util as su
+from test_gpu_attention_blocks import make
 
 pytestmark = pytest.mark.gpu
 
@@ -141,3 +142,71 @@ def test_captured_step(ff, gpu):
         for a, b in zip(eager, got):
             assert torch.equal(a, b)
         cx.add_(1)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "i8", "f32"])
+@pytest.mark.parametrize("S,T,count", [(1, 1, 8), (9, 4, 8), (200, 16, 8), (200, 40, 30), (40, 40, 150)])
+@pytest.mark.parametrize("width", [None, 2600])
+def test_rows_that_are_not_there(ff, gpu, kv, S, T, count, width):
+    """Rows padded with negative lengths, wholly or for their first tokens, beside one that is there."""
+    ctx = [500, -S, -1000, -(S // 2)]
+    c = make(S + count, [500, S, S, S], S, 8, 2, 64, "f32" if kv == "f32" else "bf16", kv, max_blocks=width)
+    k, v, ks, vs, table, _, kn, vn, q = su.device(c, gpu)
+    cx = torch.tensor(ctx, dtype=torch.int32, device=gpu)
+    pos = torch.zeros(2, 4, S, dtype=torch.int32, device=gpu)
+    before = k.clone()
+    ff.rope_append_axes(q, kn, vn, pos, (16, 16), k, v, table, cx, k_scale=ks, v_scale=vs)
+    box = ff.key_bounds(k).fill_(7)
+    ff.update_key_bounds(k, box, table, cx, S, k_scale=ks)
+    li = ff.select_blocks(q, box, table, cx, count, sinks=1, recent=(T + 14) // 16 + 1, query_block=T)
+    out = ff.paged_attention_blocks(q, k, v, table, cx, li, query_block=T, k_scale=ks, v_scale=vs)
+    for b in (1, 2):  # not there: no page written, none listed, nothing attended
+        own = torch.from_numpy(c.block_table[b][c.block_table[b] >= 0]).long().to(gpu)
+        assert torch.equal(k[own], before[own]) and (box[own] == 7).all()
+        assert (li[b] == -1).all() and not out[b].any()
+    there = S - S // 2  # tokens of row 3 from its position 0 on
+    first = S // 2
+    assert not out[3, :first].any() and (there == 0 or out[3, first:].any(dim=-1).all())
+    # both rows that are there, as without the others
+    c.ctx = np.array(ctx, np.int32)
+    c.k_pool, c.v_pool = gu.to_host(k, c.k_pool.dtype).reshape(c.k_pool.shape), gu.to_host(v, c.v_pool.dtype).reshape(c.v_pool.shape)
+    if ks is not None:
+        c.k_scale, c.v_scale = ks.cpu().numpy(), vs.cpu().numpy()
+    qv, lists = q.double().cpu().numpy(), li.cpu().numpy()
+    want = bu.select(qv, box.double().cpu().numpy(), c.block_table, c.ctx, count, 1, (T + 14) // 16 + 1, T, c.num_blocks)
+    assert np.array_equal(lists, want)
+    o, e = bu.attend(c, qv, lists, T, c.act, S, 2.0 ** -10)
+    su.check(su.host(out).reshape(o.shape), o, e, "attention")
+
+
+def test_pages_past_32_bits(ff, gpu):
+    """Pages whose bytes and elements lie past 2^32 and 2^31 of their pool: the bits of the same rows in a small pool."""
+    N, Hkv, D, B, S = 140_000, 8, 128, 2, 70
+    rng = np.random.default_rng(5)
+    small = 160
+    kp = torch.randn(small, 16, Hkv, D, device=gpu).bfloat16()
+    vp = torch.randn(small, 16, Hkv, D, device=gpu).bfloat16()
+    table = torch.from_numpy(rng.permutation(small).astype(np.int32).reshape(B, 80)).to(gpu)
+    far = table + (N - small)
+    K, V = torch.empty(N, 16, Hkv, D, dtype=kp.dtype, device=gpu), torch.empty(N, 16, Hkv, D, dtype=kp.dtype, device=gpu)
+    K[N - small:], V[N - small:] = kp, vp
+    box, Box = ff.key_bounds(kp), ff.key_bounds(K)
+    packed = torch.randn(B, S, 32 + 2 * Hkv, D, device=gpu).bfloat16()
+    q, k, v = packed[:, :, :32], packed[:, :, 32:32 + Hkv], packed[:, :, 32 + Hkv:]
+    pos = torch.randint(0, 1000, (3, B, S), dtype=torch.int32, device=gpu)
+    cx = torch.tensor([1200, 777], dtype=torch.int32, device=gpu)
+    got = []
+    for pk, pv, pb, bt in ((kp, vp, box, table), (K, V, Box, far)):
+        qr = ff.rope_append_axes(q, k, v, pos, (16, 24, 24), pk, pv, bt, cx, q_out=torch.empty(B, S, 32, D, dtype=q.dtype, device=gpu))
+        ff.update_key_bounds(pk, pb, bt, torch.zeros_like(cx), 1270)
+        res = [qr]
+        for T, count in ((1, 20), (16, 20), (70, 60)):
+            li = ff.select_blocks(qr, pb, bt, cx, count, sinks=1, recent=7, query_block=T)
+            res += [li, ff.paged_attention_blocks(qr, pk, pv, bt, cx, li, query_block=T)]
+        one = qr[:, :1].contiguous()
+        li = ff.select_blocks(one, pb, bt, cx, 20)
+        got.append(res + [li, ff.paged_attention_blocks(one, pk, pv, bt, cx, li)])
+    assert torch.equal(K[N - small:], kp) and torch.equal(V[N - small:], vp)
+    assert torch.equal(Box[far.long().flatten()], box[table.long().flatten()])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
