@@ -179,7 +179,10 @@ struct PageBounds
     }
     __device__ __forceinline__ void load(const SelectArgs& a, const int (&phys)[kScorePages], int kvh, int c)
     {
-        const int D = FULL ? LPP * 8 : a.head_dim;
+        constexpr uint32_t EB = BT == F32 ? 4 : 2;
+        const uint32_t D = FULL ? LPP * 8 : a.head_dim;
+        const uint32_t stride = a.num_kv_heads * 2u * D * EB;  // bytes of a page: below 2^28
+        const char*    base = static_cast<const char*>(a.bounds) + (kvh * 2u * D + (FULL || 8u * c < D ? 8u * c : 0u)) * EB;
         on = 0;
 #pragma unroll
         for (int k = 0; k < kScorePages; ++k)
@@ -187,9 +190,9 @@ struct PageBounds
             const bool     ok = phys[k] >= 0 && phys[k] < a.num_blocks;
             const uint32_t page = ok ? phys[k] : 0;
             on |= ok ? 1 << k : 0;
-            const size_t at = (static_cast<size_t>(page) * a.num_kv_heads + kvh) * (2 * D) + (FULL || 8 * c < D ? 8 * c : 0);
-            load_raw8<BT>(a.bounds, at, lo[k]);
-            load_raw8<BT>(a.bounds, at + D, hi[k]);
+            const char* at = base + static_cast<uint64_t>(page) * stride;
+            load_raw8<BT>(at, 0, lo[k]);
+            load_raw8<BT>(at, D, hi[k]);
         }
     }
     __device__ __forceinline__ void values(int k, bool in, double (&l)[8], double (&h)[8]) const
@@ -318,7 +321,7 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a,
     cur.load(a, phys, at.hb * heads + hd, c);
     if (x0 + 1 < x1) entries(ahead);
     sum_queries(at);
-    for (int64_t x = x0; x < x1; ++x)
+    auto round = [&](const PageBounds<BT, LPP, FULL>& cur, PageBounds<BT, LPP, FULL>& nxt, int64_t x)
     {
         if (x + 1 < x1) nxt.load(a, phys, ahead.hb * heads + hd, c);
         const Place after = next(ahead);
@@ -337,9 +340,13 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a,
         // (behind the row's last page up to stride: read by nobody)
         if (c < 4 && p < a.most_pages) out[p] = cur.on >> c & 1 ? static_cast<float>(sum) : kNegInf;  // on no page: last
         if (x + 1 < x1 && (ahead.b != at.b || ahead.hb != at.hb)) sum_queries(ahead);
-        cur = nxt;
         at = ahead;
         ahead = after;
+    };
+    for (int64_t x = x0; x < x1; x += 2)
+    {
+        round(cur, nxt, x);
+        if (x + 1 < x1) round(nxt, cur, x + 1);
     }
 }
 
