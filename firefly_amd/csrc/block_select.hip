@@ -217,7 +217,8 @@ struct PageBounds
 // workgroup takes an equal share, as many workgroups as fit the chip: tiles of their own left it waiting for the longest row
 // (57.5 us in all).  LPP lanes take four neighbouring pages' bounds, 8 dims each, and every lane adds up its dims of the
 // queries by itself; while a round is added up the next one's bounds are on their way, and the table's entries of the one
-// after.  Bound by HBM: about 4.7 TB/s behind a start of 3 us (4 rows of 8188 pages, 4 heads, 67 MB: 15.5 us).
+// after.  Bound by HBM and by fp64 (a conversion and a product per bound): 4.6 TB/s (4 rows of 8188 pages, 4 heads, 67 MB:
+// 14.5 us; the 64 rows above 32 of 37.9 in all).
 template <int BT, int QT, int LPP, bool FULL>
 __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a, int heads)
 {
@@ -849,8 +850,8 @@ hipError_t launch_scores(const SelectArgs& a, hipStream_t stream)
 // 30.9, 31.8 and 38.5 against 33.5.)
 bool select_by_lists(int seq_len, int lists, int group) { return lists > 1 || static_cast<int64_t>(seq_len) * group > kOwnRows; }
 
-// Few lists of few pages: a launch each, without a workspace, whose loads are in flight a round at a time only.  Rounds of 128 pages
-// at head_dim 128, whole calls in the other launches and in one: 8 lists of up to 64 pages 8.3 and 6.2 us, of 250 9.1 and 6.6,
+// Few lists of few pages: one launch, without a workspace, in which a list has one CU (1.5 us a round).  Rounds of 128 pages at
+// head_dim 128, whole calls in the other launches and in one: 8 lists of up to 64 pages 8.3 and 6.2 us, of 250 9.1 and 6.6,
 // 128 lists 9.9 and 7.8, 11.4 and 9.6; 32 lists of 1000 11.2 and 17.7; 512 lists of 64 11.9 and 14.4.  Where queries are
 // summed apart, 64 lists of 495 pages 14.9 and 10.4, 128 16.1 and 14.6, 128 lists of 1995 23.0 and 31.5.
 bool select_in_one(const SelectArgs& a)

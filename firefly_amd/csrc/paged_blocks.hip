@@ -72,7 +72,8 @@ __device__ __forceinline__ int listed_tokens(const BlocksArgs& a, int lp, int ph
 
 // A state of (max, denominator, accumulator) to the output, or to its piece's place in the workspace.
 template <int QT>
-__device__ __forceinline__ void store_state4(const BlocksArgs& a, int64_t row_h, int split, int D, int d4, float M, float L, f32x4 o)
+__device__ __forceinline__ void store_state4(const BlocksArgs& a, int64_t row_h, int split, int D, int d4, float M, float L,
+                                             f32x4 o)
 {
     if (a.splits == 1)
     {
