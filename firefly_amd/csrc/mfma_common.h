@@ -254,6 +254,32 @@ __device__ __forceinline__ float swap_sum(float x)
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
+// Units of a column's P on int8 pages, whose V scales, of any size, go into P's f16 operand (11 bits from 2^-14 to 65504): P, the
+// denominator and the accumulators are held 2^shift times as large, which the quotient does not see, so that the column's
+// largest P lies between 2^4 and 2^15, and what f16 loses of the others is at most 2^-29 of it.  (In the softmax's own units V
+// scales below 2^-14 lost their bits, and values below 4e-6 came out as zeros.)  The shift stays within +-40, so that pieces of a
+// list in units of their own still meet in fp32.
+struct ValueUnits
+{
+    float shift = 0.0f;
+    float known = 0.0f;  // the P that set the shift, as it weighs now: the largest is no smaller
+    // What a new P may be in these units (0: it takes new ones, as `known` weighs little beside a new maximum of the scores).
+    __device__ __forceinline__ float limit() const { return known < 16.0f ? 0.0f : 32768.0f; }
+};
+
+// The factor to new units for a column whose largest new |P| is wc: 1 where it fits, or is infinite or NaN.
+__device__ __forceinline__ float new_units(ValueUnits& u, float wc)
+{
+    if (!(wc > u.limit())) return 1.0f;
+    u.known = fmaxf(wc, u.known);
+    if (u.known == __builtin_huge_valf()) return 1.0f;
+    const float to = fminf(fmaxf(u.shift + static_cast<float>(11 - __builtin_amdgcn_frexp_expf(u.known)), -40.0f), 40.0f);
+    const float f = __builtin_amdgcn_exp2f(to - u.shift);  // (whole powers of two are exact)
+    u.shift = to;
+    u.known *= f;
+    return f;
+}
+
 }  // namespace
 
 }  // namespace ffkv

@@ -243,6 +243,7 @@ void paged_blocks_decode(BlocksArgs a)
 
     float m_run = kLowest, l_run = 0.0f;
     f32x4 acc[NT];
+    ValueUnits units;  // int8
 #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
@@ -281,7 +282,8 @@ void paged_blocks_decode(BlocksArgs a)
         }
     };
 
-    // Online softmax of a staged page and its products with V.  P in bf16 takes a hi + lo pair (16 bits); in f16 its 11 bits.
+    // Online softmax of a staged page and its products with V.  P in bf16 takes a hi + lo pair (16 bits); in f16 its 11 bits (int8
+    // pages: in units of the column, as the V scales are in it).
     auto finish_page = [&](int n_tok, float tks, float tvs, f32x4 s)
     {
         float sc[4], vs[4];
@@ -306,7 +308,7 @@ void paged_blocks_decode(BlocksArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
         {
-            const float p = __builtin_amdgcn_exp2f(sc[i] - m_new);
+            const float p = __builtin_amdgcn_exp2f(CT == I8 ? sc[i] - m_new + units.shift : sc[i] - m_new);
             psum += p;
             pv[i] = 4 * g + i < n_tok ? p * vs[i] : 0.0f;
         }
@@ -315,8 +317,24 @@ void paged_blocks_decode(BlocksArgs a)
         {
 #pragma unroll
             for (int i = 0; i < NT; ++i) acc[i] *= alpha;
+            units.known *= alpha;
         }
         m_run = m_new;
+        if constexpr (CT == I8)
+        {
+            float w = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w = fmaxf(w, __builtin_fabsf(pv[i]));
+            if (__any(w > units.limit()))
+            {
+                const float f = new_units(units, xor_max(w));
+                l_run *= f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pv[i] *= f;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) acc[i] *= f;
+            }
+        }
         uint32_t ph[4], pl[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -377,7 +395,7 @@ void paged_blocks_decode(BlocksArgs a)
 #pragma unroll
         for (int i = 0; i < NT; ++i)
             *reinterpret_cast<f32x4*>(s_acc + (wave * gc + c) * D + 16 * i + 4 * g) = acc[i] * piece_scale;
-        if (g == 0) s_ml[wave * 16 + c] = float2{m_run, l_tot};
+        if (g == 0) s_ml[wave * 16 + c] = float2{m_run - units.shift, l_tot};
     }
     __syncthreads();
     for (int k = static_cast<int>(threadIdx.x); k < gc * (D / 4); k += 64 * WAVES)
