@@ -1061,6 +1061,10 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
     // int8 pages: on the rerun below every p is scaled by 2^kRerunShift, numerator and denominator alike, so the
     // result is the same softmax
     constexpr float kRerunShift = -12.0f;
+    // int8 pages of a list: P in units of its column, for V scales of any size (a list's tokens need not be of one size), and
+    // no rerun
+    constexpr bool UNITS = LIST && CT == I8;
+    ValueUnits  units[UNITS ? RG : 1];
     float       m_run[RG], l_run[RG];
     f32x4       lacc[RG];  // L_MFMA: the denominator's product (every element holds the column's sum)
     float       m_thr[RG], m_neg[RG];  // m_run + thr_raw, and -m_run * c_log2 (0 before the first key)
@@ -1257,6 +1261,11 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
                 m_thr[gi] = m_run[gi] + thr_raw;
                 m_neg[gi] = m_run[gi] == kNegInf ? 0.0f : -m_run[gi] * c_log2;  // no key yet: every p is 0
                 if constexpr (SH) m_neg[gi] += kRerunShift;
+                if constexpr (UNITS)
+                {
+                    m_neg[gi] += units[gi].shift;
+                    units[gi].known *= alpha;
+                }
             }
 #pragma unroll
             for (int e = 0; e < KP * 4; ++e)
@@ -1288,6 +1297,34 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
                             for (int i = 0; i < 4; ++i)
                                 pv[gi][4 * u + i] = s[gi][u][i] == kNegInf ? 0.0f : pv[gi][4 * u + i];
                 }
+            if constexpr (UNITS)
+            {
+                float w[RG];
+                bool  out = false;
+#pragma unroll
+                for (int gi = 0; gi < RG; ++gi)
+                {
+                    w[gi] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < KP * 4; ++e) w[gi] = fmaxf(w[gi], __builtin_fabsf(pv[gi][e]));
+                    out = out || w[gi] > units[gi].limit();
+                }
+                if (__any(out))
+                {
+#pragma unroll
+                    for (int gi = 0; gi < RG; ++gi)
+                    {
+                        const float was = units[gi].shift;
+                        const float f = new_units(units[gi], swap_max(w[gi]));
+                        m_neg[gi] += units[gi].shift - was;
+                        l_run[gi] *= f;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) acc[gi][n] *= f;
+#pragma unroll
+                        for (int e = 0; e < KP * 4; ++e) pv[gi][e] *= f;
+                    }
+                }
+            }
         }
     };
 
@@ -1556,6 +1593,7 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
             m_thr[gi] = kNegInf;
             m_neg[gi] = 0.0f;
             l_run[gi] = 0.0f;
+            if constexpr (UNITS) units[gi] = ValueUnits{};
             lacc[gi] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[gi][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1620,6 +1658,10 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
         if (s_vover != 0)              // uniform: some V value of the workgroup's keys does not fit f16
             pipeline.template operator()<false, false, CAN_CF>();
     }
+    else if constexpr (UNITS)
+    {
+        pipeline.template operator()<false, false>();
+    }
     else if constexpr (CT == I8)
     {
         // int8 pages: P carries the keys' V scales into the f16 PV products and p < 2^8, so a V scale of 256 or
@@ -1636,15 +1678,9 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
             if (again)
             {
                 bool big = false;
-                for (int t = pg_lo * kBlockSize + lane; t < (LIST ? pg_hi * kBlockSize : min(pg_hi * kBlockSize, L)); t += 64)
+                for (int t = pg_lo * kBlockSize + lane; t < min(pg_hi * kBlockSize, L); t += 64)
                 {
-                    int lp = t / kBlockSize;
-                    if constexpr (LIST)
-                    {
-                        lp = list[lp];
-                        if (lp < 0 || lp >= a.max_blocks || static_cast<int64_t>(lp) * kBlockSize + t % kBlockSize >= L) continue;
-                    }
-                    const uint32_t pg = static_cast<uint32_t>(table_row[lp]);
+                    const uint32_t pg = static_cast<uint32_t>(table_row[t / kBlockSize]);
                     if (pg >= static_cast<uint32_t>(a.num_blocks)) continue;
                     const float vs = __builtin_fabsf(a.v_scale[(static_cast<size_t>(pg) * kBlockSize + t % kBlockSize) * Hkv + kvh]);
                     big = big || (vs >= 255.0f && vs < __builtin_huge_valf());
@@ -1672,6 +1708,13 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
         pipeline.template operator()<false, false>();
     }
 
+    // A column's maximum in the log2 domain, in the units of its P.
+    auto col_max = [&](int gi)
+    {
+        float shift = CT == I8 && s_vover != 0 ? kRerunShift : 0.0f;  // (a rerun of int8 pages)
+        if constexpr (UNITS) shift = units[gi].shift;
+        return m_run[gi] == kNegInf ? kNegInf : m_run[gi] * c_log2 - shift;
+    };
     if constexpr (PAIR)
     {
         // the second half's states through the stages, some output tiles of all rows at a time, and the first half's output
@@ -1701,7 +1744,7 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
                     for (int n = 0; n < NPR; ++n) s_o[(rg * NPR + n) * 64 + lane] = acc[gi][n0 + n];
                     const float l_tot = swap_sum(l_run[gi]) + lacc[gi][0];
                     if (n0 == 0 && g == 0)
-                        s_s[16 * rg + c] = float2{m_run[gi] == kNegInf ? kNegInf : m_run[gi] * c_log2, l_tot};
+                        s_s[16 * rg + c] = float2{col_max(gi), l_tot};
                 }
             }
             wait_lgkm0();
@@ -1714,7 +1757,7 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
                 if (n0 == 0)
                 {
                     const float  l_tot = swap_sum(l_run[gi]) + lacc[gi][0];
-                    const float  m0 = m_run[gi] == kNegInf ? kNegInf : m_run[gi] * c_log2;
+                    const float  m0 = col_max(gi);
                     const float2 other = s_s[16 * rg + c];
                     const float  m = fmaxf(fmaxf(m0, other.x), kLowest);
                     w0[gi] = __builtin_amdgcn_exp2f(m0 - m);
@@ -1768,11 +1811,7 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
 #pragma unroll
                 for (int n = 0; n < NT; ++n) dst[n * 64] = acc[gi][n] * piece_scale;
                 if (g == 0)
-                {
-                    const float shift = CT == I8 && s_vover != 0 ? kRerunShift : 0.0f;
-                    const float m = m_run[gi] == kNegInf ? kNegInf : m_run[gi] * c_log2 - shift;
-                    reinterpret_cast<float2*>(a.ws_ml)[part * kDmaRows + 16 * rg + c] = float2{m, l_tot};
-                }
+                    reinterpret_cast<float2*>(a.ws_ml)[part * kDmaRows + 16 * rg + c] = float2{col_max(gi), l_tot};
             }
         }
         else if (col_ok[gi])

@@ -89,3 +89,22 @@ def int8_of_all_sizes(ff, gpu, big, Hq, Hkv, D, ctx, S, count, T):
 @pytest.mark.parametrize("form", STEPS)
 def test_int8_steps_of_all_sizes(ff, gpu, big, form):
     int8_of_all_sizes(ff, gpu, big, *form)
+
+TILES = [  # whole, in halves, split over their lists
+    (8, 2, 128, [257], 270, 8, 2), (10, 2, 256, [700, 15], 140, 30, 40), (32, 1, 64, [500], 520, 21, 9),
+    (36, 9, 128, [1100, 1300], 120, 61, 16), (24, 12, 64, [1700, 900], 130, 107, 16),
+    (8, 2, 128, [2500, 40, 1200], 40, 150, 32), (5, 1, 64, [3000], 107, 170, 7), (20, 4, 256, [1531, 1908], 31, 100, 13),
+]
+
+
+@pytest.mark.parametrize("act,kv", [k for k in KV if k[1] != "bf16"])
+@pytest.mark.parametrize("by", [2.0 ** -10, 2.0 ** -17, 2.0 ** -40])
+@pytest.mark.parametrize("form", TILES)
+def test_tiles(ff, gpu, act, kv, by, form):
+    small(ff, gpu, act, kv, by, *form)
+
+
+@pytest.mark.parametrize("big", [1.0, 3000.0, 2.0 ** 30])
+@pytest.mark.parametrize("form", TILES)
+def test_int8_tiles_of_all_sizes(ff, gpu, big, form):
+    int8_of_all_sizes(ff, gpu, big, *form)
