@@ -1649,13 +1649,35 @@ __device__ __forceinline__ void prefill_wg(std::conditional_t<LIST, ListPrefillA
                 for (int i = 0; i < 4; ++i) t = __builtin_fmaf(acc[gi][n][i], 0.0f, t);
         return !__any(!(t == 0.0f));
     };
+    // LIST: some query's largest output lies below 2^-14 (values of zero among them).
+    auto small_out = [&]() -> bool
+    {
+        bool small = false;
+#pragma unroll
+        for (int gi = 0; gi < RG; ++gi)
+        {
+            float w = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w = fmaxf(w, __builtin_fabsf(acc[gi][n][i]));
+            w = swap_max(w);
+            const float l = swap_sum(l_run[gi]);
+            small = small || (col_ok[gi] && w < l * 0x1p-14f);
+        }
+        return __any(small);
+    };
     if constexpr (VCONV)
     {
+        // (A list's values may all be small: V rounded to f16 is off by at most 2^-25, 2^-11 of an output of 2^-14.  The scored
+        // and the plain prefill keep that error at any size.)
         pipeline.template operator()<true, false>();
-        if (!acc_finite()) s_vover = 1;
+        bool again = !acc_finite();
+        if constexpr (LIST) again = again || small_out();
+        if (again) s_vover = 1;
         wait_lgkm0();
         __builtin_amdgcn_s_barrier();  // flags written; every wave is past its last reads of the stages
-        if (s_vover != 0)              // uniform: some V value of the workgroup's keys does not fit f16
+        if (s_vover != 0)              // uniform: some V values of the workgroup's keys do not fit f16
             pipeline.template operator()<false, false, CAN_CF>();
     }
     else if constexpr (UNITS)

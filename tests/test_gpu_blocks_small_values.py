@@ -97,7 +97,7 @@ TILES = [  # whole, in halves, split over their lists
 ]
 
 
-@pytest.mark.parametrize("act,kv", [k for k in KV if k[1] != "bf16"])
+@pytest.mark.parametrize("act,kv", KV)
 @pytest.mark.parametrize("by", [2.0 ** -10, 2.0 ** -17, 2.0 ** -40])
 @pytest.mark.parametrize("form", TILES)
 def test_tiles(ff, gpu, act, kv, by, form):
