@@ -11,8 +11,8 @@
 // same order; the two that sum queries differ by 2^-50 of a sum at most, far below the rounding's step.
 //
 // Of a block's pages - those up to its last query's - the first `sinks` and the last `recent` are taken, and of the rest
-// those with the largest scores, of equal ones the lower; NaN (a NaN or infinite key) counts as the largest.  The list is in
-// ascending order, -1 behind.
+// those with the largest scores, of equal ones the lower; NaN (a NaN key, or infinite ones that cancel) counts as the largest.
+// The list is in ascending order, -1 behind.
 //
 // The bounds are read once (an eighth of K; in 8-bit caches a quarter), 4 bytes a page and list are written and read again: HBM
 // for long rows, and two or three launches with their chains of loads (few lists of few pages: one).
@@ -163,6 +163,51 @@ __device__ __forceinline__ double lane_score(const double (&down)[8], const doub
     return s;
 }
 
+// The same for a score that came out NaN: a sum of 0 takes nothing of an infinite bound (0 * inf is NaN).  The asm keeps this rare
+// case's comparisons out of the loops around it (they took 70 registers there).
+__device__ __forceinline__ double sum_times(double q, double bound)
+{
+    asm volatile("" : "+v"(q), "+v"(bound));
+    return q == 0.0 && __builtin_isinf(bound) ? 0.0 : bound;
+}
+__device__ __forceinline__ double lane_score_infinite(const double (&down)[8], const double (&up)[8], const double (&lo)[8],
+                                                      const double (&hi)[8])
+{
+    double s = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+    {
+        s = __builtin_fma(down[e], sum_times(down[e], lo[e]), s);
+        s = __builtin_fma(up[e], sum_times(up[e], hi[e]), s);
+    }
+    return s;
+}
+
+// The scores of four pages, that of page k in the lanes of the group with c % 4 == k; values(k, rare, lo, hi) gives their bounds.
+template <int LPP, typename F>
+__device__ __forceinline__ double page_scores(const double (&down)[8], const double (&up)[8], int c, F values)
+{
+    double s[kScorePages], lo[8], hi[8];
+#pragma unroll
+    for (int k = 0; k < kScorePages; ++k)
+    {
+        values(k, std::false_type{}, lo, hi);
+        s[k] = lane_score(down, up, lo, hi);
+    }
+    double sum = group_sums4<LPP>(s, c);
+    if (__builtin_expect(__any(sum != sum), 0))
+    {
+#pragma unroll
+        for (int k = 0; k < kScorePages; ++k)
+        {
+            values(k, std::true_type{}, lo, hi);
+            s[k] = lane_score_infinite(down, up, lo, hi);
+        }
+        sum = group_sums4<LPP>(s, c);
+    }
+    return sum;
+}
+
 // Four pages' bounds in flight.  FULL: head_dim fills the LPP lanes.  Pages on no table entry read page 0 instead (a pool has
 // one), and lanes past head_dim the first dims: their scores are not used, their sums of queries zero.
 template <int BT, int LPP, bool FULL>
@@ -195,11 +240,17 @@ struct PageBounds
             load_raw8<BT>(at, D, hi[k]);
         }
     }
+    // RARE: as for the first time (the values of four pages would fill 128 registers from one use to the next).
+    template <bool RARE = false>
     __device__ __forceinline__ void values(int k, bool in, double (&l)[8], double (&h)[8]) const
     {
+        Raw8 a = lo[k], b = hi[k];
+        if constexpr (RARE)
+#pragma unroll
+            for (int i = 0; i < (BT == F32 ? 8 : 4); ++i) asm volatile("" : "+v"(a.w[i]), "+v"(b.w[i]));
         float x[8], y[8];
-        unpack8<BT>(lo[k], x);
-        unpack8<BT>(hi[k], y);
+        unpack8<BT>(a, x);
+        unpack8<BT>(b, y);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
         {
@@ -327,15 +378,10 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a,
         if (x + 1 < x1) nxt.load(a, phys, ahead.hb * heads + hd, c);
         const Place after = next(ahead);
         if (x + 2 < x1) entries(after);
-        double s[kScorePages];
-#pragma unroll
-        for (int k = 0; k < kScorePages; ++k)
+        const double sum = page_scores<LPP>(down, up, c, [&](int k, auto rare, double (&lo)[8], double (&hi)[8])
         {
-            double lo[8], hi[8];
-            cur.values(k, in, lo, hi);
-            s[k] = lane_score(down, up, lo, hi);
-        }
-        const double sum = group_sums4<LPP>(s, c);
+            cur.template values<decltype(rare)::value>(k, in, lo, hi);
+        });
         const int    p = at.round * ROUND + grp * kScorePages + (c & 3);
         float*       out = a.scores + (static_cast<int64_t>(at.b) * a.num_kv_heads + at.hb * heads + hd) * a.stride;
         // (behind the row's last page up to stride: read by nobody)
@@ -434,6 +480,7 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_lists(SelectArgs a
     PageBounds<BT, LPP, FULL> raw;
     raw.load(a, phys, kvh, c);
     double lo[kScorePages][8], hi[kScorePages][8];
+    uint64_t again = 0;  // some score of the wave is NaN
     for (int m0 = l0; m0 < l1; m0 += LISTS)
     {
         const int m1 = min(l1, m0 + LISTS);
@@ -462,8 +509,55 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_lists(SelectArgs a
 #pragma unroll
             for (int k = 0; k < kScorePages; ++k) s[k] = lane_score(down, up, lo[k], hi[k]);
             const double sum = group_sums4<LPP>(s, c);
+            again |= __ballot(sum != sum);
             float*       out = a.scores + ((static_cast<int64_t>(b) * a.lists + l) * a.num_kv_heads + kvh) * a.stride;
             if (c < 4 && p + c < n) out[p + c] = raw.on >> c & 1 ? static_cast<float>(sum) : kNegInf;
+        }
+    }
+    if (again == 0) return;
+    // Infinite or NaN bounds: all from the start, a page at a time, the lane's places too (what is kept for this rare case takes
+    // registers from the loop above, and a wave a SIMD: 8 % of the time and more).
+    int id = tid;
+    asm volatile("" : "+v"(id));
+    const int  c1 = id % LPP, first = p0 + id / LPP * kScorePages;
+    const bool in1 = FULL || 8 * c1 < D;
+#pragma unroll 1
+    for (int l = l0; l < l1; ++l)
+    {
+        const int n = visible_pages(a, b, l);
+        if (p0 >= n) continue;
+        const int64_t row = (static_cast<int64_t>(b) * a.lists + l) * a.num_kv_heads + kvh;
+        const double* q = a.query_sums + row * 2 * D + (in1 ? 8 * c1 : 0);
+        double        down[8], up[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            down[e] = in1 ? q[e] : 0.0;
+            up[e] = in1 ? q[D + e] : 0.0;
+        }
+#pragma unroll 1
+        for (int k = 0; k < kScorePages; ++k)
+        {
+            const int at = first + k;
+            const int page = at < n ? a.block_table[static_cast<int64_t>(b) * a.max_blocks + at] : -1;
+            const bool on = page >= 0 && page < a.num_blocks;
+            const size_t base = (static_cast<size_t>(on ? page : 0) * a.num_kv_heads + kvh) * 2 * D + (in1 ? 8 * c1 : 0);
+            Raw8   x, y;
+            double l8[8], h8[8];
+            load_raw8<BT>(a.bounds, base, x);
+            load_raw8<BT>(a.bounds, base + D, y);
+            float fx[8], fy[8];
+            unpack8<BT>(x, fx);
+            unpack8<BT>(y, fy);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                l8[e] = in1 ? fx[e] : 0.0f;
+                h8[e] = in1 ? fy[e] : 0.0f;
+            }
+            const double one[kScorePages] = {lane_score_infinite(down, up, l8, h8), 0.0, 0.0, 0.0};
+            const double sum = group_sums4<LPP>(one, c1);
+            if (c1 == 0 && at < n) a.scores[row * a.stride + at] = on ? static_cast<float>(sum) : kNegInf;
         }
     }
 }
@@ -768,15 +862,10 @@ __global__ __launch_bounds__(kOneThreads) void block_select_one(SelectArgs a)
     {
         if (r + 1 < rounds) nxt.load(a, phys, kvh, c);
         if (r + 2 < rounds) Bounds::entries(table, (r + 2) * ROUND + grp * kScorePages, n, phys);
-        double s[kScorePages];
-#pragma unroll
-        for (int k = 0; k < kScorePages; ++k)
+        const double sum = page_scores<LPP>(down, up, c, [&](int k, auto rare, double (&lo)[8], double (&hi)[8])
         {
-            double lo[8], hi[8];
-            cur.values(k, in, lo, hi);
-            s[k] = lane_score(down, up, lo, hi);
-        }
-        const double sum = group_sums4<LPP>(s, c);
+            cur.template values<decltype(rare)::value>(k, in, lo, hi);
+        });
         const int    p = r * ROUND + grp * kScorePages + (c & 3);
         if (c < 4 && p < n) s_scores[p] = cur.on >> c & 1 ? static_cast<float>(sum) : kNegInf;  // on no page: last
         cur = nxt;
