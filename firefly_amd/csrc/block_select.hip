@@ -7,8 +7,9 @@
 // block of any size costs two dot products of head_dim per page.
 //
 // Scores are fp64 sums rounded once to fp32: they decide between pages, and a row's choice must not depend on the rest of the
-// batch or on how the pages are dealt out.  Products of 16-bit values are exact in fp64, and every form adds up a score in the
-// same order; the two that sum queries differ by 2^-50 of a sum at most, far below the rounding's step.
+// batch or on how the pages are dealt out.  So every form adds up a score in the same order, and the sums over queries too, by
+// the query rows of a block: up to kOwnRows one after the other, up to kWideRows by the groups of lanes of 512 threads, every
+// so many-th row each, joined wave by wave, more by those of 1024.
 //
 // Of a block's pages - those up to its last query's - the first `sinks` and the last `recent` are taken, and of the rest
 // those with the largest scores, of equal ones the lower; NaN (a NaN key, or infinite ones that cancel) counts as the largest.
@@ -31,7 +32,8 @@ constexpr int kScoreThreads = 256;
 constexpr int kScorePages = 4;  // neighbouring pages that a group of lanes scores together
 constexpr int kOneThreads = 512;
 constexpr int kOneRounds = 4;  // of block_select_one at most
-constexpr int kOwnRows = 8;  // query rows that every lane adds up by itself
+constexpr int kOwnRows = 8;    // query rows of a block that are added up one after the other
+constexpr int kWideRows = 256;  // more of them than that are added up by twice the threads
 
 template <int CTRL>
 __device__ __forceinline__ double dpp64(double v)
@@ -397,14 +399,60 @@ __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a,
     }
 }
 
-// Q- and Q+ of every block of queries and KV head, a workgroup each (2 x 512 tokens, 32/8 heads of 128 in blocks of 64: 7.2 us,
-// where the workgroups that score would read a block's queries once for every 64 pages).
-constexpr int kSumThreads = 1024;
-template <int QT, int LPP>
-__global__ __launch_bounds__(kSumThreads) void block_queries(SelectArgs a)
+// Query rows of a whole block: what the order of its sums goes by (and that of a shorter last block).
+__device__ __host__ __forceinline__ int64_t block_rows(int query_block, int seq_len, int group)
 {
-    constexpr int WAVES = kSumThreads / 64;
-    constexpr int STEP = kSumThreads / LPP;  // query rows that the workgroup takes at a time
+    return static_cast<int64_t>(query_block < seq_len ? query_block : seq_len) * group;
+}
+
+// Few query rows a block: Q- and Q+ by LPP lanes for each block and KV head, the rows one after the other.
+template <int QT, int LPP>
+__global__ __launch_bounds__(kScoreThreads) void block_queries_few(SelectArgs a, uint32_t sums)
+{
+    const uint32_t i = blockIdx.x * (kScoreThreads / LPP) + threadIdx.x / LPP;
+    const int      c = static_cast<int>(threadIdx.x) % LPP;
+    if (i >= sums || 8 * c >= a.head_dim) return;
+    const Split u = split_index(i, a.num_kv_heads), v = split_index(u.div, a.lists);
+    const int   kvh = u.rem, b = static_cast<int>(v.div);
+    const int   t0 = v.rem * a.query_block;
+    const int   rows = min(a.query_block, a.seq_len - t0) * a.group;
+    constexpr int UN = 4;
+    double      down[8], up[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) down[e] = up[e] = 0.0;
+    for (int r0 = 0; r0 < rows; r0 += UN)
+    {
+        Raw8 q[UN];
+#pragma unroll
+        for (int k = 0; k < UN; ++k)
+            if (r0 + k < rows) load_raw8<QT>(a.q, query_at(a, b, t0, kvh, r0 + k, c), q[k]);
+#pragma unroll
+        for (int k = 0; k < UN; ++k)
+            if (r0 + k < rows)
+            {
+                float x[8];
+                unpack8<QT>(q[k], x);
+                add_query(x, down, up);
+            }
+    }
+    double* out = a.query_sums + static_cast<int64_t>(i) * 2 * a.head_dim + 8 * c;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+    {
+        out[e] = down[e];
+        out[a.head_dim + e] = up[e];
+    }
+}
+
+// More of them: Q- and Q+ of every block of queries and KV head, a workgroup each (2 x 512 tokens, 32/8 heads of 128 in blocks of
+// 64: 7.2 us, where the workgroups that score would read a block's queries once for every 64 pages).  Whole calls over 2000 pages
+// by 512 and 1024 threads: blocks of 16 tokens 48.8 and 50.7 us, 64 23.4 and 23.0, 128 23.5 and 22.4, 512 41.4 and 36.7; blocks of
+// 4 146 and 156, of 1 in the form above 528 and (here) 585.  Few lists in one launch take 1024 in two turns: 64 tokens 11.6 and 12.9.
+template <int QT, int LPP, int THREADS>
+__global__ __launch_bounds__(THREADS) void block_queries(SelectArgs a)
+{
+    constexpr int WAVES = THREADS / 64;
+    constexpr int STEP = THREADS / LPP;  // query rows that the workgroup takes at a time
     constexpr int UN = 4;
     __shared__ double s_part[WAVES][2][LPP * 8];
     const int64_t wg = blockIdx.x;
@@ -443,7 +491,7 @@ __global__ __launch_bounds__(kSumThreads) void block_queries(SelectArgs a)
             s_part[wave][1][8 * c + e] = up[e];
         }
     __syncthreads();
-    for (int i = tid; i < 2 * a.head_dim; i += kSumThreads)
+    for (int i = tid; i < 2 * a.head_dim; i += THREADS)
     {
         const int half = i >= a.head_dim, d = i - half * a.head_dim;
         double    s = 0.0;
@@ -782,7 +830,7 @@ __global__ __launch_bounds__(kOneThreads) void block_select_one(SelectArgs a)
     constexpr int SLOTS = kOneThreads / LPP;      // groups of lanes
     constexpr int ROUND = SLOTS * kScorePages;    // pages of a round
     constexpr int UN = 4;                         // query rows whose loads go out together
-    constexpr int PARTS = WAVES * 2 * LPP * 8 * 8, CHOOSE = static_cast<int>(sizeof(ChooseLds<kOneThreads>));
+    constexpr int PARTS = 2 * WAVES * 2 * LPP * 8 * 8, CHOOSE = static_cast<int>(sizeof(ChooseLds<kOneThreads>));
     static_assert(kOneRounds * ROUND <= kOneThreads * PER, "the choice holds all scores");
     __shared__ __align__(16) float s_scores[kOneThreads * PER];
     __shared__ __align__(16) uint8_t s_mem[PARTS > CHOOSE ? PARTS : CHOOSE];
@@ -811,43 +859,55 @@ __global__ __launch_bounds__(kOneThreads) void block_select_one(SelectArgs a)
 
     const int t0 = list * a.query_block;
     const int rows = min(a.query_block, a.seq_len - t0) * a.group;
-    const bool few = rows <= kOwnRows;  // every lane adds up its dims of all rows; else the groups of lanes share the rows
+    const int64_t whole = block_rows(a.query_block, a.seq_len, a.group);
     double    down[8], up[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) down[e] = up[e] = 0.0;
-    const int step = few ? 1 : SLOTS;
-    for (int r0 = few ? 0 : grp; r0 < rows; r0 += UN * step)
+    auto sum_rows = [&](int first, int step)
     {
-        Raw8 q[UN];
 #pragma unroll
-        for (int k = 0; k < UN; ++k)
-            if (r0 + k * step < rows && in) load_raw8<QT>(a.q, query_at(a, b, t0, kvh, r0 + k * step, c), q[k]);
+        for (int e = 0; e < 8; ++e) down[e] = up[e] = 0.0;
+        for (int r0 = first; r0 < rows; r0 += UN * step)
+        {
+            Raw8 q[UN];
 #pragma unroll
-        for (int k = 0; k < UN; ++k)
-            if (r0 + k * step < rows && in)
-            {
-                float x[8];
-                unpack8<QT>(q[k], x);
-                add_query(x, down, up);
-            }
-    }
-    if (!few)
+            for (int k = 0; k < UN; ++k)
+                if (r0 + k * step < rows && in) load_raw8<QT>(a.q, query_at(a, b, t0, kvh, r0 + k * step, c), q[k]);
+#pragma unroll
+            for (int k = 0; k < UN; ++k)
+                if (r0 + k * step < rows && in)
+                {
+                    float x[8];
+                    unpack8<QT>(q[k], x);
+                    add_query(x, down, up);
+                }
+        }
+    };
+    if (whole <= kOwnRows)
+        sum_rows(0, 1);  // every lane its dims of all rows
+    else
     {
-        double* s_part = reinterpret_cast<double*>(s_mem);  // [wave][2][LPP * 8]
-        wave_sums<LPP>(down, up);
-        if (lane < LPP)
+        // in the order of block_queries, twice the threads in two turns
+        double*   s_part = reinterpret_cast<double*>(s_mem);  // [wave][2][LPP * 8]
+        const int turns = whole <= kWideRows ? 1 : 2;
+#pragma unroll 1
+        for (int turn = 0; turn < turns; ++turn)
+        {
+            sum_rows(turn * SLOTS + grp, turns * SLOTS);
+            wave_sums<LPP>(down, up);
+            if (lane < LPP)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-            {
-                s_part[(wave * 2 + 0) * (LPP * 8) + 8 * c + e] = down[e];
-                s_part[(wave * 2 + 1) * (LPP * 8) + 8 * c + e] = up[e];
-            }
+                for (int e = 0; e < 8; ++e)
+                {
+                    s_part[((turn * WAVES + wave) * 2 + 0) * (LPP * 8) + 8 * c + e] = down[e];
+                    s_part[((turn * WAVES + wave) * 2 + 1) * (LPP * 8) + 8 * c + e] = up[e];
+                }
+        }
         __syncthreads();
         double s = 0.0;  // (as many threads as sums, or more)
         static_assert(2 * LPP * 8 <= kOneThreads, "a sum per thread");
         if (tid < 2 * LPP * 8)
+            for (int turn = 0; turn < turns; ++turn)
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) s += s_part[w * (2 * LPP * 8) + tid];
+                for (int w = 0; w < WAVES; ++w) s += s_part[(turn * WAVES + w) * (2 * LPP * 8) + tid];
         __syncthreads();
         if (tid < 2 * LPP * 8) s_part[tid] = s;
         __syncthreads();
@@ -902,7 +962,16 @@ hipError_t launch_scores_l(const SelectArgs& a, hipStream_t stream)
                            stream, a, heads);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL((block_queries<QT, LPP>), dim3(static_cast<unsigned>(rows * a.lists)), dim3(kSumThreads), 0, stream, a);
+    const uint32_t sums = static_cast<uint32_t>(rows * a.lists);
+    constexpr uint32_t FEW = kScoreThreads / LPP;  // blocks of queries of a workgroup
+    const int64_t  query_rows = block_rows(a.query_block, a.seq_len, a.group);
+    if (query_rows <= kOwnRows)
+        hipLaunchKernelGGL((block_queries_few<QT, LPP>), dim3(sums / FEW + (sums % FEW != 0)), dim3(kScoreThreads), 0, stream, a,
+                           sums);
+    else if (query_rows <= kWideRows)
+        hipLaunchKernelGGL((block_queries<QT, LPP, kOneThreads>), dim3(sums), dim3(kOneThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL((block_queries<QT, LPP, 2 * kOneThreads>), dim3(sums), dim3(2 * kOneThreads), 0, stream, a);
     // blocks of queries that a workgroup goes through: as many as leave two workgroups per CU
     const int64_t per = std::max<int64_t>(1, std::min<int64_t>(a.lists, (rows * all * a.lists + 511) / 512));
     const int64_t parts = (a.lists + per - 1) / per;

@@ -56,3 +56,46 @@ def test_infinite_bounds(ff, gpu, act, dtype, Hq, Hkv, D, S, ctx, T, wide):
     with np.errstate(invalid="ignore"):
         want = bu.select(cases.decode(q, c.act).astype(np.float64), flat, c.block_table, c.ctx, 23, 1, 3, T, c.num_blocks)
     assert np.array_equal(got, want)
+
+
+def beside(rng, D, dev, rows, T, pages=60):
+    """Row 0's case for any batch: `rows` of the block's query rows in fp32, and two kinds of page whose scores differ by a rounding."""
+    S = T
+    q = np.zeros((1, S, 1, D), np.float32)
+    for at, v in rows:
+        q[0, at, 0, 0] = v
+    q[0, 0, 0, 1] = 1.0  # what the other kind's score is
+    box = np.zeros((pages, 1, 2, D), np.float32)
+    box[::2, 0, 1, 1] = 1.0
+    box[1::2, 0, 1, 0] = 1.0
+    return q, box, np.arange(pages, dtype=np.int32)[None]
+
+
+# One, half a step of fp32 beside it, and values that fp64 keeps beside that if they are added up first: which of the two kinds of
+# page comes first hangs on the order of the sum.
+TINY = [(0, 1.0), (1, 2.0 ** -24)]
+
+
+@pytest.mark.parametrize("rows,T", [
+    (TINY + [(2, 1.5 * 2.0 ** -54), (3, 1.5 * 2.0 ** -54)], 4),       # few query rows: one after the other
+    (TINY + [(i, 2.0 ** -54) for i in (32, 96, 160, 224)], 256), (TINY + [(i, 2.0 ** -54) for i in (16, 48, 80, 112)], 128),
+    (TINY + [(i, 2.0 ** -54) for i in (64, 192, 320, 448)], 512), (TINY + [(i, 2.0 ** -54) for i in (2, 3, 6, 7)], 9),
+    (TINY + [(i, 2.0 ** -54) for i in (32, 96, 160, 224)], 700), (TINY + [(i, 2.0 ** -54) for i in (64, 192, 320, 448)], 700),
+])
+@pytest.mark.parametrize("D", [64, 128, 256, 80])
+@pytest.mark.parametrize("blocks", [1, 2])
+def test_choice_does_not_hang_on_the_batch(ff, gpu, rows, T, D, blocks):
+    """fp32 queries: a row's lists alone, with its block of queries once and twice, and beside 300 others."""
+    rng = np.random.default_rng(1)
+    q, box, table = beside(rng, D, gpu, rows, T)
+    got = []
+    for B in (1, 300):
+        for wide in (0, 3000):
+            for n in (1, blocks):
+                tab = np.full((B, max(60, wide)), -1, np.int32)
+                tab[:, :60] = table
+                li = ff.select_blocks(up(np.tile(q, (B, n, 1, 1)), gpu), up(box, gpu), up(tab, gpu),
+                                      up(np.full(B, 60 * 16 - T * n, np.int32), gpu), 20, sinks=0, recent=0, query_block=T)
+                got.append(li[0, -1, 0].cpu().numpy())  # (the last block sees all pages)
+                assert (li == li[:1]).all()
+    assert all(np.array_equal(g, got[0]) for g in got[1:]), got
