@@ -939,6 +939,22 @@ __global__ __launch_bounds__(kOneThreads) void block_select_one(SelectArgs a)
 namespace
 {
 
+// Lanes that hold a page's bounds.
+int bound_lanes(int head_dim) { return head_dim <= 64 ? 8 : (head_dim <= 128 ? 16 : 32); }
+
+// Blocks of queries that a workgroup of block_scores_lists goes through, over `tiles` rounds of a row: as many as leave two
+// workgroups per CU.
+int64_t lists_of_workgroup(const SelectArgs& a, int64_t tiles)
+{
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.num_kv_heads;
+    return std::max<int64_t>(1, std::min<int64_t>(a.lists, (rows * tiles * a.lists + 511) / 512));
+}
+
+// Threads of block_choose: the fewest that hold a row in registers; a longer row is read again for every pass.  (Whole calls of 2
+// rows, 8 heads, by 256, 512 and 1024 threads: 1000 pages 10.1, 11.1, 12.0 us; 2000 13.3, 12.0, 13.0; 4000 21.0, 16.2, 16.7; 8187
+// 34.3, 25.1, 21.6.)
+int choose_threads(int most_pages) { return most_pages <= 1024 ? 256 : (most_pages <= 4096 ? 512 : 1024); }
+
 template <int BT, int QT, int LPP, bool FULL>
 hipError_t launch_scores_l(const SelectArgs& a, hipStream_t stream)
 {
@@ -972,10 +988,7 @@ hipError_t launch_scores_l(const SelectArgs& a, hipStream_t stream)
         hipLaunchKernelGGL((block_queries<QT, LPP, kOneThreads>), dim3(sums), dim3(kOneThreads), 0, stream, a);
     else
         hipLaunchKernelGGL((block_queries<QT, LPP, 2 * kOneThreads>), dim3(sums), dim3(2 * kOneThreads), 0, stream, a);
-    // blocks of queries that a workgroup goes through: as many as leave two workgroups per CU
-    const int64_t per = std::max<int64_t>(1, std::min<int64_t>(a.lists, (rows * all * a.lists + 511) / 512));
-    const int64_t parts = (a.lists + per - 1) / per;
-    if (rows * parts * all > INT32_MAX) return hipErrorInvalidConfiguration;
+    const int64_t per = lists_of_workgroup(a, all), parts = (a.lists + per - 1) / per;
     hipLaunchKernelGGL((block_scores_lists<BT, LPP, FULL>), dim3(static_cast<unsigned>(rows * parts * all)), dim3(kScoreThreads), 0,
                        stream, a, static_cast<int>(all), static_cast<int>(per), static_cast<int>(parts));
     return hipGetLastError();
@@ -1015,15 +1028,27 @@ bool select_by_lists(int seq_len, int lists, int group) { return lists > 1 || st
 bool select_in_one(const SelectArgs& a)
 {
     const int64_t lists = static_cast<int64_t>(a.batch) * a.lists * a.num_kv_heads;
-    const int     lanes = a.head_dim <= 64 ? 8 : (a.head_dim <= 128 ? 16 : 32);
     const int     rounds = select_by_lists(a.seq_len, a.lists, a.group) ? kOneRounds : 2;
-    return lists <= 256 && a.most_pages <= rounds * (kOneThreads / lanes * kScorePages);
+    return lists <= 256 && a.most_pages <= rounds * (kOneThreads / bound_lanes(a.head_dim) * kScorePages);
+}
+
+int64_t select_threads(const SelectArgs& a)
+{
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.num_kv_heads, lists = rows * a.lists;
+    const int64_t choose = lists * choose_threads(a.most_pages);
+    if (a.most_pages <= a.count || select_in_one(a) || !select_by_lists(a.seq_len, a.lists, a.group)) return choose;
+    const int64_t round = kScoreThreads / bound_lanes(a.head_dim) * kScorePages;
+    const int64_t tiles = (a.most_pages + round - 1) / round, per = lists_of_workgroup(a, tiles);
+    const int64_t scores = rows * ((a.lists + per - 1) / per) * tiles * kScoreThreads;
+    const int64_t query_rows = block_rows(a.query_block, a.seq_len, a.group);
+    const int64_t sums = query_rows <= kOwnRows ? 0 : lists * (query_rows <= kWideRows ? 1 : 2) * kOneThreads;
+    return std::max(choose, std::max(scores, sums));
 }
 
 hipError_t launch_select(const SelectArgs& a, hipStream_t stream)
 {
     const int64_t lists = static_cast<int64_t>(a.batch) * a.lists * a.num_kv_heads;
-    if (lists > INT32_MAX) return hipErrorInvalidConfiguration;
+    if (select_threads(a) > kMostThreads) return hipErrorInvalidConfiguration;
     hipError_t e = hipSuccess;
     // (rows that cannot have more pages than are taken need no scores)
     if (a.most_pages > a.count)
@@ -1032,12 +1057,10 @@ hipError_t launch_select(const SelectArgs& a, hipStream_t stream)
                                     : launch_scores<BF16>(a, stream);
     if (e != hipSuccess || (a.most_pages > a.count && select_in_one(a))) return e;
     const dim3 grid(static_cast<unsigned>(lists));
-    // The smallest that holds a row in registers; one that does not reads it again for every pass.  (Whole calls of 2 rows, 8
-    // heads, by 256, 512 and 1024 threads: 1000 pages 10.1, 11.1, 12.0 us; 2000 13.3, 12.0, 13.0; 4000 21.0, 16.2, 16.7; 8187
-    // 34.3, 25.1, 21.6.)
-    if (a.most_pages <= 1024)
+    const int threads = choose_threads(a.most_pages);
+    if (threads == 256)
         hipLaunchKernelGGL((block_choose<256, 4>), grid, dim3(256), 0, stream, a);
-    else if (a.most_pages <= 4096)
+    else if (threads == 512)
         hipLaunchKernelGGL((block_choose<512, 8>), grid, dim3(512), 0, stream, a);
     else
         hipLaunchKernelGGL((block_choose<1024, 8>), grid, dim3(1024), 0, stream, a);

@@ -148,6 +148,11 @@ void         set_blocks_workspace(BlocksArgs& a, const BlocksLayout& l, void* ws
 hipError_t launch_rope_axes(const RopeAxesArgs& a, hipStream_t stream);
 hipError_t launch_key_bounds(const KeyBoundsArgs& a, hipStream_t stream);
 bool       select_by_lists(int seq_len, int lists, int group);  // whether the choice takes query_sums
+constexpr int64_t kMostThreads = UINT32_MAX;  // of a launch
+// Threads of a call's largest launch (sizes, and for the choice most_pages, set).
+int64_t    key_bounds_threads(const KeyBoundsArgs& a);
+int64_t    select_threads(const SelectArgs& a);
+int64_t    blocks_threads(const BlocksArgs& a);
 bool       select_in_one(const SelectArgs& a);  // in one launch, without a workspace (a's sizes and most_pages set)
 hipError_t launch_select(const SelectArgs& a, hipStream_t stream);
 hipError_t launch_blocks(const BlocksArgs& a, hipStream_t stream);

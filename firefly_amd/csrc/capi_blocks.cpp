@@ -124,7 +124,7 @@ constexpr int kMostListed = 1 << 26;  // pages of a list: their tokens count in 
 // A choice's workspace: the scores, one per block of queries, KV head and page, and the queries' sums.
 struct SelectLayout
 {
-    int64_t stride, sums, total;  // total -1: beyond all memory
+    int64_t stride, sums, total;  // total -1: beyond all memory, or a launch's threads
 };
 
 SelectLayout select_layout(int batch, int seq_len, int num_heads, int num_kv_heads, int head_dim, int pages, int count,
@@ -139,8 +139,11 @@ SelectLayout select_layout(int batch, int seq_len, int num_heads, int num_kv_hea
     a.group = num_heads / num_kv_heads;
     a.head_dim = head_dim;
     a.most_pages = pages;
+    a.query_block = query_block;
     a.lists = lists;
+    a.count = count;
     if (ffkv::select_in_one(a)) return SelectLayout{};
+    if (ffkv::select_threads(a) > ffkv::kMostThreads) return SelectLayout{0, 0, -1};
     const double  each = 4.0 * pages + 16.0 * head_dim + 256.0;
     if (each * batch * lists * num_kv_heads > kMostBytes) return SelectLayout{0, 0, -1};
     const int64_t all = static_cast<int64_t>(batch) * lists * num_kv_heads;
@@ -249,6 +252,8 @@ int ffkv_key_bounds(const void* k_cache, int cache_dtype, const float* k_scale, 
     a.head_dim = head_dim;
     a.max_blocks = max_blocks;
     a.num_blocks = num_blocks;
+    if (ffkv::key_bounds_threads(a) > ffkv::kMostThreads)
+        return fail(FFKV_ERR_UNSUPPORTED, "the pages of %d new tokens are too many for one call", new_tokens);
     const hipError_t e = ffkv::launch_key_bounds(a, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? ok() : hip_fail(e, "key bounds launch");
 }
@@ -303,29 +308,14 @@ int ffkv_select_blocks(const void* q, int q_dtype, const void* bounds, int bound
     if (static_cast<int64_t>(std::min(query_block, seq_len)) * group > INT32_MAX / 2)
         return fail(FFKV_ERR_UNSUPPORTED, "query_block * group too large");
     if (need < 0 || static_cast<int64_t>(batch) * lists * num_kv_heads * ceil_div(pages, 32) > INT32_MAX)
-        return fail(FFKV_ERR_UNSUPPORTED, "the scores of %d x %d lists over %d pages are too many: give max_context_len", batch,
-                    lists, pages);
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    void*       ws = workspace;
-    if (ws != nullptr && workspace_bytes < static_cast<size_t>(need))
-        return fail(FFKV_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %lld bytes needed", workspace_bytes,
-                    static_cast<long long>(need));
-    if (ws == nullptr && need > 0)
-    {
-        bool capturing = false;
-        if (const int rc = is_capturing(s, capturing)) return rc;
-        if (capturing)
-            return fail(FFKV_ERR_WORKSPACE, "a captured call needs a workspace, of %lld bytes", static_cast<long long>(need));
-        if (const int rc = take_memory(&ws, need, s)) return rc;
-    }
+        return fail(FFKV_ERR_UNSUPPORTED, "the scores of %d x %d lists of %d KV heads over %d pages are too many: give "
+                    "max_context_len, or fewer in a call", batch, lists, num_kv_heads, pages);
     ffkv::SelectArgs a{};
     a.q = q;
     a.bounds = bounds;
     a.block_table = block_table;
     a.context_lens = context_lens;
     a.blocks = blocks;
-    a.scores = static_cast<float*>(ws);
-    a.query_sums = need > 0 ? reinterpret_cast<double*>(static_cast<char*>(ws) + lay.sums) : nullptr;
     a.stride = lay.stride;
     a.q_dtype = q_dtype;
     a.bounds_dtype = bounds_dtype;
@@ -343,6 +333,23 @@ int ffkv_select_blocks(const void* q, int q_dtype, const void* bounds, int bound
     a.count = count;
     a.sinks = sinks;
     a.recent = recent;
+    if (ffkv::select_threads(a) > ffkv::kMostThreads)
+        return fail(FFKV_ERR_UNSUPPORTED, "%d x %d lists of %d KV heads are too many for one call", batch, lists, num_kv_heads);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    void*       ws = workspace;
+    if (ws != nullptr && workspace_bytes < static_cast<size_t>(need))
+        return fail(FFKV_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %lld bytes needed", workspace_bytes,
+                    static_cast<long long>(need));
+    if (ws == nullptr && need > 0)
+    {
+        bool capturing = false;
+        if (const int rc = is_capturing(s, capturing)) return rc;
+        if (capturing)
+            return fail(FFKV_ERR_WORKSPACE, "a captured call needs a workspace, of %lld bytes", static_cast<long long>(need));
+        if (const int rc = take_memory(&ws, need, s)) return rc;
+    }
+    a.scores = static_cast<float*>(ws);
+    a.query_sums = need > 0 ? reinterpret_cast<double*>(static_cast<char*>(ws) + lay.sums) : nullptr;
     hipError_t e = ffkv::launch_select(a, s);
     if (workspace == nullptr && ws != nullptr)
     {
@@ -433,6 +440,8 @@ int ffkv_paged_attention_blocks(const void* q, void* out, int qo_dtype, const vo
     a.lists = lists_of(seq_len, query_block);
     a.count = count;
     a.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf(static_cast<float>(head_dim))) * kLog2e;
+    if (ffkv::blocks_threads(a) > ffkv::kMostThreads)
+        return fail(FFKV_ERR_UNSUPPORTED, "%d x %d tokens of %d KV heads are too many for one call", batch, seq_len, num_kv_heads);
     const ffkv::BlocksLayout lay = ffkv::plan_blocks(a);
     hipStream_t s = static_cast<hipStream_t>(stream);
     void*       ws = workspace;

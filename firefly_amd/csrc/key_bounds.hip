@@ -99,12 +99,30 @@ __global__ __launch_bounds__(kBoundsThreads) void key_bounds_kernel(KeyBoundsArg
     store_bound8<CT, false>(a.bounds, at + a.head_dim, hi);
 }
 
+namespace
+{
+
+// Pages of a row that its new tokens lie on, at most.
+int64_t new_pages(const KeyBoundsArgs& a)
+{
+    return std::min<int64_t>((static_cast<int64_t>(a.new_tokens) + kBlockSize - 2) / kBlockSize + 1, a.max_blocks);
+}
+
+}  // namespace
+
+// (of a row: the rows are the grid's second dimension)
+int64_t key_bounds_threads(const KeyBoundsArgs& a)
+{
+    const int64_t chunks = static_cast<int64_t>(a.num_kv_heads) * a.head_dim / 8;
+    return (new_pages(a) * chunks + kBoundsThreads - 1) / kBoundsThreads * kBoundsThreads;
+}
+
 hipError_t launch_key_bounds(const KeyBoundsArgs& a, hipStream_t stream)
 {
+    if (key_bounds_threads(a) > kMostThreads) return hipErrorInvalidConfiguration;
     const int     chunks = a.num_kv_heads * a.head_dim / 8;
-    const int64_t pages = std::min<int64_t>((static_cast<int64_t>(a.new_tokens) + kBlockSize - 2) / kBlockSize + 1, a.max_blocks);
-    const int64_t wgs = (pages * chunks + kBoundsThreads - 1) / kBoundsThreads;
-    if (wgs > INT32_MAX) return hipErrorInvalidConfiguration;
+    const int64_t pages = new_pages(a);
+    const int64_t wgs = key_bounds_threads(a) / kBoundsThreads;
     if (wgs <= 0) return hipSuccess;
     const dim3 grid(static_cast<unsigned>(wgs), static_cast<unsigned>(a.batch));
     auto go = [&]<int CT>()

@@ -736,6 +736,17 @@ int64_t prefill_blocks(const BlocksArgs& a)
 
 }  // namespace
 
+// (split lists and halves of them are for few)
+int64_t blocks_threads(const BlocksArgs& a)
+{
+    if (blocks_kernel(a) == BlocksKernel::kPrefill)  // whole rounds of the XCDs, eight or four waves a workgroup
+    {
+        const int64_t blocks = (static_cast<int64_t>(a.query_block) * a.group + 127) / 128;
+        return (static_cast<int64_t>(a.batch) * a.lists * a.num_kv_heads + 7) / 8 * 8 * blocks * (a.head_dim == 256 ? 512 : 256);
+    }
+    return static_cast<int64_t>(a.batch) * a.seq_len * blocks_heads(a) * 64 * kBlocksWaves;
+}
+
 // Whether the prefill's lists can be taken in two halves: a workgroup of that form fills a CU, and each half has two steps.
 bool blocks_pairable(const BlocksArgs& a)
 {
@@ -817,7 +828,7 @@ hipError_t launch_blocks(const BlocksArgs& a, hipStream_t stream)
     if (kernel == BlocksKernel::kPrefill) return launch_blocks_prefill(a, stream);
     const int64_t wgs = static_cast<int64_t>(a.batch) * a.seq_len * blocks_heads(a) * a.splits;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.seq_len * a.num_heads;
-    if (wgs > INT32_MAX || rows > INT32_MAX) return hipErrorInvalidConfiguration;
+    if (blocks_threads(a) > kMostThreads) return hipErrorInvalidConfiguration;
     const dim3 grid(static_cast<unsigned>(wgs)), block(static_cast<unsigned>(64 * a.waves));
     hipError_t e;
     if (kernel == BlocksKernel::kDecode)
