@@ -33,7 +33,7 @@ constexpr int kScorePages = 4;  // neighbouring pages that a group of lanes scor
 constexpr int kOneThreads = 512;
 constexpr int kOneRounds = 4;  // of block_select_one at most
 constexpr int kOwnRows = 8;    // query rows of a block that are added up one after the other
-constexpr int kWideRows = 256;  // more of them than that are added up by twice the threads
+constexpr int kWideRows = 128;  // more of them than that are added up by twice the threads
 
 template <int CTRL>
 __device__ __forceinline__ double dpp64(double v)
@@ -44,16 +44,17 @@ __device__ __forceinline__ double dpp64(double v)
     return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// v plus that of the lane 32 (16) away, in both.
+// In the lower half of the lanes (the even rows of 16) a plus that of the lane 32 (16) away, in the others b.
 template <bool HALF>
-__device__ __forceinline__ double swap_sum64(double v)
+__device__ __forceinline__ double swap_sum64(double a, double b)
 {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = static_cast<uint32_t>(u), hi = static_cast<uint32_t>(u >> 32);
-    const auto     l = HALF ? __builtin_amdgcn_permlane32_swap(lo, lo, false, false)
-                            : __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
-    const auto     h = HALF ? __builtin_amdgcn_permlane32_swap(hi, hi, false, false)
-                            : __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    const uint64_t x = __builtin_bit_cast(uint64_t, a), y = __builtin_bit_cast(uint64_t, b);
+    const uint32_t x0 = static_cast<uint32_t>(x), x1 = static_cast<uint32_t>(x >> 32);
+    const uint32_t y0 = static_cast<uint32_t>(y), y1 = static_cast<uint32_t>(y >> 32);
+    const auto     l = HALF ? __builtin_amdgcn_permlane32_swap(x0, y0, false, false)
+                            : __builtin_amdgcn_permlane16_swap(x0, y0, false, false);
+    const auto     h = HALF ? __builtin_amdgcn_permlane32_swap(x1, y1, false, false)
+                            : __builtin_amdgcn_permlane16_swap(x1, y1, false, false);
     return __builtin_bit_cast(double, static_cast<uint64_t>(static_cast<uint32_t>(h[0])) << 32 | static_cast<uint32_t>(l[0])) +
            __builtin_bit_cast(double, static_cast<uint64_t>(static_cast<uint32_t>(h[1])) << 32 | static_cast<uint32_t>(l[1]));
 }
@@ -74,7 +75,7 @@ __device__ __forceinline__ double group_sums4(const double (&v)[4], int lane)
         c += dpp64<0x124>(c);  // lanes 4 and 8 before it in its row of 16
         c += dpp64<0x128>(c);
     }
-    if constexpr (LPP == 32) c = swap_sum64<false>(c);
+    if constexpr (LPP == 32) c = swap_sum64<false>(c, c);
     return c;
 }
 
@@ -129,25 +130,39 @@ __device__ __forceinline__ void add_query(const float (&x)[8], double (&down)[8]
     }
 }
 
-// The sums over a wave's groups of LPP lanes, in every group.
+// The sums over a wave's groups of LPP lanes to part[2][LPP * 8] in LDS: every exchange halves the values that a lane holds.
 template <int LPP>
-__device__ __forceinline__ void wave_sums(double (&down)[8], double (&up)[8])
+__device__ __forceinline__ void wave_sums(const double (&down)[8], const double (&up)[8], int lane, double* part)
 {
+    double v[16];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < 8; ++e) v[e] = down[e], v[8 + e] = up[e];
+    int n = 16, first = 0;  // values held, and which the first of them is
+    if constexpr (LPP == 8)
     {
-        if constexpr (LPP == 8)
-        {
-            down[e] += dpp64<0x128>(down[e]);  // 8 lanes before it in its row of 16
-            up[e] += dpp64<0x128>(up[e]);
-        }
-        if constexpr (LPP <= 16)
-        {
-            down[e] = swap_sum64<false>(down[e]);
-            up[e] = swap_sum64<false>(up[e]);
-        }
-        down[e] = swap_sum64<true>(down[e]);
-        up[e] = swap_sum64<true>(up[e]);
+        n /= 2;
+        const bool odd = lane & 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)  // with 8 lanes before it in its row of 16
+            v[i] = (odd ? v[i + 8] : v[i]) + dpp64<0x128>(odd ? v[i] : v[i + 8]);
+        first += odd ? 8 : 0;
+    }
+    if constexpr (LPP <= 16)
+    {
+        n /= 2;
+#pragma unroll
+        for (int i = 0; i < (LPP == 8 ? 4 : 8); ++i) v[i] = swap_sum64<false>(v[i], v[i + n]);
+        first += lane & 16 ? n : 0;
+    }
+    n /= 2;
+#pragma unroll
+    for (int i = 0; i < LPP / 4; ++i) v[i] = swap_sum64<true>(v[i], v[i + n]);
+    first += lane & 32 ? n : 0;
+#pragma unroll
+    for (int i = 0; i < LPP / 4; ++i)
+    {
+        const int k = first + i;
+        part[(k >> 3) * (LPP * 8) + 8 * (lane % LPP) + (k & 7)] = v[i];
     }
 }
 
@@ -445,9 +460,10 @@ __global__ __launch_bounds__(kScoreThreads) void block_queries_few(SelectArgs a,
 }
 
 // More of them: Q- and Q+ of every block of queries and KV head, a workgroup each (2 x 512 tokens, 32/8 heads of 128 in blocks of
-// 64: 7.2 us, where the workgroups that score would read a block's queries once for every 64 pages).  Whole calls over 2000 pages
-// by 512 and 1024 threads: blocks of 16 tokens 48.8 and 50.7 us, 64 23.4 and 23.0, 128 23.5 and 22.4, 512 41.4 and 36.7; blocks of
-// 4 146 and 156, of 1 in the form above 528 and (here) 585.  Few lists in one launch take 1024 in two turns: 64 tokens 11.6 and 12.9.
+// 64: 6.6 us, where the workgroups that score would read a block's queries once for every 64 pages).  Whole calls over 2000 pages
+// by 512 and 1024 threads, when a wave's sums took twice the exchanges: blocks of 16 tokens 48.8 and 50.7 us, 64 23.4 and 23.0,
+// 128 23.5 and 22.4, 512 41.4 and 36.7.  (Now 47.7, 22.4, 22.0 and 36.0 by the rule; blocks of one token by the lanes above 527,
+// by 1024 threads 584.)
 template <int QT, int LPP, int THREADS>
 __global__ __launch_bounds__(THREADS) void block_queries(SelectArgs a)
 {
@@ -482,14 +498,7 @@ __global__ __launch_bounds__(THREADS) void block_queries(SelectArgs a)
                 add_query(x, down, up);
             }
     }
-    wave_sums<LPP>(down, up);
-    if (lane < LPP)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-        {
-            s_part[wave][0][8 * c + e] = down[e];
-            s_part[wave][1][8 * c + e] = up[e];
-        }
+    wave_sums<LPP>(down, up, lane, s_part[wave][0]);
     __syncthreads();
     for (int i = tid; i < 2 * a.head_dim; i += THREADS)
     {
@@ -861,53 +870,58 @@ __global__ __launch_bounds__(kOneThreads) void block_select_one(SelectArgs a)
     const int rows = min(a.query_block, a.seq_len - t0) * a.group;
     const int64_t whole = block_rows(a.query_block, a.seq_len, a.group);
     double    down[8], up[8];
-    auto sum_rows = [&](int first, int step)
+    // Q- and Q+ of rows first, first + step, ..; TWO: and of those half a step behind each, apart.
+    auto sum_rows = [&]<bool TWO>(int first, int step, double (&down2)[8], double (&up2)[8])
     {
+        constexpr int SETS = TWO ? 2 : 1;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) down[e] = up[e] = 0.0;
+        for (int e = 0; e < 8; ++e) down[e] = up[e] = down2[e] = up2[e] = 0.0;
         for (int r0 = first; r0 < rows; r0 += UN * step)
         {
-            Raw8 q[UN];
+            Raw8 q[SETS][UN];
 #pragma unroll
             for (int k = 0; k < UN; ++k)
-                if (r0 + k * step < rows && in) load_raw8<QT>(a.q, query_at(a, b, t0, kvh, r0 + k * step, c), q[k]);
 #pragma unroll
-            for (int k = 0; k < UN; ++k)
-                if (r0 + k * step < rows && in)
+                for (int h = 0; h < SETS; ++h)
                 {
-                    float x[8];
-                    unpack8<QT>(q[k], x);
-                    add_query(x, down, up);
+                    const int r = r0 + k * step + h * (step / 2);
+                    if (r < rows && in) load_raw8<QT>(a.q, query_at(a, b, t0, kvh, r, c), q[h][k]);
                 }
+#pragma unroll
+            for (int k = 0; k < UN; ++k)
+#pragma unroll
+                for (int h = 0; h < SETS; ++h)
+                    if (r0 + k * step + h * (step / 2) < rows && in)
+                    {
+                        float x[8];
+                        unpack8<QT>(q[h][k], x);
+                        add_query(x, h == 0 ? down : down2, h == 0 ? up : up2);
+                    }
         }
     };
+    double down2[8], up2[8];
     if (whole <= kOwnRows)
-        sum_rows(0, 1);  // every lane its dims of all rows
+        sum_rows.template operator()<false>(0, 1, down2, up2);  // every lane its dims of all rows
     else
     {
-        // in the order of block_queries, twice the threads in two turns
-        double*   s_part = reinterpret_cast<double*>(s_mem);  // [wave][2][LPP * 8]
-        const int turns = whole <= kWideRows ? 1 : 2;
-#pragma unroll 1
-        for (int turn = 0; turn < turns; ++turn)
+        // in the order of block_queries: twice the threads are these waves, and as many again
+        double*    s_part = reinterpret_cast<double*>(s_mem);  // [wave][2][LPP * 8]
+        const bool two = whole > kWideRows;
+        if (two)
         {
-            sum_rows(turn * SLOTS + grp, turns * SLOTS);
-            wave_sums<LPP>(down, up);
-            if (lane < LPP)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                {
-                    s_part[((turn * WAVES + wave) * 2 + 0) * (LPP * 8) + 8 * c + e] = down[e];
-                    s_part[((turn * WAVES + wave) * 2 + 1) * (LPP * 8) + 8 * c + e] = up[e];
-                }
+            sum_rows.template operator()<true>(grp, 2 * SLOTS, down2, up2);
+            wave_sums<LPP>(down2, up2, lane, s_part + (WAVES + wave) * (2 * LPP * 8));
         }
+        else
+            sum_rows.template operator()<false>(grp, SLOTS, down2, up2);
+        wave_sums<LPP>(down, up, lane, s_part + wave * (2 * LPP * 8));
         __syncthreads();
         double s = 0.0;  // (as many threads as sums, or more)
         static_assert(2 * LPP * 8 <= kOneThreads, "a sum per thread");
         if (tid < 2 * LPP * 8)
-            for (int turn = 0; turn < turns; ++turn)
+            for (int w0 = 0; w0 < (two ? 2 : 1) * WAVES; w0 += WAVES)
 #pragma unroll
-                for (int w = 0; w < WAVES; ++w) s += s_part[(turn * WAVES + w) * (2 * LPP * 8) + tid];
+                for (int w = 0; w < WAVES; ++w) s += s_part[(w0 + w) * (2 * LPP * 8) + tid];
         __syncthreads();
         if (tid < 2 * LPP * 8) s_part[tid] = s;
         __syncthreads();

@@ -79,6 +79,7 @@ TINY = [(0, 1.0), (1, 2.0 ** -24)]
 @pytest.mark.parametrize("rows,T", [
     (TINY + [(2, 1.5 * 2.0 ** -54), (3, 1.5 * 2.0 ** -54)], 4),       # few query rows: one after the other
     (TINY + [(i, 2.0 ** -54) for i in (32, 96, 160, 224)], 256), (TINY + [(i, 2.0 ** -54) for i in (16, 48, 80, 112)], 128),
+    (TINY + [(i, 2.0 ** -54) for i in (32, 64, 96, 128)], 129),
     (TINY + [(i, 2.0 ** -54) for i in (64, 192, 320, 448)], 512), (TINY + [(i, 2.0 ** -54) for i in (2, 3, 6, 7)], 9),
     (TINY + [(i, 2.0 ** -54) for i in (32, 96, 160, 224)], 700), (TINY + [(i, 2.0 ** -54) for i in (64, 192, 320, 448)], 700),
 ])
