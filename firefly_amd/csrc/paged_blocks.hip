@@ -100,7 +100,7 @@ void paged_blocks_decode(BlocksArgs a)
     constexpr int  KSTEPS = (D + 31) / 32;  // of 32 dims; head_dim 80 and 112 leave lanes of the last without any
     constexpr int  NT = D / 16;
     constexpr bool NEED_LO = !((QT == BF16 && BF) || (QT == F16 && !BF));
-    constexpr bool P_LO = VBF;
+    constexpr bool P_LO = VBF || CT == F16;
     constexpr int  DEPTH = D == 256 ? 1 : 2;
     constexpr int  EB = kElemBytes<CT>;
     constexpr int  NW = EB == 2 ? KSTEPS : (KSTEPS + 1) / 2;
@@ -282,8 +282,9 @@ void paged_blocks_decode(BlocksArgs a)
         }
     };
 
-    // Online softmax of a staged page and its products with V.  P in bf16 takes a hi + lo pair (16 bits); in f16 its 11 bits (int8
-    // pages: in units of the column, as the V scales are in it).
+    // Online softmax of a staged page and its products with V.  P takes a hi + lo pair of 16-bit values (16 bits in bf16, 21 in
+    // f16: 64 rows of f16 pages 44.0 -> 44.3 us), on 8-bit pages f16's 11 bits: the codes' own steps are larger (with a pair int8
+    // took 30.3 -> 32.1 us, fp8 25.5 -> 25.8).  int8 pages: in units of the column, as the V scales are in it.
     auto finish_page = [&](int n_tok, float tks, float tvs, f32x4 s)
     {
         float sc[4], vs[4];

@@ -105,3 +105,23 @@ def test_tiles(ff, gpu, act, kv, by, form):
 @pytest.mark.parametrize("form", TILES)
 def test_int8_tiles_of_all_sizes(ff, gpu, big, form):
     int8_of_all_sizes(ff, gpu, big, *form)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,ctx,S,count,T", [(16, 4, 64, [2, 5, 9, 14], 1, 1, 1), (16, 2, 128, [3, 7, 20], 1, 2, 1),
+                                                    (8, 2, 128, [3, 4], 6, 2, 2), (4, 2, 256, [1, 6], 1, 1, 1)])
+def test_f16_pages_keep_p(ff, gpu, Hq, Hkv, D, ctx, S, count, T):
+    """fp32 queries (fp16 values) over few tokens of fp16 pages, nearly equal weights: P takes part in 21 bits, not in fp16's 11.  The
+    bound: scores, softmax and output in fp32, 2^-20 of sum p |v|, and 2^-25 of |v| a key where P's low part is subnormal."""
+    c = make(D + S, ctx, S, Hq, Hkv, D, "f32", "f16", spread=0.1)
+    c.q = cases.decode(cases.encode(c.q, O.DTYPE_F16), O.DTYPE_F16)
+    li = lists(c, S, count, T)
+    kf, vf = su.values(c, "k"), su.values(c, "v")
+    wide = types.SimpleNamespace(B=c.B, Hq=Hq, Hkv=Hkv, D=D, ctx=c.ctx, max_blocks=c.max_blocks, num_blocks=c.num_blocks,
+                                 block_table=c.block_table, kv=O.DTYPE_F32, k_pool=kf, v_pool=vf)
+    with pytest.MonkeyPatch.context() as mp:
+        mp.setattr(su, "values", lambda o, which: o.k_pool if which == "k" else o.v_pool)
+        want, bound = bu.attend(wide, c.q.astype(np.float64), li, T, c.act, S, 0.0)
+        wide.v_pool = np.abs(vf)
+        mass, _ = bu.attend(wide, c.q.astype(np.float64), li, T, c.act, S, 0.0)
+    bound = bound + mass * 2.0 ** -20 + np.abs(vf).max() * 2.0 ** -25 * count * 16
+    su.check(su.host(run(ff, c, li, T, gpu)).reshape(want.shape), want, bound, "out")
