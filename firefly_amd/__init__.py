@@ -519,7 +519,8 @@ def select_blocks(q, bounds, block_table, context_lens, count: int, sinks: int =
     the first ``sinks``, the last ``recent`` (up to the block's last query's), and those whose key ``bounds`` allow the largest
     scores, summed over the block's queries and the KV head's query heads.  ``q`` ``[B, S, Hq, D]`` at ``context_lens[b] + t``.
     Returns ``blocks`` int32 ``[B, ceil(S / query_block), Hkv, count]``, ascending, -1 behind a row of fewer pages.  A captured
-    call needs a workspace (``select_blocks_workspace``) unless no row can have more than ``count`` pages."""
+    call needs a workspace (``select_blocks_workspace``) unless no row can have more than ``count`` pages, or lists and pages are
+    few (``ffkv_select_blocks_workspace_bytes`` gives 0)."""
     if blocks is None:
         import torch
 

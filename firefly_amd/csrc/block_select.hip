@@ -286,7 +286,7 @@ struct PageBounds
 // (57.5 us in all).  LPP lanes take four neighbouring pages' bounds, 8 dims each, and every lane adds up its dims of the
 // queries by itself; while a round is added up the next one's bounds are on their way, and the table's entries of the one
 // after.  Bound by HBM and by fp64 (a conversion and a product per bound): 4.6 TB/s (4 rows of 8188 pages, 4 heads, 67 MB:
-// 14.5 us; the 64 rows above 32 of 37.9 in all).
+// 14.5 us; the 64 rows above 32 of 38.1 in all).
 template <int BT, int QT, int LPP, bool FULL>
 __global__ __launch_bounds__(kScoreThreads) void block_scores_step(SelectArgs a, int heads)
 {
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(kScoreThreads) void block_queries_few(SelectArgs a,
 }
 
 // More of them: Q- and Q+ of every block of queries and KV head, a workgroup each (2 x 512 tokens, 32/8 heads of 128 in blocks of
-// 64: 6.6 us, where the workgroups that score would read a block's queries once for every 64 pages).  Whole calls over 2000 pages
+// 64: 7.1 us, where the workgroups that score would read a block's queries once for every 64 pages).  Whole calls over 2000 pages
 // by 512 and 1024 threads, when a wave's sums took twice the exchanges: blocks of 16 tokens 48.8 and 50.7 us, 64 23.4 and 23.0,
 // 128 23.5 and 22.4, 512 41.4 and 36.7.  (Now 47.7, 22.4, 22.0 and 36.0 by the rule; blocks of one token by the lanes above 527,
 // by 1024 threads 584.)
@@ -512,8 +512,8 @@ __global__ __launch_bounds__(THREADS) void block_queries(SelectArgs a)
 
 // Many blocks of queries: a workgroup holds one round of a row's pages, as fp64, and goes through `per` blocks of queries of
 // the row, whose sums block_queries has left, LISTS of them at a time through LDS.  (2 x 8 blocks of 64 queries over 2000 pages,
-// 8 heads: 10.5 us, the chain of table and bounds ahead of 3 us of fp64 products; 256 to 2048 workgroups in all 24.8 to 25.8 us for
-// the whole call.)
+// 8 heads: 10.5 us, the chain of table and bounds ahead of 3 us of fp64 products, of 24.2 us for the whole call; 256 to 2048
+// workgroups in all were within 1 us of each other.)
 template <int BT, int LPP, bool FULL>
 __global__ __launch_bounds__(kScoreThreads) void block_scores_lists(SelectArgs a, int tiles, int per, int parts)
 {
@@ -1038,7 +1038,8 @@ bool select_by_lists(int seq_len, int lists, int group) { return lists > 1 || st
 // Few lists of few pages: one launch, without a workspace, in which a list has one CU (1.5 us a round).  Rounds of 128 pages at
 // head_dim 128, whole calls in the other launches and in one: 8 lists of up to 64 pages 8.3 and 6.2 us, of 250 9.1 and 6.6,
 // 128 lists 9.9 and 7.8, 11.4 and 9.6; 32 lists of 1000 11.2 and 17.7; 512 lists of 64 11.9 and 14.4.  Where queries are
-// summed apart, 64 lists of 495 pages 14.9 and 10.4, 128 16.1 and 14.6, 128 lists of 1995 23.0 and 31.5.
+// summed apart, 64 lists of 495 pages 14.9 and 10.4, 128 16.1 and 14.6, 128 lists of 1995 23.0 and 31.5.  (The sums have the same
+// order in either, so no row's choice depends on which it is.)
 bool select_in_one(const SelectArgs& a)
 {
     const int64_t lists = static_cast<int64_t>(a.batch) * a.lists * a.num_kv_heads;

@@ -7,7 +7,8 @@
 // that went.
 //
 // Bound by HBM: every touched page's K is read once, an eighth of it written (8 int8 prompts of 4001 tokens, 8 heads of 128, 42 MB:
-// 7.8 us = 5.4 TB/s); a step, whose 64 pages are 2 MB, by its launch and the chain of length, table and page (3.8 us).
+// 8.5 us a call = 5.0 TB/s; a copy of 42 MB 9.9); a step, whose 64 pages are 2 MB, by its launch and the chain of length, table
+// and page (3.8 us).
 #include "blocks.h"
 #include "ffkv_device.h"
 

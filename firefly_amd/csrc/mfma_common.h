@@ -274,7 +274,7 @@ __device__ __forceinline__ float new_units(ValueUnits& u, float wc)
     u.known = fmaxf(wc, u.known);
     if (u.known == __builtin_huge_valf()) return 1.0f;
     const float to = fminf(fmaxf(u.shift + static_cast<float>(11 - __builtin_amdgcn_frexp_expf(u.known)), -40.0f), 40.0f);
-    const float f = __builtin_amdgcn_exp2f(to - u.shift);  // (whole powers of two are exact)
+    const float f = __builtin_ldexpf(1.0f, static_cast<int>(to - u.shift));
     u.shift = to;
     u.known *= f;
     return f;

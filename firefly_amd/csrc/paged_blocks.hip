@@ -4,8 +4,8 @@
 //   out[b, t, h] = sum over listed pages and their tokens j <= context_lens[b] + t of softmax_j(scale q.k_j) v_j
 //
 // Steps are bound by HBM: the listed pages are read once, at about Hq / Hkv operations a byte.  64 rows of 64 listed pages, 32/8
-// heads of 128, bf16: 270 MB in 49.4 us = 5.5 TB/s (int8 28.9, fp32 98); 4 rows of 256, 28/4 heads, f16: 14.2 us, of which
-// 3.5 of merge; 4 rows of up to 16: 7.2, a launch and its chain of loads.
+// heads of 128, bf16: 270 MB in 49.4 us = 5.5 TB/s (inputs resident: int8 30.3, fp32 98); 4 rows of 256, 28/4 heads, f16: 14.3 us,
+// of which 3.5 of merge; 4 rows of up to 16: 7.3, a launch and its chain of loads.
 //
 // On the matrix cores (16- and 8-bit caches) a workgroup of four or eight waves takes a list, or a piece of one, and up to 16
 // query heads of its KV head; a wave takes every fourth (eighth) page, with the products and the page loads of the plain decode
@@ -675,7 +675,9 @@ hipError_t for_types(const BlocksArgs& a, F f)
 BlocksKernel blocks_kernel(const BlocksArgs& a)
 {
     if (a.cache_dtype == F32 || !mfma_dim(a.head_dim)) return BlocksKernel::kVector;
-    // (the prefill has no form of head_dim 80, 96 and 112: their lists are attended token by token)
+    // (The prefill has no form of head_dim 80, 96 and 112, nor of fp32 pages: their lists are attended token by token, each token
+    // reading its block's list again.  2 x 512 tokens in blocks of 64, 128 bf16 pages, 32/8 heads: 546, 545 and 790 us, where 128
+    // dims take 58; fp32 at 128 dims 1268.)
     if (a.query_block == 1 || a.head_dim == 80 || a.head_dim == 96 || a.head_dim == 112) return BlocksKernel::kDecode;
     // Few tokens too, while the lists that each reads for itself come from the caches: by workgroups (token, KV head) and pages of
     // a list, 32/8 heads of 128, bf16, token by token and in the prefill's tiles: 32 x 256 14.7 and 17.3 us, 64 x 256 19.5 and
@@ -776,9 +778,10 @@ BlocksLayout plan_blocks(BlocksArgs& a)
         else
             plan_blocks_prefill_fp8(p);
         // More than 170 blocks make two pieces a list (or none, where lists are short): the halves of a workgroup do as well
-        // and need no merge through memory.  256 blocks at 32/8 heads of 128: 128 listed pages fp8 57.8 -> 50.9 us, bf16
-        // 63.0 -> 55.2, int8 78.1 -> 67.5; 64 pages 39.7 -> 30.2, 43.0 -> 33.6, 57.8 -> 40.4; 16 pages 15.4 -> 14.6; 8 pages
-        // 11.7 -> 12.0.  160 blocks of 128 pages take three pieces: 43.2 there, 49.4 in halves.
+        // and need no merge through memory.  256 blocks at 32/8 heads of 128, inputs resident: 128 listed pages fp8 57.8 -> 50.9
+        // us (inputs that change from call to call: 57.1 -> 53.5), bf16 63.0 -> 55.2, int8 78.1 -> 67.5; 64 pages 39.7 -> 30.2,
+        // 43.0 -> 33.6, 57.8 -> 40.4; 16 pages 15.4 -> 14.6; 8 pages 11.7 -> 12.0.  160 blocks of 128 pages take three pieces:
+        // 43.2 there, 49.4 in halves.
         a.pair = blocks_pairable(a) && (p.n_split == 1 || 3 * prefill_blocks(a) > 512);
         if (a.pair) return l;
         a.splits = p.n_split;

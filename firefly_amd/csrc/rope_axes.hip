@@ -14,7 +14,9 @@
 // the angle at most: 2^-22 + |p| 2^-48 in all (theta >= 1).
 //
 // Bound by HBM (q read and written, k and v read and written once): 8 x 1500 f16 tokens of 32/8 heads of 128, 295 MB, 58.4 us =
-// 5.1 TB/s; 32000 bf16 tokens of 28/4 heads, 590 MB, 102 us = 5.8 TB/s (a copy reaches 5.1).  A step of 4 tokens takes 3.5 us.
+// 5.1 TB/s; 32000 bf16 tokens of 28/4 heads, 590 MB, 102 us = 5.8 TB/s (device copies of as many bytes take 55.6 and 109 us: a copy
+// is no bound).  A step of 4 tokens takes 3.5 us.  Into int8 and fp8 pages the 8 x 1500 tokens take 62 and 63 us, where their
+// own type takes 50 (inputs resident): the quantization's vector work; alone, without pages, 38.5.
 #include "blocks.h"
 #include "ffkv_device.h"
 

@@ -451,12 +451,14 @@ FFKV_API int ffkv_key_bounds(const void* k_cache, int cache_dtype, const float* 
  * pages of the row.  Queries q [batch, seq_len, num_heads, head_dim] sit at positions context_lens[b] + t.  Of the pages up to
  * the block's last query's, the first `sinks` and the last `recent` are taken, and of the rest those with the largest
  *     score(page) = sum over the block's queries and the KV head's query heads of sum_d max(q_d lo_d, q_d hi_d)
- * (sums in fp64, rounded once to fp32; of equal scores the lower page; NaN counts as the largest, 0 times an infinite bound as 0;
- * a page on no block-table entry as the lowest).  count up to 2^26, num_blocks at least 1.  blocks int32 [batch, ceil(seq_len / query_block), num_kv_heads,
- * count]: ascending, -1 behind a row of fewer pages.  `recent` pages count back from the block's last query: with
- * query_block > 1 give at least (query_block + 14) / 16 + 1 for every query to have its own page.  bounds_dtype F32, F16 or BF16
- * (ffkv_key_bounds' type).  max_context_len bounds the rows' tokens, this call's included (0: the table's width); pages past it
- * are not taken.  workspace: NULL or ffkv_select_blocks_workspace_bytes (a captured call needs one where that is not 0).
+ * (sums in fp64, rounded once to fp32; of equal scores the lower page; NaN counts as the largest, 0 times an infinite bound as
+ * 0; a page on no block-table entry as the lowest).  A row's choice does not depend on the call's other rows.  count up to 2^26,
+ * num_blocks at least 1; more lists than one launch takes (4 to 16 million) are refused.  blocks int32 [batch,
+ * ceil(seq_len / query_block), num_kv_heads, count]: ascending, -1 behind a row of fewer pages.  `recent` pages count back from the
+ * block's last query: with query_block > 1 give at least (query_block + 14) / 16 + 1 for every query to have its own page.
+ * bounds_dtype F32, F16 or BF16 (ffkv_key_bounds' type).  max_context_len bounds the rows' tokens, this call's included (0: the
+ * table's width); pages past it are not taken.  workspace: NULL or ffkv_select_blocks_workspace_bytes (a captured call needs one
+ * where that is not 0).
  */
 FFKV_API size_t ffkv_select_blocks_workspace_bytes(int batch, int seq_len, int num_heads, int num_kv_heads, int head_dim,
                                                    int count, int query_block, int max_blocks, int max_context_len);
